@@ -237,6 +237,54 @@ def accumulate_1d(dst, src):
     return dst
 
 
+# ---------------------------------------------------------------- many sequences: paged cache, drafted tokens, distillation
+def paged_cache(pages, heads, page, Dh, dtype=torch.float8_e4m3fn, device="cuda"):
+    """An empty cache (k_pages, v_pages, k_scale, v_scale): pages [pages, heads, page, Dh rounded up to 16] of float8_e4m3fn with
+    scales [pages, heads], or of float16 with none."""
+    shape = (pages, heads, page, (Dh + 15) // 16 * 16)
+    k, v = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
+    if dtype is F16:
+        return k, v, None, None
+    return (k, v) + tuple(torch.ones((pages, heads), dtype=F32, device=device) for _ in range(2))
+
+
+def paged_append(k, v, cache, table, starts, lens, cos, sin, q=None, out=None, max_new=None, status=None):
+    """The new keys (rotated) and values [T, heads, Dh] of a ragged batch into the pages of `cache`; returns the queries q
+    rotated (into out where given), None without q.
+
+    Rows starts[b] .. starts[b+1]-1 are the new tokens of sequence b, lens[b] its length with them, table[b] its pages: int32
+    tensors on the GPU that the host does not read.  cos, sin: rope_tables of as many positions as any sequence has.
+    max_new: no sequence has more new rows than that.  status: a cleared int32 tensor of one element that becomes 1 + b where
+    the numbers of sequence b do not fit together (nothing of it is written then).  Rows may be strided."""
+    return _op.paged_append(k, v, *cache, table, starts, lens, cos, sin, q, out, max_new, status)
+
+
+def paged_attention(q, cache, table, starts, lens, alpha, max_new=None, out=None, status=None):
+    """Causal attention of the (rotated) queries of a ragged batch over `cache`, which holds their own positions too; the
+    arguments are those of paged_append.  Rows behind the last sequence are left as they are in out."""
+    return _op.paged_attention(q, *cache, table, starts, lens, alpha, max_new, out, status)
+
+
+def verify_draft(target, draft, tok, starts, u, r, temperature=1.0, status=None):
+    """Which drafted tokens are kept and what follows: (accepted int32 [sequences], next u16-as-int16 bits [T]).
+
+    Rows of a sequence are its last token and the drafted ones: tok u16-as-int16 [T] their tokens, target [T, V] the target
+    model's logits, draft [T, V] the drafting model's or None (tokens drafted without probabilities).  u [T], r [sequences]:
+    uniform f32 random numbers.  temperature 0: greedy.  next holds accepted[b] kept tokens, the one that follows, then 0."""
+    return _op.verify_draft(target, draft, tok, starts, u, r, temperature, status)
+
+
+def distill_topk_fwd(logit, idx, val, temperature=1.0, status=None):
+    """KL divergence of the student's softmax(logit / temperature) from the teacher's over its top logits val f16 [N, K] at the
+    ids idx u16-as-int16 [N, K]: (loss f32 [N], stats f32 [N, 2] for the adjoint)."""
+    return _op.distill_topk_fwd(logit, idx, val, temperature, status)
+
+
+def distill_topk_bwd(logit, idx, val, stats, scale, temperature=1.0, acc=None):
+    """Its gradient times scale [N] with respect to logit, f16 (added to acc where given)."""
+    return _op.distill_topk_bwd(logit, idx, val, stats, scale, temperature, acc)
+
+
 # ---------------------------------------------------------------- numerical-health digests
 def nan_count(x):
     """Number of NaNs of an f16 tensor as a 0-d int64 device tensor (src/thunk/op.rs:273-349)."""

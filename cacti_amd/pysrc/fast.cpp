@@ -11,6 +11,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -444,6 +445,225 @@ PyObject *softmax_ce_bwd(PyObject *const *v)
     return d.take();
 }
 
+// ---------------------------------------------------------------- paged cache, drafted tokens, distillation
+// The device of a call's tensors for its duration, and the stream that is current there
+struct OnDevice {
+    c10::DeviceGuard guard;
+    c10::Device dev;
+    explicit OnDevice(const at::Tensor &t) : guard(t.device()), dev(t.device()) {}
+    void *stream() const { return c10::hip::getCurrentHIPStream(dev.index()).stream(); }
+    const at::Tensor &here(const at::Tensor &t) const
+    {
+        require(t.device() == dev, "tensors of one device expected");
+        return t;
+    }
+    const at::Tensor &here(PyObject *o, at::ScalarType dtype) const { return here(checked(tensor(o), dtype)); }
+    void *pointer(PyObject *o, at::ScalarType dtype, int64_t numel) const     // or null for None
+    {
+        if (o == Py_None) return nullptr;
+        const at::Tensor &t = here(o, dtype);
+        require(t.numel() == numel, "a tensor has another number of elements");
+        return t.data_ptr();
+    }
+};
+const at::Tensor &on_gpu(const at::Tensor &t)
+{
+    require(t.is_cuda(), "tensor on the GPU expected");
+    return t;
+}
+
+// [T, H, Dh] f16 whose rows may be strided
+struct Rows {
+    const at::Tensor &t;
+    int64_t T, H, Dh, ld;
+    Rows(PyObject *o, const OnDevice &on, const char *what) : t(on.here(on_gpu(tensor(o))))
+    {
+        require(t.scalar_type() == at::kHalf && t.dim() == 3, what);
+        T = t.size(0), H = t.size(1), Dh = t.size(2);
+        require((Dh <= 1 || t.stride(2) == 1) && (H <= 1 || t.stride(1) == Dh), what);
+        ld = T > 1 ? t.stride(0) : H * Dh;
+    }
+};
+// [N, V] f16 whose rows may be strided
+struct Logits {
+    const at::Tensor &t;
+    int64_t N, V, ld;
+    Logits(PyObject *o, const OnDevice &on, const char *what) : t(on.here(on_gpu(tensor(o))))
+    {
+        require(t.scalar_type() == at::kHalf && t.dim() == 2, what);
+        N = t.size(0), V = t.size(1);
+        require(V <= 1 || t.stride(1) == 1, what);
+        ld = N > 1 ? t.stride(0) : V;
+    }
+};
+
+// (k_pages, v_pages, k_scale, v_scale, table, starts, lens), what an append and an attention call have in common
+struct Paged {
+    const at::Tensor &k, &v, &table;
+    void *ks, *vs, *starts, *lens;
+    int bits;
+    int64_t P, Hkv, page, B, W, ldt;
+    Paged(PyObject *const *o, const OnDevice &on)
+        : k(on.here(on_gpu(tensor(o[0])))), v(on.here(on_gpu(tensor(o[1])))), table(on.here(on_gpu(tensor(o[4]))))
+    {
+        bits = k.scalar_type() == at::kHalf ? 16 : 8;
+        require(k.dim() == 4 && k.is_contiguous() && v.is_contiguous() && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() &&
+                    (bits == 16 || k.scalar_type() == at::kFloat8_e4m3fn),
+                "paged cache: two contiguous tensors [pages, heads, page, Dp] of f16 or float8_e4m3fn expected");
+        P = k.size(0), Hkv = k.size(1), page = k.size(2);
+        ks = on.pointer(o[2], at::kFloat, P * Hkv), vs = on.pointer(o[3], at::kFloat, P * Hkv);
+        require(table.scalar_type() == at::kInt && table.dim() == 2 && (table.size(1) <= 1 || table.stride(1) == 1),
+                "paged cache: table [sequences, pages] of int32 expected");
+        B = table.size(0), W = table.size(1), ldt = B > 1 ? table.stride(0) : W;
+        require(o[5] != Py_None && o[6] != Py_None, "paged cache: starts [sequences + 1] and lens [sequences] of int32 expected");
+        starts = on.pointer(o[5], at::kInt, B + 1), lens = on.pointer(o[6], at::kInt, B);
+    }
+    void holds(int64_t Dh) const { require(k.size(3) == (Dh + 15) / 16 * 16, "paged cache: pages of another head dimension"); }
+};
+
+// (k, v, k_pages, v_pages, k_scale, v_scale, table, starts, lens, cos, sin, q, q_out, max_new, status)
+PyObject *paged_append(PyObject *const *o)
+{
+    const OnDevice on(on_gpu(tensor(o[0])));
+    const Rows k(o[0], on, "paged_append: k [T, heads, Dh] f16 expected"), v(o[1], on, "paged_append: v [T, heads, Dh] f16 expected");
+    const Paged c(o + 2, on);
+    const at::Tensor &cos = on.here(o[9], at::kHalf), &sin = on.here(o[10], at::kHalf);
+    c.holds(k.Dh);
+    require(v.t.sizes() == k.t.sizes() && k.H == c.Hkv, "paged_append: k, v and the pages have other shapes than each other");
+    require(cos.dim() == 2 && cos.size(1) == k.Dh && sin.sizes() == cos.sizes(), "paged_append: cos and sin [positions, Dh] expected");
+    int64_t H = k.H, ldq = 0, ldqo = 0;
+    void *q = nullptr, *qo = nullptr;
+    Result out = {at::Tensor(), nullptr};
+    if (o[11] != Py_None) {
+        const Rows r(o[11], on, "paged_append: q [T, heads, Dh] f16 expected");
+        require(r.T == k.T && r.Dh == k.Dh, "paged_append: q has other rows than k");
+        H = r.H, ldq = r.ld, q = r.t.data_ptr();
+        if (o[12] == Py_None) out.t = empty({r.T, r.H, r.Dh}, r.t, at::kHalf), ldqo = H * k.Dh;
+        else {
+            const Rows w(o[12], on, "paged_append: out [T, heads, Dh] f16 expected");
+            require(w.t.sizes() == r.t.sizes(), "paged_append: shape of out");
+            out = {w.t, o[12]}, ldqo = w.ld;
+        }
+        qo = out.t.data_ptr();
+    } else require(o[12] == Py_None, "paged_append: out without q");
+    const int64_t max_new = o[13] == Py_None ? k.T : number<int64_t>(o[13]);
+    require(max_new >= 0, "paged_append: max_new");
+    void *status = on.pointer(o[14], at::kInt, 1), *st = on.stream();
+    if (k.T > 0 && c.B > 0 && max_new > 0)
+        run([&] {
+            return cacti_hip_paged_append(k.T, c.B, H, k.H, k.Dh, max_new, q, ldq, k.t.data_ptr(), k.ld, v.t.data_ptr(), v.ld, cos.data_ptr(),
+                                          sin.data_ptr(), cos.size(0), qo, ldqo, c.k.data_ptr(), c.v.data_ptr(), c.ks, c.vs, c.bits, c.P,
+                                          c.page, c.table.data_ptr(), c.ldt, c.W, c.starts, c.lens, status, st);
+        });
+    if (!out.t.defined()) Py_RETURN_NONE;
+    return out.take();
+}
+
+// (q, k_pages, v_pages, k_scale, v_scale, table, starts, lens, alpha, max_new, out, status)
+PyObject *paged_attention(PyObject *const *o)
+{
+    const OnDevice on(on_gpu(tensor(o[0])));
+    const Rows q(o[0], on, "paged_attention: q [T, heads, Dh] f16 expected");
+    const Paged c(o + 1, on);
+    c.holds(q.Dh);
+    const float alpha = number<float>(o[8]);
+    const int64_t max_new = o[9] == Py_None ? q.T : number<int64_t>(o[9]);
+    require(max_new >= 0, "paged_attention: max_new");
+    Result out = {at::Tensor(), nullptr};
+    int64_t ldo = q.H * q.Dh;
+    if (o[10] == Py_None) out.t = empty({q.T, q.H, q.Dh}, q.t, at::kHalf);
+    else {
+        const Rows w(o[10], on, "paged_attention: out [T, heads, Dh] f16 expected");
+        require(w.t.sizes() == q.t.sizes(), "paged_attention: shape of out");
+        out = {w.t, o[10]}, ldo = w.ld;
+    }
+    void *status = on.pointer(o[11], at::kInt, 1), *st = on.stream();
+    if (q.T > 0 && c.B > 0 && max_new > 0) {
+        const size_t bytes = cacti_hip_paged_attention_workspace(q.T, c.B, q.H, c.Hkv, q.Dh, max_new, c.page, c.W);
+        const at::Tensor ws = bytes ? empty({(int64_t)bytes}, q.t, at::kByte) : at::Tensor();
+        run([&] {
+            return cacti_hip_paged_attention_f16(q.T, c.B, q.H, c.Hkv, q.Dh, max_new, alpha, q.t.data_ptr(), q.ld, c.k.data_ptr(),
+                                                 c.v.data_ptr(), c.ks, c.vs, c.bits, c.P, c.page, c.table.data_ptr(), c.ldt, c.W, c.starts,
+                                                 c.lens, out.ptr(), ldo, bytes ? ws.data_ptr() : nullptr, bytes, status, st);
+        });
+    }
+    return out.take();
+}
+
+// (target, draft, tok, starts, u, r, temperature, status): (accepted, next)
+PyObject *verify_draft(PyObject *const *o)
+{
+    const OnDevice on(on_gpu(tensor(o[0])));
+    const Logits t(o[0], on, "verify_draft: target [T, V] f16 expected");
+    const void *draft = nullptr;
+    int64_t ldd = 0;
+    if (o[1] != Py_None) {
+        const Logits d(o[1], on, "verify_draft: draft [T, V] f16 expected");
+        require(d.t.sizes() == t.t.sizes(), "verify_draft: draft has another shape than target");
+        draft = d.t.data_ptr(), ldd = d.ld;
+    }
+    const at::Tensor &starts = on.here(o[3], at::kInt);
+    const int64_t B = starts.numel() - 1;
+    require(B >= 0, "verify_draft: starts [sequences + 1] expected");
+    void *tok = on.pointer(o[2], at::kShort, t.N), *u = on.pointer(o[4], at::kFloat, t.N), *r = on.pointer(o[5], at::kFloat, B);
+    const double temperature = number<double>(o[6]);
+    void *status = on.pointer(o[7], at::kInt, 1), *st = on.stream();
+    const Result accepted = {empty({B}, t.t, at::kInt), nullptr}, next = {empty({t.N}, t.t, at::kShort), nullptr};
+    if (t.N > 0 && B > 0) {
+        const size_t bytes = cacti_hip_verify_draft_workspace(t.N, t.V);
+        const at::Tensor ws = empty({(int64_t)bytes}, t.t, at::kByte);
+        run([&] {
+            return cacti_hip_verify_draft_f16(t.N, B, t.V, t.t.data_ptr(), t.ld, draft, ldd, tok, starts.data_ptr(), u, r, temperature,
+                                              accepted.ptr(), next.ptr(), ws.data_ptr(), bytes, status, st);
+        });
+    } else if (B > 0) accepted.t.zero_();
+    return take2(accepted, next);
+}
+
+// (logit, idx, val, temperature, status): (loss, stats)
+PyObject *distill_topk_fwd(PyObject *const *o)
+{
+    const OnDevice on(on_gpu(tensor(o[0])));
+    const Logits z(o[0], on, "distill_topk: logits [N, V] f16 expected");
+    const at::Tensor &idx = on.here(o[1], at::kShort), &val = on.here(o[2], at::kHalf);
+    require(idx.dim() == 2 && idx.size(0) == z.N && val.sizes() == idx.sizes(), "distill_topk: idx and val [N, K] expected");
+    const double temperature = number<double>(o[3]);
+    void *status = on.pointer(o[4], at::kInt, 1), *st = on.stream();
+    const Result loss = {empty({z.N}, z.t, at::kFloat), nullptr}, stats = {empty({z.N, 2}, z.t, at::kFloat), nullptr};
+    if (z.N > 0)
+        run([&] {
+            return cacti_hip_distill_topk_fwd(z.N, z.V, idx.size(1), z.t.data_ptr(), z.ld, idx.data_ptr(), val.data_ptr(), temperature,
+                                              loss.ptr(), stats.ptr(), status, st);
+        });
+    return take2(loss, stats);
+}
+
+// (logit, idx, val, stats, scale, temperature, acc)
+PyObject *distill_topk_bwd(PyObject *const *o)
+{
+    const OnDevice on(on_gpu(tensor(o[0])));
+    const Logits z(o[0], on, "distill_topk: logits [N, V] f16 expected");
+    const at::Tensor &idx = on.here(o[1], at::kShort), &val = on.here(o[2], at::kHalf);
+    require(idx.dim() == 2 && idx.size(0) == z.N && val.sizes() == idx.sizes(), "distill_topk: idx and val [N, K] expected");
+    const void *stats = on.pointer(o[3], at::kFloat, 2 * z.N), *scale = on.pointer(o[4], at::kFloat, z.N);
+    const double temperature = number<double>(o[5]);
+    Result d = {at::Tensor(), nullptr};
+    int64_t ldd = z.V;
+    if (o[6] == Py_None) d.t = empty({z.N, z.V}, z.t, at::kHalf);
+    else {
+        const Logits w(o[6], on, "distill_topk: acc [N, V] f16 expected");
+        require(w.t.sizes() == z.t.sizes(), "distill_topk: shape of acc");
+        d = {w.t, o[6]}, ldd = w.ld;
+    }
+    void *st = on.stream();
+    if (z.N > 0)
+        run([&] {
+            return cacti_hip_distill_topk_bwd(z.N, z.V, idx.size(1), z.t.data_ptr(), z.ld, idx.data_ptr(), val.data_ptr(), stats, scale,
+                                              temperature, d.ptr(), ldd, d.acc(), st);
+        });
+    return d.take();
+}
+
 // (xs)
 PyObject *digests(PyObject *const *v)
 {
@@ -566,6 +786,11 @@ PyMethodDef methods[] = {
     OP(silu_gate_bwd, 5),
     OP(add_f16, 3),
     OP(softmax_ce_bwd, 4),
+    OP(paged_append, 15),
+    OP(paged_attention, 12),
+    OP(verify_draft, 8),
+    OP(distill_topk_fwd, 5),
+    OP(distill_topk_bwd, 7),
     OP(digests, 1),
     OP(adamw32_step, 6),
     OP(adamw32_scalars, 7),

@@ -426,6 +426,80 @@ int cacti_hip_embed_fwd(int64_t V, int64_t D, const void *W, int64_t S, const vo
 int cacti_hip_embed_bwd(int64_t V, int64_t D, int64_t S, const void *tok, const void *dy,
                         void *dW, int acc, void *stream);
 
+/* ------------------------------------------------------------------------- */
+/* Many sequences at once: a paged key / value cache, drafted tokens and the   */
+/* loss that trains the drafting model.  The reference decodes one sequence    */
+/* from one slab per layer (src/librarium/llama.rs:561-963); these stand       */
+/* beside cacti_hip_rows_qkv_rope_cache_f16, cacti_hip_attn_decode_f16 and     */
+/* cacti_hip_softmax_ce_*.                                                     */
+/*                                                                             */
+/* A batch of B sequences.  Rows starts[b] .. starts[b + 1] - 1 of its tensors are the new tokens of sequence b (none: left out),
+ * lens[b] its positions with them: its row i is at position lens[b] - n + i.  Position p lies in slot p % page of page
+ * table[b * ldt + p / page] of the cache.  starts [B + 1], lens [B], table [B, W] are i32 on the device and are not read by
+ * the host: nothing waits, and a captured launch follows them.  T: rows there are (those from starts[B] on are left as they
+ * are); max_new: no sequence has more new rows (T will do; the less, the fewer idle workgroups).
+ * Cache: pages [P, Hkv, page, Dp], Dp = Dh rounded up to 16, the columns from Dh on zeros; bits = 16: f16, scales NULL;
+ * bits = 8: e4m3 (OCP, no infinities) with scales [P, Hkv] f32, a value being code * scale.  A page is of one sequence where
+ * that appends; reading it may be shared.  Heads: H of the queries, Hkv of the cache, H % Hkv == 0, query head h reads
+ * h / (H / Hkv).  Dh % 4 == 0, Dh <= 128; page: a multiple of 16, at most 256; k, v, q, out: rows of ld elements, 8-byte
+ * aligned, ld % 4 == 0; pages 16-byte aligned.
+ * status [1] i32 on the device, or NULL: 1 + b where the numbers of sequence b do not fit together (rows beyond T, more new
+ * rows than max_new or than positions, more positions than its row of the table or the rotation has, a page that is not in
+ * the cache), raised with a maximum: the caller clears it.  Nothing of such a sequence is appended (with a page outside the
+ * cache: nothing of that page), and its rows of the attention are zeros (with a page outside the cache: unspecified). */
+
+/* New keys and values into their pages, the keys rotated as by symplectic_embed (src/librarium/llama.rs:463-465; tables as
+ * cacti_hip_rope_tables fills them, n_pos rows), and, where q is not NULL, q_rot = the queries rotated: in fp32, rounded once.
+ * bits = 8: the scale of a page and head is the least 2^e, -32 <= e <= 15, with all finite new values of the page up to
+ * 448 * 2^e, and no less than before where the page has older positions; their codes are carried over where it grew.  (Scales
+ * are powers of two: the quotient and, but for subnormal codes, that are exact.)  NaN and infinities become NaN.  Slots behind
+ * the new ones stay as they are. */
+int cacti_hip_paged_append(int64_t T, int64_t B, int64_t H, int64_t Hkv, int64_t Dh, int64_t max_new, const void *q, int64_t ldq,
+                           const void *k, int64_t ldk, const void *v, int64_t ldv, const void *cos16, const void *sin16,
+                           int64_t n_pos, void *q_rot, int64_t ldqr, void *k_pages, void *v_pages, void *k_scale, void *v_scale,
+                           int bits, int64_t P, int64_t page, const void *table, int64_t ldt, int64_t W, const void *starts,
+                           const void *lens, void *status, void *stream);
+
+/* out [T, ldo] f16 = softmax_j(alpha q . k_j) v over the positions j up to the row's own, which are in the cache; fp32 scores
+ * and sums, the weights rounded to f16 for the second product.  A row's result depends on nothing behind its position.  Scales
+ * are positive, any of them.  workspace: cacti_hip_paged_attention_workspace bytes (0: none), 16-byte aligned, contents
+ * undefined on return. */
+size_t cacti_hip_paged_attention_workspace(int64_t T, int64_t B, int64_t H, int64_t Hkv, int64_t Dh, int64_t max_new, int64_t page,
+                                           int64_t W);
+int cacti_hip_paged_attention_f16(int64_t T, int64_t B, int64_t H, int64_t Hkv, int64_t Dh, int64_t max_new, float alpha,
+                                  const void *q, int64_t ldq, const void *k_pages, const void *v_pages, const void *k_scale,
+                                  const void *v_scale, int bits, int64_t P, int64_t page, const void *table, int64_t ldt, int64_t W,
+                                  const void *starts, const void *lens, void *out, int64_t ldo, void *workspace,
+                                  size_t workspace_bytes, void *status, void *stream);
+
+/* Verification of drafted tokens: rows of a sequence are its last token and the drafted ones (starts as above, n - 1 of them),
+ * tok [T] u16 the rows' tokens, target [T, ldt] f16 the target model's logits of every row, draft [T, ldd] the drafting
+ * model's (its last row per sequence is not read), or NULL: a token that was drafted without probabilities.  With
+ * p = softmax(target / temperature), q = softmax(draft / temperature) (NULL: one-hot at the drafted token) the token x of row
+ * i + 1 is kept if u[i] q_i(x) < p_i(x); a = the first row whose token is not, or the last; the token behind row a is the least
+ * j with sum_{i <= j} w_i > r[b] sum w, w = max(p_a - q_a, 0), or p_a behind the last row (and where p = q).  temperature 0:
+ * the first arg max, and tokens are kept that are it.  u [T], r [B]: f32 in [0, 1).  accepted [B] i32 = a (0 for a sequence
+ * without rows), next [T] u16 = the tokens behind the rows: those that are kept, the one of row a, then 0.  In fp64.  A NaN
+ * logit counts as -inf, a row without a finite one as even.  status [1] i32 or NULL: 1 + the row of a token >= V (never
+ * kept), 1 for rows beyond T.  workspace: cacti_hip_verify_draft_workspace bytes.  V <= 65536. */
+size_t cacti_hip_verify_draft_workspace(int64_t T, int64_t V);
+int cacti_hip_verify_draft_f16(int64_t T, int64_t B, int64_t V, const void *target, int64_t ldt, const void *draft, int64_t ldd,
+                               const void *tok, const void *starts, const void *u, const void *r, double temperature,
+                               void *accepted, void *next, void *workspace, size_t workspace_bytes, void *status, void *stream);
+
+/* Distillation from a teacher's top logits: idx [N,K] u16, val16 [N,K] f16 against the student's logit16 [N,V] f16 (row pitch
+ * ld), t = softmax(val / temperature), p = softmax(logit / temperature):
+ *   loss[n] = sum_i t_i (log t_i - log p(idx_i))
+ *   dlogit[j] (+)= f16(scale[n] / temperature * (p_j sum t - sum_{idx_i = j} t_i))
+ * loss, scale: [N] f32; stats [N,2] f32: maximum and sum, written by the forward call, read by the adjoint.  An entry of -inf
+ * has no weight; a row without any has loss 0 and gradient 0; the same id twice counts twice.  K <= 1024, V <= 65536, any
+ * alignment of the rows.  status [1] i32 or NULL: 1 + the row of an id >= V (left out).  acc as everywhere. */
+int cacti_hip_distill_topk_fwd(int64_t N, int64_t V, int64_t K, const void *logit16, int64_t ld, const void *idx, const void *val16,
+                               double temperature, void *loss, void *stats, void *status, void *stream);
+int cacti_hip_distill_topk_bwd(int64_t N, int64_t V, int64_t K, const void *logit16, int64_t ld, const void *idx, const void *val16,
+                               const void *stats, const void *scale, double temperature, void *dlogit16, int64_t ldd, int acc,
+                               void *stream);
+
 /* f16 residual add y = a + b (AddFutThunkSpec src/thunk/op.rs:1480-1535); y may alias a or b. */
 int cacti_hip_add_f16(int64_t n, const void *a, const void *b, void *y, void *stream);
 
