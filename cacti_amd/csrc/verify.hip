@@ -10,211 +10,429 @@
 //
 // Exponentials and sums are fp64: what is drawn goes by on which side of a border of the running sum r lies, and with sums that
 // are off by e of their total some V e of all draws come out differently (32000 tokens, fp32 sums: one in several hundred).
+// That arithmetic, some 19 operations of 64 bits a logit, is what bounds a batch (twice the time that its bytes take).
 //
-// A workgroup per row: maxima, sums, whether the drafted token is kept and, unless it is, the token that would follow; then a
-// workgroup per sequence picks the first row that ends it.
+// A row is cut into entries of 1024 logits, one to a wave, which needs no barrier and spreads five rows over 80 workgroups: their
+// maxima and sums relative to them, of every row of both models.  Then a workgroup per sequence forms the rows' sums from
+// them, sees which drafted tokens are kept and sums what is left of p in the first row whose token is not, entry by entry; one of
+// its waves finds the entry in which r lies and the token in it.
+// us, five rows of 32000 with a drafting model / 64 sequences, 294 rows: a workgroup per row that drew for every row that might
+// end its sequence 77 / 115; a launch of its own for the last step, which waits for memory four times over, 22.5 / 38.6.
 #include "vocab_row.h"
 
 using namespace cacti;
 
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kRounds = 4, kPieces = 64 * kRounds;         // 16-byte pieces of an entry
+constexpr int kHalf = 128;                     // of an entry of what is left of p
+constexpr int kEntryWaves = 4;                 // entries of a workgroup of the first kernel
+constexpr int kThreads = 512, kWaves = kThreads / 64;
+constexpr int kDraw = 1024;                    // lanes of the last kernel: two logits each
+
+struct __attribute__((aligned(16))) Entry {
+    double z;                                  // sum of exponentials relative to the entry's maximum; greedy: its first arg max
+    double m;
+};
+// The row that ends a sequence, -1 where its numbers do not fit together
+struct Head {
+    int row, residual, x;                           // whether a drafted token was not kept, which
+    float mt, md;
+    double it, id;                             // 1 / sums
+};
+
+struct Scale {
+    double c;                                  // log2 e / temperature
+    float span;                                // 1000 / c
+};
 
 struct VerifyArgs {
-    int T, B, V;
+    int T, B, V, E, E2;                        // E, E2: entries of a row, of what is left of p
     const half_t *target, *draft;
     int64_t ldt, ldd;
     const uint16_t *tok;
     const int *starts;
     const float *u, *r;
-    double inv_temp;                           // 0: greedy
-    int *verdict;                              // [T]: -1 where the drafted token is kept, else the token that follows the row
+    Scale c;
+    Entry *entries;                            // [2][T][E]: target, draft
+    double *left;                              // [B][E2]: sums of what is left of p
+    Head *heads;
     int *accepted;
     uint16_t *next;
     int *status;
 };
 
-// A NaN is never chosen; the difference of equal infinities is 0
-__device__ __forceinline__ float clean(half_t x) { return x != x ? -INFINITY : h2f(x); }
-__device__ __forceinline__ double weight(float x, float mx, double inv_temp)
+// 2^t for -1022 <= t <= 0: t = n + f, |f| <= 1/2, a polynomial of degree 9 in f (Chebyshev interpolation on that interval,
+// 2e-14) and n added to its exponent
+__device__ __forceinline__ double exp2_neg(double t)
 {
-    return x == mx ? 1.0 : x == -INFINITY ? 0.0 : exp(((double)x - (double)mx) * inv_temp);
+    const double magic = 0x1.8p52, s = t + magic, f = t - (s - magic);        // the sum's low word is n
+    double p = 1.0205905724567723e-07;
+    p = __builtin_fma(p, f, 1.3259645239858464e-06);
+    p = __builtin_fma(p, f, 1.5252672923029364e-05);
+    p = __builtin_fma(p, f, 0.00015403433751274572);
+    p = __builtin_fma(p, f, 0.0013333558200798331);
+    p = __builtin_fma(p, f, 0.0096181291939342831);
+    p = __builtin_fma(p, f, 0.055504108664651643);
+    p = __builtin_fma(p, f, 0.24022650695640341);
+    p = __builtin_fma(p, f, 0.69314718055994617);
+    p = __builtin_fma(p, f, 1.0000000000000135);
+    return __builtin_amdgcn_ldexp(p, (int)__builtin_bit_cast(uint64_t, s));
+}
+constexpr double kNothing = 1e-290;            // weights below that are those of -inf
+
+// A NaN is never chosen
+__device__ __forceinline__ float clean(half_t x) { return fmaxf(h2f(x), -INFINITY); }
+// What makes weights of logits relative to a maximum: 2^(x c - mx c).  What is 1000 below it, and so -inf and a NaN, is held
+// there (in fp32, where the temperature's lower bound leaves 16 to spare).  A maximum that is no infinity.
+struct Weight {
+    double c, b;
+    float low;
+    __device__ __forceinline__ Weight(float mx, const Scale &s) : c(s.c), b(-(double)mx * s.c), low(mx - s.span) {}
+    __device__ __forceinline__ double operator()(float x) const { return exp2_neg(__builtin_fma((double)fmaxf(x, low), c, b)); }
+};
+// ... any: of infinities 1 for those that are it, 0 for the others
+__device__ __forceinline__ double weight(float x, float mx, const Scale &s)
+{
+    const bool fine = fabsf(mx) < INFINITY;
+    return Weight(fine ? mx : 0.f, s)(fine ? x : x == mx ? 0.f : -INFINITY);
 }
 
-__device__ double block_sum(double v, double *red)
+// inclusive sum over the lanes
+__device__ __forceinline__ double lane_f64(double v, int lane)
 {
-    v = wave_sum_f64(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    double s = 0.;
-    for (int w = 0; w < kWaves; w++) s += red[w];
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return words_f64(__builtin_amdgcn_readlane((int)u, lane), __builtin_amdgcn_readlane((int)(u >> 32), lane));
+}
+__device__ __forceinline__ double scan_f64(double v)
+{
+    v += dpp_f64<0x111>(v);                    // row_shr 1, 2, 4, 8: nothing from before the 16
+    v += dpp_f64<0x112>(v);
+    v += dpp_f64<0x114>(v);
+    v += dpp_f64<0x118>(v);
+    const double r0 = lane_f64(v, 15), r1 = lane_f64(v, 31), r2 = lane_f64(v, 47);
+    const int row = (threadIdx.x & 63) >> 4;
+    return v + (row == 0 ? 0. : row == 1 ? r0 : row == 2 ? r0 + r1 : r0 + r1 + r2);
+}
+
+template <bool GREEDY>
+__global__ void __launch_bounds__(64 * kEntryWaves) verify_entries_kernel(VerifyArgs a)
+{
+    const int row = blockIdx.x, e = blockIdx.y * kEntryWaves + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const bool drafting = blockIdx.z == 1;
+    if (e >= a.E) return;
+    const VocabRow t(drafting ? a.draft + row * a.ldd : a.target + row * a.ldt, a.V);
+    Entry *to = a.entries + ((int64_t)blockIdx.z * a.T + row) * a.E + e;
+    h8 v[kRounds];
+#pragma unroll
+    for (int r = 0; r < kRounds; r++) {
+        const int c = e * kPieces + r * 64 + lane;
+        if (c < t.pieces()) v[r] = t.load(c, (half_t)-INFINITY);
+        else
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[r].v[k] = (half_t)-INFINITY;
+    }
+    if (drafting) {                            // a sequence's last row has no drafted token behind it
+        bool last = false;
+        for (int i = 1 + lane; i <= a.B; i += 64) last = last || a.starts[i] == row + 1;
+        if (__ballot(last)) return;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < kRounds; r++)
+#pragma unroll
+        for (int k = 0; k < 8; k++) mx = fmaxf(mx, h2f(v[r].v[k]));
+    mx = wave_max(mx);
+    double z = 0.;
+    if (GREEDY) {
+        int at = 65536;
+#pragma unroll
+        for (int r = kRounds - 1; r >= 0; r--)
+#pragma unroll
+            for (int k = 7; k >= 0; k--) {
+                const int j = t.first(e * kPieces + r * 64 + lane) + k;
+                if (j >= 0 && j < a.V && clean(v[r].v[k]) == mx) at = j;
+            }
+        z = -(double)wave_max(-(float)at);
+    } else {
+        if (fabsf(mx) < INFINITY) {
+            const Weight w(mx, a.c);
+#pragma unroll
+            for (int r = 0; r < kRounds; r++)
+#pragma unroll
+                for (int k = 0; k < 8; k++) z += w(h2f(v[r].v[k]));
+        } else {
+#pragma unroll
+            for (int r = 0; r < kRounds; r++)
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const int j = t.first(e * kPieces + r * 64 + lane) + k;
+                    z += j >= 0 && j < a.V && clean(v[r].v[k]) == mx ? 1. : 0.;
+                }
+        }
+        z = wave_sum_f64(z);
+    }
+    if (lane == 0) *to = Entry{z, (double)mx};
+}
+
+// A row's maximum and sum, by a wave (with no more than 64 entries)
+struct RowSum {
+    float m;
+    double z;
+};
+__device__ __forceinline__ RowSum row_sum(const VerifyArgs &a, const Entry *en)
+{
+    const int lane = threadIdx.x & 63;
+    const Entry none = {0., -INFINITY}, e = lane < a.E ? en[lane] : none;
+    RowSum s;
+    s.m = wave_max((float)e.m);
+    s.z = wave_sum_f64(e.z * weight((float)e.m, s.m, a.c));
     return s;
 }
 
-// The sequence of a row, or B: starts do not fall
-__device__ int sequence_of(const VerifyArgs &a, int row)
+// The rows of sequence b up to the first that ends it, a wave to each; `ends` says whether a row does.  Returns that row.
+template <class F>
+__device__ __forceinline__ int first_end(int s0, int s1, int *stops, F ends)
 {
-    int c = 0;
-    for (int i0 = 1; i0 <= a.B; i0 += 64) {
-        const int i = i0 + (threadIdx.x & 63);
-        c += __popcll(__ballot(i <= a.B && a.starts[i] <= row));
+    const int wid = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    for (int i0 = s0;; i0 += kWaves) {
+        const int row = i0 + wid;
+        const bool stop = row >= s1 || ends(row, wid);
+        __syncthreads();
+        if (lane == 0) stops[wid] = stop;
+        __syncthreads();
+        for (int w = 0; w < kWaves; w++)
+            if (stops[w]) return i0 + w;       // (s1 - 1 ends, so this is below s1)
     }
-    return c;
+}
+
+__device__ __forceinline__ bool rows_of(const VerifyArgs &a, int b, int *s0, int *s1)
+{
+    *s0 = a.starts[b];
+    *s1 = a.starts[b + 1];
+    return *s0 >= 0 && *s1 <= a.T && *s1 > *s0;
+}
+
+// What follows: next[s0 .. s1 - 1] and accepted[b], of row `end` that ends the sequence and the token behind it; by NT lanes
+template <int NT>
+__device__ __forceinline__ void write_out(const VerifyArgs &a, int b, int s0, int s1, int end, int token)
+{
+    for (int i = s0 + threadIdx.x; i < s1; i += NT) a.next[i] = i < end ? a.tok[i + 1] : i == end ? (uint16_t)token : (uint16_t)0;
+    if (threadIdx.x == 0) a.accepted[b] = end - s0;
+}
+
+// The code of the next kernel runs once per lane or a few times, so it is short: what is unrolled is fetched from memory for
+// one use (16 logits of both models unrolled, in three places, were 49 KB and some 20 us).
+
+// What is left of p = softmax(target) where the drafting model's q has been taken off, or the token that was drafted
+struct Left {
+    const half_t *t, *d;                       // d null: none
+    float mt, md;
+    double it, id;
+    Scale c;
+    int x, V;
+    __device__ __forceinline__ Left(const VerifyArgs &a, const Head &h)
+        : t(a.target + h.row * a.ldt), d(a.draft && h.residual ? a.draft + h.row * a.ldd : nullptr), mt(h.mt), md(h.md), it(h.it), id(h.id),
+          c(a.c), x(h.x), V(a.V)
+    {
+    }
+    // of logit j, whose logits are ht and hd
+    __device__ __forceinline__ double operator()(half_t ht, half_t hd, int j, bool residual) const
+    {
+        double y = weight(clean(ht), mt, c) * it;
+        if (residual) {
+            if (d) y -= weight(clean(hd), md, c) * id;
+            else if (j == x) y = 0.;
+        }
+        return j >= 0 && j < V && y > kNothing ? y : 0.;
+    }
+};
+
+// Eight halves, the first taken off at a time
+struct Eight {
+    uint64_t lo, hi;
+    __device__ __forceinline__ explicit Eight(const h8 &v)
+    {
+        uint64_t w[2];
+        __builtin_memcpy(w, &v, 16);
+        lo = w[0];
+        hi = w[1];
+    }
+    __device__ __forceinline__ half_t take()
+    {
+        const half_t x = __builtin_bit_cast(half_t, (uint16_t)lo);
+        lo = lo >> 16 | hi << 48;
+        hi >>= 16;
+        return x;
+    }
+};
+
+// The first of a block's lanes that `hit`s, else (by a rounding) the last that has any weight: lane numbers, by LDS
+__device__ __forceinline__ int pick_lane(bool hit, bool any, int *first, int *last)
+{
+    if (threadIdx.x == 0) *first = INT32_MAX, *last = 0;
+    __syncthreads();
+    const uint64_t h = __ballot(hit), y = __ballot(any);
+    if ((threadIdx.x & 63) == 0) {
+        if (h) atomicMin(first, (int)threadIdx.x + __ffsll((unsigned long long)h) - 1);
+        if (y) atomicMax(last, (int)threadIdx.x + 63 - __clzll((long long)y));
+    }
+    __syncthreads();
+    return *first < INT32_MAX ? *first : *last;
 }
 
 __global__ void __launch_bounds__(kThreads) verify_rows_kernel(VerifyArgs a)
 {
-    __shared__ float red[kWaves];
-    __shared__ double redd[kWaves];
-    __shared__ unsigned found;
-    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-    const int b = sequence_of(a, row);
-    if (b >= a.B || row < a.starts[b]) return;
-    const bool last = row + 1 >= a.starts[b + 1] || row + 1 >= a.T;
-    const int x = last ? -1 : a.tok[row + 1];
-    const bool bad = !last && x >= a.V;        // never kept
-    if (bad && tid == 0 && a.status) atomicMax(a.status, row + 2);
-    const VocabRow t(a.target + row * a.ldt, a.V);
-    const bool greedy = a.inv_temp == 0.;
-    const bool drafted = a.draft && !last && !greedy;
-    const VocabRow d(drafted ? a.draft + row * a.ldd : t.row, a.V);
-    float mt = -INFINITY, md = -INFINITY;
-    for (int c = tid; c < t.pieces(); c += kThreads) {
-        const h8 v = t.load(c, (half_t)-INFINITY);
-#pragma unroll
-        for (int k = 0; k < 8; k++) mt = fmaxf(mt, clean(v.v[k]));
-    }
-    mt = block_reduce(mt, OpMax(), -INFINITY, red);
-    if (greedy) {
-        if (tid == 0) found = 0xffffffffu;
-        __syncthreads();
-        for (int c = tid; c < t.pieces(); c += kThreads) {
-            const h8 v = t.load(c, (half_t)-INFINITY);
-#pragma unroll
-            for (int k = 7; k >= 0; k--) {
-                const int j = t.first(c) + k;
-                if (j >= 0 && j < a.V && clean(v.v[k]) == mt) atomicMin(&found, (unsigned)j);
-            }
+    __shared__ int stops[kWaves];
+    __shared__ Head found[kWaves];
+    const int b = blockIdx.y, wid = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    int s0, s1;
+    if (!rows_of(a, b, &s0, &s1)) {
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
+            a.heads[b].row = -1;
+            if (s1 != s0 && a.status) atomicMax(a.status, 1);
         }
-        __syncthreads();
-        if (tid == 0) a.verdict[row] = !last && !bad && x == (int)found && a.u[row] < 1.f ? -1 : (int)found;
         return;
     }
-    double zt = 0., zd = 1.;
-    for (int c = tid; c < t.pieces(); c += kThreads) {
-        const h8 v = t.load(c, (half_t)-INFINITY);
+    const int row = first_end(s0, s1, stops, [&](int i, int w) {
+        const bool last = i + 1 >= s1, drafted = a.draft && !last;
+        const int x = last ? 0 : a.tok[i + 1], at = min(x, a.V - 1);
+        const bool bad = x >= a.V;
+        // (the drafted token's logits requested with the sums, not behind them)
+        const float xt = clean(a.target[i * a.ldt + at]), xd = drafted ? clean(a.draft[i * a.ldd + at]) : 0.f, u = a.u[i];
+        const RowSum t = row_sum(a, a.entries + (int64_t)i * a.E);
+        RowSum d = {0.f, 1.};
+        if (drafted) d = row_sum(a, a.entries + ((int64_t)a.T + i) * a.E);
+        const double it = 1. / t.z, id = 1. / d.z;
+        if (lane == 0) found[w] = Head{i, !last, x, t.m, d.m, it, id};
+        if (bad && lane == 0 && a.status) atomicMax(a.status, i + 2);
+        const double q = drafted ? weight(xd, d.m, a.c) * id : 1.;
+        return last || bad || !((double)u * q < weight(xt, t.m, a.c) * it);
+    });
+    const Head h = found[(row - s0) & (kWaves - 1)];
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.heads[b] = h;
+    const int e = blockIdx.x * kWaves + wid;
+    if (!h.residual || e >= a.E2) return;      // (the entries' sums of p are there)
+    const Left lf(a, h);
+    const VocabRow t(lf.t, a.V);
+    const bool alike = lf.d && ((reinterpret_cast<uintptr_t>(lf.d) ^ reinterpret_cast<uintptr_t>(lf.t)) & 15) == 0;
+    double sum = 0.;
+    h8 v[2] = {}, u[2] = {};
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const int j = t.first(c) + k;
-            if (j >= 0 && j < a.V) zt += weight(clean(v.v[k]), mt, a.inv_temp);
-        }
-    }
-    zt = block_sum(zt, redd);
-    if (drafted) {
-        for (int c = tid; c < d.pieces(); c += kThreads) {
-            const h8 v = d.load(c, (half_t)-INFINITY);
+    for (int r = 0; r < 2; r++) {
+        const int p = e * kHalf + r * 64 + lane, j0 = t.first(p);
+        if (p >= t.pieces()) continue;
+        v[r] = t.load(p, (half_t)0.f);
+        if (alike && t.whole(p)) u[r] = ld8(lf.d + j0);
+        else if (lf.d)
 #pragma unroll
-            for (int k = 0; k < 8; k++) md = fmaxf(md, clean(v.v[k]));
-        }
-        md = block_reduce(md, OpMax(), -INFINITY, red);
-        zd = 0.;
-        for (int c = tid; c < d.pieces(); c += kThreads) {
-            const h8 v = d.load(c, (half_t)-INFINITY);
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const int j = d.first(c) + k;
-                if (j >= 0 && j < a.V) zd += weight(clean(v.v[k]), md, a.inv_temp);
-            }
-        }
-        zd = block_sum(zd, redd);
+            for (int k = 0; k < 8; k++) u[r].v[k] = lf.d[min(max(j0 + k, 0), a.V - 1)];
     }
-    const double it = 1. / zt, id = 1. / zd;
-    if (!last && !bad) {
-        const double p = weight(clean(t.row[x]), mt, a.inv_temp) * it;
-        const double q = drafted ? weight(clean(d.row[x]), md, a.inv_temp) * id : 1.;
-        if ((double)a.u[row] * q < p) {
-            if (tid == 0) a.verdict[row] = -1;
-            return;
-        }
-    }
-    // weight of token j of what is left; residual: what the drafting model does not have of it
-    auto left = [&](int j, bool residual) {
-        double w = weight(clean(t.row[j]), mt, a.inv_temp) * it;
-        if (residual) w = drafted ? w - weight(clean(d.row[j]), md, a.inv_temp) * id : j == x ? 0. : w;
-        return w > 0. ? w : 0.;
-    };
-    // a lane has a run of tokens, lanes and waves those that follow
-    const int per = (a.V + kThreads - 1) / kThreads, j0 = min(tid * per, a.V), j1 = min(j0 + per, a.V);
-    bool residual = !last;
-    double mine = 0., total;
-    for (;;) {
-        mine = 0.;
-        for (int j = j0; j < j1; j++) mine += left(j, residual);
-        total = block_sum(mine, redd);
-        if (total > 0. || !residual) break;
-        residual = false;                      // p = q: nothing is left of it
-    }
-    const double want = (double)a.r[b] * total;
-    double before = 0.;                        // of the waves before this one
-    for (int w = 0; w < wid; w++) before += redd[w];
-    double upto = mine;                        // inclusive sum over the lanes
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-        const double o = __shfl_up(upto, s);
-        if (lane >= s) upto += o;
-    }
-    upto += before;
-    if (tid == 0) found = 0xffffffffu;
-    __syncthreads();
-    if (upto > want && mine > 0.) atomicMin(&found, (unsigned)tid);
-    __syncthreads();
-    unsigned owner = found;
-    if (owner == 0xffffffffu) {                // beyond the last by a rounding: the last with any weight
-        __syncthreads();
-        if (tid == 0) found = 0;
-        __syncthreads();
-        if (mine > 0.) atomicMax(&found, (unsigned)tid);
-        __syncthreads();
-        owner = found;
-    }
-    if (tid == (int)owner) {
-        double c = upto - mine;
-        int pick = j0;
-        for (int j = j0; j < j1; j++) {
-            const double w = left(j, residual);
-            c += w;
-            if (w > 0.) pick = j;
-            if (w > 0. && c > want) break;
-        }
-        a.verdict[row] = min(pick, a.V - 1);
-    }
+    Eight v0(v[0]), v1(v[1]), u0(u[0]), u1(u[1]);
+    const int j0 = t.first(e * kHalf + lane);
+#pragma unroll 1
+    for (int k = 0; k < 8; k++) sum += lf(v0.take(), u0.take(), j0 + k, true) + lf(v1.take(), u1.take(), j0 + 512 + k, true);
+    sum = wave_sum_f64(sum);
+    if (lane == 0) a.left[(int64_t)b * a.E2 + e] = sum;
 }
 
-__global__ void __launch_bounds__(64) verify_pick_kernel(VerifyArgs a)
+__global__ void __launch_bounds__(kDraw) verify_draw_kernel(VerifyArgs a)
 {
-    const int b = blockIdx.x, lane = threadIdx.x;
+    __shared__ double waves[kDraw / 64];
+    __shared__ int first, last;
+    const int b = blockIdx.x, wid = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const Head h = a.heads[b];
     const int s0 = a.starts[b], s1 = a.starts[b + 1];
-    if (s0 < 0 || s1 > a.T || s1 < s0) {
-        if (lane == 0 && a.status) atomicMax(a.status, 1);
-        if (lane == 0) a.accepted[b] = 0;
+    const double r = (double)a.r[b];
+    if (h.row < 0) {
+        if (threadIdx.x == 0) a.accepted[b] = 0;
         return;
     }
-    int end = s1;                              // the first row that is not kept
-    for (int i0 = s0; i0 < s1 && end == s1; i0 += 64) {
-        const uint64_t stop = __ballot(i0 + lane < s1 && a.verdict[min(i0 + lane, s1 - 1)] >= 0);
-        if (stop) end = i0 + __ffsll((unsigned long long)stop) - 1;
+    auto block_scan = [&](double v, double *total) {
+        const double in = scan_f64(v);
+        __syncthreads();
+        if (lane == 63) waves[wid] = in;
+        __syncthreads();
+        double before = 0.;
+        *total = 0.;
+        for (int w = 0; w < kDraw / 64; w++) {
+            if (w == wid) before = *total;
+            *total += waves[w];
+        }
+        return in + before;
+    };
+    // the entry in which r lies, one to a lane
+    const int en = threadIdx.x;
+    double mine = en < a.E2 && h.residual ? a.left[(int64_t)b * a.E2 + en] : 0., total;
+    double upto = block_scan(mine, &total);
+    const bool residual = h.residual && total > kNothing;        // p = q: nothing is left of it
+    if (!residual) {
+        mine = 0.;
+        if (en < a.E) {
+            const Entry x = a.entries[(int64_t)h.row * a.E + en];
+            mine = x.z * weight((float)x.m, h.mt, a.c) * h.it;
+        }
+        upto = block_scan(mine, &total);
     }
-    for (int i = s0 + lane; i < s1; i += 64) a.next[i] = i < end ? a.tok[min(i + 1, a.T - 1)] : i == end ? (uint16_t)a.verdict[i] : (uint16_t)0;
-    if (lane == 0) a.accepted[b] = s1 > s0 ? end - s0 : 0;
+    const double want = r * total;
+    const int e = pick_lane(mine > kNothing && upto > want, mine > kNothing, &first, &last);
+    if ((int)threadIdx.x == e) waves[0] = upto - mine;
+    __syncthreads();
+    const double before = waves[0];
+    // the token in it, two to a lane
+    const Left lf(a, h);
+    const VocabRow t(lf.t, a.V);
+    const int size = 8 * (residual ? kHalf : kPieces), j0 = t.first(e * size / 8), j = j0 + 2 * (int)threadIdx.x;
+    double w[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int at = min(max(j + k, 0), a.V - 1);
+        w[k] = lf(t.row[at], lf.d ? lf.d[at] : (half_t)0.f, 2 * (int)threadIdx.x < size ? j + k : -1, residual);
+    }
+    mine = w[0] + w[1];
+    upto = block_scan(mine, &total) + before;
+    const int lane_of = pick_lane(mine > 0. && upto > want, mine > 0., &first, &last);
+    if ((int)threadIdx.x == lane_of) first = j + !(w[0] > 0. && (upto - w[1] > want || !(w[1] > 0.)));
+    __syncthreads();
+    const int token = first;
+    write_out<kDraw>(a, b, s0, s1, h.row, min(max(token, 0), a.V - 1));
 }
+
+__global__ void __launch_bounds__(kThreads) verify_greedy_kernel(VerifyArgs a)
+{
+    __shared__ int stops[kWaves];
+    __shared__ int found[kWaves];
+    const int b = blockIdx.x, lane = threadIdx.x & 63;
+    int s0, s1;
+    if (!rows_of(a, b, &s0, &s1)) {
+        if (threadIdx.x == 0) {
+            a.accepted[b] = 0;
+            if (s1 != s0 && a.status) atomicMax(a.status, 1);
+        }
+        return;
+    }
+    const int row = first_end(s0, s1, stops, [&](int i, int w) {
+        const bool last = i + 1 >= s1;
+        const int x = last ? 0 : a.tok[i + 1];
+        const float u = a.u[i];
+        const Entry none = {65536., -INFINITY}, e = lane < a.E ? a.entries[(int64_t)i * a.E + lane] : none;
+        const double m = wave_max((float)e.m);
+        const int at = (int)-wave_max(e.m == m ? -(float)e.z : -65536.f);
+        if (lane == 0) found[w] = at;
+        if (x >= a.V && lane == 0 && a.status) atomicMax(a.status, i + 2);
+        return last || x != at || !(u < 1.f);
+    });
+    write_out<kThreads>(a, b, s0, s1, row, found[(row - s0) & (kWaves - 1)]);
+}
+
+int64_t entries_of(int64_t V, int size) { return ((V + 14) / 8 + size - 1) / size; }        // wherever a row begins
 
 }  // namespace
 
-CACTI_API size_t cacti_hip_verify_draft_workspace(int64_t T, int64_t V)
+CACTI_API size_t cacti_hip_verify_draft_workspace(int64_t T, int64_t B, int64_t V)
 {
-    return T > 0 && V > 0 ? (size_t)T * 4 : 0;
+    if (T <= 0 || B <= 0 || V <= 0) return 0;
+    return (size_t)(2 * T * entries_of(V, kPieces)) * sizeof(Entry) + (size_t)B * (sizeof(Head) + (size_t)entries_of(V, kHalf) * 8);
 }
 
 CACTI_API int cacti_hip_verify_draft_f16(int64_t T, int64_t B, int64_t V, const void *target, int64_t ldt, const void *draft, int64_t ldd,
@@ -223,21 +441,36 @@ CACTI_API int cacti_hip_verify_draft_f16(int64_t T, int64_t B, int64_t V, const 
 {
     CACTI_REQUIRE(T > 0 && B > 0 && V > 0, CACTI_E_INVALID, "verify_draft: empty shape");
     CACTI_REQUIRE(target && tok && starts && u && r && accepted && next && workspace, CACTI_E_INVALID, "verify_draft: null pointer");
-    CACTI_REQUIRE(V <= 65536 && T < (1 << 22) && B <= (1 << 22), CACTI_E_NOTIMPL, "verify_draft: at most 65536 tokens and 2^22 rows");
+    CACTI_REQUIRE(V <= 65536 && T < (1 << 18) && B <= 65535, CACTI_E_NOTIMPL, "verify_draft: at most 65536 tokens, 2^18 rows, 65535 sequences");
     CACTI_REQUIRE(ldt >= V && (!draft || ldd >= V), CACTI_E_INVALID, "verify_draft: row pitch below a row");
-    CACTI_REQUIRE(temperature >= 0. && temperature <= 1e30 && (temperature == 0. || temperature >= 1e-30), CACTI_E_INVALID,
-                  "verify_draft: the temperature is 0 or positive");
+    CACTI_REQUIRE(temperature >= 0. && temperature <= 1e6 && (temperature == 0. || temperature >= 1e-3), CACTI_E_INVALID,
+                  "verify_draft: the temperature is 0 or from 1e-3 to 1e6");
     CACTI_REQUIRE(aligned(target, 2) && aligned(draft, 2) && aligned(tok, 2) && aligned(next, 2) && aligned(starts, 4) && aligned(u, 4) &&
-                      aligned(r, 4) && aligned(accepted, 4) && aligned(workspace, 4) && aligned(status, 4),
+                      aligned(r, 4) && aligned(accepted, 4) && aligned(workspace, 16) && aligned(status, 4),
                   CACTI_E_INVALID, "verify_draft: misaligned operand");
-    CACTI_REQUIRE(workspace_bytes >= cacti_hip_verify_draft_workspace(T, V), CACTI_E_INVALID, "verify_draft: workspace too small");
-    const VerifyArgs a = {(int)T, (int)B, (int)V, (const half_t *)target, (const half_t *)draft, ldt, ldd, (const uint16_t *)tok,
-                          (const int *)starts, (const float *)u, (const float *)r, temperature == 0. ? 0. : 1. / temperature,
-                          (int *)workspace, (int *)accepted, (uint16_t *)next, (int *)status};
+    CACTI_REQUIRE(workspace_bytes >= cacti_hip_verify_draft_workspace(T, B, V), CACTI_E_INVALID, "verify_draft: workspace too small");
+    const bool greedy = temperature == 0.;
+    const double t = greedy ? 1. : temperature;
+    const int64_t E = entries_of(V, kPieces), E2 = entries_of(V, kHalf);
+    Entry *entries = (Entry *)workspace;
+    Head *heads = (Head *)(entries + 2 * T * E);
+    const VerifyArgs a = {(int)T, (int)B, (int)V, (int)E, (int)E2, (const half_t *)target, greedy ? nullptr : (const half_t *)draft, ldt, ldd,
+                          (const uint16_t *)tok, (const int *)starts, (const float *)u, (const float *)r,
+                          Scale{1.4426950408889634 / t, (float)(1000. / 1.4426950408889634 * t)}, entries, (double *)(heads + B), heads, (int *)accepted,
+                          (uint16_t *)next, (int *)status};
     hipStream_t st = (hipStream_t)stream;
-    hipLaunchKernelGGL(verify_rows_kernel, dim3((unsigned)T), dim3(kThreads), 0, st, a);
-    const int rc = launch_status("verify_draft");
+    const dim3 grid((unsigned)T, (unsigned)((E + kEntryWaves - 1) / kEntryWaves), a.draft ? 2 : 1), block(64 * kEntryWaves);
+    if (greedy) hipLaunchKernelGGL(verify_entries_kernel<true>, grid, block, 0, st, a);
+    else hipLaunchKernelGGL(verify_entries_kernel<false>, grid, block, 0, st, a);
+    int rc = launch_status("verify_draft");
     if (rc) return rc;
-    hipLaunchKernelGGL(verify_pick_kernel, dim3((unsigned)B), dim3(64), 0, st, a);
-    return launch_status("verify_draft (pick)");
+    if (greedy) {
+        hipLaunchKernelGGL(verify_greedy_kernel, dim3((unsigned)B), dim3(kThreads), 0, st, a);
+        return launch_status("verify_draft (greedy)");
+    }
+    hipLaunchKernelGGL(verify_rows_kernel, dim3((unsigned)((E2 + kWaves - 1) / kWaves), (unsigned)B), dim3(kThreads), 0, st, a);
+    rc = launch_status("verify_draft (rows)");
+    if (rc) return rc;
+    hipLaunchKernelGGL(verify_draw_kernel, dim3((unsigned)B), dim3(kDraw), 0, st, a);
+    return launch_status("verify_draft (draw)");
 }

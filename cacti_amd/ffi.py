@@ -120,7 +120,7 @@ SIGNATURES = {
     "cacti_hip_paged_attention_workspace": (sz, [i64] * 8),
     "cacti_hip_paged_attention_f16": (ci, [i64] * 6 + [f32, vp, i64, vp, vp, vp, vp, ci, i64, i64, vp, i64, i64, vp, vp, vp, i64, vp, sz,
                                                        vp, vp]),
-    "cacti_hip_verify_draft_workspace": (sz, [i64, i64]),
+    "cacti_hip_verify_draft_workspace": (sz, [i64, i64, i64]),
     "cacti_hip_verify_draft_f16": (ci, [i64, i64, i64, vp, i64, vp, i64, vp, vp, vp, vp, C.c_double, vp, vp, vp, sz, vp, vp]),
     "cacti_hip_distill_topk_fwd": (ci, [i64, i64, i64, vp, i64, vp, vp, C.c_double, vp, vp, vp, vp]),
     "cacti_hip_distill_topk_bwd": (ci, [i64, i64, i64, vp, i64, vp, vp, vp, vp, C.c_double, vp, i64, ci, vp]),

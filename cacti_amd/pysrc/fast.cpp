@@ -610,7 +610,7 @@ PyObject *verify_draft(PyObject *const *o)
     void *status = on.pointer(o[7], at::kInt, 1), *st = on.stream();
     const Result accepted = {empty({B}, t.t, at::kInt), nullptr}, next = {empty({t.N}, t.t, at::kShort), nullptr};
     if (t.N > 0 && B > 0) {
-        const size_t bytes = cacti_hip_verify_draft_workspace(t.N, t.V);
+        const size_t bytes = cacti_hip_verify_draft_workspace(t.N, B, t.V);
         const at::Tensor ws = empty({(int64_t)bytes}, t.t, at::kByte);
         run([&] {
             return cacti_hip_verify_draft_f16(t.N, B, t.V, t.t.data_ptr(), t.ld, draft, ldd, tok, starts.data_ptr(), u, r, temperature,

@@ -13,7 +13,7 @@ ARGS = dict(T=4, B=2, V=64, target=64, ldt=64, draft=64, ldd=64, tok=64, starts=
 
 
 @pytest.mark.parametrize("change,why", [(dict(T=0), "empty"), (dict(B=0), "empty"), (dict(V=0), "empty"), (dict(V=65537, ldt=65537, ldd=65537), "65536"),
-                                        (dict(T=1 << 22, ws_bytes=1 << 40), "2^22"), (dict(ldt=63), "pitch"), (dict(ldd=63), "pitch"),
+                                        (dict(T=1 << 18, ws_bytes=1 << 40), "2^18"), (dict(ldt=63), "pitch"), (dict(ldd=63), "pitch"),
                                         (dict(target=None), "null"), (dict(tok=None), "null"), (dict(starts=None), "null"), (dict(u=None), "null"),
                                         (dict(r=None), "null"), (dict(accepted=None), "null"), (dict(next=None), "null"), (dict(ws=None), "null"),
                                         (dict(ws_bytes=4), "workspace"), (dict(temp=-1.0), "temperature"), (dict(temp=float("nan")), "temperature"),
