@@ -25,7 +25,7 @@ using namespace cacti;
 namespace {
 
 constexpr int kRounds = 4, kPieces = 64 * kRounds;         // 16-byte pieces of an entry
-constexpr int kHalf = 128;                     // of an entry of what is left of p
+constexpr int kLeft = 64;                      // of an entry of what is left of p
 constexpr int kEntryWaves = 4;                 // entries of a workgroup of the first kernel
 constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kDraw = 1024;                    // lanes of the last kernel: two logits each
@@ -41,11 +41,6 @@ struct Head {
     double it, id;                             // 1 / sums
 };
 
-struct Scale {
-    double c;                                  // log2 e / temperature
-    float span;                                // 1000 / c
-};
-
 struct VerifyArgs {
     int T, B, V, E, E2;                        // E, E2: entries of a row, of what is left of p
     const half_t *target, *draft;
@@ -53,7 +48,7 @@ struct VerifyArgs {
     const uint16_t *tok;
     const int *starts;
     const float *u, *r;
-    Scale c;
+    double c;                                  // log2 e / temperature
     Entry *entries;                            // [2][T][E]: target, draft
     double *left;                              // [B][E2]: sums of what is left of p
     Head *heads;
@@ -62,7 +57,7 @@ struct VerifyArgs {
     int *status;
 };
 
-// 2^t for -1022 <= t <= 0: t = n + f, |f| <= 1/2, a polynomial of degree 9 in f (Chebyshev interpolation on that interval,
+// 2^t for -2^31 < t <= 0: t = n + f, |f| <= 1/2, a polynomial of degree 9 in f (Chebyshev interpolation on that interval,
 // 2e-14) and n added to its exponent
 __device__ __forceinline__ double exp2_neg(double t)
 {
@@ -79,23 +74,17 @@ __device__ __forceinline__ double exp2_neg(double t)
     p = __builtin_fma(p, f, 1.0000000000000135);
     return __builtin_amdgcn_ldexp(p, (int)__builtin_bit_cast(uint64_t, s));
 }
-constexpr double kNothing = 1e-290;            // weights below that are those of -inf
+constexpr double kNothing = 1e-290;            // weights below that are nothing
 
 // A NaN is never chosen
 __device__ __forceinline__ float clean(half_t x) { return fmaxf(h2f(x), -INFINITY); }
-// What makes weights of logits relative to a maximum: 2^(x c - mx c).  What is 1000 below it, and so -inf and a NaN, is held
-// there (in fp32, where the temperature's lower bound leaves 16 to spare).  A maximum that is no infinity.
-struct Weight {
-    double c, b;
-    float low;
-    __device__ __forceinline__ Weight(float mx, const Scale &s) : c(s.c), b(-(double)mx * s.c), low(mx - s.span) {}
-    __device__ __forceinline__ double operator()(float x) const { return exp2_neg(__builtin_fma((double)fmaxf(x, low), c, b)); }
-};
-// ... any: of infinities 1 for those that are it, 0 for the others
-__device__ __forceinline__ double weight(float x, float mx, const Scale &s)
+// 2^((x - mx) c), 0 of -inf; of a maximum that is an infinity 1 for those that are it, 0 for the others
+__device__ __forceinline__ double weight(float x, float mx, double c)
 {
     const bool fine = fabsf(mx) < INFINITY;
-    return Weight(fine ? mx : 0.f, s)(fine ? x : x == mx ? 0.f : -INFINITY);
+    const float y = fine ? x : x == mx ? 0.f : -INFINITY;
+    const double w = exp2_neg(__builtin_fma(y > -INFINITY ? (double)y : 0., c, fine ? -(double)mx * c : 0.));
+    return y > -INFINITY ? w : 0.;
 }
 
 // inclusive sum over the lanes
@@ -137,12 +126,11 @@ __global__ void __launch_bounds__(64 * kEntryWaves) verify_entries_kernel(Verify
         for (int i = 1 + lane; i <= a.B; i += 64) last = last || a.starts[i] == row + 1;
         if (__ballot(last)) return;
     }
-    float mx = -INFINITY;
+    half2_t h[kRounds * 4], m2 = {(half_t)-INFINITY, (half_t)-INFINITY};      // two at a time; a NaN is no maximum
+    __builtin_memcpy(h, v, sizeof(v));
 #pragma unroll
-    for (int r = 0; r < kRounds; r++)
-#pragma unroll
-        for (int k = 0; k < 8; k++) mx = fmaxf(mx, h2f(v[r].v[k]));
-    mx = wave_max(mx);
+    for (int i = 0; i < kRounds * 4; i++) m2 = __builtin_elementwise_max(m2, h[i]);
+    const float mx = wave_max(fmaxf(h2f(m2[0]), h2f(m2[1])));
     double z = 0.;
     if (GREEDY) {
         int at = 65536;
@@ -155,20 +143,24 @@ __global__ void __launch_bounds__(64 * kEntryWaves) verify_entries_kernel(Verify
             }
         z = -(double)wave_max(-(float)at);
     } else {
-        if (fabsf(mx) < INFINITY) {
-            const Weight w(mx, a.c);
+        const half_t lowest = (half_t)-65504.f;
+        if (fabsf(mx) < INFINITY && (-65504. - (double)mx) * a.c < -1000.) {
+            // -inf and a NaN count as the lowest number, which has no weight here
+            const double b = -(double)mx * a.c;
 #pragma unroll
-            for (int r = 0; r < kRounds; r++)
-#pragma unroll
-                for (int k = 0; k < 8; k++) z += w(h2f(v[r].v[k]));
+            for (int i = 0; i < kRounds * 4; i++) {
+                const half2_t x = __builtin_elementwise_max(h[i], half2_t{lowest, lowest});
+                z += exp2_neg(__builtin_fma((double)h2f(x[0]), a.c, b));
+                z += exp2_neg(__builtin_fma((double)h2f(x[1]), a.c, b));
+            }
         } else {
-#pragma unroll
-            for (int r = 0; r < kRounds; r++)
-#pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const int j = t.first(e * kPieces + r * 64 + lane) + k;
-                    z += j >= 0 && j < a.V && clean(v[r].v[k]) == mx ? 1. : 0.;
-                }
+#pragma unroll 1
+            for (int r = 0; r < kRounds; r++) {
+                const int c = e * kPieces + r * 64 + lane;
+#pragma unroll 1
+                for (int j = t.first(c); c < t.pieces() && j < t.first(c) + 8; j++)
+                    if (j >= 0 && j < a.V) z += weight(clean(t.row[j]), mx, a.c);
+            }
         }
         z = wave_sum_f64(z);
     }
@@ -228,8 +220,7 @@ __device__ __forceinline__ void write_out(const VerifyArgs &a, int b, int s0, in
 struct Left {
     const half_t *t, *d;                       // d null: none
     float mt, md;
-    double it, id;
-    Scale c;
+    double it, id, c;
     int x, V;
     __device__ __forceinline__ Left(const VerifyArgs &a, const Head &h)
         : t(a.target + h.row * a.ldt), d(a.draft && h.residual ? a.draft + h.row * a.ldd : nullptr), mt(h.mt), md(h.md), it(h.it), id(h.id),
@@ -316,22 +307,19 @@ __global__ void __launch_bounds__(kThreads) verify_rows_kernel(VerifyArgs a)
     const Left lf(a, h);
     const VocabRow t(lf.t, a.V);
     const bool alike = lf.d && ((reinterpret_cast<uintptr_t>(lf.d) ^ reinterpret_cast<uintptr_t>(lf.t)) & 15) == 0;
-    double sum = 0.;
-    h8 v[2] = {}, u[2] = {};
-#pragma unroll
-    for (int r = 0; r < 2; r++) {
-        const int p = e * kHalf + r * 64 + lane, j0 = t.first(p);
-        if (p >= t.pieces()) continue;
-        v[r] = t.load(p, (half_t)0.f);
-        if (alike && t.whole(p)) u[r] = ld8(lf.d + j0);
+    const int p = e * kLeft + lane, j0 = t.first(p);
+    h8 v = {}, u = {};
+    if (p < t.pieces()) {
+        v = t.load(p, (half_t)0.f);
+        if (alike && t.whole(p)) u = ld8(lf.d + j0);
         else if (lf.d)
 #pragma unroll
-            for (int k = 0; k < 8; k++) u[r].v[k] = lf.d[min(max(j0 + k, 0), a.V - 1)];
+            for (int k = 0; k < 8; k++) u.v[k] = lf.d[min(max(j0 + k, 0), a.V - 1)];
     }
-    Eight v0(v[0]), v1(v[1]), u0(u[0]), u1(u[1]);
-    const int j0 = t.first(e * kHalf + lane);
-#pragma unroll 1
-    for (int k = 0; k < 8; k++) sum += lf(v0.take(), u0.take(), j0 + k, true) + lf(v1.take(), u1.take(), j0 + 512 + k, true);
+    Eight v8(v), u8(u);
+    double sum = 0.;
+#pragma unroll 2
+    for (int k = 0; k < 8; k++) sum += lf(v8.take(), u8.take(), j0 + k, true);
     sum = wave_sum_f64(sum);
     if (lane == 0) a.left[(int64_t)b * a.E2 + e] = sum;
 }
@@ -382,7 +370,7 @@ __global__ void __launch_bounds__(kDraw) verify_draw_kernel(VerifyArgs a)
     // the token in it, two to a lane
     const Left lf(a, h);
     const VocabRow t(lf.t, a.V);
-    const int size = 8 * (residual ? kHalf : kPieces), j0 = t.first(e * size / 8), j = j0 + 2 * (int)threadIdx.x;
+    const int size = 8 * (residual ? kLeft : kPieces), j0 = t.first(e * size / 8), j = j0 + 2 * (int)threadIdx.x;
     double w[2];
 #pragma unroll
     for (int k = 0; k < 2; k++) {
@@ -432,7 +420,7 @@ int64_t entries_of(int64_t V, int size) { return ((V + 14) / 8 + size - 1) / siz
 CACTI_API size_t cacti_hip_verify_draft_workspace(int64_t T, int64_t B, int64_t V)
 {
     if (T <= 0 || B <= 0 || V <= 0) return 0;
-    return (size_t)(2 * T * entries_of(V, kPieces)) * sizeof(Entry) + (size_t)B * (sizeof(Head) + (size_t)entries_of(V, kHalf) * 8);
+    return (size_t)(2 * T * entries_of(V, kPieces)) * sizeof(Entry) + (size_t)B * (sizeof(Head) + (size_t)entries_of(V, kLeft) * 8);
 }
 
 CACTI_API int cacti_hip_verify_draft_f16(int64_t T, int64_t B, int64_t V, const void *target, int64_t ldt, const void *draft, int64_t ldd,
@@ -450,13 +438,12 @@ CACTI_API int cacti_hip_verify_draft_f16(int64_t T, int64_t B, int64_t V, const 
                   CACTI_E_INVALID, "verify_draft: misaligned operand");
     CACTI_REQUIRE(workspace_bytes >= cacti_hip_verify_draft_workspace(T, B, V), CACTI_E_INVALID, "verify_draft: workspace too small");
     const bool greedy = temperature == 0.;
-    const double t = greedy ? 1. : temperature;
-    const int64_t E = entries_of(V, kPieces), E2 = entries_of(V, kHalf);
+    const int64_t E = entries_of(V, kPieces), E2 = entries_of(V, kLeft);
     Entry *entries = (Entry *)workspace;
     Head *heads = (Head *)(entries + 2 * T * E);
     const VerifyArgs a = {(int)T, (int)B, (int)V, (int)E, (int)E2, (const half_t *)target, greedy ? nullptr : (const half_t *)draft, ldt, ldd,
                           (const uint16_t *)tok, (const int *)starts, (const float *)u, (const float *)r,
-                          Scale{1.4426950408889634 / t, (float)(1000. / 1.4426950408889634 * t)}, entries, (double *)(heads + B), heads, (int *)accepted,
+                          greedy ? 0. : 1.4426950408889634 / temperature, entries, (double *)(heads + B), heads, (int *)accepted,
                           (uint16_t *)next, (int *)status};
     hipStream_t st = (hipStream_t)stream;
     const dim3 grid((unsigned)T, (unsigned)((E + kEntryWaves - 1) / kEntryWaves), a.draft ? 2 : 1), block(64 * kEntryWaves);
