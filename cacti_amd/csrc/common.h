@@ -154,6 +154,23 @@ __device__ __forceinline__ double wave_sum_f64(double v)
     return words_f64(lo[0], hi[0]) + words_f64(lo[1], hi[1]);
 }
 
+// the value of a lane; the inclusive sum over the lanes
+__device__ __forceinline__ double lane_f64(double v, int lane)
+{
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return words_f64(__builtin_amdgcn_readlane((int)u, lane), __builtin_amdgcn_readlane((int)(u >> 32), lane));
+}
+__device__ __forceinline__ double scan_f64(double v)
+{
+    v += dpp_f64<0x111>(v);                    // row_shr 1, 2, 4, 8: nothing from before the 16
+    v += dpp_f64<0x112>(v);
+    v += dpp_f64<0x114>(v);
+    v += dpp_f64<0x118>(v);
+    const double r0 = lane_f64(v, 15), r1 = lane_f64(v, 31), r2 = lane_f64(v, 47);
+    const int row = (threadIdx.x & 63) >> 4;
+    return v + (row == 0 ? 0. : row == 1 ? r0 : row == 2 ? r0 + r1 : r0 + r1 + r2);
+}
+
 // Block reduction through LDS: `red` holds one float per wave (<= 16 waves).
 template <class Op>
 __device__ __forceinline__ float block_reduce(float v, Op op, float ident, float *red)

@@ -8,27 +8,31 @@
 // Scores, maxima, sums and o are fp32; w is rounded to f16 for the matrix instruction (2^-11 relative, each on its own, which
 // is what the rounding of the output adds once more).
 //
-// A workgroup has 16 NR rows (tokens of a sequence by the query heads that share a key head), a key head and a part of the
-// positions; its four waves take 32 positions in turn and put their sums together at the end.  The products are formed
-// transposed, S^T = K Q^T and O^T = V^T W^T with v_mfma_f32_16x16x32_f16: a lane then holds the scores of one row, at keys
-// that are exactly those its part of the second product's operand wants, so that w never leaves the lane.  Keys come from
-// memory in the order the instruction takes them (16 columns of a key to a lane); V, whose operand is a column of eight
-// keys, is read as rows of 8 columns and turned with byte permutes.  No LDS, no barrier inside.
+// A workgroup takes 16 NR rows (tokens of a sequence by the query heads that share a key head) of a key head at a time; its
+// four waves take 32 positions in turn and put their sums together at the end.  The products are formed transposed, S^T = K Q^T
+// and O^T = V^T W^T with v_mfma_f32_16x16x32_f16: a lane then holds the scores of one row, at keys that are exactly those its
+// part of the second product's operand wants, so that w never leaves the lane.  Keys come from memory in the order the
+// instruction takes them (16 columns of a key to a lane); V, whose operand is a column of eight keys, is read as rows of 8
+// columns and turned with byte permutes.  No LDS, no barrier in between; the keys after these are requested once these have
+// been multiplied, the values likewise, into the same registers.
+//
+// Work: the lengths are on the device and as different as they come, so every workgroup of a launch that just fills the device
+// forms their sum in blocks of 128 positions and takes an equal, contiguous share of it, across rows, heads and sequences.  A
+// tile of rows that ends up in more than one share leaves partial sums, which a second launch puts together.
 #include "paged.h"
 
 using namespace cacti;
 
 namespace {
 
-constexpr int kThreads = 256, kWaves = 4, kStep = 32;
-constexpr int kEntries = 128;                  // pages of a workgroup's positions at a time
-constexpr int kSegment = 2048;                 // positions of them: 128 pages of 16
+constexpr int kThreads = 256, kWaves = 4, kStep = 32, kBlock = kWaves * kStep;
+constexpr int kSegment = 8192;                 // positions whose pages a workgroup looks up at a time
+constexpr int kEntries = kSegment / 16 + 1;
 
 struct AttnArgs {
     PagedBatch pb;
-    Units units;
-    int H, Hkv, G, Dh, Dp, max_new;
-    int chunk, splits;                         // positions of a workgroup, workgroups behind one another along a sequence
+    int H, Hkv, G, Dh, Dp, max_new, groups;
+    unsigned page_magic;                       // x / page = x * page_magic >> 22 for x up to kSegment + 256
     float alpha;
     const half_t *q;
     int64_t ldq;
@@ -36,8 +40,62 @@ struct AttnArgs {
     const float *k_scale, *v_scale;
     half_t *out;
     int64_t ldo;
-    float *part, *stats;                       // [split][T][H][Dh], [split][T][H][2]
+    float *part, *stats;                       // [2 groups][16 NR][Dh], [2 groups][16 NR][2]
 };
+
+// What is the same in all lanes, in scalar registers
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x)
+{
+    return (int64_t)((uint64_t)(unsigned)uniform((int)(x >> 32)) << 32 | (unsigned)uniform((int)x));
+}
+
+// A sequence's share of the work: its tiles of 16 NR rows by its blocks of positions, by heads
+struct Share {
+    int tiles, blocks;
+    double units;
+    __device__ __forceinline__ Share(const AttnArgs &a, int tile, const Sequence &s)
+        : tiles((s.n * a.G + tile - 1) / tile), blocks((s.first + s.n + kBlock - 1) / kBlock),
+          units(s.ok && s.n > 0 ? (double)tiles * blocks * a.Hkv : 0.)
+    {
+    }
+};
+// All of it, and what there is before sequence `until` (whole numbers in fp64), by a wave
+__device__ __forceinline__ double sum_of_work(const AttnArgs &a, int tile, int until, double *before)
+{
+    const int lane = threadIdx.x & 63;
+    double all = 0., some = 0.;
+    for (int b0 = 0; b0 < a.pb.B; b0 += 64) {
+        const int b = b0 + lane;
+        const double u = b < a.pb.B ? Share(a, tile, sequence(a.pb, b, (int64_t)a.pb.W * a.pb.page, a.max_new)).units : 0.;
+        all += u;
+        some += b < until ? u : 0.;
+    }
+    *before = wave_sum_f64(some);
+    return wave_sum_f64(all);
+}
+// The sequence in whose work unit x lies, and what there is before it
+__device__ __forceinline__ int sequence_at(const AttnArgs &a, int tile, double x, double *before)
+{
+    const int lane = threadIdx.x & 63;
+    double all = 0.;
+    for (int b0 = 0; b0 < a.pb.B; b0 += 64) {
+        const int b = b0 + lane;
+        const double u = b < a.pb.B ? Share(a, tile, sequence(a.pb, b, (int64_t)a.pb.W * a.pb.page, a.max_new)).units : 0.;
+        const double upto = scan_f64(u) + all;
+        const uint64_t hit = __ballot(upto > x);
+        if (hit) {
+            const int at = __ffsll((unsigned long long)hit) - 1;
+            *before = lane_f64(upto - u, at);
+            return b0 + at;
+        }
+        all = lane_f64(upto, 63);
+    }
+    *before = all;
+    return a.pb.B;
+}
+// Of `groups` workgroups that take part, at least a unit for each, i has the units from begin_of(i) to begin_of(i + 1)
+__device__ __forceinline__ int64_t begin_of(int64_t i, int64_t units, int64_t groups) { return i * units / groups; }
 
 typedef unsigned u4_t __attribute__((ext_vector_type(4)));
 typedef unsigned u2_t __attribute__((ext_vector_type(2)));
@@ -101,13 +159,14 @@ struct VBlock<uint8_t, VD> {
 #pragma unroll
         for (int j = 0; j < VD / 4; j++) w[i][j] = 0;
     }
-    __device__ __forceinline__ bool odd(int i) const       // a NaN among them
+    __device__ __forceinline__ bool strip(int i)           // of its NaNs, whether there were any
     {
         bool any = false;
 #pragma unroll
         for (int j = 0; j < VD / 4; j++) {
-            const unsigned x = w[i][j] & 0x7f7f7f7fu;
-            any = any || ((x + 0x01010101u) & 0x80808080u);
+            const unsigned bad = ((w[i][j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+            any = any || bad;
+            w[i][j] &= ~((bad >> 7) * 0xffu);
         }
         return any;
     }
@@ -145,11 +204,15 @@ struct VBlock<half_t, VD> {
 #pragma unroll
         for (int j = 0; j < VD / 2; j++) w[i][j] = 0;
     }
-    __device__ __forceinline__ bool odd(int i) const       // a NaN or an infinity among them
+    __device__ __forceinline__ bool strip(int i)           // of its NaNs and infinities, whether there were any
     {
         bool any = false;
 #pragma unroll
-        for (int j = 0; j < VD / 2; j++) any = any || (w[i][j] & 0x7c00u) == 0x7c00u || (w[i][j] & 0x7c000000u) == 0x7c000000u;
+        for (int j = 0; j < VD / 2; j++) {
+            const unsigned low = (w[i][j] & 0x7c00u) == 0x7c00u ? 0xffffu : 0u, high = (w[i][j] & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u;
+            any = any || (low | high);
+            w[i][j] &= ~(low | high);
+        }
         return any;
     }
     __device__ __forceinline__ void columns(int c, half8_t *a, half8_t *b) const
@@ -176,342 +239,378 @@ struct Entry {
     float c, lg, iv;                           // alpha ks log2 e, log2 vs, 1 / vs
 };
 
-// ND: pieces of 64 columns of a head
+// One tile of rows and a part of its positions.  ND: pieces of 64 columns of a head
 template <int ND, int NR, class P>
-__global__ void __launch_bounds__(kThreads) paged_attention_kernel(AttnArgs a)
-{
-    constexpr int VD = 4 * ND;                 // columns of V of a lane
-    constexpr int NS = 2 * ND;                 // matrix instructions along the columns of a key
-    __shared__ Entry entry[kEntries];
-    __shared__ float merged[kWaves][16 * NR][VD * 16 + 4];
-    __shared__ float wave_m[kWaves][16 * NR], wave_l[kWaves][16 * NR];
-    const PagedBatch &pb = a.pb;
-    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, r16 = lane & 15, g = lane >> 4;
-    const int64_t x = blockIdx.x / a.splits;
-    const int split = (int)(blockIdx.x - x * a.splits), h = blockIdx.y;
-    int tile;
-    const int b = a.units.find(pb, x, &tile);
-    if (b >= pb.B) return;
-    const Sequence s = sequence(pb, b, (int64_t)pb.W * pb.page, a.max_new);
-    const int rows = s.n * a.G, row0 = tile * 16 * NR;
-    if (s.s0 < 0 || s.n < 0 || s.s0 > pb.T - s.n || row0 < 0 || row0 >= rows) return;
-    if (!s.ok) {                               // rows that there are at positions that there are not: zeros
-        if (threadIdx.x == 0) report(pb, b);
-        if (split == 0)
-            for (int i = threadIdx.x; i < 16 * NR * a.Dh; i += kThreads) {
-                const int r = row0 + i / a.Dh, d = i % a.Dh;
-                if (r < rows) a.out[(int64_t)(s.s0 + r / a.G) * a.ldo + (h * a.G + r % a.G) * a.Dh + d] = (half_t)0.f;
-            }
-        return;
-    }
-    const int end = s.first + min(rows - 1, row0 + 16 * NR - 1) / a.G + 1;         // positions that some row of the tile sees
-    const int c0 = split * a.chunk, c1 = min(end, c0 + a.chunk);
-    if (c0 >= c1) return;
-
-    // the lane's row of each 16: its query, its last position
+struct Tile {
+    static constexpr int VD = 4 * ND;          // columns of V of a lane
+    static constexpr int NS = 2 * ND;          // matrix instructions along the columns of a key
+    struct Shared {
+        Entry entry[kEntries];
+        float merged[kWaves][16 * NR][VD * 16 + 4];
+        float m[kWaves][16 * NR], l[kWaves][16 * NR];
+        int odd;                               // there was a NaN or an infinity of V that some rows see
+    };
+    const AttnArgs &a;
+    Shared &sh;
     half8_t q[NR][NS];
-    int last[NR];
+    int last[NR];                              // the lane's row of each 16: its last position
     float m[NR], l[NR];
     float4_t o[NR][VD];
-    int least = INT32_MAX;                     // positions up to here are seen by every row
-#pragma unroll
-    for (int n = 0; n < NR; n++) {
-        const int r = min(row0 + 16 * n + r16, rows - 1), t = r / a.G;
-        last[n] = s.first + t;
-        const half_t *qr = a.q + (int64_t)(s.s0 + t) * a.ldq + (h * a.G + r - t * a.G) * a.Dh;
-#pragma unroll
-        for (int c = 0; c < ND; c++)
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                Frag f;
-#pragma unroll
-                for (int j = 0; j < 2; j++) {  // pieces of four columns: Dh is a multiple of 4
-                    const int d = 64 * c + 16 * g + 8 * k + 4 * j;
-                    const u2_t w = *reinterpret_cast<const u2_t *>(qr + min(d, a.Dh - 4));
-                    f.u[2 * j] = d < a.Dh ? w[0] : 0u;
-                    f.u[2 * j + 1] = d < a.Dh ? w[1] : 0u;
-                }
-                q[n][2 * c + k] = f.h;
-            }
-        m[n] = -INFINITY;
-        l[n] = 0.f;
-#pragma unroll
-        for (int i = 0; i < VD; i++) o[n][i] = float4_t{0.f, 0.f, 0.f, 0.f};
-    }
-    least = s.first + row0 / a.G;
+    KPiece<P> kk[2][ND];
+    VBlock<P, VD> vv;
 
-    const P *kp = (const P *)a.k_pages, *vp = (const P *)a.v_pages;
-    const float log2e = 1.44269504088896340736f;
-    for (int seg = c0; seg < c1; seg += kSegment) {
-        const int seg1 = min(c1, seg + kSegment), p0 = seg / pb.page, np = (seg1 - 1) / pb.page - p0 + 1;
-        if (seg > c0) __syncthreads();
-        for (int i = threadIdx.x; i < np; i += kThreads) {
-            int id = pb.table[(int64_t)b * pb.ldt + p0 + i];
-            if (id < 0 || id >= pb.P) {
-                report(pb, b);
-                id = 0;                        // its rows are unspecified, not its reads
+    // keys and values of the 32 positions from x on, counted from the first entry's page; behind `end` the last one again
+    __device__ __forceinline__ void load_k(int x, int end)
+    {
+        const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const int j = min(x + 8 * (r16 >> 2) + 4 * t + (r16 & 3), end - 1), pg = page_of(j);
+            const P *row = (const P *)a.k_pages + sh.entry[pg].at + (j - pg * a.pb.page) * a.Dp;
+#pragma unroll
+            for (int c = 0; c < ND; c++) {
+                kk[t][c].load(row + min(64 * c + 16 * g, a.Dp - 16));
+                // (there the query is zero, and an infinity of another column would make a NaN with it)
+                if constexpr (sizeof(P) == 2)
+                    if (64 * c + 16 * g >= a.Dp) kk[t][c].zero();
             }
-            const int64_t ph = (int64_t)id * a.Hkv + h;
-            Entry e = {ph * pb.page * a.Dp, a.alpha * log2e, 0.f, 1.f};
-            if (sizeof(P) == 1) {
-                e.c *= a.k_scale[ph];
-                e.lg = log2f(a.v_scale[ph]);
-                e.iv = 1.f / a.v_scale[ph];
-            }
-            entry[i] = e;
         }
-        __syncthreads();
-        for (int j0 = seg + kStep * wid; j0 < seg1; j0 += kStep * kWaves) {
-            KPiece<P> kk[2][ND];
-            VBlock<P, VD> vv;
+    }
+    __device__ __forceinline__ void load_v(int x, int end)
+    {
+        const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
+        const int j0 = x + 8 * g, pg = page_of(min(j0, end - 1));          // one page: of 16 positions or a multiple
+        const P *row = (const P *)a.v_pages + sh.entry[pg].at + min(VD * r16, a.Dp - VD);
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const int j = min(j0 + 8 * (r16 >> 2) + 4 * t + (r16 & 3), seg1 - 1), pg = j / pb.page;
-                const P *row = kp + entry[pg - p0].at + (j - pg * pb.page) * a.Dp;
+        for (int i = 0; i < 8; i++) vv.load(i, row + (min(j0 + i, end - 1) - pg * a.pb.page) * a.Dp);
+    }
+    __device__ __forceinline__ int page_of(int x) const { return (int)((unsigned)x * a.page_magic >> 22); }
+
+    // positions c0 .. c1 - 1 of rows row0 .. of sequence s; `least`: positions up to there are seen by every row
+    __device__ __forceinline__ void run(int b, const Sequence &s, int h, int rows, int row0, int c0, int c1)
+    {
+        const int lane = threadIdx.x & 63, wid = uniform((int)threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
 #pragma unroll
-                for (int c = 0; c < ND; c++) {
-                    kk[t][c].load(row + min(64 * c + 16 * g, a.Dp - 16));
-                    // (there the query is zero, and an infinity of another column would make a NaN with it)
-                    if constexpr (sizeof(P) == 2)
-                        if (64 * c + 16 * g >= a.Dp) kk[t][c].zero();
+        for (int n = 0; n < NR; n++) {
+            const int r = min(row0 + 16 * n + r16, rows - 1), t = r / a.G;
+            last[n] = s.first + t;
+            const half_t *qr = a.q + (int64_t)(s.s0 + t) * a.ldq + (h * a.G + r - t * a.G) * a.Dh;
+#pragma unroll
+            for (int c = 0; c < ND; c++)
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    Frag f;
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {  // pieces of four columns: Dh is a multiple of 4
+                        const int d = 64 * c + 16 * g + 8 * k + 4 * j;
+                        const u2_t w = *reinterpret_cast<const u2_t *>(qr + min(d, a.Dh - 4));
+                        f.u[2 * j] = d < a.Dh ? w[0] : 0u;
+                        f.u[2 * j + 1] = d < a.Dh ? w[1] : 0u;
+                    }
+                    q[n][2 * c + k] = f.h;
                 }
+            m[n] = -INFINITY;
+            l[n] = 0.f;
+#pragma unroll
+            for (int i = 0; i < VD; i++) o[n][i] = float4_t{0.f, 0.f, 0.f, 0.f};
+        }
+        const int least = uniform(s.first + row0 / a.G);
+        for (int seg = c0; seg < c1; seg += kSegment) {
+            const int p0 = uniform(seg / a.pb.page), base = p0 * a.pb.page, end = min(c1, seg + kSegment) - base;
+            const int np = page_of(end - 1) + 1;
+            __syncthreads();                   // (the entries of before are done with)
+            if (seg == c0 && threadIdx.x == 0) sh.odd = 0;
+            for (int i = threadIdx.x; i < np; i += kThreads) {
+                int id = a.pb.table[(int64_t)b * a.pb.ldt + p0 + i];
+                if (id < 0 || id >= a.pb.P) {
+                    report(a.pb, b);
+                    id = 0;                    // its rows are unspecified, not its reads
+                }
+                const int64_t ph = (int64_t)id * a.Hkv + h;
+                Entry e = {ph * a.pb.page * a.Dp, a.alpha * 1.44269504088896340736f, 0.f, 1.f};
+                if (sizeof(P) == 1) {
+                    e.c *= a.k_scale[ph];
+                    e.lg = log2f(a.v_scale[ph]);
+                    e.iv = 1.f / a.v_scale[ph];
+                }
+                sh.entry[i] = e;
             }
-            const int mine = min(j0 + 8 * g, seg1 - 1) / pb.page - p0;       // page of the lane's eight keys
-            const float ec = entry[mine].c, lg = entry[mine].lg, iv = entry[mine].iv;
-            const P *vrow = vp + entry[mine].at + min(VD * r16, a.Dp - VD);
+            __syncthreads();
+            int x = seg - base + kStep * wid;
+            if (x >= end) continue;
+            load_k(x, end);
+            load_v(x, end);
+            for (; x < end; x += kBlock) step(x, end, least - base, base, min(x + kBlock, end - 1));
+        }
+    }
+
+    __device__ __forceinline__ void step(int x, int end, int least, int base, int next)
+    {
+        const int lane = threadIdx.x & 63, g = lane >> 4;
+        float4_t sc[NR][2];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+#pragma unroll
+            for (int n = 0; n < NR; n++) sc[n][t] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < NS; c++) {
+                const half8_t kf = kk[t][c / 2].part(c & 1);
+#pragma unroll
+                for (int n = 0; n < NR; n++) sc[n][t] = mfma(kf, q[n][c], sc[n][t]);
+            }
+        }
+        load_k(next, end);
+        const Entry &en = sh.entry[page_of(min(x + 8 * g, end - 1))];      // of the lane's eight keys
+        const float ec = en.c, lg = en.lg, iv = en.iv;
+        const bool edge = x + kStep - 1 > min(least, end - 1);             // (the same in every lane)
+        half8_t w[NR];
+#pragma unroll
+        for (int n = 0; n < NR; n++) {
+            float t[8], mx = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const int j = min(j0 + 8 * g + i, seg1 - 1);
-                vv.load(i, vrow + (j - (mine + p0) * pb.page) * a.Dp);
+                t[i] = __builtin_fmaf(i < 4 ? sc[n][0][i & 3] : sc[n][1][i & 3], ec, lg);
+                if (edge && x + 8 * g + i > min(last[n] - base, end - 1)) t[i] = -INFINITY;
+                mx = fmaxf(mx, t[i]);
             }
-            float4_t sc[NR][2];
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-#pragma unroll
-                for (int n = 0; n < NR; n++) sc[n][t] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < NS; c++) {
-                    const half8_t kf = kk[t][c / 2].part(c & 1);
-#pragma unroll
-                    for (int n = 0; n < NR; n++) sc[n][t] = mfma(kf, q[n][c], sc[n][t]);
-                }
-            }
-            const bool edge = j0 + kStep - 1 > min(least, seg1 - 1);       // (the same in every lane)
-            half8_t w[NR];
-#pragma unroll
-            for (int n = 0; n < NR; n++) {
-                float t[8], mx = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float raw = i < 4 ? sc[n][0][i & 3] : sc[n][1][i & 3];
-                    t[i] = __builtin_fmaf(raw, ec, lg);
-                    if (edge && j0 + 8 * g + i > min(last[n], seg1 - 1)) t[i] = -INFINITY;
-                    mx = fmaxf(mx, t[i]);
-                }
-                mx = with32(with16(mx, OpMax()), OpMax());
-                const float mn = fmaxf(m[n], mx), base = finite_max(mn);
-                const float f = exp2_of(m[n] - base);
+            mx = with32(with16(mx, OpMax()), OpMax());
+            const float mn = fmaxf(m[n], mx), origin = finite_max(mn);
+            if (__ballot(mn > m[n])) {         // some row's maximum has grown
+                const float f = exp2_of(m[n] - origin);
                 m[n] = mn;
-                float sum = 0.f;
-                Frag p;
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    t[i] = exp2_of(t[i] - base);
-                    sum += t[i];
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const half2_t pair = {f2h(t[2 * i]), f2h(t[2 * i + 1])};
-                    p.u[i] = __builtin_bit_cast(unsigned, pair);
-                }
-                l[n] = l[n] * f + sum * iv;
-                w[n] = p.h;
+                l[n] *= f;
 #pragma unroll
                 for (int i = 0; i < VD; i++) o[n][i] *= f;
             }
-            bool odd = false;
-            if (edge) {
-                // what no row of the tile sees is nothing; a NaN or an infinity that some rows see must not meet the zero
-                // weights of the others
+            float sum = 0.f;
+            Frag p;
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int j = j0 + 8 * g + i;
-                    if (j >= seg1) vv.zero(i);
-                    else odd = odd || (j > least && vv.odd(i));
-                }
-                odd = __ballot(odd) != 0;
+            for (int i = 0; i < 8; i++) {
+                t[i] = exp2_of(t[i] - origin);
+                sum += t[i];
             }
-            if (!odd) {
 #pragma unroll
-                for (int c = 0; c < VD / 2; c++) {
-                    half8_t v0, v1;
-                    vv.columns(c, &v0, &v1);
-#pragma unroll
-                    for (int n = 0; n < NR; n++) {
-                        o[n][2 * c] = mfma(v0, w[n], o[n][2 * c]);
-                        o[n][2 * c + 1] = mfma(v1, w[n], o[n][2 * c + 1]);
-                    }
-                }
-            } else {
-                for (int j = j0; j < min(j0 + kStep, seg1); j++) {          // one key at a time, to the rows that see it
-                    VBlock<P, VD> one = vv;
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        if (j0 + 8 * g + i != j) one.zero(i);
-#pragma unroll
-                    for (int c = 0; c < VD / 2; c++) {
-                        half8_t v0, v1;
-                        one.columns(c, &v0, &v1);
-#pragma unroll
-                        for (int n = 0; n < NR; n++) {
-                            const float4_t z = {0.f, 0.f, 0.f, 0.f};
-                            const float4_t a0 = mfma(v0, w[n], z), a1 = mfma(v1, w[n], z);
-                            if (j <= last[n]) {
-                                o[n][2 * c] += a0;
-                                o[n][2 * c + 1] += a1;
-                            }
-                        }
-                    }
-                }
+            for (int i = 0; i < 4; i++) {
+                const half2_t pair = {f2h(t[2 * i]), f2h(t[2 * i + 1])};
+                p.u[i] = __builtin_bit_cast(unsigned, pair);
             }
+            l[n] = __builtin_fmaf(sum, iv, l[n]);
+            w[n] = p.h;
         }
+        if (edge) {
+            // what no row of the tile sees is nothing; a NaN or an infinity that some rows see must not meet the zero weights of
+            // the others: it is added at the end
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int j = x + 8 * g + i;
+                if (j >= end) vv.zero(i);
+                else if (j > least) odd = vv.strip(i) || odd;
+            }
+            if (odd) sh.odd = 1;
+        }
+#pragma unroll
+        for (int c = 0; c < VD / 2; c++) {
+            half8_t v0, v1;
+            vv.columns(c, &v0, &v1);
+#pragma unroll
+            for (int n = 0; n < NR; n++) {
+                o[n][2 * c] = mfma(v0, w[n], o[n][2 * c]);
+                o[n][2 * c + 1] = mfma(v1, w[n], o[n][2 * c + 1]);
+            }
+            __builtin_amdgcn_sched_barrier(0);             // (all of V turned at once is 64 registers)
+        }
+        load_v(next, end);
     }
 
-    // the four waves' sums: a lane has columns VD (4 g + i) + c of its row in o[.][c][i]
-#pragma unroll
-    for (int n = 0; n < NR; n++) {
-        l[n] = with32(with16(l[n], OpSum()), OpSum());
-        if (g == 0) {
-            wave_m[wid][16 * n + r16] = m[n];
-            wave_l[wid][16 * n + r16] = l[n];
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int c = 0; c < VD; c++) merged[wid][16 * n + r16][VD * (4 * g + i) + c] = o[n][c][i];
-    }
-    __syncthreads();
-    const bool whole = s.first + s.n <= a.chunk;             // the sequence has one part: no partial sums
-    for (int i = threadIdx.x; i < 16 * NR * (a.Dh / 4); i += kThreads) {
-        const int r = i / (a.Dh / 4), d = 4 * (i - r * (a.Dh / 4));
-        if (row0 + r >= rows) break;
-        float mx = wave_m[0][r];
-#pragma unroll
-        for (int w = 1; w < kWaves; w++) mx = fmaxf(mx, wave_m[w][r]);
-        const float base = finite_max(mx);
-        float sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < kWaves; w++) {
-            const float f = exp2_of(wave_m[w][r] - base);
-            sum += f * wave_l[w][r];
-#pragma unroll
-            for (int k = 0; k < 4; k++) acc[k] += f * merged[w][r][d + k];
-        }
-        const int t = (row0 + r) / a.G, head = h * a.G + row0 + r - t * a.G;
-        if (whole) {
-            const float y = sum == 0.f ? 0.f : 1.f / sum;
-            half4_t v;
-#pragma unroll
-            for (int k = 0; k < 4; k++) v[k] = f2h(acc[k] * y);
-            *reinterpret_cast<half4_t *>(a.out + (int64_t)(s.s0 + t) * a.ldo + head * a.Dh + d) = v;
-        } else {
-            const int64_t at = ((int64_t)split * pb.T + s.s0 + t) * a.H + head;
-            *reinterpret_cast<float4_t *>(a.part + at * a.Dh + d) = float4_t{acc[0], acc[1], acc[2], acc[3]};
-            if (d == 0) {
-                a.stats[2 * at] = mx;
-                a.stats[2 * at + 1] = sum;
+    // NaNs and infinities of V at positions j0 .. j1 - 1, columns d .. d + 3
+    __device__ __forceinline__ void add_odd(int b, int h, int j0, int j1, int d, float (&acc)[4]) const
+    {
+        for (int j = j0; j < j1; j++) {
+            const int id = a.pb.table[(int64_t)b * a.pb.ldt + j / a.pb.page];
+            const P *v = (const P *)a.v_pages + (((int64_t)(id < 0 || id >= a.pb.P ? 0 : id) * a.Hkv + h) * a.pb.page + j % a.pb.page) * a.Dp + d;
+            for (int k = 0; k < 4; k++) {
+                const float x = value(v[k]);
+                if (!(fabsf(x) < INFINITY)) acc[k] += x;
             }
         }
+    }
+    static __device__ __forceinline__ float value(half_t x) { return h2f(x); }
+    static __device__ __forceinline__ float value(uint8_t x) { return __builtin_amdgcn_cvt_f32_fp8(x, 0); }
+
+    // The four waves' sums put together: a lane has columns VD (4 g + i) + c of its row in o[.][c][i].  slot < 0: to the output
+    __device__ __forceinline__ void write(int b, const Sequence &s, int h, int rows, int row0, int c0, int c1, int slot)
+    {
+        const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, r16 = lane & 15, g = lane >> 4;
+        __syncthreads();                       // (the sums of before are done with)
+#pragma unroll
+        for (int n = 0; n < NR; n++) {
+            l[n] = with32(with16(l[n], OpSum()), OpSum());
+            if (g == 0) {
+                sh.m[wid][16 * n + r16] = m[n];
+                sh.l[wid][16 * n + r16] = l[n];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int c = 0; c < VD; c++) sh.merged[wid][16 * n + r16][VD * (4 * g + i) + c] = o[n][c][i];
+        }
+        __syncthreads();
+        const int per = a.Dh / 4;
+        const bool odd = c0 < c1 && sh.odd;
+        for (int i = threadIdx.x; i < 16 * NR * per; i += kThreads) {
+            const int r = i / per, d = 4 * (i - r * per);
+            if (row0 + r >= rows) break;
+            float mx = sh.m[0][r];
+#pragma unroll
+            for (int w = 1; w < kWaves; w++) mx = fmaxf(mx, sh.m[w][r]);
+            const float origin = finite_max(mx);
+            float sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) {
+                const float f = exp2_of(sh.m[w][r] - origin);
+                sum += f * sh.l[w][r];
+#pragma unroll
+                for (int k = 0; k < 4; k++) acc[k] += f * sh.merged[w][r][d + k];
+            }
+            if (odd) add_odd(b, h, max(c0, s.first + row0 / a.G + 1), min(c1, s.first + (row0 + r) / a.G + 1), d, acc);
+            if (slot < 0) {
+                const int t = (row0 + r) / a.G, head = h * a.G + row0 + r - t * a.G;
+                const float y = sum == 0.f ? 0.f : 1.f / sum;
+                half4_t v;
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[k] = f2h(acc[k] * y);
+                *reinterpret_cast<half4_t *>(a.out + (int64_t)(s.s0 + t) * a.ldo + head * a.Dh + d) = v;
+            } else {
+                const int64_t at = (int64_t)slot * (16 * NR) + r;
+                *reinterpret_cast<float4_t *>(a.part + at * a.Dh + d) = float4_t{acc[0], acc[1], acc[2], acc[3]};
+                if (d == 0) {
+                    a.stats[2 * at] = mx;
+                    a.stats[2 * at + 1] = sum;
+                }
+            }
+        }
+    }
+};
+
+// Workgroups of a CU: as many as the registers are for
+constexpr int resident(int ND, int NR, int bytes) { return NR == 1 && ND * bytes < 4 ? 3 : 2; }
+
+template <int ND, int NR, class P>
+__global__ void __launch_bounds__(kThreads, resident(ND, NR, sizeof(P))) paged_attention_kernel(AttnArgs a)
+{
+    constexpr int kRows = 16 * NR;
+    __shared__ typename Tile<ND, NR, P>::Shared sh;
+    double sum;
+    const int64_t units = uniform((int64_t)sum_of_work(a, kRows, 0, &sum));
+    const int64_t groups = min((int64_t)a.groups, units);
+    if (blockIdx.x >= groups) return;
+    int64_t x = uniform(begin_of(blockIdx.x, units, groups));
+    const int64_t until = uniform(begin_of((int64_t)blockIdx.x + 1, units, groups));
+    int b = sequence_at(a, kRows, (double)x, &sum);
+    int64_t before = uniform((int64_t)sum);
+    for (; x < until; b++) {
+        const Sequence s = sequence(a.pb, b, (int64_t)a.pb.W * a.pb.page, a.max_new);
+        const Share w(a, kRows, s);
+        const int64_t behind = before + uniform((int64_t)w.units);
+        while (x < until && x < behind) {
+            const int64_t at = x - before;
+            const int u = uniform((int)(at / w.blocks)), first = uniform((int)(at - (int64_t)u * w.blocks)), h = uniform(u / w.tiles);
+            const int row0 = (u - h * w.tiles) * kRows, count = (int)min((int64_t)(w.blocks - first), until - x), rows = s.n * a.G;
+            const int end = uniform(s.first + min(rows - 1, row0 + kRows - 1) / a.G + 1);         // positions that some row of the tile sees
+            Tile<ND, NR, P> t{a, sh};
+            const int c0 = first * kBlock, c1 = min(end, (first + count) * kBlock);
+            t.run(b, s, h, rows, row0, c0, c1);
+            t.write(b, s, h, rows, row0, c0, c1, count == w.blocks ? -1 : 2 * (int)blockIdx.x + (first == 0));
+            x += count;
+        }
+        before = behind;
     }
 }
 
-// The parts of a row put together: a wave per row and head, two columns per lane.
+// The parts of a row put together, by a wave per row and head with two columns per lane; zeros for rows whose sequence's numbers
+// do not fit together.
+template <int NR>
 __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs a)
 {
+    constexpr int kRows = 16 * NR;
     const PagedBatch &pb = a.pb;
     const int lane = threadIdx.x & 63;
     const int64_t rh = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
-    const int row = (int)(rh / a.H), head = (int)(rh - (int64_t)row * a.H);
+    const int row = (int)(rh / a.H), head = (int)(rh - (int64_t)row * a.H), d = min(2 * lane, a.Dh - 2);
     if (row >= pb.T) return;
     const int b = count_below(pb.B, row, [&](int i) { return pb.starts[i]; });
     if (b >= pb.B) return;
     const Sequence s = sequence(pb, b, (int64_t)pb.W * pb.page, a.max_new);
-    if (!s.ok || row < s.s0 || row >= s.s0 + s.n || s.first + s.n <= a.chunk) return;
-    const int parts = (s.first + row - s.s0) / a.chunk + 1;
-    const int64_t step = (int64_t)pb.T * a.H;
+    if (row < s.s0 || row - s.s0 >= s.n) return;
+    half_t *out = a.out + row * a.ldo + head * a.Dh + d;
+    if (!s.ok) {
+        if (lane == 0) report(pb, b);
+        if (2 * lane < a.Dh) *reinterpret_cast<half2_t *>(out) = half2_t{};
+        return;
+    }
+    double before;
+    const int64_t units = (int64_t)sum_of_work(a, kRows, b, &before);
+    const Share w(a, kRows, s);
+    const int h = head / a.G, r = (row - s.s0) * a.G + head - h * a.G, tile = r / kRows;
+    const int64_t first = (int64_t)before + (int64_t)(h * w.tiles + tile) * w.blocks;
+    // the workgroups that have its first and last unit: the largest i with begin_of(i) <= unit
+    const int64_t groups = min((int64_t)a.groups, units);
+    const int i0 = (int)(((first + 1) * groups - 1) / units), i1 = (int)(((first + w.blocks) * groups - 1) / units);
+    if (i0 == i1) return;
+    const int parts = i1 - i0 + 1;
+    auto at = [&](int p) { return (int64_t)(p == 0 ? 2 * i0 + 1 : 2 * (i0 + p)) * kRows + r - tile * kRows; };
     float mx = -INFINITY;
-    for (int p = lane; p < parts; p += 64) mx = fmaxf(mx, a.stats[2 * (p * step + rh)]);
-    const float base = finite_max(wave_max(mx));
-    const int d = min(2 * lane, a.Dh - 2);
+    for (int p = lane; p < parts; p += 64) mx = fmaxf(mx, a.stats[2 * at(p)]);
+    const float origin = finite_max(wave_max(mx));
     float sum = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll 4
     for (int p = 0; p < parts; p++) {
-        const int64_t at = p * step + rh;
-        const float f = exp2_of(a.stats[2 * at] - base);
-        const float2 v = *reinterpret_cast<const float2 *>(a.part + at * a.Dh + d);
-        sum += f * a.stats[2 * at + 1];
+        const int64_t i = at(p);
+        const float f = exp2_of(a.stats[2 * i] - origin);
+        const float2 v = *reinterpret_cast<const float2 *>(a.part + i * a.Dh + d);
+        sum += f * a.stats[2 * i + 1];
         o0 += f * v.x;
         o1 += f * v.y;
     }
     const float y = sum == 0.f ? 0.f : 1.f / sum;
-    if (2 * lane < a.Dh) {
-        const half2_t v = {f2h(o0 * y), f2h(o1 * y)};
-        *reinterpret_cast<half2_t *>(a.out + row * a.ldo + head * a.Dh + d) = v;
-    }
+    if (2 * lane < a.Dh) *reinterpret_cast<half2_t *>(out) = half2_t{f2h(o0 * y), f2h(o1 * y)};
 }
 
 struct Plan {
-    int NR, chunk, splits;
-    Units units;
+    int NR, groups;
 };
-
-Plan plan(int64_t T, int64_t B, int64_t H, int64_t Hkv, int64_t max_new, int64_t longest)
+Plan plan(int64_t T, int64_t H, int64_t Hkv, int64_t Dh, int64_t max_new, int bytes)
 {
-    const int64_t G = H / Hkv;
-    Plan p;
-    if (max_new > T) max_new = T;
-    p.NR = max_new * G <= 16 ? 1 : 2;
-    const int64_t tile = 16 * p.NR;
-    // (s1 G) / tile - (s0 G) / tile + 1 tiles are numbered from starts / (tile / G) + b on where G divides the tile; otherwise
-    // a tile is taken to hold no more tokens than fit whole
-    const int64_t tokens = G >= tile ? 1 : tile / G;
-    const int64_t most = (max_new * G + tile - 1) / tile;
-    p.units = G >= tile ? Units{(int)most, 1, 1, most * B} : make_units(T, B, tokens, 1, most);
-    const int64_t want = 4 * device_cus(), have = p.units.count * Hkv;
-    int64_t splits = want / have;
-    const int64_t limit = (longest + 127) / 128;
-    if (splits > limit) splits = limit;
-    if (splits < 1) splits = 1;
-    p.chunk = (int)((longest + splits - 1) / splits + 127) / 128 * 128;
-    p.splits = (int)((longest + p.chunk - 1) / p.chunk);
-    return p;
+    const int64_t G = H / Hkv, rows = (max_new < T ? max_new : T) * G;
+    const int NR = rows <= 16 ? 1 : 2;
+    return {NR, resident(Dh <= 64 ? 1 : 2, NR, bytes) * device_cus()};
 }
 
-template <class P>
-int launch(const AttnArgs &a, const Plan &p, hipStream_t st)
+template <int ND, int NR, class P>
+int launch(const AttnArgs &a, hipStream_t st)
 {
-    const dim3 grid((unsigned)(p.units.count * p.splits), (unsigned)a.Hkv), block(kThreads);
-    if (a.Dh <= 64) {
-        if (p.NR == 1) hipLaunchKernelGGL((paged_attention_kernel<1, 1, P>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((paged_attention_kernel<1, 2, P>), grid, block, 0, st, a);
-    } else {
-        if (p.NR == 1) hipLaunchKernelGGL((paged_attention_kernel<2, 1, P>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((paged_attention_kernel<2, 2, P>), grid, block, 0, st, a);
-    }
+    hipLaunchKernelGGL((paged_attention_kernel<ND, NR, P>), dim3((unsigned)a.groups), dim3(kThreads), 0, st, a);
     const int rc = launch_status("paged_attention");
-    if (rc || p.splits == 1) return rc;
+    if (rc) return rc;
     const int64_t waves = (int64_t)a.pb.T * a.H;
-    hipLaunchKernelGGL(paged_attention_join_kernel, dim3((unsigned)((waves + kWaves - 1) / kWaves)), block, 0, st, a);
+    hipLaunchKernelGGL(paged_attention_join_kernel<NR>, dim3((unsigned)((waves + kWaves - 1) / kWaves)), dim3(kThreads), 0, st, a);
     return launch_status("paged_attention (parts)");
+}
+template <class P>
+int launch(const AttnArgs &a, int NR, hipStream_t st)
+{
+    if (a.Dh <= 64) return NR == 1 ? launch<1, 1, P>(a, st) : launch<1, 2, P>(a, st);
+    return NR == 1 ? launch<2, 1, P>(a, st) : launch<2, 2, P>(a, st);
 }
 
 }  // namespace
 
-CACTI_API size_t cacti_hip_paged_attention_workspace(int64_t T, int64_t B, int64_t H, int64_t Hkv, int64_t Dh, int64_t max_new, int64_t page,
-                                                     int64_t W)
+CACTI_API size_t cacti_hip_paged_attention_workspace(int64_t T, int64_t B, int64_t H, int64_t Hkv, int64_t Dh, int64_t max_new)
 {
-    if (T <= 0 || B <= 0 || H <= 0 || Hkv <= 0 || Dh <= 0 || max_new <= 0 || page <= 0 || W <= 0 || H % Hkv) return 0;
-    const Plan p = plan(T, B, H, Hkv, max_new, W * page);
-    return p.splits == 1 ? 0 : (size_t)p.splits * (size_t)(T * H) * (size_t)(Dh + 2) * 4;
+    if (T <= 0 || B <= 0 || H <= 0 || Hkv <= 0 || Dh <= 0 || max_new <= 0 || H % Hkv) return 0;
+    const Plan p = plan(T, H, Hkv, Dh, max_new, 1);        // (of 16 bits: no more)
+    return (size_t)p.groups * 2 * (16 * p.NR) * (size_t)(Dh + 2) * 4;
 }
 
 CACTI_API int cacti_hip_paged_attention_f16(int64_t T, int64_t B, int64_t H, int64_t Hkv, int64_t Dh, int64_t max_new, float alpha,
@@ -527,15 +626,13 @@ CACTI_API int cacti_hip_paged_attention_f16(int64_t T, int64_t B, int64_t H, int
     CACTI_REQUIRE(q && out, CACTI_E_INVALID, "paged_attention: null pointer");
     CACTI_REQUIRE(ldq >= H * Dh && ldo >= H * Dh && ldq % 4 == 0 && ldo % 4 == 0 && aligned(q, 8) && aligned(out, 8), CACTI_E_INVALID,
                   "paged_attention: operands must be 8-byte aligned with row pitches that are multiples of 4 and hold a row");
-    const Plan p = plan(T, B, H, Hkv, max_new, W * page);
-    const size_t need = cacti_hip_paged_attention_workspace(T, B, H, Hkv, Dh, max_new, page, W);
-    CACTI_REQUIRE(need == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= need), CACTI_E_INVALID,
-                  "paged_attention: workspace too small or not 16-byte aligned");
-    CACTI_REQUIRE(p.units.count * p.splits < (1 << 24) && (T * H + kWaves - 1) / kWaves < (1 << 24), CACTI_E_NOTIMPL,
-                  "paged_attention: too many rows in one call");
+    CACTI_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= cacti_hip_paged_attention_workspace(T, B, H, Hkv, Dh, max_new),
+                  CACTI_E_INVALID, "paged_attention: workspace too small or not 16-byte aligned");
+    CACTI_REQUIRE((T * H + kWaves - 1) / kWaves < (1 << 24), CACTI_E_NOTIMPL, "paged_attention: too many rows in one call");
+    const Plan p = plan(T, H, Hkv, Dh, max_new, bits / 8);
     float *part = (float *)workspace;
-    const AttnArgs a = {pb, p.units, (int)H, (int)Hkv, (int)(H / Hkv), (int)Dh, padded_dim((int)Dh), (int)(max_new < T ? max_new : T), p.chunk,
-                        p.splits, alpha, (const half_t *)q, ldq, k_pages, v_pages, (const float *)k_scale, (const float *)v_scale,
-                        (half_t *)out, ldo, part, part ? part + (size_t)p.splits * T * H * Dh : nullptr};
-    return bits == 8 ? launch<uint8_t>(a, p, (hipStream_t)stream) : launch<half_t>(a, p, (hipStream_t)stream);
+    const AttnArgs a = {pb, (int)H, (int)Hkv, (int)(H / Hkv), (int)Dh, padded_dim((int)Dh), (int)(max_new < T ? max_new : T), p.groups,
+                        (unsigned)((1 << 22) / page + 1), alpha, (const half_t *)q, ldq, k_pages, v_pages, (const float *)k_scale,
+                        (const float *)v_scale, (half_t *)out, ldo, part, part + (size_t)p.groups * 2 * (16 * p.NR) * Dh};
+    return bits == 8 ? launch<uint8_t>(a, p.NR, (hipStream_t)stream) : launch<half_t>(a, p.NR, (hipStream_t)stream);
 }

@@ -87,23 +87,6 @@ __device__ __forceinline__ double weight(float x, float mx, double c)
     return y > -INFINITY ? w : 0.;
 }
 
-// inclusive sum over the lanes
-__device__ __forceinline__ double lane_f64(double v, int lane)
-{
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    return words_f64(__builtin_amdgcn_readlane((int)u, lane), __builtin_amdgcn_readlane((int)(u >> 32), lane));
-}
-__device__ __forceinline__ double scan_f64(double v)
-{
-    v += dpp_f64<0x111>(v);                    // row_shr 1, 2, 4, 8: nothing from before the 16
-    v += dpp_f64<0x112>(v);
-    v += dpp_f64<0x114>(v);
-    v += dpp_f64<0x118>(v);
-    const double r0 = lane_f64(v, 15), r1 = lane_f64(v, 31), r2 = lane_f64(v, 47);
-    const int row = (threadIdx.x & 63) >> 4;
-    return v + (row == 0 ? 0. : row == 1 ? r0 : row == 2 ? r0 + r1 : r0 + r1 + r2);
-}
-
 template <bool GREEDY>
 __global__ void __launch_bounds__(64 * kEntryWaves) verify_entries_kernel(VerifyArgs a)
 {

@@ -117,7 +117,7 @@ SIGNATURES = {
     "cacti_hip_attn_decode_f16": (ci, [i64, i64, i64, i64, i64, f32, vp, i64, vp, vp, i64, i64, vp, i64, vp, sz, vp]),
     "cacti_hip_paged_append": (ci, [i64] * 6 + [vp, i64, vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, vp, vp, vp, ci, i64, i64, vp, i64, i64,
                                                 vp, vp, vp, vp]),
-    "cacti_hip_paged_attention_workspace": (sz, [i64] * 8),
+    "cacti_hip_paged_attention_workspace": (sz, [i64] * 6),
     "cacti_hip_paged_attention_f16": (ci, [i64] * 6 + [f32, vp, i64, vp, vp, vp, vp, ci, i64, i64, vp, i64, i64, vp, vp, vp, i64, vp, sz,
                                                        vp, vp]),
     "cacti_hip_verify_draft_workspace": (sz, [i64, i64, i64]),

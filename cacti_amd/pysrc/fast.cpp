@@ -579,12 +579,12 @@ PyObject *paged_attention(PyObject *const *o)
     }
     void *status = on.pointer(o[11], at::kInt, 1), *st = on.stream();
     if (q.T > 0 && c.B > 0 && max_new > 0) {
-        const size_t bytes = cacti_hip_paged_attention_workspace(q.T, c.B, q.H, c.Hkv, q.Dh, max_new, c.page, c.W);
-        const at::Tensor ws = bytes ? empty({(int64_t)bytes}, q.t, at::kByte) : at::Tensor();
+        const size_t bytes = cacti_hip_paged_attention_workspace(q.T, c.B, q.H, c.Hkv, q.Dh, max_new);
+        const at::Tensor ws = empty({(int64_t)bytes}, q.t, at::kByte);
         run([&] {
             return cacti_hip_paged_attention_f16(q.T, c.B, q.H, c.Hkv, q.Dh, max_new, alpha, q.t.data_ptr(), q.ld, c.k.data_ptr(),
                                                  c.v.data_ptr(), c.ks, c.vs, c.bits, c.P, c.page, c.table.data_ptr(), c.ldt, c.W, c.starts,
-                                                 c.lens, out.ptr(), ldo, bytes ? ws.data_ptr() : nullptr, bytes, status, st);
+                                                 c.lens, out.ptr(), ldo, ws.data_ptr(), bytes, status, st);
         });
     }
     return out.take();

@@ -462,10 +462,9 @@ int cacti_hip_paged_append(int64_t T, int64_t B, int64_t H, int64_t Hkv, int64_t
 
 /* out [T, ldo] f16 = softmax_j(alpha q . k_j) v over the positions j up to the row's own, which are in the cache; fp32 scores
  * and sums, the weights rounded to f16 for the second product.  A row's result depends on nothing behind its position.  Scales
- * are positive, any of them.  workspace: cacti_hip_paged_attention_workspace bytes (0: none), 16-byte aligned, contents
- * undefined on return. */
-size_t cacti_hip_paged_attention_workspace(int64_t T, int64_t B, int64_t H, int64_t Hkv, int64_t Dh, int64_t max_new, int64_t page,
-                                           int64_t W);
+ * are positive, any of them.  workspace: cacti_hip_paged_attention_workspace bytes, 16-byte aligned, contents undefined on
+ * return. */
+size_t cacti_hip_paged_attention_workspace(int64_t T, int64_t B, int64_t H, int64_t Hkv, int64_t Dh, int64_t max_new);
 int cacti_hip_paged_attention_f16(int64_t T, int64_t B, int64_t H, int64_t Hkv, int64_t Dh, int64_t max_new, float alpha,
                                   const void *q, int64_t ldq, const void *k_pages, const void *v_pages, const void *k_scale,
                                   const void *v_scale, int bits, int64_t P, int64_t page, const void *table, int64_t ldt, int64_t W,

@@ -42,20 +42,19 @@ def test_append_refuses(change, why):
 
 
 @pytest.mark.parametrize("change,why", COMMON + [(dict(q=None), "null"), (dict(out=None), "null"), (dict(ldo=30), "multiples of 4"),
-                                                 (dict(W=600, ldt=600, ws_bytes=64), "workspace"), (dict(W=600, ldt=600, ws=72), "workspace"),
-                                                 (dict(W=600, ldt=600, ws=None), "workspace")])
+                                                 (dict(ws_bytes=64), "workspace"), (dict(ws=72), "workspace"),
+                                                 (dict(ws=None), "workspace")])
 def test_attention_refuses(change, why):
     L = ffi.lib()
     assert L.cacti_hip_paged_attention_f16(*dict(ATTEND, **change).values()) < 0
     assert why in L.cacti_hip_last_error().decode()
 
 
-def test_workspace_holds_the_parts_of_every_row():
+def test_workspace_does_not_grow_with_the_positions():
     ws = ffi.lib().cacti_hip_paged_attention_workspace
-    for T, B, H, Hkv, Dh, new, page, W in [(1, 1, 32, 32, 100, 1, 64, 25), (48, 48, 32, 32, 100, 1, 64, 128), (700, 3, 16, 4, 128, 600, 16, 500)]:
-        assert ws(T, B, H, Hkv, Dh, new, page, W) % (T * H * (Dh + 2) * 4) == 0
-    assert ws(1, 1, 32, 32, 100, 1, 64, 25) > 0          # one sequence's positions are shared among workgroups
-    assert ws(1, 1, 32, 32, 100, 1, 16, 1) == 0
+    for T, B, H, Hkv, Dh, new in [(1, 1, 32, 32, 100, 1), (48, 48, 32, 32, 100, 1), (700, 3, 16, 4, 128, 600)]:
+        assert 0 < ws(T, B, H, Hkv, Dh, new) < 64 << 20 and ws(T, B, H, Hkv, Dh, new) % 16 == 0
+    assert ws(0, 1, 32, 32, 100, 1) == 0 and ws(1, 1, 3, 2, 100, 1) == 0
 
 
 # ---------------------------------------------------------------- plain forms
