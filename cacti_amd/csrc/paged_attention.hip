@@ -8,16 +8,16 @@
 // Scores, maxima, sums and o are fp32; w is rounded to f16 for the matrix instruction (2^-11 relative, each on its own, which
 // is what the rounding of the output adds once more).
 //
-// A workgroup takes 16 NR rows (tokens of a sequence by the query heads that share a key head) of a key head at a time; its
-// four waves take 32 positions in turn and put their sums together at the end.  The products are formed transposed, S^T = K Q^T
-// and O^T = V^T W^T with v_mfma_f32_16x16x32_f16: a lane then holds the scores of one row, at keys that are exactly those its
-// part of the second product's operand wants, so that w never leaves the lane.  Keys come from memory in the order the
-// instruction takes them (16 columns of a key to a lane); V, whose operand is a column of eight keys, is read as rows of 8
-// columns and turned with byte permutes.  No LDS, no barrier in between; the keys after these are requested once these have
-// been multiplied, the values likewise, into the same registers.
+// A wave takes 16 NR rows (tokens of a sequence by the query heads that share a key head) of a key head at a time, by itself, 32
+// positions at a time.  The products are formed transposed, S^T = K Q^T and O^T = V^T W^T with v_mfma_f32_16x16x32_f16: a lane
+// then holds the scores of one row, at keys that are exactly those its part of the second product's operand wants, so that w
+// never leaves the lane.  Keys come from memory in the order the instruction takes them (16 columns of a key to a lane); V, whose
+// operand is a column of eight keys, is read as rows of 8 columns and turned with byte permutes.  No LDS but for the pages'
+// numbers, no barrier; the keys after these are requested once these have been multiplied, the values likewise, into the same
+// registers.
 //
-// Work: the lengths are on the device and as different as they come, so every workgroup of a launch that just fills the device
-// forms their sum in blocks of 128 positions and takes an equal, contiguous share of it, across rows, heads and sequences.  A
+// Work: the lengths are on the device and as different as they come, so every wave of a launch that just fills the device
+// forms their sum in steps of 32 positions and takes an equal, contiguous share of it, across rows, heads and sequences.  A
 // tile of rows that ends up in more than one share leaves partial sums, which a second launch puts together.
 #include "paged.h"
 
@@ -25,14 +25,15 @@ using namespace cacti;
 
 namespace {
 
-constexpr int kThreads = 256, kWaves = 4, kStep = 32, kBlock = kWaves * kStep;
-constexpr int kSegment = 8192;                 // positions whose pages a workgroup looks up at a time
-constexpr int kEntries = kSegment / 16 + 1;
+constexpr int kThreads = 256, kWaves = 4, kStep = 32;
+constexpr int kEntries = 64;                   // pages that a wave looks up at a time, one to a lane
+// What a tile of rows costs a share besides its steps, in steps: queries, pages and the first keys to wait for
+constexpr int kBegin = 4;
 
 struct AttnArgs {
     PagedBatch pb;
     int H, Hkv, G, Dh, Dp, max_new, groups;
-    unsigned page_magic;                       // x / page = x * page_magic >> 22 for x up to kSegment + 256
+    unsigned page_magic;                       // x / page = x * page_magic >> 22 for x below kEntries pages
     float alpha;
     const half_t *q;
     int64_t ldq;
@@ -40,62 +41,67 @@ struct AttnArgs {
     const float *k_scale, *v_scale;
     half_t *out;
     int64_t ldo;
-    float *part, *stats;                       // [2 groups][16 NR][Dh], [2 groups][16 NR][2]
+    float *part, *stats;                       // [2 groups][16 NR][Dh], [2 groups][16 NR][2]; a group: a wave
 };
 
 // What is the same in all lanes, in scalar registers
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ int64_t uniform(int64_t x)
-{
-    return (int64_t)((uint64_t)(unsigned)uniform((int)(x >> 32)) << 32 | (unsigned)uniform((int)x));
-}
 
-// A sequence's share of the work: its tiles of 16 NR rows by its blocks of positions, by heads
+// A sequence's share of the work: its tiles of rows by its steps (and kBegin), by heads
 struct Share {
-    int tiles, blocks;
-    double units;
+    int tiles, steps;
+    unsigned units;
     __device__ __forceinline__ Share(const AttnArgs &a, int tile, const Sequence &s)
-        : tiles((s.n * a.G + tile - 1) / tile), blocks((s.first + s.n + kBlock - 1) / kBlock),
-          units(s.ok && s.n > 0 ? (double)tiles * blocks * a.Hkv : 0.)
+        : tiles((s.n * a.G + tile - 1) / tile), steps((s.first + s.n + kStep - 1) / kStep),
+          units(s.ok && s.n > 0 ? (unsigned)(tiles * (steps + kBegin) * a.Hkv) : 0u)
     {
     }
 };
-// All of it, and what there is before sequence `until` (whole numbers in fp64), by a wave
-__device__ __forceinline__ double sum_of_work(const AttnArgs &a, int tile, int until, double *before)
+__device__ __forceinline__ unsigned units_of(const AttnArgs &a, int tile, int b)
+{
+    return b < a.pb.B ? Share(a, tile, sequence(a.pb, b, (int64_t)a.pb.W * a.pb.page, a.max_new)).units : 0u;
+}
+// All of it, and what there is before sequence `until`, by a wave
+__device__ __forceinline__ unsigned sum_of_work(const AttnArgs &a, int tile, int until, unsigned *before)
 {
     const int lane = threadIdx.x & 63;
-    double all = 0., some = 0.;
+    double all = 0., some = 0.;                // (whole numbers)
     for (int b0 = 0; b0 < a.pb.B; b0 += 64) {
-        const int b = b0 + lane;
-        const double u = b < a.pb.B ? Share(a, tile, sequence(a.pb, b, (int64_t)a.pb.W * a.pb.page, a.max_new)).units : 0.;
+        const double u = units_of(a, tile, b0 + lane);
         all += u;
-        some += b < until ? u : 0.;
+        some += b0 + lane < until ? u : 0.;
     }
-    *before = wave_sum_f64(some);
-    return wave_sum_f64(all);
+    *before = (unsigned)wave_sum_f64(some);
+    return (unsigned)wave_sum_f64(all);
 }
 // The sequence in whose work unit x lies, and what there is before it
-__device__ __forceinline__ int sequence_at(const AttnArgs &a, int tile, double x, double *before)
+__device__ __forceinline__ int sequence_at(const AttnArgs &a, int tile, unsigned x, unsigned *before)
 {
     const int lane = threadIdx.x & 63;
     double all = 0.;
     for (int b0 = 0; b0 < a.pb.B; b0 += 64) {
-        const int b = b0 + lane;
-        const double u = b < a.pb.B ? Share(a, tile, sequence(a.pb, b, (int64_t)a.pb.W * a.pb.page, a.max_new)).units : 0.;
-        const double upto = scan_f64(u) + all;
-        const uint64_t hit = __ballot(upto > x);
+        const double u = units_of(a, tile, b0 + lane), upto = scan_f64(u) + all;
+        const uint64_t hit = __ballot(upto > (double)x);
         if (hit) {
             const int at = __ffsll((unsigned long long)hit) - 1;
-            *before = lane_f64(upto - u, at);
+            *before = (unsigned)lane_f64(upto - u, at);
             return b0 + at;
         }
         all = lane_f64(upto, 63);
     }
-    *before = all;
     return a.pb.B;
 }
-// Of `groups` workgroups that take part, at least a unit for each, i has the units from begin_of(i) to begin_of(i + 1)
-__device__ __forceinline__ int64_t begin_of(int64_t i, int64_t units, int64_t groups) { return i * units / groups; }
+// Equal shares of `units`: group i has those from begin(i) to begin(i + 1), the first `more` of them one more than `each`
+struct Shares {
+    unsigned each, more;
+    __device__ __forceinline__ Shares(unsigned units, unsigned groups) : each(units / groups), more(units - each * groups) {}
+    __device__ __forceinline__ unsigned begin(unsigned i) const { return i * each + min(i, more); }
+    __device__ __forceinline__ unsigned of(unsigned unit) const          // the group that has it
+    {
+        const unsigned edge = more * (each + 1);
+        return unit < edge ? unit / (each + 1) : more + (unit - edge) / each;
+    }
+};
 
 typedef unsigned u4_t __attribute__((ext_vector_type(4)));
 typedef unsigned u2_t __attribute__((ext_vector_type(2)));
@@ -118,15 +124,6 @@ template <>
 struct KPiece<uint8_t> {
     u4_t w;
     __device__ __forceinline__ void load(const uint8_t *p) { w = *reinterpret_cast<const u4_t *>(p); }
-    __device__ __forceinline__ half8_t part(int s) const
-    {
-        Frag f;
-        f.u[0] = cvt8(w[2 * s], false);
-        f.u[1] = cvt8(w[2 * s], true);
-        f.u[2] = cvt8(w[2 * s + 1], false);
-        f.u[3] = cvt8(w[2 * s + 1], true);
-        return f.h;
-    }
 };
 template <>
 struct KPiece<half_t> {
@@ -136,8 +133,111 @@ struct KPiece<half_t> {
         w[0] = *reinterpret_cast<const half8_t *>(p);
         w[1] = *reinterpret_cast<const half8_t *>(p + 8);
     }
-    __device__ __forceinline__ half8_t part(int s) const { return w[s]; }
     __device__ __forceinline__ void zero() { w[0] = w[1] = half8_t{}; }
+};
+
+typedef int i8_t __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ float4_t mfma(half8_t a, half8_t b, float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+// The lane's part of a query: of each 64 columns those that it has of a key.  f(d): 4 of them from column d on.
+template <int ND, class P>
+struct Query;
+template <int ND>
+struct Query<ND, half_t> {
+    half8_t h[2 * ND];
+    template <class F>
+    __device__ __forceinline__ float set(F f)              // returns what the products have to be multiplied by
+    {
+        const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int c = 0; c < 2 * ND; c++) {
+            Frag x;
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const u2_t w = f(64 * (c / 2) + 16 * g + 8 * (c & 1) + 4 * j);
+                x.u[2 * j] = w[0];
+                x.u[2 * j + 1] = w[1];
+            }
+            h[c] = x.h;
+        }
+        return 1.f;
+    }
+    __device__ __forceinline__ float4_t times(const KPiece<half_t> (&k)[ND]) const
+    {
+        float4_t s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 2 * ND; c++) s = mfma(k[c / 2].w[c & 1], h[c], s);
+        return s;
+    }
+};
+// Against codes: three e4m3 terms, each the rounded rest of those before, of the query scaled by a power of two to have its
+// largest element between 224 and 448.  They have 4 + 5 + 5 bits, and so all 11 of an element of at least 1/112 of the largest
+// (below, they are off by 2^-10, 2^-18 of the largest); the codes need no conversion, which is 32 vector operations of 64
+// columns by 32 keys, and the products of 8 bits have the matrix pipe to themselves.
+template <int ND>
+struct Query<ND, uint8_t> {
+    int t[3][4 * ND];
+    template <class F>
+    __device__ __forceinline__ float set(F f)
+    {
+        const int g = (threadIdx.x & 63) >> 4;
+        float x[16 * ND], mx = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4 * ND; i++) {
+            const half4_t w = __builtin_bit_cast(half4_t, f(64 * (i / 4) + 16 * g + 4 * (i & 3)));
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                x[4 * i + k] = h2f(w[k]);
+                mx = fmaxf(mx, fabsf(x[4 * i + k]));
+            }
+        }
+        mx = with32(with16(mx, OpMax()), OpMax());
+        int e = 0;
+        if (mx > 0.f && mx < INFINITY) e = __builtin_amdgcn_frexp_expf(mx) - (__builtin_amdgcn_frexp_mantf(mx) > 0.875f ? 8 : 9);
+#pragma unroll
+        for (int i = 0; i < 4 * ND; i++) {
+            float y[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) y[k] = __builtin_amdgcn_ldexpf(x[4 * i + k], -e);
+#pragma unroll
+            for (int n = 0; n < 3; n++) {
+                int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+                w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
+                t[n][i] = w;
+                y[0] -= __builtin_amdgcn_cvt_f32_fp8(w, 0);
+                y[1] -= __builtin_amdgcn_cvt_f32_fp8(w, 1);
+                y[2] -= __builtin_amdgcn_cvt_f32_fp8(w, 2);
+                y[3] -= __builtin_amdgcn_cvt_f32_fp8(w, 3);
+            }
+        }
+        return __builtin_amdgcn_ldexpf(1.f, e);
+    }
+    __device__ __forceinline__ float4_t times(const KPiece<uint8_t> (&k)[ND]) const
+    {
+        float4_t s = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (ND == 2) {
+            i8_t a;
+#pragma unroll
+            for (int i = 0; i < 8; i++) a[i] = (int)k[i / 4].w[i & 3];
+#pragma unroll
+            for (int n = 2; n >= 0; n--) {
+                i8_t b;
+#pragma unroll
+                for (int i = 0; i < 8; i++) b[i] = t[n][i];
+                // (scales of 2^0: e8m0 127 in every byte)
+                s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, s, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+            }
+        } else {
+#pragma unroll
+            for (int n = 2; n >= 0; n--)
+#pragma unroll
+                for (int c = 0; c < 2; c++)
+                    s = __builtin_amdgcn_mfma_f32_16x16x32_fp8_fp8((long)((uint64_t)k[0].w[2 * c + 1] << 32 | k[0].w[2 * c]),
+                                                                   (long)((uint64_t)(unsigned)t[n][2 * c + 1] << 32 | (unsigned)t[n][2 * c]), s, 0, 0, 0);
+        }
+        return s;
+    }
 };
 
 // Eight keys by VD columns (8 or 4) of V, as loaded: a row of columns per key
@@ -169,6 +269,11 @@ struct VBlock<uint8_t, VD> {
             w[i][j] &= ~((bad >> 7) * 0xffu);
         }
         return any;
+    }
+    __device__ __forceinline__ float value(int c) const    // of the first key
+    {
+        return (c & 3) == 0 ? __builtin_amdgcn_cvt_f32_fp8(w[0][c / 4], 0) : (c & 3) == 1 ? __builtin_amdgcn_cvt_f32_fp8(w[0][c / 4], 1)
+             : (c & 3) == 2 ? __builtin_amdgcn_cvt_f32_fp8(w[0][c / 4], 2) : __builtin_amdgcn_cvt_f32_fp8(w[0][c / 4], 3);
     }
     // columns 2 c and 2 c + 1, each over the eight keys
     __device__ __forceinline__ void columns(int c, half8_t *a, half8_t *b) const
@@ -215,6 +320,7 @@ struct VBlock<half_t, VD> {
         }
         return any;
     }
+    __device__ __forceinline__ float value(int c) const { return h2f(__builtin_bit_cast(half2_t, w[0][c / 2])[c & 1]); }
     __device__ __forceinline__ void columns(int c, half8_t *a, half8_t *b) const
     {
         Frag x, y;
@@ -228,8 +334,6 @@ struct VBlock<half_t, VD> {
     }
 };
 
-__device__ __forceinline__ float4_t mfma(half8_t a, half8_t b, float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
 
@@ -239,25 +343,22 @@ struct Entry {
     float c, lg, iv;                           // alpha ks log2 e, log2 vs, 1 / vs
 };
 
-// One tile of rows and a part of its positions.  ND: pieces of 64 columns of a head
+// One tile of rows and a part of its positions, by a wave.  ND: pieces of 64 columns of a head
 template <int ND, int NR, class P>
 struct Tile {
     static constexpr int VD = 4 * ND;          // columns of V of a lane
-    static constexpr int NS = 2 * ND;          // matrix instructions along the columns of a key
-    struct Shared {
-        Entry entry[kEntries];
-        float merged[kWaves][16 * NR][VD * 16 + 4];
-        float m[kWaves][16 * NR], l[kWaves][16 * NR];
-        int odd;                               // there was a NaN or an infinity of V that some rows see
-    };
     const AttnArgs &a;
-    Shared &sh;
-    half8_t q[NR][NS];
-    int last[NR];                              // the lane's row of each 16: its last position
+    Entry *entry;                              // the wave's, in LDS
+    Query<ND, P> q[NR];                        // the lane's row of each 16: its query, a score's factor, its last position
+    float factor[NR];
+    int last[NR];
     float m[NR], l[NR];
     float4_t o[NR][VD];
     KPiece<P> kk[2][ND];
     VBlock<P, VD> vv;
+    bool odd;                                  // there was a NaN or an infinity of V that some rows see
+
+    __device__ __forceinline__ int page_of(int x) const { return (int)(__umul24((unsigned)x, a.page_magic) >> 22); }
 
     // keys and values of the 32 positions from x on, counted from the first entry's page; behind `end` the last one again
     __device__ __forceinline__ void load_k(int x, int end)
@@ -266,7 +367,7 @@ struct Tile {
 #pragma unroll
         for (int t = 0; t < 2; t++) {
             const int j = min(x + 8 * (r16 >> 2) + 4 * t + (r16 & 3), end - 1), pg = page_of(j);
-            const P *row = (const P *)a.k_pages + sh.entry[pg].at + (j - pg * a.pb.page) * a.Dp;
+            const P *row = (const P *)a.k_pages + entry[pg].at + __umul24(j - __umul24(pg, a.pb.page), a.Dp);
 #pragma unroll
             for (int c = 0; c < ND; c++) {
                 kk[t][c].load(row + min(64 * c + 16 * g, a.Dp - 16));
@@ -280,48 +381,37 @@ struct Tile {
     {
         const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
         const int j0 = x + 8 * g, pg = page_of(min(j0, end - 1));          // one page: of 16 positions or a multiple
-        const P *row = (const P *)a.v_pages + sh.entry[pg].at + min(VD * r16, a.Dp - VD);
+        const P *row = (const P *)a.v_pages + entry[pg].at + min(VD * r16, a.Dp - VD);
 #pragma unroll
-        for (int i = 0; i < 8; i++) vv.load(i, row + (min(j0 + i, end - 1) - pg * a.pb.page) * a.Dp);
+        for (int i = 0; i < 8; i++) vv.load(i, row + __umul24(min(j0 + i, end - 1) - __umul24(pg, a.pb.page), a.Dp));
     }
-    __device__ __forceinline__ int page_of(int x) const { return (int)((unsigned)x * a.page_magic >> 22); }
 
-    // positions c0 .. c1 - 1 of rows row0 .. of sequence s; `least`: positions up to there are seen by every row
+    // positions c0 .. c1 - 1 of rows row0 .. of sequence s
     __device__ __forceinline__ void run(int b, const Sequence &s, int h, int rows, int row0, int c0, int c1)
     {
-        const int lane = threadIdx.x & 63, wid = uniform((int)threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
+        const int lane = threadIdx.x & 63, r16 = lane & 15;
+        odd = false;
 #pragma unroll
         for (int n = 0; n < NR; n++) {
             const int r = min(row0 + 16 * n + r16, rows - 1), t = r / a.G;
             last[n] = s.first + t;
             const half_t *qr = a.q + (int64_t)(s.s0 + t) * a.ldq + (h * a.G + r - t * a.G) * a.Dh;
-#pragma unroll
-            for (int c = 0; c < ND; c++)
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    Frag f;
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {  // pieces of four columns: Dh is a multiple of 4
-                        const int d = 64 * c + 16 * g + 8 * k + 4 * j;
-                        const u2_t w = *reinterpret_cast<const u2_t *>(qr + min(d, a.Dh - 4));
-                        f.u[2 * j] = d < a.Dh ? w[0] : 0u;
-                        f.u[2 * j + 1] = d < a.Dh ? w[1] : 0u;
-                    }
-                    q[n][2 * c + k] = f.h;
-                }
+            factor[n] = q[n].set([&](int d) __attribute__((always_inline)) {                      // (Dh is a multiple of 4)
+                const u2_t w = *reinterpret_cast<const u2_t *>(qr + min(d, a.Dh - 4));
+                return d < a.Dh ? w : u2_t{0u, 0u};
+            });
             m[n] = -INFINITY;
             l[n] = 0.f;
 #pragma unroll
             for (int i = 0; i < VD; i++) o[n][i] = float4_t{0.f, 0.f, 0.f, 0.f};
         }
-        const int least = uniform(s.first + row0 / a.G);
-        for (int seg = c0; seg < c1; seg += kSegment) {
-            const int p0 = uniform(seg / a.pb.page), base = p0 * a.pb.page, end = min(c1, seg + kSegment) - base;
-            const int np = page_of(end - 1) + 1;
-            __syncthreads();                   // (the entries of before are done with)
-            if (seg == c0 && threadIdx.x == 0) sh.odd = 0;
-            for (int i = threadIdx.x; i < np; i += kThreads) {
-                int id = a.pb.table[(int64_t)b * a.pb.ldt + p0 + i];
+        const int least = uniform(s.first + row0 / a.G);       // positions up to there are seen by every row
+        for (int seg = c0; seg < c1;) {
+            const int p0 = uniform(seg / a.pb.page), base = p0 * a.pb.page, end = min(c1 - base, kEntries * a.pb.page);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");         // (the entries of before are done with)
+            __builtin_amdgcn_wave_barrier();
+            if (lane <= page_of(end - 1)) {
+                int id = a.pb.table[(int64_t)b * a.pb.ldt + p0 + lane];
                 if (id < 0 || id >= a.pb.P) {
                     report(a.pb, b);
                     id = 0;                    // its rows are unspecified, not its reads
@@ -330,47 +420,45 @@ struct Tile {
                 Entry e = {ph * a.pb.page * a.Dp, a.alpha * 1.44269504088896340736f, 0.f, 1.f};
                 if (sizeof(P) == 1) {
                     e.c *= a.k_scale[ph];
-                    e.lg = log2f(a.v_scale[ph]);
-                    e.iv = 1.f / a.v_scale[ph];
+                    e.lg = __builtin_amdgcn_logf(a.v_scale[ph]);
+                    e.iv = __builtin_amdgcn_rcpf(a.v_scale[ph]);
                 }
-                sh.entry[i] = e;
+                entry[lane] = e;
             }
-            __syncthreads();
-            int x = seg - base + kStep * wid;
-            if (x >= end) continue;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            int x = seg - base;
             load_k(x, end);
             load_v(x, end);
-            for (; x < end; x += kBlock) step(x, end, least - base, base, min(x + kBlock, end - 1));
+            const int clear = min(least - base, end - 1);      // up to here everything is seen by every row
+            for (; x + kStep - 1 <= clear; x += kStep) step<false>(x, end, least - base, base, min(x + kStep, end - 1));
+            for (; x < end; x += kStep) step<true>(x, end, least - base, base, min(x + kStep, end - 1));
+            seg = base + end;
         }
     }
 
+    // EDGE: some of these 32 positions are hidden from some row
+    template <bool EDGE>
     __device__ __forceinline__ void step(int x, int end, int least, int base, int next)
     {
         const int lane = threadIdx.x & 63, g = lane >> 4;
         float4_t sc[NR][2];
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
+        for (int t = 0; t < 2; t++)
 #pragma unroll
-            for (int n = 0; n < NR; n++) sc[n][t] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < NS; c++) {
-                const half8_t kf = kk[t][c / 2].part(c & 1);
-#pragma unroll
-                for (int n = 0; n < NR; n++) sc[n][t] = mfma(kf, q[n][c], sc[n][t]);
-            }
-        }
+            for (int n = 0; n < NR; n++) sc[n][t] = q[n].times(kk[t]);
         load_k(next, end);
-        const Entry &en = sh.entry[page_of(min(x + 8 * g, end - 1))];      // of the lane's eight keys
+        const Entry &en = entry[page_of(min(x + 8 * g, end - 1))];      // of the lane's eight keys
         const float ec = en.c, lg = en.lg, iv = en.iv;
-        const bool edge = x + kStep - 1 > min(least, end - 1);             // (the same in every lane)
         half8_t w[NR];
 #pragma unroll
         for (int n = 0; n < NR; n++) {
             float t[8], mx = -INFINITY;
+            const float c = ec * factor[n];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                t[i] = __builtin_fmaf(i < 4 ? sc[n][0][i & 3] : sc[n][1][i & 3], ec, lg);
-                if (edge && x + 8 * g + i > min(last[n] - base, end - 1)) t[i] = -INFINITY;
+                t[i] = __builtin_fmaf(i < 4 ? sc[n][0][i & 3] : sc[n][1][i & 3], c, lg);
+                if (EDGE && x + 8 * g + i > min(last[n] - base, end - 1)) t[i] = -INFINITY;
                 mx = fmaxf(mx, t[i]);
             }
             mx = with32(with16(mx, OpMax()), OpMax());
@@ -397,17 +485,17 @@ struct Tile {
             l[n] = __builtin_fmaf(sum, iv, l[n]);
             w[n] = p.h;
         }
-        if (edge) {
+        if (EDGE) {
             // what no row of the tile sees is nothing; a NaN or an infinity that some rows see must not meet the zero weights of
             // the others: it is added at the end
-            bool odd = false;
+            bool any = false;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const int j = x + 8 * g + i;
                 if (j >= end) vv.zero(i);
-                else if (j > least) odd = vv.strip(i) || odd;
+                else if (j > least) any = vv.strip(i) || any;
             }
-            if (odd) sh.odd = 1;
+            if (__ballot(any)) odd = true;
         }
 #pragma unroll
         for (int c = 0; c < VD / 2; c++) {
@@ -423,106 +511,95 @@ struct Tile {
         load_v(next, end);
     }
 
-    // NaNs and infinities of V at positions j0 .. j1 - 1, columns d .. d + 3
-    __device__ __forceinline__ void add_odd(int b, int h, int j0, int j1, int d, float (&acc)[4]) const
+    // NaNs and infinities of V at positions j0 .. j1 - 1, each to the rows that see it
+    __device__ __forceinline__ void add_odd(int b, int h, int j0, int j1)
     {
+        const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll 1
         for (int j = j0; j < j1; j++) {
             const int id = a.pb.table[(int64_t)b * a.pb.ldt + j / a.pb.page];
-            const P *v = (const P *)a.v_pages + (((int64_t)(id < 0 || id >= a.pb.P ? 0 : id) * a.Hkv + h) * a.pb.page + j % a.pb.page) * a.Dp + d;
-            for (int k = 0; k < 4; k++) {
-                const float x = value(v[k]);
-                if (!(fabsf(x) < INFINITY)) acc[k] += x;
+            const P *v = (const P *)a.v_pages + (((int64_t)(id < 0 || id >= a.pb.P ? 0 : id) * a.Hkv + h) * a.pb.page + j % a.pb.page) * a.Dp;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                VBlock<P, VD> x;
+                x.load(0, v + min(VD * (4 * g + i), a.Dp - VD));
+#pragma unroll
+                for (int c = 0; c < VD; c++)
+#pragma unroll
+                    for (int n = 0; n < NR; n++)
+                        if (!(fabsf(x.value(c)) < INFINITY) && j <= last[n]) o[n][c][i] += x.value(c);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
-    static __device__ __forceinline__ float value(half_t x) { return h2f(x); }
-    static __device__ __forceinline__ float value(uint8_t x) { return __builtin_amdgcn_cvt_f32_fp8(x, 0); }
 
-    // The four waves' sums put together: a lane has columns VD (4 g + i) + c of its row in o[.][c][i].  slot < 0: to the output
-    __device__ __forceinline__ void write(int b, const Sequence &s, int h, int rows, int row0, int c0, int c1, int slot)
+    // A lane has columns VD (4 g + i) + c of its row in o[.][c][i].  slot < 0: to the output
+    __device__ __forceinline__ void write(const Sequence &s, int h, int rows, int row0, int slot)
     {
-        const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, r16 = lane & 15, g = lane >> 4;
-        __syncthreads();                       // (the sums of before are done with)
+        const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
 #pragma unroll
         for (int n = 0; n < NR; n++) {
-            l[n] = with32(with16(l[n], OpSum()), OpSum());
-            if (g == 0) {
-                sh.m[wid][16 * n + r16] = m[n];
-                sh.l[wid][16 * n + r16] = l[n];
-            }
+            const float sum = with32(with16(l[n], OpSum()), OpSum());
+            const int r = row0 + 16 * n + r16, t = r / a.G;
+            if (r >= rows) continue;
+            const float y = slot >= 0 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+            const int64_t at = (int64_t)slot * (16 * NR) + 16 * n + r16;
+            half_t *out = a.out + (int64_t)(s.s0 + t) * a.ldo + (h * a.G + r - t * a.G) * a.Dh;
+            float *part = a.part + at * a.Dh;
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int c = 0; c < VD; c++) sh.merged[wid][16 * n + r16][VD * (4 * g + i) + c] = o[n][c][i];
-        }
-        __syncthreads();
-        const int per = a.Dh / 4;
-        const bool odd = c0 < c1 && sh.odd;
-        for (int i = threadIdx.x; i < 16 * NR * per; i += kThreads) {
-            const int r = i / per, d = 4 * (i - r * per);
-            if (row0 + r >= rows) break;
-            float mx = sh.m[0][r];
-#pragma unroll
-            for (int w = 1; w < kWaves; w++) mx = fmaxf(mx, sh.m[w][r]);
-            const float origin = finite_max(mx);
-            float sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int w = 0; w < kWaves; w++) {
-                const float f = exp2_of(sh.m[w][r] - origin);
-                sum += f * sh.l[w][r];
-#pragma unroll
-                for (int k = 0; k < 4; k++) acc[k] += f * sh.merged[w][r][d + k];
-            }
-            if (odd) add_odd(b, h, max(c0, s.first + row0 / a.G + 1), min(c1, s.first + (row0 + r) / a.G + 1), d, acc);
-            if (slot < 0) {
-                const int t = (row0 + r) / a.G, head = h * a.G + row0 + r - t * a.G;
-                const float y = sum == 0.f ? 0.f : 1.f / sum;
-                half4_t v;
-#pragma unroll
-                for (int k = 0; k < 4; k++) v[k] = f2h(acc[k] * y);
-                *reinterpret_cast<half4_t *>(a.out + (int64_t)(s.s0 + t) * a.ldo + head * a.Dh + d) = v;
-            } else {
-                const int64_t at = (int64_t)slot * (16 * NR) + r;
-                *reinterpret_cast<float4_t *>(a.part + at * a.Dh + d) = float4_t{acc[0], acc[1], acc[2], acc[3]};
-                if (d == 0) {
-                    a.stats[2 * at] = mx;
-                    a.stats[2 * at + 1] = sum;
+                for (int c = 0; c < VD; c += 4) {
+                    const int d = VD * (4 * g + i) + c;
+                    if (d >= a.Dh) continue;
+                    const float4_t v = {o[n][c][i] * y, o[n][c + 1][i] * y, o[n][c + 2][i] * y, o[n][c + 3][i] * y};
+                    if (slot >= 0) *reinterpret_cast<float4_t *>(part + d) = v;
+                    else *reinterpret_cast<half4_t *>(out + d) = half4_t{f2h(v[0]), f2h(v[1]), f2h(v[2]), f2h(v[3])};
                 }
+            if (slot >= 0 && g == 0) {
+                a.stats[2 * at] = m[n];
+                a.stats[2 * at + 1] = sum;
             }
         }
     }
 };
 
-// Workgroups of a CU: as many as the registers are for
+// Waves of a SIMD: as many as the registers are for
 constexpr int resident(int ND, int NR, int bytes) { return NR == 1 && ND * bytes < 4 ? 3 : 2; }
 
 template <int ND, int NR, class P>
 __global__ void __launch_bounds__(kThreads, resident(ND, NR, sizeof(P))) paged_attention_kernel(AttnArgs a)
 {
     constexpr int kRows = 16 * NR;
-    __shared__ typename Tile<ND, NR, P>::Shared sh;
-    double sum;
-    const int64_t units = uniform((int64_t)sum_of_work(a, kRows, 0, &sum));
-    const int64_t groups = min((int64_t)a.groups, units);
-    if (blockIdx.x >= groups) return;
-    int64_t x = uniform(begin_of(blockIdx.x, units, groups));
-    const int64_t until = uniform(begin_of((int64_t)blockIdx.x + 1, units, groups));
-    int b = sequence_at(a, kRows, (double)x, &sum);
-    int64_t before = uniform((int64_t)sum);
+    __shared__ Entry entries[kWaves][kEntries];
+    const int wid = uniform((int)threadIdx.x >> 6);
+    const unsigned group = blockIdx.x * kWaves + wid;
+    unsigned sum;
+    const unsigned units = uniform((int)sum_of_work(a, kRows, 0, &sum)), groups = min((unsigned)a.groups, units);
+    if (group >= groups) return;
+    const Shares shares(units, groups);
+    unsigned x = uniform((int)shares.begin(group));
+    const unsigned until = uniform((int)shares.begin(group + 1));
+    int b = uniform(sequence_at(a, kRows, x, &sum));
+    unsigned before = uniform((int)sum);
     for (; x < until; b++) {
         const Sequence s = sequence(a.pb, b, (int64_t)a.pb.W * a.pb.page, a.max_new);
         const Share w(a, kRows, s);
-        const int64_t behind = before + uniform((int64_t)w.units);
+        const unsigned behind = before + w.units;
         while (x < until && x < behind) {
-            const int64_t at = x - before;
-            const int u = uniform((int)(at / w.blocks)), first = uniform((int)(at - (int64_t)u * w.blocks)), h = uniform(u / w.tiles);
-            const int row0 = (u - h * w.tiles) * kRows, count = (int)min((int64_t)(w.blocks - first), until - x), rows = s.n * a.G;
-            const int end = uniform(s.first + min(rows - 1, row0 + kRows - 1) / a.G + 1);         // positions that some row of the tile sees
-            Tile<ND, NR, P> t{a, sh};
-            const int c0 = first * kBlock, c1 = min(end, (first + count) * kBlock);
-            t.run(b, s, h, rows, row0, c0, c1);
-            t.write(b, s, h, rows, row0, c0, c1, count == w.blocks ? -1 : 2 * (int)blockIdx.x + (first == 0));
-            x += count;
+            const unsigned at = x - before, whole = w.steps + kBegin;
+            const int u = uniform((int)(at / whole)), h = uniform(u / w.tiles), row0 = (u - h * w.tiles) * kRows, rows = s.n * a.G;
+            const int from = (int)(at - u * whole), to = (int)min((unsigned)(whole), from + (until - x));      // of the tile's units
+            const int end = uniform(s.first + min(rows - 1, row0 + kRows - 1) / a.G + 1);         // positions that some row sees
+            const int first = max(from - kBegin, 0), behind_last = to - kBegin;
+            if (behind_last > first) {
+                const int c0 = first * kStep, c1 = min(end, behind_last * kStep);
+                Tile<ND, NR, P> t{a, entries[wid]};
+                t.run(b, s, h, rows, row0, c0, c1);
+                if (t.odd) t.add_odd(b, h, max(c0, s.first + row0 / a.G + 1), c1);
+                t.write(s, h, rows, row0, first == 0 && behind_last == w.steps ? -1 : 2 * (int)group + (first == 0));
+            }
+            x += to - from;
         }
         before = behind;
     }
@@ -549,14 +626,13 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs
         if (2 * lane < a.Dh) *reinterpret_cast<half2_t *>(out) = half2_t{};
         return;
     }
-    double before;
-    const int64_t units = (int64_t)sum_of_work(a, kRows, b, &before);
+    unsigned before;
+    const unsigned units = sum_of_work(a, kRows, b, &before);
     const Share w(a, kRows, s);
     const int h = head / a.G, r = (row - s.s0) * a.G + head - h * a.G, tile = r / kRows;
-    const int64_t first = (int64_t)before + (int64_t)(h * w.tiles + tile) * w.blocks;
-    // the workgroups that have its first and last unit: the largest i with begin_of(i) <= unit
-    const int64_t groups = min((int64_t)a.groups, units);
-    const int i0 = (int)(((first + 1) * groups - 1) / units), i1 = (int)(((first + w.blocks) * groups - 1) / units);
+    const unsigned first = before + (unsigned)(h * w.tiles + tile) * (w.steps + kBegin) + kBegin;
+    const Shares shares(units, min((unsigned)a.groups, units));
+    const int i0 = (int)shares.of(first), i1 = (int)shares.of(first + w.steps - 1);
     if (i0 == i1) return;
     const int parts = i1 - i0 + 1;
     auto at = [&](int p) { return (int64_t)(p == 0 ? 2 * i0 + 1 : 2 * (i0 + p)) * kRows + r - tile * kRows; };
@@ -584,13 +660,13 @@ Plan plan(int64_t T, int64_t H, int64_t Hkv, int64_t Dh, int64_t max_new, int by
 {
     const int64_t G = H / Hkv, rows = (max_new < T ? max_new : T) * G;
     const int NR = rows <= 16 ? 1 : 2;
-    return {NR, resident(Dh <= 64 ? 1 : 2, NR, bytes) * device_cus()};
+    return {NR, resident(Dh <= 64 ? 1 : 2, NR, bytes) * kWaves * device_cus()};
 }
 
 template <int ND, int NR, class P>
 int launch(const AttnArgs &a, hipStream_t st)
 {
-    hipLaunchKernelGGL((paged_attention_kernel<ND, NR, P>), dim3((unsigned)a.groups), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((paged_attention_kernel<ND, NR, P>), dim3((unsigned)(a.groups / kWaves)), dim3(kThreads), 0, st, a);
     const int rc = launch_status("paged_attention");
     if (rc) return rc;
     const int64_t waves = (int64_t)a.pb.T * a.H;
@@ -628,7 +704,9 @@ CACTI_API int cacti_hip_paged_attention_f16(int64_t T, int64_t B, int64_t H, int
                   "paged_attention: operands must be 8-byte aligned with row pitches that are multiples of 4 and hold a row");
     CACTI_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= cacti_hip_paged_attention_workspace(T, B, H, Hkv, Dh, max_new),
                   CACTI_E_INVALID, "paged_attention: workspace too small or not 16-byte aligned");
-    CACTI_REQUIRE((T * H + kWaves - 1) / kWaves < (1 << 24), CACTI_E_NOTIMPL, "paged_attention: too many rows in one call");
+    const int64_t most = (max_new < T ? max_new : T) * (H / Hkv) / 16 + 1;         // tiles of a sequence; work is counted in 32 bits
+    CACTI_REQUIRE((T * H + kWaves - 1) / kWaves < (1 << 24) && (most < T * (H / Hkv) / 16 + B ? most * B : T * (H / Hkv) / 16 + B) * Hkv <
+                      INT32_MAX / (W * page / kStep + 1 + kBegin), CACTI_E_NOTIMPL, "paged_attention: too many rows and positions in one call");
     const Plan p = plan(T, H, Hkv, Dh, max_new, bits / 8);
     float *part = (float *)workspace;
     const AttnArgs a = {pb, (int)H, (int)Hkv, (int)(H / Hkv), (int)Dh, padded_dim((int)Dh), (int)(max_new < T ? max_new : T), p.groups,
