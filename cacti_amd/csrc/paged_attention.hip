@@ -27,8 +27,9 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = 4, kStep = 32;
 constexpr int kEntries = 64;                   // pages that a wave looks up at a time, one to a lane
-// What a tile of rows costs a share besides its steps, in steps: queries, pages and the first keys to wait for
-constexpr int kBegin = 4;
+// What a tile of rows costs a share besides its steps, in steps: queries, pages and the first keys to wait for.  (48 sequences
+// of 120 to 8192 positions, 16 rows, 2 / 4 / 8 / 16: 134 / 134 / 137 / 140 us; 24 of 100 to 6000, 32 rows 38.3 / 37.3 / 36.1 / 35.8)
+constexpr int begin_of(int tile) { return tile / 4; }
 
 struct AttnArgs {
     PagedBatch pb;
@@ -47,50 +48,35 @@ struct AttnArgs {
 // What is the same in all lanes, in scalar registers
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// A sequence's share of the work: its tiles of rows by its steps (and kBegin), by heads
+// A sequence's share of the work: its tiles of rows by its steps (and begin_of), by heads
 struct Share {
     int tiles, steps;
     unsigned units;
     __device__ __forceinline__ Share(const AttnArgs &a, int tile, const Sequence &s)
         : tiles((s.n * a.G + tile - 1) / tile), steps((s.first + s.n + kStep - 1) / kStep),
-          units(s.ok && s.n > 0 ? (unsigned)(tiles * (steps + kBegin) * a.Hkv) : 0u)
+          units(s.ok && s.n > 0 ? (unsigned)(tiles * (steps + begin_of(tile)) * a.Hkv) : 0u)
     {
     }
 };
-__device__ __forceinline__ unsigned units_of(const AttnArgs &a, int tile, int b)
+// A lane's sequence of 64 from b0 on
+__device__ __forceinline__ Sequence lane_sequence(const AttnArgs &a, int b0)
 {
-    return b < a.pb.B ? Share(a, tile, sequence(a.pb, b, (int64_t)a.pb.W * a.pb.page, a.max_new)).units : 0u;
+    const int b = b0 + (threadIdx.x & 63);
+    Sequence s = sequence(a.pb, min(b, a.pb.B - 1), (int64_t)a.pb.W * a.pb.page, a.max_new);
+    if (b >= a.pb.B) s.n = 0, s.ok = false;
+    return s;
 }
-// All of it, and what there is before sequence `until`, by a wave
-__device__ __forceinline__ unsigned sum_of_work(const AttnArgs &a, int tile, int until, unsigned *before)
+__device__ __forceinline__ Sequence of_lane(const Sequence &s, int lane)
 {
-    const int lane = threadIdx.x & 63;
-    double all = 0., some = 0.;                // (whole numbers)
-    for (int b0 = 0; b0 < a.pb.B; b0 += 64) {
-        const double u = units_of(a, tile, b0 + lane);
-        all += u;
-        some += b0 + lane < until ? u : 0.;
-    }
-    *before = (unsigned)wave_sum_f64(some);
-    return (unsigned)wave_sum_f64(all);
+    return {__builtin_amdgcn_readlane(s.s0, lane), __builtin_amdgcn_readlane(s.n, lane), __builtin_amdgcn_readlane(s.first, lane),
+            __builtin_amdgcn_readlane((int)s.ok, lane) != 0};
 }
-// The sequence in whose work unit x lies, and what there is before it
-__device__ __forceinline__ int sequence_at(const AttnArgs &a, int tile, unsigned x, unsigned *before)
-{
-    const int lane = threadIdx.x & 63;
-    double all = 0.;
-    for (int b0 = 0; b0 < a.pb.B; b0 += 64) {
-        const double u = units_of(a, tile, b0 + lane), upto = scan_f64(u) + all;
-        const uint64_t hit = __ballot(upto > (double)x);
-        if (hit) {
-            const int at = __ffsll((unsigned long long)hit) - 1;
-            *before = (unsigned)lane_f64(upto - u, at);
-            return b0 + at;
-        }
-        all = lane_f64(upto, 63);
-    }
-    return a.pb.B;
-}
+
+// A share is at least that many units: fewer steps are more parts to put together than they save (one sequence of 1540 positions,
+// 32 heads of 100, 1 / 2 / 4 / 8: 14.5 / 13.6 / 13.5 / 16.1 us)
+constexpr unsigned kLeast = 4;
+__device__ __forceinline__ unsigned groups_of(const AttnArgs &a, unsigned units) { return min((unsigned)a.groups, max(units / kLeast, 1u)); }
+
 // Equal shares of `units`: group i has those from begin(i) to begin(i + 1), the first `more` of them one more than `each`
 struct Shares {
     unsigned each, more;
@@ -140,22 +126,34 @@ typedef int i8_t __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ float4_t mfma(half8_t a, half8_t b, float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
-// The lane's part of a query: of each 64 columns those that it has of a key.  f(d): 4 of them from column d on.
+// The lane's part of a query: of each 64 columns those that it has of a key.
+template <int ND>
+struct QueryWords {
+    u2_t w[4 * ND];                            // as loaded: word i at column 64 (i / 4) + 16 g + 4 (i % 4)
+    __device__ __forceinline__ void load(const half_t *q, int Dh)          // (Dh is a multiple of 4)
+    {
+        const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int i = 0; i < 4 * ND; i++) w[i] = *reinterpret_cast<const u2_t *>(q + min(64 * (i / 4) + 16 * g + 4 * (i & 3), Dh - 4));
+    }
+    __device__ __forceinline__ u2_t at(int i, int Dh) const
+    {
+        return 64 * (i / 4) + 16 * (int)((threadIdx.x & 63) >> 4) + 4 * (i & 3) < Dh ? w[i] : u2_t{0u, 0u};
+    }
+};
 template <int ND, class P>
 struct Query;
 template <int ND>
 struct Query<ND, half_t> {
     half8_t h[2 * ND];
-    template <class F>
-    __device__ __forceinline__ float set(F f)              // returns what the products have to be multiplied by
+    __device__ __forceinline__ float set(const QueryWords<ND> &q, int Dh)  // returns what the products have to be multiplied by
     {
-        const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
         for (int c = 0; c < 2 * ND; c++) {
             Frag x;
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                const u2_t w = f(64 * (c / 2) + 16 * g + 8 * (c & 1) + 4 * j);
+                const u2_t w = q.at(2 * c + j, Dh);
                 x.u[2 * j] = w[0];
                 x.u[2 * j + 1] = w[1];
             }
@@ -178,14 +176,12 @@ struct Query<ND, half_t> {
 template <int ND>
 struct Query<ND, uint8_t> {
     int t[3][4 * ND];
-    template <class F>
-    __device__ __forceinline__ float set(F f)
+    __device__ __forceinline__ float set(const QueryWords<ND> &q, int Dh)
     {
-        const int g = (threadIdx.x & 63) >> 4;
         float x[16 * ND], mx = 0.f;
 #pragma unroll
         for (int i = 0; i < 4 * ND; i++) {
-            const half4_t w = __builtin_bit_cast(half4_t, f(64 * (i / 4) + 16 * g + 4 * (i & 3)));
+            const half4_t w = __builtin_bit_cast(half4_t, q.at(i, Dh));
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 x[4 * i + k] = h2f(w[k]);
@@ -337,10 +333,10 @@ struct VBlock<half_t, VD> {
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
 
-// What a page of a workgroup's positions is: where its rows of this head begin and what its scales make of a score
+// What the pages of a wave's positions are: where their rows of this head begin and what their scales make of a score
 struct Entry {
-    int64_t at;
-    float c, lg, iv;                           // alpha ks log2 e, log2 vs, 1 / vs
+    int64_t at[kEntries];
+    float c[kEntries], lg[kEntries], iv[kEntries];         // alpha ks log2 e, log2 vs, 1 / vs
 };
 
 // One tile of rows and a part of its positions, by a wave.  ND: pieces of 64 columns of a head
@@ -348,7 +344,7 @@ template <int ND, int NR, class P>
 struct Tile {
     static constexpr int VD = 4 * ND;          // columns of V of a lane
     const AttnArgs &a;
-    Entry *entry;                              // the wave's, in LDS
+    Entry &entry;                              // the wave's, in LDS
     Query<ND, P> q[NR];                        // the lane's row of each 16: its query, a score's factor, its last position
     float factor[NR];
     int last[NR];
@@ -367,7 +363,7 @@ struct Tile {
 #pragma unroll
         for (int t = 0; t < 2; t++) {
             const int j = min(x + 8 * (r16 >> 2) + 4 * t + (r16 & 3), end - 1), pg = page_of(j);
-            const P *row = (const P *)a.k_pages + entry[pg].at + __umul24(j - __umul24(pg, a.pb.page), a.Dp);
+            const P *row = (const P *)a.k_pages + entry.at[pg] + __umul24(j - __umul24(pg, a.pb.page), a.Dp);
 #pragma unroll
             for (int c = 0; c < ND; c++) {
                 kk[t][c].load(row + min(64 * c + 16 * g, a.Dp - 16));
@@ -381,7 +377,7 @@ struct Tile {
     {
         const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
         const int j0 = x + 8 * g, pg = page_of(min(j0, end - 1));          // one page: of 16 positions or a multiple
-        const P *row = (const P *)a.v_pages + entry[pg].at + min(VD * r16, a.Dp - VD);
+        const P *row = (const P *)a.v_pages + entry.at[pg] + min(VD * r16, a.Dp - VD);
 #pragma unroll
         for (int i = 0; i < 8; i++) vv.load(i, row + __umul24(min(j0 + i, end - 1) - __umul24(pg, a.pb.page), a.Dp));
     }
@@ -391,49 +387,79 @@ struct Tile {
     {
         const int lane = threadIdx.x & 63, r16 = lane & 15;
         odd = false;
+        if (c0 >= c1) {                        // none of these positions is seen: nothing of them
+#pragma unroll
+            for (int n = 0; n < NR; n++) {
+                m[n] = -INFINITY;
+                l[n] = 0.f;
+#pragma unroll
+                for (int i = 0; i < VD; i++) o[n][i] = float4_t{0.f, 0.f, 0.f, 0.f};
+            }
+            return;
+        }
+        const int least = uniform(s.first + row0 / a.G);       // positions up to there are seen by every row
+        int base, end;
+        float ks = 1.f, vs = 1.f;
+        // the pages from position `seg` on: their numbers, their addresses and the first keys and values, what their scales make
+        auto look_up = [&](int seg) __attribute__((always_inline)) {
+            const int p0 = uniform(seg / a.pb.page);
+            base = p0 * a.pb.page;
+            end = min(c1 - base, kEntries * a.pb.page);
+            return a.pb.table[(int64_t)b * a.pb.ldt + p0 + min(lane, page_of(end - 1))];
+        };
+        auto request = [&](int id, int x) __attribute__((always_inline)) {
+            if (id < 0 || id >= a.pb.P) {
+                report(a.pb, b);
+                id = 0;                        // its rows are unspecified, not its reads
+            }
+            const int64_t ph = (int64_t)id * a.Hkv + h;
+            if (sizeof(P) == 1) ks = a.k_scale[ph], vs = a.v_scale[ph];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");         // (the entries of before are done with)
+            __builtin_amdgcn_wave_barrier();
+            entry.at[lane] = ph * a.pb.page * a.Dp;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            load_k(x, end);
+            load_v(x, end);
+        };
+        auto scales = [&]() __attribute__((always_inline)) {
+            entry.c[lane] = ks * (a.alpha * 1.44269504088896340736f);
+            entry.lg[lane] = __builtin_amdgcn_logf(vs);
+            entry.iv[lane] = __builtin_amdgcn_rcpf(vs);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        };
+        {
+            const int id = look_up(c0);
+            QueryWords<ND> words[NR];          // requested with the pages' numbers
+#pragma unroll
+            for (int n = 0; n < NR; n++) {
+                const int r = min(row0 + 16 * n + r16, rows - 1), t = r / a.G;
+                last[n] = s.first + t;
+                words[n].load(a.q + (int64_t)(s.s0 + t) * a.ldq + (h * a.G + r - t * a.G) * a.Dh, a.Dh);
+            }
+            request(id, c0 - base);
+#pragma unroll
+            for (int n = 0; n < NR; n++) factor[n] = q[n].set(words[n], a.Dh);
+            scales();
+        }
 #pragma unroll
         for (int n = 0; n < NR; n++) {
-            const int r = min(row0 + 16 * n + r16, rows - 1), t = r / a.G;
-            last[n] = s.first + t;
-            const half_t *qr = a.q + (int64_t)(s.s0 + t) * a.ldq + (h * a.G + r - t * a.G) * a.Dh;
-            factor[n] = q[n].set([&](int d) __attribute__((always_inline)) {                      // (Dh is a multiple of 4)
-                const u2_t w = *reinterpret_cast<const u2_t *>(qr + min(d, a.Dh - 4));
-                return d < a.Dh ? w : u2_t{0u, 0u};
-            });
             m[n] = -INFINITY;
             l[n] = 0.f;
 #pragma unroll
             for (int i = 0; i < VD; i++) o[n][i] = float4_t{0.f, 0.f, 0.f, 0.f};
         }
-        const int least = uniform(s.first + row0 / a.G);       // positions up to there are seen by every row
-        for (int seg = c0; seg < c1;) {
-            const int p0 = uniform(seg / a.pb.page), base = p0 * a.pb.page, end = min(c1 - base, kEntries * a.pb.page);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");         // (the entries of before are done with)
-            __builtin_amdgcn_wave_barrier();
-            if (lane <= page_of(end - 1)) {
-                int id = a.pb.table[(int64_t)b * a.pb.ldt + p0 + lane];
-                if (id < 0 || id >= a.pb.P) {
-                    report(a.pb, b);
-                    id = 0;                    // its rows are unspecified, not its reads
-                }
-                const int64_t ph = (int64_t)id * a.Hkv + h;
-                Entry e = {ph * a.pb.page * a.Dp, a.alpha * 1.44269504088896340736f, 0.f, 1.f};
-                if (sizeof(P) == 1) {
-                    e.c *= a.k_scale[ph];
-                    e.lg = __builtin_amdgcn_logf(a.v_scale[ph]);
-                    e.iv = __builtin_amdgcn_rcpf(a.v_scale[ph]);
-                }
-                entry[lane] = e;
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            int x = seg - base;
-            load_k(x, end);
-            load_v(x, end);
+        for (int x = c0 - base;;) {
             const int clear = min(least - base, end - 1);      // up to here everything is seen by every row
             for (; x + kStep - 1 <= clear; x += kStep) step<false>(x, end, least - base, base, min(x + kStep, end - 1));
             for (; x < end; x += kStep) step<true>(x, end, least - base, base, min(x + kStep, end - 1));
-            seg = base + end;
+            const int seg = base + end;
+            if (seg >= c1) break;
+            const int id = look_up(seg);
+            x = seg - base;
+            request(id, x);
+            scales();
         }
     }
 
@@ -448,8 +474,8 @@ struct Tile {
 #pragma unroll
             for (int n = 0; n < NR; n++) sc[n][t] = q[n].times(kk[t]);
         load_k(next, end);
-        const Entry &en = entry[page_of(min(x + 8 * g, end - 1))];      // of the lane's eight keys
-        const float ec = en.c, lg = en.lg, iv = en.iv;
+        const int pg = page_of(min(x + 8 * g, end - 1));       // of the lane's eight keys
+        const float ec = entry.c[pg], lg = entry.lg[pg], iv = entry.iv[pg];
         half8_t w[NR];
 #pragma unroll
         for (int n = 0; n < NR; n++) {
@@ -571,27 +597,41 @@ template <int ND, int NR, class P>
 __global__ void __launch_bounds__(kThreads, resident(ND, NR, sizeof(P))) paged_attention_kernel(AttnArgs a)
 {
     constexpr int kRows = 16 * NR;
-    __shared__ Entry entries[kWaves][kEntries];
+    __shared__ Entry entries[kWaves];
     const int wid = uniform((int)threadIdx.x >> 6);
     const unsigned group = blockIdx.x * kWaves + wid;
-    unsigned sum;
-    const unsigned units = uniform((int)sum_of_work(a, kRows, 0, &sum)), groups = min((unsigned)a.groups, units);
+    const Sequence s64 = lane_sequence(a, 0);              // of the first 64 sequences, which mostly are all
+    const double u64 = Share(a, kRows, s64).units;         // (whole numbers)
+    double all = u64;
+    for (int b0 = 64; b0 < a.pb.B; b0 += 64) all += Share(a, kRows, lane_sequence(a, b0)).units;
+    const unsigned units = uniform((int)(unsigned)wave_sum_f64(all)), groups = groups_of(a, units);
     if (group >= groups) return;
     const Shares shares(units, groups);
     unsigned x = uniform((int)shares.begin(group));
     const unsigned until = uniform((int)shares.begin(group + 1));
-    int b = uniform(sequence_at(a, kRows, x, &sum));
-    unsigned before = uniform((int)sum);
+    // the sequence in whose work x lies, and what there is before it
+    int b = 0;
+    unsigned before = 0;
+    for (int b0 = 0; b0 < a.pb.B; b0 += 64) {
+        const double u = b0 == 0 ? u64 : Share(a, kRows, lane_sequence(a, b0)).units, upto = scan_f64(u) + (double)before;
+        const uint64_t hit = __ballot(upto > (double)x);
+        const int at = hit ? __ffsll((unsigned long long)hit) - 1 : 63;
+        before = (unsigned)uniform((int)(unsigned)lane_f64(hit ? upto - u : upto, at));
+        if (hit) {
+            b = b0 + at;
+            break;
+        }
+    }
     for (; x < until; b++) {
-        const Sequence s = sequence(a.pb, b, (int64_t)a.pb.W * a.pb.page, a.max_new);
+        const Sequence s = b < 64 ? of_lane(s64, b) : sequence(a.pb, b, (int64_t)a.pb.W * a.pb.page, a.max_new);
         const Share w(a, kRows, s);
         const unsigned behind = before + w.units;
         while (x < until && x < behind) {
-            const unsigned at = x - before, whole = w.steps + kBegin;
+            const unsigned at = x - before, whole = w.steps + begin_of(kRows);
             const int u = uniform((int)(at / whole)), h = uniform(u / w.tiles), row0 = (u - h * w.tiles) * kRows, rows = s.n * a.G;
             const int from = (int)(at - u * whole), to = (int)min((unsigned)(whole), from + (until - x));      // of the tile's units
             const int end = uniform(s.first + min(rows - 1, row0 + kRows - 1) / a.G + 1);         // positions that some row sees
-            const int first = max(from - kBegin, 0), behind_last = to - kBegin;
+            const int first = max(from - begin_of(kRows), 0), behind_last = to - begin_of(kRows);
             if (behind_last > first) {
                 const int c0 = first * kStep, c1 = min(end, behind_last * kStep);
                 Tile<ND, NR, P> t{a, entries[wid]};
@@ -605,52 +645,87 @@ __global__ void __launch_bounds__(kThreads, resident(ND, NR, sizeof(P))) paged_a
     }
 }
 
-// The parts of a row put together, by a wave per row and head with two columns per lane; zeros for rows whose sequence's numbers
-// do not fit together.
-template <int NR>
+// The parts of a row put together, two columns per lane; zeros for rows whose sequence's numbers do not fit together.  J waves to
+// a row and head: kWaves where they do not fill the device, 1 where they do.
+template <int NR, int J>
 __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs a)
 {
-    constexpr int kRows = 16 * NR;
+    constexpr int kRows = 16 * NR, kAtOnce = 8;
+    __shared__ float o[kWaves][2][64];
     const PagedBatch &pb = a.pb;
-    const int lane = threadIdx.x & 63;
-    const int64_t rh = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
-    const int row = (int)(rh / a.H), head = (int)(rh - (int64_t)row * a.H), d = min(2 * lane, a.Dh - 2);
+    const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), wid = J == 1 ? 0 : wave;
+    const int rh = J == 1 ? blockIdx.x * kWaves + wave : blockIdx.x, row = rh / a.H, head = rh - row * a.H;
     if (row >= pb.T) return;
-    const int b = count_below(pb.B, row, [&](int i) { return pb.starts[i]; });
-    if (b >= pb.B) return;
-    const Sequence s = sequence(pb, b, (int64_t)pb.W * pb.page, a.max_new);
-    if (row < s.s0 || row - s.s0 >= s.n) return;
+    const int d = min(2 * lane, a.Dh - 2);
+    // all work, that of the sequences before the row's, and the row's sequence
+    double all = 0., some = 0.;
+    Sequence s = {0, 0, 0, false};
+    int b = -1;
+    for (int b0 = 0; b0 < pb.B; b0 += 64) {
+        const Sequence q = lane_sequence(a, b0);
+        const double u = Share(a, kRows, q).units;
+        const uint64_t hit = __ballot(b0 + lane < pb.B && row >= q.s0 && row - q.s0 < q.n);
+        all += u;
+        some += b < 0 && (!hit || lane < __ffsll((unsigned long long)hit) - 1) ? u : 0.;
+        if (hit && b < 0) {
+            const int at = __ffsll((unsigned long long)hit) - 1;
+            b = b0 + at;
+            s = of_lane(q, at);
+        }
+    }
+    if (b < 0) return;
     half_t *out = a.out + row * a.ldo + head * a.Dh + d;
     if (!s.ok) {
         if (lane == 0) report(pb, b);
-        if (2 * lane < a.Dh) *reinterpret_cast<half2_t *>(out) = half2_t{};
+        if (wid == 0 && 2 * lane < a.Dh) *reinterpret_cast<half2_t *>(out) = half2_t{};
         return;
     }
-    unsigned before;
-    const unsigned units = sum_of_work(a, kRows, b, &before);
+    const unsigned units = uniform((int)(unsigned)wave_sum_f64(all)), before = uniform((int)(unsigned)wave_sum_f64(some));
     const Share w(a, kRows, s);
     const int h = head / a.G, r = (row - s.s0) * a.G + head - h * a.G, tile = r / kRows;
-    const unsigned first = before + (unsigned)(h * w.tiles + tile) * (w.steps + kBegin) + kBegin;
-    const Shares shares(units, min((unsigned)a.groups, units));
-    const int i0 = (int)shares.of(first), i1 = (int)shares.of(first + w.steps - 1);
+    const unsigned first = before + (unsigned)(h * w.tiles + tile) * (w.steps + begin_of(kRows)) + begin_of(kRows);
+    const Shares shares(units, groups_of(a, units));
+    const int i0 = uniform((int)shares.of(first)), i1 = uniform((int)shares.of(first + w.steps - 1));
     if (i0 == i1) return;
     const int parts = i1 - i0 + 1;
     auto at = [&](int p) { return (int64_t)(p == 0 ? 2 * i0 + 1 : 2 * (i0 + p)) * kRows + r - tile * kRows; };
-    float mx = -INFINITY;
+    float mx = -INFINITY, sum = 0.f, o0 = 0.f, o1 = 0.f;
     for (int p = lane; p < parts; p += 64) mx = fmaxf(mx, a.stats[2 * at(p)]);
     const float origin = finite_max(wave_max(mx));
-    float sum = 0.f, o0 = 0.f, o1 = 0.f;
-#pragma unroll 4
-    for (int p = 0; p < parts; p++) {
-        const int64_t i = at(p);
-        const float f = exp2_of(a.stats[2 * i] - origin);
-        const float2 v = *reinterpret_cast<const float2 *>(a.part + i * a.Dh + d);
-        sum += f * a.stats[2 * i + 1];
-        o0 += f * v.x;
-        o1 += f * v.y;
+    for (int p0 = 0; p0 < parts; p0 += 64) {
+        const int p = min(p0 + lane, parts - 1);
+        const float f = p0 + lane < parts ? exp2_of(a.stats[2 * at(p)] - origin) : 0.f;
+        sum += f * a.stats[2 * at(p) + 1];
+        for (int k0 = wid; k0 < min(64, parts - p0); k0 += J * kAtOnce) {
+            float2 v[kAtOnce];
+#pragma unroll
+            for (int k = 0; k < kAtOnce; k++)
+                v[k] = *reinterpret_cast<const float2 *>(a.part + at(min(p0 + k0 + k * J, parts - 1)) * a.Dh + d);
+#pragma unroll
+            for (int k = 0; k < kAtOnce; k++) {
+                const int from = k0 + k * J;
+                if (from >= min(64, parts - p0)) break;
+                const float fk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), from));
+                o0 += fk * v[k].x;
+                o1 += fk * v[k].y;
+            }
+        }
     }
+    sum = wave_sum(sum);
+    if (J > 1) {
+        o[wid][0][lane] = o0;
+        o[wid][1][lane] = o1;
+        __syncthreads();
+        if (wid > 0) return;
+#pragma unroll
+        for (int w4 = 1; w4 < J; w4++) {
+            o0 += o[w4][0][lane];
+            o1 += o[w4][1][lane];
+        }
+    }
+    if (2 * lane >= a.Dh) return;
     const float y = sum == 0.f ? 0.f : 1.f / sum;
-    if (2 * lane < a.Dh) *reinterpret_cast<half2_t *>(out) = half2_t{f2h(o0 * y), f2h(o1 * y)};
+    *reinterpret_cast<half2_t *>(out) = half2_t{f2h(o0 * y), f2h(o1 * y)};
 }
 
 struct Plan {
@@ -669,8 +744,9 @@ int launch(const AttnArgs &a, hipStream_t st)
     hipLaunchKernelGGL((paged_attention_kernel<ND, NR, P>), dim3((unsigned)(a.groups / kWaves)), dim3(kThreads), 0, st, a);
     const int rc = launch_status("paged_attention");
     if (rc) return rc;
-    const int64_t waves = (int64_t)a.pb.T * a.H;
-    hipLaunchKernelGGL(paged_attention_join_kernel<NR>, dim3((unsigned)((waves + kWaves - 1) / kWaves)), dim3(kThreads), 0, st, a);
+    const int64_t rh = (int64_t)a.pb.T * a.H;
+    if (rh < 4 * device_cus()) hipLaunchKernelGGL((paged_attention_join_kernel<NR, kWaves>), dim3((unsigned)rh), dim3(kThreads), 0, st, a);
+    else hipLaunchKernelGGL((paged_attention_join_kernel<NR, 1>), dim3((unsigned)((rh + kWaves - 1) / kWaves)), dim3(kThreads), 0, st, a);
     return launch_status("paged_attention (parts)");
 }
 template <class P>
@@ -705,8 +781,8 @@ CACTI_API int cacti_hip_paged_attention_f16(int64_t T, int64_t B, int64_t H, int
     CACTI_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= cacti_hip_paged_attention_workspace(T, B, H, Hkv, Dh, max_new),
                   CACTI_E_INVALID, "paged_attention: workspace too small or not 16-byte aligned");
     const int64_t most = (max_new < T ? max_new : T) * (H / Hkv) / 16 + 1;         // tiles of a sequence; work is counted in 32 bits
-    CACTI_REQUIRE((T * H + kWaves - 1) / kWaves < (1 << 24) && (most < T * (H / Hkv) / 16 + B ? most * B : T * (H / Hkv) / 16 + B) * Hkv <
-                      INT32_MAX / (W * page / kStep + 1 + kBegin), CACTI_E_NOTIMPL, "paged_attention: too many rows and positions in one call");
+    CACTI_REQUIRE(T * H < (1 << 24) && (most < T * (H / Hkv) / 16 + B ? most * B : T * (H / Hkv) / 16 + B) * Hkv <
+                      INT32_MAX / (W * page / kStep + 1 + begin_of(32)), CACTI_E_NOTIMPL, "paged_attention: too many rows and positions in one call");
     const Plan p = plan(T, H, Hkv, Dh, max_new, bits / 8);
     float *part = (float *)workspace;
     const AttnArgs a = {pb, (int)H, (int)Hkv, (int)(H / Hkv), (int)Dh, padded_dim((int)Dh), (int)(max_new < T ? max_new : T), p.groups,
