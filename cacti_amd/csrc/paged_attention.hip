@@ -43,10 +43,21 @@ struct AttnArgs {
     half_t *out;
     int64_t ldo;
     float *part, *stats;                       // [2 groups][16 NR][Dh], [2 groups][16 NR][2]; a group: a wave
+    int few;                                   // sequences with more rows than that (by the query heads of a key head) are prompts
+    int big_groups;                            // ... for which a group is a workgroup; 0: there are none
+    float *big_part, *big_stats;               // [2 big_groups][kPrompt][Dh], ...[2]
 };
 
 // What is the same in all lanes, in scalar registers
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+// The lane's number, of which the compiler does not know that it is the same every time: what is formed from it for one tile of
+// rows (some hundred addresses) is formed there and not held in registers, or out of them, over all tiles of a share.
+__device__ __forceinline__ int lane_here()
+{
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
 
 // A sequence's share of the work: its tiles of rows by its steps (and begin_of), by heads
 struct Share {
@@ -54,7 +65,7 @@ struct Share {
     unsigned units;
     __device__ __forceinline__ Share(const AttnArgs &a, int tile, const Sequence &s)
         : tiles((s.n * a.G + tile - 1) / tile), steps((s.first + s.n + kStep - 1) / kStep),
-          units(s.ok && s.n > 0 ? (unsigned)(tiles * (steps + begin_of(tile)) * a.Hkv) : 0u)
+          units(s.ok && s.n > 0 && s.n * a.G <= a.few ? (unsigned)(tiles * (steps + begin_of(tile)) * a.Hkv) : 0u)
     {
     }
 };
@@ -76,6 +87,10 @@ __device__ __forceinline__ Sequence of_lane(const Sequence &s, int lane)
 // 32 heads of 100, 1 / 2 / 4 / 8: 14.5 / 13.6 / 13.5 / 16.1 us)
 constexpr unsigned kLeast = 4;
 __device__ __forceinline__ unsigned groups_of(const AttnArgs &a, unsigned units) { return min((unsigned)a.groups, max(units / kLeast, 1u)); }
+
+constexpr unsigned kBigLeast = 4;              // the same of steps of 64 positions
+// Workgroups go round the 8 XCDs: those of one XCD get neighbouring numbers (of n, a multiple of 8)
+__device__ __forceinline__ unsigned xcd_order(unsigned i, unsigned n) { return (i & 7) * (n / 8) + i / 8; }
 
 // Equal shares of `units`: group i has those from begin(i) to begin(i + 1), the first `more` of them one more than `each`
 struct Shares {
@@ -385,7 +400,7 @@ struct Tile {
     // positions c0 .. c1 - 1 of rows row0 .. of sequence s
     __device__ __forceinline__ void run(int b, const Sequence &s, int h, int rows, int row0, int c0, int c1)
     {
-        const int lane = threadIdx.x & 63, r16 = lane & 15;
+        const int lane = lane_here(), r16 = lane & 15;
         odd = false;
         if (c0 >= c1) {                        // none of these positions is seen: nothing of them
 #pragma unroll
@@ -562,7 +577,7 @@ struct Tile {
     // A lane has columns VD (4 g + i) + c of its row in o[.][c][i].  slot < 0: to the output
     __device__ __forceinline__ void write(const Sequence &s, int h, int rows, int row0, int slot)
     {
-        const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
+        const int lane = lane_here(), r16 = lane & 15, g = lane >> 4;
 #pragma unroll
         for (int n = 0; n < NR; n++) {
             const float sum = with32(with16(l[n], OpSum()), OpSum());
@@ -594,12 +609,9 @@ struct Tile {
 constexpr int resident(int ND, int NR, int bytes) { return NR == 1 && ND * bytes < 4 ? 3 : 2; }
 
 template <int ND, int NR, class P>
-__global__ void __launch_bounds__(kThreads, resident(ND, NR, sizeof(P))) paged_attention_kernel(AttnArgs a)
+__device__ __forceinline__ void wave_share(const AttnArgs &a, unsigned group, Entry &entry)
 {
     constexpr int kRows = 16 * NR;
-    __shared__ Entry entries[kWaves];
-    const int wid = uniform((int)threadIdx.x >> 6);
-    const unsigned group = blockIdx.x * kWaves + wid;
     const Sequence s64 = lane_sequence(a, 0);              // of the first 64 sequences, which mostly are all
     const double u64 = Share(a, kRows, s64).units;         // (whole numbers)
     double all = u64;
@@ -634,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, resident(ND, NR, sizeof(P))) paged_a
             const int first = max(from - begin_of(kRows), 0), behind_last = to - begin_of(kRows);
             if (behind_last > first) {
                 const int c0 = first * kStep, c1 = min(end, behind_last * kStep);
-                Tile<ND, NR, P> t{a, entries[wid]};
+                Tile<ND, NR, P> t{a, entry};
                 t.run(b, s, h, rows, row0, c0, c1);
                 if (t.odd) t.add_odd(b, h, max(c0, s.first + row0 / a.G + 1), c1);
                 t.write(s, h, rows, row0, first == 0 && behind_last == w.steps ? -1 : 2 * (int)group + (first == 0));
@@ -643,6 +655,383 @@ __global__ void __launch_bounds__(kThreads, resident(ND, NR, sizeof(P))) paged_a
         }
         before = behind;
     }
+}
+
+template <int ND, int NR, class P>
+__global__ void __launch_bounds__(kThreads, resident(ND, NR, sizeof(P))) paged_attention_kernel(AttnArgs a)
+{
+    __shared__ Entry entries[kWaves];
+    const int wid = uniform((int)threadIdx.x >> 6);
+    wave_share<ND, NR, P>(a, blockIdx.x * kWaves + wid, entries[wid]);
+}
+
+// ---------------------------------------------------------------- prompts
+// Sequences with many new rows: 128 of them (tokens by the query heads of a key head) to a workgroup, 32 to a wave, 64 positions
+// at a time, whose keys and values go through LDS as f16: converted and V turned once for all four waves, while the products of
+// the 64 before them run, in two buffers with one barrier a step.  16-byte pieces of LDS rows are swapped by f(row), which spreads
+// the sixteen rows of an operand, and the rows that a wave writes, evenly over the banks.  What bounds it: the matrix pipe and
+// LDS about evenly (32 KB of operands to a wave for 1024 cycles of products), then the softmax between them.
+//
+// Shares are cut as above, a workgroup to a share and by steps of 64.  A tile's steps grow by those of its own 128 rows: counted
+// by a line that is never below them, so that what lies before a tile is a formula; steps behind a tile's last position are
+// nothing.  Workgroups of an XCD have neighbouring shares: the tiles of a head read its keys and values from one L2.
+constexpr int kPrompt = 128, kBig = 64;
+constexpr int kBigBegin = 2;                   // as begin_of, in steps
+
+__device__ __forceinline__ int swap_of(int row) { return ((row >> 2) ^ row) & 7; }
+
+struct BigShare {
+    int tiles, base, slope, run;               // steps of tile t: base + slope (t + 1), or, slope 0, base + t / run + 1
+    __device__ __forceinline__ BigShare(const AttnArgs &a, const Sequence &s)
+    {
+        const int tokens = (kPrompt + a.G - 1) / a.G;
+        tiles = s.ok && s.n * a.G > a.few ? (s.n * a.G + kPrompt - 1) / kPrompt : 0;
+        base = (s.first + kBig - 1) / kBig + kBigBegin;
+        slope = tokens >= kBig ? (tokens + kBig - 1) / kBig : 0;
+        run = slope ? 1 : kBig / tokens;
+    }
+    __device__ __forceinline__ unsigned before(int t) const      // tile t
+    {
+        if (slope) return (unsigned)(t * base + slope * (t * (t + 1) / 2));
+        const int q = t / run, r = t - q * run;
+        return (unsigned)(t * base + run * (q * (q - 1) / 2) + r * q + t);
+    }
+    __device__ __forceinline__ unsigned units(const AttnArgs &a) const { return before(tiles) * (unsigned)a.Hkv; }
+};
+
+template <int ND, class P>
+struct Prompt {
+    static constexpr int NR = 2, NS = 2 * ND;  // of a wave: rows by 16; matrix instructions along the columns of a key
+    static constexpr int kPieces = kBig * 64 * ND * (int)sizeof(P) / 16 / kThreads;          // 16-byte pieces of keys of a lane
+    struct Shared {
+        half_t k[2][kBig][64 * ND], v[2][64 * ND][kBig];
+        Entry entry;
+        int odd;
+    };
+    const AttnArgs &a;
+    Shared &sh;
+    half8_t q[NR][NS];
+    int last[NR];
+    float m[NR], l[NR];
+    float4_t o[NR][4 * ND];
+    u4_t kr[kPieces];                          // the next 64 positions, as they come
+    VBlock<P, 4> vr;
+
+    __device__ __forceinline__ int page_of(int x) const { return (int)(__umul24((unsigned)x, a.page_magic) >> 22); }
+    __device__ __forceinline__ bool turns() const { return ND == 2 || threadIdx.x < 128; }   // has four columns of eight values
+
+    __device__ __forceinline__ void load(int x, int end)
+    {
+        constexpr int per = 64 * ND * (int)sizeof(P) / 16;                 // pieces of a key
+        const int tid = 64 * uniform((int)threadIdx.x >> 6) + lane_here();
+#pragma unroll
+        for (int i = 0; i < kPieces; i++) {
+            const int piece = tid + i * kThreads, j = min(x + piece / per, end - 1), pg = page_of(j);
+            const P *row = (const P *)a.k_pages + sh.entry.at[pg] + __umul24(j - __umul24(pg, a.pb.page), a.Dp);
+            kr[i] = *reinterpret_cast<const u4_t *>(row + min(piece % per * (16 / (int)sizeof(P)), a.Dp - 16 / (int)sizeof(P)));
+        }
+        if (!turns()) return;
+        const int j0 = x + 8 * (tid / (16 * ND)), pg = page_of(min(j0, end - 1));
+        const P *row = (const P *)a.v_pages + sh.entry.at[pg] + min(4 * (tid % (16 * ND)), a.Dp - 4);
+#pragma unroll
+        for (int i = 0; i < 8; i++) vr.load(i, row + __umul24(min(j0 + i, end - 1) - __umul24(pg, a.pb.page), a.Dp));
+    }
+    // ... into buffer `to`; least: positions up to there are seen by every row of the tile
+    __device__ __forceinline__ void store(int to, int x, int end, int least)
+    {
+        constexpr int per = 64 * ND * (int)sizeof(P) / 16;
+        const int tid = 64 * uniform((int)threadIdx.x >> 6) + lane_here();
+#pragma unroll
+        for (int i = 0; i < kPieces; i++) {
+            const int piece = tid + i * kThreads, j = piece / per, d = piece % per * (16 / (int)sizeof(P));
+            const bool in = d < a.Dp;          // (beside the columns the queries are zeros, and so must the keys be)
+#pragma unroll
+            for (int k = 0; k < 16 / (int)sizeof(P) / 8; k++) {
+                Frag f;
+#pragma unroll
+                for (int w = 0; w < 4; w++) f.u[w] = !in ? 0u : sizeof(P) == 2 ? kr[i][w] : cvt8(kr[i][2 * k + w / 2], w & 1);
+                *reinterpret_cast<half8_t *>(&sh.k[to][j][((d / 8 + k) ^ swap_of(j)) * 8]) = f.h;
+            }
+        }
+        if (!turns()) return;
+        const int kg = tid / (16 * ND), d = 4 * (tid % (16 * ND));
+        if (x + kBig - 1 > min(least, end - 1)) {
+            bool any = false;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int j = x + 8 * kg + i;
+                if (j >= end) vr.zero(i);
+                else if (j > least) any = vr.strip(i) || any;
+            }
+            if (any) sh.odd = 1;
+        }
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            half8_t v0, v1;
+            vr.columns(c, &v0, &v1);
+            *reinterpret_cast<half8_t *>(&sh.v[to][d + 2 * c][(kg ^ swap_of(d + 2 * c)) * 8]) = v0;
+            *reinterpret_cast<half8_t *>(&sh.v[to][d + 2 * c + 1][(kg ^ swap_of(d + 2 * c + 1)) * 8]) = v1;
+        }
+    }
+
+    // Where a lane reads its operands, in halves from the start of a buffer.  A key's row is j = 32 b + 8 (r16 / 4) + 4 t + r16 % 4,
+    // so swap_of(j) = 2 (r16 / 4) ^ r16 % 4 ^ 5 t; a row of V is d = 16 c + r16, swap_of(d) = r16 / 4 ^ r16 & 7 ^ 4 (c & 1): what b, c
+    // and t make of a piece's place but for these swaps is a constant of the instruction.
+    struct Places {
+        int k[2][2], v[2];                     // [t][c & 1], [b ^ c & 1]
+    };
+    __device__ __forceinline__ Places places() const
+    {
+        const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4, a4 = r16 >> 2, b4 = r16 & 3;
+        Places p;
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) p.k[t][c] = (8 * a4 + 4 * t + b4) * 64 * ND + ((4 * c + g) ^ (2 * a4) ^ b4 ^ (5 * t)) * 8;
+#pragma unroll
+        for (int x = 0; x < 2; x++) p.v[x] = r16 * kBig + ((4 * x + g) ^ ((a4 ^ r16) & 7)) * 8;
+        return p;
+    }
+
+    // 32 positions, those from x on, block b of the buffer (the scores of all 64 at once are more registers than there are)
+    template <bool EDGE>
+    __device__ __forceinline__ void step(const Places &at, int from, int b, int x, int end, int base)
+    {
+        const int lane = threadIdx.x & 63, g = lane >> 4;
+        float4_t sc[NR][2];
+        const half_t *kb = &sh.k[from][0][0] + 32 * b * 64 * ND, *vb = &sh.v[from][0][0];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+#pragma unroll
+            for (int n = 0; n < NR; n++) sc[n][t] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < NS; c++) {
+                const half8_t kf = *reinterpret_cast<const half8_t *>(kb + at.k[t][c & 1] + (c >> 1) * 64);
+#pragma unroll
+                for (int n = 0; n < NR; n++) sc[n][t] = mfma(kf, q[n][c], sc[n][t]);
+            }
+        }
+        const int pg = page_of(min(x + 8 * g, end - 1));
+        const float ec = sh.entry.c[pg], lg = sh.entry.lg[pg], iv = sh.entry.iv[pg];
+        Frag p[NR];
+#pragma unroll
+        for (int n = 0; n < NR; n++) {
+            float t[8], mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                t[i] = __builtin_fmaf(sc[n][i / 4][i & 3], ec, lg);
+                if (EDGE && x + 8 * g + i > min(last[n] - base, end - 1)) t[i] = -INFINITY;
+                mx = fmaxf(mx, t[i]);
+            }
+            mx = with32(with16(mx, OpMax()), OpMax());
+            const float mn = fmaxf(m[n], mx), origin = finite_max(mn);
+            if (__ballot(mn > m[n])) {
+                const float f = exp2_of(m[n] - origin);
+                m[n] = mn;
+                l[n] *= f;
+#pragma unroll
+                for (int i = 0; i < 4 * ND; i++) o[n][i] *= f;
+            }
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                t[i] = exp2_of(t[i] - origin);
+                sum += t[i];
+            }
+            l[n] = __builtin_fmaf(sum, iv, l[n]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const half2_t pair = {f2h(t[2 * i]), f2h(t[2 * i + 1])};
+                p[n].u[i] = __builtin_bit_cast(unsigned, pair);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 4 * ND; c++) {
+            const half8_t vf = *reinterpret_cast<const half8_t *>(vb + at.v[b ^ (c & 1)] + 16 * c * kBig);
+#pragma unroll
+            for (int n = 0; n < NR; n++) o[n][c] = mfma(vf, p[n].h, o[n][c]);
+        }
+    }
+
+    // positions c0 .. c1 - 1 (some) of rows row0 .. of sequence s
+    __device__ __forceinline__ void run(int b, const Sequence &s, int h, int rows, int row0, int c0, int c1)
+    {
+        const int wid = uniform((int)threadIdx.x >> 6), lane = lane_here(), tid = 64 * wid + lane, r16 = lane & 15, g = lane >> 4;
+        const int mine = row0 + 16 * NR * wid;                 // the wave's first row
+#pragma unroll
+        for (int n = 0; n < NR; n++) {
+            const int r = min(mine + 16 * n + r16, rows - 1), t = r / a.G;
+            last[n] = s.first + t;
+            const half_t *qr = a.q + (int64_t)(s.s0 + t) * a.ldq + (h * a.G + r - t * a.G) * a.Dh;
+#pragma unroll
+            for (int c = 0; c < NS; c++) {
+                Frag f;
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int d = 32 * c + 8 * g + 4 * j;
+                    const u2_t w = *reinterpret_cast<const u2_t *>(qr + min(d, a.Dh - 4));
+                    f.u[2 * j] = d < a.Dh ? w[0] : 0u;
+                    f.u[2 * j + 1] = d < a.Dh ? w[1] : 0u;
+                }
+                q[n][c] = f.h;
+            }
+            m[n] = -INFINITY;
+            l[n] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4 * ND; i++) o[n][i] = float4_t{0.f, 0.f, 0.f, 0.f};
+        }
+        const int least = uniform(s.first + row0 / a.G);                               // seen by every row of the tile
+        const int wave_least = uniform(s.first + min(mine, rows - 1) / a.G), wave_last = uniform(mine < rows ? s.first + (min(mine + 16 * NR, rows) - 1) / a.G : -1);
+        const Places at = places();
+        for (int seg = c0; seg < c1;) {
+            const int p0 = uniform(seg / a.pb.page), base = p0 * a.pb.page, end = min(c1 - base, kEntries * a.pb.page);
+            __syncthreads();                   // (entries and buffers of before are done with)
+            if (tid < 64) {
+                int id = a.pb.table[(int64_t)b * a.pb.ldt + p0 + min(lane, page_of(end - 1))];
+                if (id < 0 || id >= a.pb.P) {
+                    report(a.pb, b);
+                    id = 0;                    // its rows are unspecified, not its reads
+                }
+                const int64_t ph = (int64_t)id * a.Hkv + h;
+                float ks = 1.f, vs = 1.f;
+                if (sizeof(P) == 1) ks = a.k_scale[ph], vs = a.v_scale[ph];
+                sh.entry.at[lane] = ph * a.pb.page * a.Dp;
+                sh.entry.c[lane] = ks * (a.alpha * 1.44269504088896340736f);
+                sh.entry.lg[lane] = __builtin_amdgcn_logf(vs);
+                sh.entry.iv[lane] = __builtin_amdgcn_rcpf(vs);
+                if (seg == c0 && lane == 0) sh.odd = 0;
+            }
+            __syncthreads();
+            int x = seg - base, buffer = 0;
+            load(x, end);
+            store(0, x, end, least - base);
+            __syncthreads();
+            for (; x < end; x += kBig) {
+                const bool more = x + kBig < end;
+                load(more ? x + kBig : x, end);
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    const int x32 = x + 32 * half;
+                    if (x32 > min(wave_last - base, end - 1)) continue;
+                    if (x32 + 31 > min(wave_least - base, end - 1)) step<true>(at, buffer, half, x32, end, base);
+                    else step<false>(at, buffer, half, x32, end, base);
+                }
+                buffer ^= 1;
+                if (more) store(buffer, x + kBig, end, least - base);
+                __syncthreads();
+            }
+            seg = base + end;
+        }
+    }
+
+    __device__ __forceinline__ void write(int b, const Sequence &s, int h, int rows, int row0, int c0, int c1, int slot)
+    {
+        const int lane = lane_here(), wid = uniform((int)threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4, mine = row0 + 16 * NR * wid;
+        if (c0 < c1 && sh.odd) {               // NaNs and infinities of V, each to the rows that see it
+#pragma unroll 1
+            for (int j = max(c0, s.first + row0 / a.G + 1); j < c1; j++) {
+                const int id = a.pb.table[(int64_t)b * a.pb.ldt + j / a.pb.page];
+                const P *v = (const P *)a.v_pages + (((int64_t)(id < 0 || id >= a.pb.P ? 0 : id) * a.Hkv + h) * a.pb.page + j % a.pb.page) * a.Dp;
+#pragma unroll
+                for (int c = 0; c < 4 * ND; c++) {
+                    VBlock<P, 4> x;
+                    x.load(0, v + min(16 * c + 4 * g, a.Dp - 4));
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+#pragma unroll
+                        for (int n = 0; n < NR; n++)
+                            if (!(fabsf(x.value(i)) < INFINITY) && j <= last[n]) o[n][c][i] += x.value(i);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NR; n++) {
+            const float sum = with32(with16(l[n], OpSum()), OpSum());
+            const int r = mine + 16 * n + r16, t = r / a.G;
+            if (r >= rows) continue;
+            const float y = slot >= 0 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+            const int64_t at = (int64_t)slot * kPrompt + r - row0;
+            half_t *out = a.out + (int64_t)(s.s0 + t) * a.ldo + (h * a.G + r - t * a.G) * a.Dh;
+            float *part = a.big_part + at * a.Dh;
+#pragma unroll
+            for (int c = 0; c < 4 * ND; c++) {
+                const int d = 16 * c + 4 * g;
+                if (d >= a.Dh) continue;
+                const float4_t v = o[n][c] * y;
+                if (slot >= 0) *reinterpret_cast<float4_t *>(part + d) = v;
+                else *reinterpret_cast<half4_t *>(out + d) = half4_t{f2h(v[0]), f2h(v[1]), f2h(v[2]), f2h(v[3])};
+            }
+            if (slot >= 0 && g == 0) {
+                a.big_stats[2 * at] = m[n];
+                a.big_stats[2 * at + 1] = sum;
+            }
+        }
+    }
+};
+
+// The prompts' share of a workgroup, then the other sequences' shares of its waves
+template <int ND, class P>
+__global__ void __launch_bounds__(kThreads, 2) paged_prompt_kernel(AttnArgs a)
+{
+    __shared__ union {
+        typename Prompt<ND, P>::Shared big;
+        Entry entries[kWaves];
+    } sh;
+    const int wid = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const Sequence s64 = lane_sequence(a, 0);
+    const double u64 = BigShare(a, s64).units(a);
+    double all = u64;
+    for (int b0 = 64; b0 < a.pb.B; b0 += 64) all += BigShare(a, lane_sequence(a, b0)).units(a);
+    const unsigned units = uniform((int)(unsigned)wave_sum_f64(all)), groups = min((unsigned)a.big_groups, max(units / kBigLeast, 1u));
+    const unsigned group = xcd_order(blockIdx.x, a.big_groups);
+    if (units > 0 && group < groups) {
+        const Shares shares(units, groups);
+        unsigned x = uniform((int)shares.begin(group));
+        const unsigned until = uniform((int)shares.begin(group + 1));
+        int b = 0;
+        unsigned before = 0;
+        for (int b0 = 0; b0 < a.pb.B; b0 += 64) {
+            const double u = b0 == 0 ? u64 : BigShare(a, lane_sequence(a, b0)).units(a), upto = scan_f64(u) + (double)before;
+            const uint64_t hit = __ballot(upto > (double)x);
+            const int at = hit ? __ffsll((unsigned long long)hit) - 1 : 63;
+            before = (unsigned)uniform((int)(unsigned)lane_f64(hit ? upto - u : upto, at));
+            if (hit) {
+                b = b0 + at;
+                break;
+            }
+        }
+        for (; x < until; b++) {
+            const Sequence s = b < 64 ? of_lane(s64, b) : sequence(a.pb, b, (int64_t)a.pb.W * a.pb.page, a.max_new);
+            const BigShare w(a, s);
+            const unsigned head = w.before(w.tiles), behind = before + w.units(a);
+            while (x < until && x < behind) {
+                const int h = uniform((int)((x - before) / head)), rows = s.n * a.G;
+                const unsigned in = x - before - h * head;
+                int tile = 0;                  // that unit `in` of the head lies in
+                for (int t0 = 0; t0 < w.tiles; t0 += 64) {
+                    const int n = __popcll(__ballot(t0 + lane < w.tiles && w.before(t0 + lane + 1) <= in));
+                    tile += n;
+                    if (n < 64) break;
+                }
+                tile = uniform(tile);
+                const unsigned start = uniform((int)w.before(tile)), whole = uniform((int)w.before(tile + 1)) - start;
+                const int from = (int)(in - start), to = (int)min(whole, from + (until - x)), row0 = tile * kPrompt;
+                const int end = uniform(s.first + min(rows - 1, row0 + kPrompt - 1) / a.G + 1);
+                const int first = max(from - kBigBegin, 0), behind_last = to - kBigBegin;
+                if (behind_last > first) {
+                    const int c0 = first * kBig, c1 = min(end, behind_last * kBig);
+                    Prompt<ND, P> t{a, sh.big};
+                    t.run(b, s, h, rows, row0, c0, c1);
+                    t.write(b, s, h, rows, row0, c0, c1, first == 0 && behind_last == (int)whole - kBigBegin ? -1 : 2 * (int)group + (first == 0));
+                }
+                x += to - from;
+            }
+            before = behind;
+        }
+        __syncthreads();
+    }
+    wave_share<ND, 2, P>(a, blockIdx.x * kWaves + wid, sh.entries[wid]);
 }
 
 // The parts of a row put together, two columns per lane; zeros for rows whose sequence's numbers do not fit together.  J waves to
@@ -658,7 +1047,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs
     if (row >= pb.T) return;
     const int d = min(2 * lane, a.Dh - 2);
     // all work, that of the sequences before the row's, and the row's sequence
-    double all = 0., some = 0.;
+    double all = 0., some = 0., big_all = 0., big_some = 0.;
     Sequence s = {0, 0, 0, false};
     int b = -1;
     for (int b0 = 0; b0 < pb.B; b0 += 64) {
@@ -666,7 +1055,13 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs
         const double u = Share(a, kRows, q).units;
         const uint64_t hit = __ballot(b0 + lane < pb.B && row >= q.s0 && row - q.s0 < q.n);
         all += u;
-        some += b < 0 && (!hit || lane < __ffsll((unsigned long long)hit) - 1) ? u : 0.;
+        const bool earlier = b < 0 && (!hit || lane < __ffsll((unsigned long long)hit) - 1);
+        some += earlier ? u : 0.;
+        if (a.big_groups) {
+            const double v = BigShare(a, q).units(a);
+            big_all += v;
+            big_some += earlier ? v : 0.;
+        }
         if (hit && b < 0) {
             const int at = __ffsll((unsigned long long)hit) - 1;
             b = b0 + at;
@@ -680,27 +1075,40 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs
         if (wid == 0 && 2 * lane < a.Dh) *reinterpret_cast<half2_t *>(out) = half2_t{};
         return;
     }
-    const unsigned units = uniform((int)(unsigned)wave_sum_f64(all)), before = uniform((int)(unsigned)wave_sum_f64(some));
-    const Share w(a, kRows, s);
-    const int h = head / a.G, r = (row - s.s0) * a.G + head - h * a.G, tile = r / kRows;
-    const unsigned first = before + (unsigned)(h * w.tiles + tile) * (w.steps + begin_of(kRows)) + begin_of(kRows);
-    const Shares shares(units, groups_of(a, units));
-    const int i0 = uniform((int)shares.of(first)), i1 = uniform((int)shares.of(first + w.steps - 1));
+    const bool big = s.n * a.G > a.few;
+    const unsigned units = uniform((int)(unsigned)wave_sum_f64(big ? big_all : all));
+    unsigned first = uniform((int)(unsigned)wave_sum_f64(big ? big_some : some)), steps, groups;       // the tile's first step, its steps
+    const int h = head / a.G, r = (row - s.s0) * a.G + head - h * a.G;
+    if (big) {
+        const BigShare w(a, s);
+        const int tile = r / kPrompt;
+        first += h * w.before(w.tiles) + w.before(tile) + kBigBegin;
+        steps = w.before(tile + 1) - w.before(tile) - kBigBegin;
+        groups = min((unsigned)a.big_groups, max(units / kBigLeast, 1u));
+    } else {
+        const Share w(a, kRows, s);
+        first += (unsigned)(h * w.tiles + r / kRows) * (w.steps + begin_of(kRows)) + begin_of(kRows);
+        steps = w.steps;
+        groups = groups_of(a, units);
+    }
+    const Shares shares(units, groups);
+    const int i0 = uniform((int)shares.of(first)), i1 = uniform((int)shares.of(first + steps - 1));
     if (i0 == i1) return;
-    const int parts = i1 - i0 + 1;
-    auto at = [&](int p) { return (int64_t)(p == 0 ? 2 * i0 + 1 : 2 * (i0 + p)) * kRows + r - tile * kRows; };
+    const int parts = i1 - i0 + 1, tile_rows = big ? kPrompt : kRows, in_tile = r % tile_rows;
+    const float *part = big ? a.big_part : a.part, *stats = big ? a.big_stats : a.stats;
+    auto at = [&](int p) { return (int64_t)(p == 0 ? 2 * i0 + 1 : 2 * (i0 + p)) * tile_rows + in_tile; };
     float mx = -INFINITY, sum = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int p = lane; p < parts; p += 64) mx = fmaxf(mx, a.stats[2 * at(p)]);
+    for (int p = lane; p < parts; p += 64) mx = fmaxf(mx, stats[2 * at(p)]);
     const float origin = finite_max(wave_max(mx));
     for (int p0 = 0; p0 < parts; p0 += 64) {
         const int p = min(p0 + lane, parts - 1);
-        const float f = p0 + lane < parts ? exp2_of(a.stats[2 * at(p)] - origin) : 0.f;
-        sum += f * a.stats[2 * at(p) + 1];
+        const float f = p0 + lane < parts ? exp2_of(stats[2 * at(p)] - origin) : 0.f;
+        sum += f * stats[2 * at(p) + 1];
         for (int k0 = wid; k0 < min(64, parts - p0); k0 += J * kAtOnce) {
             float2 v[kAtOnce];
 #pragma unroll
             for (int k = 0; k < kAtOnce; k++)
-                v[k] = *reinterpret_cast<const float2 *>(a.part + at(min(p0 + k0 + k * J, parts - 1)) * a.Dh + d);
+                v[k] = *reinterpret_cast<const float2 *>(part + at(min(p0 + k0 + k * J, parts - 1)) * a.Dh + d);
 #pragma unroll
             for (int k = 0; k < kAtOnce; k++) {
                 const int from = k0 + k * J;
@@ -729,29 +1137,49 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs
 }
 
 struct Plan {
-    int NR, groups;
+    int NR, groups, few, big_groups;
+    size_t floats(int64_t Dh) const
+    {
+        return ((size_t)groups * 2 * (16 * NR) + (size_t)big_groups * 2 * kPrompt) * (size_t)(Dh + 2);
+    }
 };
+// Rows of a sequence (tokens by the query heads of a key head) that are a prompt's: from there on a workgroup of 128 of them reads
+// the keys fewer times than waves of 32 do
+constexpr int kFew = 64;
 Plan plan(int64_t T, int64_t H, int64_t Hkv, int64_t Dh, int64_t max_new, int bytes)
 {
     const int64_t G = H / Hkv, rows = (max_new < T ? max_new : T) * G;
     const int NR = rows <= 16 ? 1 : 2;
-    return {NR, resident(Dh <= 64 ? 1 : 2, NR, bytes) * kWaves * device_cus()};
+    if (rows > kFew) return {2, 2 * kWaves * device_cus(), kFew, 2 * device_cus()};
+    return {NR, resident(Dh <= 64 ? 1 : 2, NR, bytes) * kWaves * device_cus(), INT32_MAX, 0};
 }
 
-template <int ND, int NR, class P>
-int launch(const AttnArgs &a, hipStream_t st)
+template <int NR>
+int launch_join(const AttnArgs &a, hipStream_t st)
 {
-    hipLaunchKernelGGL((paged_attention_kernel<ND, NR, P>), dim3((unsigned)(a.groups / kWaves)), dim3(kThreads), 0, st, a);
-    const int rc = launch_status("paged_attention");
-    if (rc) return rc;
     const int64_t rh = (int64_t)a.pb.T * a.H;
     if (rh < 4 * device_cus()) hipLaunchKernelGGL((paged_attention_join_kernel<NR, kWaves>), dim3((unsigned)rh), dim3(kThreads), 0, st, a);
     else hipLaunchKernelGGL((paged_attention_join_kernel<NR, 1>), dim3((unsigned)((rh + kWaves - 1) / kWaves)), dim3(kThreads), 0, st, a);
     return launch_status("paged_attention (parts)");
 }
+template <int ND, int NR, class P>
+int launch(const AttnArgs &a, hipStream_t st)
+{
+    hipLaunchKernelGGL((paged_attention_kernel<ND, NR, P>), dim3((unsigned)(a.groups / kWaves)), dim3(kThreads), 0, st, a);
+    const int rc = launch_status("paged_attention");
+    return rc ? rc : launch_join<NR>(a, st);
+}
+template <int ND, class P>
+int launch_prompts(const AttnArgs &a, hipStream_t st)
+{
+    hipLaunchKernelGGL((paged_prompt_kernel<ND, P>), dim3((unsigned)a.big_groups), dim3(kThreads), 0, st, a);
+    const int rc = launch_status("paged_attention (prompts)");
+    return rc ? rc : launch_join<2>(a, st);
+}
 template <class P>
 int launch(const AttnArgs &a, int NR, hipStream_t st)
 {
+    if (a.big_groups) return a.Dh <= 64 ? launch_prompts<1, P>(a, st) : launch_prompts<2, P>(a, st);
     if (a.Dh <= 64) return NR == 1 ? launch<1, 1, P>(a, st) : launch<1, 2, P>(a, st);
     return NR == 1 ? launch<2, 1, P>(a, st) : launch<2, 2, P>(a, st);
 }
@@ -762,7 +1190,7 @@ CACTI_API size_t cacti_hip_paged_attention_workspace(int64_t T, int64_t B, int64
 {
     if (T <= 0 || B <= 0 || H <= 0 || Hkv <= 0 || Dh <= 0 || max_new <= 0 || H % Hkv) return 0;
     const Plan p = plan(T, H, Hkv, Dh, max_new, 1);        // (of 16 bits: no more)
-    return (size_t)p.groups * 2 * (16 * p.NR) * (size_t)(Dh + 2) * 4;
+    return p.floats(Dh) * 4;
 }
 
 CACTI_API int cacti_hip_paged_attention_f16(int64_t T, int64_t B, int64_t H, int64_t Hkv, int64_t Dh, int64_t max_new, float alpha,
@@ -785,8 +1213,10 @@ CACTI_API int cacti_hip_paged_attention_f16(int64_t T, int64_t B, int64_t H, int
                       INT32_MAX / (W * page / kStep + 1 + begin_of(32)), CACTI_E_NOTIMPL, "paged_attention: too many rows and positions in one call");
     const Plan p = plan(T, H, Hkv, Dh, max_new, bits / 8);
     float *part = (float *)workspace;
+    const size_t small = (size_t)p.groups * 2 * (16 * p.NR);
     const AttnArgs a = {pb, (int)H, (int)Hkv, (int)(H / Hkv), (int)Dh, padded_dim((int)Dh), (int)(max_new < T ? max_new : T), p.groups,
                         (unsigned)((1 << 22) / page + 1), alpha, (const half_t *)q, ldq, k_pages, v_pages, (const float *)k_scale,
-                        (const float *)v_scale, (half_t *)out, ldo, part, part + (size_t)p.groups * 2 * (16 * p.NR) * Dh};
+                        (const float *)v_scale, (half_t *)out, ldo, part, part + small * Dh, p.few, p.big_groups,
+                        part + small * (Dh + 2), part + small * (Dh + 2) + (size_t)p.big_groups * 2 * kPrompt * Dh};
     return bits == 8 ? launch<uint8_t>(a, p.NR, (hipStream_t)stream) : launch<half_t>(a, p.NR, (hipStream_t)stream);
 }
