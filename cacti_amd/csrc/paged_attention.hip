@@ -35,7 +35,8 @@ struct AttnArgs {
     PagedBatch pb;
     int H, Hkv, G, Dh, Dp, max_new, groups;
     unsigned page_magic;                       // x / page = x * page_magic >> 22 for x below kEntries pages
-    float alpha;
+    float alpha;                               // |alpha|; its sign goes to the queries
+    unsigned sign;                             // 0x80008000 where it is negative
     const half_t *q;
     int64_t ldq;
     const void *k_pages, *v_pages;
@@ -151,9 +152,9 @@ struct QueryWords {
 #pragma unroll
         for (int i = 0; i < 4 * ND; i++) w[i] = *reinterpret_cast<const u2_t *>(q + min(64 * (i / 4) + 16 * g + 4 * (i & 3), Dh - 4));
     }
-    __device__ __forceinline__ u2_t at(int i, int Dh) const
+    __device__ __forceinline__ u2_t at(int i, int Dh, unsigned sign) const
     {
-        return 64 * (i / 4) + 16 * (int)((threadIdx.x & 63) >> 4) + 4 * (i & 3) < Dh ? w[i] : u2_t{0u, 0u};
+        return 64 * (i / 4) + 16 * (int)((threadIdx.x & 63) >> 4) + 4 * (i & 3) < Dh ? w[i] ^ sign : u2_t{0u, 0u};
     }
 };
 template <int ND, class P>
@@ -161,14 +162,14 @@ struct Query;
 template <int ND>
 struct Query<ND, half_t> {
     half8_t h[2 * ND];
-    __device__ __forceinline__ float set(const QueryWords<ND> &q, int Dh)  // returns what the products have to be multiplied by
+    __device__ __forceinline__ float set(const QueryWords<ND> &q, int Dh, unsigned sign)  // returns what the products have to be multiplied by
     {
 #pragma unroll
         for (int c = 0; c < 2 * ND; c++) {
             Frag x;
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                const u2_t w = q.at(2 * c + j, Dh);
+                const u2_t w = q.at(2 * c + j, Dh, sign);
                 x.u[2 * j] = w[0];
                 x.u[2 * j + 1] = w[1];
             }
@@ -191,12 +192,12 @@ struct Query<ND, half_t> {
 template <int ND>
 struct Query<ND, uint8_t> {
     int t[3][4 * ND];
-    __device__ __forceinline__ float set(const QueryWords<ND> &q, int Dh)
+    __device__ __forceinline__ float set(const QueryWords<ND> &q, int Dh, unsigned sign)
     {
         float x[16 * ND], mx = 0.f;
 #pragma unroll
         for (int i = 0; i < 4 * ND; i++) {
-            const half4_t w = __builtin_bit_cast(half4_t, q.at(i, Dh));
+            const half4_t w = __builtin_bit_cast(half4_t, q.at(i, Dh, sign));
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 x[4 * i + k] = h2f(w[k]);
@@ -351,8 +352,44 @@ __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0
 // What the pages of a wave's positions are: where their rows of this head begin and what their scales make of a score
 struct Entry {
     int64_t at[kEntries];
-    float c[kEntries], lg[kEntries], iv[kEntries];         // alpha ks log2 e, log2 vs, 1 / vs
+    float c[kEntries], lg[kEntries], iv[kEntries];         // alpha ks log2 e (more than 0), log2 vs, 1 / vs
 };
+
+// The scores s of 32 positions of a lane's row (eight of them, in two registers of four) to weights: with c > 0 and lg of the
+// lane's page, t = s c + lg.  Takes part in the running maximum m and sum l (of weights by iv) and scales o where m grows; returns
+// the weights in f16.  seen: how many of the lane's eight positions its row sees; edge (the same in all lanes): not all of all.
+template <int N>
+__device__ __forceinline__ half8_t weigh(float4_t (&s)[2], float c, float lg, float iv, float &m, float &l, float4_t (&o)[N], bool edge, int seen)
+{
+    if (edge) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) s[i / 4][i & 3] = i < seen ? s[i / 4][i & 3] : -INFINITY;
+    }
+    float raw = s[0][0];                       // (c > 0: the largest of t is that of the largest of s)
+#pragma unroll
+    for (int i = 1; i < 8; i++) raw = fmaxf(raw, s[i / 4][i & 3]);
+    float mx = __builtin_fmaf(raw, c, lg);
+    mx = with32(with16(mx, OpMax()), OpMax());
+    const float mn = fmaxf(m, mx), origin = finite_max(mn);
+    if (__ballot(mn > m)) {                    // some row's maximum has grown
+        const float f = exp2_of(m - origin);
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < N; i++) o[i] *= f;
+    }
+    float sum = 0.f;
+    Frag p;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float x = exp2_of(__builtin_fmaf(s[i / 2][2 * i & 3], c, lg - origin)), y = exp2_of(__builtin_fmaf(s[i / 2][(2 * i & 3) + 1], c, lg - origin));
+        sum += x + y;
+        const half2_t pair = {f2h(x), f2h(y)};
+        p.u[i] = __builtin_bit_cast(unsigned, pair);
+    }
+    l = __builtin_fmaf(sum, iv, l);
+    return p.h;
+}
 
 // One tile of rows and a part of its positions, by a wave.  ND: pieces of 64 columns of a head
 template <int ND, int NR, class P>
@@ -438,7 +475,7 @@ struct Tile {
             load_v(x, end);
         };
         auto scales = [&]() __attribute__((always_inline)) {
-            entry.c[lane] = ks * (a.alpha * 1.44269504088896340736f);
+            entry.c[lane] = fmaxf(ks * (a.alpha * 1.44269504088896340736f), 1e-30f);
             entry.lg[lane] = __builtin_amdgcn_logf(vs);
             entry.iv[lane] = __builtin_amdgcn_rcpf(vs);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -455,7 +492,7 @@ struct Tile {
             }
             request(id, c0 - base);
 #pragma unroll
-            for (int n = 0; n < NR; n++) factor[n] = q[n].set(words[n], a.Dh);
+            for (int n = 0; n < NR; n++) factor[n] = q[n].set(words[n], a.Dh, a.sign);
             scales();
         }
 #pragma unroll
@@ -466,9 +503,7 @@ struct Tile {
             for (int i = 0; i < VD; i++) o[n][i] = float4_t{0.f, 0.f, 0.f, 0.f};
         }
         for (int x = c0 - base;;) {
-            const int clear = min(least - base, end - 1);      // up to here everything is seen by every row
-            for (; x + kStep - 1 <= clear; x += kStep) step<false>(x, end, least - base, base, min(x + kStep, end - 1));
-            for (; x < end; x += kStep) step<true>(x, end, least - base, base, min(x + kStep, end - 1));
+            for (; x < end; x += kStep) step(x, end, least - base, base, min(x + kStep, end - 1));
             const int seg = base + end;
             if (seg >= c1) break;
             const int id = look_up(seg);
@@ -478,11 +513,10 @@ struct Tile {
         }
     }
 
-    // EDGE: some of these 32 positions are hidden from some row
-    template <bool EDGE>
     __device__ __forceinline__ void step(int x, int end, int least, int base, int next)
     {
         const int lane = threadIdx.x & 63, g = lane >> 4;
+        const bool edge = x + kStep - 1 > min(least, end - 1);             // some of these 32 positions are hidden from some row
         float4_t sc[NR][2];
 #pragma unroll
         for (int t = 0; t < 2; t++)
@@ -493,40 +527,9 @@ struct Tile {
         const float ec = entry.c[pg], lg = entry.lg[pg], iv = entry.iv[pg];
         half8_t w[NR];
 #pragma unroll
-        for (int n = 0; n < NR; n++) {
-            float t[8], mx = -INFINITY;
-            const float c = ec * factor[n];
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                t[i] = __builtin_fmaf(i < 4 ? sc[n][0][i & 3] : sc[n][1][i & 3], c, lg);
-                if (EDGE && x + 8 * g + i > min(last[n] - base, end - 1)) t[i] = -INFINITY;
-                mx = fmaxf(mx, t[i]);
-            }
-            mx = with32(with16(mx, OpMax()), OpMax());
-            const float mn = fmaxf(m[n], mx), origin = finite_max(mn);
-            if (__ballot(mn > m[n])) {         // some row's maximum has grown
-                const float f = exp2_of(m[n] - origin);
-                m[n] = mn;
-                l[n] *= f;
-#pragma unroll
-                for (int i = 0; i < VD; i++) o[n][i] *= f;
-            }
-            float sum = 0.f;
-            Frag p;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                t[i] = exp2_of(t[i] - origin);
-                sum += t[i];
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const half2_t pair = {f2h(t[2 * i]), f2h(t[2 * i + 1])};
-                p.u[i] = __builtin_bit_cast(unsigned, pair);
-            }
-            l[n] = __builtin_fmaf(sum, iv, l[n]);
-            w[n] = p.h;
-        }
-        if (EDGE) {
+        for (int n = 0; n < NR; n++)
+            w[n] = weigh(sc[n], ec * factor[n], lg, iv, m[n], l[n], o[n], edge, min(last[n] - base, end - 1) - (x + 8 * g) + 1);
+        if (edge) {
             // what no row of the tile sees is nothing; a NaN or an infinity that some rows see must not meet the zero weights of
             // the others: it is added at the end
             bool any = false;
@@ -666,11 +669,13 @@ __global__ void __launch_bounds__(kThreads, resident(ND, NR, sizeof(P))) paged_a
 }
 
 // ---------------------------------------------------------------- prompts
-// Sequences with many new rows: 128 of them (tokens by the query heads of a key head) to a workgroup, 32 to a wave, 64 positions
-// at a time, whose keys and values go through LDS as f16: converted and V turned once for all four waves, while the products of
-// the 64 before them run, in two buffers with one barrier a step.  16-byte pieces of LDS rows are swapped by f(row), which spreads
-// the sixteen rows of an operand, and the rows that a wave writes, evenly over the banks.  What bounds it: the matrix pipe and
-// LDS about evenly (32 KB of operands to a wave for 1024 cycles of products), then the softmax between them.
+// Sequences with many new rows: 128 of them (tokens by the query heads of a key head) to a workgroup, 16 to each of its eight waves,
+// 64 positions at a time, whose keys and values go through LDS as f16: converted and V turned once for all waves (four of them
+// see to the keys, four to the values), while the products of the 64 before them run, in two buffers with one barrier a step.
+// 16-byte pieces of LDS rows are swapped by f(row), which spreads the sixteen rows of an operand, and the rows that a wave writes,
+// evenly over the banks.  What bounds it: LDS (16 KB of operands to a wave for 32 positions, 1024 cycles of a CU for all eight) and
+// the softmax's vector operations about evenly, the matrix pipe half as much.  (32 rows to a wave halve the first, but with the
+// registers of two waves a SIMD some are held in memory, whose loads wait for the next keys: 89 against kHalfRows us.)
 //
 // Shares are cut as above, a workgroup to a share and by steps of 64.  A tile's steps grow by those of its own 128 rows: counted
 // by a line that is never below them, so that what lies before a tile is a formula; steps behind a tile's last position are
@@ -699,10 +704,15 @@ struct BigShare {
     __device__ __forceinline__ unsigned units(const AttnArgs &a) const { return before(tiles) * (unsigned)a.Hkv; }
 };
 
+constexpr int kBigThreads = 512, kBigWaves = kBigThreads / 64;
+
 template <int ND, class P>
 struct Prompt {
-    static constexpr int NR = 2, NS = 2 * ND;  // of a wave: rows by 16; matrix instructions along the columns of a key
-    static constexpr int kPieces = kBig * 64 * ND * (int)sizeof(P) / 16 / kThreads;          // 16-byte pieces of keys of a lane
+    static constexpr int NS = 2 * ND;          // matrix instructions along the columns of a key
+    static constexpr int kHalf = kBigThreads / 2;                          // lanes that load keys, and that load values
+    static constexpr int kPer = 64 * ND * (int)sizeof(P) / 16;             // 16-byte pieces of a key
+    static constexpr int kPieces = kBig * kPer / kHalf;                    // of a lane
+    static constexpr int kCols = 16 * ND;                                  // lanes that have a key's columns, four each, of V
     struct Shared {
         half_t k[2][kBig][64 * ND], v[2][64 * ND][kBig];
         Entry entry;
@@ -710,158 +720,162 @@ struct Prompt {
     };
     const AttnArgs &a;
     Shared &sh;
-    half8_t q[NR][NS];
-    int last[NR];
-    float m[NR], l[NR];
-    float4_t o[NR][4 * ND];
-    u4_t kr[kPieces];                          // the next 64 positions, as they come
-    VBlock<P, 4> vr;
+    half8_t q[NS];
+    int last;
+    float m, l;
+    float4_t o[4 * ND];
+    // the next 64 positions, as they come: keys (waves 4 to 7) or values (waves 0 to 3; ND 1: 0 and 1)
+    union {
+        u4_t k[kPieces];
+        VBlock<P, 4> v;
+    } next;
 
     __device__ __forceinline__ int page_of(int x) const { return (int)(__umul24((unsigned)x, a.page_magic) >> 22); }
-    __device__ __forceinline__ bool turns() const { return ND == 2 || threadIdx.x < 128; }   // has four columns of eight values
 
-    __device__ __forceinline__ void load(int x, int end)
+    // 16 positions in a row are of one page, and so is all that a wave loads at once: the address of its first row is a scalar, a
+    // lane's part of it the same every time (but for the positions behind `end`).
+    __device__ __forceinline__ const P *page_at(const void *pages, int x) const
     {
-        constexpr int per = 64 * ND * (int)sizeof(P) / 16;                 // pieces of a key
-        const int tid = 64 * uniform((int)threadIdx.x >> 6) + lane_here();
-#pragma unroll
-        for (int i = 0; i < kPieces; i++) {
-            const int piece = tid + i * kThreads, j = min(x + piece / per, end - 1), pg = page_of(j);
-            const P *row = (const P *)a.k_pages + sh.entry.at[pg] + __umul24(j - __umul24(pg, a.pb.page), a.Dp);
-            kr[i] = *reinterpret_cast<const u4_t *>(row + min(piece % per * (16 / (int)sizeof(P)), a.Dp - 16 / (int)sizeof(P)));
+        const int pg = page_of(x);
+        const int64_t at = sh.entry.at[pg];
+        const int64_t uni = (int64_t)((uint64_t)(unsigned)uniform((int)(at >> 32)) << 32 | (unsigned)uniform((int)at));
+        return (const P *)pages + uni + (int64_t)((x - pg * a.pb.page) * a.Dp);
+    }
+    // What of the addresses is a lane's own: its row and columns in memory, elements from the wave's first row, and its place in
+    // LDS, halves from a buffer's start (keys: piece i is 16 rows on, whose swap has another bit 2, or 32; values: column 0 of 4)
+    struct Own {
+        unsigned from;
+        int to;
+    };
+    __device__ __forceinline__ Own own() const
+    {
+        const int tid = threadIdx.x & (kHalf - 1), lane = tid & 63;
+        Own w;
+        if (threadIdx.x >= kHalf) {
+            w.from = __umul24(lane / kPer, a.Dp) + min(lane % kPer * (16 / (int)sizeof(P)), a.Dp - 16 / (int)sizeof(P));
+            const int j = tid / kPer, c = tid % kPer * (16 / (int)sizeof(P)) / 8;
+            w.to = j * 64 * ND + (c ^ swap_of(j)) * 8;
+        } else {
+            w.from = __umul24((8 * (lane / kCols)) & 15, a.Dp) + min(4 * (lane % kCols), a.Dp - 4);
+            const int kg = tid / kCols, d = 4 * (tid % kCols);
+            w.to = d * kBig + (kg ^ swap_of(d)) * 8;
         }
-        if (!turns()) return;
-        const int j0 = x + 8 * (tid / (16 * ND)), pg = page_of(min(j0, end - 1));
-        const P *row = (const P *)a.v_pages + sh.entry.at[pg] + min(4 * (tid % (16 * ND)), a.Dp - 4);
+        return w;
+    }
+    __device__ __forceinline__ void load(const Own &w, int x, int end)
+    {
+        const int wid = uniform((int)threadIdx.x >> 6);
+        if (wid >= kBigWaves / 2) {
+            const int first = 64 * (wid - kBigWaves / 2) / kPer;
+            if (x + kBig <= end) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) vr.load(i, row + __umul24(min(j0 + i, end - 1) - __umul24(pg, a.pb.page), a.Dp));
+                for (int i = 0; i < kPieces; i++)
+                    next.k[i] = *reinterpret_cast<const u4_t *>(page_at(a.k_pages, x + first + i * (kHalf / kPer)) + w.from);
+                return;
+            }
+            const int lane = lane_here();
+#pragma unroll
+            for (int i = 0; i < kPieces; i++) {
+                const int j = min(x + first + i * (kHalf / kPer) + lane / kPer, end - 1), pg = page_of(j);
+                const P *row = (const P *)a.k_pages + sh.entry.at[pg] + __umul24(j - __umul24(pg, a.pb.page), a.Dp);
+                next.k[i] = *reinterpret_cast<const u4_t *>(row + min(lane % kPer * (16 / (int)sizeof(P)), a.Dp - 16 / (int)sizeof(P)));
+            }
+        } else if (ND == 2 || wid < 2) {
+            const int first = 8 * (64 / kCols) * wid;          // 16 positions to a wave or, ND 1, 32
+            if (x + kBig <= end) {
+                const P *v = page_at(a.v_pages, x + first);
+                if (ND == 1) {
+                    const P *v1 = page_at(a.v_pages, x + first + 16);
+                    v = (threadIdx.x & 32) ? v1 : v;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++) next.v.load(i, v + i * a.Dp + w.from);
+                return;
+            }
+            const int lane = lane_here(), j0 = x + first + 8 * (lane / kCols), pg = page_of(min(j0, end - 1));
+            const P *row = (const P *)a.v_pages + sh.entry.at[pg] + min(4 * (lane % kCols), a.Dp - 4);
+#pragma unroll
+            for (int i = 0; i < 8; i++) next.v.load(i, row + __umul24(min(j0 + i, end - 1) - __umul24(pg, a.pb.page), a.Dp));
+        }
     }
     // ... into buffer `to`; least: positions up to there are seen by every row of the tile
-    __device__ __forceinline__ void store(int to, int x, int end, int least)
+    __device__ __forceinline__ void store(const Own &own, int to, int x, int end, int least)
     {
-        constexpr int per = 64 * ND * (int)sizeof(P) / 16;
-        const int tid = 64 * uniform((int)threadIdx.x >> 6) + lane_here();
+        const int wid = uniform((int)threadIdx.x >> 6);
+        half_t *kb = &sh.k[to][0][0], *vb = &sh.v[to][0][0];
+        if (wid >= kBigWaves / 2) {
+            if ((threadIdx.x & 63) % kPer * (16 / (int)sizeof(P)) >= a.Dp) // (beside the columns the queries are zeros, and so must the keys be)
 #pragma unroll
-        for (int i = 0; i < kPieces; i++) {
-            const int piece = tid + i * kThreads, j = piece / per, d = piece % per * (16 / (int)sizeof(P));
-            const bool in = d < a.Dp;          // (beside the columns the queries are zeros, and so must the keys be)
+                for (int i = 0; i < kPieces; i++) next.k[i] = u4_t{0u, 0u, 0u, 0u};
 #pragma unroll
-            for (int k = 0; k < 16 / (int)sizeof(P) / 8; k++) {
-                Frag f;
+            for (int i = 0; i < kPieces; i++)
 #pragma unroll
-                for (int w = 0; w < 4; w++) f.u[w] = !in ? 0u : sizeof(P) == 2 ? kr[i][w] : cvt8(kr[i][2 * k + w / 2], w & 1);
-                *reinterpret_cast<half8_t *>(&sh.k[to][j][((d / 8 + k) ^ swap_of(j)) * 8]) = f.h;
+                for (int k = 0; k < 16 / (int)sizeof(P) / 8; k++) {
+                    Frag f;
+#pragma unroll
+                    for (int w = 0; w < 4; w++) f.u[w] = sizeof(P) == 2 ? next.k[i][w] : cvt8(next.k[i][2 * k + w / 2], w & 1);
+                    *reinterpret_cast<half8_t *>(kb + (own.to ^ (8 * k) ^ (kHalf / kPer == 16 ? 32 * (i & 1) : 0)) + i * (kHalf / kPer) * 64 * ND) = f.h;
+                }
+        } else if (ND == 2 || wid < 2) {
+            if (x + kBig - 1 > min(least, end - 1)) {
+                const int j0 = x + 8 * ((64 * wid + lane_here()) / kCols);
+                bool any = false;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    if (j0 + i >= end) next.v.zero(i);
+                    else if (j0 + i > least) any = next.v.strip(i) || any;
+                }
+                if (any) sh.odd = 1;
             }
-        }
-        if (!turns()) return;
-        const int kg = tid / (16 * ND), d = 4 * (tid % (16 * ND));
-        if (x + kBig - 1 > min(least, end - 1)) {
-            bool any = false;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int j = x + 8 * kg + i;
-                if (j >= end) vr.zero(i);
-                else if (j > least) any = vr.strip(i) || any;
+            for (int c = 0; c < 2; c++) {
+                half8_t v0, v1;
+                next.v.columns(c, &v0, &v1);
+                *reinterpret_cast<half8_t *>(vb + (own.to ^ (16 * c)) + 2 * c * kBig) = v0;             // swap_of(d + e) = swap_of(d) ^ e
+                *reinterpret_cast<half8_t *>(vb + (own.to ^ (16 * c + 8)) + (2 * c + 1) * kBig) = v1;
             }
-            if (any) sh.odd = 1;
-        }
-#pragma unroll
-        for (int c = 0; c < 2; c++) {
-            half8_t v0, v1;
-            vr.columns(c, &v0, &v1);
-            *reinterpret_cast<half8_t *>(&sh.v[to][d + 2 * c][(kg ^ swap_of(d + 2 * c)) * 8]) = v0;
-            *reinterpret_cast<half8_t *>(&sh.v[to][d + 2 * c + 1][(kg ^ swap_of(d + 2 * c + 1)) * 8]) = v1;
         }
     }
 
     // Where a lane reads its operands, in halves from the start of a buffer.  A key's row is j = 32 b + 8 (r16 / 4) + 4 t + r16 % 4,
-    // so swap_of(j) = 2 (r16 / 4) ^ r16 % 4 ^ 5 t; a row of V is d = 16 c + r16, swap_of(d) = r16 / 4 ^ r16 & 7 ^ 4 (c & 1): what b, c
-    // and t make of a piece's place but for these swaps is a constant of the instruction.
+    // so swap_of(j) = 2 (r16 / 4) ^ r16 % 4 ^ 5 t; a row of V is d = 16 c + r16, swap_of(d) = r16 / 4 ^ r16 & 7 ^ 4 (c & 1).  The
+    // lane's place with b, c and t all 0; these swaps turn bits of it, the rest is a constant of the instruction.
     struct Places {
-        int k[2][2], v[2];                     // [t][c & 1], [b ^ c & 1]
+        int k, v;
     };
     __device__ __forceinline__ Places places() const
     {
         const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4, a4 = r16 >> 2, b4 = r16 & 3;
-        Places p;
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int c = 0; c < 2; c++) p.k[t][c] = (8 * a4 + 4 * t + b4) * 64 * ND + ((4 * c + g) ^ (2 * a4) ^ b4 ^ (5 * t)) * 8;
-#pragma unroll
-        for (int x = 0; x < 2; x++) p.v[x] = r16 * kBig + ((4 * x + g) ^ ((a4 ^ r16) & 7)) * 8;
-        return p;
+        return {(8 * a4 + b4) * 64 * ND + (g ^ (2 * a4) ^ b4) * 8, r16 * kBig + (g ^ ((a4 ^ r16) & 7)) * 8};
     }
 
-    // 32 positions, those from x on, block b of the buffer (the scores of all 64 at once are more registers than there are)
-    template <bool EDGE>
-    __device__ __forceinline__ void step(const Places &at, int from, int b, int x, int end, int base)
+    // 32 positions, those from x on, block b of the buffer; least: positions up to there are seen by every row of the wave
+    __device__ __forceinline__ void step(const Places &at, int from, int b, int x, int end, int base, int least)
     {
         const int lane = threadIdx.x & 63, g = lane >> 4;
-        float4_t sc[NR][2];
         const half_t *kb = &sh.k[from][0][0] + 32 * b * 64 * ND, *vb = &sh.v[from][0][0];
+        float4_t sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
+        for (int c = 0; c < NS; c++)
 #pragma unroll
-            for (int n = 0; n < NR; n++) sc[n][t] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < NS; c++) {
-                const half8_t kf = *reinterpret_cast<const half8_t *>(kb + at.k[t][c & 1] + (c >> 1) * 64);
-#pragma unroll
-                for (int n = 0; n < NR; n++) sc[n][t] = mfma(kf, q[n][c], sc[n][t]);
-            }
-        }
+            for (int t = 0; t < 2; t++)
+                sc[t] = mfma(*reinterpret_cast<const half8_t *>(kb + (at.k ^ (40 * t) ^ (32 * (c & 1))) + 4 * t * 64 * ND + (c >> 1) * 64), q[c], sc[t]);
         const int pg = page_of(min(x + 8 * g, end - 1));
-        const float ec = sh.entry.c[pg], lg = sh.entry.lg[pg], iv = sh.entry.iv[pg];
-        Frag p[NR];
+        const half8_t p = weigh(sc, sh.entry.c[pg], sh.entry.lg[pg], sh.entry.iv[pg], m, l, o, x + 31 > min(least, end - 1),
+                                min(last - base, end - 1) - (x + 8 * g) + 1);
+        const int v0 = at.v ^ (32 * b);
 #pragma unroll
-        for (int n = 0; n < NR; n++) {
-            float t[8], mx = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                t[i] = __builtin_fmaf(sc[n][i / 4][i & 3], ec, lg);
-                if (EDGE && x + 8 * g + i > min(last[n] - base, end - 1)) t[i] = -INFINITY;
-                mx = fmaxf(mx, t[i]);
-            }
-            mx = with32(with16(mx, OpMax()), OpMax());
-            const float mn = fmaxf(m[n], mx), origin = finite_max(mn);
-            if (__ballot(mn > m[n])) {
-                const float f = exp2_of(m[n] - origin);
-                m[n] = mn;
-                l[n] *= f;
-#pragma unroll
-                for (int i = 0; i < 4 * ND; i++) o[n][i] *= f;
-            }
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                t[i] = exp2_of(t[i] - origin);
-                sum += t[i];
-            }
-            l[n] = __builtin_fmaf(sum, iv, l[n]);
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const half2_t pair = {f2h(t[2 * i]), f2h(t[2 * i + 1])};
-                p[n].u[i] = __builtin_bit_cast(unsigned, pair);
-            }
-        }
-#pragma unroll
-        for (int c = 0; c < 4 * ND; c++) {
-            const half8_t vf = *reinterpret_cast<const half8_t *>(vb + at.v[b ^ (c & 1)] + 16 * c * kBig);
-#pragma unroll
-            for (int n = 0; n < NR; n++) o[n][c] = mfma(vf, p[n].h, o[n][c]);
-        }
+        for (int c = 0; c < 4 * ND; c++) o[c] = mfma(*reinterpret_cast<const half8_t *>(vb + (v0 ^ (32 * (c & 1))) + 16 * c * kBig), p, o[c]);
     }
 
     // positions c0 .. c1 - 1 (some) of rows row0 .. of sequence s
     __device__ __forceinline__ void run(int b, const Sequence &s, int h, int rows, int row0, int c0, int c1)
     {
         const int wid = uniform((int)threadIdx.x >> 6), lane = lane_here(), tid = 64 * wid + lane, r16 = lane & 15, g = lane >> 4;
-        const int mine = row0 + 16 * NR * wid;                 // the wave's first row
-#pragma unroll
-        for (int n = 0; n < NR; n++) {
-            const int r = min(mine + 16 * n + r16, rows - 1), t = r / a.G;
-            last[n] = s.first + t;
+        const int mine = row0 + 16 * wid;      // the wave's first row
+        {
+            const int r = min(mine + r16, rows - 1), t = r / a.G;
+            last = s.first + t;
             const half_t *qr = a.q + (int64_t)(s.s0 + t) * a.ldq + (h * a.G + r - t * a.G) * a.Dh;
 #pragma unroll
             for (int c = 0; c < NS; c++) {
@@ -870,19 +884,20 @@ struct Prompt {
                 for (int j = 0; j < 2; j++) {
                     const int d = 32 * c + 8 * g + 4 * j;
                     const u2_t w = *reinterpret_cast<const u2_t *>(qr + min(d, a.Dh - 4));
-                    f.u[2 * j] = d < a.Dh ? w[0] : 0u;
-                    f.u[2 * j + 1] = d < a.Dh ? w[1] : 0u;
+                    f.u[2 * j] = d < a.Dh ? w[0] ^ a.sign : 0u;
+                    f.u[2 * j + 1] = d < a.Dh ? w[1] ^ a.sign : 0u;
                 }
-                q[n][c] = f.h;
+                q[c] = f.h;
             }
-            m[n] = -INFINITY;
-            l[n] = 0.f;
+            m = -INFINITY;
+            l = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4 * ND; i++) o[n][i] = float4_t{0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < 4 * ND; i++) o[i] = float4_t{0.f, 0.f, 0.f, 0.f};
         }
         const int least = uniform(s.first + row0 / a.G);                               // seen by every row of the tile
-        const int wave_least = uniform(s.first + min(mine, rows - 1) / a.G), wave_last = uniform(mine < rows ? s.first + (min(mine + 16 * NR, rows) - 1) / a.G : -1);
+        const int wave_least = uniform(s.first + min(mine, rows - 1) / a.G), wave_last = uniform(mine < rows ? s.first + (min(mine + 16, rows) - 1) / a.G : -1);
         const Places at = places();
+        const Own w = own();
         for (int seg = c0; seg < c1;) {
             const int p0 = uniform(seg / a.pb.page), base = p0 * a.pb.page, end = min(c1 - base, kEntries * a.pb.page);
             __syncthreads();                   // (entries and buffers of before are done with)
@@ -896,28 +911,24 @@ struct Prompt {
                 float ks = 1.f, vs = 1.f;
                 if (sizeof(P) == 1) ks = a.k_scale[ph], vs = a.v_scale[ph];
                 sh.entry.at[lane] = ph * a.pb.page * a.Dp;
-                sh.entry.c[lane] = ks * (a.alpha * 1.44269504088896340736f);
+                sh.entry.c[lane] = fmaxf(ks * (a.alpha * 1.44269504088896340736f), 1e-30f);
                 sh.entry.lg[lane] = __builtin_amdgcn_logf(vs);
                 sh.entry.iv[lane] = __builtin_amdgcn_rcpf(vs);
                 if (seg == c0 && lane == 0) sh.odd = 0;
             }
             __syncthreads();
             int x = seg - base, buffer = 0;
-            load(x, end);
-            store(0, x, end, least - base);
+            load(w, x, end);
+            store(w, 0, x, end, least - base);
             __syncthreads();
             for (; x < end; x += kBig) {
                 const bool more = x + kBig < end;
-                load(more ? x + kBig : x, end);
-#pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    const int x32 = x + 32 * half;
-                    if (x32 > min(wave_last - base, end - 1)) continue;
-                    if (x32 + 31 > min(wave_least - base, end - 1)) step<true>(at, buffer, half, x32, end, base);
-                    else step<false>(at, buffer, half, x32, end, base);
-                }
+                load(w, more ? x + kBig : x, end);
+#pragma unroll 1
+                for (int half = 0; half < 2; half++)
+                    if (x + 32 * half <= min(wave_last - base, end - 1)) step(at, buffer, half, x + 32 * half, end, base, wave_least - base);
                 buffer ^= 1;
-                if (more) store(buffer, x + kBig, end, least - base);
+                if (more) store(w, buffer, x + kBig, end, least - base);
                 __syncthreads();
             }
             seg = base + end;
@@ -926,7 +937,7 @@ struct Prompt {
 
     __device__ __forceinline__ void write(int b, const Sequence &s, int h, int rows, int row0, int c0, int c1, int slot)
     {
-        const int lane = lane_here(), wid = uniform((int)threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4, mine = row0 + 16 * NR * wid;
+        const int lane = lane_here(), wid = uniform((int)threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
         if (c0 < c1 && sh.odd) {               // NaNs and infinities of V, each to the rows that see it
 #pragma unroll 1
             for (int j = max(c0, s.first + row0 / a.G + 1); j < c1; j++) {
@@ -938,113 +949,123 @@ struct Prompt {
                     x.load(0, v + min(16 * c + 4 * g, a.Dp - 4));
 #pragma unroll
                     for (int i = 0; i < 4; i++)
-#pragma unroll
-                        for (int n = 0; n < NR; n++)
-                            if (!(fabsf(x.value(i)) < INFINITY) && j <= last[n]) o[n][c][i] += x.value(i);
+                        if (!(fabsf(x.value(i)) < INFINITY) && j <= last) o[c][i] += x.value(i);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
         }
+        const float sum = with32(with16(l, OpSum()), OpSum());
+        const int r = row0 + 16 * wid + r16, t = r / a.G;
+        if (r >= rows) return;
+        const float y = slot >= 0 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+        const int64_t at = (int64_t)slot * kPrompt + r - row0;
+        half_t *out = a.out + (int64_t)(s.s0 + t) * a.ldo + (h * a.G + r - t * a.G) * a.Dh;
+        float *part = a.big_part + at * a.Dh;
 #pragma unroll
-        for (int n = 0; n < NR; n++) {
-            const float sum = with32(with16(l[n], OpSum()), OpSum());
-            const int r = mine + 16 * n + r16, t = r / a.G;
-            if (r >= rows) continue;
-            const float y = slot >= 0 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
-            const int64_t at = (int64_t)slot * kPrompt + r - row0;
-            half_t *out = a.out + (int64_t)(s.s0 + t) * a.ldo + (h * a.G + r - t * a.G) * a.Dh;
-            float *part = a.big_part + at * a.Dh;
-#pragma unroll
-            for (int c = 0; c < 4 * ND; c++) {
-                const int d = 16 * c + 4 * g;
-                if (d >= a.Dh) continue;
-                const float4_t v = o[n][c] * y;
-                if (slot >= 0) *reinterpret_cast<float4_t *>(part + d) = v;
-                else *reinterpret_cast<half4_t *>(out + d) = half4_t{f2h(v[0]), f2h(v[1]), f2h(v[2]), f2h(v[3])};
-            }
-            if (slot >= 0 && g == 0) {
-                a.big_stats[2 * at] = m[n];
-                a.big_stats[2 * at + 1] = sum;
-            }
+        for (int c = 0; c < 4 * ND; c++) {
+            const int d = 16 * c + 4 * g;
+            if (d >= a.Dh) continue;
+            const float4_t v = o[c] * y;
+            if (slot >= 0) *reinterpret_cast<float4_t *>(part + d) = v;
+            else *reinterpret_cast<half4_t *>(out + d) = half4_t{f2h(v[0]), f2h(v[1]), f2h(v[2]), f2h(v[3])};
+        }
+        if (slot >= 0 && g == 0) {
+            a.big_stats[2 * at] = m;
+            a.big_stats[2 * at + 1] = sum;
         }
     }
 };
 
-// The prompts' share of a workgroup, then the other sequences' shares of its waves
 template <int ND, class P>
-__global__ void __launch_bounds__(kThreads, 2) paged_prompt_kernel(AttnArgs a)
+__global__ void __launch_bounds__(kBigThreads, 4) paged_prompt_kernel(AttnArgs a)
 {
-    __shared__ union {
-        typename Prompt<ND, P>::Shared big;
-        Entry entries[kWaves];
-    } sh;
-    const int wid = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+    __shared__ typename Prompt<ND, P>::Shared sh;
+    const int lane = threadIdx.x & 63;
     const Sequence s64 = lane_sequence(a, 0);
     const double u64 = BigShare(a, s64).units(a);
     double all = u64;
     for (int b0 = 64; b0 < a.pb.B; b0 += 64) all += BigShare(a, lane_sequence(a, b0)).units(a);
     const unsigned units = uniform((int)(unsigned)wave_sum_f64(all)), groups = min((unsigned)a.big_groups, max(units / kBigLeast, 1u));
     const unsigned group = xcd_order(blockIdx.x, a.big_groups);
-    if (units > 0 && group < groups) {
-        const Shares shares(units, groups);
-        unsigned x = uniform((int)shares.begin(group));
-        const unsigned until = uniform((int)shares.begin(group + 1));
-        int b = 0;
-        unsigned before = 0;
-        for (int b0 = 0; b0 < a.pb.B; b0 += 64) {
-            const double u = b0 == 0 ? u64 : BigShare(a, lane_sequence(a, b0)).units(a), upto = scan_f64(u) + (double)before;
-            const uint64_t hit = __ballot(upto > (double)x);
-            const int at = hit ? __ffsll((unsigned long long)hit) - 1 : 63;
-            before = (unsigned)uniform((int)(unsigned)lane_f64(hit ? upto - u : upto, at));
-            if (hit) {
-                b = b0 + at;
-                break;
-            }
+    if (units == 0 || group >= groups) return;
+    const Shares shares(units, groups);
+    unsigned x = uniform((int)shares.begin(group));
+    const unsigned until = uniform((int)shares.begin(group + 1));
+    int b = 0;
+    unsigned before = 0;
+    for (int b0 = 0; b0 < a.pb.B; b0 += 64) {
+        const double u = b0 == 0 ? u64 : BigShare(a, lane_sequence(a, b0)).units(a), upto = scan_f64(u) + (double)before;
+        const uint64_t hit = __ballot(upto > (double)x);
+        const int at = hit ? __ffsll((unsigned long long)hit) - 1 : 63;
+        before = (unsigned)uniform((int)(unsigned)lane_f64(hit ? upto - u : upto, at));
+        if (hit) {
+            b = b0 + at;
+            break;
         }
-        for (; x < until; b++) {
-            const Sequence s = b < 64 ? of_lane(s64, b) : sequence(a.pb, b, (int64_t)a.pb.W * a.pb.page, a.max_new);
-            const BigShare w(a, s);
-            const unsigned head = w.before(w.tiles), behind = before + w.units(a);
-            while (x < until && x < behind) {
-                const int h = uniform((int)((x - before) / head)), rows = s.n * a.G;
-                const unsigned in = x - before - h * head;
-                int tile = 0;                  // that unit `in` of the head lies in
-                for (int t0 = 0; t0 < w.tiles; t0 += 64) {
-                    const int n = __popcll(__ballot(t0 + lane < w.tiles && w.before(t0 + lane + 1) <= in));
-                    tile += n;
-                    if (n < 64) break;
-                }
-                tile = uniform(tile);
-                const unsigned start = uniform((int)w.before(tile)), whole = uniform((int)w.before(tile + 1)) - start;
-                const int from = (int)(in - start), to = (int)min(whole, from + (until - x)), row0 = tile * kPrompt;
-                const int end = uniform(s.first + min(rows - 1, row0 + kPrompt - 1) / a.G + 1);
-                const int first = max(from - kBigBegin, 0), behind_last = to - kBigBegin;
-                if (behind_last > first) {
-                    const int c0 = first * kBig, c1 = min(end, behind_last * kBig);
-                    Prompt<ND, P> t{a, sh.big};
-                    t.run(b, s, h, rows, row0, c0, c1);
-                    t.write(b, s, h, rows, row0, c0, c1, first == 0 && behind_last == (int)whole - kBigBegin ? -1 : 2 * (int)group + (first == 0));
-                }
-                x += to - from;
-            }
-            before = behind;
-        }
-        __syncthreads();
     }
-    wave_share<ND, 2, P>(a, blockIdx.x * kWaves + wid, sh.entries[wid]);
+    for (; x < until; b++) {
+        const Sequence s = b < 64 ? of_lane(s64, b) : sequence(a.pb, b, (int64_t)a.pb.W * a.pb.page, a.max_new);
+        const BigShare w(a, s);
+        const unsigned head = w.before(w.tiles), behind = before + w.units(a);
+        while (x < until && x < behind) {
+            const int h = uniform((int)((x - before) / head)), rows = s.n * a.G;
+            const unsigned in = x - before - h * head;
+            int tile = 0;                  // that unit `in` of the head lies in
+            for (int t0 = 0; t0 < w.tiles; t0 += 64) {
+                const int n = __popcll(__ballot(t0 + lane < w.tiles && w.before(t0 + lane + 1) <= in));
+                tile += n;
+                if (n < 64) break;
+            }
+            tile = uniform(tile);
+            const unsigned start = uniform((int)w.before(tile)), whole = uniform((int)w.before(tile + 1)) - start;
+            const int from = (int)(in - start), to = (int)min(whole, from + (until - x)), row0 = tile * kPrompt;
+            const int end = uniform(s.first + min(rows - 1, row0 + kPrompt - 1) / a.G + 1);
+            const int first = max(from - kBigBegin, 0), behind_last = to - kBigBegin;
+            if (behind_last > first) {
+                const int c0 = first * kBig, c1 = min(end, behind_last * kBig);
+                Prompt<ND, P> t{a, sh};
+                t.run(b, s, h, rows, row0, c0, c1);
+                t.write(b, s, h, rows, row0, c0, c1, first == 0 && behind_last == (int)whole - kBigBegin ? -1 : 2 * (int)group + (first == 0));
+            }
+            x += to - from;
+        }
+        before = behind;
+    }
 }
 
-// The parts of a row put together, two columns per lane; zeros for rows whose sequence's numbers do not fit together.  J waves to
-// a row and head: kWaves where they do not fill the device, 1 where they do.
-template <int NR, int J>
+// Where the parts of a tile of rows are: those of its first step's group, of the next ones and of its last step's
+struct Parts {
+    int i0, count;
+    __device__ __forceinline__ Parts(const AttnArgs &a, const Sequence &s, int rows, int h, int tile, unsigned units, unsigned before)
+    {
+        unsigned first, steps, groups;
+        if (s.n * a.G > a.few) {
+            const BigShare w(a, s);
+            first = before + h * w.before(w.tiles) + w.before(tile) + kBigBegin;
+            steps = w.before(tile + 1) - w.before(tile) - kBigBegin;
+            groups = min((unsigned)a.big_groups, max(units / kBigLeast, 1u));
+        } else {
+            const Share w(a, rows, s);
+            first = before + (unsigned)(h * w.tiles + tile) * (w.steps + begin_of(rows)) + begin_of(rows);
+            steps = w.steps;
+            groups = groups_of(a, units);
+        }
+        const Shares shares(units, groups);
+        i0 = uniform((int)shares.of(first));
+        count = uniform((int)shares.of(first + steps - 1)) - i0 + 1;
+    }
+    __device__ __forceinline__ int slot(int p) const { return p == 0 ? 2 * i0 + 1 : 2 * (i0 + p); }
+};
+
+// The parts of a row put together, two columns per lane, by a workgroup per row and head; zeros for rows whose sequence's numbers
+// do not fit together.  For few rows: every fourth part to a wave.
+template <int NR>
 __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs a)
 {
     constexpr int kRows = 16 * NR, kAtOnce = 8;
     __shared__ float o[kWaves][2][64];
     const PagedBatch &pb = a.pb;
-    const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), wid = J == 1 ? 0 : wave;
-    const int rh = J == 1 ? blockIdx.x * kWaves + wave : blockIdx.x, row = rh / a.H, head = rh - row * a.H;
-    if (row >= pb.T) return;
+    const int lane = threadIdx.x & 63, wid = uniform((int)threadIdx.x >> 6), row = blockIdx.x / a.H, head = blockIdx.x - row * a.H;
     const int d = min(2 * lane, a.Dh - 2);
     // all work, that of the sequences before the row's, and the row's sequence
     double all = 0., some = 0., big_all = 0., big_some = 0.;
@@ -1076,27 +1097,13 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs
         return;
     }
     const bool big = s.n * a.G > a.few;
-    const unsigned units = uniform((int)(unsigned)wave_sum_f64(big ? big_all : all));
-    unsigned first = uniform((int)(unsigned)wave_sum_f64(big ? big_some : some)), steps, groups;       // the tile's first step, its steps
-    const int h = head / a.G, r = (row - s.s0) * a.G + head - h * a.G;
-    if (big) {
-        const BigShare w(a, s);
-        const int tile = r / kPrompt;
-        first += h * w.before(w.tiles) + w.before(tile) + kBigBegin;
-        steps = w.before(tile + 1) - w.before(tile) - kBigBegin;
-        groups = min((unsigned)a.big_groups, max(units / kBigLeast, 1u));
-    } else {
-        const Share w(a, kRows, s);
-        first += (unsigned)(h * w.tiles + r / kRows) * (w.steps + begin_of(kRows)) + begin_of(kRows);
-        steps = w.steps;
-        groups = groups_of(a, units);
-    }
-    const Shares shares(units, groups);
-    const int i0 = uniform((int)shares.of(first)), i1 = uniform((int)shares.of(first + steps - 1));
-    if (i0 == i1) return;
-    const int parts = i1 - i0 + 1, tile_rows = big ? kPrompt : kRows, in_tile = r % tile_rows;
+    const int h = head / a.G, r = (row - s.s0) * a.G + head - h * a.G, tile_rows = big ? kPrompt : kRows, tile = r / tile_rows;
+    const Parts in(a, s, kRows, h, tile, uniform((int)(unsigned)wave_sum_f64(big ? big_all : all)),
+                   uniform((int)(unsigned)wave_sum_f64(big ? big_some : some)));
+    const int parts = in.count;
+    if (parts == 1) return;
     const float *part = big ? a.big_part : a.part, *stats = big ? a.big_stats : a.stats;
-    auto at = [&](int p) { return (int64_t)(p == 0 ? 2 * i0 + 1 : 2 * (i0 + p)) * tile_rows + in_tile; };
+    auto at = [&](int p) { return (int64_t)in.slot(p) * tile_rows + r - tile * tile_rows; };
     float mx = -INFINITY, sum = 0.f, o0 = 0.f, o1 = 0.f;
     for (int p = lane; p < parts; p += 64) mx = fmaxf(mx, stats[2 * at(p)]);
     const float origin = finite_max(wave_max(mx));
@@ -1104,14 +1111,14 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs
         const int p = min(p0 + lane, parts - 1);
         const float f = p0 + lane < parts ? exp2_of(stats[2 * at(p)] - origin) : 0.f;
         sum += f * stats[2 * at(p) + 1];
-        for (int k0 = wid; k0 < min(64, parts - p0); k0 += J * kAtOnce) {
+        for (int k0 = wid; k0 < min(64, parts - p0); k0 += kWaves * kAtOnce) {
             float2 v[kAtOnce];
 #pragma unroll
             for (int k = 0; k < kAtOnce; k++)
-                v[k] = *reinterpret_cast<const float2 *>(part + at(min(p0 + k0 + k * J, parts - 1)) * a.Dh + d);
+                v[k] = *reinterpret_cast<const float2 *>(part + at(min(p0 + k0 + k * kWaves, parts - 1)) * a.Dh + d);
 #pragma unroll
             for (int k = 0; k < kAtOnce; k++) {
-                const int from = k0 + k * J;
+                const int from = k0 + k * kWaves;
                 if (from >= min(64, parts - p0)) break;
                 const float fk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), from));
                 o0 += fk * v[k].x;
@@ -1120,20 +1127,76 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs
         }
     }
     sum = wave_sum(sum);
-    if (J > 1) {
-        o[wid][0][lane] = o0;
-        o[wid][1][lane] = o1;
-        __syncthreads();
-        if (wid > 0) return;
+    o[wid][0][lane] = o0;
+    o[wid][1][lane] = o1;
+    __syncthreads();
+    if (wid > 0 || 2 * lane >= a.Dh) return;
 #pragma unroll
-        for (int w4 = 1; w4 < J; w4++) {
-            o0 += o[w4][0][lane];
-            o1 += o[w4][1][lane];
-        }
+    for (int w4 = 1; w4 < kWaves; w4++) {
+        o0 += o[w4][0][lane];
+        o1 += o[w4][1][lane];
     }
-    if (2 * lane >= a.Dh) return;
     const float y = sum == 0.f ? 0.f : 1.f / sum;
     *reinterpret_cast<half2_t *>(out) = half2_t{f2h(o0 * y), f2h(o1 * y)};
+}
+
+// The same for many rows: a row to 32 lanes, four columns to a lane, 8 rows of a tile and key head to a workgroup, of a prompt's 32
+// (tiles numbered as they are in a batch of any lengths: most workgroups of a launch find nothing to do, and looking takes 2 us).
+constexpr int kJoinRows = 8, kBigJoinRows = 32;
+template <int NR>
+__global__ void __launch_bounds__(kThreads) paged_attention_join_tiles_kernel(AttnArgs a, Units big, Units few)
+{
+    constexpr int kRows = 16 * NR;
+    const PagedBatch &pb = a.pb;
+    const int lane = threadIdx.x & 63, h = blockIdx.y;
+    constexpr int kBigCut = kPrompt / kBigJoinRows, kCut = kRows / kJoinRows;
+    const int64_t bigs = big.count * kBigCut, x = blockIdx.x < bigs ? blockIdx.x : blockIdx.x - bigs;
+    const bool prompts = blockIdx.x < bigs;
+    const int cut = prompts ? kBigCut : kCut, per = prompts ? kBigJoinRows : kJoinRows, part_of = (int)(x % cut);
+    int tile;
+    const int b = uniform(prompts ? big.find(pb, x / cut, &tile) : few.find(pb, x / cut, &tile));
+    tile = uniform(tile);
+    if (b >= pb.B) return;
+    const Sequence s = sequence(pb, b, (int64_t)pb.W * pb.page, a.max_new);
+    const int tile_rows = prompts ? kPrompt : kRows, rows = s.n * a.G, row0 = tile * tile_rows, here = min(tile_rows, rows - row0);
+    if (s.s0 < 0 || s.n <= 0 || s.s0 > pb.T - s.n || tile < 0 || here <= 0) return;
+    auto out_of = [&](int r) { return a.out + (int64_t)(s.s0 + r / a.G) * a.ldo + (h * a.G + r % a.G) * a.Dh; };
+    const int d = 4 * (lane & 31), r = per * part_of + 2 * (int)(threadIdx.x >> 6) + (lane >> 5);
+    if (per * part_of >= here) return;
+    if (!s.ok) {
+        if (!prompts && r < here && d < a.Dh) *reinterpret_cast<half4_t *>(out_of(row0 + r) + d) = half4_t{};
+        if (threadIdx.x == 0) report(pb, b);
+        return;
+    }
+    if (prompts != (rows > a.few)) return;
+    double all = 0., some = 0.;
+    for (int b0 = 0; b0 < pb.B; b0 += 64) {
+        const Sequence q = lane_sequence(a, b0);
+        const double u = prompts ? BigShare(a, q).units(a) : Share(a, kRows, q).units;
+        all += u;
+        some += b0 + lane < b ? u : 0.;
+    }
+    const Parts in(a, s, kRows, h, tile, uniform((int)(unsigned)wave_sum_f64(all)), uniform((int)(unsigned)wave_sum_f64(some)));
+    if (in.count == 1) return;
+    const float *part = prompts ? a.big_part : a.part, *stats = prompts ? a.big_stats : a.stats;
+    for (int k = 0; k < per && per * part_of + k < here; k += 2 * kWaves) {
+        const int row = min(r + k, here - 1);
+        float m = -INFINITY, sum = 0.f;
+        float4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int p = 0; p < in.count; p++) {
+            const int64_t at = (int64_t)in.slot(p) * tile_rows + row;
+            const float2 st = *reinterpret_cast<const float2 *>(stats + 2 * at);
+            const float4_t v = *reinterpret_cast<const float4_t *>(part + at * a.Dh + min(d, a.Dh - 4));
+            const float mn = fmaxf(m, st.x), origin = finite_max(mn), f = exp2_of(m - origin), fp = exp2_of(st.x - origin);
+            m = mn;
+            sum = sum * f + st.y * fp;
+            o = o * f + v * fp;
+        }
+        const float y = sum == 0.f ? 0.f : 1.f / sum;
+        if (r + k < here && d < a.Dh)
+            *reinterpret_cast<half4_t *>(out_of(row0 + r + k) + d) = half4_t{f2h(o[0] * y), f2h(o[1] * y), f2h(o[2] * y), f2h(o[3] * y)};
+    }
 }
 
 struct Plan {
@@ -1146,20 +1209,31 @@ struct Plan {
 // Rows of a sequence (tokens by the query heads of a key head) that are a prompt's: from there on a workgroup of 128 of them reads
 // the keys fewer times than waves of 32 do
 constexpr int kFew = 64;
-Plan plan(int64_t T, int64_t H, int64_t Hkv, int64_t Dh, int64_t max_new, int bytes)
+Plan plan(int64_t T, int64_t B, int64_t H, int64_t Hkv, int64_t Dh, int64_t max_new, int bytes)
 {
     const int64_t G = H / Hkv, rows = (max_new < T ? max_new : T) * G;
     const int NR = rows <= 16 ? 1 : 2;
-    if (rows > kFew) return {2, 2 * kWaves * device_cus(), kFew, 2 * device_cus()};
+    if (rows > kFew) return {2, 2 * kWaves * device_cus(), B == 1 ? 0 : kFew, 2 * device_cus()};
     return {NR, resident(Dh <= 64 ? 1 : 2, NR, bytes) * kWaves * device_cus(), INT32_MAX, 0};
 }
 
+// Tiles of `rows` rows of the key heads' queries
+Units tiles_of(const AttnArgs &a, int rows)
+{
+    const int tokens = rows >= a.G ? rows / a.G : 1;           // whole ones of a tile; more tiles than it takes where G does not divide it
+    const int64_t most = ((int64_t)a.max_new * a.G + rows - 1) / rows;
+    return a.G > rows ? Units{(int)most, 1, 1, most * a.pb.B} : make_units(a.pb.T, a.pb.B, tokens, 1, most);
+}
 template <int NR>
 int launch_join(const AttnArgs &a, hipStream_t st)
 {
     const int64_t rh = (int64_t)a.pb.T * a.H;
-    if (rh < 4 * device_cus()) hipLaunchKernelGGL((paged_attention_join_kernel<NR, kWaves>), dim3((unsigned)rh), dim3(kThreads), 0, st, a);
-    else hipLaunchKernelGGL((paged_attention_join_kernel<NR, 1>), dim3((unsigned)((rh + kWaves - 1) / kWaves)), dim3(kThreads), 0, st, a);
+    if (rh < 4 * device_cus()) hipLaunchKernelGGL(paged_attention_join_kernel<NR>, dim3((unsigned)rh), dim3(kThreads), 0, st, a);
+    else {
+        const Units few = tiles_of(a, 16 * NR), big = a.big_groups ? tiles_of(a, kPrompt) : Units{1, 1, 1, 0};
+        const int64_t grid = few.count * (16 * NR / kJoinRows) + big.count * (kPrompt / kBigJoinRows);
+        hipLaunchKernelGGL(paged_attention_join_tiles_kernel<NR>, dim3((unsigned)grid, (unsigned)a.Hkv), dim3(kThreads), 0, st, a, big, few);
+    }
     return launch_status("paged_attention (parts)");
 }
 template <int ND, int NR, class P>
@@ -1172,9 +1246,10 @@ int launch(const AttnArgs &a, hipStream_t st)
 template <int ND, class P>
 int launch_prompts(const AttnArgs &a, hipStream_t st)
 {
-    hipLaunchKernelGGL((paged_prompt_kernel<ND, P>), dim3((unsigned)a.big_groups), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((paged_prompt_kernel<ND, P>), dim3((unsigned)a.big_groups), dim3(kBigThreads), 0, st, a);
     const int rc = launch_status("paged_attention (prompts)");
-    return rc ? rc : launch_join<2>(a, st);
+    if (rc) return rc;
+    return a.few > 0 ? launch<ND, 2, P>(a, st) : launch_join<2>(a, st);        // (one sequence: there are no others)
 }
 template <class P>
 int launch(const AttnArgs &a, int NR, hipStream_t st)
@@ -1189,7 +1264,7 @@ int launch(const AttnArgs &a, int NR, hipStream_t st)
 CACTI_API size_t cacti_hip_paged_attention_workspace(int64_t T, int64_t B, int64_t H, int64_t Hkv, int64_t Dh, int64_t max_new)
 {
     if (T <= 0 || B <= 0 || H <= 0 || Hkv <= 0 || Dh <= 0 || max_new <= 0 || H % Hkv) return 0;
-    const Plan p = plan(T, H, Hkv, Dh, max_new, 1);        // (of 16 bits: no more)
+    const Plan p = plan(T, B, H, Hkv, Dh, max_new, 1);        // (of 16 bits: no more)
     return p.floats(Dh) * 4;
 }
 
@@ -1211,11 +1286,11 @@ CACTI_API int cacti_hip_paged_attention_f16(int64_t T, int64_t B, int64_t H, int
     const int64_t most = (max_new < T ? max_new : T) * (H / Hkv) / 16 + 1;         // tiles of a sequence; work is counted in 32 bits
     CACTI_REQUIRE(T * H < (1 << 24) && (most < T * (H / Hkv) / 16 + B ? most * B : T * (H / Hkv) / 16 + B) * Hkv <
                       INT32_MAX / (W * page / kStep + 1 + begin_of(32)), CACTI_E_NOTIMPL, "paged_attention: too many rows and positions in one call");
-    const Plan p = plan(T, H, Hkv, Dh, max_new, bits / 8);
+    const Plan p = plan(T, B, H, Hkv, Dh, max_new, bits / 8);
     float *part = (float *)workspace;
     const size_t small = (size_t)p.groups * 2 * (16 * p.NR);
     const AttnArgs a = {pb, (int)H, (int)Hkv, (int)(H / Hkv), (int)Dh, padded_dim((int)Dh), (int)(max_new < T ? max_new : T), p.groups,
-                        (unsigned)((1 << 22) / page + 1), alpha, (const half_t *)q, ldq, k_pages, v_pages, (const float *)k_scale,
+                        (unsigned)((1 << 22) / page + 1), fabsf(alpha), alpha < 0.f ? 0x80008000u : 0u, (const half_t *)q, ldq, k_pages, v_pages, (const float *)k_scale,
                         (const float *)v_scale, (half_t *)out, ldo, part, part + small * Dh, p.few, p.big_groups,
                         part + small * (Dh + 2), part + small * (Dh + 2) + (size_t)p.big_groups * 2 * kPrompt * Dh};
     return bits == 8 ? launch<uint8_t>(a, p.NR, (hipStream_t)stream) : launch<half_t>(a, p.NR, (hipStream_t)stream);
