@@ -704,7 +704,7 @@ struct BigShare {
     __device__ __forceinline__ unsigned units(const AttnArgs &a) const { return before(tiles) * (unsigned)a.Hkv; }
 };
 
-constexpr int kBigThreads = 512, kBigWaves = kBigThreads / 64;
+constexpr int kBigThreads = 256, kBigWaves = kBigThreads / 64;
 
 template <int ND, class P>
 struct Prompt {
@@ -712,7 +712,9 @@ struct Prompt {
     static constexpr int kHalf = kBigThreads / 2;                          // lanes that load keys, and that load values
     static constexpr int kPer = 64 * ND * (int)sizeof(P) / 16;             // 16-byte pieces of a key
     static constexpr int kPieces = kBig * kPer / kHalf;                    // of a lane
+    static constexpr int kApart = kHalf / kPer;                            // keys from one to the next
     static constexpr int kCols = 16 * ND;                                  // lanes that have a key's columns, four each, of V
+    static constexpr int kBlocks = ND, kKeys = kBig / kBlocks;             // blocks of V of a lane, kKeys positions apart
     struct Shared {
         half_t k[2][kBig][64 * ND], v[2][64 * ND][kBig];
         Entry entry;
@@ -720,14 +722,14 @@ struct Prompt {
     };
     const AttnArgs &a;
     Shared &sh;
-    half8_t q[NS];
-    int last;
-    float m, l;
-    float4_t o[4 * ND];
-    // the next 64 positions, as they come: keys (waves 4 to 7) or values (waves 0 to 3; ND 1: 0 and 1)
+    half8_t q[2][NS];
+    int last[2];
+    float m[2], l[2];
+    float4_t o[2][4 * ND];
+    // the next 64 positions, as they come: keys (waves 2 and 3) or values
     union {
         u4_t k[kPieces];
-        VBlock<P, 4> v;
+        VBlock<P, 4> v[kBlocks];
     } next;
 
     __device__ __forceinline__ int page_of(int x) const { return (int)(__umul24((unsigned)x, a.page_magic) >> 22); }
@@ -742,7 +744,7 @@ struct Prompt {
         return (const P *)pages + uni + (int64_t)((x - pg * a.pb.page) * a.Dp);
     }
     // What of the addresses is a lane's own: its row and columns in memory, elements from the wave's first row, and its place in
-    // LDS, halves from a buffer's start (keys: piece i is 16 rows on, whose swap has another bit 2, or 32; values: column 0 of 4)
+    // LDS, halves from a buffer's start (keys: of the first piece; values: of column 0 of 4)
     struct Own {
         unsigned from;
         int to;
@@ -769,33 +771,39 @@ struct Prompt {
             const int first = 64 * (wid - kBigWaves / 2) / kPer;
             if (x + kBig <= end) {
 #pragma unroll
-                for (int i = 0; i < kPieces; i++)
-                    next.k[i] = *reinterpret_cast<const u4_t *>(page_at(a.k_pages, x + first + i * (kHalf / kPer)) + w.from);
+                for (int i = 0; i < kPieces; i++) next.k[i] = *reinterpret_cast<const u4_t *>(page_at(a.k_pages, x + first + i * kApart) + w.from);
                 return;
             }
             const int lane = lane_here();
 #pragma unroll
             for (int i = 0; i < kPieces; i++) {
-                const int j = min(x + first + i * (kHalf / kPer) + lane / kPer, end - 1), pg = page_of(j);
+                const int j = min(x + first + i * kApart + lane / kPer, end - 1), pg = page_of(j);
                 const P *row = (const P *)a.k_pages + sh.entry.at[pg] + __umul24(j - __umul24(pg, a.pb.page), a.Dp);
                 next.k[i] = *reinterpret_cast<const u4_t *>(row + min(lane % kPer * (16 / (int)sizeof(P)), a.Dp - 16 / (int)sizeof(P)));
             }
-        } else if (ND == 2 || wid < 2) {
+        } else {
             const int first = 8 * (64 / kCols) * wid;          // 16 positions to a wave or, ND 1, 32
             if (x + kBig <= end) {
-                const P *v = page_at(a.v_pages, x + first);
-                if (ND == 1) {
-                    const P *v1 = page_at(a.v_pages, x + first + 16);
-                    v = (threadIdx.x & 32) ? v1 : v;
-                }
 #pragma unroll
-                for (int i = 0; i < 8; i++) next.v.load(i, v + i * a.Dp + w.from);
+                for (int k = 0; k < kBlocks; k++) {
+                    const P *v = page_at(a.v_pages, x + first + k * kKeys);
+                    if (ND == 1) {
+                        const P *v1 = page_at(a.v_pages, x + first + 16);
+                        v = (threadIdx.x & 32) ? v1 : v;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; i++) next.v[k].load(i, v + i * a.Dp + w.from);
+                }
                 return;
             }
-            const int lane = lane_here(), j0 = x + first + 8 * (lane / kCols), pg = page_of(min(j0, end - 1));
-            const P *row = (const P *)a.v_pages + sh.entry.at[pg] + min(4 * (lane % kCols), a.Dp - 4);
+            const int lane = lane_here();
 #pragma unroll
-            for (int i = 0; i < 8; i++) next.v.load(i, row + __umul24(min(j0 + i, end - 1) - __umul24(pg, a.pb.page), a.Dp));
+            for (int k = 0; k < kBlocks; k++) {
+                const int j0 = x + first + k * kKeys + 8 * (lane / kCols), pg = page_of(min(j0, end - 1));
+                const P *row = (const P *)a.v_pages + sh.entry.at[pg] + min(4 * (lane % kCols), a.Dp - 4);
+#pragma unroll
+                for (int i = 0; i < 8; i++) next.v[k].load(i, row + __umul24(min(j0 + i, end - 1) - __umul24(pg, a.pb.page), a.Dp));
+            }
         }
     }
     // ... into buffer `to`; least: positions up to there are seen by every row of the tile
@@ -814,25 +822,29 @@ struct Prompt {
                     Frag f;
 #pragma unroll
                     for (int w = 0; w < 4; w++) f.u[w] = sizeof(P) == 2 ? next.k[i][w] : cvt8(next.k[i][2 * k + w / 2], w & 1);
-                    *reinterpret_cast<half8_t *>(kb + (own.to ^ (8 * k) ^ (kHalf / kPer == 16 ? 32 * (i & 1) : 0)) + i * (kHalf / kPer) * 64 * ND) = f.h;
+                    *reinterpret_cast<half8_t *>(kb + (own.to ^ (8 * k) ^ 8 * (i * kApart / 4 & 7)) + i * kApart * 64 * ND) = f.h;
                 }
-        } else if (ND == 2 || wid < 2) {
-            if (x + kBig - 1 > min(least, end - 1)) {
-                const int j0 = x + 8 * ((64 * wid + lane_here()) / kCols);
-                bool any = false;
+        } else {
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    if (j0 + i >= end) next.v.zero(i);
-                    else if (j0 + i > least) any = next.v.strip(i) || any;
+            for (int b = 0; b < kBlocks; b++) {
+                VBlock<P, 4> &v = next.v[b];
+                if (x + kBig - 1 > min(least, end - 1)) {
+                    const int j0 = x + b * kKeys + 8 * ((64 * wid + lane_here()) / kCols);
+                    bool any = false;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        if (j0 + i >= end) v.zero(i);
+                        else if (j0 + i > least) any = v.strip(i) || any;
+                    }
+                    if (any) sh.odd = 1;
                 }
-                if (any) sh.odd = 1;
-            }
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
-                half8_t v0, v1;
-                next.v.columns(c, &v0, &v1);
-                *reinterpret_cast<half8_t *>(vb + (own.to ^ (16 * c)) + 2 * c * kBig) = v0;             // swap_of(d + e) = swap_of(d) ^ e
-                *reinterpret_cast<half8_t *>(vb + (own.to ^ (16 * c + 8)) + (2 * c + 1) * kBig) = v1;
+                for (int c = 0; c < 2; c++) {
+                    half8_t v0, v1;
+                    v.columns(c, &v0, &v1);
+                    *reinterpret_cast<half8_t *>(vb + (own.to ^ b * kKeys ^ (16 * c)) + 2 * c * kBig) = v0;            // swap_of(d + e) = swap_of(d) ^ e
+                    *reinterpret_cast<half8_t *>(vb + (own.to ^ b * kKeys ^ (16 * c + 8)) + (2 * c + 1) * kBig) = v1;
+                }
             }
         }
     }
@@ -854,28 +866,39 @@ struct Prompt {
     {
         const int lane = threadIdx.x & 63, g = lane >> 4;
         const half_t *kb = &sh.k[from][0][0] + 32 * b * 64 * ND, *vb = &sh.v[from][0][0];
-        float4_t sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        float4_t sc[2][2] = {};
 #pragma unroll
         for (int c = 0; c < NS; c++)
 #pragma unroll
-            for (int t = 0; t < 2; t++)
-                sc[t] = mfma(*reinterpret_cast<const half8_t *>(kb + (at.k ^ (40 * t) ^ (32 * (c & 1))) + 4 * t * 64 * ND + (c >> 1) * 64), q[c], sc[t]);
+            for (int t = 0; t < 2; t++) {
+                const half8_t k = *reinterpret_cast<const half8_t *>(kb + (at.k ^ (40 * t) ^ (32 * (c & 1))) + 4 * t * 64 * ND + (c >> 1) * 64);
+#pragma unroll
+                for (int n = 0; n < 2; n++) sc[n][t] = mfma(k, q[n][c], sc[n][t]);
+            }
         const int pg = page_of(min(x + 8 * g, end - 1));
-        const half8_t p = weigh(sc, sh.entry.c[pg], sh.entry.lg[pg], sh.entry.iv[pg], m, l, o, x + 31 > min(least, end - 1),
-                                min(last - base, end - 1) - (x + 8 * g) + 1);
+        const bool edge = x + 31 > min(least, end - 1);
+        half8_t p[2];
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+            p[n] = weigh(sc[n], sh.entry.c[pg], sh.entry.lg[pg], sh.entry.iv[pg], m[n], l[n], o[n], edge, min(last[n] - base, end - 1) - (x + 8 * g) + 1);
         const int v0 = at.v ^ (32 * b);
 #pragma unroll
-        for (int c = 0; c < 4 * ND; c++) o[c] = mfma(*reinterpret_cast<const half8_t *>(vb + (v0 ^ (32 * (c & 1))) + 16 * c * kBig), p, o[c]);
+        for (int c = 0; c < 4 * ND; c++) {
+            const half8_t v = *reinterpret_cast<const half8_t *>(vb + (v0 ^ (32 * (c & 1))) + 16 * c * kBig);
+#pragma unroll
+            for (int n = 0; n < 2; n++) o[n][c] = mfma(v, p[n], o[n][c]);
+        }
     }
 
     // positions c0 .. c1 - 1 (some) of rows row0 .. of sequence s
     __device__ __forceinline__ void run(int b, const Sequence &s, int h, int rows, int row0, int c0, int c1)
     {
         const int wid = uniform((int)threadIdx.x >> 6), lane = lane_here(), tid = 64 * wid + lane, r16 = lane & 15, g = lane >> 4;
-        const int mine = row0 + 16 * wid;      // the wave's first row
-        {
-            const int r = min(mine + r16, rows - 1), t = r / a.G;
-            last = s.first + t;
+        const int mine = row0 + 32 * wid;      // the wave's first row
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+            const int r = min(mine + 16 * n + r16, rows - 1), t = r / a.G;
+            last[n] = s.first + t;
             const half_t *qr = a.q + (int64_t)(s.s0 + t) * a.ldq + (h * a.G + r - t * a.G) * a.Dh;
 #pragma unroll
             for (int c = 0; c < NS; c++) {
@@ -887,15 +910,15 @@ struct Prompt {
                     f.u[2 * j] = d < a.Dh ? w[0] ^ a.sign : 0u;
                     f.u[2 * j + 1] = d < a.Dh ? w[1] ^ a.sign : 0u;
                 }
-                q[c] = f.h;
+                q[n][c] = f.h;
             }
-            m = -INFINITY;
-            l = 0.f;
+            m[n] = -INFINITY;
+            l[n] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4 * ND; i++) o[i] = float4_t{0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < 4 * ND; i++) o[n][i] = float4_t{0.f, 0.f, 0.f, 0.f};
         }
         const int least = uniform(s.first + row0 / a.G);                               // seen by every row of the tile
-        const int wave_least = uniform(s.first + min(mine, rows - 1) / a.G), wave_last = uniform(mine < rows ? s.first + (min(mine + 16, rows) - 1) / a.G : -1);
+        const int wave_least = uniform(s.first + min(mine, rows - 1) / a.G), wave_last = uniform(mine < rows ? s.first + (min(mine + 32, rows) - 1) / a.G : -1);
         const Places at = places();
         const Own w = own();
         for (int seg = c0; seg < c1;) {
@@ -949,35 +972,40 @@ struct Prompt {
                     x.load(0, v + min(16 * c + 4 * g, a.Dp - 4));
 #pragma unroll
                     for (int i = 0; i < 4; i++)
-                        if (!(fabsf(x.value(i)) < INFINITY) && j <= last) o[c][i] += x.value(i);
+#pragma unroll
+                        for (int n = 0; n < 2; n++)
+                            if (!(fabsf(x.value(i)) < INFINITY) && j <= last[n]) o[n][c][i] += x.value(i);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
         }
-        const float sum = with32(with16(l, OpSum()), OpSum());
-        const int r = row0 + 16 * wid + r16, t = r / a.G;
-        if (r >= rows) return;
-        const float y = slot >= 0 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
-        const int64_t at = (int64_t)slot * kPrompt + r - row0;
-        half_t *out = a.out + (int64_t)(s.s0 + t) * a.ldo + (h * a.G + r - t * a.G) * a.Dh;
-        float *part = a.big_part + at * a.Dh;
 #pragma unroll
-        for (int c = 0; c < 4 * ND; c++) {
-            const int d = 16 * c + 4 * g;
-            if (d >= a.Dh) continue;
-            const float4_t v = o[c] * y;
-            if (slot >= 0) *reinterpret_cast<float4_t *>(part + d) = v;
-            else *reinterpret_cast<half4_t *>(out + d) = half4_t{f2h(v[0]), f2h(v[1]), f2h(v[2]), f2h(v[3])};
-        }
-        if (slot >= 0 && g == 0) {
-            a.big_stats[2 * at] = m;
-            a.big_stats[2 * at + 1] = sum;
+        for (int n = 0; n < 2; n++) {
+            const float sum = with32(with16(l[n], OpSum()), OpSum());
+            const int r = row0 + 32 * wid + 16 * n + r16, t = r / a.G;
+            if (r >= rows) continue;
+            const float y = slot >= 0 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+            const int64_t at = (int64_t)slot * kPrompt + r - row0;
+            half_t *out = a.out + (int64_t)(s.s0 + t) * a.ldo + (h * a.G + r - t * a.G) * a.Dh;
+            float *part = a.big_part + at * a.Dh;
+#pragma unroll
+            for (int c = 0; c < 4 * ND; c++) {
+                const int d = 16 * c + 4 * g;
+                if (d >= a.Dh) continue;
+                const float4_t v = o[n][c] * y;
+                if (slot >= 0) *reinterpret_cast<float4_t *>(part + d) = v;
+                else *reinterpret_cast<half4_t *>(out + d) = half4_t{f2h(v[0]), f2h(v[1]), f2h(v[2]), f2h(v[3])};
+            }
+            if (slot >= 0 && g == 0) {
+                a.big_stats[2 * at] = m[n];
+                a.big_stats[2 * at + 1] = sum;
+            }
         }
     }
 };
 
 template <int ND, class P>
-__global__ void __launch_bounds__(kBigThreads, 4) paged_prompt_kernel(AttnArgs a)
+__global__ void __launch_bounds__(kBigThreads, 2) paged_prompt_kernel(AttnArgs a)
 {
     __shared__ typename Prompt<ND, P>::Shared sh;
     const int lane = threadIdx.x & 63;
@@ -1022,7 +1050,7 @@ __global__ void __launch_bounds__(kBigThreads, 4) paged_prompt_kernel(AttnArgs a
             const int end = uniform(s.first + min(rows - 1, row0 + kPrompt - 1) / a.G + 1);
             const int first = max(from - kBigBegin, 0), behind_last = to - kBigBegin;
             if (behind_last > first) {
-                const int c0 = first * kBig, c1 = min(end, behind_last * kBig);
+                const int c0 = uniform(first * kBig), c1 = uniform(min(end, behind_last * kBig));
                 Prompt<ND, P> t{a, sh};
                 t.run(b, s, h, rows, row0, c0, c1);
                 t.write(b, s, h, rows, row0, c0, c1, first == 0 && behind_last == (int)whole - kBigBegin ? -1 : 2 * (int)group + (first == 0));
