@@ -5,16 +5,15 @@
 //   dz_j = scale / tau (p_j sum(t) - sum_{i: idx_i = j} t_i)
 // An entry of -inf has no weight (padding); a row of none but such has loss 0 and gradient 0.
 //
-// Forward: one pass for the maximum, one for the sum (out of L2).  It keeps both per row (stats), so that the gradient is a
-// stream over the logits: nothing to reduce, one fma and one exponential per element.  The K entries are written again
-// afterwards by the same workgroup, behind its barrier.
+// A workgroup to a row, which it holds in registers from one read on: the forward pass is bound by that read, the adjoint, which
+// takes the maximum and the sum from the forward pass (stats) and has nothing to reduce over the row, by a read and a write.
+// 2048 rows of 32000, K = 64: forward FWD us (a maximum and then a sum out of memory again: 55), adjoint BWD us.
 #include "vocab_row.h"
 
 using namespace cacti;
 
 namespace {
 
-constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kMaxK = 1024;
 
 struct DistillArgs {
@@ -31,142 +30,263 @@ struct DistillArgs {
     int *status;
 };
 
-// The teacher's K probabilities of a row by thread i (i, i + kThreads): max and sum of exponentials over the block
-struct Teacher {
-    float mx, sum;
-};
-__device__ __forceinline__ Teacher teacher(const DistillArgs &a, int64_t n, float *red)
-{
-    const half_t *v = a.val + n * a.K;
-    Teacher t;
-    float m = -INFINITY;
-    bool nan = false;
-    for (int i = threadIdx.x; i < a.K; i += kThreads) {
-        m = fmaxf(m, h2f(v[i]));
-        nan = nan || v[i] != v[i];
+// A row of up to 8 T NP + 7 elements, held by T threads: of its whole 16-byte pieces those lo + tid + i T, and of up to 14
+// elements beside them one for each of the first threads.
+template <int T, int NP>
+struct Held {
+    int lo, hi, edge;                          // whole pieces lo .. hi - 1; the element, or -1
+    half8_t x[NP];
+    half_t e;
+    __device__ __forceinline__ Held(const VocabRow &z) : lo(z.off > 0), hi(max((z.V + z.off) / 8, lo))
+    {
+        const int head = lo ? min(8 - z.off, z.V) : 0, tail = max(8 * hi - z.off, head), j = (int)threadIdx.x < head ? (int)threadIdx.x : tail + (int)threadIdx.x - head;
+        edge = threadIdx.x < 16 && j < z.V ? j : -1;
     }
-    t.mx = block_reduce(m, OpMax(), -INFINITY, red);
-    float s = 0.f;
-    if (t.mx > -INFINITY)
-        for (int i = threadIdx.x; i < a.K; i += kThreads) s += expf((float)(((double)h2f(v[i]) - (double)t.mx) * a.inv_temp));
-    if (nan) s = NAN;
-    t.sum = block_reduce(s, OpSum(), 0.f, red);
-    return t;
+    __device__ __forceinline__ bool has(int i) const { return lo + (int)threadIdx.x + i * T < hi; }
+    __device__ __forceinline__ int piece(int i) const { return min(lo + (int)threadIdx.x + i * T, hi - 1); }
+    __device__ __forceinline__ void load(const VocabRow &z)                // (what it does not have is some other of the row)
+    {
+        e = z.row[max(edge, 0)];
+        if (hi > lo)
+#pragma unroll
+            for (int i = 0; i < NP; i++) x[i] = *reinterpret_cast<const half8_t *>(z.row + z.first(piece(i)));
+    }
+};
+
+// The teacher's entries of a thread: tid, tid + T, ...
+template <int T>
+struct Entries {
+    static constexpr int kOf = kMaxK / T;
+    half_t v[kOf], z[kOf];                     // the teacher's logit (-inf behind the last) and the student's
+    int j[kOf];
+    __device__ __forceinline__ void load(const DistillArgs &a, int64_t n, const half_t *row)
+    {
+#pragma unroll
+        for (int e = 0; e < kOf; e++) {
+            v[e] = z[e] = (half_t)-INFINITY;
+            j[e] = a.V;
+            if (e > 0 && e * T >= a.K) continue;
+            const int i = (int)threadIdx.x + e * T, ic = min(i, a.K - 1);
+            const half_t x = a.val[n * a.K + ic];
+            j[e] = a.idx[n * a.K + ic];
+            z[e] = row[min(j[e], a.V - 1)];
+            v[e] = i < a.K ? x : (half_t)-INFINITY;
+            j[e] = i < a.K ? j[e] : -1;
+        }
+    }
+    __device__ __forceinline__ float max() const
+    {
+        float m = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < kOf; e++) m = fmaxf(m, h2f(v[e]));
+        return m;
+    }
+    // e^((v - mx) / tau); mx = -inf: there is none but -inf and NaN
+    __device__ __forceinline__ float weight(int e, float mx, double inv_temp) const
+    {
+        if (mx == -INFINITY) return v[e] != v[e] ? NAN : 0.f;
+        return expf((float)(((double)h2f(v[e]) - (double)mx) * inv_temp));
+    }
+};
+
+template <int T>
+__device__ __forceinline__ void block_max2(float &x, float &y)
+{
+    __shared__ float red[T / 64][2];
+    x = wave_reduce(x, OpMax());
+    y = wave_reduce(y, OpMax());
+    if ((threadIdx.x & 63) == 0) {
+        red[threadIdx.x >> 6][0] = x;
+        red[threadIdx.x >> 6][1] = y;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < T / 64; w++) {
+        x = fmaxf(x, red[w][0]);
+        y = fmaxf(y, red[w][1]);
+    }
 }
 
-__global__ void __launch_bounds__(kThreads) distill_fwd_kernel(DistillArgs a)
+template <int T, int NP>
+__global__ void __launch_bounds__(T) distill_fwd_kernel(DistillArgs a)
 {
-    __shared__ float red[kWaves];
-    __shared__ double redd[kWaves];
+    __shared__ float sums[T / 64][3];
+    __shared__ double parts[T / 64];
     const int64_t n = blockIdx.x;
     const VocabRow z(a.logit + n * a.ld, a.V);
+    Entries<T> t;
+    Held<T, NP> h(z);
+    t.load(a, n, z.row);
+    h.load(z);
     const float c2 = (float)(a.inv_temp * 1.44269504088896340736);
-    float mx = -INFINITY;
-    for (int c = threadIdx.x; c < z.pieces(); c += kThreads) {
-        const h8 v = z.load(c, (half_t)-INFINITY);
+    if (h.edge < 0) h.e = (half_t)-INFINITY;
+    float mx = h2f(h.e), tmx = t.max();
+    if (h.hi > h.lo) {                         // (what a thread does not have is some other element of the row)
+        half8_t m8 = h.x[0];
 #pragma unroll
-        for (int k = 0; k < 8; k++) mx = fmaxf(mx, h2f(v.v[k]));
-    }
-    mx = block_reduce(mx, OpMax(), -INFINITY, red);
-    float s = 0.f;
-    for (int c = threadIdx.x; c < z.pieces(); c += kThreads) {
-        const h8 v = z.load(c, (half_t)-INFINITY);
+        for (int i = 1; i < NP; i++) m8 = __builtin_elementwise_max(m8, h.x[i]);
 #pragma unroll
-        for (int k = 0; k < 8; k++) s += __builtin_amdgcn_exp2f((h2f(v.v[k]) - mx) * c2);
+        for (int k = 0; k < 8; k++) mx = fmaxf(mx, h2f(m8[k]));
     }
-    const float sum = block_reduce(s, OpSum(), 0.f, red);
-    const Teacher t = teacher(a, n, red);
+    block_max2<T>(mx, tmx);
+    float s = __builtin_amdgcn_exp2f((h2f(h.e) - mx) * c2);
+    s = h.edge < 0 ? 0.f : s;
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+        float p = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) p += __builtin_amdgcn_exp2f((h2f(h.x[i][k]) - mx) * c2);
+        s += h.has(i) ? p : 0.f;
+    }
     // log t_i - log p_i = ((val_i - val_max) - (z_i - z_max)) / tau + log(sum_z / sum_t)
-    const double shift = log((double)sum) - log((double)t.sum);
-    double loss = 0.;
-    for (int i = threadIdx.x; i < a.K; i += kThreads) {
-        const int j = a.idx[n * a.K + i];
-        if (j >= a.V) {
-            if (a.status) atomicMax(a.status, (int)min(n + 1, (int64_t)INT32_MAX));
-            continue;
-        }
-        const double dv = ((double)h2f(a.val[n * a.K + i]) - (double)t.mx) * a.inv_temp;
-        const float w = expf((float)dv) / t.sum;
-        if (w != 0.f) loss += (double)w * (dv - ((double)h2f(z.row[j]) - (double)mx) * a.inv_temp + shift);
+    float sum = 0.f, valid = 0.f;
+    double part = 0.;
+#pragma unroll
+    for (int e = 0; e < Entries<T>::kOf; e++) {
+        if (e * T >= a.K) break;
+        const float w = t.weight(e, tmx, a.inv_temp);
+        sum += w;
+        if (t.j[e] >= a.V && a.status) atomicMax(a.status, (int)min(n + 1, (int64_t)INT32_MAX));
+        if (t.j[e] >= a.V || w == 0.f) continue;
+        valid += w;
+        part += (double)w * (((double)h2f(t.v[e]) - (double)tmx) * a.inv_temp - ((double)h2f(t.z[e]) - (double)mx) * a.inv_temp);
     }
-    loss = wave_sum_f64(loss);
-    if ((threadIdx.x & 63) == 0) redd[threadIdx.x >> 6] = loss;
+    s = wave_sum(s);
+    sum = wave_sum(sum);
+    valid = wave_sum(valid);
+    part = wave_sum_f64(part);
+    if ((threadIdx.x & 63) == 0) {
+        const int w = threadIdx.x >> 6;
+        sums[w][0] = s;
+        sums[w][1] = sum;
+        sums[w][2] = valid;
+        parts[w] = part;
+    }
     __syncthreads();
     if (threadIdx.x == 0) {
-        double l = 0.;
-        for (int w = 0; w < kWaves; w++) l += redd[w];
-        a.loss[n] = t.mx == -INFINITY && t.sum == 0.f ? 0.f : (float)l;
+        s = sum = valid = 0.f;
+        part = 0.;
+#pragma unroll
+        for (int w = 0; w < T / 64; w++) {
+            s += sums[w][0];
+            sum += sums[w][1];
+            valid += sums[w][2];
+            part += parts[w];
+        }
+        a.loss[n] = valid == 0.f && sum == sum ? 0.f : (float)((part + (double)valid * (log((double)s) - log((double)sum))) / (double)sum);
         a.stats[2 * n] = mx;
-        a.stats[2 * n + 1] = sum;
+        a.stats[2 * n + 1] = s;
     }
 }
 
 __device__ __forceinline__ half_t combined(float d, int acc, half_t old) { return acc ? f2h(h2f(old) + rnd16(d)) : f2h(d); }
 
-__global__ void __launch_bounds__(kThreads) distill_bwd_kernel(DistillArgs a)
+template <int T, int NP>
+__global__ void __launch_bounds__(T) distill_bwd_kernel(DistillArgs a)
 {
-    __shared__ float red[kWaves];
-    __shared__ uint16_t ids[kMaxK];
-    __shared__ float ts[kMaxK];
+    constexpr int kOf = Entries<T>::kOf;
+    __shared__ float sums[T / 64][2];
+    __shared__ int ids[kMaxK];
+    __shared__ float es[kMaxK];
     const int64_t n = blockIdx.x;
-    const VocabRow z(a.logit + n * a.ld, a.V);
+    const VocabRow z(a.logit + n * a.ld, a.V), g(a.grad + n * a.ldd, a.V);
     half_t *gr = a.grad + n * a.ldd;
-    const float c2 = (float)(a.inv_temp * 1.44269504088896340736), sc = (float)(a.scale[n] * a.inv_temp);
-    const float mx = a.stats[2 * n], inv = 1.f / a.stats[2 * n + 1];
-    const Teacher t = teacher(a, n, red);
-    const bool empty = t.mx == -INFINITY && t.sum == 0.f;
-    for (int i = threadIdx.x; i < a.K; i += kThreads) {
-        const int j = a.idx[n * a.K + i];
-        ids[i] = (uint16_t)j;
-        ts[i] = j < a.V && !empty ? expf((float)(((double)h2f(a.val[n * a.K + i]) - (double)t.mx) * a.inv_temp)) / t.sum : 0.f;
+    Entries<T> t;
+    Held<T, NP> h(g);                          // the gradient's pieces
+    t.load(a, n, z.row);
+    const float mx = a.stats[2 * n], row_sum = a.stats[2 * n + 1], scale = a.scale[n];
+    // all that is read of the logits and, of other threads' pieces, of the gradient is read before anything is written
+    const bool same = z.off == g.off;
+    if (same) h.load(z);
+    half_t old[kOf];
+#pragma unroll
+    for (int e = 0; e < kOf; e++) {
+        old[e] = (half_t)0.f;
+        if (a.acc && e * T < a.K) old[e] = gr[min(max(t.j[e], 0), a.V - 1)];
     }
-    __syncthreads();
-    // the entries: the first of those with an id has them all, in order; what is there before is read before it is written over
-    half_t entry[(kMaxK + kThreads - 1) / kThreads];
-    int at[(kMaxK + kThreads - 1) / kThreads];
+    float tmx = t.max(), none = 0.f;
+    block_max2<T>(tmx, none);
+    float sum = 0.f, valid = 0.f;
 #pragma unroll
-    for (int e = 0; e < (kMaxK + kThreads - 1) / kThreads; e++) {
-        const int i = threadIdx.x + e * kThreads;
-        at[e] = -1;
-        if (i >= a.K || ids[i] >= a.V) continue;
-        float w = 0.f;
-        bool mine = true;
-        for (int k = 0; k < a.K; k++)
-            if (ids[k] == ids[i]) {
-                mine = mine && k >= i;
-                w += ts[k];
-            }
-        if (!mine) continue;
-        at[e] = ids[i];
-        const float p = empty ? 0.f : __builtin_amdgcn_exp2f((h2f(z.row[at[e]]) - mx) * c2) * inv;
-        entry[e] = combined(empty ? 0.f : sc * (p - w), a.acc, a.acc ? gr[at[e]] : (half_t)0.f);
-    }
-    __syncthreads();
-    const VocabRow g(gr, a.V);
-    for (int c = threadIdx.x; c < g.pieces(); c += kThreads) {
-        const int j0 = g.first(c);
-        h8 v, o;
-        if (g.whole(c) && z.off == g.off) v = ld8(z.row + j0);
-        else
-#pragma unroll
-            for (int k = 0; k < 8; k++) v.v[k] = j0 + k >= 0 && j0 + k < a.V ? z.row[j0 + k] : (half_t)0.f;
-        if (a.acc) o = g.load(c, (half_t)0.f);
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const float d = empty ? 0.f : sc * (__builtin_amdgcn_exp2f((h2f(v.v[k]) - mx) * c2) * inv);
-            o.v[k] = combined(d, a.acc, o.v[k]);
+    for (int e = 0; e < kOf; e++) {
+        if (e * T >= a.K) break;
+        const float w = t.weight(e, tmx, a.inv_temp);
+        sum += w;
+        if (t.j[e] < a.V) valid += w;
+        if ((int)threadIdx.x + e * T < a.K) {
+            ids[threadIdx.x + e * T] = t.j[e];
+            es[threadIdx.x + e * T] = w;
         }
-        if (g.whole(c)) st8(gr + j0, o);
-        else
-#pragma unroll
-            for (int k = 0; k < 8; k++)
-                if (j0 + k >= 0 && j0 + k < a.V) gr[j0 + k] = o.v[k];
+    }
+    sum = wave_sum(sum);
+    valid = wave_sum(valid);
+    if ((threadIdx.x & 63) == 0) {
+        sums[threadIdx.x >> 6][0] = sum;
+        sums[threadIdx.x >> 6][1] = valid;
     }
     __syncthreads();
+    sum = valid = 0.f;
 #pragma unroll
-    for (int e = 0; e < (kMaxK + kThreads - 1) / kThreads; e++)
-        if (at[e] >= 0) gr[at[e]] = entry[e];
+    for (int w = 0; w < T / 64; w++) {
+        sum += sums[w][0];
+        valid += sums[w][1];
+    }
+    const bool empty = valid == 0.f && sum == sum;
+    const float c2 = (float)(a.inv_temp * 1.44269504088896340736), sc = (float)(scale * a.inv_temp), inv = valid / sum / row_sum;
+    auto stream = [&](half_t x) __attribute__((always_inline)) { return empty ? 0.f : sc * (__builtin_amdgcn_exp2f((h2f(x) - mx) * c2) * inv); };
+    // the entries: the last of those with an id has them all, in order
+    half_t entry[kOf];
+    bool mine[kOf];
+#pragma unroll
+    for (int e = 0; e < kOf; e++) {
+        const int i = (int)threadIdx.x + e * T, j = t.j[e];
+        mine[e] = i < a.K && j < a.V;
+        if (!mine[e]) continue;
+        float w = 0.f;
+        for (int k = 0; k < a.K; k++)
+            if (ids[k] == j) {
+                mine[e] = mine[e] && k <= i;
+                w += es[k];
+            }
+        const float p = __builtin_amdgcn_exp2f((h2f(t.z[e]) - mx) * c2) * inv;
+        entry[e] = combined(empty ? 0.f : sc * (p - w / sum), a.acc, old[e]);
+    }
+    if (same)
+#pragma unroll
+        for (int i = 0; i < NP; i++) {
+            if (!h.has(i)) break;
+            half_t *to = gr + g.first(h.piece(i));
+            half8_t o = {};
+            if (a.acc) o = *reinterpret_cast<const half8_t *>(to);
+#pragma unroll
+            for (int k = 0; k < 8; k++) o[k] = combined(stream(h.x[i][k]), a.acc, o[k]);
+            *reinterpret_cast<half8_t *>(to) = o;
+        }
+    else
+        for (int c = h.lo + threadIdx.x; c < h.hi; c += T) {
+            const int j0 = g.first(c);
+            half8_t o = {};
+            if (a.acc) o = *reinterpret_cast<const half8_t *>(gr + j0);
+#pragma unroll
+            for (int k = 0; k < 8; k++) o[k] = combined(stream(z.row[j0 + k]), a.acc, o[k]);
+            *reinterpret_cast<half8_t *>(gr + j0) = o;
+        }
+    if (h.edge >= 0) gr[h.edge] = combined(stream(same ? h.e : z.row[h.edge]), a.acc, a.acc ? gr[h.edge] : (half_t)0.f);
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kOf; e++)
+        if (mine[e]) gr[t.j[e]] = entry[e];
 }
+
+// The least threads and registers that hold a row
+#define CACTI_DISTILL(kernel, a, st)                                                                                                  \
+    do {                                                                                                                              \
+        const dim3 grid((unsigned)(a).N);                                                                                             \
+        if ((a).V < 8 * 256 * 4 + 8) hipLaunchKernelGGL((kernel<256, 4>), grid, dim3(256), 0, st, a);                                 \
+        else if ((a).V < 8 * 512 * 4 + 8) hipLaunchKernelGGL((kernel<512, 4>), grid, dim3(512), 0, st, a);                            \
+        else if ((a).V < 8 * 512 * 8 + 8) hipLaunchKernelGGL((kernel<512, 8>), grid, dim3(512), 0, st, a);                            \
+        else hipLaunchKernelGGL((kernel<512, 16>), grid, dim3(512), 0, st, a);                                                        \
+    } while (0)
 
 int check(const char *who, int64_t N, int64_t V, int64_t K, const void *logit, int64_t ld, const void *idx, const void *val, const void *stats,
           double temperature, DistillArgs *a)
@@ -194,7 +314,7 @@ CACTI_API int cacti_hip_distill_topk_fwd(int64_t N, int64_t V, int64_t K, const 
     CACTI_REQUIRE(loss && aligned(loss, 4) && aligned(status, 4), CACTI_E_INVALID, "distill_topk_fwd: loss null or misaligned");
     a.loss = (float *)loss;
     a.status = (int *)status;
-    hipLaunchKernelGGL(distill_fwd_kernel, dim3((unsigned)N), dim3(kThreads), 0, (hipStream_t)stream, a);
+    CACTI_DISTILL(distill_fwd_kernel, a, (hipStream_t)stream);
     return launch_status("distill_topk_fwd");
 }
 
@@ -211,6 +331,6 @@ CACTI_API int cacti_hip_distill_topk_bwd(int64_t N, int64_t V, int64_t K, const 
     a.grad = (half_t *)dlogit16;
     a.ldd = ldd;
     a.acc = acc;
-    hipLaunchKernelGGL(distill_bwd_kernel, dim3((unsigned)N), dim3(kThreads), 0, (hipStream_t)stream, a);
+    CACTI_DISTILL(distill_bwd_kernel, a, (hipStream_t)stream);
     return launch_status("distill_topk_bwd");
 }

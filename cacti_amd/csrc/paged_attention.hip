@@ -669,13 +669,12 @@ __global__ void __launch_bounds__(kThreads, resident(ND, NR, sizeof(P))) paged_a
 }
 
 // ---------------------------------------------------------------- prompts
-// Sequences with many new rows: 128 of them (tokens by the query heads of a key head) to a workgroup, 16 to each of its eight waves,
-// 64 positions at a time, whose keys and values go through LDS as f16: converted and V turned once for all waves (four of them
-// see to the keys, four to the values), while the products of the 64 before them run, in two buffers with one barrier a step.
+// Sequences with many new rows: 128 of them (tokens by the query heads of a key head) to a workgroup, 32 to each of its four waves,
+// 64 positions at a time, whose keys and values go through LDS as f16: converted and V turned once for all waves (two of them
+// see to the keys, two to the values), while the products of the 64 before them run, in two buffers with one barrier a step.
 // 16-byte pieces of LDS rows are swapped by f(row), which spreads the sixteen rows of an operand, and the rows that a wave writes,
-// evenly over the banks.  What bounds it: LDS (16 KB of operands to a wave for 32 positions, 1024 cycles of a CU for all eight) and
-// the softmax's vector operations about evenly, the matrix pipe half as much.  (32 rows to a wave halve the first, but with the
-// registers of two waves a SIMD some are held in memory, whose loads wait for the next keys: 89 against kHalfRows us.)
+// evenly over the banks.  (16 rows to each of eight waves read the operands twice as often and have half the registers: 88.6
+// against 83 us for three sequences of up to 900 rows and 4000 positions, 16 heads of 128.)
 //
 // Shares are cut as above, a workgroup to a share and by steps of 64.  A tile's steps grow by those of its own 128 rows: counted
 // by a line that is never below them, so that what lies before a tile is a formula; steps behind a tile's last position are
@@ -734,16 +733,16 @@ struct Prompt {
 
     __device__ __forceinline__ int page_of(int x) const { return (int)(__umul24((unsigned)x, a.page_magic) >> 22); }
 
-    // 16 positions in a row are of one page, and so is all that a wave loads at once: the address of its first row is a scalar, a
-    // lane's part of it the same every time (but for the positions behind `end`).
-    __device__ __forceinline__ const P *page_at(const void *pages, int x) const
+    // 16 positions in a row are of one page (x: the first of them, of full ones), and so is all that a wave loads at once: the address
+    // of its first row is a scalar, a lane's part of it the same every time (but for the positions behind `end`).
+    __device__ __forceinline__ const char *page_at(const void *pages, int x) const
     {
-        const int pg = page_of(x);
+        const int pg = uniform((int)((unsigned)x * a.page_magic >> 22));
         const int64_t at = sh.entry.at[pg];
-        const int64_t uni = (int64_t)((uint64_t)(unsigned)uniform((int)(at >> 32)) << 32 | (unsigned)uniform((int)at));
-        return (const P *)pages + uni + (int64_t)((x - pg * a.pb.page) * a.Dp);
+        const uint64_t first = (uint64_t)(unsigned)uniform((int)(at >> 32)) << 32 | (unsigned)uniform((int)at);
+        return (const char *)pages + (first + (unsigned)((x - pg * a.pb.page) * a.Dp)) * sizeof(P);
     }
-    // What of the addresses is a lane's own: its row and columns in memory, elements from the wave's first row, and its place in
+    // What of the addresses is a lane's own: its row and columns in memory, bytes from the wave's first row, and its place in
     // LDS, halves from a buffer's start (keys: of the first piece; values: of column 0 of 4)
     struct Own {
         unsigned from;
@@ -754,11 +753,11 @@ struct Prompt {
         const int tid = threadIdx.x & (kHalf - 1), lane = tid & 63;
         Own w;
         if (threadIdx.x >= kHalf) {
-            w.from = __umul24(lane / kPer, a.Dp) + min(lane % kPer * (16 / (int)sizeof(P)), a.Dp - 16 / (int)sizeof(P));
+            w.from = (__umul24(lane / kPer, a.Dp) + min(lane % kPer * (16 / (int)sizeof(P)), a.Dp - 16 / (int)sizeof(P))) * (unsigned)sizeof(P);
             const int j = tid / kPer, c = tid % kPer * (16 / (int)sizeof(P)) / 8;
             w.to = j * 64 * ND + (c ^ swap_of(j)) * 8;
         } else {
-            w.from = __umul24((8 * (lane / kCols)) & 15, a.Dp) + min(4 * (lane % kCols), a.Dp - 4);
+            w.from = (__umul24((8 * (lane / kCols)) & 15, a.Dp) + min(4 * (lane % kCols), a.Dp - 4)) * (unsigned)sizeof(P);
             const int kg = tid / kCols, d = 4 * (tid % kCols);
             w.to = d * kBig + (kg ^ swap_of(d)) * 8;
         }
@@ -770,8 +769,14 @@ struct Prompt {
         if (wid >= kBigWaves / 2) {
             const int first = 64 * (wid - kBigWaves / 2) / kPer;
             if (x + kBig <= end) {
+                const char *before = nullptr;
 #pragma unroll
-                for (int i = 0; i < kPieces; i++) next.k[i] = *reinterpret_cast<const u4_t *>(page_at(a.k_pages, x + first + i * kApart) + w.from);
+                for (int i = 0; i < kPieces; i++) {    // (first < 16; kApart: 8 or a multiple of 16)
+                    const char *k = kApart < 16 && (i & 1) ? nullptr : page_at(a.k_pages, x + i * kApart) + first * a.Dp * (int)sizeof(P);
+                    if (kApart < 16 && (i & 1)) k = before + kApart * a.Dp * (int)sizeof(P);
+                    next.k[i] = *reinterpret_cast<const u4_t *>(k + w.from);
+                    before = k;
+                }
                 return;
             }
             const int lane = lane_here();
@@ -786,13 +791,13 @@ struct Prompt {
             if (x + kBig <= end) {
 #pragma unroll
                 for (int k = 0; k < kBlocks; k++) {
-                    const P *v = page_at(a.v_pages, x + first + k * kKeys);
+                    const char *v = page_at(a.v_pages, x + first + k * kKeys);
                     if (ND == 1) {
-                        const P *v1 = page_at(a.v_pages, x + first + 16);
+                        const char *v1 = page_at(a.v_pages, x + first + 16);
                         v = (threadIdx.x & 32) ? v1 : v;
                     }
 #pragma unroll
-                    for (int i = 0; i < 8; i++) next.v[k].load(i, v + i * a.Dp + w.from);
+                    for (int i = 0; i < 8; i++) next.v[k].load(i, (const P *)(v + i * a.Dp * (int)sizeof(P) + w.from));
                 }
                 return;
             }
@@ -875,19 +880,28 @@ struct Prompt {
 #pragma unroll
                 for (int n = 0; n < 2; n++) sc[n][t] = mfma(k, q[n][c], sc[n][t]);
             }
+        const int v0 = at.v ^ (32 * b);
+        half8_t vf[4];                         // four operands ahead (one by one, waited for: 87 against 83 us)
+#pragma unroll
+        for (int c = 0; c < 4; c++) vf[c] = *reinterpret_cast<const half8_t *>(vb + (v0 ^ (32 * (c & 1))) + 16 * c * kBig);
         const int pg = page_of(min(x + 8 * g, end - 1));
         const bool edge = x + 31 > min(least, end - 1);
         half8_t p[2];
 #pragma unroll
         for (int n = 0; n < 2; n++)
             p[n] = weigh(sc[n], sh.entry.c[pg], sh.entry.lg[pg], sh.entry.iv[pg], m[n], l[n], o[n], edge, min(last[n] - base, end - 1) - (x + 8 * g) + 1);
-        const int v0 = at.v ^ (32 * b);
 #pragma unroll
         for (int c = 0; c < 4 * ND; c++) {
-            const half8_t v = *reinterpret_cast<const half8_t *>(vb + (v0 ^ (32 * (c & 1))) + 16 * c * kBig);
 #pragma unroll
-            for (int n = 0; n < 2; n++) o[n][c] = mfma(v, p[n], o[n][c]);
+            for (int n = 0; n < 2; n++) o[n][c] = mfma(vf[c & 3], p[n], o[n][c]);
+            if (c + 4 < 4 * ND) vf[c & 3] = *reinterpret_cast<const half8_t *>(vb + (v0 ^ (32 * (c & 1))) + 16 * (c + 4) * kBig);
         }
+#pragma unroll
+        for (int c = 0; c < 4 * ND - 4; c++) {             // (two matrix instructions, one read)
+            __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, 8, 0);
     }
 
     // positions c0 .. c1 - 1 (some) of rows row0 .. of sequence s

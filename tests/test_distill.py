@@ -56,7 +56,7 @@ def reference(z, idx, val, scale, temp):
         hot = np.zeros(V)
         np.add.at(hot, ids, t)
         p = np.exp(log_p)
-        grad[n] = scale[n] / temp * (p - hot)
+        grad[n] = scale[n] / temp * (p * t.sum() - hot)          # (t of the ids that there are: the loss has no others)
         spread = (zz.max() - zz[np.isfinite(zz)].min()) + (v.max() - v[np.isfinite(v)].min())
         rel = 2.0 ** -23 * (2 + spread) + 2.0 ** -24 * (V / 512 + K / 512 + 40)
         loss_tol[n] = rel + 2.0 ** -21 * (t[use] * np.abs(diff)).sum()
