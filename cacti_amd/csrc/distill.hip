@@ -7,7 +7,8 @@
 //
 // A workgroup to a row, which it holds in registers from one read on: the forward pass is bound by that read, the adjoint, which
 // takes the maximum and the sum from the forward pass (stats) and has nothing to reduce over the row, by a read and a write.
-// 2048 rows of 32000, K = 64: forward FWD us (a maximum and then a sum out of memory again: 55), adjoint BWD us.
+// 2048 rows of 32000, K = 64: forward 27.3 us, 4.8 TB/s (a maximum and then a sum out of memory again: 43.8), adjoint 46.7 us,
+// 5.6 TB/s; 611 of 8191, K = 20: 5.9 and 7.0 us; 128 of 1024, K = 8: 4.0 and 3.3 us, latency.
 #include "vocab_row.h"
 
 using namespace cacti;
@@ -31,7 +32,9 @@ struct DistillArgs {
 };
 
 // A row of up to 8 T NP + 7 elements, held by T threads: of its whole 16-byte pieces those lo + tid + i T, and of up to 14
-// elements beside them one for each of the first threads.
+// elements beside them one for each of the first threads.  (The pieces may be those of another row: loads of 16 bytes may begin
+// at any element.)
+typedef half8_t __attribute__((aligned(2))) half8_any_t;
 template <int T, int NP>
 struct Held {
     int lo, hi, edge;                          // whole pieces lo .. hi - 1; the element, or -1
@@ -44,12 +47,12 @@ struct Held {
     }
     __device__ __forceinline__ bool has(int i) const { return lo + (int)threadIdx.x + i * T < hi; }
     __device__ __forceinline__ int piece(int i) const { return min(lo + (int)threadIdx.x + i * T, hi - 1); }
-    __device__ __forceinline__ void load(const VocabRow &z)                // (what it does not have is some other of the row)
+    __device__ __forceinline__ void load(const VocabRow &z, const VocabRow &of)        // (what it does not have is some other of the row)
     {
         e = z.row[max(edge, 0)];
         if (hi > lo)
 #pragma unroll
-            for (int i = 0; i < NP; i++) x[i] = *reinterpret_cast<const half8_t *>(z.row + z.first(piece(i)));
+            for (int i = 0; i < NP; i++) x[i] = *reinterpret_cast<const half8_any_t *>(z.row + of.first(piece(i)));
     }
 };
 
@@ -117,7 +120,7 @@ __global__ void __launch_bounds__(T) distill_fwd_kernel(DistillArgs a)
     Entries<T> t;
     Held<T, NP> h(z);
     t.load(a, n, z.row);
-    h.load(z);
+    h.load(z, z);
     const float c2 = (float)(a.inv_temp * 1.44269504088896340736);
     if (h.edge < 0) h.e = (half_t)-INFINITY;
     float mx = h2f(h.e), tmx = t.max();
@@ -186,8 +189,8 @@ __global__ void __launch_bounds__(T) distill_bwd_kernel(DistillArgs a)
 {
     constexpr int kOf = Entries<T>::kOf;
     __shared__ float sums[T / 64][2];
-    __shared__ int ids[kMaxK];
-    __shared__ float es[kMaxK];
+    __shared__ __attribute__((aligned(16))) int ids[kMaxK];
+    __shared__ __attribute__((aligned(16))) float es[kMaxK];
     const int64_t n = blockIdx.x;
     const VocabRow z(a.logit + n * a.ld, a.V), g(a.grad + n * a.ldd, a.V);
     half_t *gr = a.grad + n * a.ldd;
@@ -196,8 +199,7 @@ __global__ void __launch_bounds__(T) distill_bwd_kernel(DistillArgs a)
     t.load(a, n, z.row);
     const float mx = a.stats[2 * n], row_sum = a.stats[2 * n + 1], scale = a.scale[n];
     // all that is read of the logits and, of other threads' pieces, of the gradient is read before anything is written
-    const bool same = z.off == g.off;
-    if (same) h.load(z);
+    h.load(z, g);
     half_t old[kOf];
 #pragma unroll
     for (int e = 0; e < kOf; e++) {
@@ -213,10 +215,8 @@ __global__ void __launch_bounds__(T) distill_bwd_kernel(DistillArgs a)
         const float w = t.weight(e, tmx, a.inv_temp);
         sum += w;
         if (t.j[e] < a.V) valid += w;
-        if ((int)threadIdx.x + e * T < a.K) {
-            ids[threadIdx.x + e * T] = t.j[e];
-            es[threadIdx.x + e * T] = w;
-        }
+        ids[threadIdx.x + e * T] = t.j[e];     // (-1 behind the last)
+        es[threadIdx.x + e * T] = w;
     }
     sum = wave_sum(sum);
     valid = wave_sum(valid);
@@ -233,6 +233,7 @@ __global__ void __launch_bounds__(T) distill_bwd_kernel(DistillArgs a)
     }
     const bool empty = valid == 0.f && sum == sum;
     const float c2 = (float)(a.inv_temp * 1.44269504088896340736), sc = (float)(scale * a.inv_temp), inv = valid / sum / row_sum;
+    // (empty: a student's NaN must not meet the zero)
     auto stream = [&](half_t x) __attribute__((always_inline)) { return empty ? 0.f : sc * (__builtin_amdgcn_exp2f((h2f(x) - mx) * c2) * inv); };
     // the entries: the last of those with an id has them all, in order
     half_t entry[kOf];
@@ -243,42 +244,42 @@ __global__ void __launch_bounds__(T) distill_bwd_kernel(DistillArgs a)
         mine[e] = i < a.K && j < a.V;
         if (!mine[e]) continue;
         float w = 0.f;
-        for (int k = 0; k < a.K; k++)
-            if (ids[k] == j) {
-                mine[e] = mine[e] && k <= i;
-                w += es[k];
-            }
+        for (int k = 0; k < a.K; k += 4) {
+            const int4 id = *reinterpret_cast<const int4 *>(ids + k);
+            const float4 x = *reinterpret_cast<const float4 *>(es + k);
+            w += id.x == j ? x.x : 0.f;
+            w += id.y == j ? x.y : 0.f;
+            w += id.z == j ? x.z : 0.f;
+            w += id.w == j ? x.w : 0.f;
+            const int last = id.w == j ? 3 : id.z == j ? 2 : id.y == j ? 1 : id.x == j ? 0 : -k;
+            mine[e] = mine[e] && k + last <= i;
+        }
         const float p = __builtin_amdgcn_exp2f((h2f(t.z[e]) - mx) * c2) * inv;
         entry[e] = combined(empty ? 0.f : sc * (p - w / sum), a.acc, old[e]);
     }
-    if (same)
 #pragma unroll
-        for (int i = 0; i < NP; i++) {
-            if (!h.has(i)) break;
-            half_t *to = gr + g.first(h.piece(i));
-            half8_t o = {};
-            if (a.acc) o = *reinterpret_cast<const half8_t *>(to);
+    for (int i = 0; i < NP; i++) {
+        if (!h.has(i)) break;
+        half_t *to = gr + g.first(h.piece(i));
+        half8_t o;
+        if (a.acc) {
+            o = *reinterpret_cast<const half8_t *>(to);
 #pragma unroll
-            for (int k = 0; k < 8; k++) o[k] = combined(stream(h.x[i][k]), a.acc, o[k]);
-            *reinterpret_cast<half8_t *>(to) = o;
-        }
-    else
-        for (int c = h.lo + threadIdx.x; c < h.hi; c += T) {
-            const int j0 = g.first(c);
-            half8_t o = {};
-            if (a.acc) o = *reinterpret_cast<const half8_t *>(gr + j0);
+            for (int k = 0; k < 8; k++) o[k] = combined(stream(h.x[i][k]), 1, o[k]);
+        } else
 #pragma unroll
-            for (int k = 0; k < 8; k++) o[k] = combined(stream(z.row[j0 + k]), a.acc, o[k]);
-            *reinterpret_cast<half8_t *>(gr + j0) = o;
-        }
-    if (h.edge >= 0) gr[h.edge] = combined(stream(same ? h.e : z.row[h.edge]), a.acc, a.acc ? gr[h.edge] : (half_t)0.f);
+            for (int k = 0; k < 8; k++) o[k] = f2h(stream(h.x[i][k]));
+        *reinterpret_cast<half8_t *>(to) = o;
+    }
+    if (h.edge >= 0) gr[h.edge] = combined(stream(h.e), a.acc, a.acc ? gr[h.edge] : (half_t)0.f);
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < kOf; e++)
         if (mine[e]) gr[t.j[e]] = entry[e];
 }
 
-// The least threads and registers that hold a row
+// The least threads and registers that hold a row.  (Forward and adjoint, 611 rows of 8191: 256 threads 5.9 and 8.8 us, 512 8.0 and
+// 9.4; 2048 of 32000: 256 26.8 and 55.1, 512 27.3 and 50.5, 1024 33.5 and 57.7)
 #define CACTI_DISTILL(kernel, a, st)                                                                                                  \
     do {                                                                                                                              \
         const dim3 grid((unsigned)(a).N);                                                                                             \
