@@ -42,6 +42,20 @@ __device__ __forceinline__ Sequence sequence(const PagedBatch &pb, int b, int64_
     return q;
 }
 
+// A lane's sequence of 64 from b0 on, and a lane's to all of the wave
+__device__ __forceinline__ Sequence lane_sequence(const PagedBatch &pb, int b0, int64_t limit, int max_new)
+{
+    const int b = b0 + (threadIdx.x & 63);
+    Sequence s = sequence(pb, min(b, pb.B - 1), limit, max_new);
+    if (b >= pb.B) s.n = 0, s.ok = false;
+    return s;
+}
+__device__ __forceinline__ Sequence of_lane(const Sequence &s, int lane)
+{
+    return {__builtin_amdgcn_readlane(s.s0, lane), __builtin_amdgcn_readlane(s.n, lane), __builtin_amdgcn_readlane(s.first, lane),
+            __builtin_amdgcn_readlane((int)s.ok, lane) != 0};
+}
+
 // How many of f(1) .. f(B) are <= x, for an f that does not fall: the sequence that unit x of them belongs to.  Every lane
 // of a wave that calls looks at some (one round trip to memory for up to 64 sequences) and all get the answer.
 template <class F>

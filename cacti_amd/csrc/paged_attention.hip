@@ -70,18 +70,9 @@ struct Share {
     {
     }
 };
-// A lane's sequence of 64 from b0 on
 __device__ __forceinline__ Sequence lane_sequence(const AttnArgs &a, int b0)
 {
-    const int b = b0 + (threadIdx.x & 63);
-    Sequence s = sequence(a.pb, min(b, a.pb.B - 1), (int64_t)a.pb.W * a.pb.page, a.max_new);
-    if (b >= a.pb.B) s.n = 0, s.ok = false;
-    return s;
-}
-__device__ __forceinline__ Sequence of_lane(const Sequence &s, int lane)
-{
-    return {__builtin_amdgcn_readlane(s.s0, lane), __builtin_amdgcn_readlane(s.n, lane), __builtin_amdgcn_readlane(s.first, lane),
-            __builtin_amdgcn_readlane((int)s.ok, lane) != 0};
+    return lane_sequence(a.pb, b0, (int64_t)a.pb.W * a.pb.page, a.max_new);
 }
 
 // A share is at least that many units: fewer steps are more parts to put together than they save (one sequence of 1540 positions,
