@@ -1090,18 +1090,44 @@ struct Parts {
     __device__ __forceinline__ int slot(int p) const { return p == 0 ? 2 * i0 + 1 : 2 * (i0 + p); }
 };
 
-// The parts of a row put together, two columns per lane, by a workgroup per row and head; zeros for rows whose sequence's numbers
-// do not fit together.  For few rows: every fourth part to a wave.
-template <int NR>
+// Parts put together as they come: maximum and sum of weights, and the weighted sums of N columns
+template <int N>
+struct Joined {
+    float m = -INFINITY, l = 0.f, o[N] = {};
+    // `AT` parts (m, l, o) at once; `there`: how many of them there are
+    template <int AT>
+    __device__ __forceinline__ void add(const float2 (&st)[AT], const float (&v)[AT][N], int there)
+    {
+        float mn = m;
+#pragma unroll
+        for (int k = 0; k < AT; k++) mn = k < there ? fmaxf(mn, st[k].x) : mn;
+        const float origin = finite_max(mn), f = exp2_of(m - origin);
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < N; i++) o[i] *= f;
+#pragma unroll
+        for (int k = 0; k < AT; k++) {
+            if (k >= there) continue;
+            const float fk = exp2_of(st[k].x - origin);
+            l = __builtin_fmaf(st[k].y, fk, l);
+#pragma unroll
+            for (int i = 0; i < N; i++) o[i] = __builtin_fmaf(v[k][i], fk, o[i]);
+        }
+    }
+};
+
+// The parts of a row put together, two columns per lane, by a wave or, for few rows, a workgroup of four waves; zeros for rows whose
+// sequence's numbers do not fit together.  Bound by latency: eight parts are requested at once, their sums with their values.
+template <int NR, int WAVES>
 __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs a)
 {
     constexpr int kRows = 16 * NR, kAtOnce = 8;
-    __shared__ float o[kWaves][2][64];
     const PagedBatch &pb = a.pb;
-    const int lane = threadIdx.x & 63, wid = uniform((int)threadIdx.x >> 6), row = blockIdx.x / a.H, head = blockIdx.x - row * a.H;
-    const int d = min(2 * lane, a.Dh - 2);
+    const int lane = threadIdx.x & 63, wid = uniform((int)threadIdx.x >> 6), at_row = (int)blockIdx.x * (kWaves / WAVES) + (WAVES == 1 ? wid : 0);
+    const int row = at_row / a.H, head = at_row - row * a.H, first = WAVES == 1 ? 0 : wid, d = min(2 * lane, a.Dh - 2);
     // all work, that of the sequences before the row's, and the row's sequence
-    double all = 0., some = 0., big_all = 0., big_some = 0.;
+    double all = 0., some = 0.;
     Sequence s = {0, 0, 0, false};
     int b = -1;
     for (int b0 = 0; b0 < pb.B; b0 += 64) {
@@ -1109,68 +1135,59 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs
         const double u = Share(a, kRows, q).units;
         const uint64_t hit = __ballot(b0 + lane < pb.B && row >= q.s0 && row - q.s0 < q.n);
         all += u;
-        const bool earlier = b < 0 && (!hit || lane < __ffsll((unsigned long long)hit) - 1);
-        some += earlier ? u : 0.;
-        if (a.big_groups) {
-            const double v = BigShare(a, q).units(a);
-            big_all += v;
-            big_some += earlier ? v : 0.;
-        }
+        some += b < 0 && (!hit || lane < __ffsll((unsigned long long)hit) - 1) ? u : 0.;
         if (hit && b < 0) {
             const int at = __ffsll((unsigned long long)hit) - 1;
             b = b0 + at;
             s = of_lane(q, at);
         }
     }
-    if (b < 0) return;
+    if (b < 0 || row >= pb.T) return;
     half_t *out = a.out + row * a.ldo + head * a.Dh + d;
     if (!s.ok) {
         if (lane == 0) report(pb, b);
-        if (wid == 0 && 2 * lane < a.Dh) *reinterpret_cast<half2_t *>(out) = half2_t{};
+        if (first == 0 && 2 * lane < a.Dh) *reinterpret_cast<half2_t *>(out) = half2_t{};
         return;
     }
-    const bool big = s.n * a.G > a.few;
-    const int h = head / a.G, r = (row - s.s0) * a.G + head - h * a.G, tile_rows = big ? kPrompt : kRows, tile = r / tile_rows;
-    const Parts in(a, s, kRows, h, tile, uniform((int)(unsigned)wave_sum_f64(big ? big_all : all)),
-                   uniform((int)(unsigned)wave_sum_f64(big ? big_some : some)));
+    const int h = head / a.G, r = (row - s.s0) * a.G + head - h * a.G, tile = r / kRows;
+    const Parts in(a, s, kRows, h, tile, uniform((int)(unsigned)wave_sum_f64(all)), uniform((int)(unsigned)wave_sum_f64(some)));
     const int parts = in.count;
     if (parts == 1) return;
-    const float *part = big ? a.big_part : a.part, *stats = big ? a.big_stats : a.stats;
-    auto at = [&](int p) { return (int64_t)in.slot(p) * tile_rows + r - tile * tile_rows; };
-    float mx = -INFINITY, sum = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int p = lane; p < parts; p += 64) mx = fmaxf(mx, stats[2 * at(p)]);
-    const float origin = finite_max(wave_max(mx));
-    for (int p0 = 0; p0 < parts; p0 += 64) {
-        const int p = min(p0 + lane, parts - 1);
-        const float f = p0 + lane < parts ? exp2_of(stats[2 * at(p)] - origin) : 0.f;
-        sum += f * stats[2 * at(p) + 1];
-        for (int k0 = wid; k0 < min(64, parts - p0); k0 += kWaves * kAtOnce) {
-            float2 v[kAtOnce];
+    Joined<2> j;
+    for (int p0 = first; p0 < parts; p0 += WAVES * kAtOnce) {
+        float2 st[kAtOnce];
+        float v[kAtOnce][2];
 #pragma unroll
-            for (int k = 0; k < kAtOnce; k++)
-                v[k] = *reinterpret_cast<const float2 *>(part + at(min(p0 + k0 + k * kWaves, parts - 1)) * a.Dh + d);
-#pragma unroll
-            for (int k = 0; k < kAtOnce; k++) {
-                const int from = k0 + k * kWaves;
-                if (from >= min(64, parts - p0)) break;
-                const float fk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), from));
-                o0 += fk * v[k].x;
-                o1 += fk * v[k].y;
-            }
+        for (int k = 0; k < kAtOnce; k++) {
+            const int64_t at = (int64_t)in.slot(min(p0 + k * WAVES, parts - 1)) * kRows + r - tile * kRows;
+            st[k] = *reinterpret_cast<const float2 *>(a.stats + 2 * at);
+            const float2 x = *reinterpret_cast<const float2 *>(a.part + at * a.Dh + d);
+            v[k][0] = x.x;
+            v[k][1] = x.y;
         }
+        j.add(st, v, (parts - p0 + WAVES - 1) / WAVES);
     }
-    sum = wave_sum(sum);
-    o[wid][0][lane] = o0;
-    o[wid][1][lane] = o1;
-    __syncthreads();
-    if (wid > 0 || 2 * lane >= a.Dh) return;
+    if constexpr (WAVES > 1) {
+        __shared__ float o[kWaves][2][64];
+        __shared__ float2 ml[kWaves];
+        o[wid][0][lane] = j.o[0];
+        o[wid][1][lane] = j.o[1];
+        ml[wid] = {j.m, j.l};
+        __syncthreads();
+        if (wid > 0) return;
+        float2 st[kWaves];
+        float v[kWaves][2];
 #pragma unroll
-    for (int w4 = 1; w4 < kWaves; w4++) {
-        o0 += o[w4][0][lane];
-        o1 += o[w4][1][lane];
+        for (int w = 0; w < kWaves; w++) {
+            st[w] = ml[w];
+            v[w][0] = o[w][0][lane];
+            v[w][1] = o[w][1][lane];
+        }
+        j = Joined<2>();
+        j.add(st, v, kWaves);
     }
-    const float y = sum == 0.f ? 0.f : 1.f / sum;
-    *reinterpret_cast<half2_t *>(out) = half2_t{f2h(o0 * y), f2h(o1 * y)};
+    const float y = j.l == 0.f ? 0.f : 1.f / j.l;
+    if (2 * lane < a.Dh) *reinterpret_cast<half2_t *>(out) = half2_t{f2h(j.o[0] * y), f2h(j.o[1] * y)};
 }
 
 // The same for many rows: a row to 32 lanes, four columns to a lane, 8 rows of a tile and key head to a workgroup, of a prompt's 32
@@ -1212,23 +1229,32 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_tiles_kernel(At
     const Parts in(a, s, kRows, h, tile, uniform((int)(unsigned)wave_sum_f64(all)), uniform((int)(unsigned)wave_sum_f64(some)));
     if (in.count == 1) return;
     const float *part = prompts ? a.big_part : a.part, *stats = prompts ? a.big_stats : a.stats;
-    for (int k = 0; k < per && per * part_of + k < here; k += 2 * kWaves) {
-        const int row = min(r + k, here - 1);
-        float m = -INFINITY, sum = 0.f;
-        float4_t o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-        for (int p = 0; p < in.count; p++) {
-            const int64_t at = (int64_t)in.slot(p) * tile_rows + row;
-            const float2 st = *reinterpret_cast<const float2 *>(stats + 2 * at);
-            const float4_t v = *reinterpret_cast<const float4_t *>(part + at * a.Dh + min(d, a.Dh - 4));
-            const float mn = fmaxf(m, st.x), origin = finite_max(mn), f = exp2_of(m - origin), fp = exp2_of(st.x - origin);
-            m = mn;
-            sum = sum * f + st.y * fp;
-            o = o * f + v * fp;
+    constexpr int kAtOnce = 4;                 // parts at once, of two rows
+    for (int k = 0; k < per && per * part_of + k < here; k += 4 * kWaves) {
+        Joined<4> j[2];
+        for (int p0 = 0; p0 < in.count; p0 += kAtOnce) {
+            float2 st[2][kAtOnce];
+            float v[2][kAtOnce][4];
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+#pragma unroll
+                for (int p = 0; p < kAtOnce; p++) {
+                    const int64_t at = (int64_t)in.slot(min(p0 + p, in.count - 1)) * tile_rows + min(r + k + 2 * kWaves * e, here - 1);
+                    st[e][p] = *reinterpret_cast<const float2 *>(stats + 2 * at);
+                    const float4_t x = *reinterpret_cast<const float4_t *>(part + at * a.Dh + min(d, a.Dh - 4));
+#pragma unroll
+                    for (int i = 0; i < 4; i++) v[e][p][i] = x[i];
+                }
+#pragma unroll
+            for (int e = 0; e < 2; e++) j[e].add(st[e], v[e], in.count - p0);
         }
-        const float y = sum == 0.f ? 0.f : 1.f / sum;
-        if (r + k < here && d < a.Dh)
-            *reinterpret_cast<half4_t *>(out_of(row0 + r + k) + d) = half4_t{f2h(o[0] * y), f2h(o[1] * y), f2h(o[2] * y), f2h(o[3] * y)};
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const float y = j[e].l == 0.f ? 0.f : 1.f / j[e].l;
+            const int row = r + k + 2 * kWaves * e;
+            if (row < here && row < per * (part_of + 1) && d < a.Dh)
+                *reinterpret_cast<half4_t *>(out_of(row0 + row) + d) = half4_t{f2h(j[e].o[0] * y), f2h(j[e].o[1] * y), f2h(j[e].o[2] * y), f2h(j[e].o[3] * y)};
+        }
     }
 }
 
@@ -1261,7 +1287,9 @@ template <int NR>
 int launch_join(const AttnArgs &a, hipStream_t st)
 {
     const int64_t rh = (int64_t)a.pb.T * a.H;
-    if (rh < 4 * device_cus()) hipLaunchKernelGGL(paged_attention_join_kernel<NR>, dim3((unsigned)rh), dim3(kThreads), 0, st, a);
+    if (a.big_groups == 0 && rh < 4 * device_cus()) hipLaunchKernelGGL((paged_attention_join_kernel<NR, kWaves>), dim3((unsigned)rh), dim3(kThreads), 0, st, a);
+    else if (a.big_groups == 0 && rh < 32 * device_cus())
+        hipLaunchKernelGGL((paged_attention_join_kernel<NR, 1>), dim3((unsigned)((rh + kWaves - 1) / kWaves)), dim3(kThreads), 0, st, a);
     else {
         const Units few = tiles_of(a, 16 * NR), big = a.big_groups ? tiles_of(a, kPrompt) : Units{1, 1, 1, 0};
         const int64_t grid = few.count * (16 * NR / kJoinRows) + big.count * (kPrompt / kBigJoinRows);
