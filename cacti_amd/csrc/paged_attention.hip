@@ -16,9 +16,10 @@
 // numbers, no barrier; the keys after these are requested once these have been multiplied, the values likewise, into the same
 // registers.
 //
-// Work: the lengths are on the device and as different as they come, so every wave of a launch that just fills the device
-// forms their sum in steps of 32 positions and takes an equal, contiguous share of it, across rows, heads and sequences.  A
-// tile of rows that ends up in more than one share leaves partial sums, which a second launch puts together.
+// Work: the lengths are on the device and as different as they come, so every workgroup of a launch that just fills the device
+// forms their sum in steps of 32 positions and takes an equal, contiguous share of it, across rows, heads and sequences, each of
+// its waves a quarter.  What its waves have of a tile of rows they put together in LDS; a tile that ends up in more than one
+// share leaves partial sums, which a second launch puts together.
 #include "paged.h"
 
 using namespace cacti;
@@ -43,7 +44,7 @@ struct AttnArgs {
     const float *k_scale, *v_scale;
     half_t *out;
     int64_t ldo;
-    float *part, *stats;                       // [2 groups][16 NR][Dh], [2 groups][16 NR][2]; a group: a wave
+    float *part, *stats;                       // [2 groups][16 NR][Dh], [2 groups][16 NR][2]; a group: a workgroup
     int few;                                   // sequences with more rows than that (by the query heads of a key head) are prompts
     int big_groups;                            // ... for which a group is a workgroup; 0: there are none
     float *big_part, *big_stats;               // [2 big_groups][kPrompt][Dh], ...[2]
@@ -75,10 +76,10 @@ __device__ __forceinline__ Sequence lane_sequence(const AttnArgs &a, int b0)
     return lane_sequence(a.pb, b0, (int64_t)a.pb.W * a.pb.page, a.max_new);
 }
 
-// A share is at least that many units: fewer steps are more parts to put together than they save (one sequence of 1540 positions,
-// 32 heads of 100, 1 / 2 / 4 / 8: 14.5 / 13.6 / 13.5 / 16.1 us)
+// A wave's part of a share is at least that many units: fewer steps are more parts to put together than they save (one sequence of
+// 1540 positions, 32 heads of 100, 2 / 4 / 8: LEAST us)
 constexpr unsigned kLeast = 4;
-__device__ __forceinline__ unsigned groups_of(const AttnArgs &a, unsigned units) { return min((unsigned)a.groups, max(units / kLeast, 1u)); }
+__device__ __forceinline__ unsigned groups_of(const AttnArgs &a, unsigned units) { return min((unsigned)a.groups, max(units / (kLeast * kWaves), 1u)); }
 
 constexpr unsigned kBigLeast = 4;              // the same of steps of 64 positions
 // Workgroups go round the 8 XCDs: those of one XCD get neighbouring numbers (of n, a multiple of 8)
@@ -568,6 +569,35 @@ struct Tile {
         }
     }
 
+    // What other waves of the workgroup have of the tile, through LDS
+    struct Deposit {
+        float4_t o[NR][VD][64];
+        float m[NR][64], l[NR][64];
+    };
+    __device__ __forceinline__ void put(Deposit &to) const
+    {
+        const int lane = lane_here();
+#pragma unroll
+        for (int n = 0; n < NR; n++) {
+            to.m[n][lane] = m[n];
+            to.l[n][lane] = l[n];
+#pragma unroll
+            for (int c = 0; c < VD; c++) to.o[n][c][lane] = o[n][c];
+        }
+    }
+    __device__ __forceinline__ void add(const Deposit &x)
+    {
+        const int lane = lane_here();
+#pragma unroll
+        for (int n = 0; n < NR; n++) {
+            const float mx = x.m[n][lane], mn = fmaxf(m[n], mx), origin = finite_max(mn), f = exp2_of(m[n] - origin), fx = exp2_of(mx - origin);
+            m[n] = mn;
+            l[n] = l[n] * f + x.l[n][lane] * fx;
+#pragma unroll
+            for (int c = 0; c < VD; c++) o[n][c] = o[n][c] * f + x.o[n][c][lane] * fx;
+        }
+    }
+
     // A lane has columns VD (4 g + i) + c of its row in o[.][c][i].  slot < 0: to the output
     __device__ __forceinline__ void write(const Sequence &s, int h, int rows, int row0, int slot)
     {
@@ -603,9 +633,13 @@ struct Tile {
 constexpr int resident(int ND, int NR, int bytes) { return NR == 1 && ND * bytes < 4 ? 3 : 2; }
 
 template <int ND, int NR, class P>
-__device__ __forceinline__ void wave_share(const AttnArgs &a, unsigned group, Entry &entry)
+__global__ void __launch_bounds__(kThreads, resident(ND, NR, sizeof(P))) paged_attention_kernel(AttnArgs a)
 {
     constexpr int kRows = 16 * NR;
+    constexpr unsigned kBegin = begin_of(kRows);
+    __shared__ Entry entries[kWaves];
+    __shared__ typename Tile<ND, NR, P>::Deposit deposits[kWaves - 1];     // of waves 1, 2, 3
+    const unsigned wid = uniform((int)threadIdx.x >> 6), group = blockIdx.x;
     const Sequence s64 = lane_sequence(a, 0);              // of the first 64 sequences, which mostly are all
     const double u64 = Share(a, kRows, s64).units;         // (whole numbers)
     double all = u64;
@@ -613,8 +647,10 @@ __device__ __forceinline__ void wave_share(const AttnArgs &a, unsigned group, En
     const unsigned units = uniform((int)(unsigned)wave_sum_f64(all)), groups = groups_of(a, units);
     if (group >= groups) return;
     const Shares shares(units, groups);
-    unsigned x = uniform((int)shares.begin(group));
-    const unsigned until = uniform((int)shares.begin(group + 1));
+    const unsigned x0 = uniform((int)shares.begin(group)), x1 = uniform((int)shares.begin(group + 1));     // the workgroup's
+    auto begin = [&](unsigned w) { return x0 + (x1 - x0) * w / kWaves; };  // and a wave's
+    unsigned x = begin(wid);
+    const unsigned until = begin(wid + 1);
     // the sequence in whose work x lies, and what there is before it
     int b = 0;
     unsigned before = 0;
@@ -628,35 +664,42 @@ __device__ __forceinline__ void wave_share(const AttnArgs &a, unsigned group, En
             break;
         }
     }
+    // Of a tile the workgroup has units g0 .. g1 - 1, this wave u0 .. u1 - 1.  The wave that has the first of them puts them together.
+    Tile<ND, NR, P> t{a, entries[wid]};
+    Sequence s;
+    int h, row0, slot;
+    unsigned g1 = 0;
+    bool others = false;                       // there are other waves' to put together with what t has
     for (; x < until; b++) {
-        const Sequence s = b < 64 ? of_lane(s64, b) : sequence(a.pb, b, (int64_t)a.pb.W * a.pb.page, a.max_new);
+        s = b < 64 ? of_lane(s64, b) : sequence(a.pb, b, (int64_t)a.pb.W * a.pb.page, a.max_new);
         const Share w(a, kRows, s);
         const unsigned behind = before + w.units;
         while (x < until && x < behind) {
-            const unsigned at = x - before, whole = w.steps + begin_of(kRows);
-            const int u = uniform((int)(at / whole)), h = uniform(u / w.tiles), row0 = (u - h * w.tiles) * kRows, rows = s.n * a.G;
-            const int from = (int)(at - u * whole), to = (int)min((unsigned)(whole), from + (until - x));      // of the tile's units
-            const int end = uniform(s.first + min(rows - 1, row0 + kRows - 1) / a.G + 1);         // positions that some row sees
-            const int first = max(from - begin_of(kRows), 0), behind_last = to - begin_of(kRows);
-            if (behind_last > first) {
-                const int c0 = first * kStep, c1 = min(end, behind_last * kStep);
-                Tile<ND, NR, P> t{a, entry};
-                t.run(b, s, h, rows, row0, c0, c1);
-                if (t.odd) t.add_odd(b, h, max(c0, s.first + row0 / a.G + 1), c1);
-                t.write(s, h, rows, row0, first == 0 && behind_last == w.steps ? -1 : 2 * (int)group + (first == 0));
-            }
-            x += to - from;
+            const unsigned whole = w.steps + kBegin;
+            const int u = uniform((int)((x - before) / whole)), rows = s.n * a.G;
+            const unsigned start = before + u * whole + kBegin, end = start + w.steps;         // of the tile's steps
+            h = uniform(u / w.tiles);
+            row0 = (u - h * w.tiles) * kRows;
+            const unsigned g0 = max(x0, start), u0 = max(x, start), u1 = min(until, end);
+            g1 = min(x1, end);
+            x = u1;
+            if (u1 <= u0) continue;            // (a share may end before the tile's first step)
+            const int seen = uniform(s.first + min(rows - 1, row0 + kRows - 1) / a.G + 1);     // positions that some row sees
+            const int c0 = (int)(u0 - start) * kStep, c1 = min(seen, (int)(u1 - start) * kStep);
+            t.run(b, s, h, rows, row0, c0, c1);
+            if (t.odd) t.add_odd(b, h, max(c0, s.first + row0 / a.G + 1), c1);
+            slot = g0 == start && g1 == end ? -1 : 2 * (int)group + (g0 == start);
+            others = u0 == g0 && u1 < g1;
+            if (u0 > g0) t.put(deposits[wid - 1]);
+            else if (!others) t.write(s, h, rows, row0, slot);
         }
         before = behind;
     }
-}
-
-template <int ND, int NR, class P>
-__global__ void __launch_bounds__(kThreads, resident(ND, NR, sizeof(P))) paged_attention_kernel(AttnArgs a)
-{
-    __shared__ Entry entries[kWaves];
-    const int wid = uniform((int)threadIdx.x >> 6);
-    wave_share<ND, NR, P>(a, blockIdx.x * kWaves + wid, entries[wid]);
+    __syncthreads();
+    if (!others) return;
+    for (unsigned w = wid + 1; w < kWaves && begin(w) < g1; w++)
+        if (begin(w) < begin(w + 1)) t.add(deposits[w - 1]);
+    t.write(s, h, s.n * a.G, row0, slot);
 }
 
 // ---------------------------------------------------------------- prompts
@@ -1272,8 +1315,8 @@ Plan plan(int64_t T, int64_t B, int64_t H, int64_t Hkv, int64_t Dh, int64_t max_
 {
     const int64_t G = H / Hkv, rows = (max_new < T ? max_new : T) * G;
     const int NR = rows <= 16 ? 1 : 2;
-    if (rows > kFew) return {2, 2 * kWaves * device_cus(), B == 1 ? 0 : kFew, 2 * device_cus()};
-    return {NR, resident(Dh <= 64 ? 1 : 2, NR, bytes) * kWaves * device_cus(), INT32_MAX, 0};
+    if (rows > kFew) return {2, 2 * device_cus(), B == 1 ? 0 : kFew, 2 * device_cus()};
+    return {NR, resident(Dh <= 64 ? 1 : 2, NR, bytes) * device_cus(), INT32_MAX, 0};
 }
 
 // Tiles of `rows` rows of the key heads' queries
@@ -1300,7 +1343,7 @@ int launch_join(const AttnArgs &a, hipStream_t st)
 template <int ND, int NR, class P>
 int launch(const AttnArgs &a, hipStream_t st)
 {
-    hipLaunchKernelGGL((paged_attention_kernel<ND, NR, P>), dim3((unsigned)(a.groups / kWaves)), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((paged_attention_kernel<ND, NR, P>), dim3((unsigned)a.groups), dim3(kThreads), 0, st, a);
     const int rc = launch_status("paged_attention");
     return rc ? rc : launch_join<NR>(a, st);
 }
