@@ -29,8 +29,9 @@ namespace {
 constexpr int kThreads = 256, kWaves = 4, kStep = 32;
 constexpr int kEntries = 64;                   // pages that a wave looks up at a time, one to a lane
 // What a tile of rows costs a share besides its steps, in steps: queries, pages and the first keys to wait for.  (48 sequences
-// of 120 to 8192 positions, 16 rows, 2 / 4 / 8 / 16: 134 / 134 / 137 / 140 us; 24 of 100 to 6000, 32 rows 38.3 / 37.3 / 36.1 / 35.8)
-constexpr int begin_of(int tile) { return tile / 4; }
+// of 120 to 8192 positions, 16 rows, 1 / 2 / 4 / 8: 130.2 / 128.4 / 129.4 / 131.3 us; 24 of 100 to 6000, 32 rows, 2 / 4 / 8 / 16:
+// 29.1 / 27.7 / 28.5 / 29.4)
+constexpr int begin_of(int tile) { return tile / 8; }
 
 struct AttnArgs {
     PagedBatch pb;
@@ -77,8 +78,8 @@ __device__ __forceinline__ Sequence lane_sequence(const AttnArgs &a, int b0)
 }
 
 // A wave's part of a share is at least that many units: fewer steps are more parts to put together than they save (one sequence of
-// 1540 positions, 32 heads of 100, 2 / 4 / 8: LEAST us)
-constexpr unsigned kLeast = 4;
+// 1540 positions, 32 heads of 100, 1 / 2 / 3 / 4: 13.7 / 12.4 / 13.1 / 13.5 us)
+constexpr unsigned kLeast = 2;
 __device__ __forceinline__ unsigned groups_of(const AttnArgs &a, unsigned units) { return min((unsigned)a.groups, max(units / (kLeast * kWaves), 1u)); }
 
 constexpr unsigned kBigLeast = 4;              // the same of steps of 64 positions
