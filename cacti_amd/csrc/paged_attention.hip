@@ -944,23 +944,36 @@ struct Prompt {
     {
         const int wid = uniform((int)threadIdx.x >> 6), lane = lane_here(), tid = 64 * wid + lane, r16 = lane & 15, g = lane >> 4;
         const int mine = row0 + 32 * wid;      // the wave's first row
+        // the pages from position `seg` on: the lane's number of them
+        auto look_up = [&](int seg) __attribute__((always_inline)) {
+            const int p0 = uniform(seg / a.pb.page), most = page_of(min(c1 - p0 * a.pb.page, kEntries * a.pb.page) - 1);
+            return a.pb.table[(int64_t)b * a.pb.ldt + p0 + min(lane, most)];
+        };
+        int id = look_up(c0);                  // requested with the queries
+        u2_t words[2][2 * NS];
 #pragma unroll
         for (int n = 0; n < 2; n++) {
             const int r = min(mine + 16 * n + r16, rows - 1), t = r / a.G;
             last[n] = s.first + t;
             const half_t *qr = a.q + (int64_t)(s.s0 + t) * a.ldq + (h * a.G + r - t * a.G) * a.Dh;
 #pragma unroll
+            for (int c = 0; c < 2 * NS; c++) words[n][c] = *reinterpret_cast<const u2_t *>(qr + min(32 * (c / 2) + 8 * g + 4 * (c & 1), a.Dh - 4));
+        }
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
             for (int c = 0; c < NS; c++) {
                 Frag f;
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    const int d = 32 * c + 8 * g + 4 * j;
-                    const u2_t w = *reinterpret_cast<const u2_t *>(qr + min(d, a.Dh - 4));
-                    f.u[2 * j] = d < a.Dh ? w[0] ^ a.sign : 0u;
-                    f.u[2 * j + 1] = d < a.Dh ? w[1] ^ a.sign : 0u;
+                    const bool there = 32 * c + 8 * g + 4 * j < a.Dh;
+                    f.u[2 * j] = there ? words[n][2 * c + j][0] ^ a.sign : 0u;
+                    f.u[2 * j + 1] = there ? words[n][2 * c + j][1] ^ a.sign : 0u;
                 }
                 q[n][c] = f.h;
             }
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
             m[n] = -INFINITY;
             l[n] = 0.f;
 #pragma unroll
@@ -973,8 +986,8 @@ struct Prompt {
         for (int seg = c0; seg < c1;) {
             const int p0 = uniform(seg / a.pb.page), base = p0 * a.pb.page, end = min(c1 - base, kEntries * a.pb.page);
             __syncthreads();                   // (entries and buffers of before are done with)
+            if (seg != c0) id = look_up(seg);
             if (tid < 64) {
-                int id = a.pb.table[(int64_t)b * a.pb.ldt + p0 + min(lane, page_of(end - 1))];
                 if (id < 0 || id >= a.pb.P) {
                     report(a.pb, b);
                     id = 0;                    // its rows are unspecified, not its reads
@@ -1234,47 +1247,52 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs
     if (2 * lane < a.Dh) *reinterpret_cast<half2_t *>(out) = half2_t{f2h(j.o[0] * y), f2h(j.o[1] * y)};
 }
 
-// The same for many rows: a row to 32 lanes, four columns to a lane, 8 rows of a tile and key head to a workgroup, of a prompt's 32
-// (tiles numbered as they are in a batch of any lengths: most workgroups of a launch find nothing to do, and looking takes 2 us).
-constexpr int kJoinRows = 8, kBigJoinRows = 32;
-template <int NR>
+// The same for prompts, and for the few rows of other sequences of the batch: a row to 32 lanes, four columns to a lane, 32 rows of a
+// tile and key head to a workgroup (tiles numbered as they are in a batch of any lengths: many find nothing to do).
+constexpr int kJoinRows = 32;
 __global__ void __launch_bounds__(kThreads) paged_attention_join_tiles_kernel(AttnArgs a, Units big, Units few)
 {
-    constexpr int kRows = 16 * NR;
+    constexpr int kRows = 32, kCut = kPrompt / kJoinRows;
     const PagedBatch &pb = a.pb;
     const int lane = threadIdx.x & 63, h = blockIdx.y;
-    constexpr int kBigCut = kPrompt / kBigJoinRows, kCut = kRows / kJoinRows;
-    const int64_t bigs = big.count * kBigCut, x = blockIdx.x < bigs ? blockIdx.x : blockIdx.x - bigs;
+    const int64_t bigs = big.count * kCut;
     const bool prompts = blockIdx.x < bigs;
-    const int cut = prompts ? kBigCut : kCut, per = prompts ? kBigJoinRows : kJoinRows, part_of = (int)(x % cut);
-    int tile;
-    const int b = uniform(prompts ? big.find(pb, x / cut, &tile) : few.find(pb, x / cut, &tile));
-    tile = uniform(tile);
+    const int64_t number = prompts ? blockIdx.x / kCut : blockIdx.x - bigs;
+    const int from = prompts ? (int)(blockIdx.x % kCut) * kJoinRows : 0;       // the first row
+    // the unit's sequence (as Units::find has it, from what the lanes have of the sequences), all work and that of those before it
+    const Units &u = prompts ? big : few;
+    int b = u.even ? (int)(number / u.even) : 0;
+    double all = 0., some = 0.;
+    Sequence s = {0, 0, 0, false};
+    for (int b0 = 0; b0 < pb.B; b0 += 64) {
+        const Sequence q = lane_sequence(a, b0);
+        const int i = b0 + lane;
+        if (!u.even) b += __popcll(__ballot(i < pb.B && max(q.s0 + q.n, 0) / u.per + (int64_t)u.more * (i + 1) <= number));
+        const double w = prompts ? BigShare(a, q).units(a) : Share(a, kRows, q).units;
+        all += w;
+        some += i < b ? w : 0.;                // (b grows only while all of these are before it)
+        if (b >= b0 && b < b0 + 64) s = of_lane(q, b - b0);
+    }
+    b = uniform(b);
     if (b >= pb.B) return;
-    const Sequence s = sequence(pb, b, (int64_t)pb.W * pb.page, a.max_new);
+    const int tile = uniform((int)(number - (u.even ? (int64_t)b * u.even : (int64_t)max(s.s0, 0) / u.per + (int64_t)u.more * b)));
     const int tile_rows = prompts ? kPrompt : kRows, rows = s.n * a.G, row0 = tile * tile_rows, here = min(tile_rows, rows - row0);
     if (s.s0 < 0 || s.n <= 0 || s.s0 > pb.T - s.n || tile < 0 || here <= 0) return;
     auto out_of = [&](int r) { return a.out + (int64_t)(s.s0 + r / a.G) * a.ldo + (h * a.G + r % a.G) * a.Dh; };
-    const int d = 4 * (lane & 31), r = per * part_of + 2 * (int)(threadIdx.x >> 6) + (lane >> 5);
-    if (per * part_of >= here) return;
+    const int d = 4 * (lane & 31), r = from + 2 * (int)(threadIdx.x >> 6) + (lane >> 5), to = min(here, from + kJoinRows);
+    if (from >= here) return;
     if (!s.ok) {
-        if (!prompts && r < here && d < a.Dh) *reinterpret_cast<half4_t *>(out_of(row0 + r) + d) = half4_t{};
+        if (!prompts || a.few == 0)
+            for (int k = r; k < to && d < a.Dh; k += 2 * kWaves) *reinterpret_cast<half4_t *>(out_of(row0 + k) + d) = half4_t{};
         if (threadIdx.x == 0) report(pb, b);
         return;
     }
     if (prompts != (rows > a.few)) return;
-    double all = 0., some = 0.;
-    for (int b0 = 0; b0 < pb.B; b0 += 64) {
-        const Sequence q = lane_sequence(a, b0);
-        const double u = prompts ? BigShare(a, q).units(a) : Share(a, kRows, q).units;
-        all += u;
-        some += b0 + lane < b ? u : 0.;
-    }
     const Parts in(a, s, kRows, h, tile, uniform((int)(unsigned)wave_sum_f64(all)), uniform((int)(unsigned)wave_sum_f64(some)));
     if (in.count == 1) return;
     const float *part = prompts ? a.big_part : a.part, *stats = prompts ? a.big_stats : a.stats;
     constexpr int kAtOnce = 4;                 // parts at once, of two rows
-    for (int k = 0; k < per && per * part_of + k < here; k += 4 * kWaves) {
+    for (int k = from; k < to; k += 4 * kWaves) {
         Joined<4> j[2];
         for (int p0 = 0; p0 < in.count; p0 += kAtOnce) {
             float2 st[2][kAtOnce];
@@ -1283,7 +1301,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_tiles_kernel(At
             for (int e = 0; e < 2; e++)
 #pragma unroll
                 for (int p = 0; p < kAtOnce; p++) {
-                    const int64_t at = (int64_t)in.slot(min(p0 + p, in.count - 1)) * tile_rows + min(r + k + 2 * kWaves * e, here - 1);
+                    const int64_t at = (int64_t)in.slot(min(p0 + p, in.count - 1)) * tile_rows + min(r + k - from + 2 * kWaves * e, to - 1);
                     st[e][p] = *reinterpret_cast<const float2 *>(stats + 2 * at);
                     const float4_t x = *reinterpret_cast<const float4_t *>(part + at * a.Dh + min(d, a.Dh - 4));
 #pragma unroll
@@ -1295,8 +1313,8 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_tiles_kernel(At
 #pragma unroll
         for (int e = 0; e < 2; e++) {
             const float y = j[e].l == 0.f ? 0.f : 1.f / j[e].l;
-            const int row = r + k + 2 * kWaves * e;
-            if (row < here && row < per * (part_of + 1) && d < a.Dh)
+            const int row = r + k - from + 2 * kWaves * e;
+            if (row < to && d < a.Dh)
                 *reinterpret_cast<half4_t *>(out_of(row0 + row) + d) = half4_t{f2h(j[e].o[0] * y), f2h(j[e].o[1] * y), f2h(j[e].o[2] * y), f2h(j[e].o[3] * y)};
         }
     }
@@ -1327,18 +1345,20 @@ Units tiles_of(const AttnArgs &a, int rows)
     const int64_t most = ((int64_t)a.max_new * a.G + rows - 1) / rows;
     return a.G > rows ? Units{(int)most, 1, 1, most * a.pb.B} : make_units(a.pb.T, a.pb.B, tokens, 1, most);
 }
+int launch_join_prompts(const AttnArgs &a, hipStream_t st)
+{
+    const Units few = a.few ? tiles_of(a, 32) : Units{1, 1, 1, 0}, big = tiles_of(a, kPrompt);
+    const int64_t grid = few.count + big.count * (kPrompt / kJoinRows);
+    hipLaunchKernelGGL(paged_attention_join_tiles_kernel, dim3((unsigned)grid, (unsigned)a.Hkv), dim3(kThreads), 0, st, a, big, few);
+    return launch_status("paged_attention (parts)");
+}
 template <int NR>
 int launch_join(const AttnArgs &a, hipStream_t st)
 {
+    if (a.big_groups) return launch_join_prompts(a, st);
     const int64_t rh = (int64_t)a.pb.T * a.H;
-    if (a.big_groups == 0 && rh < 4 * device_cus()) hipLaunchKernelGGL((paged_attention_join_kernel<NR, kWaves>), dim3((unsigned)rh), dim3(kThreads), 0, st, a);
-    else if (a.big_groups == 0 && rh < 32 * device_cus())
-        hipLaunchKernelGGL((paged_attention_join_kernel<NR, 1>), dim3((unsigned)((rh + kWaves - 1) / kWaves)), dim3(kThreads), 0, st, a);
-    else {
-        const Units few = tiles_of(a, 16 * NR), big = a.big_groups ? tiles_of(a, kPrompt) : Units{1, 1, 1, 0};
-        const int64_t grid = few.count * (16 * NR / kJoinRows) + big.count * (kPrompt / kBigJoinRows);
-        hipLaunchKernelGGL(paged_attention_join_tiles_kernel<NR>, dim3((unsigned)grid, (unsigned)a.Hkv), dim3(kThreads), 0, st, a, big, few);
-    }
+    if (rh < 4 * device_cus()) hipLaunchKernelGGL((paged_attention_join_kernel<NR, kWaves>), dim3((unsigned)rh), dim3(kThreads), 0, st, a);
+    else hipLaunchKernelGGL((paged_attention_join_kernel<NR, 1>), dim3((unsigned)((rh + kWaves - 1) / kWaves)), dim3(kThreads), 0, st, a);
     return launch_status("paged_attention (parts)");
 }
 template <int ND, int NR, class P>
@@ -1354,7 +1374,7 @@ int launch_prompts(const AttnArgs &a, hipStream_t st)
     hipLaunchKernelGGL((paged_prompt_kernel<ND, P>), dim3((unsigned)a.big_groups), dim3(kBigThreads), 0, st, a);
     const int rc = launch_status("paged_attention (prompts)");
     if (rc) return rc;
-    return a.few > 0 ? launch<ND, 2, P>(a, st) : launch_join<2>(a, st);        // (one sequence: there are no others)
+    return a.few > 0 ? launch<ND, 2, P>(a, st) : launch_join_prompts(a, st);        // (one sequence: there are no others)
 }
 template <class P>
 int launch(const AttnArgs &a, int NR, hipStream_t st)
