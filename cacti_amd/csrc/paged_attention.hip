@@ -806,8 +806,9 @@ struct Prompt {
             if (x + kBig <= end) {
                 const char *before = nullptr;
 #pragma unroll
-                for (int i = 0; i < kPieces; i++) {    // (first < 16; kApart: 8 or a multiple of 16)
-                    const char *k = kApart < 16 && (i & 1) ? nullptr : page_at(a.k_pages, x + i * kApart) + first * a.Dp * (int)sizeof(P);
+                for (int i = 0; i < kPieces; i++) {    // (kApart: 8, two pieces to 16 positions, or a multiple of 16)
+                    const char *k = kApart < 16 && (i & 1) ? nullptr
+                                                           : page_at(a.k_pages, x + (first & ~15) + i * kApart) + (first & 15) * a.Dp * (int)sizeof(P);
                     if (kApart < 16 && (i & 1)) k = before + kApart * a.Dp * (int)sizeof(P);
                     next.k[i] = *reinterpret_cast<const u4_t *>(k + w.from);
                     before = k;

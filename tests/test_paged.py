@@ -412,6 +412,10 @@ ATTENDS = [
     ([130, 1, 47], [131, 900, 100], 4, 4, 100, 64),          # prompts
     ([90], [777], 4, 2, 80, 48),
     ([3], [260], 2, 1, 128, 256),
+    ([37, 5, 64], [37, 5, 64], 4, 2, 36, 16),                # prompts of narrow heads and single tokens, pages of 16
+    ([100, 70], [300, 333], 2, 2, 64, 16),
+    ([100, 1, 70], [310, 400, 333], 2, 1, 4, 32),
+    ([200, 2], [211, 130], 3, 1, 128, 16),
 ]
 
 
