@@ -7,8 +7,9 @@
 //
 // A workgroup to a row, which it holds in registers from one read on: the forward pass is bound by that read, the adjoint, which
 // takes the maximum and the sum from the forward pass (stats) and has nothing to reduce over the row, by a read and a write.
-// 2048 rows of 32000, K = 64: forward 27.3 us, 4.8 TB/s (a maximum and then a sum out of memory again: 43.8), adjoint 46.7 us,
-// 5.6 TB/s; 611 of 8191, K = 20: 5.9 and 7.0 us; 128 of 1024, K = 8: 4.0 and 3.3 us, latency.
+// 2048 rows of 32000, K = 64: forward 29 us, 4.5 TB/s (a maximum and then a sum out of memory again: 44), adjoint 46.7 us,
+// 5.6 TB/s, and one after the other, when the forward pass has the gradients written before it go to memory beside it, 85.7;
+// 611 of 8191, K = 20: 6.9 and 8.1 us; 128 of 1024, K = 8: 4.0 and 3.3 us, latency.
 #include "vocab_row.h"
 
 using namespace cacti;

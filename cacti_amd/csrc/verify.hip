@@ -10,14 +10,14 @@
 //
 // Exponentials and sums are fp64: what is drawn goes by on which side of a border of the running sum r lies, and with sums that
 // are off by e of their total some V e of all draws come out differently (32000 tokens, fp32 sums: one in several hundred).
-// That arithmetic, some 19 operations of 64 bits a logit, is what bounds a batch (twice the time that its bytes take).
+// That arithmetic, some 17 operations of 64 bits a logit, is what bounds a batch (twice the time that its bytes take).
 //
-// A row is cut into entries of 1024 logits, one to a wave, which needs no barrier and spreads five rows over 80 workgroups: their
-// maxima and sums relative to them, of every row of both models.  Then a workgroup per sequence forms the rows' sums from
-// them, sees which drafted tokens are kept and sums what is left of p in the first row whose token is not, entry by entry; one of
-// its waves finds the entry in which r lies and the token in it.
-// us, five rows of 32000 with a drafting model / 64 sequences, 294 rows: a workgroup per row that drew for every row that might
-// end its sequence 77 / 115; a launch of its own for the last step, which waits for memory four times over, 22.5 / 38.6.
+// Three launches, each as wide as its work.  A row is cut into entries of 2048 logits, one to a wave, which needs no barrier and
+// spreads five rows over 20 workgroups: their maxima and sums relative to them, of every row of both models.  Then workgroups of
+// each sequence form the rows' sums from them, see which drafted tokens are kept and sum what is left of p in the first row whose
+// token is not, 512 logits to a wave.  Then a workgroup of each sequence finds the entry in which r lies and the token in it.
+// us, five rows of 32000 with a drafting model / 64 sequences, 294 rows: 16.6 / 34.0, of which the first launch is 4 / 18; a
+// workgroup per row that drew for every row that might end its sequence 77 / 115, one per sequence for the last two steps 22.5 / 38.6.
 #include "vocab_row.h"
 
 using namespace cacti;
