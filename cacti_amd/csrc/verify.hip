@@ -16,8 +16,9 @@
 // spreads five rows over 20 workgroups: their maxima and sums relative to them, of every row of both models.  Then workgroups of
 // each sequence form the rows' sums from them, see which drafted tokens are kept and sum what is left of p in the first row whose
 // token is not, 512 logits to a wave.  Then a workgroup of each sequence finds the entry in which r lies and the token in it.
-// us, five rows of 32000 with a drafting model / 64 sequences, 294 rows: 16.6 / 34.0, of which the first launch is 4 / 18; a
-// workgroup per row that drew for every row that might end its sequence 77 / 115, one per sequence for the last two steps 22.5 / 38.6.
+// us, five rows of 32000 with a drafting model / 64 sequences, 294 rows: 15.9 / 33.9, of which the first launch is 4 / 18; a
+// workgroup per row that drew for every row that might end its sequence 77 / 115, one per sequence for the last two steps 22.5 / 38.6;
+// the last step by the last of a sequence's workgroups to write, which takes fences between the XCDs, 18.1 / 116.
 #include "vocab_row.h"
 
 using namespace cacti;
@@ -310,7 +311,7 @@ __global__ void __launch_bounds__(kThreads) verify_rows_kernel(VerifyArgs a)
 __global__ void __launch_bounds__(kDraw) verify_draw_kernel(VerifyArgs a)
 {
     __shared__ double waves[kDraw / 64];
-    __shared__ int first, last;
+    __shared__ int first, last, token;
     const int b = blockIdx.x, wid = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const Head h = a.heads[b];
     const int s0 = a.starts[b], s1 = a.starts[b + 1];
@@ -363,9 +364,8 @@ __global__ void __launch_bounds__(kDraw) verify_draw_kernel(VerifyArgs a)
     mine = w[0] + w[1];
     upto = block_scan(mine, &total) + before;
     const int lane_of = pick_lane(mine > 0. && upto > want, mine > 0., &first, &last);
-    if ((int)threadIdx.x == lane_of) first = j + !(w[0] > 0. && (upto - w[1] > want || !(w[1] > 0.)));
+    if ((int)threadIdx.x == lane_of) token = j + !(w[0] > 0. && (upto - w[1] > want || !(w[1] > 0.)));
     __syncthreads();
-    const int token = first;
     write_out<kDraw>(a, b, s0, s1, h.row, min(max(token, 0), a.V - 1));
 }
 
