@@ -212,8 +212,18 @@ __global__ void __launch_bounds__(T) paged_append_kernel(AppendArgs a)
             Item<HV> it;
             it.rotated(x[e], c[e], sn[e]);
             half_t *to = a.q_out + (int64_t)(row0 + e) * a.ldqo + h * a.Dh + d;
-            put<HV>(to, it.a, 1.f);
-            put<HV>(to + half, it.b, 1.f);
+            // an item that reaches back writes its own columns only: the others may be the input's, which another thread has yet to read
+            const int own = (i - i / a.per * a.per) * HV - d;
+            if (own == 0) {
+                put<HV>(to, it.a, 1.f);
+                put<HV>(to + half, it.b, 1.f);
+            } else
+#pragma unroll
+                for (int k = 2; k < HV; k++)
+                    if (k >= own) {
+                        to[k] = f2h(it.a[k]);
+                        to[half + k] = f2h(it.b[k]);
+                    }
         }
         return;
     }

@@ -1409,6 +1409,8 @@ CACTI_API int cacti_hip_paged_attention_f16(int64_t T, int64_t B, int64_t H, int
                   "paged_attention: operands must be 8-byte aligned with row pitches that are multiples of 4 and hold a row");
     CACTI_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= cacti_hip_paged_attention_workspace(T, B, H, Hkv, Dh, max_new),
                   CACTI_E_INVALID, "paged_attention: workspace too small or not 16-byte aligned");
+    CACTI_REQUIRE(fabsf(alpha) < INFINITY, CACTI_E_INVALID, "paged_attention: alpha is not finite");
+    CACTI_REQUIRE(q != out, CACTI_E_INVALID, "paged_attention: the output cannot take the queries' place, which other workgroups read");
     const int64_t most = (max_new < T ? max_new : T) * (H / Hkv) / 16 + 1;         // tiles of a sequence; work is counted in 32 bits
     CACTI_REQUIRE(T * H < (1 << 24) && (most < T * (H / Hkv) / 16 + B ? most * B : T * (H / Hkv) / 16 + B) * Hkv <
                       INT32_MAX / (W * page / kStep + 1 + begin_of(32)), CACTI_E_NOTIMPL, "paged_attention: too many rows and positions in one call");

@@ -46,7 +46,8 @@ def test_append_refuses(change, why):
 
 @pytest.mark.parametrize("change,why", COMMON + [(dict(q=None), "null"), (dict(out=None), "null"), (dict(ldo=30), "multiples of 4"),
                                                  (dict(ws_bytes=64), "workspace"), (dict(ws=72), "workspace"),
-                                                 (dict(ws=None), "workspace")])
+                                                 (dict(ws=None), "workspace"), (dict(alpha=float("nan")), "alpha"),
+                                                 (dict(alpha=float("-inf")), "alpha"), (dict(), "output")])
 def test_attention_refuses(change, why):
     L = ffi.lib()
     assert L.cacti_hip_paged_attention_f16(*dict(ATTEND, **change).values()) < 0
@@ -306,6 +307,19 @@ def test_append_values_at_the_edge():
 
 
 @GPU
+@pytest.mark.parametrize("Dh", [4, 36, 100, 128])
+def test_append_rotates_queries_in_place(Dh):
+    import torch
+    from cacti_amd import ops
+    for n, lens in (([1, 1], [9, 70]), ([90, 3], [95, 16])):
+        B = Batch(18 + Dh, n, lens, 8, 2, Dh, 64, 16)
+        cache = B.put()
+        want = ops.paged_append(B.d["k"], B.d["v"], cache, *B.at(), B.d["cos"], B.d["sin"], q=B.d["q"]).clone()
+        got = ops.paged_append(B.d["k"], B.d["v"], cache, *B.at(), B.d["cos"], B.d["sin"], q=B.d["q"], out=B.d["q"])
+        assert got is B.d["q"] and torch.equal(got, want)
+
+
+@GPU
 def test_append_leaves_the_rest_alone():
     """Slots behind the new ones, rows behind the last sequence and their queries; appending the same rows again changes nothing."""
     import torch
@@ -416,6 +430,8 @@ ATTENDS = [
     ([100, 70], [300, 333], 2, 2, 64, 16),
     ([100, 1, 70], [310, 400, 333], 2, 1, 4, 32),
     ([200, 2], [211, 130], 3, 1, 128, 16),
+    ([1, 3], [300, 90], 72, 1, 64, 16),                      # a token's query heads fill more than a tile
+    ([2], [70], 130, 1, 20, 16),
 ]
 
 
@@ -491,6 +507,40 @@ def test_attention_looks_at_nothing_hidden(bits):
             if which is vp or np.isnan(v) or bits == 8:
                 check_attention(B, (kp, vp, B.ks, B.vs))
             which[:] = was
+
+
+@GPU
+@pytest.mark.parametrize("n,lens", [([70], [75]), ([70, 2], [75, 40])])
+def test_attention_of_a_prompt_that_does_not_fit(n, lens):
+    """A prompt with more positions than its row of the table has: zeros, and whoever stands beside it as ever."""
+    import torch
+    from cacti_amd import ops
+    for bits in (8, 16):
+        B = Batch(43, n, lens, 4, 2, 64, 16, bits)
+        want, tol = B.attend(B.split()[0], (B.kp, B.vp, B.ks, B.vs))
+        cache = B.put()
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        bad = torch.tensor([B.W * B.page + 1] + lens[1:], dtype=torch.int32, device="cuda")
+        out = torch.full((B.T, 4, 64), 7.0, dtype=torch.float16, device="cuda")
+        ops.paged_attention(B.d["q"], cache, B.d["table"], B.d["starts"], bad, B.alpha, out=out, status=status)
+        assert int(status) == 1
+        out = out.cpu().numpy().astype(np.float64)
+        assert (out[:70] == 0).all() and (np.abs(out[70:] - want[70:]) <= tol[70:]).all()
+
+
+@GPU
+def test_attention_infinite_keys_of_a_prompt():
+    """A key with an infinity of a prompt: rows that see it have no number where the score is +inf, no weight where it is -inf."""
+    B = Batch(35, [80], [90], 2, 2, 100, 16, 16)
+    B.kp[B.table[0, 1], 0, 3, 40] = np.inf
+    q = B.split()[0]
+    q[:, 0, 40] = -np.abs(q[:, 0, 40]) - np.float16(1)
+    check_attention(B)
+    q[:, 0, 40] *= np.float16(-1)
+    import torch
+    from cacti_amd import ops
+    out = ops.paged_attention(torch.from_numpy(q.copy()).cuda(), B.put(), *B.at(), B.alpha).cpu().numpy()
+    assert np.isfinite(out[:9]).all() and np.isnan(out[9:, 0]).all() and np.isfinite(out[:, 1]).all()
 
 
 @GPU
