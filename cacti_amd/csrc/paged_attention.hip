@@ -1,9 +1,9 @@
 // Causal attention of the new rows of a ragged batch over a paged cache, in e4m3 with a scale per page and head or in f16:
 //   o = sum_j softmax_j(alpha q . k_j) v_j     over the positions j up to the row's own
 //
-// One pass over the keys with a running maximum.  The codes meet the queries as they are (e4m3 to f16 is exact) and a page's
-// scales join the scores: with t_j = alpha ks q . k_j log2 e + log2 vs and m the maximum of t so far,
-//   w_j = 2^(t_j - m) <= 1,  o = sum w_j code(v_j) / sum w_j / vs
+// One pass over the keys with a running m, which is the maximum of a row's scores so far or up to kSlack less.  The codes meet the
+// queries as they are (e4m3 to f16 is exact) and a page's scales join the scores: with t_j = alpha ks q . k_j log2 e + log2 vs,
+//   w_j = 2^(t_j - m) <= 2^kSlack,  o = sum w_j code(v_j) / sum w_j / vs
 // so that the weight that meets a code already holds its page's scale, and no w exceeds f16 whatever the scales are.
 // Scores, maxima, sums and o are fp32; w is rounded to f16 for the matrix instruction (2^-11 relative, each on its own, which
 // is what the rounding of the output adds once more).
@@ -347,10 +347,23 @@ struct Entry {
     int64_t at[kEntries];
     float c[kEntries], lg[kEntries], iv[kEntries];         // alpha ks log2 e (more than 0), log2 vs, 1 / vs
 };
+struct Scales {
+    float c, lg, iv;
+};
+// ... of page pg; pages of 16 bits have none
+template <class P>
+__device__ __forceinline__ Scales scales_of(const Entry &e, int pg, float alpha)
+{
+    if (sizeof(P) == 2) return {fmaxf(alpha * 1.44269504088896340736f, 1e-30f), 0.f, 1.f};
+    return {e.c[pg], e.lg[pg], e.iv[pg]};
+}
 
 // The scores s of 32 positions of a lane's row (eight of them, in two registers of four) to weights: with c > 0 and lg of the
-// lane's page, t = s c + lg.  Takes part in the running maximum m and sum l (of weights by iv) and scales o where m grows; returns
-// the weights in f16.  seen: how many of the lane's eight positions its row sees; edge (the same in all lanes): not all of all.
+// lane's page, t = s c + lg.  Takes part in the running m and sum l (of weights by iv) and scales o where m grows; returns the
+// weights in f16.  seen: how many of the lane's eight positions its row sees; edge (the same in all lanes): not all of all.
+// m grows only where a lane has more than kSlack above it: else the row's lanes need not hear of each other's scores (prompts of
+// up to 900 rows and 4000 positions, 16 heads of 128: 78.6 -> 74.1 us against no slack).
+constexpr float kSlack = 8.f;
 template <int N>
 __device__ __forceinline__ half8_t weigh(float4_t (&s)[2], float c, float lg, float iv, float &m, float &l, float4_t (&o)[N], bool edge, int seen)
 {
@@ -361,21 +374,20 @@ __device__ __forceinline__ half8_t weigh(float4_t (&s)[2], float c, float lg, fl
     float raw = s[0][0];                       // (c > 0: the largest of t is that of the largest of s)
 #pragma unroll
     for (int i = 1; i < 8; i++) raw = fmaxf(raw, s[i / 4][i & 3]);
-    float mx = __builtin_fmaf(raw, c, lg);
-    mx = with32(with16(mx, OpMax()), OpMax());
-    const float mn = fmaxf(m, mx), origin = finite_max(mn);
-    if (__ballot(mn > m)) {                    // some row's maximum has grown
-        const float f = exp2_of(m - origin);
+    const float mine = __builtin_fmaf(raw, c, lg);
+    if (__ballot(mine > m + kSlack)) {
+        const float mn = fmaxf(m, with32(with16(mine, OpMax()), OpMax())), f = exp2_of(m - finite_max(mn));
         m = mn;
         l *= f;
 #pragma unroll
         for (int i = 0; i < N; i++) o[i] *= f;
     }
+    const float off = lg - finite_max(m);
     float sum = 0.f;
     Frag p;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const float x = exp2_of(__builtin_fmaf(s[i / 2][2 * i & 3], c, lg - origin)), y = exp2_of(__builtin_fmaf(s[i / 2][(2 * i & 3) + 1], c, lg - origin));
+        const float x = exp2_of(__builtin_fmaf(s[i / 2][2 * i & 3], c, off)), y = exp2_of(__builtin_fmaf(s[i / 2][(2 * i & 3) + 1], c, off));
         sum += x + y;
         const half2_t pair = {f2h(x), f2h(y)};
         p.u[i] = __builtin_bit_cast(unsigned, pair);
@@ -517,11 +529,11 @@ struct Tile {
             for (int n = 0; n < NR; n++) sc[n][t] = q[n].times(kk[t]);
         load_k(next, end);
         const int pg = page_of(min(x + 8 * g, end - 1));       // of the lane's eight keys
-        const float ec = entry.c[pg], lg = entry.lg[pg], iv = entry.iv[pg];
+        const Scales sc8 = scales_of<P>(entry, pg, a.alpha);
         half8_t w[NR];
 #pragma unroll
         for (int n = 0; n < NR; n++)
-            w[n] = weigh(sc[n], ec * factor[n], lg, iv, m[n], l[n], o[n], edge, min(last[n] - base, end - 1) - (x + 8 * g) + 1);
+            w[n] = weigh(sc[n], sc8.c * factor[n], sc8.lg, sc8.iv, m[n], l[n], o[n], edge, min(last[n] - base, end - 1) - (x + 8 * g) + 1);
         if (edge) {
             // what no row of the tile sees is nothing; a NaN or an infinity that some rows see must not meet the zero weights of
             // the others: it is added at the end
@@ -921,11 +933,12 @@ struct Prompt {
 #pragma unroll
         for (int c = 0; c < 4; c++) vf[c] = *reinterpret_cast<const half8_t *>(vb + (v0 ^ (32 * (c & 1))) + 16 * c * kBig);
         const int pg = page_of(min(x + 8 * g, end - 1));
+        const Scales sc8 = scales_of<P>(sh.entry, pg, a.alpha);
         const bool edge = x + 31 > min(least, end - 1);
         half8_t p[2];
 #pragma unroll
         for (int n = 0; n < 2; n++)
-            p[n] = weigh(sc[n], sh.entry.c[pg], sh.entry.lg[pg], sh.entry.iv[pg], m[n], l[n], o[n], edge, min(last[n] - base, end - 1) - (x + 8 * g) + 1);
+            p[n] = weigh(sc[n], sc8.c, sc8.lg, sc8.iv, m[n], l[n], o[n], edge, min(last[n] - base, end - 1) - (x + 8 * g) + 1);
 #pragma unroll
         for (int c = 0; c < 4 * ND; c++) {
 #pragma unroll
