@@ -1343,14 +1343,16 @@ struct Plan {
         return ((size_t)groups * 2 * (16 * NR) + (size_t)big_groups * 2 * kPrompt) * (size_t)(Dh + 2);
     }
 };
-// Rows of a sequence (tokens by the query heads of a key head) that are a prompt's: from there on a workgroup of 128 of them reads
-// the keys fewer times than waves of 32 do
-constexpr int kFew = 64;
+// Rows of a sequence (tokens by the query heads of a key head) up to which waves of 32 of them read the keys no more often than costs
+// less than a prompt's workgroup, where no sequence may have more and where some may: two launches one after the other then.
+// (24 sequences of up to 128 rows, as prompts from 64 / 96 / 128 on: 58 / 66 / 39 us, 8 of 192, from 128 / 192: 63 / 92; beside others, 12
+// of up to 160, kFew 32 / 64 / 128: 72 / 77 / 92)
+constexpr int kNoPrompt = 128, kFew = 32;
 Plan plan(int64_t T, int64_t B, int64_t H, int64_t Hkv, int64_t Dh, int64_t max_new, int bytes)
 {
     const int64_t G = H / Hkv, rows = (max_new < T ? max_new : T) * G;
     const int NR = rows <= 16 ? 1 : 2;
-    if (rows > kFew) return {2, 2 * device_cus(), B == 1 ? 0 : kFew, 2 * device_cus()};
+    if (rows > kNoPrompt) return {2, 2 * device_cus(), B == 1 ? 0 : kFew, 2 * device_cus()};
     return {NR, resident(Dh <= 64 ? 1 : 2, NR, bytes) * device_cus(), INT32_MAX, 0};
 }
 

@@ -426,8 +426,9 @@ ATTENDS = [
     ([130, 1, 47], [131, 900, 100], 4, 4, 100, 64),          # prompts
     ([90], [777], 4, 2, 80, 48),
     ([3], [260], 2, 1, 128, 256),
-    ([37, 5, 64], [37, 5, 64], 4, 2, 36, 16),                # prompts of narrow heads and single tokens, pages of 16
-    ([100, 70], [300, 333], 2, 2, 64, 16),
+    ([37, 5, 64], [37, 5, 64], 4, 2, 36, 16),                # up to 128 rows of a key head
+    ([37, 5, 80], [37, 5, 80], 4, 2, 36, 16),                # prompts of narrow heads, pages of 16
+    ([140, 33, 32], [300, 333, 90], 2, 2, 64, 16),
     ([100, 1, 70], [310, 400, 333], 2, 1, 4, 32),
     ([200, 2], [211, 130], 3, 1, 128, 16),
     ([1, 3], [300, 90], 72, 1, 64, 16),                      # a token's query heads fill more than a tile
@@ -481,10 +482,11 @@ def test_attention_of_large_scores():
 
 @GPU
 @pytest.mark.parametrize("bits", [8, 16])
-def test_attention_looks_at_nothing_hidden(bits):
+@pytest.mark.parametrize("last", [40, 70])                   # 70: a prompt
+def test_attention_looks_at_nothing_hidden(last, bits):
     """NaN (and infinities) behind the last position, in other sequences' and in spare pages; rows that see a NaN have it,
     rows before it do not."""
-    B = Batch(33, [6, 1, 40], [70, 31, 40], 4, 2, 64, 16, bits)
+    B = Batch(33, [6, 1, last], [70, 31, last], 4, 2, 64, 16, bits)
     clean = check_attention(B)
     poison = np.uint8(0x7f) if bits == 8 else np.float16(np.nan)
     kp, vp = B.kp.copy(), B.vp.copy()
@@ -531,7 +533,7 @@ def test_attention_of_a_prompt_that_does_not_fit(n, lens):
 @GPU
 def test_attention_infinite_keys_of_a_prompt():
     """A key with an infinity of a prompt: rows that see it have no number where the score is +inf, no weight where it is -inf."""
-    B = Batch(35, [80], [90], 2, 2, 100, 16, 16)
+    B = Batch(35, [140], [150], 2, 2, 100, 16, 16)
     B.kp[B.table[0, 1], 0, 3, 40] = np.inf
     q = B.split()[0]
     q[:, 0, 40] = -np.abs(q[:, 0, 40]) - np.float16(1)

@@ -78,7 +78,7 @@ def test_draft_and_verify(bits, captured):
     import torch
     from cacti_amd import ops
     r = np.random.default_rng(40 + bits)
-    prompts, rounds, W = [list(r.integers(0, V, n)) for n in (37, 5, 64)], 5, 7
+    prompts, rounds, W = [list(r.integers(0, V, n)) for n in (37, 5, 80)], 5, 7
     B = len(prompts)
     target, draft = Model(r, bits, B, W, 0.12), Model(r, bits, B, W, 0.12)
     # the drafting model is near the target model
