@@ -1,12 +1,14 @@
 // Causal attention of the new rows of a ragged batch over a paged cache, in e4m3 with a scale per page and head or in f16:
 //   o = sum_j softmax_j(alpha q . k_j) v_j     over the positions j up to the row's own
 //
-// One pass over the keys with a running m, which is the maximum of a row's scores so far or up to kSlack less.  The codes meet the
-// queries as they are (e4m3 to f16 is exact) and a page's scales join the scores: with t_j = alpha ks q . k_j log2 e + log2 vs,
-//   w_j = 2^(t_j - m) <= 2^kSlack,  o = sum w_j code(v_j) / sum w_j / vs
+// One pass over the keys with a running m, the maximum of a row's scores so far (or, prompts in 16 bits, up to kSlack less).  The codes
+// meet the queries as they are (e4m3 to f16 is exact) and a page's scales join the scores: with t_j = alpha ks q . k_j log2 e + log2 vs,
+//   w_j = 2^(t_j - m),  o = sum w_j code(v_j) / sum w_j / vs
 // so that the weight that meets a code already holds its page's scale, and no w exceeds f16 whatever the scales are.
 // Scores, maxima, sums and o are fp32; w is rounded to f16 for the matrix instruction (2^-11 relative, each on its own, which
-// is what the rounding of the output adds once more).
+// is what the rounding of the output adds once more).  The sum is that of w as it was, since a page of small values may have
+// weights that are nothing in f16 and most of the probability; the largest w is 1, and exact.  With kSlack it need not be, but there
+// are no scales then: the sum is that of the rounded w, and what a large one is off by is off in both.
 //
 // A wave takes 16 NR rows (tokens of a sequence by the query heads that share a key head) of a key head at a time, by itself, 32
 // positions at a time.  The products are formed transposed, S^T = K Q^T and O^T = V^T W^T with v_mfma_f32_16x16x32_f16: a lane
@@ -361,10 +363,22 @@ __device__ __forceinline__ Scales scales_of(const Entry &e, int pg, float alpha)
 // The scores s of 32 positions of a lane's row (eight of them, in two registers of four) to weights: with c > 0 and lg of the
 // lane's page, t = s c + lg.  Takes part in the running m and sum l (of weights by iv) and scales o where m grows; returns the
 // weights in f16.  seen: how many of the lane's eight positions its row sees; edge (the same in all lanes): not all of all.
-// m grows only where a lane has more than kSlack above it: else the row's lanes need not hear of each other's scores (prompts of
-// up to 900 rows and 4000 positions, 16 heads of 128: 78.6 -> 74.1 us against no slack).
+// SLACK: m grows only where a lane has more than kSlack above it, else the row's lanes need not hear of each other's scores, and w
+// may be up to 2^kSlack (prompts in 16 bits of up to 900 rows and 4000 positions, 16 heads of 128: 78.6 -> 74.1 us; single tokens, bound
+// by memory, gain nothing).
 constexpr float kSlack = 8.f;
-template <int N>
+// x + a half of h, the conversion and the sum (in fp32) in one operation
+__device__ __forceinline__ float plus_low(float x, unsigned h)
+{
+    asm("v_fma_mix_f32 %0, %1, 1.0, %0 op_sel:[0,0,0] op_sel_hi:[1,0,0]" : "+v"(x) : "v"(h));
+    return x;
+}
+__device__ __forceinline__ float plus_high(float x, unsigned h)
+{
+    asm("v_fma_mix_f32 %0, %1, 1.0, %0 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(x) : "v"(h));
+    return x;
+}
+template <bool SLACK, int N>
 __device__ __forceinline__ half8_t weigh(float4_t (&s)[2], float c, float lg, float iv, float &m, float &l, float4_t (&o)[N], bool edge, int seen)
 {
     if (edge) {
@@ -375,7 +389,7 @@ __device__ __forceinline__ half8_t weigh(float4_t (&s)[2], float c, float lg, fl
 #pragma unroll
     for (int i = 1; i < 8; i++) raw = fmaxf(raw, s[i / 4][i & 3]);
     const float mine = __builtin_fmaf(raw, c, lg);
-    if (__ballot(mine > m + kSlack)) {
+    if (__ballot(mine > (SLACK ? m + kSlack : m))) {
         const float mn = fmaxf(m, with32(with16(mine, OpMax()), OpMax())), f = exp2_of(m - finite_max(mn));
         m = mn;
         l *= f;
@@ -383,16 +397,17 @@ __device__ __forceinline__ half8_t weigh(float4_t (&s)[2], float c, float lg, fl
         for (int i = 0; i < N; i++) o[i] *= f;
     }
     const float off = lg - finite_max(m);
-    float sum = 0.f;
+    float even = 0.f, uneven = 0.f;
     Frag p;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const float x = exp2_of(__builtin_fmaf(s[i / 2][2 * i & 3], c, off)), y = exp2_of(__builtin_fmaf(s[i / 2][(2 * i & 3) + 1], c, off));
-        sum += x + y;
         const half2_t pair = {f2h(x), f2h(y)};
         p.u[i] = __builtin_bit_cast(unsigned, pair);
+        even = SLACK ? plus_low(even, p.u[i]) : even + x;
+        uneven = SLACK ? plus_high(uneven, p.u[i]) : uneven + y;
     }
-    l = __builtin_fmaf(sum, iv, l);
+    l = __builtin_fmaf(even + uneven, iv, l);
     return p.h;
 }
 
@@ -533,7 +548,7 @@ struct Tile {
         half8_t w[NR];
 #pragma unroll
         for (int n = 0; n < NR; n++)
-            w[n] = weigh(sc[n], sc8.c * factor[n], sc8.lg, sc8.iv, m[n], l[n], o[n], edge, min(last[n] - base, end - 1) - (x + 8 * g) + 1);
+            w[n] = weigh<false>(sc[n], sc8.c * factor[n], sc8.lg, sc8.iv, m[n], l[n], o[n], edge, min(last[n] - base, end - 1) - (x + 8 * g) + 1);
         if (edge) {
             // what no row of the tile sees is nothing; a NaN or an infinity that some rows see must not meet the zero weights of
             // the others: it is added at the end
@@ -940,7 +955,7 @@ struct Prompt {
         half8_t p[2];
 #pragma unroll
         for (int n = 0; n < 2; n++)
-            p[n] = weigh(sc[n], sc8.c, sc8.lg, sc8.iv, m[n], l[n], o[n], edge, min(last[n] - base, end - 1) - (x + 8 * g) + 1);
+            p[n] = weigh<sizeof(P) == 2>(sc[n], sc8.c, sc8.lg, sc8.iv, m[n], l[n], o[n], edge, min(last[n] - base, end - 1) - (x + 8 * g) + 1);
 #pragma unroll
         for (int c = 0; c < 4 * ND; c++) {
 #pragma unroll

@@ -4,10 +4,10 @@ Appending is compared bit for bit: the rotation's products are exact in fp32 (11
 once more into the page, and the quotient by a power of two rounds nothing (the values stay clear of fp32's subnormals).
 
 Attention is compared with float64.  What the kernel rounds: the output, half a step of f16, 2^-11 |o|; each weight once to
-f16, 2^-11 of it, so at most 2^-11 sum p |v| in the numerator and no more in the sum of the weights, which is of unrounded ones;
-a score, a sum of up to 128 products in fp32, 128 * 2^-24 A with A = max_j alpha sum_d |q_d k_jd|, and the exponent's own
+f16, w (1 + d) with |d| <= 2^-11, in the numerator and, prompts in 16 bits, in the sum of the weights, so that o is off by sum p d (v - o) (to
+first order), at most 2^-11 (sum p |v| + |o|); a score, a sum of up to 128 products in fp32, 128 * 2^-24 A with A = max_j alpha sum_d |q_d k_jd|, and the exponent's own
 rounding and the exponential's (2^-22 (1 + A)), a relative error of each weight in numerator and denominator.  Together
-  2^-11 |o| + (2^-11 + 2 (2^-17 A + 2^-22 (1 + A))) sum p |v| + 2^-25 (half a step of f16's subnormals)
+  2^-10 |o| + (2^-11 + 2 (2^-17 A + 2^-22 (1 + A))) sum p |v| + 2^-25 (half a step of f16's subnormals)
 Against codes of 8 bits a query is the sum of three e4m3 terms, scaled to have its largest element between 224 and 448: an element
 of 11 bits takes 4 + 5 + 5 of them exactly unless its lowest fall below half a step of e4m3's subnormals, 2^-10, which is 2^-17.8
 of the largest; so a score is off by at most 2^-17.8 alpha max|q| sum_d |k_d| more.
@@ -195,7 +195,7 @@ class Batch:
                         eps = 2.0 ** -17 * A + 2.0 ** -22 * (1 + A)
                         if self.bits == 8:
                             eps += 2.0 ** -17.8 * self.alpha * np.abs(qv).max() * np.abs(k).sum(1).max()
-                    tol[row, h] += 2.0 ** -11 * np.abs(o[row, h]) + (2.0 ** -11 + 2.0 ** -15 + 2 * eps) * near
+                    tol[row, h] += 2.0 ** -10 * np.abs(o[row, h]) + (2.0 ** -11 + 2.0 ** -15 + 2 * eps) * near
         return o, tol
 
     # ---- on the device
