@@ -970,7 +970,7 @@ struct Prompt {
         __builtin_amdgcn_sched_group_barrier(0x8, 8, 0);
     }
 
-    // positions c0 .. c1 - 1 (some) of rows row0 .. of sequence s
+    // positions c0 .. c1 - 1 of rows row0 .. of sequence s; none where a share is behind the last that is seen (c1 > 0)
     __device__ __forceinline__ void run(int b, const Sequence &s, int h, int rows, int row0, int c0, int c1)
     {
         const int wid = uniform((int)threadIdx.x >> 6), lane = lane_here(), tid = 64 * wid + lane, r16 = lane & 15, g = lane >> 4;
@@ -980,7 +980,7 @@ struct Prompt {
             const int p0 = uniform(seg / a.pb.page), most = page_of(min(c1 - p0 * a.pb.page, kEntries * a.pb.page) - 1);
             return a.pb.table[(int64_t)b * a.pb.ldt + p0 + min(lane, most)];
         };
-        int id = look_up(c0);                  // requested with the queries
+        int id = look_up(min(c0, c1 - 1));     // requested with the queries, of a page that there is
         u2_t words[2][2 * NS];
 #pragma unroll
         for (int n = 0; n < 2; n++) {

@@ -511,6 +511,28 @@ def test_attention_looks_at_nothing_hidden(last, bits):
             which[:] = was
 
 
+@pytest.mark.parametrize("G", [1, 2, 3, 4, 7, 8, 16, 40, 130])
+@pytest.mark.parametrize("page", [16, 48, 160, 256])
+def test_prompts_look_up_pages_that_there_are(G, page):
+    """A prompt's tiles are counted by a line that is never below their steps, so a share may begin behind the last position that its
+    tile sees: the kernel's lookup of the first pages, restated, stays within the table's row there, too."""
+    for n in (1, 5, 40, 89, 217, 600):
+        for first in (0, 1, 63, 64, 1000):
+            W = -(-(first + n) // page)
+            tokens = (128 + G - 1) // G
+            base, slope = (first + 63) // 64, (tokens + 63) // 64 if tokens >= 64 else 0
+            for t in range(-(-n * G // 128)):
+                steps = base + slope * (t + 1) if slope else base + t // (64 // tokens) + 1
+                end = first + min(n * G - 1, 128 * t + 127) // G + 1
+                assert 0 < end <= 64 * steps                  # the line: nothing that is seen is left out
+                for k in range(steps):
+                    c0, c1 = 64 * k, end
+                    at = min(c0, c1 - 1)                      # (c0 itself is behind the table's row in some of these)
+                    p0 = at // page
+                    most = (min(c1 - p0 * page, 64 * page) - 1) // page
+                    assert 0 <= p0 and most >= 0 and p0 + min(63, most) < W
+
+
 @GPU
 @pytest.mark.parametrize("n,lens", [([70], [75]), ([70, 2], [75, 40])])
 def test_attention_of_a_prompt_that_does_not_fit(n, lens):
