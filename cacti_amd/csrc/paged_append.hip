@@ -8,7 +8,7 @@
 //
 // A workgroup owns a page and a head: it holds the new rows of that page in registers, takes the least scale that holds them and
 // no less than that of older rows, codes those again where it grew, and writes.  No other workgroup touches that page and head.
-// Bound by memory: four sequences of up to 2048 rows, 32 heads of 100 in 8 bits 37.3 us, of which 16 are the queries' (reading the
+// Bound by memory: four sequences of up to 2048 rows, 32 heads of 100 in 8 bits 38 to 40 us, of which 18 are the queries' (reading the
 // rows once for the scale and again for the codes, two columns at a time: 56.4); 96 of up to 6 rows, 8 heads of 128: 5.4 us; one
 // row 4.0 us, latency.
 #include "paged.h"
@@ -219,10 +219,10 @@ __global__ void __launch_bounds__(T) paged_append_kernel(AppendArgs a)
                 put<HV>(to + half, it.b, 1.f);
             } else
 #pragma unroll
-                for (int k = 2; k < HV; k++)
+                for (int k = 2; k < HV; k += 2)            // (own and the columns are even)
                     if (k >= own) {
-                        to[k] = f2h(it.a[k]);
-                        to[half + k] = f2h(it.b[k]);
+                        *reinterpret_cast<half2_t *>(to + k) = half2_t{f2h(it.a[k]), f2h(it.a[k + 1])};
+                        *reinterpret_cast<half2_t *>(to + half + k) = half2_t{f2h(it.b[k]), f2h(it.b[k + 1])};
                     }
         }
         return;
