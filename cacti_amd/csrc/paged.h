@@ -36,9 +36,9 @@ __device__ __forceinline__ Sequence sequence(const PagedBatch &pb, int b, int64_
     Sequence q;
     const int s1 = pb.starts[b + 1], len = pb.lens[b];
     q.s0 = pb.starts[b];
-    q.n = s1 - q.s0;
-    q.first = len - q.n;
-    q.ok = q.s0 >= 0 && s1 >= q.s0 && s1 <= pb.T && q.n <= max_new && q.first >= 0 && len <= limit;
+    q.n = (int)((unsigned)s1 - (unsigned)q.s0);            // (any numbers: what of this does not fit into 32 bits is not ok)
+    q.first = (int)((unsigned)len - (unsigned)q.n);
+    q.ok = q.s0 >= 0 && s1 >= q.s0 && s1 <= pb.T && q.n <= max_new && len >= q.n && len <= limit;
     return q;
 }
 
