@@ -29,7 +29,7 @@ int paged_batch(const char *who, int64_t T, int64_t B, int64_t H, int64_t Hkv, i
     CACTI_REQUIRE(H % Hkv == 0, CACTI_E_INVALID, "%s: %lld query heads for %lld key heads", who, (long long)H, (long long)Hkv);
     CACTI_REQUIRE(Dh % 4 == 0 && Dh >= 4 && Dh <= 128, CACTI_E_NOTIMPL, "%s: need Dh %% 4 == 0 and Dh <= 128", who);
     CACTI_REQUIRE(page % 16 == 0 && page >= 16 && page <= 256, CACTI_E_NOTIMPL, "%s: pages of 16 to 256 positions, a multiple of 16", who);
-    CACTI_REQUIRE(T <= INT32_MAX / H && B < 65536 * 16 && P <= INT32_MAX && W <= INT32_MAX / page && H <= 4096 && ldt >= W, CACTI_E_NOTIMPL,
+    CACTI_REQUIRE(T <= INT32_MAX / H && B < 65536 * 16 && P <= INT32_MAX && W <= (1 << 30) / page && H <= 4096 && ldt >= W, CACTI_E_NOTIMPL,
                   "%s: too many rows, sequences or pages, or a table pitch below its width", who);
     CACTI_REQUIRE(aligned(k_pages, 16) && aligned(v_pages, 16) && aligned(table, 4) && aligned(starts, 4) && aligned(lens, 4) &&
                       aligned(k_scale, 4) && aligned(v_scale, 4) && aligned(status, 4),

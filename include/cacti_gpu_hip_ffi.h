@@ -442,7 +442,7 @@ int cacti_hip_embed_bwd(int64_t V, int64_t D, int64_t S, const void *tok, const 
  * bits = 8: e4m3 (OCP, no infinities) with scales [P, Hkv] f32, a value being code * scale.  A page is of one sequence where
  * that appends; reading it may be shared.  Heads: H of the queries, Hkv of the cache, H % Hkv == 0, query head h reads
  * h / (H / Hkv).  Dh % 4 == 0, Dh <= 128; page: a multiple of 16, at most 256; k, v, q, out: rows of ld elements, 8-byte
- * aligned, ld % 4 == 0; pages 16-byte aligned.
+ * aligned, ld % 4 == 0; pages 16-byte aligned; W page <= 2^30.
  * status [1] i32 on the device, or NULL: 1 + b where the numbers of sequence b do not fit together (rows beyond T, more new
  * rows than max_new or than positions, more positions than its row of the table or the rotation has, a page that is not in
  * the cache), raised with a maximum: the caller clears it.  Nothing of such a sequence is appended (with a page outside the

@@ -3,7 +3,8 @@ of their ranges.  The plain forms and bounds are those of test_paged.py."""
 import numpy as np
 import pytest
 
-from test_paged import Batch, numpy_of, same_bits
+from cacti_amd import ffi
+from test_paged import APPEND, ATTEND, Batch, numpy_of, same_bits
 
 GPU = pytest.mark.gpu
 
@@ -35,3 +36,16 @@ def test_lengths_at_the_ends_of_32_bits(n, H, Hkv, max_new, length):
         status.zero_()
         out = ops.paged_attention(B.d["q"], cache, B.d["table"], B.d["starts"], lens, B.alpha, status=status, max_new=max_new)
         assert int(status) == bad + 1 and not out[B.starts[bad]:].any()
+
+
+# ---------------------------------------------------------------- sizes at the ends of their ranges
+@pytest.mark.parametrize("page", [16, 48, 256])
+def test_no_more_positions_than_are_counted_in_32_bits(page):
+    """Positions and steps of up to 64 of them, with what a tile of rows has too many, are formed in 32 bits: 2^30 at most."""
+    L = ffi.lib()
+    W = (1 << 31) // page - 1
+    for W, refused in ((W, True), ((1 << 30) // page + 1, True), ((1 << 30) // page, False)):
+        for f, args in ((L.cacti_hip_paged_append, APPEND), (L.cacti_hip_paged_attention_f16, ATTEND)):
+            # (a wrong pitch of the rotation's and of the output's rows ends the calls that are not refused for their table)
+            assert f(*dict(args, page=page, W=W, ldt=W, **({"ldk": 12} if args is APPEND else {"ldo": 30})).values()) < 0
+            assert ("too many rows, sequences or pages" in L.cacti_hip_last_error().decode()) == refused
