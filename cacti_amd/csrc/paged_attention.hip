@@ -1279,8 +1279,24 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs
     if (2 * lane < a.Dh) *reinterpret_cast<half2_t *>(out) = half2_t{f2h(j.o[0] * y), f2h(j.o[1] * y)};
 }
 
+// Of the 64 sequences from b0 on those whose numbers do not fit together: named, and the rows that there are of them zeros (of the query
+// heads of key head h)
+__device__ __forceinline__ void clear_misfits(const AttnArgs &a, int b0, int h)
+{
+    const int lane = threadIdx.x & 63, b = min(b0 + lane, a.pb.B - 1);
+    const bool bad = b0 + lane < a.pb.B && !lane_sequence(a, b0).ok;
+    const int from = max(a.pb.starts[b], 0), to = bad ? min(a.pb.starts[b + 1], a.pb.T) : 0;
+    if (bad && h == 0 && threadIdx.x < 64) report(a.pb, b);
+    for (uint64_t rest = __ballot(from < to); rest; rest &= rest - 1) {
+        const int at = __ffsll((unsigned long long)rest) - 1, end = __builtin_amdgcn_readlane(to, at);
+        for (int row = __builtin_amdgcn_readlane(from, at) + uniform((int)threadIdx.x >> 6); row < end; row += kWaves)
+            for (int d = 4 * lane; d < a.G * a.Dh; d += 256) *reinterpret_cast<half4_t *>(a.out + row * a.ldo + h * a.G * a.Dh + d) = half4_t{};
+    }
+}
+
 // The same for prompts, and for the few rows of other sequences of the batch: a row to 32 lanes, four columns to a lane, 32 rows of a
-// tile and key head to a workgroup (tiles numbered as they are in a batch of any lengths: many find nothing to do).
+// tile and key head to a workgroup (tiles numbered as they are in a batch of any lengths: many find nothing to do).  The last workgroups
+// have 64 sequences each to look at: one that does not fit may have more rows than there are tiles numbered for it, or none.
 constexpr int kJoinRows = 32;
 __global__ void __launch_bounds__(kThreads) paged_attention_join_tiles_kernel(AttnArgs a, Units big, Units few)
 {
@@ -1289,6 +1305,10 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_tiles_kernel(At
     const int lane = threadIdx.x & 63, h = blockIdx.y;
     const int64_t bigs = big.count * kCut;
     const bool prompts = blockIdx.x < bigs;
+    if (blockIdx.x >= bigs + few.count) {
+        clear_misfits(a, (int)(blockIdx.x - bigs - few.count) * 64, h);
+        return;
+    }
     const int64_t number = prompts ? blockIdx.x / kCut : blockIdx.x - bigs;
     const int from = prompts ? (int)(blockIdx.x % kCut) * kJoinRows : 0;       // the first row
     // the unit's sequence (as Units::find has it, from what the lanes have of the sequences), all work and that of those before it
@@ -1309,16 +1329,10 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_tiles_kernel(At
     if (b >= pb.B) return;
     const int tile = uniform((int)(number - (u.even ? (int64_t)b * u.even : (int64_t)max(s.s0, 0) / u.per + (int64_t)u.more * b)));
     const int tile_rows = prompts ? kPrompt : kRows, rows = s.n * a.G, row0 = tile * tile_rows, here = min(tile_rows, rows - row0);
-    if (s.s0 < 0 || s.n <= 0 || s.s0 > pb.T - s.n || tile < 0 || here <= 0) return;
+    if (!s.ok || tile < 0 || here <= 0) return;
     auto out_of = [&](int r) { return a.out + (int64_t)(s.s0 + r / a.G) * a.ldo + (h * a.G + r % a.G) * a.Dh; };
     const int d = 4 * (lane & 31), r = from + 2 * (int)(threadIdx.x >> 6) + (lane >> 5), to = min(here, from + kJoinRows);
     if (from >= here) return;
-    if (!s.ok) {
-        if (!prompts || a.few == 0)
-            for (int k = r; k < to && d < a.Dh; k += 2 * kWaves) *reinterpret_cast<half4_t *>(out_of(row0 + k) + d) = half4_t{};
-        if (threadIdx.x == 0) report(pb, b);
-        return;
-    }
     if (prompts != (rows > a.few)) return;
     const Parts in(a, s, kRows, h, tile, uniform((int)(unsigned)wave_sum_f64(all)), uniform((int)(unsigned)wave_sum_f64(some)));
     if (in.count == 1) return;
@@ -1382,7 +1396,7 @@ Units tiles_of(const AttnArgs &a, int rows)
 int launch_join_prompts(const AttnArgs &a, hipStream_t st)
 {
     const Units few = a.few ? tiles_of(a, 32) : Units{1, 1, 1, 0}, big = tiles_of(a, kPrompt);
-    const int64_t grid = few.count + big.count * (kPrompt / kJoinRows);
+    const int64_t grid = few.count + big.count * (kPrompt / kJoinRows) + (a.pb.B + 63) / 64;
     hipLaunchKernelGGL(paged_attention_join_tiles_kernel, dim3((unsigned)grid, (unsigned)a.Hkv), dim3(kThreads), 0, st, a, big, few);
     return launch_status("paged_attention (parts)");
 }

@@ -10,8 +10,66 @@ GPU = pytest.mark.gpu
 
 
 # ---------------------------------------------------------------- numbers that do not fit together
+MISFITS = ["len too long", "more rows than positions", "rows beyond T", "all rows beyond T", "rows before 0", "falling starts",
+           "more than max_new"]
 # n, H, Hkv, max_new: few rows; a prompt by itself; prompts and a token beside them; query heads that fill more than a tile
 BATCHES = [([2, 3, 2], 4, 2, None), ([300], 4, 2, None), ([140, 1, 90], 4, 2, None), ([3, 2], 72, 1, None)]
+
+
+def misfit(B, what, max_new):
+    """(starts, lens, max_new, the bad sequence) of batch B where one sequence's numbers do not fit."""
+    starts, lens, bad = B.starts.astype(np.int64), np.asarray(B.lens, np.int64), B.B - 1
+    if what == "len too long":
+        lens[bad] = B.W * B.page + 1
+    elif what == "more rows than positions":
+        lens[bad] = B.n[bad] - 1
+    elif what == "rows beyond T":
+        starts[-1] = B.T + 5
+    elif what == "all rows beyond T":
+        starts[-2:] = B.T + 5, B.T + 9
+        if B.B > 1:
+            starts[-2] = B.T                                  # (the sequence before it has all rows from its first on)
+            lens[-2] = max(lens[-2], starts[-2] - starts[-3])
+    elif what == "rows before 0":
+        starts[0], bad = -2, 0
+    elif what == "falling starts":
+        starts[-1] = starts[-2] - 1
+    else:
+        bad = int(np.argmax(B.n))
+        max_new = max(1, B.n[bad] - 1) if B.n[bad] < 100 else 70
+        lens[bad] = max(lens[bad], B.n[bad])
+    return starts, lens, max_new, bad
+
+
+@GPU
+@pytest.mark.parametrize("what", MISFITS)
+@pytest.mark.parametrize("n,H,Hkv,max_new", BATCHES[1:])
+def test_attention_names_and_clears_what_does_not_fit(n, H, Hkv, max_new, what):
+    """status is 1 + b, every row of sequence b that there is is zeros, rows of no sequence stay, the others are as ever."""
+    import torch
+    from cacti_amd import ops
+    if what == "more than max_new" and max(n) > 100 and len(n) > 1:
+        n = [300, 1, 60]
+    for bits in (8, 16):
+        print("paged_attention", n, H, Hkv, what, bits, flush=True)
+        B = Batch(len(n) + sum(n) + bits, n, [x + 20 for x in n], H, Hkv, 64, 16, bits, spare_rows=2)
+        starts, lens, mn, bad = misfit(B, what, max_new)
+        B.n = [int(starts[b + 1] - starts[b]) if b != bad else 0 for b in range(B.B)]
+        B.starts, B.lens = starts.astype(np.int32), [int(x) for x in lens]
+        want, tol = np.full((B.T, H, 64), 7.0), np.zeros((B.T, H, 64))
+        good = [b for b in range(B.B) if b != bad]
+        o, t = B.attend(B.split()[0], (B.kp, B.vp, B.ks, B.vs))
+        for b in good:
+            rows = slice(starts[b], starts[b + 1])
+            want[rows], tol[rows] = o[rows], t[rows]
+        want[max(starts[bad], 0):max(min(starts[bad + 1], B.T), 0)] = 0
+        cache = B.put()
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        out = torch.full((B.T, H, 64), 7.0, dtype=torch.float16, device="cuda")
+        ops.paged_attention(B.d["q"], cache, *B.at(), B.alpha, max_new=mn, out=out, status=status)
+        assert int(status) == bad + 1
+        off = np.abs(out.cpu().numpy().astype(np.float64) - want) > tol
+        assert not off.any(), "rows %s" % np.unique(np.argwhere(off)[:, 0])
 
 
 @GPU
