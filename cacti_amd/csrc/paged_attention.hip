@@ -1222,7 +1222,9 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs
     for (int b0 = 0; b0 < pb.B; b0 += 64) {
         const Sequence q = lane_sequence(a, b0);
         const double u = Share(a, kRows, q).units;
-        const uint64_t hit = __ballot(b0 + lane < pb.B && row >= q.s0 && row - q.s0 < q.n);
+        const bool there = b0 + lane < pb.B;
+        const uint64_t hit = __ballot(there && row >= q.s0 && row < (int)((unsigned)q.s0 + (unsigned)q.n));
+        if (at_row == 0 && there && !q.ok) report(pb, b0 + lane);
         all += u;
         some += b < 0 && (!hit || lane < __ffsll((unsigned long long)hit) - 1) ? u : 0.;
         if (hit && b < 0) {
@@ -1234,7 +1236,6 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs
     if (b < 0 || row >= pb.T) return;
     half_t *out = a.out + row * a.ldo + head * a.Dh + d;
     if (!s.ok) {
-        if (lane == 0) report(pb, b);
         if (first == 0 && 2 * lane < a.Dh) *reinterpret_cast<half2_t *>(out) = half2_t{};
         return;
     }

@@ -43,7 +43,7 @@ def misfit(B, what, max_new):
 
 @GPU
 @pytest.mark.parametrize("what", MISFITS)
-@pytest.mark.parametrize("n,H,Hkv,max_new", BATCHES[1:])
+@pytest.mark.parametrize("n,H,Hkv,max_new", BATCHES)
 def test_attention_names_and_clears_what_does_not_fit(n, H, Hkv, max_new, what):
     """status is 1 + b, every row of sequence b that there is is zeros, rows of no sequence stay, the others are as ever."""
     import torch
