@@ -166,7 +166,8 @@ __device__ __forceinline__ float rescale(uint8_t *page, int slot0, int Dp, float
 }
 
 // Workgroups of T threads: one for each unit (page of a sequence) and head, whose rows they hold, two items of the keys and of the
-// values to a thread; then groups of up to 256 threads, `slices` of them for kRows rows of the queries.
+// values to a thread; then those that name 64 sequences each that do not fit together (units are numbered by starts that do not fall, and
+// a sequence behind which they do may have none); then groups of up to 256 threads, `slices` of them for kRows rows of the queries.
 // Rows of the queries to a thread (4 sequences of up to 2048 rows, 32 heads of 100: 1 / 2 / 4 rows 38.5 / 37.3 / 37.9 us)
 template <int T>
 constexpr int rows_of() { return T == 64 ? 1 : 2; }
@@ -177,11 +178,11 @@ __global__ void __launch_bounds__(T) paged_append_kernel(AppendArgs a)
     constexpr int kRows = rows_of<T>();
     const PagedBatch &pb = a.pb;
     const int64_t limit = min((int64_t)pb.W * pb.page, a.n_pos);
-    const int pages = (int)a.units.count * a.Hkv, half = a.Dh / 2;
+    const int pages = (int)a.units.count * a.Hkv, named = pages + (pb.B + 63) / 64, half = a.Dh / 2;
     auto column = [&](int i) { return min(i * HV, half - HV); };
-    if ((int)blockIdx.x >= pages) {
+    if ((int)blockIdx.x >= named) {
         constexpr int TQ = T < 256 ? T : 256;
-        const int u = ((int)blockIdx.x - pages) * (T / TQ) + __builtin_amdgcn_readfirstlane((int)threadIdx.x / TQ), r = u / a.slices;
+        const int u = ((int)blockIdx.x - named) * (T / TQ) + __builtin_amdgcn_readfirstlane((int)threadIdx.x / TQ), r = u / a.slices;
         const int i = (u - r * a.slices) * TQ + (int)threadIdx.x % TQ, h = min(i / a.per, a.H - 1), d = column(i - i / a.per * a.per), row0 = r * kRows;
         if (row0 >= pb.T) return;
         Loaded<HV> x[kRows];                   // (these rows there are, if not of a sequence)
@@ -208,7 +209,7 @@ __global__ void __launch_bounds__(T) paged_append_kernel(AppendArgs a)
         if (i >= a.H * a.per) return;
 #pragma unroll
         for (int e = 0; e < kRows; e++) {
-            if (!of[e].ok) continue;           // reported by the pages' workgroups
+            if (!of[e].ok) continue;
             Item<HV> it;
             it.rotated(x[e], c[e], sn[e]);
             half_t *to = a.q_out + (int64_t)(row0 + e) * a.ldqo + h * a.Dh + d;
@@ -227,6 +228,11 @@ __global__ void __launch_bounds__(T) paged_append_kernel(AppendArgs a)
         }
         return;
     }
+    if ((int)blockIdx.x >= pages) {
+        const int b = ((int)blockIdx.x - pages) * 64 + (int)threadIdx.x;
+        if (threadIdx.x < 64 && b < pb.B && !sequence(pb, b, limit, a.max_new).ok) report(pb, b);
+        return;
+    }
     // heads of a page next to each other on an XCD: they share 128-byte lines of the rows
     const int chunk = pages / 8, number = (int)blockIdx.x < 8 * chunk ? (int)(blockIdx.x & 7) * chunk + (int)(blockIdx.x >> 3) : (int)blockIdx.x;
     const int x = number / a.Hkv, h = number - x * a.Hkv;
@@ -234,10 +240,7 @@ __global__ void __launch_bounds__(T) paged_append_kernel(AppendArgs a)
     const int b = a.units.find(pb, x, &unit);
     if (b >= pb.B) return;
     const Sequence s = sequence(pb, b, limit, a.max_new);
-    if (!s.ok || s.n <= 0) {
-        if (!s.ok && threadIdx.x == 0) report(pb, b);
-        return;
-    }
+    if (!s.ok || s.n <= 0) return;
     const int pi = s.first / pb.page + unit, p0 = max(s.first, pi * pb.page), m = min(s.first + s.n, (pi + 1) * pb.page) - p0;
     if (m <= 0) return;
     const int id = pb.table[(int64_t)b * pb.ldt + pi];
@@ -324,7 +327,8 @@ int launch(AppendArgs a, hipStream_t st)
 {
     constexpr int TQ = T < 256 ? T : 256, kRows = rows_of<T>();
     a.slices = (a.H * a.per + TQ - 1) / TQ;
-    const int64_t rows = a.q ? ((int64_t)a.pb.T + kRows - 1) / kRows * a.slices : 0, grid = a.units.count * a.Hkv + (rows + T / TQ - 1) / (T / TQ);
+    const int64_t rows = a.q ? ((int64_t)a.pb.T + kRows - 1) / kRows * a.slices : 0;
+    const int64_t grid = a.units.count * a.Hkv + (a.pb.B + 63) / 64 + (rows + T / TQ - 1) / (T / TQ);
     CACTI_REQUIRE(grid * T <= UINT32_MAX, CACTI_E_NOTIMPL, "paged_append: too many pages or rows in one call");
     hipLaunchKernelGGL((paged_append_kernel<T, HV, P>), dim3((unsigned)grid), dim3(T), 0, st, a);
     return launch_status("paged_append");

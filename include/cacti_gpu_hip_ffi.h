@@ -436,8 +436,9 @@ int cacti_hip_embed_bwd(int64_t V, int64_t D, int64_t S, const void *tok, const 
 /* A batch of B sequences.  Rows starts[b] .. starts[b + 1] - 1 of its tensors are the new tokens of sequence b (none: left out),
  * lens[b] its positions with them: its row i is at position lens[b] - n + i.  Position p lies in slot p % page of page
  * table[b * ldt + p / page] of the cache.  starts [B + 1], lens [B], table [B, W] are i32 on the device and are not read by
- * the host: nothing waits, and a captured launch follows them.  T: rows there are (those from starts[B] on are left as they
- * are); max_new: no sequence has more new rows (T will do; the less, the fewer idle workgroups).
+ * the host: nothing waits, and a captured launch follows them.  starts does not fall (where it does, starts[b + 1] < starts[b],
+ * sequence b does not fit, and what the others get is unspecified).  T: rows there are (those from starts[B] on are left as they are);
+ * max_new: no sequence has more new rows (T will do; the less, the fewer idle workgroups).
  * Cache: pages [P, Hkv, page, Dp], Dp = Dh rounded up to 16, the columns from Dh on zeros; bits = 16: f16, scales NULL;
  * bits = 8: e4m3 (OCP, no infinities) with scales [P, Hkv] f32, a value being code * scale.  A page is of one sequence where
  * that appends; reading it may be shared.  Heads: H of the queries, Hkv of the cache, H % Hkv == 0, query head h reads

@@ -95,6 +95,23 @@ def test_lengths_at_the_ends_of_32_bits(n, H, Hkv, max_new, length):
         out = ops.paged_attention(B.d["q"], cache, B.d["table"], B.d["starts"], lens, B.alpha, status=status, max_new=max_new)
         assert int(status) == bad + 1 and not out[B.starts[bad]:].any()
 
+@GPU
+@pytest.mark.parametrize("starts", [[0, 100, 68, 120], [0, 100, 70, 90], [0, 16, 0, 90]])
+def test_append_names_falling_starts(starts):
+    """Wherever the numbers of the pages' units put the sequence that they fall behind."""
+    import torch
+    from cacti_amd import ops
+    for bits in (8, 16):
+        B = Batch(17, [100, 0, 20], [110, 5, 100], 4, 2, 64, 16, bits)
+        cache, was = B.put(), B.put()
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        d = torch.tensor(starts, dtype=torch.int32, device="cuda")
+        ops.paged_append(B.d["k"], B.d["v"], cache, B.d["table"], d, B.d["lens"], B.d["cos"], B.d["sin"], status=status)
+        assert int(status) == 2
+        for g, w in zip(cache, was):
+            if w is not None:
+                same_bits(numpy_of(g)[B.table[1]], numpy_of(w)[B.table[1]], "pages")
+
 
 # ---------------------------------------------------------------- sizes at the ends of their ranges
 @pytest.mark.parametrize("page", [16, 48, 256])
