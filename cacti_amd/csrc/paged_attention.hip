@@ -1458,10 +1458,11 @@ CACTI_API int cacti_hip_paged_attention_f16(int64_t T, int64_t B, int64_t H, int
     CACTI_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= cacti_hip_paged_attention_workspace(T, B, H, Hkv, Dh, max_new),
                   CACTI_E_INVALID, "paged_attention: workspace too small or not 16-byte aligned");
     CACTI_REQUIRE(fabsf(alpha) < INFINITY, CACTI_E_INVALID, "paged_attention: alpha is not finite");
+    // tiles of 16 rows of one sequence, of all, whichever is less; work is counted in 32 bits
+    const int64_t most = (max_new < T ? max_new : T) * (H / Hkv) / 16 + 1, tiles = T * (H / Hkv) / 16 + B < most * B ? T * (H / Hkv) / 16 + B : most * B;
+    CACTI_REQUIRE(T * H < (1 << 24) && tiles * Hkv < INT32_MAX / (W * page / kStep + 1 + begin_of(32)), CACTI_E_NOTIMPL,
+                  "paged_attention: too many rows and positions in one call");
     CACTI_REQUIRE(q != out, CACTI_E_INVALID, "paged_attention: the output cannot take the queries' place, which other workgroups read");
-    const int64_t most = (max_new < T ? max_new : T) * (H / Hkv) / 16 + 1;         // tiles of a sequence; work is counted in 32 bits
-    CACTI_REQUIRE(T * H < (1 << 24) && (most < T * (H / Hkv) / 16 + B ? most * B : T * (H / Hkv) / 16 + B) * Hkv <
-                      INT32_MAX / (W * page / kStep + 1 + begin_of(32)), CACTI_E_NOTIMPL, "paged_attention: too many rows and positions in one call");
     const Plan p = plan(T, B, H, Hkv, Dh, max_new, bits / 8);
     float *part = (float *)workspace;
     const size_t small = (size_t)p.groups * 2 * (16 * p.NR);

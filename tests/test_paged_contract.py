@@ -124,3 +124,15 @@ def test_no_more_positions_than_are_counted_in_32_bits(page):
             # (a wrong pitch of the rotation's and of the output's rows ends the calls that are not refused for their table)
             assert f(*dict(args, page=page, W=W, ldt=W, **({"ldk": 12} if args is APPEND else {"ldo": 30})).values()) < 0
             assert ("too many rows, sequences or pages" in L.cacti_hip_last_error().decode()) == refused
+
+
+@pytest.mark.parametrize("T,B,H,Hkv,max_new,W,refused", [(8192, 2048, 64, 8, 8192, 512, False), (8192, 2048, 64, 8, 8, 512, False),
+                                                         (65536, 1024, 64, 64, 65536, 4096, False), (65536, 1024, 64, 64, 65536, 32768, True),
+                                                         (1, 1, 8, 8, 1, 1 << 22, False), (1 << 18, 64, 64, 8, 4096, 64, True)])
+def test_work_that_is_counted_in_32_bits(T, B, H, Hkv, max_new, W, refused):
+    """Tiles of a batch are no more than its rows make, however many one sequence may have.  (The output in the queries' place ends the
+    calls that are not refused for their work.)"""
+    L = ffi.lib()
+    args = dict(ATTEND, T=T, B=B, H=H, Hkv=Hkv, max_new=max_new, W=W, ldt=W, ldq=H * 8, ldo=H * 8, ws_bytes=1 << 40)
+    assert L.cacti_hip_paged_attention_f16(*args.values()) < 0
+    assert ("too many rows and positions" if refused else "output") in L.cacti_hip_last_error().decode()
