@@ -85,6 +85,10 @@ __device__ __forceinline__ Sequence lane_sequence(const AttnArgs &a, int b0)
 constexpr unsigned kLeast = 2;
 __device__ __forceinline__ unsigned groups_of(const AttnArgs &a, unsigned units) { return min((unsigned)a.groups, max(units / (kLeast * kWaves), 1u)); }
 
+// Work is counted in 32 bits; the host has seen to it that rows which each are of one sequence are not more.  (Where starts fall a row may
+// be of many: nothing is done then.)
+__device__ __forceinline__ bool too_much(double units) { return units > (double)INT32_MAX; }
+
 constexpr unsigned kBigLeast = 4;              // the same of steps of 64 positions
 // Workgroups go round the 8 XCDs: those of one XCD get neighbouring numbers (of n, a multiple of 8)
 __device__ __forceinline__ unsigned xcd_order(unsigned i, unsigned n) { return (i & 7) * (n / 8) + i / 8; }
@@ -673,7 +677,9 @@ __global__ void __launch_bounds__(kThreads, resident(ND, NR, sizeof(P))) paged_a
     const double u64 = Share(a, kRows, s64).units;         // (whole numbers)
     double all = u64;
     for (int b0 = 64; b0 < a.pb.B; b0 += 64) all += Share(a, kRows, lane_sequence(a, b0)).units;
-    const unsigned units = uniform((int)(unsigned)wave_sum_f64(all)), groups = groups_of(a, units);
+    all = wave_sum_f64(all);
+    if (too_much(all)) return;
+    const unsigned units = uniform((int)(unsigned)all), groups = groups_of(a, units);
     if (group >= groups) return;
     const Shares shares(units, groups);
     const unsigned x0 = uniform((int)shares.begin(group)), x1 = uniform((int)shares.begin(group + 1));     // the workgroup's
@@ -1107,7 +1113,9 @@ __global__ void __launch_bounds__(kBigThreads, 2) paged_prompt_kernel(AttnArgs a
     const double u64 = BigShare(a, s64).units(a);
     double all = u64;
     for (int b0 = 64; b0 < a.pb.B; b0 += 64) all += BigShare(a, lane_sequence(a, b0)).units(a);
-    const unsigned units = uniform((int)(unsigned)wave_sum_f64(all)), groups = min((unsigned)a.big_groups, max(units / kBigLeast, 1u));
+    all = wave_sum_f64(all);
+    if (too_much(all)) return;
+    const unsigned units = uniform((int)(unsigned)all), groups = min((unsigned)a.big_groups, max(units / kBigLeast, 1u));
     const unsigned group = xcd_order(blockIdx.x, a.big_groups);
     if (units == 0 || group >= groups) return;
     const Shares shares(units, groups);
@@ -1240,7 +1248,9 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs
         return;
     }
     const int h = head / a.G, r = (row - s.s0) * a.G + head - h * a.G, tile = r / kRows;
-    const Parts in(a, s, kRows, h, tile, uniform((int)(unsigned)wave_sum_f64(all)), uniform((int)(unsigned)wave_sum_f64(some)));
+    all = wave_sum_f64(all);
+    if (too_much(all)) return;
+    const Parts in(a, s, kRows, h, tile, uniform((int)(unsigned)all), uniform((int)(unsigned)wave_sum_f64(some)));
     const int parts = in.count;
     if (parts == 1) return;
     Joined<2> j;
@@ -1335,7 +1345,9 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_tiles_kernel(At
     const int d = 4 * (lane & 31), r = from + 2 * (int)(threadIdx.x >> 6) + (lane >> 5), to = min(here, from + kJoinRows);
     if (from >= here) return;
     if (prompts != (rows > a.few)) return;
-    const Parts in(a, s, kRows, h, tile, uniform((int)(unsigned)wave_sum_f64(all)), uniform((int)(unsigned)wave_sum_f64(some)));
+    all = wave_sum_f64(all);
+    if (too_much(all)) return;
+    const Parts in(a, s, kRows, h, tile, uniform((int)(unsigned)all), uniform((int)(unsigned)wave_sum_f64(some)));
     if (in.count == 1) return;
     const float *part = prompts ? a.big_part : a.part, *stats = prompts ? a.big_stats : a.stats;
     constexpr int kAtOnce = 4;                 // parts at once, of two rows

@@ -136,3 +136,20 @@ def test_work_that_is_counted_in_32_bits(T, B, H, Hkv, max_new, W, refused):
     args = dict(ATTEND, T=T, B=B, H=H, Hkv=Hkv, max_new=max_new, W=W, ldt=W, ldq=H * 8, ldo=H * 8, ws_bytes=1 << 40)
     assert L.cacti_hip_paged_attention_f16(*args.values()) < 0
     assert ("too many rows and positions" if refused else "output") in L.cacti_hip_last_error().decode()
+
+
+@GPU
+@pytest.mark.parametrize("T,W", [(65536, 256), (128, 4060)])
+def test_rows_of_many_sequences_are_no_endless_work(T, W):
+    """Starts that fall again and again give every second sequence all rows, which is more work than 32 bits count: nothing is done."""
+    import torch
+    from cacti_amd import ops
+    B, H, page = 1024, 64, 256
+    print("paged_attention", T, W, flush=True)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    cache = ops.paged_cache(1, H, page, 4, dtype=torch.float16)
+    q = torch.zeros((T, H, 4), dtype=torch.float16, device="cuda")
+    status = i32([0])
+    ops.paged_attention(q, cache, torch.zeros((B, W), dtype=torch.int32, device="cuda"), i32([0, T] * (B // 2) + [0]), i32([W * page] * B), 0.5,
+                        status=status)
+    assert int(status) == B
