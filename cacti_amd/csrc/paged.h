@@ -72,11 +72,12 @@ __device__ __forceinline__ int count_below(int B, int64_t x, F f)
 
 // Units of the sequences of a launch (pages they touch, tiles of their rows) are numbered so that the host need not know the
 // lengths.  even > 0: `even` numbers for each sequence.  Otherwise a sequence of rows s0 .. s1 - 1 has those from
-// s0 / per + more b on: s1 / per - s0 / per + more of them, which is enough where n rows need no more than n / per + more.
+// s0 / per times + more b on: at least (s1 - s0) / per times + more of them, which has to be enough for its n rows.
 struct Units {
-    int even, per, more;
+    int even, per, times, more;
     int64_t count;
-    __device__ __forceinline__ int64_t first(const PagedBatch &pb, int i) const { return (int64_t)max(pb.starts[i], 0) / per + (int64_t)more * i; }
+    __device__ __forceinline__ int64_t begin(int b, int s0) const { return even ? (int64_t)b * even : (int64_t)(max(s0, 0) / per) * times + (int64_t)more * b; }
+    __device__ __forceinline__ int64_t first(const PagedBatch &pb, int i) const { return begin(i, pb.starts[i]); }
     // (sequence, unit of it) of number x; sequence B: none
     __device__ __forceinline__ int find(const PagedBatch &pb, int64_t x, int *unit) const
     {
@@ -91,11 +92,11 @@ struct Units {
     }
 };
 // units of a launch over T rows: `most` for a sequence of max_new rows
-inline Units make_units(int64_t T, int64_t B, int64_t per, int more, int64_t most)
+inline Units make_units(int64_t T, int64_t B, int64_t per, int64_t times, int more, int64_t most)
 {
-    const int64_t searched = T / per + (int64_t)more * B;
-    if (most * B <= searched) return {(int)most, (int)per, more, most * B};
-    return {0, (int)per, more, searched};
+    const int64_t searched = T / per * times + (int64_t)more * B;
+    if (most * B <= searched) return {(int)most, (int)per, (int)times, more, most * B};
+    return {0, (int)per, (int)times, more, searched};
 }
 
 // What is the same of the calls' checks; sets pb

@@ -361,7 +361,7 @@ CACTI_API int cacti_hip_paged_append(int64_t T, int64_t B, int64_t H, int64_t Hk
                   CACTI_E_INVALID, "paged_append: operands must be 8-byte aligned with row pitches that are multiples of 4");
     if (max_new > T) max_new = T;
     // n rows touch up to (n + page - 2) / page + 1 pages, which is no more than n / page + 2
-    const Units units = make_units(T, B, page, 2, (max_new + page - 2) / page + 1);
+    const Units units = make_units(T, B, page, 1, 2, (max_new + page - 2) / page + 1);
     const int HV = Dh >= 16 ? 8 : 2, per = (int)((Dh / 2 + HV - 1) / HV);
     const AppendArgs a = {pb,   units, (int)H,           (int)Hkv, (int)Dh, (int)max_new, per, 0, 65536u / per + 1, n_pos, (const half_t *)q,
                           (const half_t *)k, (const half_t *)v, (const half_t *)cos16, (const half_t *)sin16, ldq, ldk, ldv, ldqr,

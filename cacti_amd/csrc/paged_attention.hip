@@ -1330,7 +1330,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_tiles_kernel(At
     for (int b0 = 0; b0 < pb.B; b0 += 64) {
         const Sequence q = lane_sequence(a, b0);
         const int i = b0 + lane;
-        if (!u.even) b += __popcll(__ballot(i < pb.B && max(q.s0 + q.n, 0) / u.per + (int64_t)u.more * (i + 1) <= number));
+        if (!u.even) b += __popcll(__ballot(i < pb.B && u.begin(i + 1, (int)((unsigned)q.s0 + (unsigned)q.n)) <= number));
         const double w = prompts ? BigShare(a, q).units(a) : Share(a, kRows, q).units;
         all += w;
         some += i < b ? w : 0.;                // (b grows only while all of these are before it)
@@ -1338,7 +1338,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_tiles_kernel(At
     }
     b = uniform(b);
     if (b >= pb.B) return;
-    const int tile = uniform((int)(number - (u.even ? (int64_t)b * u.even : (int64_t)max(s.s0, 0) / u.per + (int64_t)u.more * b)));
+    const int tile = uniform((int)(number - u.begin(b, s.s0)));
     const int tile_rows = prompts ? kPrompt : kRows, rows = s.n * a.G, row0 = tile * tile_rows, here = min(tile_rows, rows - row0);
     if (!s.ok || tile < 0 || here <= 0) return;
     auto out_of = [&](int r) { return a.out + (int64_t)(s.s0 + r / a.G) * a.ldo + (h * a.G + r % a.G) * a.Dh; };
@@ -1399,16 +1399,16 @@ Plan plan(int64_t T, int64_t B, int64_t H, int64_t Hkv, int64_t Dh, int64_t max_
     return {NR, resident(Dh <= 64 ? 1 : 2, NR, bytes) * device_cus(), INT32_MAX, 0};
 }
 
-// Tiles of `rows` rows of the key heads' queries
+// Tiles of `rows` rows of the key heads' queries: a tile to as many whole tokens as it holds and one more to a sequence, or, of more
+// heads than that, as many to a token as hold it (more than it takes where one does not divide the other)
 Units tiles_of(const AttnArgs &a, int rows)
 {
-    const int tokens = rows >= a.G ? rows / a.G : 1;           // whole ones of a tile; more tiles than it takes where G does not divide it
     const int64_t most = ((int64_t)a.max_new * a.G + rows - 1) / rows;
-    return a.G > rows ? Units{(int)most, 1, 1, most * a.pb.B} : make_units(a.pb.T, a.pb.B, tokens, 1, most);
+    return a.G > rows ? make_units(a.pb.T, a.pb.B, 1, (a.G + rows - 1) / rows, 0, most) : make_units(a.pb.T, a.pb.B, rows / a.G, 1, 1, most);
 }
 int launch_join_prompts(const AttnArgs &a, hipStream_t st)
 {
-    const Units few = a.few ? tiles_of(a, 32) : Units{1, 1, 1, 0}, big = tiles_of(a, kPrompt);
+    const Units few = a.few ? tiles_of(a, 32) : Units{1, 1, 1, 1, 0}, big = tiles_of(a, kPrompt);
     const int64_t grid = few.count + big.count * (kPrompt / kJoinRows) + (a.pb.B + 63) / 64;
     hipLaunchKernelGGL(paged_attention_join_tiles_kernel, dim3((unsigned)grid, (unsigned)a.Hkv), dim3(kThreads), 0, st, a, big, few);
     return launch_status("paged_attention (parts)");

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from cacti_amd import ffi
-from test_paged import APPEND, ATTEND, Batch, numpy_of, same_bits
+from test_paged import APPEND, ATTEND, Batch, check_attention, numpy_of, same_bits
 
 GPU = pytest.mark.gpu
 
@@ -153,3 +153,15 @@ def test_rows_of_many_sequences_are_no_endless_work(T, W):
     ops.paged_attention(q, cache, torch.zeros((B, W), dtype=torch.int32, device="cuda"), i32([0, T] * (B // 2) + [0]), i32([W * page] * B), 0.5,
                         status=status)
     assert int(status) == B
+
+
+@GPU
+@pytest.mark.parametrize("H", [64, 160])
+def test_many_sequences_of_many_heads_to_a_key_head(H):
+    """A token's query heads fill more than a tile of the few rows, or than a prompt's: what puts the parts together is launched for the
+    tiles that all rows make, not for those that each sequence might have."""
+    B = Batch(H, [1 if b % 50 == 3 else 0 for b in range(2048)], [40 + b % 50 for b in range(2048)], H, 1, 8, 16, 16, spare_rows=8151)
+    assert B.T == 8192
+    check_attention(B)
+    B = Batch(H + 1, [2, 0, 3, 1, 0], [70, 1, 300, 20, 5], H, 1, 8, 16, 8, spare_rows=3)
+    check_attention(B)
