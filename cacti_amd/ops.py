@@ -254,7 +254,7 @@ def paged_append(k, v, cache, table, starts, lens, cos, sin, q=None, out=None, m
 
     Rows starts[b] .. starts[b+1]-1 are the new tokens of sequence b, lens[b] its length with them, table[b] its pages: int32
     tensors on the GPU that the host does not read.  cos, sin: rope_tables of as many positions as any sequence has.
-    max_new: no sequence has more new rows than that.  status: a cleared int32 tensor of one element that becomes 1 + b where
+    max_new: no sequence has more new rows than that (at least 1).  status: a cleared int32 tensor of one element that becomes 1 + b where
     the numbers of sequence b do not fit together (nothing of it is written then).  Rows may be strided."""
     return _op.paged_append(k, v, *cache, table, starts, lens, cos, sin, q, out, max_new, status)
 

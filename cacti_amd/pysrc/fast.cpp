@@ -518,6 +518,10 @@ struct Paged {
         require(o[5] != Py_None && o[6] != Py_None, "paged cache: starts [sequences + 1] and lens [sequences] of int32 expected");
         starts = on.pointer(o[5], at::kInt, B + 1), lens = on.pointer(o[6], at::kInt, B);
     }
+    void bounds(int64_t max_new, int64_t T) const
+    {
+        require(max_new > 0 || (max_new == 0 && (T == 0 || B == 0)), "paged cache: max_new is at least 1 where there are rows and sequences");
+    }
     void holds(int64_t Dh) const { require(k.size(3) == (Dh + 15) / 16 * 16, "paged cache: pages of another head dimension"); }
 };
 
@@ -547,9 +551,9 @@ PyObject *paged_append(PyObject *const *o)
         qo = out.t.data_ptr();
     } else require(o[12] == Py_None, "paged_append: out without q");
     const int64_t max_new = o[13] == Py_None ? k.T : number<int64_t>(o[13]);
-    require(max_new >= 0, "paged_append: max_new");
+    c.bounds(max_new, k.T);
     void *status = on.pointer(o[14], at::kInt, 1), *st = on.stream();
-    if (k.T > 0 && c.B > 0 && max_new > 0)
+    if (k.T > 0 && c.B > 0)
         run([&] {
             return cacti_hip_paged_append(k.T, c.B, H, k.H, k.Dh, max_new, q, ldq, k.t.data_ptr(), k.ld, v.t.data_ptr(), v.ld, cos.data_ptr(),
                                           sin.data_ptr(), cos.size(0), qo, ldqo, c.k.data_ptr(), c.v.data_ptr(), c.ks, c.vs, c.bits, c.P,
@@ -568,7 +572,7 @@ PyObject *paged_attention(PyObject *const *o)
     c.holds(q.Dh);
     const float alpha = number<float>(o[8]);
     const int64_t max_new = o[9] == Py_None ? q.T : number<int64_t>(o[9]);
-    require(max_new >= 0, "paged_attention: max_new");
+    c.bounds(max_new, q.T);
     Result out = {at::Tensor(), nullptr};
     int64_t ldo = q.H * q.Dh;
     if (o[10] == Py_None) out.t = empty({q.T, q.H, q.Dh}, q.t, at::kHalf);
@@ -578,7 +582,7 @@ PyObject *paged_attention(PyObject *const *o)
         out = {w.t, o[10]}, ldo = w.ld;
     }
     void *status = on.pointer(o[11], at::kInt, 1), *st = on.stream();
-    if (q.T > 0 && c.B > 0 && max_new > 0) {
+    if (q.T > 0 && c.B > 0) {
         const size_t bytes = cacti_hip_paged_attention_workspace(q.T, c.B, q.H, c.Hkv, q.Dh, max_new);
         const at::Tensor ws = empty({(int64_t)bytes}, q.t, at::kByte);
         run([&] {

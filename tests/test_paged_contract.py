@@ -165,3 +165,19 @@ def test_many_sequences_of_many_heads_to_a_key_head(H):
     check_attention(B)
     B = Batch(H + 1, [2, 0, 3, 1, 0], [70, 1, 300, 20, 5], H, 1, 8, 16, 8, spare_rows=3)
     check_attention(B)
+
+
+@GPU
+def test_a_bound_of_no_rows_is_refused():
+    """max_new = 0 with rows and sequences there, as the C calls refuse it; nothing is returned that nobody wrote."""
+    from cacti_amd import ops
+    B = Batch(91, [2, 1], [20, 40], 4, 2, 64, 16, 8)
+    cache = B.put()
+    append = lambda rows, max_new: ops.paged_append(B.d["k"][:rows], B.d["v"][:rows], cache, *B.at(), B.d["cos"], B.d["sin"], q=B.d["q"][:rows],
+                                                    max_new=max_new)
+    attend = lambda rows, max_new: ops.paged_attention(B.d["q"][:rows], cache, *B.at(), 1.0, max_new=max_new)
+    for f in (append, attend):
+        for max_new in (0, -1):
+            with pytest.raises(AssertionError, match="max_new"):
+                f(3, max_new)
+        assert f(0, 0).shape == (0, 4, 64)
