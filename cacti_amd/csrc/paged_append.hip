@@ -11,6 +11,7 @@
 // Bound by memory: four sequences of up to 2048 rows, 32 heads of 100 in 8 bits 38 to 40 us, of which 18 are the queries' (reading the
 // rows once for the scale and again for the codes, two columns at a time: 56.4); 96 of up to 6 rows, 8 heads of 128: 5.4 us; one
 // row 4.0 us, latency.
+#include "operands.h"
 #include "paged.h"
 
 using namespace cacti;
@@ -359,6 +360,11 @@ CACTI_API int cacti_hip_paged_append(int64_t T, int64_t B, int64_t H, int64_t Hk
     CACTI_REQUIRE(ldk % 4 == 0 && ldv % 4 == 0 && (!q || (ldq % 4 == 0 && ldqr % 4 == 0)) && aligned(k, 8) && aligned(v, 8) && aligned(q, 8) &&
                       aligned(q_rot, 8) && aligned(cos16, 8) && aligned(sin16, 8),
                   CACTI_E_INVALID, "paged_append: operands must be 8-byte aligned with row pitches that are multiples of 4");
+    // queries in place: a workgroup reads what it writes; anything else that is written here another may yet have to read
+    CACTI_REQUIRE(!q || ((q == q_rot && (ldq == ldqr || T == 1)) || !rows_share(T, q, ldq, H * Dh, q_rot, ldqr, H * Dh)), CACTI_E_INVALID,
+                  "paged_append: the rotated queries take the queries' place, with the same pitch, or share no memory with them");
+    CACTI_REQUIRE(!q || (!rows_share(T, k, ldk, Hkv * Dh, q_rot, ldqr, H * Dh) && !rows_share(T, v, ldv, Hkv * Dh, q_rot, ldqr, H * Dh)),
+                  CACTI_E_INVALID, "paged_append: the rotated queries share memory with the keys or values");
     if (max_new > T) max_new = T;
     // n rows touch up to (n + page - 2) / page + 1 pages, which is no more than n / page + 2
     const Units units = make_units(T, B, page, 1, 2, (max_new + page - 2) / page + 1);

@@ -23,6 +23,7 @@
 // forms their sum in steps of 32 positions and takes an equal, contiguous share of it, across rows, heads and sequences, each of
 // its waves a quarter.  What its waves have of a tile of rows they put together in LDS; a tile that ends up in more than one
 // share leaves partial sums, which a second launch puts together.
+#include "operands.h"
 #include "paged.h"
 
 using namespace cacti;
@@ -1474,7 +1475,8 @@ CACTI_API int cacti_hip_paged_attention_f16(int64_t T, int64_t B, int64_t H, int
     const int64_t most = (max_new < T ? max_new : T) * (H / Hkv) / 16 + 1, tiles = T * (H / Hkv) / 16 + B < most * B ? T * (H / Hkv) / 16 + B : most * B;
     CACTI_REQUIRE(T * H < (1 << 24) && tiles * Hkv < INT32_MAX / (W * page / kStep + 1 + begin_of(32)), CACTI_E_NOTIMPL,
                   "paged_attention: too many rows and positions in one call");
-    CACTI_REQUIRE(q != out, CACTI_E_INVALID, "paged_attention: the output cannot take the queries' place, which other workgroups read");
+    CACTI_REQUIRE(!rows_share(T, q, ldq, H * Dh, out, ldo, H * Dh), CACTI_E_INVALID,
+                  "paged_attention: the output shares memory with the queries, which other workgroups read");
     const Plan p = plan(T, B, H, Hkv, Dh, max_new, bits / 8);
     float *part = (float *)workspace;
     const size_t small = (size_t)p.groups * 2 * (16 * p.NR);

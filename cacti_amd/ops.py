@@ -250,7 +250,7 @@ def paged_cache(pages, heads, page, Dh, dtype=torch.float8_e4m3fn, device="cuda"
 
 def paged_append(k, v, cache, table, starts, lens, cos, sin, q=None, out=None, max_new=None, status=None):
     """The new keys (rotated) and values [T, heads, Dh] of a ragged batch into the pages of `cache`; returns the queries q
-    rotated (into out where given, which may be q), None without q.
+    rotated (into out where given, which may be q and otherwise shares no memory with q, k and v), None without q.
 
     Rows starts[b] .. starts[b+1]-1 are the new tokens of sequence b, lens[b] its length with them, table[b] its pages: int32
     tensors on the GPU that the host does not read.  cos, sin: rope_tables of as many positions as any sequence has.
@@ -261,7 +261,7 @@ def paged_append(k, v, cache, table, starts, lens, cos, sin, q=None, out=None, m
 
 def paged_attention(q, cache, table, starts, lens, alpha, max_new=None, out=None, status=None):
     """Causal attention of the (rotated) queries of a ragged batch over `cache`, which holds their own positions too; the
-    arguments are those of paged_append.  Rows behind the last sequence are left as they are in out, which is not q."""
+    arguments are those of paged_append.  Rows behind the last sequence are left as they are in out, which shares no memory with q."""
     return _op.paged_attention(q, *cache, table, starts, lens, alpha, max_new, out, status)
 
 

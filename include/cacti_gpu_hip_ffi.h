@@ -451,7 +451,7 @@ int cacti_hip_embed_bwd(int64_t V, int64_t D, int64_t S, const void *tok, const 
 
 /* New keys and values into their pages, the keys rotated as by symplectic_embed (src/librarium/llama.rs:463-465; tables as
  * cacti_hip_rope_tables fills them, n_pos rows), and, where q is not NULL, q_rot = the queries rotated: in fp32, rounded once;
- * q_rot may be q itself, with the same pitch.
+ * q_rot may be q itself, with the same pitch, and shares no memory with q, k and v otherwise.
  * bits = 8: the scale of a page and head is the least 2^e, -32 <= e <= 15, with all finite new values of the page up to
  * 448 * 2^e, and no less than before where the page has older positions; their codes are carried over where it grew.  (Scales
  * are powers of two: the quotient and, but for subnormal codes, that are exact.)  NaN and infinities become NaN.  Slots behind
@@ -462,7 +462,7 @@ int cacti_hip_paged_append(int64_t T, int64_t B, int64_t H, int64_t Hkv, int64_t
                            int bits, int64_t P, int64_t page, const void *table, int64_t ldt, int64_t W, const void *starts,
                            const void *lens, void *status, void *stream);
 
-/* out [T, ldo] f16, not q itself, = softmax_j(alpha q . k_j) v over the positions j up to the row's own, which are in the cache; fp32 scores
+/* out [T, ldo] f16, which shares no memory with q, = softmax_j(alpha q . k_j) v over the positions j up to the row's own, which are in the cache; fp32 scores
  * and sums, the weights rounded to f16 for the second product.  A row's result depends on nothing behind its position.  Scales
  * are positive, any of them.  workspace: cacti_hip_paged_attention_workspace bytes, 16-byte aligned, contents undefined on
  * return. */

@@ -1,5 +1,8 @@
 """What the paged calls promise of batches whose numbers do not fit together, of operands that share memory and of sizes at the ends
 of their ranges.  The plain forms and bounds are those of test_paged.py."""
+import os
+import subprocess
+
 import numpy as np
 import pytest
 
@@ -7,6 +10,7 @@ from cacti_amd import ffi
 from test_paged import APPEND, ATTEND, Batch, check_attention, numpy_of, same_bits
 
 GPU = pytest.mark.gpu
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "cacti_amd", "csrc")
 
 
 # ---------------------------------------------------------------- numbers that do not fit together
@@ -181,3 +185,90 @@ def test_a_bound_of_no_rows_is_refused():
             with pytest.raises(AssertionError, match="max_new"):
                 f(3, max_new)
         assert f(0, 0).shape == (0, 4, 64)
+
+
+# ---------------------------------------------------------------- operands that share memory
+SHARE = r"""
+#include <stdio.h>
+
+#include <set>
+
+#include "operands.h"
+
+int main()
+{
+    for (int64_t rows : {1, 2, 3})
+        for (int64_t lda = 1; lda <= 7; lda++)
+            for (int64_t ldb = 1; ldb <= 7; ldb++)
+                for (int64_t wa = 1; wa <= lda; wa++)
+                    for (int64_t wb = 1; wb <= ldb; wb++)
+                        for (int64_t d = -25; d <= 25; d++) {
+                            std::set<int64_t> of_a;
+                            bool share = false;
+                            for (int64_t i = 0; i < rows; i++)
+                                for (int64_t k = 0; k < wa; k++) of_a.insert(i * lda + k);
+                            for (int64_t i = 0; i < rows; i++)
+                                for (int64_t k = 0; k < wb; k++) share = share || of_a.count(d + i * ldb + k);
+                            const bool got = cacti::rows_share(rows, (void *)1000, lda, wa, (void *)(1000 + 2 * d), ldb, wb);
+                            if (got != share && (share || lda == ldb || rows == 1)) {
+                                printf("rows %ld, pitches %ld %ld, widths %ld %ld, %ld apart: %d\n", (long)rows, (long)lda, (long)ldb, (long)wa, (long)wb,
+                                       (long)d, (int)got);
+                                return 1;
+                            }
+                        }
+    return 0;
+}
+"""
+
+
+def test_rows_that_share_memory_are_found(tmp_path):
+    """Against sets of addresses; of different pitches rows may be taken to share that lie between each other."""
+    src, exe = tmp_path / "t.cpp", tmp_path / "t"
+    src.write_text(SHARE)
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-g", "-fsanitize=undefined", "-fno-sanitize-recover", "-Wall", "-Werror", "-I" + CSRC, str(src),
+                           "-o", str(exe)])
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
+# rows of 64 heads of queries, 32 of keys, 32 of values, as the product before leaves them; so many sequences that a call that passes is
+# too large to be launched
+Q, K, V, FAR = 0x100000, 0x100000 + 1024, 0x100000 + 1536, 0x900000
+QKV = dict(APPEND, T=5, B=(1 << 20) - 1, H=64, Hkv=32, max_new=5, q=Q, k=K, v=V, qr=Q, ldq=1024, ldk=1024, ldv=1024, ldqr=1024)
+
+
+@pytest.mark.parametrize("change,why", [
+    (dict(), "in one call"), (dict(qr=FAR), "in one call"), (dict(qr=FAR, ldqr=512), "in one call"), (dict(q=FAR, ldq=512, qr=Q), "in one call"),
+    (dict(qr=Q - 5 * 2048), "in one call"), (dict(ldqr=2048), "place"), (dict(ldqr=512), "place"),
+    (dict(qr=Q + 2048), "place"), (dict(qr=Q - 4 * 2048), "place"), (dict(qr=Q + 8), "place"), (dict(q=FAR, qr=K), "keys or values"),
+    (dict(q=FAR, qr=V - 8), "keys or values"), (dict(q=FAR, qr=V, k=FAR), "keys or values"), (dict(q=FAR, qr=Q + 8), "keys or values"),
+    (dict(q=FAR, ldqr=512), "keys or values")])
+def test_append_refuses_rotated_queries_in_another_place(change, why):
+    """The queries' own place, with their pitch, or memory of their own; the columns of q, k and v may lie in the same rows."""
+    L = ffi.lib()
+    assert L.cacti_hip_paged_append(*dict(QKV, **change).values()) < 0
+    assert why in L.cacti_hip_last_error().decode()
+
+
+@pytest.mark.parametrize("change", [dict(), dict(out=64 + 8), dict(out=64 + 3 * 64), dict(ldo=64), dict(out=128, ldo=32), dict(ldq=64, ldo=64, out=64 + 56)])
+def test_attention_refuses_an_output_that_shares_memory_with_the_queries(change):
+    L = ffi.lib()
+    assert L.cacti_hip_paged_attention_f16(*dict(ATTEND, **change).values()) < 0
+    assert "shares memory" in L.cacti_hip_last_error().decode()
+
+
+@GPU
+def test_queries_and_output_in_the_columns_of_one_buffer():
+    import torch
+    from cacti_amd import ops
+    for n, lens in (([2, 1], [30, 70]), ([150, 3], [160, 20])):
+        B = Batch(92, n, lens, 4, 2, 100, 16, 16)
+        cache = B.put()
+        want = ops.paged_attention(B.d["q"], cache, *B.at(), B.alpha)
+        both = torch.full((B.T, 1000), 7.0, dtype=torch.float16, device="cuda")
+        q, out = both[:, 40:440].view(-1, 4, 100), both[:, 440:840].view(-1, 4, 100)
+        q.copy_(B.d["q"])
+        assert ops.paged_attention(q, cache, *B.at(), B.alpha, out=out) is out
+        assert torch.equal(out, want) and torch.equal(q, B.d["q"]) and bool((both[:, :40] == 7).all()) and bool((both[:, 840:] == 7).all())
+        with pytest.raises(ffi.CactiError, match="shares memory"):
+            ops.paged_attention(q, cache, *B.at(), B.alpha, out=both[:, 436:836].view(-1, 4, 100))
