@@ -10,6 +10,7 @@
 // 2048 rows of 32000, K = 64: forward 29 us, 4.5 TB/s (a maximum and then a sum out of memory again: 44), adjoint 46.7 us,
 // 5.6 TB/s, and one after the other, when the forward pass has the gradients written before it go to memory beside it, 85.7;
 // 611 of 8191, K = 20: 6.9 and 8.1 us; 128 of 1024, K = 8: 4.0 and 3.3 us, latency.
+#include "operands.h"
 #include "vocab_row.h"
 
 using namespace cacti;
@@ -329,6 +330,9 @@ CACTI_API int cacti_hip_distill_topk_bwd(int64_t N, int64_t V, int64_t K, const 
     if (rc) return rc;
     CACTI_REQUIRE(scale && dlogit16 && aligned(scale, 4) && aligned(dlogit16, 2), CACTI_E_INVALID, "distill_topk_bwd: null pointer or misaligned operand");
     CACTI_REQUIRE(ldd >= V, CACTI_E_INVALID, "distill_topk_bwd: row pitch below a row");
+    // in place: a workgroup has read its row before it writes one
+    CACTI_REQUIRE((logit16 == dlogit16 && (ld == ldd || N == 1)) || !rows_share(N, logit16, ld, V, dlogit16, ldd, V), CACTI_E_INVALID,
+                  "distill_topk_bwd: the gradient takes the logits' place, with the same pitch, or shares no memory with them");
     a.scale = (const float *)scale;
     a.grad = (half_t *)dlogit16;
     a.ldd = ldd;

@@ -494,7 +494,8 @@ int cacti_hip_verify_draft_f16(int64_t T, int64_t B, int64_t V, const void *targ
  *   dlogit[j] (+)= f16(scale[n] / temperature * (p_j sum t - sum_{idx_i = j} t_i))
  * loss, scale: [N] f32; stats [N,2] f32: maximum and sum, written by the forward call, read by the adjoint.  An entry of -inf
  * has no weight; a row without any has loss 0 and gradient 0; the same id twice counts twice.  K <= 1024, V <= 65536, any
- * alignment of the rows.  status [1] i32 or NULL: 1 + the row of an id >= V (left out).  acc as everywhere. */
+ * alignment of the rows.  dlogit16 may be logit16 itself, with the same pitch, and shares no memory with it otherwise.  status [1] i32 or
+ * NULL: 1 + the row of an id >= V (left out).  acc as everywhere. */
 int cacti_hip_distill_topk_fwd(int64_t N, int64_t V, int64_t K, const void *logit16, int64_t ld, const void *idx, const void *val16,
                                double temperature, void *loss, void *stats, void *status, void *stream);
 int cacti_hip_distill_topk_bwd(int64_t N, int64_t V, int64_t K, const void *logit16, int64_t ld, const void *idx, const void *val16,

@@ -248,3 +248,33 @@ def test_captured_and_replayed():
         torch.cuda.synchronize()
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
         z.copy_(torch.roll(z, 3, 1))
+
+
+@pytest.mark.parametrize("change", [dict(d=66), dict(d=64 + 2 * 64), dict(ldd=65), dict(ld=128, ldd=128, d=64 + 2 * 63), dict(d=64 - 2 * 64)])
+def test_adjoint_refuses_a_gradient_that_overlaps_the_logits(change):
+    L = ffi.lib()
+    assert L.cacti_hip_distill_topk_bwd(*dict(BWD, logit=0x1040, **{"d": 0x1000 + change["d"]} if "d" in change else {"d": 0x1040},
+                                              **{k: v for k, v in change.items() if k != "d"}).values()) < 0
+    assert "place" in L.cacti_hip_last_error().decode()
+
+
+@GPU
+@pytest.mark.parametrize("N,V,ld,off", [(3, 1001, 1001, 0), (2, 32000, 32003, 5), (2, 65536, 65536, 0)])
+def test_gradient_in_the_logits_place(N, V, ld, off):
+    """Instead of the logits, and added to them."""
+    import torch
+    from cacti_amd import ops
+    z, idx, val, scale, temp = make(8, N, V, 40, 1.2)
+    di, dv, ds = dev(idx), dev(val), dev(scale)
+    buf = torch.zeros(N * ld + off, dtype=torch.float16, device="cuda")
+    rows = buf[off:].view(N, ld)[:, :V]
+    for acc in (False, True):
+        rows.copy_(dev(z))
+        _, stats = ops.distill_topk_fwd(rows, di, dv, temp)
+        want = ops.distill_topk_bwd(rows, di, dv, stats, ds, temp, acc=rows.clone() if acc else None)
+        if acc:
+            ops.distill_topk_bwd(rows, di, dv, stats, ds, temp, acc=rows)
+        else:
+            assert ffi.lib().cacti_hip_distill_topk_bwd(N, V, 40, rows.data_ptr(), ld, di.data_ptr(), dv.data_ptr(), stats.data_ptr(), ds.data_ptr(),
+                                                        temp, rows.data_ptr(), ld, 0, torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(rows, want)
