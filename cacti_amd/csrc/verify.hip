@@ -19,6 +19,7 @@
 // us, five rows of 32000 with a drafting model / 64 sequences, 294 rows: 15.9 / 33.9, of which the first launch is 4 / 18; a
 // workgroup per row that drew for every row that might end its sequence 77 / 115, one per sequence for the last two steps 22.5 / 38.6;
 // the last step by the last of a sequence's workgroups to write, which takes fences between the XCDs, 18.1 / 116.
+#include "operands.h"
 #include "vocab_row.h"
 
 using namespace cacti;
@@ -420,6 +421,7 @@ CACTI_API int cacti_hip_verify_draft_f16(int64_t T, int64_t B, int64_t V, const 
                       aligned(r, 4) && aligned(accepted, 4) && aligned(workspace, 16) && aligned(status, 4),
                   CACTI_E_INVALID, "verify_draft: misaligned operand");
     CACTI_REQUIRE(workspace_bytes >= cacti_hip_verify_draft_workspace(T, B, V), CACTI_E_INVALID, "verify_draft: workspace too small");
+    CACTI_REQUIRE(!rows_share(1, tok, T, T, next, T, T), CACTI_E_INVALID, "verify_draft: the tokens behind the rows share memory with theirs");
     const bool greedy = temperature == 0.;
     const int64_t E = entries_of(V, kPieces), E2 = entries_of(V, kLeft);
     Entry *entries = (Entry *)workspace;

@@ -270,7 +270,8 @@ def verify_draft(target, draft, tok, starts, u, r, temperature=1.0, status=None)
 
     Rows of a sequence are its last token and the drafted ones: tok u16-as-int16 [T] their tokens, target [T, V] the target
     model's logits, draft [T, V] the drafting model's or None (tokens drafted without probabilities).  u [T], r [sequences]:
-    uniform f32 random numbers.  temperature 0: greedy.  next holds accepted[b] kept tokens, the one that follows, then 0."""
+    uniform f32 random numbers.  temperature 0: greedy.  next holds accepted[b] kept tokens, the one that follows, then 0;
+    its rows of no sequence are not written."""
     return _op.verify_draft(target, draft, tok, starts, u, r, temperature, status)
 
 

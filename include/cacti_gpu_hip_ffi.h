@@ -480,9 +480,10 @@ int cacti_hip_paged_attention_f16(int64_t T, int64_t B, int64_t H, int64_t Hkv, 
  * i + 1 is kept if u[i] q_i(x) < p_i(x); a = the first row whose token is not, or the last; the token behind row a is the least
  * j with sum_{i <= j} w_i > r[b] sum w, w = max(p_a - q_a, 0), or p_a behind the last row (and where p = q).  temperature 0
  * (else 1e-3 to 1e6): the first arg max, and tokens are kept that are it.  u [T], r [B]: f32 in [0, 1).  accepted [B] i32 = a (0 for a sequence
- * without rows), next [T] u16 = the tokens behind the rows: those that are kept, the one of row a, then 0.  In fp64.  A NaN
- * logit counts as -inf, a row without a finite one as even.  status [1] i32 or NULL: 1 + the row of a token >= V (never
- * kept), 1 for rows beyond T.  workspace: cacti_hip_verify_draft_workspace bytes, 16-byte aligned.  V <= 65536, T < 2^18, B <= 65535. */
+ * without rows), next [T] u16, which shares no memory with tok, = the tokens behind the rows: those that are kept, the one of row a,
+ * then 0 (rows of no sequence, or of one whose rows there are not, are left as they are).  In fp64.  A NaN logit counts as -inf, a row
+ * without a finite one as even.  status [1] i32 or NULL: 1 + the row of a token >= V (never kept), 1 for rows beyond T.  workspace:
+ * cacti_hip_verify_draft_workspace bytes, 16-byte aligned.  V <= 65536, T < 2^18, B <= 65535. */
 size_t cacti_hip_verify_draft_workspace(int64_t T, int64_t B, int64_t V);
 int cacti_hip_verify_draft_f16(int64_t T, int64_t B, int64_t V, const void *target, int64_t ldt, const void *draft, int64_t ldd,
                                const void *tok, const void *starts, const void *u, const void *r, double temperature,

@@ -24,6 +24,14 @@ def test_refuses(change, why):
     assert why in L.cacti_hip_last_error().decode()
 
 
+@pytest.mark.parametrize("change", [dict(), dict(next=66), dict(next=64 + 6), dict(next=64 - 6)])
+def test_refuses_tokens_in_place(change):
+    """A row's token is read by the lane of the row before it."""
+    L = ffi.lib()
+    assert L.cacti_hip_verify_draft_f16(*dict(ARGS, **change).values()) < 0
+    assert "share memory" in L.cacti_hip_last_error().decode()
+
+
 def probabilities(z, temp):
     z = np.where(np.isnan(z), -np.inf, z.astype(np.float64))
     if temp == 0:
