@@ -1324,7 +1324,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_tiles_kernel(At
     const int64_t number = prompts ? blockIdx.x / kCut : blockIdx.x - bigs;
     const int from = prompts ? (int)(blockIdx.x % kCut) * kJoinRows : 0;       // the first row
     // the unit's sequence (as Units::find has it, from what the lanes have of the sequences), all work and that of those before it
-    const Units &u = prompts ? big : few;
+    const Units u = {prompts ? big.even : few.even, prompts ? big.per : few.per, prompts ? big.times : few.times, prompts ? big.more : few.more, 0};
     int b = u.even ? (int)(number / u.even) : 0;
     double all = 0., some = 0.;
     Sequence s = {0, 0, 0, false};
