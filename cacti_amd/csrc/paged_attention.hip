@@ -3,12 +3,14 @@
 //
 // One pass over the keys with a running m, the maximum of a row's scores so far (or, prompts in 16 bits, up to kSlack less).  The codes
 // meet the queries as they are (e4m3 to f16 is exact) and a page's scales join the scores: with t_j = alpha ks q . k_j log2 e + log2 vs,
-//   w_j = 2^(t_j - m),  o = sum w_j code(v_j) / sum w_j / vs
-// so that the weight that meets a code already holds its page's scale, and no w exceeds f16 whatever the scales are.
+//   w_j = 2^(15 + t_j - m),  o = sum w_j code(v_j) / sum w_j / vs
+// so that the weight that meets a code already holds its page's scale, and no w exceeds f16 whatever the scales are.  The largest w is
+// 2^15, at the upper end of f16, to leave those of a row's other pages their bits down to 2^-29 of it: with 1 for the largest, one large
+// value in a page, 2^18 above the others, cost those 4 bits of their 11.
 // Scores, maxima, sums and o are fp32; w is rounded to f16 for the matrix instruction (2^-11 relative, each on its own, which
 // is what the rounding of the output adds once more).  The sum is that of w as it was, since a page of small values may have
-// weights that are nothing in f16 and most of the probability; the largest w is 1, and exact.  With kSlack it need not be, but there
-// are no scales then: the sum is that of the rounded w, and what a large one is off by is off in both.
+// weights that are nothing in f16 and most of the probability; the largest w is a power of two, and exact.  With kSlack it need not be,
+// but there are no scales then: the sum is that of the rounded w, and what a large one is off by is off in both.
 //
 // A wave takes 16 NR rows (tokens of a sequence by the query heads that share a key head) of a key head at a time, by itself, 32
 // positions at a time.  The products are formed transposed, S^T = K Q^T and O^T = V^T W^T with v_mfma_f32_16x16x32_f16: a lane
@@ -369,10 +371,10 @@ __device__ __forceinline__ Scales scales_of(const Entry &e, int pg, float alpha)
 // The scores s of 32 positions of a lane's row (eight of them, in two registers of four) to weights: with c > 0 and lg of the
 // lane's page, t = s c + lg.  Takes part in the running m and sum l (of weights by iv) and scales o where m grows; returns the
 // weights in f16.  seen: how many of the lane's eight positions its row sees; edge (the same in all lanes): not all of all.
-// SLACK: m grows only where a lane has more than kSlack above it, else the row's lanes need not hear of each other's scores, and w
-// may be up to 2^kSlack (prompts in 16 bits of up to 900 rows and 4000 positions, 16 heads of 128: 78.6 -> 74.1 us; single tokens, bound
-// by memory, gain nothing).
-constexpr float kSlack = 8.f;
+// SLACK: m grows only where a lane has more than kSlack above it, else the row's lanes need not hear of each other's scores; weights are
+// 2^-kSlack of what they are otherwise, for they may be 2^kSlack too large (prompts in 16 bits of up to 900 rows and 4000 positions, 16
+// heads of 128: 78.6 -> 74.1 us; single tokens, bound by memory, gain nothing).
+constexpr float kTop = 15.f, kSlack = 8.f;
 // x + a half of h, the conversion and the sum (in fp32) in one operation
 __device__ __forceinline__ float plus_low(float x, unsigned h)
 {
@@ -402,7 +404,7 @@ __device__ __forceinline__ half8_t weigh(float4_t (&s)[2], float c, float lg, fl
 #pragma unroll
         for (int i = 0; i < N; i++) o[i] *= f;
     }
-    const float off = lg - finite_max(m);
+    const float off = lg + (SLACK ? kTop - kSlack : kTop) - finite_max(m);
     float even = 0.f, uneven = 0.f;
     Frag p;
 #pragma unroll

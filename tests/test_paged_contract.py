@@ -272,3 +272,19 @@ def test_queries_and_output_in_the_columns_of_one_buffer():
         assert torch.equal(out, want) and torch.equal(q, B.d["q"]) and bool((both[:, :40] == 7).all()) and bool((both[:, 840:] == 7).all())
         with pytest.raises(ffi.CactiError, match="shares memory"):
             ops.paged_attention(q, cache, *B.at(), B.alpha, out=both[:, 436:836].view(-1, 4, 100))
+
+
+# ---------------------------------------------------------------- scales
+@GPU
+@pytest.mark.parametrize("apart", [12, 18, 24])
+@pytest.mark.parametrize("n,lens", [([1], [300]), ([2, 1], [200, 90]), ([150, 1], [260, 70])])
+def test_attention_of_a_page_with_one_large_value(n, lens, apart):
+    """A page whose scale one value made: the weights of the other pages' codes are 2^-apart of its own, and have their bits all the same."""
+    B = Batch(93 + apart, n, lens, 4, 2, 64, 16, 8)
+    B.vs[:] = 2.0 ** -14
+    for b in range(B.B):
+        p = B.table[b, 1]
+        B.vs[p] = 2.0 ** (apart - 14)
+        B.vp[p] = 0
+        B.vp[p, :, 5, 3] = 0x70                               # 128
+    check_attention(B)
