@@ -462,10 +462,13 @@ int cacti_hip_paged_append(int64_t T, int64_t B, int64_t H, int64_t Hkv, int64_t
                            int bits, int64_t P, int64_t page, const void *table, int64_t ldt, int64_t W, const void *starts,
                            const void *lens, void *status, void *stream);
 
-/* out [T, ldo] f16, which shares no memory with q, = softmax_j(alpha q . k_j) v over the positions j up to the row's own, which are in the cache; fp32 scores
- * and sums, the weights rounded to f16 for the second product.  A row's result depends on nothing behind its position.  Scales
- * are positive, any of them.  workspace: cacti_hip_paged_attention_workspace bytes, 16-byte aligned, contents undefined on
- * return. */
+/* out [T, ldo] f16, which shares no memory with q, = softmax_j(alpha q . k_j) v over the positions j up to the row's own, which are in
+ * the cache; scores, maxima and sums in fp32.  What is rounded on the way: a query against e4m3 to three e4m3 terms, all 11 bits of
+ * elements of at least 1/112 of the row's largest, the others to 2^-18 of that; for the second product a weight, probability by its
+ * page's value scale, to f16: 2^-11 of itself, but no less than 2^-32 of the row's largest.  Prompts in 16 bits (where
+ * max_new H / Hkv > 128) divide by the sum of the rounded weights.  A row's result depends on nothing behind its position.  Key scales
+ * are positive, value scales between 2^-40 and 2^40 (an append's are 2^-32 to 2^15).  workspace:
+ * cacti_hip_paged_attention_workspace bytes, 16-byte aligned, contents undefined on return. */
 size_t cacti_hip_paged_attention_workspace(int64_t T, int64_t B, int64_t H, int64_t Hkv, int64_t Dh, int64_t max_new);
 int cacti_hip_paged_attention_f16(int64_t T, int64_t B, int64_t H, int64_t Hkv, int64_t Dh, int64_t max_new, float alpha,
                                   const void *q, int64_t ldq, const void *k_pages, const void *v_pages, const void *k_scale,

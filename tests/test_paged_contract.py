@@ -288,3 +288,25 @@ def test_attention_of_a_page_with_one_large_value(n, lens, apart):
         B.vp[p] = 0
         B.vp[p, :, 5, 3] = 0x70                               # 128
     check_attention(B)
+
+
+@GPU
+@pytest.mark.parametrize("n,lens", [([2], [200]), ([90], [200])])
+def test_attention_of_scales_at_the_ends(n, lens):
+    """The least and the largest of the value scales, and key scales that are subnormal or near the largest."""
+    for what in ("least", "largest beside small ones", "keys of nothing", "keys far up"):
+        print("paged_attention", n, what, flush=True)
+        B = Batch(94, n, lens, 4, 2, 64, 16, 8)
+        odd, even = B.table[0, 1::2], B.table[0, ::2]
+        if what == "least":
+            B.vs[:] = 2.0 ** -40
+        elif what == "largest beside small ones":                 # scores of about 80 against 0
+            B.vs[odd], B.vs[even] = 2.0 ** 40, 2.0 ** -10
+            B.vp[odd], B.kp[odd], B.kp[even] = 0, 0, 0x38             # 1
+            B.qkv[:, :256] = np.abs(B.qkv[:, :256])
+            B.ks[:] = 16.0
+        elif what == "keys of nothing":
+            B.ks[:] = 2.0 ** -140
+        else:
+            B.ks[:], B.kp[:] = 2.0 ** 100, 0
+        check_attention(B)
