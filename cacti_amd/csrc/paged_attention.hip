@@ -149,9 +149,8 @@ __device__ __forceinline__ float4_t mfma(half8_t a, half8_t b, float4_t c) { ret
 template <int ND>
 struct QueryWords {
     u2_t w[4 * ND];                            // as loaded: word i at column 64 (i / 4) + 16 g + 4 (i % 4)
-    __device__ __forceinline__ void load(const half_t *q, int Dh)          // (Dh is a multiple of 4)
+    __device__ __forceinline__ void load(const half_t *q, int Dh, int g)   // (Dh is a multiple of 4)
     {
-        const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
         for (int i = 0; i < 4 * ND; i++) w[i] = *reinterpret_cast<const u2_t *>(q + min(64 * (i / 4) + 16 * g + 4 * (i & 3), Dh - 4));
     }
@@ -516,7 +515,7 @@ struct Tile {
             for (int n = 0; n < NR; n++) {
                 const int r = min(row0 + 16 * n + r16, rows - 1), t = r / a.G;
                 last[n] = s.first + t;
-                words[n].load(a.q + (int64_t)(s.s0 + t) * a.ldq + (h * a.G + r - t * a.G) * a.Dh, a.Dh);
+                words[n].load(a.q + (int64_t)(s.s0 + t) * a.ldq + (h * a.G + r - t * a.G) * a.Dh, a.Dh, lane >> 4);
             }
             request(id, c0 - base);
 #pragma unroll

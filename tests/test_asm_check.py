@@ -78,3 +78,22 @@ def test_kernels_that_hold_more_registers_than_they_may():
     assert asm_check.check(text, registers=[("kern", 136)]) == []
     assert asm_check.check(text, registers=[("kern", 128)]) == ["kernel: 136 registers, 128 at most"]
     assert asm_check.check(text, registers=[("other", 128)]) == ["no kernel is named like other"]
+
+
+@pytest.mark.parametrize("src", ["gemm_direct.hip", "paged_attention.hip"])
+def test_the_build_refuses_spills_of_kernels_that_hold_all_registers(src, tmp_path, monkeypatch):
+    from cacti_amd import build
+    monkeypatch.setattr(build, "OUT_DIR", str(tmp_path))
+    monkeypatch.setattr(build, "REGISTERS", {})
+
+    def compiled(text):
+        def hipcc(src, obj, *more):
+            for name, what in ((obj, ""), (obj[:-2] + "-gfx950.s", text)):
+                with open(name, "w") as f:
+                    f.write(what)
+        monkeypatch.setattr(build, "_hipcc", hipcc)
+        return build._compile(src)
+
+    assert compiled(GOOD).endswith(src.replace(".hip", ".o"))
+    with pytest.raises(RuntimeError, match="48 bytes of registers in memory"):
+        compiled(GOOD.replace("; ScratchSize: 0", "; ScratchSize: 48"))
