@@ -1217,7 +1217,7 @@ struct Joined {
 };
 
 // The parts of a row put together, two columns per lane, by a wave or, for few rows, a workgroup of four waves; zeros for rows whose
-// sequence's numbers do not fit together.  Bound by latency: eight parts are requested at once, their sums with their values.
+// sequence's numbers do not fit together, which the last workgroup names.  Bound by latency: eight parts are requested at once, their sums with their values.
 template <int NR, int WAVES>
 __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs a)
 {
@@ -1225,6 +1225,11 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs
     const PagedBatch &pb = a.pb;
     const int lane = threadIdx.x & 63, wid = uniform((int)threadIdx.x >> 6), at_row = (int)blockIdx.x * (kWaves / WAVES) + (WAVES == 1 ? wid : 0);
     const int row = at_row / a.H, head = at_row - row * a.H, first = WAVES == 1 ? 0 : wid, d = min(2 * lane, a.Dh - 2);
+    if (blockIdx.x == gridDim.x - 1) {         // names what does not fit, whether it has rows or not
+        for (int b = threadIdx.x; b < pb.B; b += kThreads)
+            if (!sequence(pb, b, (int64_t)pb.W * pb.page, a.max_new).ok) report(pb, b);
+        return;
+    }
     // all work, that of the sequences before the row's, and the row's sequence
     double all = 0., some = 0.;
     Sequence s = {0, 0, 0, false};
@@ -1232,9 +1237,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs
     for (int b0 = 0; b0 < pb.B; b0 += 64) {
         const Sequence q = lane_sequence(a, b0);
         const double u = Share(a, kRows, q).units;
-        const bool there = b0 + lane < pb.B;
-        const uint64_t hit = __ballot(there && row >= q.s0 && row < (int)((unsigned)q.s0 + (unsigned)q.n));
-        if (at_row == 0 && there && !q.ok) report(pb, b0 + lane);
+        const uint64_t hit = __ballot(b0 + lane < pb.B && row >= q.s0 && row < (int)((unsigned)q.s0 + (unsigned)q.n));
         all += u;
         some += b < 0 && (!hit || lane < __ffsll((unsigned long long)hit) - 1) ? u : 0.;
         if (hit && b < 0) {
@@ -1251,8 +1254,9 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs
     }
     const int h = head / a.G, r = (row - s.s0) * a.G + head - h * a.G, tile = r / kRows;
     all = wave_sum_f64(all);
+    some = wave_sum_f64(some);
     if (too_much(all)) return;
-    const Parts in(a, s, kRows, h, tile, uniform((int)(unsigned)all), uniform((int)(unsigned)wave_sum_f64(some)));
+    const Parts in(a, s, kRows, h, tile, uniform((int)(unsigned)all), uniform((int)(unsigned)some));
     const int parts = in.count;
     if (parts == 1) return;
     Joined<2> j;
@@ -1348,8 +1352,9 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_tiles_kernel(At
     if (from >= here) return;
     if (prompts != (rows > a.few)) return;
     all = wave_sum_f64(all);
+    some = wave_sum_f64(some);
     if (too_much(all)) return;
-    const Parts in(a, s, kRows, h, tile, uniform((int)(unsigned)all), uniform((int)(unsigned)wave_sum_f64(some)));
+    const Parts in(a, s, kRows, h, tile, uniform((int)(unsigned)all), uniform((int)(unsigned)some));
     if (in.count == 1) return;
     const float *part = prompts ? a.big_part : a.part, *stats = prompts ? a.big_stats : a.stats;
     constexpr int kAtOnce = 4;                 // parts at once, of two rows
@@ -1420,8 +1425,8 @@ int launch_join(const AttnArgs &a, hipStream_t st)
 {
     if (a.big_groups) return launch_join_prompts(a, st);
     const int64_t rh = (int64_t)a.pb.T * a.H;
-    if (rh < 4 * device_cus()) hipLaunchKernelGGL((paged_attention_join_kernel<NR, kWaves>), dim3((unsigned)rh), dim3(kThreads), 0, st, a);
-    else hipLaunchKernelGGL((paged_attention_join_kernel<NR, 1>), dim3((unsigned)((rh + kWaves - 1) / kWaves)), dim3(kThreads), 0, st, a);
+    if (rh < 4 * device_cus()) hipLaunchKernelGGL((paged_attention_join_kernel<NR, kWaves>), dim3((unsigned)rh + 1), dim3(kThreads), 0, st, a);
+    else hipLaunchKernelGGL((paged_attention_join_kernel<NR, 1>), dim3((unsigned)((rh + kWaves - 1) / kWaves) + 1), dim3(kThreads), 0, st, a);
     return launch_status("paged_attention (parts)");
 }
 template <int ND, int NR, class P>
