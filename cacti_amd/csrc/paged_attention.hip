@@ -27,17 +27,15 @@
 // share leaves partial sums, which a second launch puts together.
 #include "operands.h"
 #include "paged.h"
+#include "paged_shares.h"
 
 using namespace cacti;
 
 namespace {
 
-constexpr int kThreads = 256, kWaves = 4, kStep = 32;
-constexpr int kEntries = 64;                   // pages that a wave looks up at a time, one to a lane
-// What a tile of rows costs a share besides its steps, in steps: queries, pages and the first keys to wait for.  (48 sequences
-// of 120 to 8192 positions, 16 rows, 1 / 2 / 4 / 8: 130.2 / 128.4 / 129.4 / 131.3 us; 24 of 100 to 6000, 32 rows, 2 / 4 / 8 / 16:
-// 29.1 / 27.7 / 28.5 / 29.4)
-constexpr int begin_of(int tile) { return tile / 8; }
+using namespace cacti::shares;
+
+constexpr int kThreads = 64 * kWaves;
 
 struct AttnArgs {
     PagedBatch pb;
@@ -68,45 +66,23 @@ __device__ __forceinline__ int lane_here()
     return lane;
 }
 
-// A sequence's share of the work: its tiles of rows by its steps (and begin_of), by heads
-struct Share {
-    int tiles, steps;
-    unsigned units;
-    __device__ __forceinline__ Share(const AttnArgs &a, int tile, const Sequence &s)
-        : tiles((s.n * a.G + tile - 1) / tile), steps((s.first + s.n + kStep - 1) / kStep),
-          units(s.ok && s.n > 0 && s.n * a.G <= a.few ? (unsigned)(tiles * (steps + begin_of(tile)) * a.Hkv) : 0u)
-    {
-    }
-};
+// A sequence's share of the work, as one of few rows and as a prompt
+__device__ __forceinline__ Share share_of(const AttnArgs &a, int tile, const Sequence &s)
+{
+    return Share(tile, s.n * a.G, s.first + s.n, a.Hkv, s.ok && s.n > 0 && s.n * a.G <= a.few);
+}
+__device__ __forceinline__ BigShare big_share_of(const AttnArgs &a, const Sequence &s) { return BigShare(a.G, s.n * a.G, s.first, s.ok && s.n * a.G > a.few); }
 __device__ __forceinline__ Sequence lane_sequence(const AttnArgs &a, int b0)
 {
     return lane_sequence(a.pb, b0, (int64_t)a.pb.W * a.pb.page, a.max_new);
 }
 
-// A wave's part of a share is at least that many units: fewer steps are more parts to put together than they save (one sequence of
-// 1540 positions, 32 heads of 100, 1 / 2 / 3 / 4: 13.7 / 12.4 / 13.1 / 13.5 us)
-constexpr unsigned kLeast = 2;
-__device__ __forceinline__ unsigned groups_of(const AttnArgs &a, unsigned units) { return min((unsigned)a.groups, max(units / (kLeast * kWaves), 1u)); }
-
 // Work is counted in 32 bits; the host has seen to it that rows which each are of one sequence are not more.  (Where starts fall a row may
 // be of many: nothing is done then.)
 __device__ __forceinline__ bool too_much(double units) { return units > (double)INT32_MAX; }
 
-constexpr unsigned kBigLeast = 4;              // the same of steps of 64 positions
 // Workgroups go round the 8 XCDs: those of one XCD get neighbouring numbers (of n, a multiple of 8)
 __device__ __forceinline__ unsigned xcd_order(unsigned i, unsigned n) { return (i & 7) * (n / 8) + i / 8; }
-
-// Equal shares of `units`: group i has those from begin(i) to begin(i + 1), the first `more` of them one more than `each`
-struct Shares {
-    unsigned each, more;
-    __device__ __forceinline__ Shares(unsigned units, unsigned groups) : each(units / groups), more(units - each * groups) {}
-    __device__ __forceinline__ unsigned begin(unsigned i) const { return i * each + min(i, more); }
-    __device__ __forceinline__ unsigned of(unsigned unit) const          // the group that has it
-    {
-        const unsigned edge = more * (each + 1);
-        return unit < edge ? unit / (each + 1) : more + (unit - edge) / each;
-    }
-};
 
 typedef unsigned u4_t __attribute__((ext_vector_type(4)));
 typedef unsigned u2_t __attribute__((ext_vector_type(2)));
@@ -433,7 +409,7 @@ struct Tile {
     VBlock<P, VD> vv;
     bool odd;                                  // there was a NaN or an infinity of V that some rows see
 
-    __device__ __forceinline__ int page_of(int x) const { return (int)(__umul24((unsigned)x, a.page_magic) >> 22); }
+    __device__ __forceinline__ int page_of(int x) const { return shares::page_of(x, a.page_magic); }
 
     // keys and values of the 32 positions from x on, counted from the first entry's page; behind `end` the last one again
     __device__ __forceinline__ void load_k(int x, int end)
@@ -481,10 +457,10 @@ struct Tile {
         float ks = 1.f, vs = 1.f;
         // the pages from position `seg` on: their numbers, their addresses and the first keys and values, what their scales make
         auto look_up = [&](int seg) __attribute__((always_inline)) {
-            const int p0 = uniform(seg / a.pb.page);
-            base = p0 * a.pb.page;
-            end = min(c1 - base, kEntries * a.pb.page);
-            return a.pb.table[(int64_t)b * a.pb.ldt + p0 + min(lane, page_of(end - 1))];
+            const Pages p(uniform(seg), c1, a.pb.page);
+            base = p.base;
+            end = p.end;
+            return a.pb.table[(int64_t)b * a.pb.ldt + p.p0 + min(lane, p.last(a.page_magic))];
         };
         auto request = [&](int id, int x) __attribute__((always_inline)) {
             if (id < 0 || id >= a.pb.P) {
@@ -671,17 +647,16 @@ template <int ND, int NR, class P>
 __global__ void __launch_bounds__(kThreads, resident(ND, NR, sizeof(P))) paged_attention_kernel(AttnArgs a)
 {
     constexpr int kRows = 16 * NR;
-    constexpr unsigned kBegin = begin_of(kRows);
     __shared__ Entry entries[kWaves];
     __shared__ typename Tile<ND, NR, P>::Deposit deposits[kWaves - 1];     // of waves 1, 2, 3
     const unsigned wid = uniform((int)threadIdx.x >> 6), group = blockIdx.x;
     const Sequence s64 = lane_sequence(a, 0);              // of the first 64 sequences, which mostly are all
-    const double u64 = Share(a, kRows, s64).units;         // (whole numbers)
+    const double u64 = share_of(a, kRows, s64).units;      // (whole numbers)
     double all = u64;
-    for (int b0 = 64; b0 < a.pb.B; b0 += 64) all += Share(a, kRows, lane_sequence(a, b0)).units;
+    for (int b0 = 64; b0 < a.pb.B; b0 += 64) all += share_of(a, kRows, lane_sequence(a, b0)).units;
     all = wave_sum_f64(all);
     if (too_much(all)) return;
-    const unsigned units = uniform((int)(unsigned)all), groups = groups_of(a, units);
+    const unsigned units = uniform((int)(unsigned)all), groups = groups_of(a.groups, units);
     if (group >= groups) return;
     const Shares shares(units, groups);
     const unsigned x0 = uniform((int)shares.begin(group)), x1 = uniform((int)shares.begin(group + 1));     // the workgroup's
@@ -692,7 +667,7 @@ __global__ void __launch_bounds__(kThreads, resident(ND, NR, sizeof(P))) paged_a
     int b = 0;
     unsigned before = 0;
     for (int b0 = 0; b0 < a.pb.B; b0 += 64) {
-        const double u = b0 == 0 ? u64 : Share(a, kRows, lane_sequence(a, b0)).units, upto = scan_f64(u) + (double)before;
+        const double u = b0 == 0 ? u64 : share_of(a, kRows, lane_sequence(a, b0)).units, upto = scan_f64(u) + (double)before;
         const uint64_t hit = __ballot(upto > (double)x);
         const int at = hit ? __ffsll((unsigned long long)hit) - 1 : 63;
         before = (unsigned)uniform((int)(unsigned)lane_f64(hit ? upto - u : upto, at));
@@ -709,25 +684,24 @@ __global__ void __launch_bounds__(kThreads, resident(ND, NR, sizeof(P))) paged_a
     bool others = false;                       // there are other waves' to put together with what t has
     for (; x < until; b++) {
         s = b < 64 ? of_lane(s64, b) : sequence(a.pb, b, (int64_t)a.pb.W * a.pb.page, a.max_new);
-        const Share w(a, kRows, s);
+        const Share w = share_of(a, kRows, s);
         const unsigned behind = before + w.units;
         while (x < until && x < behind) {
-            const unsigned whole = w.steps + kBegin;
-            const int u = uniform((int)((x - before) / whole)), rows = s.n * a.G;
-            const unsigned start = before + u * whole + kBegin, end = start + w.steps;         // of the tile's steps
-            h = uniform(u / w.tiles);
-            row0 = (u - h * w.tiles) * kRows;
-            const unsigned g0 = max(x0, start), u0 = max(x, start), u1 = min(until, end);
-            g1 = min(x1, end);
-            x = u1;
-            if (u1 <= u0) continue;            // (a share may end before the tile's first step)
+            const Part p(w, kRows, before, x, until, x0, x1);
+            const int rows = s.n * a.G;
+            h = p.h;
+            row0 = p.row0;
+            g1 = p.g1;
+            x = p.u1;
+            if (p.u1 <= p.u0) continue;        // (a share may end before the tile's first step)
             const int seen = uniform(s.first + min(rows - 1, row0 + kRows - 1) / a.G + 1);     // positions that some row sees
-            const int c0 = (int)(u0 - start) * kStep, c1 = min(seen, (int)(u1 - start) * kStep);
+            const int c0 = p.c0(), c1 = p.c1(seen);
+            const bool mine = p.u0 == p.g0;    // else it goes to the wave that has the tile's first
+            slot = p.slot(group);
+            others = mine && p.u1 < g1;
             t.run(b, s, h, rows, row0, c0, c1);
             if (t.odd) t.add_odd(b, h, max(c0, s.first + row0 / a.G + 1), c1);
-            slot = g0 == start && g1 == end ? -1 : 2 * (int)group + (g0 == start);
-            others = u0 == g0 && u1 < g1;
-            if (u0 > g0) t.put(deposits[wid - 1]);
+            if (!mine) t.put(deposits[wid - 1]);
             else if (!others) t.write(s, h, rows, row0, slot);
         }
         before = behind;
@@ -747,34 +721,9 @@ __global__ void __launch_bounds__(kThreads, resident(ND, NR, sizeof(P))) paged_a
 // evenly over the banks.  (16 rows to each of eight waves read the operands twice as often and have half the registers: 88.6
 // against 83 us for three sequences of up to 900 rows and 4000 positions, 16 heads of 128.)
 //
-// Shares are cut as above, a workgroup to a share and by steps of 64.  A tile's steps grow by those of its own 128 rows: counted
-// by a line that is never below them, so that what lies before a tile is a formula; steps behind a tile's last position are
-// nothing.  Workgroups of an XCD have neighbouring shares: the tiles of a head read its keys and values from one L2.
-constexpr int kPrompt = 128, kBig = 64;
-// As begin_of, in steps.  (Prompts of up to 900 rows and 4000 positions, 16 heads of 128, 2 / 3 / 4 / 5: 74.9 / 73.3 / 71.4 / 74.0 us; one
-// of 4096 130 / 121 / 122 / 125)
-constexpr int kBigBegin = 4;
-
+// Shares are cut as above, a workgroup to a share and by steps of 64.  Workgroups of an XCD have neighbouring shares: the tiles of a
+// head read its keys and values from one L2.
 __device__ __forceinline__ int swap_of(int row) { return ((row >> 2) ^ row) & 7; }
-
-struct BigShare {
-    int tiles, base, slope, run;               // steps of tile t: base + slope (t + 1), or, slope 0, base + t / run + 1
-    __device__ __forceinline__ BigShare(const AttnArgs &a, const Sequence &s)
-    {
-        const int tokens = (kPrompt + a.G - 1) / a.G;
-        tiles = s.ok && s.n * a.G > a.few ? (s.n * a.G + kPrompt - 1) / kPrompt : 0;
-        base = (s.first + kBig - 1) / kBig + kBigBegin;
-        slope = tokens >= kBig ? (tokens + kBig - 1) / kBig : 0;
-        run = slope ? 1 : kBig / tokens;
-    }
-    __device__ __forceinline__ unsigned before(int t) const      // tile t
-    {
-        if (slope) return (unsigned)(t * base + slope * (t * (t + 1) / 2));
-        const int q = t / run, r = t - q * run;
-        return (unsigned)(t * base + run * (q * (q - 1) / 2) + r * q + t);
-    }
-    __device__ __forceinline__ unsigned units(const AttnArgs &a) const { return before(tiles) * (unsigned)a.Hkv; }
-};
 
 constexpr int kBigThreads = 256, kBigWaves = kBigThreads / 64;
 
@@ -804,7 +753,7 @@ struct Prompt {
         VBlock<P, 4> v[kBlocks];
     } next;
 
-    __device__ __forceinline__ int page_of(int x) const { return (int)(__umul24((unsigned)x, a.page_magic) >> 22); }
+    __device__ __forceinline__ int page_of(int x) const { return shares::page_of(x, a.page_magic); }
 
     // 16 positions in a row are of one page (x: the first of them, of full ones), and so is all that a wave loads at once: the address
     // of its first row is a scalar, a lane's part of it the same every time (but for the positions behind `end`).
@@ -986,10 +935,10 @@ struct Prompt {
         const int mine = row0 + 32 * wid;      // the wave's first row
         // the pages from position `seg` on: the lane's number of them
         auto look_up = [&](int seg) __attribute__((always_inline)) {
-            const int p0 = uniform(seg / a.pb.page), most = page_of(min(c1 - p0 * a.pb.page, kEntries * a.pb.page) - 1);
-            return a.pb.table[(int64_t)b * a.pb.ldt + p0 + min(lane, most)];
+            const Pages p(uniform(seg), c1, a.pb.page);
+            return a.pb.table[(int64_t)b * a.pb.ldt + p.p0 + min(lane, p.last(a.page_magic))];
         };
-        int id = look_up(min(c0, c1 - 1));     // requested with the queries, of a page that there is
+        int id = look_up(BigPart::look(c0, c1));           // requested with the queries
         u2_t words[2][2 * NS];
 #pragma unroll
         for (int n = 0; n < 2; n++) {
@@ -1024,7 +973,8 @@ struct Prompt {
         const Places at = places();
         const Own w = own();
         for (int seg = c0; seg < c1;) {
-            const int p0 = uniform(seg / a.pb.page), base = p0 * a.pb.page, end = min(c1 - base, kEntries * a.pb.page);
+            const Pages pages(uniform(seg), c1, a.pb.page);
+            const int base = pages.base, end = pages.end;
             __syncthreads();                   // (entries and buffers of before are done with)
             if (seg != c0) id = look_up(seg);
             if (tid < 64) {
@@ -1112,12 +1062,12 @@ __global__ void __launch_bounds__(kBigThreads, 2) paged_prompt_kernel(AttnArgs a
     __shared__ typename Prompt<ND, P>::Shared sh;
     const int lane = threadIdx.x & 63;
     const Sequence s64 = lane_sequence(a, 0);
-    const double u64 = BigShare(a, s64).units(a);
+    const double u64 = big_share_of(a, s64).units(a.Hkv);
     double all = u64;
-    for (int b0 = 64; b0 < a.pb.B; b0 += 64) all += BigShare(a, lane_sequence(a, b0)).units(a);
+    for (int b0 = 64; b0 < a.pb.B; b0 += 64) all += big_share_of(a, lane_sequence(a, b0)).units(a.Hkv);
     all = wave_sum_f64(all);
     if (too_much(all)) return;
-    const unsigned units = uniform((int)(unsigned)all), groups = min((unsigned)a.big_groups, max(units / kBigLeast, 1u));
+    const unsigned units = uniform((int)(unsigned)all), groups = big_groups_of(a.big_groups, units);
     const unsigned group = xcd_order(blockIdx.x, a.big_groups);
     if (units == 0 || group >= groups) return;
     const Shares shares(units, groups);
@@ -1126,7 +1076,7 @@ __global__ void __launch_bounds__(kBigThreads, 2) paged_prompt_kernel(AttnArgs a
     int b = 0;
     unsigned before = 0;
     for (int b0 = 0; b0 < a.pb.B; b0 += 64) {
-        const double u = b0 == 0 ? u64 : BigShare(a, lane_sequence(a, b0)).units(a), upto = scan_f64(u) + (double)before;
+        const double u = b0 == 0 ? u64 : big_share_of(a, lane_sequence(a, b0)).units(a.Hkv), upto = scan_f64(u) + (double)before;
         const uint64_t hit = __ballot(upto > (double)x);
         const int at = hit ? __ffsll((unsigned long long)hit) - 1 : 63;
         before = (unsigned)uniform((int)(unsigned)lane_f64(hit ? upto - u : upto, at));
@@ -1137,8 +1087,8 @@ __global__ void __launch_bounds__(kBigThreads, 2) paged_prompt_kernel(AttnArgs a
     }
     for (; x < until; b++) {
         const Sequence s = b < 64 ? of_lane(s64, b) : sequence(a.pb, b, (int64_t)a.pb.W * a.pb.page, a.max_new);
-        const BigShare w(a, s);
-        const unsigned head = w.before(w.tiles), behind = before + w.units(a);
+        const BigShare w = big_share_of(a, s);
+        const unsigned head = w.before(w.tiles), behind = before + w.units(a.Hkv);
         while (x < until && x < behind) {
             const int h = uniform((int)((x - before) / head)), rows = s.n * a.G;
             const unsigned in = x - before - h * head;
@@ -1152,12 +1102,12 @@ __global__ void __launch_bounds__(kBigThreads, 2) paged_prompt_kernel(AttnArgs a
             const unsigned start = uniform((int)w.before(tile)), whole = uniform((int)w.before(tile + 1)) - start;
             const int from = (int)(in - start), to = (int)min(whole, from + (until - x)), row0 = tile * kPrompt;
             const int end = uniform(s.first + min(rows - 1, row0 + kPrompt - 1) / a.G + 1);
-            const int first = max(from - kBigBegin, 0), behind_last = to - kBigBegin;
-            if (behind_last > first) {
-                const int c0 = uniform(first * kBig), c1 = uniform(min(end, behind_last * kBig));
+            const BigPart p(from, to, (int)whole);
+            if (p.behind > p.first) {
+                const int c0 = uniform(p.c0()), c1 = uniform(p.c1(end));
                 Prompt<ND, P> t{a, sh};
                 t.run(b, s, h, rows, row0, c0, c1);
-                t.write(b, s, h, rows, row0, c0, c1, first == 0 && behind_last == (int)whole - kBigBegin ? -1 : 2 * (int)group + (first == 0));
+                t.write(b, s, h, rows, row0, c0, c1, p.slot(group));
             }
             x += to - from;
         }
@@ -1165,29 +1115,26 @@ __global__ void __launch_bounds__(kBigThreads, 2) paged_prompt_kernel(AttnArgs a
     }
 }
 
-// Where the parts of a tile of rows are: those of its first step's group, of the next ones and of its last step's
-struct Parts {
-    int i0, count;
-    __device__ __forceinline__ Parts(const AttnArgs &a, const Sequence &s, int rows, int h, int tile, unsigned units, unsigned before)
-    {
-        unsigned first, steps, groups;
-        if (s.n * a.G > a.few) {
-            const BigShare w(a, s);
-            first = before + h * w.before(w.tiles) + w.before(tile) + kBigBegin;
-            steps = w.before(tile + 1) - w.before(tile) - kBigBegin;
-            groups = min((unsigned)a.big_groups, max(units / kBigLeast, 1u));
-        } else {
-            const Share w(a, rows, s);
-            first = before + (unsigned)(h * w.tiles + tile) * (w.steps + begin_of(rows)) + begin_of(rows);
-            steps = w.steps;
-            groups = groups_of(a, units);
-        }
-        const Shares shares(units, groups);
-        i0 = uniform((int)shares.of(first));
-        count = uniform((int)shares.of(first + steps - 1)) - i0 + 1;
+// Where the parts of a tile of rows are
+__device__ __forceinline__ Parts parts_of(const AttnArgs &a, const Sequence &s, int rows, int h, int tile, unsigned units, unsigned before)
+{
+    unsigned first, steps, groups;
+    if (s.n * a.G > a.few) {
+        const BigShare w = big_share_of(a, s);
+        first = before + h * w.before(w.tiles) + w.before(tile) + kBigBegin;
+        steps = w.before(tile + 1) - w.before(tile) - kBigBegin;
+        groups = big_groups_of(a.big_groups, units);
+    } else {
+        const Share w = share_of(a, rows, s);
+        first = before + (unsigned)(h * w.tiles + tile) * (w.steps + begin_of(rows)) + begin_of(rows);
+        steps = w.steps;
+        groups = groups_of(a.groups, units);
     }
-    __device__ __forceinline__ int slot(int p) const { return p == 0 ? 2 * i0 + 1 : 2 * (i0 + p); }
-};
+    Parts p(units, groups, first, steps);
+    p.i0 = uniform(p.i0);
+    p.count = uniform(p.count);
+    return p;
+}
 
 // Parts put together as they come: maximum and sum of weights, and the weighted sums of N columns
 template <int N>
@@ -1236,7 +1183,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs
     int b = -1;
     for (int b0 = 0; b0 < pb.B; b0 += 64) {
         const Sequence q = lane_sequence(a, b0);
-        const double u = Share(a, kRows, q).units;
+        const double u = share_of(a, kRows, q).units;
         const uint64_t hit = __ballot(b0 + lane < pb.B && row >= q.s0 && row < (int)((unsigned)q.s0 + (unsigned)q.n));
         all += u;
         some += b < 0 && (!hit || lane < __ffsll((unsigned long long)hit) - 1) ? u : 0.;
@@ -1256,7 +1203,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs
     all = wave_sum_f64(all);
     some = wave_sum_f64(some);
     if (too_much(all)) return;
-    const Parts in(a, s, kRows, h, tile, uniform((int)(unsigned)all), uniform((int)(unsigned)some));
+    const Parts in = parts_of(a, s, kRows, h, tile, uniform((int)(unsigned)all), uniform((int)(unsigned)some));
     const int parts = in.count;
     if (parts == 1) return;
     Joined<2> j;
@@ -1337,7 +1284,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_tiles_kernel(At
         const Sequence q = lane_sequence(a, b0);
         const int i = b0 + lane;
         if (!u.even) b += __popcll(__ballot(i < pb.B && u.begin(i + 1, (int)((unsigned)q.s0 + (unsigned)q.n)) <= number));
-        const double w = prompts ? BigShare(a, q).units(a) : Share(a, kRows, q).units;
+        const double w = prompts ? big_share_of(a, q).units(a.Hkv) : share_of(a, kRows, q).units;
         all += w;
         some += i < b ? w : 0.;                // (b grows only while all of these are before it)
         if (b >= b0 && b < b0 + 64) s = of_lane(q, b - b0);
@@ -1354,7 +1301,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_join_tiles_kernel(At
     all = wave_sum_f64(all);
     some = wave_sum_f64(some);
     if (too_much(all)) return;
-    const Parts in(a, s, kRows, h, tile, uniform((int)(unsigned)all), uniform((int)(unsigned)some));
+    const Parts in = parts_of(a, s, kRows, h, tile, uniform((int)(unsigned)all), uniform((int)(unsigned)some));
     if (in.count == 1) return;
     const float *part = prompts ? a.big_part : a.part, *stats = prompts ? a.big_stats : a.stats;
     constexpr int kAtOnce = 4;                 // parts at once, of two rows
@@ -1487,7 +1434,7 @@ CACTI_API int cacti_hip_paged_attention_f16(int64_t T, int64_t B, int64_t H, int
     float *part = (float *)workspace;
     const size_t small = (size_t)p.groups * 2 * (16 * p.NR);
     const AttnArgs a = {pb, (int)H, (int)Hkv, (int)(H / Hkv), (int)Dh, padded_dim((int)Dh), (int)(max_new < T ? max_new : T), p.groups,
-                        (unsigned)((1 << 22) / page + 1), fabsf(alpha), alpha < 0.f ? 0x80008000u : 0u, (const half_t *)q, ldq, k_pages, v_pages, (const float *)k_scale,
+                        magic_of(page), fabsf(alpha), alpha < 0.f ? 0x80008000u : 0u, (const half_t *)q, ldq, k_pages, v_pages, (const float *)k_scale,
                         (const float *)v_scale, (half_t *)out, ldo, part, part + small * Dh, p.few, p.big_groups,
                         part + small * (Dh + 2), part + small * (Dh + 2) + (size_t)p.big_groups * 2 * kPrompt * Dh};
     return bits == 8 ? launch<uint8_t>(a, p.NR, (hipStream_t)stream) : launch<half_t>(a, p.NR, (hipStream_t)stream);

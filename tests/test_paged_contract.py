@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 from cacti_amd import ffi
-from test_paged import APPEND, ATTEND, Batch, check_attention, numpy_of, same_bits
+from test_paged import APPEND, ATTEND, ATTENDS, Batch, check_attention, numpy_of, same_bits
 
 GPU = pytest.mark.gpu
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "cacti_amd", "csrc")
@@ -310,3 +310,37 @@ def test_attention_of_scales_at_the_ends(n, lens):
         else:
             B.ks[:], B.kp[:] = 2.0 ** 100, 0
         check_attention(B)
+
+
+# ---------------------------------------------------------------- tables without a page to spare
+def tight(B, r):
+    """B's table as wide as its longest sequence, no page's number where a sequence has no position."""
+    B.W = max(1, max(-(-l // B.page) for l in B.lens))
+    B.table = np.ascontiguousarray(B.table[:, :B.W])
+    for b, l in enumerate(B.lens):
+        B.table[b, -(-l // B.page):] = r.choice([-1, B.P, 2 ** 31 - 1, -2 ** 31])
+    return B
+
+
+@GPU
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("n,lens,H,Hkv,Dh,page", ATTENDS)
+def test_pages_that_are_not_a_sequences_are_not_looked_up(n, lens, H, Hkv, Dh, page, bits):
+    """(A number of the table that is no page's is named in status, and check_attention wants none.)"""
+    print("paged_attention", n, lens, H, Hkv, Dh, page, bits, flush=True)
+    r = np.random.default_rng(bits)
+    for more in (dict(), dict(max_new=max(n))):
+        check_attention(tight(Batch(sum(lens) + Dh + bits + 5, n, lens, H, Hkv, Dh, page, bits), r), **more)
+
+
+@GPU
+@pytest.mark.parametrize("seed", range(6))
+def test_pages_of_drawn_batches(seed):
+    r = np.random.default_rng(seed)
+    G = int(r.choice([1, 2, 3, 8]))
+    B = int(r.integers(1, 9))
+    n = [int(x) for x in r.integers(0, 180 if seed % 2 else 9, B)]
+    lens = [x + int(r.integers(0, 700)) for x in n]
+    Hkv, Dh, page, bits = int(r.choice([1, 2])), int(r.choice([20, 64, 100])), 16 * int(r.integers(1, 9)), 8 if seed % 3 else 16
+    print("paged_attention", n, lens, G * Hkv, Hkv, Dh, page, bits, flush=True)
+    check_attention(tight(Batch(seed, n, lens, G * Hkv, Hkv, Dh, page, bits, spare_rows=1), r))
