@@ -447,7 +447,8 @@ int cacti_hip_embed_bwd(int64_t V, int64_t D, int64_t S, const void *tok, const 
  * status [1] i32 on the device, or NULL: 1 + b where the numbers of sequence b do not fit together (rows beyond T, more new
  * rows than max_new or than positions, more positions than its row of the table or the rotation has, a page that is not in
  * the cache), raised with a maximum: the caller clears it.  Nothing of such a sequence is appended (with a page outside the
- * cache: nothing of that page), and its rows of the attention are zeros (with a page outside the cache: unspecified). */
+ * cache: nothing of that page) and its queries are left as they are; those of its rows that there are are zeros in the attention (with a
+ * page outside the cache: unspecified). */
 
 /* New keys and values into their pages, the keys rotated as by symplectic_embed (src/librarium/llama.rs:463-465; tables as
  * cacti_hip_rope_tables fills them, n_pos rows), and, where q is not NULL, q_rot = the queries rotated: in fp32, rounded once;
@@ -455,7 +456,8 @@ int cacti_hip_embed_bwd(int64_t V, int64_t D, int64_t S, const void *tok, const 
  * bits = 8: the scale of a page and head is the least 2^e, -32 <= e <= 15, with all finite new values of the page up to
  * 448 * 2^e, and no less than before where the page has older positions; their codes are carried over where it grew.  (Scales
  * are powers of two: the quotient and, but for subnormal codes, that are exact.)  NaN and infinities become NaN.  Slots behind
- * the new ones stay as they are. */
+ * the new ones stay as they are.  A length that goes back takes the positions behind it back, not the scale that they gave a page with
+ * older positions, nor what the older codes lost to it: that page keeps both until it is begun anew.  (In 16 bits nothing is left.) */
 int cacti_hip_paged_append(int64_t T, int64_t B, int64_t H, int64_t Hkv, int64_t Dh, int64_t max_new, const void *q, int64_t ldq,
                            const void *k, int64_t ldk, const void *v, int64_t ldv, const void *cos16, const void *sin16,
                            int64_t n_pos, void *q_rot, int64_t ldqr, void *k_pages, void *v_pages, void *k_scale, void *v_scale,

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 from cacti_amd import ffi
-from test_paged import APPEND, ATTEND, ATTENDS, Batch, check_attention, numpy_of, same_bits
+from test_paged import APPEND, ATTEND, ATTENDS, Batch, E4M3, check_append, check_attention, numpy_of, same_bits
 
 GPU = pytest.mark.gpu
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "cacti_amd", "csrc")
@@ -365,3 +365,32 @@ EXACT = [c + (bits,) for c in ATTENDS + [([1], [4000], 2, 2, 64, 32), ([6, 1], [
 def test_attention_divides_by_the_weights_as_they_were(n, lens, H, Hkv, Dh, page, bits):
     print("paged_attention", n, lens, H, Hkv, Dh, page, bits, flush=True)
     check_attention(Exact(sum(lens) + Dh + bits + 9, n, lens, H, Hkv, Dh, page, bits), max_new=max(n))
+
+
+# ---------------------------------------------------------------- drafted tokens that are taken back
+@GPU
+@pytest.mark.parametrize("slot", [5, 0])
+def test_a_large_draft_that_is_taken_back_leaves_its_page_the_scale(slot):
+    """In 8 bits a sequence's length takes back the positions of drafted tokens, not what they did to a page that has older ones: its
+    scale stays, and the older codes are those of the larger scale.  A page that begins with the drafted tokens is as if new."""
+    import torch
+    from cacti_amd import ops
+    first = 16 + slot
+    was = Batch(95, [3], [first + 3], 2, 2, 64, 16, 8)
+    was.qkv[2, 128:] = 3000                                   # the second drafted token
+    cache, drafted = check_append(was)
+    now = Batch(96, [2], [first + 2], 2, 2, 64, 16, 8)
+    now.table, now.W, now.P = was.table, was.W, was.P
+    now.kp, now.vp, now.ks, now.vs = drafted
+    _, want = now.append()
+    now.put()
+    ops.paged_append(now.d["k"], now.d["v"], cache, *now.at(), now.d["cos"], now.d["sin"])
+    for name, g, w in zip(("k pages", "v pages", "k scale", "v scale"), cache, want):
+        same_bits(numpy_of(g), w, name)
+    page = was.table[0, 1]
+    for before, after_draft, after in ((was.ks, drafted[2], want[2]), (was.vs, drafted[3], want[3])):
+        assert (after_draft[page] >= 4).all() and (before[page] < 0.1).all()
+        assert (after[page] == after_draft[page]).all() if slot else (after[page] < 0.1).all()
+    if slot:                                                  # older values, whose codes were up to 448 at a scale below 2^-4
+        old, new = E4M3[was.vp[page, :, :slot]] * was.vs[page][:, None, None], E4M3[want[1][page, :, :slot]] * want[3][page][:, None, None]
+        assert (np.abs(old - new) <= 2.0 ** -10 * want[3][page].max() + 2.0 ** -4 * np.abs(old)).all() and (old != new).any()
