@@ -7,9 +7,9 @@
 //
 // A workgroup to a row, which it holds in registers from one read on: the forward pass is bound by that read, the adjoint, which
 // takes the maximum and the sum from the forward pass (stats) and has nothing to reduce over the row, by a read and a write.
-// 2048 rows of 32000, K = 64: forward 29 us, 4.5 TB/s (a maximum and then a sum out of memory again: 44), adjoint 46.7 us,
-// 5.6 TB/s, and one after the other, when the forward pass has the gradients written before it go to memory beside it, 85.7;
-// 611 of 8191, K = 20: 6.9 and 8.1 us; 128 of 1024, K = 8: 4.0 and 3.3 us, latency.
+// 2048 rows of 32000, K = 64, each call after calls of its kind: forward 26 us, 5.0 TB/s (a maximum and then a sum out of memory again:
+// 44), adjoint 47 us, 5.6 TB/s, and one after the other, when the forward pass has the gradients written before it go to memory beside
+// it, 86; 611 of 8191, K = 20: 5.8 and 6.7 us; 128 of 1024, K = 8: 4.2 and 3.9 us, latency.
 #include "operands.h"
 #include "vocab_row.h"
 
@@ -280,8 +280,8 @@ __global__ void __launch_bounds__(T) distill_bwd_kernel(DistillArgs a)
         if (mine[e]) gr[t.j[e]] = entry[e];
 }
 
-// The least threads and registers that hold a row.  (Forward and adjoint, 611 rows of 8191: 256 threads 5.9 and 8.8 us, 512 8.0 and
-// 9.4; 2048 of 32000: 256 26.8 and 55.1, 512 27.3 and 50.5, 1024 33.5 and 57.7)
+// The least threads and registers that hold a row.  (Forward and adjoint, 611 rows of 8191: 256 threads 5.8 and 6.7 us, 512 6.6 and
+// 7.3; 2048 of 32000: 256 25.9 and 48.8, 512 26.1 and 47.0, 1024 32.6 and 58.6)
 #define CACTI_DISTILL(kernel, a, st)                                                                                                  \
     do {                                                                                                                              \
         const dim3 grid((unsigned)(a).N);                                                                                             \

@@ -9,8 +9,8 @@
 // A workgroup owns a page and a head: it holds the new rows of that page in registers, takes the least scale that holds them and
 // no less than that of older rows, codes those again where it grew, and writes.  No other workgroup touches that page and head.
 // Bound by memory: four sequences of up to 2048 rows, 32 heads of 100 in 8 bits 38 to 40 us, of which 18 are the queries' (reading the
-// rows once for the scale and again for the codes, two columns at a time: 56.4); 96 of up to 6 rows, 8 heads of 128: 5.4 us; one
-// row 4.0 us, latency.
+// rows once for the scale and again for the codes, two columns at a time: 56.4), in 16 bits 53; 96 of up to 6 rows, 8 heads of 128: 5.4 us;
+// one row 4.2 us, latency.
 #include "operands.h"
 #include "paged.h"
 

@@ -19,7 +19,8 @@
 // operand is a column of eight keys, is read as rows of 8 columns and turned with byte permutes.  LDS has the pages' numbers and
 // no operand, and nobody waits on the way; the keys after these are requested once these have been multiplied, the values likewise,
 // into the same registers.  48 sequences of 120 to 8192 positions, 32 heads of 100 in 8 bits, which memory bounds: 129 us, 24 of 100 to
-// 6000 with up to 6 rows of 32 / 8 heads of 128, vector operations as much as memory: 27.4 us; one of 1540, latency: 12.3 us.
+// 6000 with up to 6 rows of 32 / 8 heads of 128, vector operations as much as memory: 27.5 us; one of 1540, latency: 12.3 us; the first
+// two in 16 bits, which memory bounds: 236 and 41.7 us.
 //
 // Work: the lengths are on the device and as different as they come, so every workgroup of a launch that just fills the device
 // forms their sum in steps of 32 positions and takes an equal, contiguous share of it, across rows, heads and sequences, each of
@@ -719,7 +720,8 @@ __global__ void __launch_bounds__(kThreads, resident(ND, NR, sizeof(P))) paged_a
 // see to the keys, two to the values), while the products of the 64 before them run, in two buffers with one barrier a step.
 // 16-byte pieces of LDS rows are swapped by f(row), which spreads the sixteen rows of an operand, and the rows that a wave writes,
 // evenly over the banks.  (16 rows to each of eight waves read the operands twice as often and have half the registers: 88.6
-// against 83 us for three sequences of up to 900 rows and 4000 positions, 16 heads of 128.)
+// against 83 us for three sequences of up to 900 rows and 4000 positions, 16 heads of 128, which are 71.5 us now, in 8 bits 73; one of 900
+// and 24 single tokens of 1000 to 4000 in 8 bits 99, 39 of them the prompt's launch and 46 the tokens' behind it.)
 //
 // Shares are cut as above, a workgroup to a share and by steps of 64.  Workgroups of an XCD have neighbouring shares: the tiles of a
 // head read its keys and values from one L2.

@@ -10,13 +10,15 @@
 //
 // Exponentials and sums are fp64: what is drawn goes by on which side of a border of the running sum r lies, and with sums that
 // are off by e of their total some V e of all draws come out differently (32000 tokens, fp32 sums: one in several hundred).
-// That arithmetic, some 17 operations of 64 bits a logit, is what bounds a batch (twice the time that its bytes take).
+// That arithmetic, some 17 operations of 64 bits a logit, bounds the first launch (twice the time that its bytes take), which is half of a
+// batch; the other half is the latency of the two launches behind it.
 //
 // Three launches, each as wide as its work.  A row is cut into entries of 2048 logits, one to a wave, which needs no barrier and
 // spreads five rows over 20 workgroups: their maxima and sums relative to them, of every row of both models.  Then workgroups of
 // each sequence form the rows' sums from them, see which drafted tokens are kept and sum what is left of p in the first row whose
 // token is not, 512 logits to a wave.  Then a workgroup of each sequence finds the entry in which r lies and the token in it.
-// us, five rows of 32000 with a drafting model / 64 sequences, 294 rows: 15.9 / 33.9, of which the first launch is 4 / 18; a
+// us, five rows of 32000 with a drafting model / 64 sequences, 310 rows: 16.7 / 33.3, of which the first launch is 4 / 18; the same batch
+// without the drafting model's logits 23.4, greedy (two launches) 9.9.  A
 // workgroup per row that drew for every row that might end its sequence 77 / 115, one per sequence for the last two steps 22.5 / 38.6;
 // the last step by the last of a sequence's workgroups to write, which takes fences between the XCDs, 18.1 / 116.
 #include "operands.h"
