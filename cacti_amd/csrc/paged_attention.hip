@@ -1166,7 +1166,8 @@ struct Joined {
 };
 
 // The parts of a row put together, two columns per lane, by a wave or, for few rows, a workgroup of four waves; zeros for rows whose
-// sequence's numbers do not fit together, which the last workgroup names.  Bound by latency: eight parts are requested at once, their sums with their values.
+// sequence's numbers do not fit together, which the last workgroup names.  Bound by latency: eight parts are requested at once, their
+// sums with their values.
 template <int NR, int WAVES>
 __global__ void __launch_bounds__(kThreads) paged_attention_join_kernel(AttnArgs a)
 {
