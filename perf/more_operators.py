@@ -501,8 +501,8 @@ def _plain_compact(refs, table):
     to = torch.arange(P + 1, device="cuda", dtype=I32)
     to.scatter_(0, torch.where(moves, src, P).long(), dst)
     table.copy_(torch.where(table >= 0, to[table.clamp(min=0).long()], table))
-    refs.copy_(torch.where(at < count, torch.where(holes, refs.scatter(0, torch.where(moves, dst, 0).long(),
-               torch.where(moves, refs[src.clamp(min=0).long()], refs[0])), refs), 0))
+    moved = torch.cat([refs, refs[:1]]).scatter_(0, torch.where(moves, dst, P).long(), refs[src.clamp(min=0).long()])[:P]
+    refs.copy_(torch.where(at < count, moved, 0))
     return src, dst, count.to(I32).view(1)
 
 
