@@ -1,0 +1,413 @@
+// Pages of a cache handed out, shared, copied and packed, with all numbers on the device.  refs [P] counts who holds a page, a row of
+// the table has a sequence's pages in order and -1 behind them.
+//
+//   fork     sequence b goes on as sequence parent[b]: its row becomes that one's, up to the pages that its positions take
+//   fit      each sequence gets what its positions need: pages behind them go back, missing ones are the lowest free ones, in the
+//            order of sequences and positions, and a page that is going to be written on by others too is copied first
+//   compact  the held pages to the lowest places
+//   copy     the pages that the other two say, of all layers' caches in one launch
+//
+// Fork is a launch over rows, whose counts are sums of whole numbers, in any order the same.  Fit and the scan of compact are one
+// workgroup: what is free depends on everything that is given back, and a barrier costs less there than a launch (a batch's table and
+// counts are some ten kilobytes).  Copying is bound by memory.
+#include "common.h"
+
+using namespace cacti;
+
+namespace {
+
+__device__ __forceinline__ int load_now(const int *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ void store_now(int *p, int v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+// A barrier behind which the workgroup's counts in memory are what it made them: they are written and read past the first cache, in
+// an order that the barrier alone does not promise.
+__device__ __forceinline__ void settled()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_s_waitcnt(0x0f70);        // vmcnt(0)
+    __syncthreads();
+}
+__device__ __forceinline__ void name(int *status, int b)
+{
+    if (status) atomicMax(status, b + 1);
+}
+__device__ __forceinline__ bool fits(int len, int W, int page) { return len >= 0 && len <= W * page; }
+
+// ---------------------------------------------------------------- fork
+struct ForkArgs {
+    int P, B, W, page;
+    int64_t ldt, ldn;
+    int *refs;
+    const int *table, *lens, *parent;
+    int *new_table, *new_lens, *status;
+};
+
+// A workgroup to a sequence
+__global__ void __launch_bounds__(256) fork_kernel(ForkArgs a)
+{
+    const int b = blockIdx.x;
+    int p = a.parent[b], need = 0, len = 0;
+    bool stays = p < -1 || p >= a.B;
+    if (!stays && p >= 0) {
+        len = a.lens[p];
+        stays = !fits(len, a.W, a.page);
+        need = (len + a.page - 1) / a.page;
+    }
+    if (stays) {                               // what cannot be: left as it is
+        if (threadIdx.x == 0) name(a.status, b);
+        p = b;
+        len = a.lens[b];
+        need = a.W;
+    }
+    const int *was = a.table + b * a.ldt, *from = a.table + max(p, 0) * a.ldt;
+    int *to = a.new_table + b * a.ldn;
+    for (int j = threadIdx.x; j < a.W; j += 256) {
+        const int x = was[j], y = j < need ? from[j] : -1;
+        to[j] = y;
+        if (x == y) continue;
+        if (x >= 0 && x < a.P) atomicSub(a.refs + x, 1);
+        if (y >= 0 && y < a.P) atomicAdd(a.refs + y, 1);
+    }
+    if (threadIdx.x == 0) a.new_lens[b] = len;
+}
+
+// ---------------------------------------------------------------- fit
+struct FitArgs {
+    int P, B, W, page;
+    int64_t ldt;
+    int *refs, *table;
+    const int *first, *lens;
+    int *src, *dst, *slots;
+    int *asked, *free;                         // workspace: [B] pages that each sequence asks for, [P] free ones in order
+    int *status;
+};
+
+constexpr int kThreads = 1024, kWaves = kThreads / 64;
+
+// the sum over the threads before this one, and of all
+__device__ __forceinline__ int scan(int v, int *total, int *red)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int s = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(s, o);
+        if (lane >= o) s += x;
+    }
+    __syncthreads();
+    if (lane == 63) red[wave] = s;
+    __syncthreads();
+    int before = 0, sum = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) {
+        const int x = red[w];
+        before += w < wave ? x : 0;
+        sum += x;
+    }
+    *total = sum;
+    return before + s - v;
+}
+
+// A sequence's entries that it lets go of, first .. , of which those below need are wanted again; part: slots of the first one
+// that are to be kept
+struct Span {
+    int begin, need, part;
+    bool ok;
+};
+__device__ __forceinline__ Span span(const FitArgs &a, int b)
+{
+    const int f = a.first[b], l = a.lens[b];
+    Span s = {0, 0, 0, fits(l, a.W, a.page) && f >= 0 && f <= l};
+    if (!s.ok) return s;
+    s.need = (l + a.page - 1) / a.page;
+    s.begin = l > f ? f / a.page : s.need;
+    s.part = l > f ? f % a.page : 0;
+    return s;
+}
+
+// A wave to a sequence, 64 entries at a time
+__global__ void __launch_bounds__(kThreads) fit_kernel(FitArgs a)
+{
+    __shared__ int red[kWaves];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // all that is written on or not needed is let go of
+    for (int b = wave; b < a.B; b += kWaves) {
+        const Span s = span(a, b);
+        if (!s.ok) {
+            if (lane == 0) name(a.status, b);
+            continue;
+        }
+        for (int j = s.begin + lane; j < a.W; j += 64) {
+            const int x = a.table[b * a.ldt + j];
+            if (x >= 0 && x < a.P) atomicSub(a.refs + x, 1);
+        }
+    }
+    settled();
+    // a page that no one keeps goes to the first of those who want it again: b - B, below all counts
+    for (int b = wave; b < a.B; b += kWaves) {
+        const Span s = span(a, b);
+        for (int j = s.begin + lane; j < s.need; j += 64) {
+            const int x = a.table[b * a.ldt + j];
+            if (x >= 0 && x < a.P && load_now(a.refs + x) <= 0) atomicMin(a.refs + x, b - a.B);
+        }
+    }
+    settled();
+    // who has none of its own asks for one: marked in the table as -2 - the page that is to be copied, or as -1
+    for (int b = wave; b < a.B; b += kWaves) {
+        const Span s = span(a, b);
+        int count = 0;
+        if (lane == 0) a.src[b] = a.dst[b] = -1, a.slots[b] = 0;
+        if (s.ok)
+            for (int j0 = s.begin; j0 < a.W; j0 += 64) {
+                const int j = j0 + lane;
+                bool asks = false;
+                if (j < a.W) {
+                    int *e = a.table + b * a.ldt + j;
+                    const int x = *e;
+                    if (j < s.need) asks = !(x >= 0 && x < a.P && load_now(a.refs + x) == b - a.B);
+                    if (asks && s.part && j == s.begin && x >= 0 && x < a.P) a.src[b] = x;
+                    if (asks || j >= s.need) *e = -1;
+                }
+                count += __popcll(__ballot(asks));
+            }
+        if (lane == 0) a.asked[b] = count;
+    }
+    settled();
+    for (int b = wave; b < a.B; b += kWaves) {
+        const Span s = span(a, b);
+        for (int j = s.begin + lane; j < s.need; j += 64) {
+            const int x = a.table[b * a.ldt + j];
+            if (x >= 0) store_now(a.refs + x, 1);
+        }
+    }
+    // how many are asked for before each sequence
+    int all = 0;
+    for (int b0 = 0; b0 < a.B; b0 += kThreads) {
+        const int b = b0 + (int)threadIdx.x;
+        int total;
+        const int before = scan(b < a.B ? a.asked[b] : 0, &total, red);
+        if (b < a.B) a.asked[b] = all + before;
+        all += total;
+    }
+    settled();
+    // the lowest free pages, as many as are asked for
+    int found = 0;
+    for (int p0 = 0; p0 < a.P && found < all; p0 += 4 * kThreads) {
+        const int p = p0 + 4 * (int)threadIdx.x;
+        int is[4], n = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) n += is[k] = p + k < a.P && load_now(a.refs + p + k) == 0;
+        int total, at = found + scan(n, &total, red);
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (is[k]) a.free[at++] = p + k;
+        found += total;
+    }
+    settled();
+    // .. handed out
+    for (int b = wave; b < a.B; b += kWaves) {
+        const Span s = span(a, b);
+        int at = a.asked[b];
+        for (int j0 = s.begin; j0 < s.need; j0 += 64) {
+            const int j = j0 + lane;
+            int *e = a.table + b * a.ldt + j;
+            const bool asks = j < s.need && *e == -1;
+            const uint64_t mask = __ballot(asks);
+            const int k = at + __popcll(mask & ((1ull << lane) - 1));
+            const bool got = asks && k < found;
+            if (got) {
+                const int x = a.free[k];
+                *e = x;
+                store_now(a.refs + x, 1);
+                if (s.part && j == s.begin && a.src[b] >= 0) a.dst[b] = x, a.slots[b] = s.part;
+            } else if (asks) {
+                name(a.status, b);
+                if (s.part && j == s.begin) a.src[b] = -1;
+            }
+            at += __popcll(mask);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- compact
+struct CompactArgs {
+    int P, B, W;
+    int64_t ldt;
+    int *refs, *table, *src, *dst, *used;
+    int *to;                                   // workspace [P]: where a page goes that moves
+};
+
+__global__ void __launch_bounds__(kThreads) compact_kernel(CompactArgs a)
+{
+    __shared__ int red[kWaves];
+    int mine = 0, used;
+    for (int p = threadIdx.x; p < a.P; p += kThreads) mine += a.refs[p] > 0;
+    scan(mine, &used, red);
+    if (threadIdx.x == 0) *a.used = used;
+    const int half = a.P / 2;
+    for (int i = threadIdx.x; i < half; i += kThreads) a.src[i] = a.dst[i] = -1;
+    __syncthreads();
+    // free places below `used` and held pages from there on: as many of the one as of the other
+    int moves = 0;
+    for (int side = 0; side < 2; side++) {
+        const int end = side ? a.P : used;
+        int n = 0;
+        for (int p0 = side ? used : 0; p0 < end; p0 += kThreads) {
+            const int p = p0 + (int)threadIdx.x;
+            const bool is = p < end && (a.refs[p] > 0) == (side == 1);
+            int total;
+            const int at = n + scan(is, &total, red);
+            if (is) (side ? a.src : a.dst)[at] = p;
+            if (side && p < end && !is) a.to[p] = p;
+            n += total;
+        }
+        moves = n;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < moves; i += kThreads) {
+        const int s = a.src[i], d = a.dst[i];
+        a.refs[d] = a.refs[s];
+        a.refs[s] = 0;
+        a.to[s] = d;
+    }
+}
+
+__global__ void __launch_bounds__(256) renumber_kernel(CompactArgs a)
+{
+    const int used = *a.used;
+    int *row = a.table + blockIdx.x * a.ldt;
+    for (int j = threadIdx.x; j < a.W; j += 256) {
+        const int x = row[j];
+        if (x >= used && x < a.P) row[j] = a.to[x];
+    }
+}
+
+// ---------------------------------------------------------------- copy
+constexpr int kLayers = 32;
+struct CopyArgs {
+    char *k[kLayers], *v[kLayers];
+    float *ks[kLayers], *vs[kLayers];
+    const int *src, *dst, *slots;
+    int64_t n, P, items;
+    int layers, heads, page, slot_bytes;       // of a position of a head
+};
+
+// An item: the keys or the values of a page of a layer
+__global__ void __launch_bounds__(256) copy_kernel(CopyArgs a)
+{
+    for (int64_t i = blockIdx.x; i < a.items; i += gridDim.x) {
+        const int64_t which = i / (2 * a.layers);
+        const int of = (int)(i % (2 * a.layers)), layer = of >> 1;
+        const int64_t s = a.src[which], d = a.dst[which];
+        if (s < 0 || d < 0 || s >= a.P || d >= a.P || s == d) continue;
+        const int slots = a.slots ? min(max(a.slots[which], 0), a.page) : a.page;
+        char *pages = of & 1 ? a.v[layer] : a.k[layer];
+        float *scales = of & 1 ? a.vs[layer] : a.ks[layer];
+        const int64_t head = (int64_t)a.page * a.slot_bytes, bytes = head * a.heads;
+        const int pieces = slots * a.slot_bytes / 16;
+        for (int e = threadIdx.x; e < a.heads * pieces; e += 256) {
+            const int64_t at = (e / pieces) * head + 16 * (e % pieces);
+            *reinterpret_cast<uint4 *>(pages + d * bytes + at) = *reinterpret_cast<const uint4 *>(pages + s * bytes + at);
+        }
+        if (scales && slots)
+            for (int h = threadIdx.x; h < a.heads; h += 256) scales[d * a.heads + h] = scales[s * a.heads + h];
+    }
+}
+
+int check(const char *who, int64_t P, int64_t B, int64_t W, int64_t page, const void *refs, const void *table, int64_t ldt, const void *status)
+{
+    CACTI_REQUIRE(P > 0 && B > 0 && W > 0 && page > 0, CACTI_E_INVALID, "%s: empty shape", who);
+    CACTI_REQUIRE(refs && table, CACTI_E_INVALID, "%s: null pointer", who);
+    CACTI_REQUIRE(P <= (1 << 28) && B <= (1 << 20) && W <= (1 << 30) / page && ldt >= W, CACTI_E_NOTIMPL,
+                  "%s: too many pages or sequences, or a table pitch below its width", who);
+    CACTI_REQUIRE(aligned(refs, 4) && aligned(table, 4) && aligned(status, 4), CACTI_E_INVALID, "%s: misaligned operand", who);
+    return 0;
+}
+
+}  // namespace
+
+CACTI_API int cacti_hip_paged_fork(int64_t P, int64_t B, int64_t W, int64_t page, void *refs, const void *table, int64_t ldt, const void *lens,
+                                   const void *parent, void *new_table, int64_t ldn, void *new_lens, void *status, void *stream)
+{
+    const int rc = check("paged_fork", P, B, W, page, refs, table, ldt, status);
+    if (rc) return rc;
+    CACTI_REQUIRE(lens && parent && new_table && new_lens, CACTI_E_INVALID, "paged_fork: null pointer");
+    CACTI_REQUIRE(aligned(lens, 4) && aligned(parent, 4) && aligned(new_table, 4) && aligned(new_lens, 4), CACTI_E_INVALID, "paged_fork: misaligned operand");
+    CACTI_REQUIRE(ldn >= W, CACTI_E_INVALID, "paged_fork: a table pitch below its width");
+    const char *t = (const char *)table, *n = (const char *)new_table, *l = (const char *)lens, *m = (const char *)new_lens;
+    CACTI_REQUIRE(n >= t + 4 * ((B - 1) * ldt + W) || t >= n + 4 * ((B - 1) * ldn + W), CACTI_E_INVALID, "paged_fork: the new table shares memory with the old one");
+    CACTI_REQUIRE(m >= l + 4 * B || l >= m + 4 * B, CACTI_E_INVALID, "paged_fork: the new lengths share memory with the old ones");
+    const ForkArgs a = {(int)P, (int)B, (int)W, (int)page, ldt, ldn, (int *)refs, (const int *)table, (const int *)lens, (const int *)parent,
+                        (int *)new_table, (int *)new_lens, (int *)status};
+    hipLaunchKernelGGL(fork_kernel, dim3((unsigned)B), dim3(256), 0, (hipStream_t)stream, a);
+    return launch_status("paged_fork");
+}
+
+CACTI_API size_t cacti_hip_paged_fit_workspace(int64_t P, int64_t B) { return P > 0 && B > 0 ? (size_t)(P + B) * 4 : 0; }
+
+CACTI_API int cacti_hip_paged_fit(int64_t P, int64_t B, int64_t W, int64_t page, void *refs, void *table, int64_t ldt, const void *first,
+                                  const void *lens, void *src, void *dst, void *slots, void *workspace, size_t workspace_bytes, void *status,
+                                  void *stream)
+{
+    const int rc = check("paged_fit", P, B, W, page, refs, table, ldt, status);
+    if (rc) return rc;
+    CACTI_REQUIRE(first && lens && src && dst && slots && workspace, CACTI_E_INVALID, "paged_fit: null pointer");
+    CACTI_REQUIRE(aligned(first, 4) && aligned(lens, 4) && aligned(src, 4) && aligned(dst, 4) && aligned(slots, 4) && aligned(workspace, 4), CACTI_E_INVALID,
+                  "paged_fit: misaligned operand");
+    CACTI_REQUIRE(workspace_bytes >= cacti_hip_paged_fit_workspace(P, B), CACTI_E_INVALID, "paged_fit: workspace of %zu bytes, %zu needed", workspace_bytes,
+                  cacti_hip_paged_fit_workspace(P, B));
+    const FitArgs a = {(int)P, (int)B, (int)W, (int)page, ldt, (int *)refs, (int *)table, (const int *)first, (const int *)lens, (int *)src, (int *)dst,
+                       (int *)slots, (int *)workspace, (int *)workspace + B, (int *)status};
+    hipLaunchKernelGGL(fit_kernel, dim3(1), dim3(kThreads), 0, (hipStream_t)stream, a);
+    return launch_status("paged_fit");
+}
+
+CACTI_API size_t cacti_hip_paged_compact_workspace(int64_t P) { return P > 0 ? (size_t)P * 4 : 0; }
+
+CACTI_API int cacti_hip_paged_compact(int64_t P, int64_t B, int64_t W, void *refs, void *table, int64_t ldt, void *src, void *dst, void *used,
+                                      void *workspace, size_t workspace_bytes, void *stream)
+{
+    const int rc = check("paged_compact", P, B, W, 1, refs, table, ldt, nullptr);
+    if (rc) return rc;
+    CACTI_REQUIRE(((src && dst) || P < 2) && used && workspace, CACTI_E_INVALID, "paged_compact: null pointer");
+    CACTI_REQUIRE(aligned(src, 4) && aligned(dst, 4) && aligned(used, 4) && aligned(workspace, 4), CACTI_E_INVALID, "paged_compact: misaligned operand");
+    CACTI_REQUIRE(workspace_bytes >= cacti_hip_paged_compact_workspace(P), CACTI_E_INVALID, "paged_compact: workspace of %zu bytes, %zu needed",
+                  workspace_bytes, cacti_hip_paged_compact_workspace(P));
+    const CompactArgs a = {(int)P, (int)B, (int)W, ldt, (int *)refs, (int *)table, (int *)src, (int *)dst, (int *)used, (int *)workspace};
+    hipLaunchKernelGGL(compact_kernel, dim3(1), dim3(kThreads), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(renumber_kernel, dim3((unsigned)B), dim3(256), 0, (hipStream_t)stream, a);
+    return launch_status("paged_compact");
+}
+
+CACTI_API int cacti_hip_paged_copy(int64_t layers, void *const *k_pages, void *const *v_pages, void *const *k_scale, void *const *v_scale, int bits,
+                                   int64_t P, int64_t Hkv, int64_t page, int64_t Dh, int64_t n, const void *src, const void *dst, const void *slots,
+                                   void *stream)
+{
+    CACTI_REQUIRE(layers >= 0 && P > 0 && Hkv > 0 && page > 0 && Dh > 0 && n >= 0, CACTI_E_INVALID, "paged_copy: empty shape");
+    CACTI_REQUIRE(bits == 8 || bits == 16, CACTI_E_INVALID, "paged_copy: pages of 8 or 16 bits");
+    CACTI_REQUIRE(Dh <= 4096 && page <= 4096 && Hkv <= 4096 && P <= (1 << 28) && n <= (1 << 28) && layers <= (1 << 16), CACTI_E_NOTIMPL,
+                  "paged_copy: pages too large or too many");
+    CACTI_REQUIRE(Hkv * page * ((Dh + 15) / 16 * 16) * (bits / 8) <= (1 << 30), CACTI_E_NOTIMPL, "paged_copy: pages too large or too many");
+    if (layers == 0 || n == 0) return 0;
+    CACTI_REQUIRE(k_pages && v_pages && src && dst && (bits == 16 || (k_scale && v_scale)), CACTI_E_INVALID, "paged_copy: null pointer");
+    CACTI_REQUIRE(aligned(src, 4) && aligned(dst, 4) && aligned(slots, 4), CACTI_E_INVALID, "paged_copy: misaligned operand");
+    for (int64_t l = 0; l < layers; l++) {
+        CACTI_REQUIRE(k_pages[l] && v_pages[l] && aligned(k_pages[l], 16) && aligned(v_pages[l], 16), CACTI_E_INVALID,
+                      "paged_copy: pages null or not 16-byte aligned");
+        CACTI_REQUIRE(bits == 16 || (k_scale[l] && v_scale[l] && aligned(k_scale[l], 4) && aligned(v_scale[l], 4)), CACTI_E_INVALID,
+                      "paged_copy: pages of 8 bits have scales");
+    }
+    for (int64_t l0 = 0; l0 < layers; l0 += kLayers) {
+        CopyArgs a{};
+        a.layers = (int)(layers - l0 < kLayers ? layers - l0 : kLayers);
+        for (int l = 0; l < a.layers; l++) {
+            a.k[l] = (char *)k_pages[l0 + l], a.v[l] = (char *)v_pages[l0 + l];
+            if (bits == 8) a.ks[l] = (float *)k_scale[l0 + l], a.vs[l] = (float *)v_scale[l0 + l];
+        }
+        a.src = (const int *)src, a.dst = (const int *)dst, a.slots = (const int *)slots;
+        a.n = n, a.P = P, a.items = n * 2 * a.layers;
+        a.heads = (int)Hkv, a.page = (int)page, a.slot_bytes = (int)((Dh + 15) / 16 * 16 * bits / 8);
+        const int64_t blocks = a.items < 2048 ? a.items : 2048;
+        hipLaunchKernelGGL(copy_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
+    }
+    return launch_status("paged_copy");
+}

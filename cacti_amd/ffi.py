@@ -124,6 +124,19 @@ SIGNATURES = {
     "cacti_hip_verify_draft_f16": (ci, [i64, i64, i64, vp, i64, vp, i64, vp, vp, vp, vp, C.c_double, vp, vp, vp, sz, vp, vp]),
     "cacti_hip_distill_topk_fwd": (ci, [i64, i64, i64, vp, i64, vp, vp, C.c_double, vp, vp, vp, vp]),
     "cacti_hip_distill_topk_bwd": (ci, [i64, i64, i64, vp, i64, vp, vp, vp, vp, C.c_double, vp, i64, ci, vp]),
+    "cacti_hip_token_logp_fwd": (ci, [i64, i64, vp, i64, vp, vp, C.c_double, vp, vp, vp, vp]),
+    "cacti_hip_token_logp_bwd": (ci, [i64, i64, vp, i64, vp, vp, vp, C.c_double, vp, i64, ci, vp]),
+    "cacti_hip_policy_loss": (ci, [i64, i64, vp, i64] + [vp] * 6 + [C.c_double] * 4 + [vp, vp, vp, i64, ci, vp, vp]),
+    "cacti_hip_preference_loss": (ci, [i64, i64] + [vp] * 5 + [C.c_double, C.c_double, ci, vp, vp, vp, vp, vp]),
+    "cacti_hip_adapter_fwd": (ci, [i64] * 7 + [vp, i64] + [vp] * 6 + [i64, vp, i64, vp, vp, vp]),
+    "cacti_hip_adapter_bwd_workspace": (sz, [i64] * 5),
+    "cacti_hip_adapter_bwd": (ci, [i64] * 7 + [vp, i64] + [vp] * 7 + [i64, vp, i64, ci, vp, ci, vp, ci, vp, sz, vp, vp]),
+    "cacti_hip_paged_fork": (ci, [i64] * 4 + [vp, vp, i64, vp, vp, vp, i64, vp, vp, vp]),
+    "cacti_hip_paged_fit_workspace": (sz, [i64, i64]),
+    "cacti_hip_paged_fit": (ci, [i64] * 4 + [vp, vp, i64] + [vp] * 6 + [sz, vp, vp]),
+    "cacti_hip_paged_compact_workspace": (sz, [i64]),
+    "cacti_hip_paged_compact": (ci, [i64] * 3 + [vp, vp, i64, vp, vp, vp, vp, sz, vp]),
+    "cacti_hip_paged_copy": (ci, [i64] + [vp] * 4 + [ci] + [i64] * 5 + [vp] * 4),
     "cacti_hip_append_token_u16": (ci, [vp, i64, vp, i64, vp]),
     "cacti_hip_raw_cast_bf16_f16": (ci, [i64, vp, vp, vp]),
     "cacti_hip_raw_cast_bf16_f32": (ci, [i64, vp, vp, vp]),

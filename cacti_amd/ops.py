@@ -286,6 +286,81 @@ def distill_topk_bwd(logit, idx, val, stats, scale, temperature=1.0, acc=None):
     return _op.distill_topk_bwd(logit, idx, val, stats, scale, temperature, acc)
 
 
+# ---------------------------------------------------------------- tuning by answers: drawn tokens, adapters, several answers in one cache
+def token_logp_fwd(logit, tok, temperature=1.0, mask=None, status=None):
+    """Log-probabilities of drawn tokens: (log softmax(logit / temperature)[tok] f32 [N], stats f32 [N, 2] for the adjoint).
+
+    logit f16 [N, V], rows may be strided; tok u16-as-int16 [N]; mask bool [N]: rows where it is False have 0 and are not read."""
+    return _op.token_logp_fwd(logit, tok, temperature, mask, status)
+
+
+def token_logp_bwd(logit, tok, stats, dlogp, temperature=1.0, acc=None):
+    """Their gradient times dlogp f32 [N] with respect to logit, f16 (added to acc where given).  A row with dlogp 0 has gradient 0
+    and is not read."""
+    return _op.token_logp_bwd(logit, tok, stats, dlogp, temperature, acc)
+
+
+def policy_loss(logit, tok, old, adv, scale, ref=None, mask=None, clip=(0.2, 0.2), beta=0.0, temperature=1.0, acc=None, status=None):
+    """Clipped policy loss of drawn tokens: (loss f32 [N], their log-probabilities f32 [N], scale times its gradient with respect to
+    logit f16), in one pass over the logits.
+
+    With r = exp(logp - old) and d = ref - logp the loss of a row is -min(r adv, clip(r, 1 - clip[0], 1 + clip[1]) adv)
+    + beta (exp(d) - d - 1), the last term where ref is given.  old, adv, scale, ref: f32 [N]; mask as in token_logp_fwd."""
+    return _op.policy_loss(logit, tok, old, adv, scale, ref, mask, clip[0], clip[1], beta, temperature, acc, status)
+
+
+def preference_loss(logp, ref, starts, scale, beta=0.1, smoothing=0.0, mask=None, mean=False, status=None):
+    """Loss over pairs of texts of which the first is preferred: (loss f32 [pairs], rewards f32 [2 pairs], scale times its gradient with
+    respect to logp f32 [N]).
+
+    Rows starts[t] .. starts[t+1]-1 (int32 [2 pairs + 1] on the GPU) are text t, texts 2 i and 2 i + 1 pair i.  A text's reward is beta times
+    the sum (mean: the mean) of logp - ref over its rows where mask is True, the loss -log sigmoid of the rewards' difference, with
+    smoothing a share of that of its opposite.  ref f32 [N] or None; scale f32 [pairs]."""
+    return _op.preference_loss(logp, ref, starts, scale, beta, smoothing, mask, mean, status)
+
+
+def adapter_fwd(x, A, B, starts, ids, scale, base=None, out=None, max_new=None, status=None):
+    """Low-rank adapters of many requests beside a shared projection: (y, h) with h = x A[a]^T f32 [T, R] and
+    y = base + scale[a] h B[a]^T f16 [T, N] (into out where given, which may be base).
+
+    Rows starts[s] .. starts[s+1]-1 of x f16 [T, K] are those of sequence s, whose adapter is a = ids[s] (-1: none, y = base): int32 tensors
+    on the GPU that the host does not read.  A f16 [adapters, R, K], B f16 [adapters, N, R], scale f32 [adapters]; K, N, R multiples of 8,
+    R <= 128.  Rows of x, base and out may be strided by multiples of 8.  max_new: no sequence has more rows than that.  status: a
+    cleared int32 tensor of one element that becomes 1 + s where the numbers of sequence s do not fit."""
+    return _op.adapter_fwd(x, A, B, starts, ids, scale, base, out, max_new, status)
+
+
+def adapter_bwd(x, A, B, starts, ids, scale, h, dy, dx_acc=None, dA_acc=None, dB_acc=None, max_new=None, status=None):
+    """Its adjoint: (dx, dA, dB), f16.  h: what adapter_fwd returned; *_acc: tensors to add to, in place."""
+    return _op.adapter_bwd(x, A, B, starts, ids, scale, h, dy, dx_acc, dA_acc, dB_acc, max_new, status)
+
+
+def paged_fork(refs, table, lens, parent, page, out=None, status=None):
+    """Sequences of a paged cache go on as others: (table, lens) in which sequence b has the pages and the length of parent[b] (b itself: as
+    it is; -1: empty).  refs [pages], who holds each page, is brought up to date.  Nothing is copied: paged_fit does what is needed
+    before the next append.  All int32 tensors on the GPU; out = (table, lens) to write to, other memory than the old ones."""
+    return _op.paged_fork(refs, table, lens, parent, page, out, status)
+
+
+def paged_fit(refs, table, first, lens, page, status=None):
+    """Gives each sequence the pages that lens[b] positions need, of which the first first[b] are there and the others will be written;
+    pages behind them go back, and a page that others hold too is not written on.  refs and table are changed in place; returns (src, dst,
+    slots) for paged_copy, which comes before the append.  lens 0 frees a sequence.  status becomes 1 + b where there was no page."""
+    return _op.paged_fit(refs, table, first, lens, page, status)
+
+
+def paged_compact(refs, table):
+    """The pages that are held to the lowest places, in place: (src, dst, used) with the moves for paged_copy and the number of held pages
+    (int32 [1])."""
+    return _op.paged_compact(refs, table)
+
+
+def paged_copy(caches, src, dst, slots=None):
+    """Copies page src[i] to page dst[i] (its first slots[i] positions), with the scales, in each of a list of caches; pairs with -1 are
+    left out."""
+    _op.paged_copy(caches, src, dst, slots)
+
+
 # ---------------------------------------------------------------- numerical-health digests
 def nan_count(x):
     """Number of NaNs of an f16 tensor as a 0-d int64 device tensor (src/thunk/op.rs:273-349)."""

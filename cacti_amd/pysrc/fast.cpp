@@ -18,6 +18,7 @@
 
 #include <stdint.h>
 
+#include <initializer_list>
 #include <tuple>
 #include <type_traits>
 #include <utility>
@@ -492,7 +493,7 @@ struct Logits {
     {
         require(t.scalar_type() == at::kHalf && t.dim() == 2, what);
         N = t.size(0), V = t.size(1);
-        require(V <= 1 || t.stride(1) == 1, what);
+        require(N == 0 || V <= 1 || t.stride(1) == 1, what);
         ld = N > 1 ? t.stride(0) : V;
     }
 };
@@ -668,6 +669,333 @@ PyObject *distill_topk_bwd(PyObject *const *o)
     return d.take();
 }
 
+// ---------------------------------------------------------------- drawn tokens, adapters, several answers in one cache
+PyObject *tuple_of(std::initializer_list<Result> rs)
+{
+    PyObject *r = PyTuple_New((Py_ssize_t)rs.size());
+    if (!r) throw PyFailed();
+    Py_ssize_t i = 0;
+    for (const Result &x : rs) PyTuple_SET_ITEM(r, i++, x.take());
+    return r;
+}
+// a gradient of the logits' shape: the argument that is added to, or a new one
+struct LogitGradient {
+    Result r = {at::Tensor(), nullptr};
+    int64_t ld;
+    LogitGradient(PyObject *acc, const Logits &z, const OnDevice &on, const char *what) : ld(z.V)
+    {
+        if (acc == Py_None) r.t = empty({z.N, z.V}, z.t, at::kHalf);
+        else {
+            const Logits w(acc, on, what);
+            require(w.t.sizes() == z.t.sizes(), what);
+            r = {w.t, acc}, ld = w.ld;
+        }
+    }
+};
+Result new_f32(at::IntArrayRef sizes, const at::Tensor &like) { return {empty(sizes, like, at::kFloat), nullptr}; }
+Result new_i32(at::IntArrayRef sizes, const at::Tensor &like) { return {empty(sizes, like, at::kInt), nullptr}; }
+void given(PyObject *o, const char *what) { require(o != Py_None, what); }
+
+// (logit, tok, temperature, mask, status): (logp, stats)
+PyObject *token_logp_fwd(PyObject *const *o)
+{
+    const OnDevice on(on_gpu(tensor(o[0])));
+    const Logits z(o[0], on, "token_logp: logits [N, V] f16 expected");
+    given(o[1], "token_logp: tok [N] expected");
+    const void *tok = on.pointer(o[1], at::kShort, z.N), *mask = on.pointer(o[3], at::kBool, z.N);
+    const double temperature = number<double>(o[2]);
+    void *status = on.pointer(o[4], at::kInt, 1), *st = on.stream();
+    const Result logp = new_f32({z.N}, z.t), stats = new_f32({z.N, 2}, z.t);
+    if (z.N > 0)
+        run([&] {
+            return cacti_hip_token_logp_fwd(z.N, z.V, z.t.data_ptr(), z.ld, tok, mask, temperature, logp.ptr(), stats.ptr(), status, st);
+        });
+    return take2(logp, stats);
+}
+
+// (logit, tok, stats, dlogp, temperature, acc)
+PyObject *token_logp_bwd(PyObject *const *o)
+{
+    const OnDevice on(on_gpu(tensor(o[0])));
+    const Logits z(o[0], on, "token_logp: logits [N, V] f16 expected");
+    given(o[1], "token_logp: tok [N] expected"), given(o[2], "token_logp: stats [N, 2] expected"), given(o[3], "token_logp: dlogp [N] expected");
+    const void *tok = on.pointer(o[1], at::kShort, z.N), *stats = on.pointer(o[2], at::kFloat, 2 * z.N), *dlogp = on.pointer(o[3], at::kFloat, z.N);
+    const double temperature = number<double>(o[4]);
+    const LogitGradient d(o[5], z, on, "token_logp: acc [N, V] f16 expected");
+    void *st = on.stream();
+    if (z.N > 0)
+        run([&] {
+            return cacti_hip_token_logp_bwd(z.N, z.V, z.t.data_ptr(), z.ld, tok, stats, dlogp, temperature, d.r.ptr(), d.ld, d.r.acc(), st);
+        });
+    return d.r.take();
+}
+
+// (logit, tok, old, adv, scale, ref, mask, clip_lo, clip_hi, beta, temperature, acc, status): (loss, logp, dlogit)
+PyObject *policy_loss(PyObject *const *o)
+{
+    const OnDevice on(on_gpu(tensor(o[0])));
+    const Logits z(o[0], on, "policy_loss: logits [N, V] f16 expected");
+    for (int i = 1; i <= 4; i++) given(o[i], "policy_loss: tok, old, adv and scale [N] expected");
+    const void *tok = on.pointer(o[1], at::kShort, z.N), *old = on.pointer(o[2], at::kFloat, z.N), *adv = on.pointer(o[3], at::kFloat, z.N),
+               *scale = on.pointer(o[4], at::kFloat, z.N), *ref = on.pointer(o[5], at::kFloat, z.N), *mask = on.pointer(o[6], at::kBool, z.N);
+    const double lo = number<double>(o[7]), hi = number<double>(o[8]), beta = number<double>(o[9]), temperature = number<double>(o[10]);
+    const LogitGradient d(o[11], z, on, "policy_loss: acc [N, V] f16 expected");
+    void *status = on.pointer(o[12], at::kInt, 1), *st = on.stream();
+    const Result loss = new_f32({z.N}, z.t), logp = new_f32({z.N}, z.t);
+    if (z.N > 0)
+        run([&] {
+            return cacti_hip_policy_loss(z.N, z.V, z.t.data_ptr(), z.ld, tok, mask, old, adv, ref, scale, lo, hi, beta, temperature, loss.ptr(),
+                                         logp.ptr(), d.r.ptr(), d.ld, d.r.acc(), status, st);
+        });
+    return tuple_of({loss, logp, d.r});
+}
+
+// (logp, ref, starts, scale, beta, smoothing, mask, mean, status): (loss, reward, dlogp)
+PyObject *preference_loss(PyObject *const *o)
+{
+    const OnDevice on(on_gpu(tensor(o[0])));
+    const at::Tensor &logp = on.here(o[0], at::kFloat), &starts = on.here(o[2], at::kInt);
+    const int64_t N = logp.numel(), pairs = (starts.numel() - 1) / 2;
+    require(starts.numel() % 2 == 1, "preference_loss: starts [2 pairs + 1] expected");
+    given(o[3], "preference_loss: scale [pairs] expected");
+    const void *ref = on.pointer(o[1], at::kFloat, N), *scale = on.pointer(o[3], at::kFloat, pairs), *mask = on.pointer(o[6], at::kBool, N);
+    const double beta = number<double>(o[4]), smoothing = number<double>(o[5]);
+    const int mean = truth(o[7]);
+    void *status = on.pointer(o[8], at::kInt, 1), *st = on.stream();
+    const Result loss = new_f32({pairs}, logp), reward = new_f32({2 * pairs}, logp), dlogp = new_f32({N}, logp);
+    if (N > 0 && pairs > 0)
+        run([&] {
+            return cacti_hip_preference_loss(N, pairs, logp.data_ptr(), ref, mask, starts.data_ptr(), scale, beta, smoothing, mean, loss.ptr(),
+                                             reward.ptr(), dlogp.ptr(), status, st);
+        });
+    else {
+        // no pairs, or texts of no rows: their rewards are 0
+        dlogp.t.zero_();
+        reward.t.zero_();
+        loss.t.fill_(0.69314718055994530942);
+    }
+    return tuple_of({loss, reward, dlogp});
+}
+
+// x, A, B, starts, ids, scale of a call over adapters
+struct Adapters {
+    const Logits x;
+    const at::Tensor &A, &B, &starts;
+    const void *ids, *scale;
+    int64_t n, R, K, N, S, max_new;
+    Adapters(PyObject *const *o, PyObject *most, const OnDevice &on)
+        : x(o[0], on, "adapter: x [T, K] f16 expected"), A(on.here(o[1], at::kHalf)), B(on.here(o[2], at::kHalf)), starts(on.here(o[3], at::kInt))
+    {
+        require(A.dim() == 3 && B.dim() == 3 && A.size(0) == B.size(0) && A.size(1) == B.size(2), "adapter: A [n, R, K] and B [n, N, R] expected");
+        n = A.size(0), R = A.size(1), K = A.size(2), N = B.size(1), S = starts.numel() - 1;
+        require(x.V == K, "adapter: x has rows of another length than A");
+        require(S >= 0, "adapter: starts [sequences + 1] expected");
+        given(o[4], "adapter: ids [sequences] expected"), given(o[5], "adapter: scale [adapters] expected");
+        ids = on.pointer(o[4], at::kInt, S), scale = on.pointer(o[5], at::kFloat, n);
+        max_new = most == Py_None ? x.N : number<int64_t>(most);
+        require(max_new > 0 || (max_new == 0 && (x.N == 0 || S == 0)), "adapter: max_new is at least 1 where there are rows and sequences");
+    }
+    bool some() const { return x.N > 0 && S > 0; }
+};
+
+// (x, A, B, starts, ids, scale, base, out, max_new, status): (y, h)
+PyObject *adapter_fwd(PyObject *const *o)
+{
+    const OnDevice on(on_gpu(tensor(o[0])));
+    const Adapters g(o, o[8], on);
+    const int64_t T = g.x.N;
+    const void *base = nullptr;
+    int64_t ldb = 0, ldy = g.N;
+    auto rows = [&](PyObject *p, const char *what) {
+        Logits r(p, on, what);
+        require(r.N == T && r.V == g.N, what);
+        return r;
+    };
+    if (o[6] != Py_None) {
+        const Logits b = rows(o[6], "adapter_fwd: base [T, N] f16 expected");
+        base = b.t.data_ptr(), ldb = b.ld;
+    }
+    Result y = {at::Tensor(), nullptr};
+    if (o[7] == Py_None) y.t = empty({T, g.N}, g.x.t, at::kHalf);
+    else {
+        const Logits w = rows(o[7], "adapter_fwd: out [T, N] f16 expected");
+        y = {w.t, o[7]}, ldy = w.ld;
+    }
+    const Result h = new_f32({T, g.R}, g.x.t);
+    void *status = on.pointer(o[9], at::kInt, 1), *st = on.stream();
+    if (g.some())
+        run([&] {
+            return cacti_hip_adapter_fwd(T, g.S, g.K, g.N, g.R, g.n, g.max_new, g.x.t.data_ptr(), g.x.ld, g.A.data_ptr(), g.B.data_ptr(),
+                                         g.starts.data_ptr(), g.ids, g.scale, base, ldb, y.ptr(), ldy, h.ptr(), status, st);
+        });
+    return take2(y, h);
+}
+
+// (x, A, B, starts, ids, scale, h, dy, dx_acc, dA_acc, dB_acc, max_new, status): (dx, dA, dB)
+PyObject *adapter_bwd(PyObject *const *o)
+{
+    const OnDevice on(on_gpu(tensor(o[0])));
+    const Adapters g(o, o[11], on);
+    const int64_t T = g.x.N;
+    const at::Tensor &h = on.here(o[6], at::kFloat);
+    require(h.dim() == 2 && h.size(0) == T && h.size(1) == g.R, "adapter_bwd: h [T, R] f32 expected");
+    const Logits dy(o[7], on, "adapter_bwd: dy [T, N] f16 expected");
+    require(dy.N == T && dy.V == g.N, "adapter_bwd: dy [T, N] f16 expected");
+    Result dx = {at::Tensor(), nullptr};
+    int64_t lddx = g.K;
+    if (o[8] == Py_None) dx.t = empty({T, g.K}, g.x.t, at::kHalf);
+    else {
+        const Logits w(o[8], on, "adapter_bwd: dx_acc [T, K] f16 expected");
+        require(w.N == T && w.V == g.K, "adapter_bwd: dx_acc [T, K] f16 expected");
+        dx = {w.t, o[8]}, lddx = w.ld;
+    }
+    auto weights = [&](PyObject *acc, const at::Tensor &like) {
+        const Result r = result(acc, like);
+        require(r.t.sizes() == like.sizes(), "adapter_bwd: a gradient of another shape than its adapter");
+        on.here(r.t);
+        return r;
+    };
+    const Result dA = weights(o[9], g.A), dB = weights(o[10], g.B);
+    void *status = on.pointer(o[12], at::kInt, 1), *st = on.stream();
+    if (g.some()) {
+        const size_t bytes = cacti_hip_adapter_bwd_workspace(T, g.K, g.N, g.R, g.n);
+        const at::Tensor ws = empty({(int64_t)bytes}, g.x.t, at::kByte);
+        run([&] {
+            return cacti_hip_adapter_bwd(T, g.S, g.K, g.N, g.R, g.n, g.max_new, g.x.t.data_ptr(), g.x.ld, g.A.data_ptr(), g.B.data_ptr(),
+                                         g.starts.data_ptr(), g.ids, g.scale, h.data_ptr(), dy.t.data_ptr(), dy.ld, dx.ptr(), lddx, dx.acc(),
+                                         dA.ptr(), dA.acc(), dB.ptr(), dB.acc(), ws.data_ptr(), bytes, status, st);
+        });
+    } else {
+        if (!dA.acc()) dA.t.zero_();
+        if (!dB.acc()) dB.t.zero_();
+    }
+    return tuple_of({dx, dA, dB});
+}
+
+// refs and table of a call that hands pages out
+struct Book {
+    const at::Tensor &refs, &table;
+    int64_t P, B, W, ldt;
+    Book(PyObject *r, PyObject *t, const OnDevice &on) : refs(on.here(r, at::kInt)), table(on.here(on_gpu(tensor(t))))
+    {
+        require(table.scalar_type() == at::kInt && table.dim() == 2 && (table.size(1) <= 1 || table.stride(1) == 1),
+                "paged cache: table [sequences, pages] of int32 expected");
+        P = refs.numel(), B = table.size(0), W = table.size(1), ldt = B > 1 ? table.stride(0) : W;
+    }
+    bool some() const { return P > 0 && B > 0 && W > 0; }
+};
+
+// (refs, table, lens, parent, page, out, status): (table, lens)
+PyObject *paged_fork(PyObject *const *o)
+{
+    const OnDevice on(on_gpu(tensor(o[0])));
+    const Book k(o[0], o[1], on);
+    given(o[2], "paged_fork: lens [sequences] expected"), given(o[3], "paged_fork: parent [sequences] expected");
+    const void *lens = on.pointer(o[2], at::kInt, k.B), *parent = on.pointer(o[3], at::kInt, k.B);
+    const int64_t page = number<int64_t>(o[4]);
+    Result table = {at::Tensor(), nullptr}, now = {at::Tensor(), nullptr};
+    int64_t ldn = k.W;
+    if (o[5] == Py_None) table = new_i32({k.B, k.W}, k.refs), now = new_i32({k.B}, k.refs);
+    else {
+        require(PyTuple_Check(o[5]) && PyTuple_GET_SIZE(o[5]) == 2, "paged_fork: out = (table, lens) expected");
+        PyObject *t = PyTuple_GET_ITEM(o[5], 0), *l = PyTuple_GET_ITEM(o[5], 1);
+        const Book w(o[0], t, on);
+        require(w.table.sizes() == k.table.sizes() && on.here(l, at::kInt).numel() == k.B, "paged_fork: shapes of out");
+        table = {w.table, t}, now = {tensor(l), l}, ldn = w.ldt;
+    }
+    void *status = on.pointer(o[6], at::kInt, 1), *st = on.stream();
+    if (k.some())
+        run([&] {
+            return cacti_hip_paged_fork(k.P, k.B, k.W, page, k.refs.data_ptr(), k.table.data_ptr(), k.ldt, lens, parent, table.ptr(), ldn, now.ptr(),
+                                        status, st);
+        });
+    else require(k.B == 0, "paged_fork: a cache or a table without pages");
+    return take2(table, now);
+}
+
+// (refs, table, first, lens, page, status): (src, dst, slots)
+PyObject *paged_fit(PyObject *const *o)
+{
+    const OnDevice on(on_gpu(tensor(o[0])));
+    const Book k(o[0], o[1], on);
+    given(o[2], "paged_fit: first [sequences] expected"), given(o[3], "paged_fit: lens [sequences] expected");
+    const void *first = on.pointer(o[2], at::kInt, k.B), *lens = on.pointer(o[3], at::kInt, k.B);
+    const int64_t page = number<int64_t>(o[4]);
+    void *status = on.pointer(o[5], at::kInt, 1), *st = on.stream();
+    const Result src = new_i32({k.B}, k.refs), dst = new_i32({k.B}, k.refs), slots = new_i32({k.B}, k.refs);
+    if (k.some()) {
+        const size_t bytes = cacti_hip_paged_fit_workspace(k.P, k.B);
+        const at::Tensor ws = empty({(int64_t)bytes}, k.refs, at::kByte);
+        run([&] {
+            return cacti_hip_paged_fit(k.P, k.B, k.W, page, k.refs.data_ptr(), k.table.data_ptr(), k.ldt, first, lens, src.ptr(), dst.ptr(),
+                                       slots.ptr(), ws.data_ptr(), bytes, status, st);
+        });
+    } else require(k.B == 0, "paged_fit: a cache or a table without pages");
+    return tuple_of({src, dst, slots});
+}
+
+// (refs, table): (src, dst, used)
+PyObject *paged_compact(PyObject *const *o)
+{
+    const OnDevice on(on_gpu(tensor(o[0])));
+    const Book k(o[0], o[1], on);
+    void *st = on.stream();
+    const Result src = new_i32({k.P / 2}, k.refs), dst = new_i32({k.P / 2}, k.refs), used = new_i32({1}, k.refs);
+    require(k.some(), "paged_compact: a cache or a table without pages");
+    const size_t bytes = cacti_hip_paged_compact_workspace(k.P);
+    const at::Tensor ws = empty({(int64_t)bytes}, k.refs, at::kByte);
+    run([&] {
+        return cacti_hip_paged_compact(k.P, k.B, k.W, k.refs.data_ptr(), k.table.data_ptr(), k.ldt, src.ptr(), dst.ptr(), used.ptr(), ws.data_ptr(),
+                                       bytes, st);
+    });
+    return tuple_of({src, dst, used});
+}
+
+// (caches, src, dst, slots)
+PyObject *paged_copy(PyObject *const *o)
+{
+    const OnDevice on(on_gpu(tensor(o[1])));
+    const at::Tensor &src = on.here(o[1], at::kInt);
+    const int64_t n = src.numel();
+    given(o[2], "paged_copy: dst, as many as src, expected");
+    const void *dst = on.pointer(o[2], at::kInt, n), *slots = on.pointer(o[3], at::kInt, n);
+    PyObject *seq = PySequence_Fast(o[0], "paged_copy: a list of caches expected");
+    if (!seq) throw PyFailed();
+    struct Held {
+        PyObject *o;
+        ~Held() { Py_DECREF(o); }
+    } hold{seq};
+    const int64_t layers = PySequence_Fast_GET_SIZE(seq);
+    std::vector<at::Tensor> held;
+    std::vector<void *> k, v, ks, vs;
+    for (int64_t l = 0; l < layers; l++) {
+        PyObject *c = PySequence_Fast_GET_ITEM(seq, l);
+        require(PyTuple_Check(c) && PyTuple_GET_SIZE(c) == 4, "paged_copy: a cache is (k_pages, v_pages, k_scale, v_scale)");
+        const at::Tensor &kt = on.here(on_gpu(tensor(PyTuple_GET_ITEM(c, 0)))), &vt = on.here(on_gpu(tensor(PyTuple_GET_ITEM(c, 1))));
+        require(kt.dim() == 4 && kt.is_contiguous() && vt.is_contiguous() && vt.sizes() == kt.sizes() && vt.scalar_type() == kt.scalar_type() &&
+                    (kt.scalar_type() == at::kHalf || kt.scalar_type() == at::kFloat8_e4m3fn) && kt.size(3) % 16 == 0,
+                "paged cache: two contiguous tensors [pages, heads, page, Dp] of f16 or float8_e4m3fn expected");
+        require(held.empty() || (held[0].sizes() == kt.sizes() && held[0].scalar_type() == kt.scalar_type()), "paged_copy: caches of one shape and type expected");
+        const bool scaled = kt.scalar_type() != at::kHalf;
+        for (int i = 2; i < 4; i++) require((PyTuple_GET_ITEM(c, i) != Py_None) == scaled, "paged cache: pages of 8 bits have scales, pages of 16 bits none");
+        k.push_back(kt.data_ptr()), v.push_back(vt.data_ptr());
+        ks.push_back(on.pointer(PyTuple_GET_ITEM(c, 2), at::kFloat, kt.size(0) * kt.size(1)));
+        vs.push_back(on.pointer(PyTuple_GET_ITEM(c, 3), at::kFloat, kt.size(0) * kt.size(1)));
+        // (held: another thread may change the list while the call runs)
+        held.push_back(kt), held.push_back(vt);
+        for (int i = 2; i < 4 && scaled; i++) held.push_back(tensor(PyTuple_GET_ITEM(c, i)));
+    }
+    void *st = on.stream();
+    if (layers > 0 && n > 0 && held[0].numel() > 0) {
+        const at::Tensor &t = held[0];
+        run([&] {
+            return cacti_hip_paged_copy(layers, k.data(), v.data(), ks.data(), vs.data(), t.scalar_type() == at::kHalf ? 16 : 8, t.size(0), t.size(1),
+                                        t.size(2), t.size(3), n, src.data_ptr(), dst, slots, st);
+        });
+    }
+    Py_RETURN_NONE;
+}
+
 // (xs)
 PyObject *digests(PyObject *const *v)
 {
@@ -795,6 +1123,16 @@ PyMethodDef methods[] = {
     OP(verify_draft, 8),
     OP(distill_topk_fwd, 5),
     OP(distill_topk_bwd, 7),
+    OP(token_logp_fwd, 5),
+    OP(token_logp_bwd, 6),
+    OP(policy_loss, 13),
+    OP(preference_loss, 9),
+    OP(adapter_fwd, 10),
+    OP(adapter_bwd, 13),
+    OP(paged_fork, 7),
+    OP(paged_fit, 6),
+    OP(paged_compact, 2),
+    OP(paged_copy, 4),
     OP(digests, 1),
     OP(adamw32_step, 6),
     OP(adamw32_scalars, 7),

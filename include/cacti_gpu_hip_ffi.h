@@ -508,6 +508,95 @@ int cacti_hip_distill_topk_bwd(int64_t N, int64_t V, int64_t K, const void *logi
                                const void *stats, const void *scale, double temperature, void *dlogit16, int64_t ldd, int acc,
                                void *stream);
 
+/* ------------------------------------------------------------------------- */
+/* Tuning a model by its own answers: log-probabilities of drawn tokens, losses */
+/* over them, adapters of many requests, and several answers in one cache.      */
+
+/* logp[n] = log softmax(logit[n] / temperature)[tok[n]], and its adjoint dlogit[j] (+)= f16(dlogp[n] / temperature * ([j = tok[n]] - p_j)).
+ * logit16 [N,V] f16 of pitch ld, tok [N] u16, logp, dlogp [N] f32; stats [N,2] f32: maximum and sum, written by the forward call, read by
+ * the adjoint.  mask [N] u8 or NULL: a row where it is 0, or whose token is >= V (status [1] i32 or NULL: 1 + the row), has logp 0 and is
+ * not read; in the adjoint a row with dlogp 0 or such a token has gradient 0 and is not read.  V <= 65536, N < 2^23, any alignment of the
+ * rows.  dlogit16 may be logit16 itself, with the same pitch, and shares no memory with it otherwise.  acc as everywhere.  Sums in fp32. */
+int cacti_hip_token_logp_fwd(int64_t N, int64_t V, const void *logit16, int64_t ld, const void *tok, const void *mask, double temperature,
+                             void *logp, void *stats, void *status, void *stream);
+int cacti_hip_token_logp_bwd(int64_t N, int64_t V, const void *logit16, int64_t ld, const void *tok, const void *stats, const void *dlogp,
+                             double temperature, void *dlogit16, int64_t ldd, int acc, void *stream);
+
+/* Clipped policy loss of drawn tokens and its gradient in one pass over the logits: with lp as above, r = exp(lp - old), d = ref - lp
+ *   loss[n] = -min(r A, clip(r, 1 - clip_lo, 1 + clip_hi) A) + beta (exp(d) - d - 1)
+ *   dlogit[j] (+)= f16(scale[n] / temperature * dloss/dlp * ([j = tok[n]] - p_j)),  dloss/dlp = -[r A <= clip(r) A] r A + beta (1 - exp(d))
+ * old, adv (A), scale, loss, logp (lp), ref: [N] f32; ref NULL: without the last term.  mask, tok, status, dlogit16 as above (a row that is
+ * left out: loss 0, logp 0, gradient 0). */
+int cacti_hip_policy_loss(int64_t N, int64_t V, const void *logit16, int64_t ld, const void *tok, const void *mask, const void *old,
+                          const void *adv, const void *ref, const void *scale, double clip_lo, double clip_hi, double beta,
+                          double temperature, void *loss, void *logp, void *dlogit16, int64_t ldd, int acc, void *status, void *stream);
+
+/* Loss over pairs of texts, of which the first is preferred, and its gradient.  Text t has rows starts[t] .. starts[t + 1] - 1 (starts
+ * [2 pairs + 1] i32 on the device), pair i texts 2 i and 2 i + 1:
+ *   reward[t] = beta sum (logp - ref) over its rows whose mask is not 0 (mean: divided by their number, at least 1)
+ *   h = reward[2 i] - reward[2 i + 1],  loss[i] = -(1 - smoothing) log sigma(h) - smoothing log sigma(-h)
+ *   dlogp[n] = scale[i] dloss/dlogp, 0 for rows that the mask leaves out and rows of no text
+ * logp, ref (or NULL: 0), dlogp: [N] f32; scale, loss: [pairs]; reward: [2 pairs].  In fp64.  status: 1 + a pair whose rows there are not
+ * (its loss, rewards and gradient are 0; what others that share rows with it get is unspecified). */
+int cacti_hip_preference_loss(int64_t N, int64_t pairs, const void *logp, const void *ref, const void *mask, const void *starts,
+                              const void *scale, double beta, double smoothing, int mean, void *loss, void *reward, void *dlogp,
+                              void *status, void *stream);
+
+/* Low-rank adapters of many requests beside a shared projection.  Rows starts[s] .. starts[s + 1] - 1 of x [T,K] are those of sequence s
+ * (starts [S + 1], ids [S] i32 on the device, not read by the host; starts does not fall), which has adapter a = ids[s] of n, or none (-1):
+ *   h = x A_a^T,  y = f16(base + scale[a] h B_a^T)        A [n,R,K], B [n,N,R] f16, contiguous; scale [n] f32; h [T,R] f32
+ * Rows of a sequence without an adapter: y = base, h = 0.  Rows of no sequence are left as they are in y and h.  base NULL: 0; it may be y,
+ * with the same pitch (so that the adapters' part is added to a product), and shares no memory with it otherwise; nor does x.  The
+ * adjoint, with dy [T,N] and h as the forward call wrote it:
+ *   dh = dy B_a,  dx (+)= f16(scale[a] dh A_a),  dA_a (+)= f16(scale[a] sum dh^T x),  dB_a (+)= f16(scale[a] sum dy^T h)   (over a's rows)
+ * (an adapter without rows: 0).  *_acc: 0 first write, 1 added in fp32 before the one rounding.  Sums in fp32 and in a fixed order; h and dh
+ * meet the second product as two f16 terms, 22 bits, 2^-25 of the largest of their row (for dA and dB: of the adapter's rows).  K, N, R multiples of 8, R <= 128; rows of x, y, base,
+ * dy, dx of pitches that are multiples of 8; all 16-byte aligned; n <= 1024.  max_new: no sequence has more rows.  status [1] i32 or NULL: 1 + s
+ * where the rows of sequence s are not there or more than max_new (it has none then), or its id is neither -1 nor below n (it has no
+ * adapter then); the caller clears it.  workspace: cacti_hip_adapter_bwd_workspace bytes, 16-byte aligned, contents undefined on return. */
+int cacti_hip_adapter_fwd(int64_t T, int64_t S, int64_t K, int64_t N, int64_t R, int64_t n, int64_t max_new, const void *x, int64_t ldx,
+                          const void *A, const void *B, const void *starts, const void *ids, const void *scale, const void *base,
+                          int64_t ldb, void *y, int64_t ldy, void *h, void *status, void *stream);
+size_t cacti_hip_adapter_bwd_workspace(int64_t T, int64_t K, int64_t N, int64_t R, int64_t n);
+int cacti_hip_adapter_bwd(int64_t T, int64_t S, int64_t K, int64_t N, int64_t R, int64_t n, int64_t max_new, const void *x, int64_t ldx,
+                          const void *A, const void *B, const void *starts, const void *ids, const void *scale, const void *h,
+                          const void *dy, int64_t lddy, void *dx, int64_t lddx, int dx_acc, void *dA, int dA_acc, void *dB, int dB_acc,
+                          void *workspace, size_t workspace_bytes, void *status, void *stream);
+
+/* Pages of the cache above, handed out on the device.  refs [P] i32: how many hold a page (sequences of the table, and whoever else the
+ * caller counts); table [B,W] i32 of pitch ldt: a sequence's pages in order, -1 behind them; lens [B] i32: its positions, page to a page.
+ * Where nothing else is said lengths are 0 to W page.  A number that is no page of the cache is handed on and not counted.  P, B <= 2^28,
+ * 2^20; W page <= 2^30.  status [1] i32 or NULL: 1 + a sequence whose numbers do not fit, or for which there was no page.
+ *
+ * Sequence b goes on as sequence parent[b] (itself: as it is; -1: empty): row b of new_table = row parent[b] of table as far as its
+ * positions go, -1 behind; new_lens[b] = lens[parent[b]].  All at once, into other memory; refs is brought up to date.  Pages are shared then, also
+ * one that is not full: cacti_hip_paged_fit before the next append.  A sequence whose parent or whose parent's length cannot be stays
+ * as it is and is named. */
+int cacti_hip_paged_fork(int64_t P, int64_t B, int64_t W, int64_t page, void *refs, const void *table, int64_t ldt, const void *lens,
+                         const void *parent, void *new_table, int64_t ldn, void *new_lens, void *status, void *stream);
+/* Each sequence gets the pages that lens[b] positions need, of which the first first[b] are there and the others are going to be written
+ * (first <= lens; equal: nothing is written).  In place: pages behind those it needs go back.  A page from position first on that others hold
+ * too is given up: where everybody who holds it does so, the first of them keeps it.  What is missing then is taken from the pages that
+ * no one holds (refs 0), the lowest first, in the order of sequences and positions.  src, dst, slots [B] i32: the page of sequence b that
+ * is to be copied, where to, and how many of its slots (-1, -1, 0: none) -- by cacti_hip_paged_copy, before anything is appended.
+ * Where pages run out entries stay -1 and the sequence is named.  One workgroup: some us for a batch, 1 us more for 30000 pages that
+ * it has to look through. */
+size_t cacti_hip_paged_fit_workspace(int64_t P, int64_t B);
+int cacti_hip_paged_fit(int64_t P, int64_t B, int64_t W, int64_t page, void *refs, void *table, int64_t ldt, const void *first,
+                        const void *lens, void *src, void *dst, void *slots, void *workspace, size_t workspace_bytes, void *status,
+                        void *stream);
+/* The held pages (refs > 0) to the lowest places: of `used` [1] i32 of them those from place `used` on move, in order, to the places below it that no
+ * one holds.  src, dst [P / 2] i32: from where and to where, -1 behind the last; refs and table follow. */
+size_t cacti_hip_paged_compact_workspace(int64_t P);
+int cacti_hip_paged_compact(int64_t P, int64_t B, int64_t W, void *refs, void *table, int64_t ldt, void *src, void *dst, void *used,
+                            void *workspace, size_t workspace_bytes, void *stream);
+/* Page src[i] to page dst[i], i < n, with its scales, in the caches of `layers` layers (host arrays of device pointers, read before the
+ * call returns; scales: NULL arrays for bits = 16): the first slots[i] positions, or all (slots NULL).  Pairs with a number that is no page
+ * are left out.  A page that is copied to by two of them, or from one that is copied to, has either's values. */
+int cacti_hip_paged_copy(int64_t layers, void *const *k_pages, void *const *v_pages, void *const *k_scale, void *const *v_scale, int bits,
+                         int64_t P, int64_t Hkv, int64_t page, int64_t Dh, int64_t n, const void *src, const void *dst, const void *slots,
+                         void *stream);
+
 /* f16 residual add y = a + b (AddFutThunkSpec src/thunk/op.rs:1480-1535); y may alias a or b. */
 int cacti_hip_add_f16(int64_t n, const void *a, const void *b, void *y, void *stream);
 
