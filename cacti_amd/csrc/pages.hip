@@ -16,8 +16,11 @@ using namespace cacti;
 
 namespace {
 
-__device__ __forceinline__ int load_now(const int *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ void store_now(int *p, int v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+// Counts that one workgroup alone changes: past its first cache, no further
+__device__ __forceinline__ int load_now(const int *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
+__device__ __forceinline__ void store_now(int *p, int v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
+__device__ __forceinline__ void less_one(int *p) { __hip_atomic_fetch_add(p, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
+__device__ __forceinline__ void no_more_than(int *p, int v) { __hip_atomic_fetch_min(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
 // A barrier behind which the workgroup's counts in memory are what it made them: they are written and read past the first cache, in
 // an order that the barrier alone does not promise.
 __device__ __forceinline__ void settled()
@@ -107,78 +110,87 @@ __device__ __forceinline__ int scan(int v, int *total, int *red)
     return before + s - v;
 }
 
-// A sequence's entries that it lets go of, first .. , of which those below need are wanted again; part: slots of the first one
-// that are to be kept
+// A sequence's entries that it lets go of, those from begin on, of which those below need are wanted again; part: slots of the first
+// one that are to be kept.  What does not fit together lets go of nothing.
 struct Span {
     int begin, need, part;
-    bool ok;
 };
-__device__ __forceinline__ Span span(const FitArgs &a, int b)
+__device__ __forceinline__ Span span(const FitArgs &a, int b, bool *ok)
 {
     const int f = a.first[b], l = a.lens[b];
-    Span s = {0, 0, 0, fits(l, a.W, a.page) && f >= 0 && f <= l};
-    if (!s.ok) return s;
-    s.need = (l + a.page - 1) / a.page;
-    s.begin = l > f ? f / a.page : s.need;
-    s.part = l > f ? f % a.page : 0;
-    return s;
+    *ok = fits(l, a.W, a.page) && f >= 0 && f <= l;
+    if (!*ok) return {a.W, 0, 0};
+    const int need = (int)((unsigned)(l + a.page - 1) / (unsigned)a.page), whole = (int)((unsigned)f / (unsigned)a.page);
+    return {l > f ? whole : need, need, l > f ? f - whole * a.page : 0};
 }
 
-// A wave to a sequence, 64 entries at a time
+constexpr int kHeld = 2048;                    // sequences whose spans are in LDS
+constexpr int kLanes = 8;                      // that look at the entries of a sequence which it lets go of and wants again: most have 1 to 3
+// f(sequence, its span, entry of the lane's own or one behind the last, whether it is the first time)
+template <class F>
+__device__ __forceinline__ void each(const FitArgs &a, const Span *held, F f)
+{
+    for (int b = threadIdx.x / kLanes; b < a.B; b += kThreads / kLanes) {
+        bool ok;
+        const Span s = b < kHeld ? held[b] : span(a, b, &ok);
+        for (int j = s.begin; j < s.need; j += kLanes) f(b, s, j + (int)threadIdx.x % kLanes, j == s.begin);
+    }
+}
+// the lanes of a sequence of which something holds
+__device__ __forceinline__ int lanes_with(bool x) { return (int)(__ballot(x) >> (threadIdx.x & 63 & ~(kLanes - 1))) & ((1 << kLanes) - 1); }
+
 __global__ void __launch_bounds__(kThreads) fit_kernel(FitArgs a)
 {
     __shared__ int red[kWaves];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    // all that is written on or not needed is let go of
-    for (int b = wave; b < a.B; b += kWaves) {
-        const Span s = span(a, b);
-        if (!s.ok) {
-            if (lane == 0) name(a.status, b);
-            continue;
-        }
-        for (int j = s.begin + lane; j < a.W; j += 64) {
-            const int x = a.table[b * a.ldt + j];
-            if (x >= 0 && x < a.P) atomicSub(a.refs + x, 1);
+    __shared__ Span held[kHeld];
+    auto entry = [&](int b, int j) __attribute__((always_inline)) { return a.table + b * a.ldt + j; };
+    auto page = [&](int x) __attribute__((always_inline)) { return x >= 0 && x < a.P; };
+    for (int b = threadIdx.x; b < a.B; b += kThreads) {
+        bool ok;
+        const Span s = span(a, b, &ok);
+        if (b < kHeld) held[b] = s;
+        if (!ok) name(a.status, b);
+        a.src[b] = a.dst[b] = -1;
+        a.slots[b] = a.asked[b] = 0;
+    }
+    __syncthreads();
+    // what is not needed goes back
+    {
+        int b = (int)threadIdx.x / a.W, j = (int)threadIdx.x - b * a.W;
+        const int db = kThreads / a.W, dj = kThreads - db * a.W;
+        for (; b < a.B; b += db, j += dj) {
+            if (j >= a.W && ++b >= a.B) break;
+            if (j >= a.W) j -= a.W;
+            bool ok;
+            const Span s = b < kHeld ? held[b] : span(a, b, &ok);
+            if (j < s.begin || j < s.need) continue;
+            const int x = *entry(b, j);
+            if (page(x)) less_one(a.refs + x);
+            if (x != -1) *entry(b, j) = -1;
         }
     }
+    // what is written on is let go of
+    each(a, held, [&](int b, const Span &s, int j, bool) __attribute__((always_inline)) {
+        const int x = j < s.need ? *entry(b, j) : -1;
+        if (page(x)) less_one(a.refs + x);
+    });
     settled();
     // a page that no one keeps goes to the first of those who want it again: b - B, below all counts
-    for (int b = wave; b < a.B; b += kWaves) {
-        const Span s = span(a, b);
-        for (int j = s.begin + lane; j < s.need; j += 64) {
-            const int x = a.table[b * a.ldt + j];
-            if (x >= 0 && x < a.P && load_now(a.refs + x) <= 0) atomicMin(a.refs + x, b - a.B);
-        }
-    }
+    each(a, held, [&](int b, const Span &s, int j, bool) __attribute__((always_inline)) {
+        const int x = j < s.need ? *entry(b, j) : -1;
+        if (page(x) && load_now(a.refs + x) <= 0) no_more_than(a.refs + x, b - a.B);
+    });
     settled();
-    // who has none of its own asks for one: marked in the table as -2 - the page that is to be copied, or as -1
-    for (int b = wave; b < a.B; b += kWaves) {
-        const Span s = span(a, b);
-        int count = 0;
-        if (lane == 0) a.src[b] = a.dst[b] = -1, a.slots[b] = 0;
-        if (s.ok)
-            for (int j0 = s.begin; j0 < a.W; j0 += 64) {
-                const int j = j0 + lane;
-                bool asks = false;
-                if (j < a.W) {
-                    int *e = a.table + b * a.ldt + j;
-                    const int x = *e;
-                    if (j < s.need) asks = !(x >= 0 && x < a.P && load_now(a.refs + x) == b - a.B);
-                    if (asks && s.part && j == s.begin && x >= 0 && x < a.P) a.src[b] = x;
-                    if (asks || j >= s.need) *e = -1;
-                }
-                count += __popcll(__ballot(asks));
-            }
-        if (lane == 0) a.asked[b] = count;
-    }
+    // who has none of its own asks for one
+    each(a, held, [&](int b, const Span &s, int j, bool first) __attribute__((always_inline)) {
+        const int x = j < s.need ? *entry(b, j) : -1;
+        const bool asks = j < s.need && !(page(x) && load_now(a.refs + x) == b - a.B);
+        if (asks && s.part && j == s.begin && page(x)) a.src[b] = x;
+        if (asks) *entry(b, j) = -1;
+        const int n = __popc(lanes_with(asks));
+        if (threadIdx.x % kLanes == 0) a.asked[b] = (first ? 0 : a.asked[b]) + n;
+    });
     settled();
-    for (int b = wave; b < a.B; b += kWaves) {
-        const Span s = span(a, b);
-        for (int j = s.begin + lane; j < s.need; j += 64) {
-            const int x = a.table[b * a.ldt + j];
-            if (x >= 0) store_now(a.refs + x, 1);
-        }
-    }
     // how many are asked for before each sequence
     int all = 0;
     for (int b0 = 0; b0 < a.B; b0 += kThreads) {
@@ -188,44 +200,38 @@ __global__ void __launch_bounds__(kThreads) fit_kernel(FitArgs a)
         if (b < a.B) a.asked[b] = all + before;
         all += total;
     }
-    settled();
     // the lowest free pages, as many as are asked for
     int found = 0;
     for (int p0 = 0; p0 < a.P && found < all; p0 += 4 * kThreads) {
         const int p = p0 + 4 * (int)threadIdx.x;
         int is[4], n = 0;
 #pragma unroll
-        for (int k = 0; k < 4; k++) n += is[k] = p + k < a.P && load_now(a.refs + p + k) == 0;
-        int total, at = found + scan(n, &total, red);
+        for (int k = 0; k < 4; k++) is[k] = p + k < a.P ? load_now(a.refs + p + k) : 1;
+#pragma unroll
+        for (int k = 0; k < 4; k++) n += is[k] == 0;
+        int total, to = found + scan(n, &total, red);
 #pragma unroll
         for (int k = 0; k < 4; k++)
-            if (is[k]) a.free[at++] = p + k;
+            if (is[k] == 0) a.free[to++] = p + k;
         found += total;
     }
     settled();
-    // .. handed out
-    for (int b = wave; b < a.B; b += kWaves) {
-        const Span s = span(a, b);
-        int at = a.asked[b];
-        for (int j0 = s.begin; j0 < s.need; j0 += 64) {
-            const int j = j0 + lane;
-            int *e = a.table + b * a.ldt + j;
-            const bool asks = j < s.need && *e == -1;
-            const uint64_t mask = __ballot(asks);
-            const int k = at + __popcll(mask & ((1ull << lane) - 1));
-            const bool got = asks && k < found;
-            if (got) {
-                const int x = a.free[k];
-                *e = x;
-                store_now(a.refs + x, 1);
-                if (s.part && j == s.begin && a.src[b] >= 0) a.dst[b] = x, a.slots[b] = s.part;
-            } else if (asks) {
-                name(a.status, b);
-                if (s.part && j == s.begin) a.src[b] = -1;
-            }
-            at += __popcll(mask);
-        }
-    }
+    // .. handed out; what is kept counts one
+    int at = 0;
+    each(a, held, [&](int b, const Span &s, int j, bool first) __attribute__((always_inline)) {
+        if (first) at = a.asked[b];
+        int x = j < s.need ? *entry(b, j) : -2;
+        const bool asks = x == -1;
+        const int mask = lanes_with(asks), k = at + __popc(mask & ((1 << threadIdx.x % kLanes) - 1));
+        at += __popc(mask);
+        if (asks && k < found) *entry(b, j) = x = a.free[k];
+        if (x >= 0) store_now(a.refs + x, 1);
+        if (!asks) return;
+        const bool copied = s.part && j == s.begin && a.src[b] >= 0;
+        if (x < 0) name(a.status, b);
+        if (copied && x >= 0) a.dst[b] = x, a.slots[b] = s.part;
+        if (copied && x < 0) a.src[b] = -1;
+    });
 }
 
 // ---------------------------------------------------------------- compact
@@ -287,29 +293,34 @@ struct CopyArgs {
     char *k[kLayers], *v[kLayers];
     float *ks[kLayers], *vs[kLayers];
     const int *src, *dst, *slots;
-    int64_t n, P, items;
-    int layers, heads, page, slot_bytes;       // of a position of a head
+    int64_t n, P;
+    unsigned items;
+    int parts, layers, heads, page, slot_bytes;        // (of a position of a head)
 };
 
-// An item: the keys or the values of a page of a layer
+// An item: four heads of the keys or the values of a page of a layer, a wave to each
 __global__ void __launch_bounds__(256) copy_kernel(CopyArgs a)
 {
-    for (int64_t i = blockIdx.x; i < a.items; i += gridDim.x) {
-        const int64_t which = i / (2 * a.layers);
-        const int of = (int)(i % (2 * a.layers)), layer = of >> 1;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (unsigned i = blockIdx.x; i < a.items; i += gridDim.x) {
+        const unsigned part = i % a.parts, of = i / a.parts % (2 * a.layers), which = i / a.parts / (2 * a.layers), layer = of >> 1;
         const int64_t s = a.src[which], d = a.dst[which];
         if (s < 0 || d < 0 || s >= a.P || d >= a.P || s == d) continue;
-        const int slots = a.slots ? min(max(a.slots[which], 0), a.page) : a.page;
+        const int slots = a.slots ? min(max(a.slots[which], 0), a.page) : a.page, h = 4 * (int)part + wave;
+        if (h >= a.heads || slots == 0) continue;
+        const int64_t head = (int64_t)a.page * a.slot_bytes;
         char *pages = of & 1 ? a.v[layer] : a.k[layer];
-        float *scales = of & 1 ? a.vs[layer] : a.ks[layer];
-        const int64_t head = (int64_t)a.page * a.slot_bytes, bytes = head * a.heads;
+        const uint4 *from = reinterpret_cast<const uint4 *>(pages + (s * a.heads + h) * head);
+        uint4 *to = reinterpret_cast<uint4 *>(pages + (d * a.heads + h) * head);
         const int pieces = slots * a.slot_bytes / 16;
-        for (int e = threadIdx.x; e < a.heads * pieces; e += 256) {
-            const int64_t at = (e / pieces) * head + 16 * (e % pieces);
-            *reinterpret_cast<uint4 *>(pages + d * bytes + at) = *reinterpret_cast<const uint4 *>(pages + s * bytes + at);
+        int e = lane;
+        for (; e + 192 < pieces; e += 256) {   // 4 KB under way
+            const uint4 x0 = from[e], x1 = from[e + 64], x2 = from[e + 128], x3 = from[e + 192];
+            to[e] = x0, to[e + 64] = x1, to[e + 128] = x2, to[e + 192] = x3;
         }
-        if (scales && slots)
-            for (int h = threadIdx.x; h < a.heads; h += 256) scales[d * a.heads + h] = scales[s * a.heads + h];
+        for (; e < pieces; e += 64) to[e] = from[e];
+        float *scales = of & 1 ? a.vs[layer] : a.ks[layer];
+        if (scales && lane == 0) scales[d * a.heads + h] = scales[s * a.heads + h];
     }
 }
 
@@ -404,9 +415,11 @@ CACTI_API int cacti_hip_paged_copy(int64_t layers, void *const *k_pages, void *c
             if (bits == 8) a.ks[l] = (float *)k_scale[l0 + l], a.vs[l] = (float *)v_scale[l0 + l];
         }
         a.src = (const int *)src, a.dst = (const int *)dst, a.slots = (const int *)slots;
-        a.n = n, a.P = P, a.items = n * 2 * a.layers;
         a.heads = (int)Hkv, a.page = (int)page, a.slot_bytes = (int)((Dh + 15) / 16 * 16 * bits / 8);
-        const int64_t blocks = a.items < 2048 ? a.items : 2048;
+        const int64_t parts = (Hkv + 3) / 4, items = n * 2 * a.layers * parts;
+        CACTI_REQUIRE(items <= INT32_MAX, CACTI_E_NOTIMPL, "paged_copy: too many pages");
+        a.n = n, a.P = P, a.parts = (int)parts, a.items = (unsigned)items;
+        const int64_t blocks = a.items < 4096 ? a.items : 4096;
         hipLaunchKernelGGL(copy_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
     }
     return launch_status("paged_copy");

@@ -19,7 +19,7 @@ REFUSED = [("cacti_hip_paged_fork", FORK, c) for c in BOOK + [
     (dict(lens=0x3004), "share memory")]] + \
           [("cacti_hip_paged_fit", FIT, c) for c in BOOK + [
               (dict(page=0), "empty"), (dict(first=None), "null"), (dict(src=None), "null"), (dict(slots=66), "misaligned"), (dict(ws=None), "null"),
-              (dict(ws_bytes=40), "workspace")]] + \
+              (dict(ws_bytes=32), "workspace")]] + \
           [("cacti_hip_paged_compact", COMPACT, c) for c in [x for x in BOOK if "status" not in x[0]] + [
               (dict(src=None), "null"), (dict(used=None), "null"), (dict(used=66), "misaligned"), (dict(ws_bytes=32), "workspace")]]
 
