@@ -7,6 +7,12 @@
 // and what its rounding left, 22 bits in all, so that results are rounded once.  They are scaled by a power of two first, that of the
 // largest of a row (for y and dx) or of the rows so far (for dA and dB): a gradient may lie far below f16's range and h beyond it.
 // The terms lie side by side as 2 R columns, which for R = 16 fill the 32 that an instruction takes.
+//
+// A matrix instruction wants 16 rows in 16 lanes side by side.  Loads in that order take 64 looks at the cache each, a quarter of what a
+// compute unit can read (measured: 26 GB/s of it); here 4 lanes read 64 bytes of a row, and a wave turns its tiles of 16 rows of 64
+// bytes in LDS, on the way in and on the way out.
+#include <algorithm>
+
 #include "operands.h"
 #include "paged.h"
 
@@ -46,10 +52,11 @@ __device__ __forceinline__ int adapter_of(const AdapterArgs &g, int b)
     const int a = g.ids[b];
     return a >= 0 && a < g.n ? a : -1;
 }
-__device__ __forceinline__ Tile find_tile(const AdapterArgs &g, int64_t u, int per)
+__device__ __forceinline__ Tile find_tile(const AdapterArgs &g, int u, int per)
 {
-    int i, s0, n;
-    const int b = g.units.find(g.pb, u, &i);
+    int i, s0, n, b;
+    if (g.units.even) b = u / g.units.even, i = u - b * g.units.even;
+    else b = g.units.find(g.pb, u, &i);
     if (b >= g.pb.B || !rows_of(g, b, &s0, &n) || (int64_t)i * per >= n) return {0, 0, -1};
     return {s0 + i * per, min(per, n - i * per), adapter_of(g, b)};
 }
@@ -62,6 +69,7 @@ __device__ void look_over(const AdapterArgs &g)
     }
 }
 
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 __device__ __forceinline__ half8_t zero8() { return half8_t{0, 0, 0, 0, 0, 0, 0, 0}; }
 __device__ __forceinline__ float4_t zero4() { return float4_t{0.f, 0.f, 0.f, 0.f}; }
 __device__ __forceinline__ half8_t load8(const half_t *p) { return *reinterpret_cast<const half8_t *>(p); }
@@ -94,175 +102,430 @@ __device__ __forceinline__ half4_t read_tr(const half_t *q)
 }
 __device__ __forceinline__ half8_t both(half4_t a, half4_t b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
-// ---------------------------------------------------------------- h of a tile of 16 rows
-// acc[i][e]: row of the tile lane & 15, column 16 i + 4 (lane >> 4) + e of h, over the steps of 32 of the contraction that the wave has.
-// W: [R, K] (TR = false) or [K, R] (true), lds: 32 rows of 2 R + 16 bytes of its own for each wave.
-template <int RT, int WAVES, bool TR>
-__device__ __forceinline__ void tile_h(const half_t *x, int64_t ldx, int rows, int K, const half_t *W, int R, half_t *lds, float4_t (&acc)[RT])
+// ---------------------------------------------------------------- tiles of 16 rows of 64 bytes, a wave's own
+// A lane's 16 bytes of one, row lane / 4 as it lies in memory or row lane % 16 as an operand; where in LDS they are, without conflicts
+// in either order.
+constexpr int kTileHalves = 16 * 32;
+__device__ __forceinline__ int mem_row() { return (threadIdx.x & 63) >> 2; }
+__device__ __forceinline__ int mem_col() { return 8 * (threadIdx.x & 3); }
+__device__ __forceinline__ int place(int row, int piece) { return 32 * row + 8 * (piece ^ (row >> 2)); }
+__device__ __forceinline__ half_t *as_memory(half_t *tile) { return tile + place(mem_row(), threadIdx.x & 3); }
+__device__ __forceinline__ half_t *as_operand(half_t *tile)
 {
-    constexpr int U = TR ? (RT <= 2 ? 2 : 1) : RT <= 2 ? 4 : RT <= 4 ? 2 : 1;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
-    const half_t *xr = x + (int64_t)min(m, rows - 1) * ldx + 8 * g;
-    const int pitch = R + 8;
-#pragma unroll
-    for (int i = 0; i < RT; i++) acc[i] = zero4();
-    const int steps = (K + 31) / 32;
-    for (int c0 = wave * U; c0 < steps; c0 += WAVES * U) {
-        half8_t xf[U], wf[U][RT];
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int k0 = 32 * (c0 + u);
-            xf[u] = load8(xr + min(k0, K - 8 - 8 * g));
-            if constexpr (!TR) {
-#pragma unroll
-                for (int i = 0; i < RT; i++) wf[u][i] = load8(W + (int64_t)min(16 * i + m, R - 1) * K + min(k0 + 8 * g, K - 8));
-            } else {
-#pragma unroll
-                for (int i = 0; i < RT; i++) {
-                    const int piece = 64 * i + lane, per = R / 8, k = piece / per;
-                    wf[u][i] = load8(W + (int64_t)min(k0 + min(k, 31), K - 1) * R + 8 * (piece % per));
-                }
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int k0 = 32 * (c0 + u);
-            if (k0 >= K) break;
-            if constexpr (TR) {
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-                for (int i = 0; i < RT; i++) {
-                    const int piece = 64 * i + lane, per = R / 8, k = piece / per;
-                    if (k < 32) *reinterpret_cast<half8_t *>(lds + k * pitch + 8 * (piece % per)) = k0 + k < K ? wf[u][i] : zero8();
-                }
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-                for (int i = 0; i < RT; i++) {
-                    // (columns from R on are those of a row of h that is not used; the last piece stays within the row's padding)
-                    const half_t *q = lds + (8 * g + (m >> 2)) * pitch + min(16 * i + 4 * (m & 3), R + 4);
-                    wf[u][i] = both(read_tr(q), read_tr(q + 4 * pitch));
-                }
-            }
-            if (k0 + 8 * g >= K) {
-                xf[u] = zero8();
-#pragma unroll
-                for (int i = 0; i < RT; i++) wf[u][i] = zero8();
-            }
-#pragma unroll
-            for (int i = 0; i < RT; i++) acc[i] = mfma(wf[u][i], xf[u], acc[i]);
-        }
-    }
+    const int lane = threadIdx.x & 63;
+    return tile + place(lane & 15, lane >> 4);
 }
+__device__ __forceinline__ void put8(half_t *p, half8_t v) { *reinterpret_cast<half8_t *>(p) = v; }
+// what a wave's lanes have written to LDS before is there for its lanes after (they take turns in order)
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
-// what the waves have of it added up: put(item, row, column, sum) for a thread's items of [16][16 RT]
-template <int RT, int WAVES, class Put>
-__device__ __forceinline__ void join_h(float *red, const float4_t (&acc)[RT], Put put)
-{
-    constexpr int C = 16 * RT;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// ---------------------------------------------------------------- h of a tile of 16 TB rows
+// acc[t][i][e]: row 16 t + (lane & 15) of the tile, column 16 i + 4 (lane >> 4) + e of h, over those of steps s0 .. s1 - 1 of 32 that the wave
+// has.  W: [R, K] (TR = false) or [K, R] (true); lds: kLds halves, the wave's own.  Loads are a turn ahead.
+template <int RT, int TB, int WAVES, bool TR>
+struct TileH {
+    static constexpr int U = RT + TB <= 2 && WAVES <= 8 ? 4 : RT + TB <= 6 ? 2 : 1, kLds = TB * kTileHalves + (TR ? 32 * (16 * RT + 8) : RT * kTileHalves);
+    const half_t *xr[TB], *W;
+    int K, R, m, g;
+    half_t *lds;
+    float4_t acc[TB][RT];
+    struct Turn {
+        half8_t x[U][TB], w[U][RT];
+    };
+    __device__ __forceinline__ TileH(const half_t *x, int64_t ldx, int rows, int k, const half_t *w, int r, half_t *l) : W(w), K(k), R(r), lds(l)
+    {
+        const int lane = threadIdx.x & 63;
+        m = lane & 15, g = lane >> 4;
 #pragma unroll
-    for (int i = 0; i < RT; i++)
-        *reinterpret_cast<float4_t *>(red + (wave * kTile + (lane & 15)) * C + 16 * i + 4 * (lane >> 4)) = acc[i];
-    __syncthreads();
+        for (int t = 0; t < TB; t++) {
+            xr[t] = x + (int64_t)min(16 * t + mem_row(), rows - 1) * ldx;
 #pragma unroll
-    for (int i = 0; i < (kTile * C + 64 * WAVES - 1) / (64 * WAVES); i++) {
-        const int e = threadIdx.x + 64 * WAVES * i;
-        if (e >= kTile * C) break;
-        float s = 0.f;
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) s += red[w * kTile * C + e];
-        put(i, e / C, e % C, s);
+            for (int i = 0; i < RT; i++) acc[t][i] = zero4();
+        }
     }
-}
+    // (a load behind a branch would be one that is waited for with all later ones: what there is not is some other step)
+    __device__ __forceinline__ void load(Turn &o, int c0) const
+    {
+        const int lane = threadIdx.x & 63;
+        // (both halves of a cache line one after the other)
+#pragma unroll
+        for (int t = 0; t < TB; t++)
+#pragma unroll
+            for (int u = 0; u < U; u++) o.x[u][t] = load8(xr[t] + min(32 * (c0 + u) + mem_col(), K - 8));
+#pragma unroll
+        for (int i = 0; i < RT; i++)
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int k0 = 32 * (c0 + u);
+                if constexpr (!TR) o.w[u][i] = load8(W + (int64_t)min(16 * i + mem_row(), R - 1) * K + min(k0 + mem_col(), K - 8));
+                else {
+                    const int piece = 64 * i + lane, per = R / 8, k = piece / per;
+                    o.w[u][i] = load8(W + (int64_t)min(k0 + min(k, 31), K - 1) * R + 8 * (piece % per));
+                }
+            }
+    }
+    __device__ __forceinline__ void add(Turn &o, int c0, int s1)
+    {
+        const int lane = threadIdx.x & 63, pitch = R + 8;
+        half_t *const wl = lds + TB * kTileHalves;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int k0 = 32 * (c0 + u);
+            if (c0 + u >= s1) break;
+            if (k0 + 32 > K && k0 + mem_col() >= K) {
+#pragma unroll
+                for (int t = 0; t < TB; t++) o.x[u][t] = zero8();
+                if constexpr (!TR)
+#pragma unroll
+                    for (int i = 0; i < RT; i++) o.w[u][i] = zero8();
+            }
+            in_order();
+#pragma unroll
+            for (int t = 0; t < TB; t++) put8(as_memory(lds + t * kTileHalves), o.x[u][t]);
+#pragma unroll
+            for (int i = 0; i < RT; i++) {
+                if constexpr (!TR) put8(as_memory(wl + i * kTileHalves), o.w[u][i]);
+                else {
+                    const int piece = 64 * i + lane, per = R / 8, k = piece / per;
+                    if (k < 32) put8(wl + k * pitch + 8 * (piece % per), k0 + k < K ? o.w[u][i] : zero8());
+                }
+            }
+            in_order();
+            half8_t xf[TB];
+#pragma unroll
+            for (int t = 0; t < TB; t++) xf[t] = load8(as_operand(lds + t * kTileHalves));
+#pragma unroll
+            for (int i = 0; i < RT; i++) {
+                half8_t wf;
+                if constexpr (!TR) wf = load8(as_operand(wl + i * kTileHalves));
+                else {
+                    // (columns from R on are those of a row of h that is not used; the last piece stays within the row's padding)
+                    const half_t *q = wl + (8 * g + (m >> 2)) * pitch + min(16 * i + 4 * (m & 3), R + 4);
+                    wf = both(read_tr(q), read_tr(q + 4 * pitch));
+                }
+#pragma unroll
+                for (int t = 0; t < TB; t++) acc[t][i] = mfma(wf, xf[t], acc[t][i]);
+            }
+        }
+    }
+    __device__ __forceinline__ void run(int s0, int s1)
+    {
+        constexpr int stride = U * WAVES;
+        Turn a, b;
+        int c = s0 + U * wave_id();
+        if (c >= s1) return;
+        load(a, c);
+        for (; c + 2 * stride < s1; c += 2 * stride) {
+            load(b, c + stride);
+            add(a, c, s1);
+            load(a, c + 2 * stride);
+            add(b, c + stride, s1);
+        }
+        if (c + stride < s1) {
+            load(b, c + stride);
+            add(a, c, s1);
+            add(b, c + stride, s1);
+        } else
+            add(a, c, s1);
+    }
+    // what the waves have of it added up: put(item, row, column, sum) for a thread's items of [16 TB][16 RT]
+    static constexpr int kItems = (16 * TB * 16 * RT + 64 * WAVES - 1) / (64 * WAVES);
+    template <class Put>
+    __device__ __forceinline__ void join(float *red, Put put)
+    {
+        constexpr int C = 16 * RT, all = 16 * TB * C;
+        const int wave = threadIdx.x >> 6;
+        __syncthreads();                       // (red takes the place of the waves' tiles)
+#pragma unroll
+        for (int t = 0; t < TB; t++)
+#pragma unroll
+            for (int i = 0; i < RT; i++) *reinterpret_cast<float4_t *>(red + wave * all + (16 * t + m) * C + 16 * i + 4 * g) = acc[t][i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kItems; i++) {
+            const int e = threadIdx.x + 64 * WAVES * i;
+            if (e >= all) break;
+            float s = 0.f;
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) s += red[w * all + e];
+            put(i, e / C, e % C, s);
+        }
+    }
+};
 
 // ---------------------------------------------------------------- forward
-// A workgroup to 16 rows of a sequence and 1 / splits of the columns of y; h is formed by each of them.
+// h of a row in LDS: its two terms, the second one 16 RT columns behind the first, zeros from R on in either.  RT = 1: both within the 32
+// columns of one instruction, which B (or A) meets twice.
 template <int RT>
-__global__ void __launch_bounds__(512) adapter_kernel(AdapterArgs g)
-{
-    constexpr int W = 8, C = 16 * RT, HP = 32 * RT + 8;
-    __shared__ __attribute__((aligned(16))) float red[W * kTile * C];
-    __shared__ __attribute__((aligned(16))) half_t hs[kTile * HP];
-    __shared__ int largest[kTile];
-    const int64_t blocks = g.units.count * g.splits;
-    if (blockIdx.x >= blocks) return look_over(g);
-    // the splits of a tile 8 apart, on one XCD: they read the same x and A
-    const int64_t group = blockIdx.x / (8 * g.splits), left = min((int64_t)8, g.units.count - 8 * group);
-    const int in = (int)(blockIdx.x - 8 * group * g.splits), split = in / (int)left;
-    const Tile t = find_tile(g, 8 * group + in % left, kTile);
-    if (t.rows == 0) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, q4 = lane >> 4;
-    const int R = g.R, K = g.K, N = g.N;
-    const float scale = t.a < 0 ? 0.f : g.scale[t.a];
-    if (t.a < 0) {                             // no adapter
-        if (split == 0)
-            for (int e = threadIdx.x; e < t.rows * R; e += 64 * W) g.h[(int64_t)t.row0 * R + e] = 0.f;
-        if (g.base == g.y) return;
-        for (int e = split * 64 * W + threadIdx.x; e < t.rows * (N / 8); e += g.splits * 64 * W) {
-            const int64_t r = t.row0 + e / (N / 8);
-            const int c = 8 * (e % (N / 8));
-            *reinterpret_cast<half8_t *>(g.y + r * g.ldy + c) = g.base ? load8(g.base + r * g.ldb + c) : zero8();
-        }
-        return;
+struct Terms {
+    static constexpr int kPitch = 32 * RT + 8, kLo = 16 * RT, kN = RT == 1 ? 1 : RT / 2, kM = RT == 1 ? 1 : 2;
+    // the row of B that a lane's 8 values of operand i begin at; the columns of h that they meet, part p of kM
+    __device__ __forceinline__ static int of(int i, int q4) { return RT == 1 ? 8 * (q4 & 1) : 32 * i + 8 * q4; }
+    __device__ __forceinline__ static int column(int i, int p, int q4) { return p * kLo + 32 * i + 8 * q4; }
+    __device__ __forceinline__ static void put(half_t *row, int c, float v) { two_terms(v, row + c, row + kLo + c); }
+    __device__ __forceinline__ static void clear(half_t *h, int rows)
+    {
+        for (int e = threadIdx.x; e < rows * kPitch / 8; e += blockDim.x) *reinterpret_cast<half8_t *>(h + 8 * e) = zero8();
     }
-    float4_t acc[RT];
-    tile_h<RT, W, false>(g.x + t.row0 * g.ldx, g.ldx, t.rows, K, g.A + (int64_t)t.a * R * K, R, nullptr, acc);
-    for (int e = threadIdx.x; e < kTile * HP / 8; e += 64 * W) *reinterpret_cast<half8_t *>(hs + 8 * e) = zero8();
+};
+
+// Scale of a row's results: the adapter's and what its h was scaled by.  (Within fp32's range, so that it does not make a 0 a NaN: what it is
+// multiplied with is 0 or no less than 2^-48, which f16 takes for infinite either way.)
+__device__ __forceinline__ float factor_of(float scale, int bits)
+{
+    const float f = scale * two_to(exponent(bits));
+    return fabsf(f) < INFINITY || fabsf(scale) == INFINITY || scale != scale ? f : copysignf(3.4028234664e38f, f);
+}
+
+// Results of a tile of 16 rows and 32 columns to memory, as they are or added to what `old`, as it came from memory, holds: o[j] those of
+// row lane & 15, columns 8 (lane >> 4) + 4 j ..; returns the lane's 16 bytes of row mem_row(), columns mem_col() ..  (Turned as fp32 instead,
+// in one trip and two tiles at a time: the same for y, and LDS for a workgroup less in the gradients, 22.7 -> 26.8 us.)
+template <bool BASE>
+__device__ __forceinline__ half8_t turned(half_t *tile, half8_t old, const float4_t (&o)[2], float factor)
+{
+    half8_t v = zero8();
+    in_order();
+    if constexpr (BASE) {
+        put8(as_memory(tile), old);
+        in_order();
+        v = load8(as_operand(tile));
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = f2h(BASE ? __builtin_fmaf(factor, o[e / 4][e % 4], h2f(v[e])) : factor * o[e / 4][e % 4]);
+    in_order();
+    put8(as_operand(tile), v);
+    in_order();
+    return load8(as_memory(tile));
+}
+
+// 32 columns of y for 16 TB rows whose h is in LDS: 32 rows of B, in an order that leaves a lane 8 columns side by side.
+// lds: kLds halves, the wave's own.
+template <int RT, int TB, bool BASE>
+struct Columns {
+    typedef Terms<RT> H;
+    static constexpr int kLds = kTileHalves + 32 * (16 * RT + 8);
+    half8_t w[RT], old[TB];
+    int n0;
+    __device__ __forceinline__ void load(const AdapterArgs &g, const Tile &t, const half_t *B, int n)
+    {
+        n0 = n;
+        const int last = g.N * (g.R / 8) - 1;  // (rows of B are contiguous)
+#pragma unroll
+        for (int i = 0; i < RT; i++) w[i] = load8(B + 8 * (int64_t)min(n0 * (g.R / 8) + min(64 * i + (int)(threadIdx.x & 63), 4 * g.R - 1), last));
+        if constexpr (BASE)
+#pragma unroll
+            for (int b = 0; b < TB; b++)
+                old[b] = load8(g.base + (int64_t)(t.row0 + min(16 * b + mem_row(), t.rows - 1)) * g.ldb + min(n0 + mem_col(), g.N - 8));
+    }
+    __device__ __forceinline__ void put(const AdapterArgs &g, const Tile &t, const float (&factor)[TB], const half_t *hs, half_t *lds)
+    {
+        const int lane = threadIdx.x & 63, m = lane & 15, q4 = lane >> 4, per = g.R / 8, pitch = g.R + 8;
+        half_t *const tile = lds, *const bl = lds + kTileHalves;
+        in_order();
+#pragma unroll
+        for (int i = 0; i < RT; i++) {
+            const int piece = 64 * i + lane;
+            if (piece < 32 * per) put8(bl + (piece / per) * pitch + 8 * (piece % per), w[i]);
+        }
+        in_order();
+        half8_t wf[2][H::kN];
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int i = 0; i < H::kN; i++) {
+                wf[j][i] = load8(bl + (8 * (m >> 2) + 4 * j + (m & 3)) * pitch + min(H::of(i, q4), g.R - 8));
+                wf[j][i] = H::of(i, q4) < g.R ? wf[j][i] : zero8();
+            }
+#pragma unroll
+        for (int b = 0; b < TB; b++) {
+            if (16 * b >= t.rows) break;
+            float4_t o[2] = {zero4(), zero4()};
+#pragma unroll
+            for (int i = 0; i < H::kN; i++)
+#pragma unroll
+                for (int p = 0; p < H::kM; p++) {
+                    const half8_t hf = load8(hs + (16 * b + m) * H::kPitch + H::column(i, p, q4));
+#pragma unroll
+                    for (int j = 0; j < 2; j++) o[j] = mfma(wf[j][i], hf, o[j]);
+                }
+            const half8_t v = turned<BASE>(tile, old[b], o, factor[b]);
+            const int r = 16 * b + mem_row(), c = n0 + mem_col();
+            if (r < t.rows && c < g.N) *reinterpret_cast<half8_t *>(g.y + (int64_t)(t.row0 + r) * g.ldy + c) = v;
+        }
+    }
+};
+// The columns of a wave, the next ones' operands under way: those from 32 first on, every `stride`-th 32
+template <int RT, int TB, bool BASE>
+struct Wave {
+    typedef Columns<RT, TB, BASE> C;
+    const AdapterArgs &g;
+    const Tile &t;
+    const half_t *B;
+    int n, step;
+    C a, b;
+    __device__ __forceinline__ Wave(const AdapterArgs &g_, const Tile &t_, int first, int stride) : g(g_), t(t_), n(32 * first), step(32 * stride)
+    {
+        B = g.B + (int64_t)t.a * g.N * g.R;
+        a.load(g, t, B, n);
+    }
+    // largest: bits of the largest of each row of h
+    __device__ __forceinline__ void run(float scale, const half_t *hs, const int *largest, half_t *lds)
+    {
+        if (n >= g.N) return;
+        float factor[TB];
+#pragma unroll
+        for (int i = 0; i < TB; i++) factor[i] = factor_of(scale, largest[16 * i + (threadIdx.x & 15)]);
+        for (; n + 2 * step < g.N; n += 2 * step) {
+            b.load(g, t, B, n + step);
+            a.put(g, t, factor, hs, lds);
+            a.load(g, t, B, n + 2 * step);
+            b.put(g, t, factor, hs, lds);
+        }
+        if (n + step < g.N) {
+            b.load(g, t, B, n + step);
+            a.put(g, t, factor, hs, lds);
+            b.put(g, t, factor, hs, lds);
+        } else
+            a.put(g, t, factor, hs, lds);
+    }
+};
+
+// rows without an adapter: the base, or nothing; of / splits of the work, by a workgroup
+__device__ __forceinline__ void put_base(const AdapterArgs &g, const Tile &t, int of, int splits)
+{
+    if (of == 0)
+        for (int e = threadIdx.x; e < t.rows * g.R; e += blockDim.x) g.h[(int64_t)t.row0 * g.R + e] = 0.f;
+    if (g.base == g.y) return;
+    for (int e = of * blockDim.x + threadIdx.x; e < t.rows * (g.N / 8); e += splits * blockDim.x) {
+        const int64_t r = t.row0 + e / (g.N / 8);
+        const int c = 8 * (e % (g.N / 8));
+        *reinterpret_cast<half8_t *>(g.y + r * g.ldy + c) = g.base ? load8(g.base + r * g.ldb + c) : zero8();
+    }
+}
+
+// Unit and split of a workgroup: the splits of a unit 8 apart, on one XCD, as they read the same
+__device__ __forceinline__ int unit_and_split(const AdapterArgs &g, int *split)
+{
+    const int group = blockIdx.x / (8 * g.splits), left = min(8, (int)g.units.count - 8 * group);
+    const int in = (int)blockIdx.x - 8 * group * g.splits;
+    *split = in / left;
+    return 8 * group + in % left;
+}
+
+// Few rows: a workgroup to 16 rows of a sequence and 1 / splits of the columns of y; h is formed by each of them.
+constexpr int few_waves(int RT) { return RT <= 2 ? 16 : 8; }      // (the registers of more leave room for 8)
+template <int RT, bool BASE>
+__global__ void __launch_bounds__(64 * few_waves(RT)) few_kernel(AdapterArgs g)
+{
+    constexpr int W = few_waves(RT), C = 16 * RT;
+    typedef TileH<RT, 1, W, false> H;
+    typedef Wave<RT, 1, BASE> Y;
+    typedef Terms<RT> Two;
+    constexpr int kLds = std::max(std::max(W * H::kLds, 2 * W * kTile * C), W * Y::C::kLds);
+    __shared__ __attribute__((aligned(16))) half_t lds[kLds], hs[kTile * Two::kPitch];
+    __shared__ int largest[kTile];
+    if ((int)blockIdx.x >= (int)g.units.count * g.splits) return look_over(g);
+    int split;
+    const int u = unit_and_split(g, &split);
+    const Tile t = find_tile(g, u, kTile);
+    if (t.rows == 0) return;
+    if (t.a < 0) return put_base(g, t, split, g.splits);
+    const float scale = g.scale[t.a];
+    // (the first columns' operands are on their way before h is there)
+    Y y(g, t, split * W + wave_id(), W * g.splits);
+    H h(g.x + t.row0 * g.ldx, g.ldx, t.rows, g.K, g.A + (int64_t)t.a * g.R * g.K, g.R, lds + wave_id() * H::kLds);
+    h.run(0, (g.K + 31) / 32);
+    Two::clear(hs, kTile);
     if (threadIdx.x < kTile) largest[threadIdx.x] = 0;
-    float sum[(RT + 1) / 2];
-    join_h<RT, W>(red, acc, [&](int i, int r, int c, float s) __attribute__((always_inline)) {
+    float sum[H::kItems];
+    h.join(reinterpret_cast<float *>(lds), [&](int i, int r, int c, float s) __attribute__((always_inline)) {
         sum[i] = s;
-        if (c >= R) return;
+        if (c >= g.R) return;
         atomicMax(largest + r, finite_bits(s));
-        if (split == 0 && r < t.rows) g.h[(int64_t)(t.row0 + r) * R + c] = s;
+        if (split == 0 && r < t.rows) g.h[(int64_t)(t.row0 + r) * g.R + c] = s;
     });
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < (RT + 1) / 2; i++) {
+    for (int i = 0; i < H::kItems; i++) {
         const int e = threadIdx.x + 64 * W * i, r = e / C, c = e % C;
-        if (e < kTile * C && c < R) two_terms(sum[i] * two_to(-exponent(largest[r])), hs + r * HP + c, hs + r * HP + R + c);
+        if (e < kTile * C && c < g.R) Two::put(hs + r * Two::kPitch, c, sum[i] * two_to(-exponent(largest[r])));
     }
     __syncthreads();
-    const float up = two_to(exponent(largest[m]));
-    half8_t hf[RT];
+    y.run(scale, hs, largest, lds + wave_id() * Y::C::kLds);
+}
+
+// Many rows, h first: 16 TB rows of a sequence and 1 / splits of the contraction to a workgroup, sums to a plane of [splits][T, R]
+constexpr int h_blocks(int) { return 2; }
+template <int RT, int TB>
+__global__ void __launch_bounds__(512) h_kernel(AdapterArgs g, float *planes)
+{
+    constexpr int WAVES = 8;
+    typedef TileH<RT, TB, WAVES, false> H;
+    __shared__ __attribute__((aligned(16))) half_t lds[std::max(WAVES * H::kLds, 2 * WAVES * 16 * TB * 16 * RT)];
+    if ((int)blockIdx.x >= (int)g.units.count * g.splits) return look_over(g);
+    int split;
+    const int u = unit_and_split(g, &split);
+    const Tile t = find_tile(g, u, 16 * TB);
+    if (t.rows == 0 || t.a < 0) return;
+    H h(g.x + t.row0 * g.ldx, g.ldx, t.rows, g.K, g.A + (int64_t)t.a * g.R * g.K, g.R, lds + wave_id() * H::kLds);
+    const int steps = (g.K + 31) / 32;
+    h.run(steps * split / g.splits, steps * (split + 1) / g.splits);
+    h.join(reinterpret_cast<float *>(lds), [&](int, int r, int c, float s) __attribute__((always_inline)) {
+        if (c < g.R && r < t.rows) planes[((int64_t)split * g.pb.T + t.row0 + r) * g.R + c] = s;
+    });
+}
+
+// .. then y: 64 rows and 1 / splits of the columns to a workgroup
+constexpr int kRows = 64;
+template <int RT, bool BASE>
+__global__ void __launch_bounds__(512) y_kernel(AdapterArgs g, const float *planes, int count)
+{
+    constexpr int W = 8, NI = (RT + 1) / 2;
+    typedef Terms<RT> Two;
+    typedef Wave<RT, kRows / 16, BASE> Y;
+    __shared__ __attribute__((aligned(16))) half_t hs[kRows * Two::kPitch], lds[W * Y::C::kLds];
+    __shared__ int largest[kRows];
+    int split;
+    const int u = unit_and_split(g, &split);
+    const Tile t = find_tile(g, u, kRows);
+    if (t.rows == 0) return;
+    if (t.a < 0) return put_base(g, t, split, g.splits);
+    const float scale = g.scale[t.a];
+    const int R = g.R;
+    Y y(g, t, split * W + wave_id(), W * g.splits);
+    Two::clear(hs, kRows);
+    if (threadIdx.x < kRows) largest[threadIdx.x] = 0;
+    float4_t v[NI];
 #pragma unroll
-    for (int i = 0; i < RT; i++) hf[i] = load8(hs + m * HP + 32 * i + 8 * q4);
-    // a wave to 64 columns: rows of B in an order that leaves a lane 16 columns of its row side by side
-    const half_t *B = g.B + (int64_t)t.a * N * R;
-    for (int n0 = 64 * (split * W + wave); n0 < N; n0 += 64 * W * g.splits) {
-        float4_t o[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            o[j] = zero4();
-            const half_t *row = B + (int64_t)min(n0 + 16 * (m >> 2) + 4 * j + (m & 3), N - 1) * R;
-#pragma unroll
-            for (int i = 0; i < RT; i++) {
-                const int kk = 32 * i + 8 * q4;
-                half8_t w = load8(row + (kk < R ? kk : kk < 2 * R ? kk - R : 0));
-                w = kk < 2 * R ? w : zero8();
-                o[j] = mfma(w, hf[i], o[j]);
-            }
-        }
-        if (m >= t.rows) continue;
-#pragma unroll
-        for (int p = 0; p < 2; p++) {
-            const int c = n0 + 16 * q4 + 8 * p;
-            if (c >= N) break;
-            half8_t v;
-            if (g.base) {
-                v = load8(g.base + (t.row0 + m) * g.ldb + c);
-#pragma unroll
-                for (int k = 0; k < 8; k++) v[k] = f2h(h2f(v[k]) + scale * (up * o[2 * p + k / 4][k % 4]));
-            } else
-#pragma unroll
-                for (int k = 0; k < 8; k++) v[k] = f2h(scale * (up * o[2 * p + k / 4][k % 4]));
-            *reinterpret_cast<half8_t *>(g.y + (t.row0 + m) * g.ldy + c) = v;
-        }
+    for (int i = 0; i < NI; i++) {
+        const int e = threadIdx.x + 64 * W * i, r = min(e / (R / 4), t.rows - 1), c = 4 * (e % (R / 4));
+        const int64_t at = (int64_t)(t.row0 + r) * R + c;
+        v[i] = *reinterpret_cast<const float4_t *>(planes + at);
+        for (int q = 1; q < count; q++) v[i] += *reinterpret_cast<const float4_t *>(planes + q * (int64_t)g.pb.T * R + at);
     }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+        const int e = threadIdx.x + 64 * W * i, r = e / (R / 4), c = 4 * (e % (R / 4));
+        if (r >= t.rows) break;
+        if (split == 0 && count > 1) *reinterpret_cast<float4_t *>(g.h + (int64_t)(t.row0 + r) * R + c) = v[i];
+        atomicMax(largest + r, max(max(finite_bits(v[i][0]), finite_bits(v[i][1])), max(finite_bits(v[i][2]), finite_bits(v[i][3]))));
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+        const int e = threadIdx.x + 64 * W * i, r = e / (R / 4), c = 4 * (e % (R / 4));
+        if (r >= t.rows) break;
+        const float own = two_to(-exponent(largest[r]));
+#pragma unroll
+        for (int k = 0; k < 4; k++) Two::put(hs + r * Two::kPitch, c + k, v[i][k] * own);
+    }
+    __syncthreads();
+    y.run(scale, hs, largest, lds + wave_id() * Y::C::kLds);
 }
 
 // ---------------------------------------------------------------- gradients
-constexpr int kRows = 64, kCols = 128;         // rows and columns of a step of the second kernel
+constexpr int kCols = 128;                     // (and kRows rows) of a step of the second kernel
 
 struct GradArgs {
     AdapterArgs f;                             // x, A, B, h as in the forward pass; y, ldy: dx; base: what it is added to, or null
@@ -327,14 +590,14 @@ __device__ void plan(const GradArgs &d, int *counts)
 template <int RT>
 __global__ void __launch_bounds__(512) dh_kernel(GradArgs d)
 {
-    constexpr int W = 8, C = 16 * RT;
-    __shared__ __attribute__((aligned(16))) float red[W * kTile * C];
-    __shared__ __attribute__((aligned(16))) half_t lds[W][32 * (C + 8)];
+    constexpr int W = 8;
+    typedef TileH<RT, 1, W, true> H;
+    __shared__ __attribute__((aligned(16))) half_t lds[std::max(W * H::kLds, 2 * W * kTile * 16 * RT)];
     __shared__ int counts[kMaxAdapters + 1];
     const AdapterArgs &g = d.f;
     if (blockIdx.x == 0) return plan(d, counts);
-    const int64_t u = (int64_t)blockIdx.x - 1;
-    if (u >= g.units.count) return look_over(g);
+    const int u = (int)blockIdx.x - 1;
+    if (u >= (int)g.units.count) return look_over(g);
     const Tile t = find_tile(g, u, kTile);
     if (t.rows == 0) return;
     const int R = g.R, K = g.K;
@@ -344,9 +607,9 @@ __global__ void __launch_bounds__(512) dh_kernel(GradArgs d)
             *reinterpret_cast<half8_t *>(g.y + (int64_t)(t.row0 + e / (K / 8)) * g.ldy + 8 * (e % (K / 8))) = zero8();
         return;
     }
-    float4_t acc[RT];
-    tile_h<RT, W, true>(d.dy + t.row0 * d.lddy, d.lddy, t.rows, g.N, g.B + (int64_t)t.a * g.N * R, R, lds[threadIdx.x >> 6], acc);
-    join_h<RT, W>(red, acc, [&](int, int r, int c, float s) __attribute__((always_inline)) {
+    H h(d.dy + t.row0 * d.lddy, d.lddy, t.rows, g.N, g.B + (int64_t)t.a * g.N * R, R, lds + wave_id() * H::kLds);
+    h.run(0, (g.N + 31) / 32);
+    h.join(reinterpret_cast<float *>(lds), [&](int, int r, int c, float s) __attribute__((always_inline)) {
         if (c < R && r < t.rows) d.dh[(int64_t)(t.row0 + r) * R + c] = s;
     });
 }
@@ -354,57 +617,82 @@ __global__ void __launch_bounds__(512) dh_kernel(GradArgs d)
 // units of adapter a begin at begin[a] / per + a
 __device__ __forceinline__ int64_t unit_of(const GradArgs &d, int a) { return (int64_t)(d.begin[a] / d.per) + a; }
 
-// A block of an adapter's rows and 128 columns: of x, for dx and the block's part of dA, or of dy, for its part of dB.
+// A block of an adapter's rows and 128 columns: of x, for dx and the block's part of dA, or of dy, for its part of dB.  64 rows at a time
+// in LDS, the next ones under way.
+constexpr int kMostRows = 512;                 // of a block
 template <int RT>
 __global__ void __launch_bounds__(256) grad_kernel(GradArgs d)
 {
-    constexpr int HP = 32 * RT + 8, XP = kCols + 16;
-    __shared__ __attribute__((aligned(16))) half_t xs[kRows * XP], hs[kRows * HP], hr[kRows * HP], as[16 * RT * XP];
-    __shared__ int largest[2][kRows];
+    typedef Terms<RT> Two;
+    constexpr int HP = Two::kPitch, XP = kCols + 16, NX = kRows * kCols / 8 / 256;
+    __shared__ __attribute__((aligned(16))) half_t xs[kRows * XP], hs[kRows * HP], hr[kRows * HP], as[16 * RT * XP], tiles[4][kTileHalves];
+    __shared__ int largest[2][kRows], rows[kMostRows];
     const AdapterArgs &g = d.f;
     const int R = g.R, K = g.K, N = g.N, kchunks = (K + kCols - 1) / kCols, chunks = kchunks + (N + kCols - 1) / kCols;
-    const int64_t u = blockIdx.x / chunks;
-    const int chunk = (int)(blockIdx.x % chunks);
+    const int u = (int)blockIdx.x / chunks, chunk = (int)blockIdx.x - u * chunks;
     const bool of_x = chunk < kchunks;
     const int c0 = kCols * (of_x ? chunk : chunk - kchunks), width = of_x ? K : N;
     // (unit 0 is adapter 0's: one more than the adapters that begin behind it)
-    const int a = count_below(g.n - 1, u, [&](int i) { return unit_of(d, i); });
+    const int a = __builtin_amdgcn_readfirstlane(count_below(g.n - 1, u, [&](int i) { return unit_of(d, i); }));
     const int first = d.begin[a] + (int)(u - unit_of(d, a)) * d.per, count = min(d.per, d.begin[a + 1] - first);
     if (count <= 0) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, q4 = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = wave_id(), m = lane & 15, q4 = lane >> 4;
     const float scale = g.scale[a];
     const half_t *src = of_x ? g.x : d.dy;
     const int64_t ld = of_x ? g.ldx : d.lddy;
     const float *hsrc = of_x ? d.dh : g.h;
+    for (int e = threadIdx.x; e < count; e += 256) rows[e] = d.rows[first + e];
     if (of_x)
         for (int e = threadIdx.x; e < 16 * RT * (kCols / 8); e += 256) {
             const int r = e / (kCols / 8), c = 8 * (e % (kCols / 8));
-            *reinterpret_cast<half8_t *>(as + r * XP + c) = r < R && c0 + c < K ? load8(g.A + ((int64_t)a * R + r) * K + c0 + c) : zero8();
+            const half8_t w = load8(g.A + ((int64_t)a * R + min(r, R - 1)) * K + min(c0 + c, K - 8));
+            *reinterpret_cast<half8_t *>(as + r * XP + c) = r < R && c0 + c < K ? w : zero8();
         }
-    for (int e = threadIdx.x; e < kRows * HP / 8; e += 256)
-        *reinterpret_cast<half8_t *>(hs + 8 * e) = *reinterpret_cast<half8_t *>(hr + 8 * e) = zero8();
+    Two::clear(hs, kRows);
+    Two::clear(hr, kRows);
     if (threadIdx.x < kRows) largest[0][threadIdx.x] = 0;
+    __syncthreads();
+    half8_t x[NX];
+    float4_t v[RT];
+    const int xc = 8 * (threadIdx.x % (kCols / 8)), xr = threadIdx.x / (kCols / 8);
+    auto load = [&](int r0) __attribute__((always_inline)) {      // (rows that there are not: others)
+#pragma unroll
+        for (int i = 0; i < NX; i++) x[i] = load8(src + (int64_t)rows[min(r0 + xr + 256 / (kCols / 8) * i, count - 1)] * ld + min(c0 + xc, width - 8));
+#pragma unroll
+        for (int i = 0; i < RT; i++) {
+            const int e = threadIdx.x + 256 * i, r = e / (R / 4), c = 4 * (e % (R / 4));
+            v[i] = *reinterpret_cast<const float4_t *>(hsrc + (int64_t)rows[min(r0 + r, count - 1)] * R + c);
+        }
+    };
+    load(0);
+    // A of 32 columns a wave, 8 of them side by side in a lane
+    half8_t w[Two::kN][2];
+#pragma unroll
+    for (int i = 0; i < Two::kN; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const half_t *q = as + (Two::of(i, q4) + (m >> 2)) * XP + 32 * wave + 8 * (m & 3) + 4 * j;
+            w[i][j] = both(read_tr(q), read_tr(q + 4 * XP));
+        }
     float4_t acc[RT][2];
 #pragma unroll
     for (int i = 0; i < RT; i++) acc[i][0] = acc[i][1] = zero4();
     int top = -126;                            // exponent that the sums are scaled by
     for (int r0 = 0, turn = 0; r0 < count; r0 += kRows, turn ^= 1) {
-        __syncthreads();
-        if (threadIdx.x < kRows) largest[turn ^ 1][threadIdx.x] = 0;
-        for (int e = threadIdx.x; e < kRows * (kCols / 8); e += 256) {
-            const int r = e / (kCols / 8), c = 8 * (e % (kCols / 8));
-            *reinterpret_cast<half8_t *>(xs + r * XP + c) =
-                r0 + r < count && c0 + c < width ? load8(src + (int64_t)d.rows[first + r0 + r] * ld + c0 + c) : zero8();
+        const int left = count - r0;
+#pragma unroll
+        for (int i = 0; i < NX; i++) {
+            const int r = xr + 256 / (kCols / 8) * i;
+            *reinterpret_cast<half8_t *>(xs + r * XP + xc) = r < left && c0 + xc < width ? x[i] : zero8();
         }
-        float4_t v[RT];
 #pragma unroll
         for (int i = 0; i < RT; i++) {
-            const int e = threadIdx.x + 256 * i, r = e / (R / 4), c = 4 * (e % (R / 4));
-            if (r >= kRows) break;
-            v[i] = r0 + r < count ? *reinterpret_cast<const float4_t *>(hsrc + (int64_t)d.rows[first + r0 + r] * R + c) : zero4();
-            atomicMax(&largest[turn][r], max(max(finite_bits(v[i][0]), finite_bits(v[i][1])), max(finite_bits(v[i][2]), finite_bits(v[i][3]))));
+            const int r = (threadIdx.x + 256 * i) / (R / 4);
+            if (r >= left) v[i] = zero4();
+            if (r < kRows) atomicMax(&largest[turn][r], max(max(finite_bits(v[i][0]), finite_bits(v[i][1])), max(finite_bits(v[i][2]), finite_bits(v[i][3]))));
         }
         __syncthreads();
+        if (threadIdx.x < kRows) largest[turn ^ 1][threadIdx.x] = 0;
         const int now = max(top, exponent(__builtin_bit_cast(int, wave_max(__builtin_bit_cast(float, largest[turn][lane])))));
         const float less = two_to(max(top - now, -126));
         top = now;
@@ -417,10 +705,11 @@ __global__ void __launch_bounds__(256) grad_kernel(GradArgs d)
             const float all = two_to(-top), own = two_to(-exponent(largest[turn][r]));
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                two_terms(v[i][k] * all, hs + r * HP + c + k, hs + r * HP + R + c + k);
-                if (of_x) two_terms(v[i][k] * own, hr + r * HP + c + k, hr + r * HP + R + c + k);
+                Two::put(hs + r * HP, c + k, v[i][k] * all);
+                if (of_x) Two::put(hr + r * HP, c + k, v[i][k] * own);
             }
         }
+        load(r0 + kRows);
         __syncthreads();
         // the sums over rows: step s has rows 32 s + 4 q4 + 0 .. 3 and those 16 further, in both operands
 #pragma unroll
@@ -436,46 +725,37 @@ __global__ void __launch_bounds__(256) grad_kernel(GradArgs d)
             for (int i = 0; i < RT; i++)
 #pragma unroll
                 for (int p = 0; p < 2; p++) {
-                    const half_t *q = hs + row * HP + p * R + 16 * i + 4 * (m & 3);
+                    const half_t *q = hs + row * HP + p * Two::kLo + 16 * i + 4 * (m & 3);
                     const half8_t hf = both(read_tr(q), read_tr(q + 16 * HP));
 #pragma unroll
                     for (int c = 0; c < 2; c++) acc[i][c] = of_x ? mfma(hf, xf[c], acc[i][c]) : mfma(xf[c], hf, acc[i][c]);
                 }
         }
-        if (!of_x) continue;
-        // dx of 32 columns a wave, 8 of them side by side in a lane
+        if (of_x)
 #pragma unroll
-        for (int t = 0; t < kRows / 16; t++) {
-            float4_t o[2] = {zero4(), zero4()};
+            for (int t = 0; t < kRows / 16; t++) {
+                if (16 * t >= left) break;
+                float4_t o[2] = {zero4(), zero4()};
 #pragma unroll
-            for (int i = 0; i < RT; i++) {
-                const int kk = 32 * i + 8 * q4, r = kk < R ? kk : kk < 2 * R ? kk - R : 0;
-                const half8_t hf = load8(hr + (16 * t + m) * HP + kk);
+                for (int i = 0; i < Two::kN; i++)
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const half_t *q = as + (r + (m >> 2)) * XP + 32 * wave + 8 * (m & 3) + 4 * j;
-                    half8_t w = both(read_tr(q), read_tr(q + 4 * XP));
-                    w = kk < 2 * R ? w : zero8();
-                    o[j] = mfma(w, hf, o[j]);
-                }
+                    for (int p = 0; p < Two::kM; p++) {
+                        const half8_t hf = load8(hr + (16 * t + m) * HP + Two::column(i, p, q4));
+#pragma unroll
+                        for (int j = 0; j < 2; j++) o[j] = mfma(w[i][j], hf, o[j]);
+                    }
+                const float factor = factor_of(scale, largest[turn][16 * t + m]);
+                const int r = 16 * t + mem_row(), c = c0 + 32 * wave + mem_col();
+                const int64_t row = rows[r0 + min(r, left - 1)];
+                half8_t y;
+                if (g.base) y = turned<true>(tiles[wave], load8(g.base + row * g.ldb + min(c, K - 8)), o, factor);
+                else y = turned<false>(tiles[wave], zero8(), o, factor);
+                if (r < left && c < K) *reinterpret_cast<half8_t *>(g.y + row * g.ldy + c) = y;
             }
-            const int r = r0 + 16 * t + m, c = c0 + 32 * wave + 8 * q4;
-            if (r >= count || c >= K) continue;
-            const int64_t row = d.rows[first + r];
-            const float up = two_to(exponent(largest[turn][16 * t + m]));
-            half8_t v;
-            if (g.base) {
-                v = load8(g.base + row * g.ldb + c);
-#pragma unroll
-                for (int k = 0; k < 8; k++) v[k] = f2h(h2f(v[k]) + scale * (up * o[k / 4][k % 4]));
-            } else
-#pragma unroll
-                for (int k = 0; k < 8; k++) v[k] = f2h(scale * (up * o[k / 4][k % 4]));
-            *reinterpret_cast<half8_t *>(g.y + row * g.ldy + c) = v;
-        }
+        __syncthreads();
     }
     const float up = two_to(top);
-    float *part = d.parts + u * R * (K + N);
+    float *part = d.parts + (int64_t)u * R * (K + N);
 #pragma unroll
     for (int i = 0; i < RT; i++)
 #pragma unroll
@@ -555,7 +835,7 @@ int64_t block_rows(int64_t T, int64_t K, int64_t N)
 {
     const int64_t chunks = (K + kCols - 1) / kCols + (N + kCols - 1) / kCols, steps = (T + kRows - 1) / kRows;
     int64_t per = steps * chunks / 768;
-    per = per < 1 ? 1 : per > 64 ? 64 : per;
+    per = per < 1 ? 1 : per > kMostRows / kRows ? kMostRows / kRows : per;
     return per * kRows;
 }
 
@@ -577,11 +857,44 @@ Workspace workspace(int64_t T, int64_t K, int64_t N, int64_t R, int64_t n)
     return w;
 }
 
+// How the forward pass is cut.  Few rows: one launch, whose workgroups each form the h that they need; columns are split until the device is
+// full.  Many: h first.
+struct ForwardPlan {
+    bool many;
+    int splits, planes;
+    Units h_units, y_units;
+    size_t bytes;
+};
+ForwardPlan forward_plan(int64_t T, int64_t S, int64_t K, int64_t N, int64_t R, int64_t max_new)
+{
+    ForwardPlan w{};
+    auto units = [&](int64_t rows) { return make_units(T, S, rows, 1, 1, (max_new + rows - 1) / rows); };
+    auto fill = [](int64_t target, int64_t count, int64_t most) { return (int)std::max<int64_t>(1, std::min(target / count, most)); };
+    const int64_t cus = device_cus();
+    const int rank = R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8;
+    w.many = max_new > 16;
+    if (!w.many) {
+        w.splits = fill(cus, units(kTile).count, (N + 32 * few_waves(rank) - 1) / (32 * few_waves(rank)));
+        return w;
+    }
+    w.h_units = units(16 * h_blocks(rank));
+    w.y_units = units(kRows);
+    w.planes = fill(cus, w.h_units.count, std::min<int64_t>(8, (K + 255) / 256));
+    w.splits = fill(2 * cus, w.y_units.count, (N + 255) / 256);
+    w.bytes = w.planes > 1 ? (size_t)w.planes * T * R * 4 : 0;
+    return w;
+}
+
 }  // namespace
+
+CACTI_API size_t cacti_hip_adapter_fwd_workspace(int64_t T, int64_t S, int64_t K, int64_t N, int64_t R, int64_t max_new)
+{
+    return T > 0 && S > 0 && K > 0 && N > 0 && R > 0 && max_new > 0 ? forward_plan(T, S, K, N, R, max_new < T ? max_new : T).bytes : 0;
+}
 
 CACTI_API int cacti_hip_adapter_fwd(int64_t T, int64_t S, int64_t K, int64_t N, int64_t R, int64_t n, int64_t max_new, const void *x, int64_t ldx,
                                     const void *A, const void *B, const void *starts, const void *ids, const void *scale, const void *base,
-                                    int64_t ldb, void *y, int64_t ldy, void *h, void *status, void *stream)
+                                    int64_t ldb, void *y, int64_t ldy, void *h, void *ws, size_t ws_bytes, void *status, void *stream)
 {
     AdapterArgs g;
     const int rc = check("adapter_fwd", T, S, K, N, R, n, max_new, x, ldx, A, B, starts, ids, scale, status, &g);
@@ -596,12 +909,37 @@ CACTI_API int cacti_hip_adapter_fwd(int64_t T, int64_t S, int64_t K, int64_t N, 
     g.base = (const half_t *)base, g.ldb = ldb;
     g.y = (half_t *)y, g.ldy = ldy;
     g.h = (float *)h;
-    // (columns are split until the device is full: 512 of them are an iteration of a workgroup)
-    const int64_t most = (N + 511) / 512, want = (device_cus() + g.units.count - 1) / g.units.count;
-    g.splits = (int)(want < 1 ? 1 : want < most ? want : most);
-    const int64_t blocks = g.units.count * g.splits + (status ? 1 : 0);
-    CACTI_REQUIRE(blocks <= INT32_MAX, CACTI_E_NOTIMPL, "adapter_fwd: too many tiles");
-#define LAUNCH(RT) hipLaunchKernelGGL((adapter_kernel<RT>), dim3((unsigned)blocks), dim3(512), 0, (hipStream_t)stream, g)
+    const ForwardPlan w = forward_plan(T, S, K, N, R, g.max_new);
+    CACTI_REQUIRE(ws_bytes >= w.bytes && (ws || !w.bytes) && aligned(ws, 16), CACTI_E_INVALID, "adapter_fwd: workspace of %zu bytes, %zu needed, 16-byte aligned",
+                  ws_bytes, w.bytes);
+    hipStream_t st = (hipStream_t)stream;
+    if (!w.many) {
+        g.splits = w.splits;
+        const int64_t blocks = g.units.count * g.splits + (status ? 1 : 0);
+        CACTI_REQUIRE(blocks <= INT32_MAX, CACTI_E_NOTIMPL, "adapter_fwd: too many tiles");
+#define LAUNCH(RT)                                                                                                       \
+    do {                                                                                                                 \
+        if (base) hipLaunchKernelGGL((few_kernel<RT, true>), dim3((unsigned)blocks), dim3(64 * few_waves(RT)), 0, st, g); \
+        else hipLaunchKernelGGL((few_kernel<RT, false>), dim3((unsigned)blocks), dim3(64 * few_waves(RT)), 0, st, g);     \
+    } while (0)
+        CACTI_BY_RANK(R, LAUNCH);
+#undef LAUNCH
+        return launch_status("adapter_fwd");
+    }
+    float *planes = w.planes > 1 ? (float *)ws : g.h;
+    AdapterArgs first = g;
+    first.units = w.h_units;
+    first.splits = w.planes;
+    g.units = w.y_units;
+    g.splits = w.splits;
+    const int64_t blocks1 = first.units.count * first.splits + (status ? 1 : 0), blocks2 = g.units.count * g.splits;
+    CACTI_REQUIRE(blocks1 <= INT32_MAX && blocks2 <= INT32_MAX, CACTI_E_NOTIMPL, "adapter_fwd: too many tiles");
+#define LAUNCH(RT)                                                                                                       \
+    do {                                                                                                                 \
+        hipLaunchKernelGGL((h_kernel<RT, h_blocks(RT)>), dim3((unsigned)blocks1), dim3(512), 0, st, first, planes);                 \
+        if (base) hipLaunchKernelGGL((y_kernel<RT, true>), dim3((unsigned)blocks2), dim3(512), 0, st, g, (const float *)planes, w.planes); \
+        else hipLaunchKernelGGL((y_kernel<RT, false>), dim3((unsigned)blocks2), dim3(512), 0, st, g, (const float *)planes, w.planes);     \
+    } while (0)
     CACTI_BY_RANK(R, LAUNCH);
 #undef LAUNCH
     return launch_status("adapter_fwd");

@@ -128,7 +128,8 @@ SIGNATURES = {
     "cacti_hip_token_logp_bwd": (ci, [i64, i64, vp, i64, vp, vp, vp, C.c_double, vp, i64, ci, vp]),
     "cacti_hip_policy_loss": (ci, [i64, i64, vp, i64] + [vp] * 6 + [C.c_double] * 4 + [vp, vp, vp, i64, ci, vp, vp]),
     "cacti_hip_preference_loss": (ci, [i64, i64] + [vp] * 5 + [C.c_double, C.c_double, ci, vp, vp, vp, vp, vp]),
-    "cacti_hip_adapter_fwd": (ci, [i64] * 7 + [vp, i64] + [vp] * 6 + [i64, vp, i64, vp, vp, vp]),
+    "cacti_hip_adapter_fwd_workspace": (sz, [i64] * 6),
+    "cacti_hip_adapter_fwd": (ci, [i64] * 7 + [vp, i64] + [vp] * 6 + [i64, vp, i64, vp, vp, sz, vp, vp]),
     "cacti_hip_adapter_bwd_workspace": (sz, [i64] * 5),
     "cacti_hip_adapter_bwd": (ci, [i64] * 7 + [vp, i64] + [vp] * 7 + [i64, vp, i64, ci, vp, ci, vp, ci, vp, sz, vp, vp]),
     "cacti_hip_paged_fork": (ci, [i64] * 4 + [vp, vp, i64, vp, vp, vp, i64, vp, vp, vp]),

@@ -823,11 +823,15 @@ PyObject *adapter_fwd(PyObject *const *o)
     }
     const Result h = new_f32({T, g.R}, g.x.t);
     void *status = on.pointer(o[9], at::kInt, 1), *st = on.stream();
-    if (g.some())
+    if (g.some()) {
+        const size_t bytes = cacti_hip_adapter_fwd_workspace(T, g.S, g.K, g.N, g.R, g.max_new);
+        at::Tensor ws;
+        if (bytes) ws = empty({(int64_t)bytes}, g.x.t, at::kByte);
         run([&] {
             return cacti_hip_adapter_fwd(T, g.S, g.K, g.N, g.R, g.n, g.max_new, g.x.t.data_ptr(), g.x.ld, g.A.data_ptr(), g.B.data_ptr(),
-                                         g.starts.data_ptr(), g.ids, g.scale, base, ldb, y.ptr(), ldy, h.ptr(), status, st);
+                                         g.starts.data_ptr(), g.ids, g.scale, base, ldb, y.ptr(), ldy, h.ptr(), bytes ? ws.data_ptr() : nullptr, bytes, status, st);
         });
+    }
     return take2(y, h);
 }
 

@@ -553,10 +553,11 @@ int cacti_hip_preference_loss(int64_t N, int64_t pairs, const void *logp, const 
  * meet the second product as two f16 terms, 22 bits, 2^-25 of the largest of their row (for dA and dB: of the adapter's rows).  K, N, R multiples of 8, R <= 128; rows of x, y, base,
  * dy, dx of pitches that are multiples of 8; all 16-byte aligned; n <= 1024.  max_new: no sequence has more rows.  status [1] i32 or NULL: 1 + s
  * where the rows of sequence s are not there or more than max_new (it has none then), or its id is neither -1 nor below n (it has no
- * adapter then); the caller clears it.  workspace: cacti_hip_adapter_bwd_workspace bytes, 16-byte aligned, contents undefined on return. */
+ * adapter then); the caller clears it.  workspace: cacti_hip_adapter_{fwd,bwd}_workspace bytes (0: NULL will do), 16-byte aligned, contents undefined on return. */
+size_t cacti_hip_adapter_fwd_workspace(int64_t T, int64_t S, int64_t K, int64_t N, int64_t R, int64_t max_new);
 int cacti_hip_adapter_fwd(int64_t T, int64_t S, int64_t K, int64_t N, int64_t R, int64_t n, int64_t max_new, const void *x, int64_t ldx,
                           const void *A, const void *B, const void *starts, const void *ids, const void *scale, const void *base,
-                          int64_t ldb, void *y, int64_t ldy, void *h, void *status, void *stream);
+                          int64_t ldb, void *y, int64_t ldy, void *h, void *workspace, size_t workspace_bytes, void *status, void *stream);
 size_t cacti_hip_adapter_bwd_workspace(int64_t T, int64_t K, int64_t N, int64_t R, int64_t n);
 int cacti_hip_adapter_bwd(int64_t T, int64_t S, int64_t K, int64_t N, int64_t R, int64_t n, int64_t max_new, const void *x, int64_t ldx,
                           const void *A, const void *B, const void *starts, const void *ids, const void *scale, const void *h,

@@ -13,7 +13,7 @@ from cacti_amd import ffi
 GPU = pytest.mark.gpu
 P0, STEP = 0x100000, 0x10000
 FWD = dict(T=4, S=2, K=64, N=64, R=16, n=2, max_new=4, x=P0, ldx=64, A=P0 + STEP, B=P0 + 2 * STEP, starts=64, ids=64, scale=64, base=P0 + 3 * STEP, ldb=64,
-           y=P0 + 4 * STEP, ldy=64, h=P0 + 5 * STEP, status=None, stream=None)
+           y=P0 + 4 * STEP, ldy=64, h=P0 + 5 * STEP, ws=None, ws_bytes=0, status=None, stream=None)
 BWD = dict(T=4, S=2, K=64, N=64, R=16, n=2, max_new=4, x=P0, ldx=64, A=P0 + STEP, B=P0 + 2 * STEP, starts=64, ids=64, scale=64, h=P0 + 3 * STEP,
            dy=P0 + 4 * STEP, lddy=64, dx=P0 + 5 * STEP, lddx=64, dx_acc=0, dA=P0 + 6 * STEP, dA_acc=0, dB=P0 + 7 * STEP, dB_acc=0, ws=P0 + 8 * STEP,
            ws_bytes=1 << 30, status=None, stream=None)
@@ -24,7 +24,8 @@ COMMON = [(dict(T=0), "empty"), (dict(S=0), "empty"), (dict(K=0), "empty"), (dic
           (dict(A=P0 + STEP + 2), "aligned"), (dict(starts=66), "aligned"), (dict(status=66), "aligned")]
 REFUSED = [("cacti_hip_adapter_fwd", FWD, c) for c in COMMON + [
     (dict(y=None), "null"), (dict(h=None), "null"), (dict(ldy=56), "pitch"), (dict(ldb=66), "multiple"), (dict(base=P0 + 3 * STEP + 8), "aligned"),
-    (dict(y=P0), "shares"), (dict(y=P0 + 128), "shares"), (dict(y=P0 + 3 * STEP, ldy=72), "place"), (dict(y=P0 + 3 * STEP + 16), "place")]] + \
+    (dict(y=P0), "shares"), (dict(y=P0 + 128), "shares"), (dict(y=P0 + 3 * STEP, ldy=72), "place"), (dict(y=P0 + 3 * STEP + 16), "place"),
+    (dict(T=100, max_new=100, K=1024, ldx=1024, x=1 << 30), "workspace")]] + \
           [("cacti_hip_adapter_bwd", BWD, c) for c in COMMON + [
               (dict(h=None), "null"), (dict(dy=None), "null"), (dict(dx=None), "null"), (dict(dA=None), "null"), (dict(dB=None), "null"), (dict(ws=None), "null"),
               (dict(lddy=56), "pitch"), (dict(lddx=68), "multiple"), (dict(dx=P0), "shares"), (dict(dx=P0 + 4 * STEP + 16), "shares"),
