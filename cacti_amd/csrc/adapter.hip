@@ -75,8 +75,10 @@ __device__ __forceinline__ float4_t zero4() { return float4_t{0.f, 0.f, 0.f, 0.f
 __device__ __forceinline__ half8_t load8(const half_t *p) { return *reinterpret_cast<const half8_t *>(p); }
 __device__ __forceinline__ float4_t mfma(half8_t a, half8_t b, float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
-// Exponent of the largest of finite values, whose bits are given, and a power of two
-__device__ __forceinline__ int exponent(int bits) { return min(max((bits >> 23) - 127, -126), 126); }
+// Values are scaled so that the largest is in 2^kTop .. 2^(kTop + 1): exponent that the largest of finite values, whose bits are given, has
+// beyond that; a power of two
+constexpr int kTop = 10;
+__device__ __forceinline__ int exponent(int bits) { return min(max((bits >> 23) - 127, -100), 126) - kTop; }
 __device__ __forceinline__ float two_to(int e) { return __builtin_bit_cast(float, (e + 127) << 23); }
 __device__ __forceinline__ int finite_bits(float v)
 {
@@ -271,9 +273,9 @@ struct Terms {
 
 // Scale of a row's results: the adapter's and what its h was scaled by.  (Within fp32's range, so that it does not make a 0 a NaN: what it is
 // multiplied with is 0 or no less than 2^-48, which f16 takes for infinite either way.)
-__device__ __forceinline__ float factor_of(float scale, int bits)
+__device__ __forceinline__ float factor_of(float scale, int exp)
 {
-    const float f = scale * two_to(exponent(bits));
+    const float f = scale * two_to(max(exp, -126));
     return fabsf(f) < INFINITY || fabsf(scale) == INFINITY || scale != scale ? f : copysignf(3.4028234664e38f, f);
 }
 
@@ -374,7 +376,7 @@ struct Wave {
         if (n >= g.N) return;
         float factor[TB];
 #pragma unroll
-        for (int i = 0; i < TB; i++) factor[i] = factor_of(scale, largest[16 * i + (threadIdx.x & 15)]);
+        for (int i = 0; i < TB; i++) factor[i] = factor_of(scale, exponent(largest[16 * i + (threadIdx.x & 15)]));
         for (; n + 2 * step < g.N; n += 2 * step) {
             b.load(g, t, B, n + step);
             a.put(g, t, factor, hs, lds);
@@ -531,7 +533,8 @@ struct GradArgs {
     AdapterArgs f;                             // x, A, B, h as in the forward pass; y, ldy: dx; base: what it is added to, or null
     const half_t *dy;
     int64_t lddy;
-    float *dh;                                 // [T, R], without the scale
+    half_t *terms[2];                          // of dh (without the scale) and h: rows of 32 RT, as in LDS, scaled by
+    int *exps[2];                              // powers of two of their own
     int *rows, *begin;                         // rows of adapter a: rows[begin[a]] .. rows[begin[a + 1] - 1]
     float *parts;                              // of dA [R, K] and dB [N, R], a block of rows each
     half_t *dA, *dB;
@@ -586,14 +589,15 @@ __device__ void plan(const GradArgs &d, int *counts)
     }
 }
 
-// dh of 16 rows of a sequence; dx of rows without an adapter.  The last two workgroups: the plan, and what does not fit.
+// The two terms of dh and h of 16 rows of a sequence; dx of rows without an adapter.  The first workgroup: the plan, the last: what does not fit.
 template <int RT>
 __global__ void __launch_bounds__(512) dh_kernel(GradArgs d)
 {
-    constexpr int W = 8;
+    constexpr int W = 8, C = 16 * RT;
     typedef TileH<RT, 1, W, true> H;
-    __shared__ __attribute__((aligned(16))) half_t lds[std::max(W * H::kLds, 2 * W * kTile * 16 * RT)];
-    __shared__ int counts[kMaxAdapters + 1];
+    typedef Terms<RT> Two;
+    __shared__ __attribute__((aligned(16))) half_t lds[std::max(W * H::kLds, 2 * W * kTile * C)], hs[kTile * Two::kPitch];
+    __shared__ int counts[kMaxAdapters + 1], largest[2][kTile];
     const AdapterArgs &g = d.f;
     if (blockIdx.x == 0) return plan(d, counts);
     const int u = (int)blockIdx.x - 1;
@@ -607,11 +611,36 @@ __global__ void __launch_bounds__(512) dh_kernel(GradArgs d)
             *reinterpret_cast<half8_t *>(g.y + (int64_t)(t.row0 + e / (K / 8)) * g.ldy + 8 * (e % (K / 8))) = zero8();
         return;
     }
+    float sum[2][H::kItems];
+#pragma unroll
+    for (int i = 0; i < H::kItems; i++) {
+        const int e = threadIdx.x + 64 * W * i, r = min(e / C, t.rows - 1), c = min(e % C, R - 1);
+        sum[1][i] = g.h[(int64_t)(t.row0 + r) * R + c];
+    }
     H h(d.dy + t.row0 * d.lddy, d.lddy, t.rows, g.N, g.B + (int64_t)t.a * g.N * R, R, lds + wave_id() * H::kLds);
     h.run(0, (g.N + 31) / 32);
-    h.join(reinterpret_cast<float *>(lds), [&](int, int r, int c, float s) __attribute__((always_inline)) {
-        if (c < R && r < t.rows) d.dh[(int64_t)(t.row0 + r) * R + c] = s;
+    if (threadIdx.x < 2 * kTile) largest[threadIdx.x / kTile][threadIdx.x % kTile] = 0;
+    h.join(reinterpret_cast<float *>(lds), [&](int i, int r, int c, float s) __attribute__((always_inline)) {
+        sum[0][i] = s;
+        if (c >= R) return;
+        atomicMax(&largest[0][r], finite_bits(s));
+        atomicMax(&largest[1][r], finite_bits(sum[1][i]));
     });
+#pragma unroll
+    for (int of = 0; of < 2; of++) {
+        __syncthreads();
+        Two::clear(hs, kTile);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < H::kItems; i++) {
+            const int e = threadIdx.x + 64 * W * i, r = e / C, c = e % C;
+            if (e < kTile * C && c < R) Two::put(hs + r * Two::kPitch, c, sum[of][i] * two_to(-exponent(largest[of][r])));
+        }
+        __syncthreads();
+        for (int e = threadIdx.x; e < t.rows * 4 * RT; e += 64 * W)
+            put8(d.terms[of] + ((int64_t)t.row0 * 4 * RT + e) * 8, load8(hs + e / (4 * RT) * Two::kPitch + 8 * (e % (4 * RT))));
+        if ((int)threadIdx.x < t.rows) d.exps[of][t.row0 + threadIdx.x] = exponent(largest[of][threadIdx.x]);
+    }
 }
 
 // units of adapter a begin at begin[a] / per + a
@@ -621,12 +650,14 @@ __device__ __forceinline__ int64_t unit_of(const GradArgs &d, int a) { return (i
 // in LDS, the next ones under way.
 constexpr int kMostRows = 512;                 // of a block
 template <int RT>
-__global__ void __launch_bounds__(256) grad_kernel(GradArgs d)
+__global__ void __launch_bounds__(256, RT == 8 ? 2 : 1) grad_kernel(GradArgs d)
 {
     typedef Terms<RT> Two;
     constexpr int HP = Two::kPitch, XP = kCols + 16, NX = kRows * kCols / 8 / 256;
-    __shared__ __attribute__((aligned(16))) half_t xs[kRows * XP], hs[kRows * HP], hr[kRows * HP], as[16 * RT * XP], tiles[4][kTileHalves];
-    __shared__ int largest[2][kRows], rows[kMostRows];
+    // (A is in registers before the first rows come)
+    __shared__ __attribute__((aligned(16))) half_t lds[std::max(kRows * (XP + HP), 16 * RT * XP)], tiles[4][kTileHalves], less[4][kRows];
+    __shared__ int exps[2][kRows], rows[kMostRows];
+    half_t *const xs = lds, *const hs = lds + kRows * XP, *const as = lds;
     const AdapterArgs &g = d.f;
     const int R = g.R, K = g.K, N = g.N, kchunks = (K + kCols - 1) / kCols, chunks = kchunks + (N + kCols - 1) / kCols;
     const int u = (int)blockIdx.x / chunks, chunk = (int)blockIdx.x - u * chunks;
@@ -638,31 +669,26 @@ __global__ void __launch_bounds__(256) grad_kernel(GradArgs d)
     if (count <= 0) return;
     const int lane = threadIdx.x & 63, wave = wave_id(), m = lane & 15, q4 = lane >> 4;
     const float scale = g.scale[a];
-    const half_t *src = of_x ? g.x : d.dy;
+    const half_t *src = of_x ? g.x : d.dy, *terms = d.terms[of_x ? 0 : 1];
     const int64_t ld = of_x ? g.ldx : d.lddy;
-    const float *hsrc = of_x ? d.dh : g.h;
+    const int *from_exps = d.exps[of_x ? 0 : 1];
     for (int e = threadIdx.x; e < count; e += 256) rows[e] = d.rows[first + e];
     if (of_x)
         for (int e = threadIdx.x; e < 16 * RT * (kCols / 8); e += 256) {
             const int r = e / (kCols / 8), c = 8 * (e % (kCols / 8));
             const half8_t w = load8(g.A + ((int64_t)a * R + min(r, R - 1)) * K + min(c0 + c, K - 8));
-            *reinterpret_cast<half8_t *>(as + r * XP + c) = r < R && c0 + c < K ? w : zero8();
+            put8(as + r * XP + c, r < R && c0 + c < K ? w : zero8());
         }
-    Two::clear(hs, kRows);
-    Two::clear(hr, kRows);
-    if (threadIdx.x < kRows) largest[0][threadIdx.x] = 0;
     __syncthreads();
-    half8_t x[NX];
-    float4_t v[RT];
-    const int xc = 8 * (threadIdx.x % (kCols / 8)), xr = threadIdx.x / (kCols / 8);
+    half8_t x[NX], v[RT];
+    int exp;
+    const int xc = 8 * (threadIdx.x % (kCols / 8)), xr = threadIdx.x / (kCols / 8), vc = 8 * (threadIdx.x % (4 * RT)), vr = threadIdx.x / (4 * RT);
     auto load = [&](int r0) __attribute__((always_inline)) {      // (rows that there are not: others)
 #pragma unroll
         for (int i = 0; i < NX; i++) x[i] = load8(src + (int64_t)rows[min(r0 + xr + 256 / (kCols / 8) * i, count - 1)] * ld + min(c0 + xc, width - 8));
 #pragma unroll
-        for (int i = 0; i < RT; i++) {
-            const int e = threadIdx.x + 256 * i, r = e / (R / 4), c = 4 * (e % (R / 4));
-            v[i] = *reinterpret_cast<const float4_t *>(hsrc + (int64_t)rows[min(r0 + r, count - 1)] * R + c);
-        }
+        for (int i = 0; i < RT; i++) v[i] = load8(terms + (int64_t)rows[min(r0 + vr + 64 / RT * i, count - 1)] * (32 * RT) + vc);
+        exp = from_exps[rows[min(r0 + lane, count - 1)]];
     };
     load(0);
     // A of 32 columns a wave, 8 of them side by side in a lane
@@ -674,40 +700,33 @@ __global__ void __launch_bounds__(256) grad_kernel(GradArgs d)
             const half_t *q = as + (Two::of(i, q4) + (m >> 2)) * XP + 32 * wave + 8 * (m & 3) + 4 * j;
             w[i][j] = both(read_tr(q), read_tr(q + 4 * XP));
         }
+    __syncthreads();
     float4_t acc[RT][2];
 #pragma unroll
     for (int i = 0; i < RT; i++) acc[i][0] = acc[i][1] = zero4();
-    int top = -126;                            // exponent that the sums are scaled by
+    int top = -127;                            // exponent that the sums are scaled by
     for (int r0 = 0, turn = 0; r0 < count; r0 += kRows, turn ^= 1) {
         const int left = count - r0;
 #pragma unroll
         for (int i = 0; i < NX; i++) {
             const int r = xr + 256 / (kCols / 8) * i;
-            *reinterpret_cast<half8_t *>(xs + r * XP + xc) = r < left && c0 + xc < width ? x[i] : zero8();
+            put8(xs + r * XP + xc, r < left && c0 + xc < width ? x[i] : zero8());
         }
 #pragma unroll
         for (int i = 0; i < RT; i++) {
-            const int r = (threadIdx.x + 256 * i) / (R / 4);
-            if (r >= left) v[i] = zero4();
-            if (r < kRows) atomicMax(&largest[turn][r], max(max(finite_bits(v[i][0]), finite_bits(v[i][1])), max(finite_bits(v[i][2]), finite_bits(v[i][3]))));
+            const int r = vr + 64 / RT * i;
+            put8(hs + r * HP + vc, r < left ? v[i] : zero8());
         }
-        __syncthreads();
-        if (threadIdx.x < kRows) largest[turn ^ 1][threadIdx.x] = 0;
-        const int now = max(top, exponent(__builtin_bit_cast(int, wave_max(__builtin_bit_cast(float, largest[turn][lane])))));
-        const float less = two_to(max(top - now, -126));
-        top = now;
+        // rows' scales, as parts of the largest so far: one below 2^-24 of it is lost
+        if (lane >= left) exp = -127;
+        const int now = max(top, (int)wave_max((float)exp));
+        less[wave][lane] = f2h(two_to(max(exp - now, -126)));
+        if (wave == 0) exps[turn][lane] = exp;
+        if (now > top) {
+            const float f = two_to(max(top - now, -126));
+            top = now;
 #pragma unroll
-        for (int i = 0; i < RT; i++) acc[i][0] *= less, acc[i][1] *= less;
-#pragma unroll
-        for (int i = 0; i < RT; i++) {
-            const int e = threadIdx.x + 256 * i, r = e / (R / 4), c = 4 * (e % (R / 4));
-            if (r >= kRows) break;
-            const float all = two_to(-top), own = two_to(-exponent(largest[turn][r]));
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                Two::put(hs + r * HP, c + k, v[i][k] * all);
-                if (of_x) Two::put(hr + r * HP, c + k, v[i][k] * own);
-            }
+            for (int i = 0; i < RT; i++) acc[i][0] *= f, acc[i][1] *= f;
         }
         load(r0 + kRows);
         __syncthreads();
@@ -715,6 +734,8 @@ __global__ void __launch_bounds__(256) grad_kernel(GradArgs d)
 #pragma unroll
         for (int s = 0; s < kRows / 32; s++) {
             const int row = 32 * s + 4 * q4 + (m >> 2);
+            const half_t *f = less[wave] + 32 * s + 4 * q4;
+            const half8_t part = both(*reinterpret_cast<const half4_t *>(f), *reinterpret_cast<const half4_t *>(f + 16));
             half8_t xf[2];
 #pragma unroll
             for (int c = 0; c < 2; c++) {
@@ -726,7 +747,7 @@ __global__ void __launch_bounds__(256) grad_kernel(GradArgs d)
 #pragma unroll
                 for (int p = 0; p < 2; p++) {
                     const half_t *q = hs + row * HP + p * Two::kLo + 16 * i + 4 * (m & 3);
-                    const half8_t hf = both(read_tr(q), read_tr(q + 16 * HP));
+                    const half8_t hf = both(read_tr(q), read_tr(q + 16 * HP)) * part;
 #pragma unroll
                     for (int c = 0; c < 2; c++) acc[i][c] = of_x ? mfma(hf, xf[c], acc[i][c]) : mfma(xf[c], hf, acc[i][c]);
                 }
@@ -740,11 +761,11 @@ __global__ void __launch_bounds__(256) grad_kernel(GradArgs d)
                 for (int i = 0; i < Two::kN; i++)
 #pragma unroll
                     for (int p = 0; p < Two::kM; p++) {
-                        const half8_t hf = load8(hr + (16 * t + m) * HP + Two::column(i, p, q4));
+                        const half8_t hf = load8(hs + (16 * t + m) * HP + Two::column(i, p, q4));
 #pragma unroll
                         for (int j = 0; j < 2; j++) o[j] = mfma(w[i][j], hf, o[j]);
                     }
-                const float factor = factor_of(scale, largest[turn][16 * t + m]);
+                const float factor = factor_of(scale, exps[turn][16 * t + m]);
                 const int r = 16 * t + mem_row(), c = c0 + 32 * wave + mem_col();
                 const int64_t row = rows[r0 + min(r, left - 1)];
                 half8_t y;
@@ -754,7 +775,7 @@ __global__ void __launch_bounds__(256) grad_kernel(GradArgs d)
             }
         __syncthreads();
     }
-    const float up = two_to(top);
+    const float up = two_to(max(top, -126));
     float *part = d.parts + (int64_t)u * R * (K + N);
 #pragma unroll
     for (int i = 0; i < RT; i++)
@@ -822,6 +843,7 @@ int check(const char *who, int64_t T, int64_t S, int64_t K, int64_t N, int64_t R
 }
 
 // RT of 1, 2, 4 or 8: R rounded up to 16 of them
+int rank_of(int64_t R) { return R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8; }
 #define CACTI_BY_RANK(R, launch)        \
     do {                                \
         if ((R) <= 16) launch(1);       \
@@ -840,20 +862,27 @@ int64_t block_rows(int64_t T, int64_t K, int64_t N)
 }
 
 struct Workspace {
-    size_t dh, rows, begin, parts, bytes;
+    size_t terms[2], exps[2], rows, begin, parts, bytes;
     int64_t per, blocks;
 };
 Workspace workspace(int64_t T, int64_t K, int64_t N, int64_t R, int64_t n)
 {
     Workspace w;
-    auto up = [](size_t b) { return (b + 255) / 256 * 256; };
+    w.bytes = 0;
+    auto room = [&](size_t b) {
+        const size_t at = w.bytes;
+        w.bytes += (b + 255) / 256 * 256;
+        return at;
+    };
     w.per = block_rows(T, K, N);
     w.blocks = T / w.per + n;
-    w.dh = 0;
-    w.rows = w.dh + up((size_t)T * R * 4);
-    w.begin = w.rows + up((size_t)T * 4);
-    w.parts = w.begin + up((size_t)(n + 1) * 4);
-    w.bytes = w.parts + (size_t)w.blocks * R * (K + N) * 4;
+    for (int i = 0; i < 2; i++) {
+        w.terms[i] = room((size_t)T * 64 * rank_of(R));
+        w.exps[i] = room((size_t)T * 4);
+    }
+    w.rows = room((size_t)T * 4);
+    w.begin = room((size_t)(n + 1) * 4);
+    w.parts = room((size_t)w.blocks * R * (K + N) * 4);
     return w;
 }
 
@@ -871,7 +900,7 @@ ForwardPlan forward_plan(int64_t T, int64_t S, int64_t K, int64_t N, int64_t R, 
     auto units = [&](int64_t rows) { return make_units(T, S, rows, 1, 1, (max_new + rows - 1) / rows); };
     auto fill = [](int64_t target, int64_t count, int64_t most) { return (int)std::max<int64_t>(1, std::min(target / count, most)); };
     const int64_t cus = device_cus();
-    const int rank = R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8;
+    const int rank = rank_of(R);
     w.many = max_new > 16;
     if (!w.many) {
         w.splits = fill(cus, units(kTile).count, (N + 32 * few_waves(rank) - 1) / (32 * few_waves(rank)));
@@ -973,7 +1002,7 @@ CACTI_API int cacti_hip_adapter_bwd(int64_t T, int64_t S, int64_t K, int64_t N, 
     d.f.y = (half_t *)dx, d.f.ldy = lddx;
     d.f.base = dx_acc ? (const half_t *)dx : nullptr, d.f.ldb = lddx;
     d.dy = (const half_t *)dy, d.lddy = lddy;
-    d.dh = (float *)(p + w.dh);
+    for (int i = 0; i < 2; i++) d.terms[i] = (half_t *)(p + w.terms[i]), d.exps[i] = (int *)(p + w.exps[i]);
     d.rows = (int *)(p + w.rows), d.begin = (int *)(p + w.begin);
     d.parts = (float *)(p + w.parts);
     d.dA = (half_t *)dA, d.dB = (half_t *)dB, d.dA_acc = dA_acc, d.dB_acc = dB_acc;

@@ -1,8 +1,9 @@
 """Low-rank adapters of many requests, forward and adjoint, against float64.
 
 What the kernels round.  h: a sum of K exact products in fp32, at most K 2^-24 sum |x A| (K steps in any order); dh the same over N.  Of
-either, f16 takes two terms, scaled by the power of two that brings the largest of a row to 1 .. 2 (for dA and dB: the largest of the
-adapter's rows so far): what is left is 2^-22 of it, or half a step of the second term's subnormal range, 2^-25 of that largest.  y: R products of those and two
+either, f16 takes two terms, scaled by the power of two that brings the largest of a row to 2^10 .. 2^11: what is left is 2^-22 of it, or half a
+step of the second term's subnormal range, 2^-25 for a largest of 2^10, of which 2^-25 is far more than that.  For dA and dB a row's scale is
+made that of the largest row so far: a row 2^-25 and less of that scale, whose largest is below 2^-24 of that row's, is lost.  y: R products of those and two
 terms each, 2 R 2^-24 sum |h B|, the scale and the base in fp32 (2^-22 of either), and half a step of f16: 2^-11 |y|, 2^-25 below its normal
 range.  dA and dB: 2 T + T / 64 additions.  In what follows each product carries the errors of both factors."""
 import numpy as np
@@ -100,7 +101,7 @@ class Case:
             dh = dy @ B
             own = self.N * 2.0 ** -24 * (np.abs(dy) @ np.abs(B)) + 2.0 ** -22 * np.abs(dh)
             left = own + 2.0 ** -25 * np.abs(dh).max(1, keepdims=True)
-            most = lambda v: 2.0 ** -25 * np.abs(v).max() if len(at) else 0.0
+            most = lambda v: 2.0 ** -24 * np.abs(v).max() if len(at) else 0.0
             adds = (2 * len(at) + len(at) / 64 + 4) * 2.0 ** -24
             d = s * (dh @ A)
             dx[at] += d
