@@ -364,7 +364,7 @@ struct Wave {
     const Tile &t;
     const half_t *B;
     int n, step;
-    C a, b;
+    C a;
     __device__ __forceinline__ Wave(const AdapterArgs &g_, const Tile &t_, int first, int stride) : g(g_), t(t_), n(32 * first), step(32 * stride)
     {
         B = g.B + (int64_t)t.a * g.N * g.R;
@@ -377,18 +377,12 @@ struct Wave {
         float factor[TB];
 #pragma unroll
         for (int i = 0; i < TB; i++) factor[i] = factor_of(scale, exponent(largest[16 * i + (threadIdx.x & 15)]));
-        for (; n + 2 * step < g.N; n += 2 * step) {
-            b.load(g, t, B, n + step);
+        for (;;) {
             a.put(g, t, factor, hs, lds);
-            a.load(g, t, B, n + 2 * step);
-            b.put(g, t, factor, hs, lds);
+            n += step;
+            if (n >= g.N) break;
+            a.load(g, t, B, n);
         }
-        if (n + step < g.N) {
-            b.load(g, t, B, n + step);
-            a.put(g, t, factor, hs, lds);
-            b.put(g, t, factor, hs, lds);
-        } else
-            a.put(g, t, factor, hs, lds);
     }
 };
 
@@ -414,12 +408,12 @@ __device__ __forceinline__ int unit_and_split(const AdapterArgs &g, int *split)
     return 8 * group + in % left;
 }
 
-// Few rows: a workgroup to 16 rows of a sequence and 1 / splits of the columns of y; h is formed by each of them.
-constexpr int few_waves(int RT) { return RT <= 2 ? 16 : 8; }      // (the registers of more leave room for 8)
+// In one launch: a workgroup to 16 rows of a sequence and 1 / splits of the columns of y; h is formed by each of them.
+constexpr int one_waves(int RT) { return RT <= 2 ? 16 : 8; }      // (the registers of more leave room for 8)
 template <int RT, bool BASE>
-__global__ void __launch_bounds__(64 * few_waves(RT)) few_kernel(AdapterArgs g)
+__global__ void __launch_bounds__(64 * one_waves(RT)) one_kernel(AdapterArgs g)
 {
-    constexpr int W = few_waves(RT), C = 16 * RT;
+    constexpr int W = one_waves(RT), C = 16 * RT;
     typedef TileH<RT, 1, W, false> H;
     typedef Wave<RT, 1, BASE> Y;
     typedef Terms<RT> Two;
@@ -456,7 +450,7 @@ __global__ void __launch_bounds__(64 * few_waves(RT)) few_kernel(AdapterArgs g)
     y.run(scale, hs, largest, lds + wave_id() * Y::C::kLds);
 }
 
-// Many rows, h first: 16 TB rows of a sequence and 1 / splits of the contraction to a workgroup, sums to a plane of [splits][T, R]
+// In two, h first: 16 TB rows of a sequence and 1 / splits of the contraction to a workgroup, sums to a plane of [splits][T, R]
 constexpr int h_blocks(int) { return 2; }
 template <int RT, int TB>
 __global__ void __launch_bounds__(512) h_kernel(AdapterArgs g, float *planes)
@@ -886,10 +880,17 @@ Workspace workspace(int64_t T, int64_t K, int64_t N, int64_t R, int64_t n)
     return w;
 }
 
-// How the forward pass is cut.  Few rows: one launch, whose workgroups each form the h that they need; columns are split until the device is
-// full.  Many: h first.
+// How the forward pass is cut: in one launch, whose workgroups of 16 rows each form the h that they need, over all of K, with the columns
+// split until the device is full; or h first, from parts of K, and then y by 64 rows: a launch more, but A and B are read less often.  The
+// second, by us of both (the second's first), where
+//   K is long and A large, and the tiles leave half of the device idle: one row of 8640 to 3200, R = 32 10.9 and 13.3, R = 128 18.7 and 32.5,
+//     1200 rows 33 and 53; not with K = 3200, whose 600 rows with R = 128 take 27.2 and 24.3;
+//   there are rows for several rounds of tiles: 16 x 600 rows of 2048 to 2048, R = 8 27 and 29, R = 32 33 and 38, R = 128 70 and 80;
+//   the tiles are too few to fill the device and too many to split their columns, and A and B are large: 4 x 557 rows of 3200 to 8640,
+//     R = 64 34 and 45, but R = 16 24.0 and 23.4.
+// Everywhere else the first: one row of 3200 to 8640, R = 16 8.5 and 6.2, 2048 rows of 3200 to 3200 12.9 and 10.2, 4096 19.3 and 15.7.
 struct ForwardPlan {
-    bool many;
+    bool two;
     int splits, planes;
     Units h_units, y_units;
     size_t bytes;
@@ -901,9 +902,11 @@ ForwardPlan forward_plan(int64_t T, int64_t S, int64_t K, int64_t N, int64_t R, 
     auto fill = [](int64_t target, int64_t count, int64_t most) { return (int)std::max<int64_t>(1, std::min(target / count, most)); };
     const int64_t cus = device_cus();
     const int rank = rank_of(R);
-    w.many = max_new > 16;
-    if (!w.many) {
-        w.splits = fill(cus, units(kTile).count, (N + 32 * few_waves(rank) - 1) / (32 * few_waves(rank)));
+    const int64_t tiles = units(kTile).count;
+    w.two = (K > 4096 && R * K > (1 << 18) && tiles <= cus / 2) || T >= 32 * cus ||
+            (tiles > cus / 2 && tiles < cus * 7 / 8 && R * (K + N) > (1 << 18));
+    if (!w.two) {
+        w.splits = fill(cus, tiles, (N + 32 * one_waves(rank) - 1) / (32 * one_waves(rank)));
         return w;
     }
     w.h_units = units(16 * h_blocks(rank));
@@ -942,14 +945,14 @@ CACTI_API int cacti_hip_adapter_fwd(int64_t T, int64_t S, int64_t K, int64_t N, 
     CACTI_REQUIRE(ws_bytes >= w.bytes && (ws || !w.bytes) && aligned(ws, 16), CACTI_E_INVALID, "adapter_fwd: workspace of %zu bytes, %zu needed, 16-byte aligned",
                   ws_bytes, w.bytes);
     hipStream_t st = (hipStream_t)stream;
-    if (!w.many) {
+    if (!w.two) {
         g.splits = w.splits;
         const int64_t blocks = g.units.count * g.splits + (status ? 1 : 0);
         CACTI_REQUIRE(blocks <= INT32_MAX, CACTI_E_NOTIMPL, "adapter_fwd: too many tiles");
 #define LAUNCH(RT)                                                                                                       \
     do {                                                                                                                 \
-        if (base) hipLaunchKernelGGL((few_kernel<RT, true>), dim3((unsigned)blocks), dim3(64 * few_waves(RT)), 0, st, g); \
-        else hipLaunchKernelGGL((few_kernel<RT, false>), dim3((unsigned)blocks), dim3(64 * few_waves(RT)), 0, st, g);     \
+        if (base) hipLaunchKernelGGL((one_kernel<RT, true>), dim3((unsigned)blocks), dim3(64 * one_waves(RT)), 0, st, g); \
+        else hipLaunchKernelGGL((one_kernel<RT, false>), dim3((unsigned)blocks), dim3(64 * one_waves(RT)), 0, st, g);     \
     } while (0)
         CACTI_BY_RANK(R, LAUNCH);
 #undef LAUNCH

@@ -26,7 +26,7 @@ COMMON = [(dict(T=0), "empty"), (dict(S=0), "empty"), (dict(K=0), "empty"), (dic
 REFUSED = [("cacti_hip_adapter_fwd", FWD, c) for c in COMMON + [
     (dict(y=None), "null"), (dict(h=None), "null"), (dict(ldy=56), "pitch"), (dict(ldb=66), "multiple"), (dict(base=P0 + 3 * STEP + 8), "aligned"),
     (dict(y=P0), "shares"), (dict(y=P0 + 128), "shares"), (dict(y=P0 + 3 * STEP, ldy=72), "place"), (dict(y=P0 + 3 * STEP + 16), "place"),
-    (dict(T=100, max_new=100, K=1024, ldx=1024, x=1 << 30), "workspace")]] + \
+    (dict(T=100, max_new=100, K=8192, R=64, ldx=8192, x=1 << 30), "workspace")]] + \
           [("cacti_hip_adapter_bwd", BWD, c) for c in COMMON + [
               (dict(h=None), "null"), (dict(dy=None), "null"), (dict(dx=None), "null"), (dict(dA=None), "null"), (dict(dB=None), "null"), (dict(ws=None), "null"),
               (dict(lddy=56), "pitch"), (dict(lddx=68), "multiple"), (dict(dx=P0), "shares"), (dict(dx=P0 + 4 * STEP + 16), "shares"),
@@ -157,6 +157,50 @@ def test_adapter(counts, ids, K, N, R):
 def test_adapter_of_a_models_widths(counts, ids, K, N, R, n):
     print("adapter", len(counts), K, N, R, flush=True)
     check(Case(K + N + R, counts, ids, K, N, R, n), max_new=max(counts))
+
+
+TWO = [([1] * 9, [0, 2, -1, 2, 1, 0, 0, -1, 2], 8640, 264, 32), ([3, 0, 16, 33, 1], [1, 0, -1, 1, 2], 8640, 1032, 64), ([70], [1], 4104, 520, 128),
+       ([1] * 140, [i % 4 - 1 for i in range(140)], 4000, 264, 64), ([17] * 70, [i % 3 for i in range(70)], 2000, 72, 128),
+       ([5000, 7, 3400], [2, -1, 0], 72, 40, 16), ([8200], [1], 264, 136, 24)]
+
+
+@pytest.mark.parametrize("counts,ids,K,N,R", TWO)
+def test_parts_of_two_launches_have_a_workspace(counts, ids, K, N, R):
+    ws = ffi.lib().cacti_hip_adapter_fwd_workspace
+    T = sum(counts)
+    assert ws(T, len(ids), K, N, R, max(counts)) % (T * R * 4) == 0
+    if K > 4096:
+        assert ws(T, len(ids), K, N, R, max(counts)) >= 2 * T * R * 4
+
+
+@GPU
+@pytest.mark.parametrize("counts,ids,K,N,R", TWO)
+def test_in_two_launches(counts, ids, K, N, R):
+    """Sizes whose h is formed first: a long K, tiles between half the device and all of it, many rows; with the base's place, numbers that do
+    not fit, and adapters of NaN that nobody has."""
+    import torch
+    from cacti_amd import ops
+    print("adapter", len(counts), sum(counts), K, N, R, flush=True)
+    c = Case(K + N + R, counts, ids, K, N, R, 4, behind=3)
+    c.A[3], c.B[3] = np.nan, np.inf
+    x, A, B, starts, scale, base = c.of("x A B starts scale base")
+    c.n = 3
+    used, most = int(c.starts[-1]), max(counts)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    wy, ty, wh, th = c.forward(True)
+    bare, _ = ops.adapter_fwd(x, A, B, starts, dev(c.ids), scale, max_new=most)
+    near(bare[:used], *[v[:used] for v in c.forward(False)[:2]], "y alone")
+    got, h = ops.adapter_fwd(x, A, B, starts, dev(c.ids), scale, base=base, max_new=most, status=status)
+    near(h[:used], wh[:used], th[:used], "h")
+    near(got[:used], wy[:used], ty[:used], "y")
+    own = base.clone()
+    ops.adapter_fwd(x, A, B, starts, dev(c.ids), scale, base=own, out=own, max_new=most)
+    assert torch.equal(own[:used], got[:used]) and torch.equal(own[used:], base[used:]) and int(status) == 0
+    bad = c.ids.copy()
+    bad[-1] = 4
+    y, _ = ops.adapter_fwd(x, A, B, starts, dev(bad), scale, base=base, max_new=most, status=status)
+    last = slice(int(c.starts[-2]), used)
+    assert int(status) == len(ids) and torch.equal(y[last], base[last]) and torch.equal(y[:last.start], got[:last.start])
 
 
 @GPU
