@@ -151,6 +151,13 @@ def test_policy(N, V, temp, with_ref):
 
 
 @GPU
+@pytest.mark.parametrize("V", [65, 2048, 2055, 2056, 8199, 8200, 10247, 10248, 16391, 16392, 32775, 32776])
+def test_widths_on_either_side_of_what_threads_hold(V):
+    test_logp_and_adjoint(9, V, 0.9)
+    test_policy(9, V, 1.0, True)
+
+
+@GPU
 def test_gradients_against_differences():
     """Central differences of the float64 loss at the kernels' own gradients."""
     from cacti_amd import ops
