@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(T) logp_fwd_kernel(TokenArgs a)
 {
     const int64_t n = blockIdx.x;
     const int x = token(a, n, threadIdx.x == 0);
-    RowStats r = {0.f, 1.f, 0.f};
+    RowStats r = {0.f, 0.f, 0.f};              // (a sum of 0, which no row has: left out, and so by the adjoint)
     if (x >= 0) {
         const VocabRow z(a.logit + n * a.ld, a.V);
         Held<T, NP> h(z);
@@ -162,11 +162,11 @@ __global__ void __launch_bounds__(T) logp_bwd_kernel(TokenArgs a)
     const VocabRow z(a.logit + n * a.ld, a.V), g(a.grad + n * a.ldd, a.V);
     half_t *to = a.grad + n * a.ldd;
     Held<T, NP> h(g);
-    const float d = a.dlogp[n];
+    const float d = a.dlogp[n], mx = a.stats[2 * n], sum = a.stats[2 * n + 1];
     const int x = a.tok[n];
-    if (d == 0.f || x >= a.V) return put_nothing(a, to, g, h);
+    if (d == 0.f || sum == 0.f || x >= a.V) return put_nothing(a, to, g, h);
     h.load(z, g);
-    put_gradient(a, to, g, h, x, a.stats[2 * n], a.stats[2 * n + 1], d * a.inv_temp);
+    put_gradient(a, to, g, h, x, mx, sum, d * a.inv_temp);
 }
 
 // e^d - 1 - d, also where d is small and the difference would cancel

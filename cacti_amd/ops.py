@@ -295,8 +295,8 @@ def token_logp_fwd(logit, tok, temperature=1.0, mask=None, status=None):
 
 
 def token_logp_bwd(logit, tok, stats, dlogp, temperature=1.0, acc=None):
-    """Their gradient times dlogp f32 [N] with respect to logit, f16 (added to acc where given).  A row with dlogp 0 has gradient 0
-    and is not read."""
+    """Their gradient times dlogp f32 [N] with respect to logit, f16 (added to acc where given).  A row with dlogp 0, and one that the mask
+    left out, has gradient 0 and is not read."""
     return _op.token_logp_bwd(logit, tok, stats, dlogp, temperature, acc)
 
 
@@ -336,8 +336,8 @@ def adapter_bwd(x, A, B, starts, ids, scale, h, dy, dx_acc=None, dA_acc=None, dB
 
 
 def paged_fork(refs, table, lens, parent, page, out=None, status=None):
-    """Sequences of a paged cache go on as others: (table, lens) in which sequence b has the pages and the length of parent[b] (b itself: as
-    it is; -1: empty).  refs [pages], who holds each page, is brought up to date.  Nothing is copied: paged_fit does what is needed
+    """Sequences of a paged cache go on as others: (table, lens) in which sequence b has the pages and the length of parent[b] (which may
+    be b; -1: empty).  refs [pages], who holds each page, is brought up to date.  Nothing is copied: paged_fit does what is needed
     before the next append.  All int32 tensors on the GPU; out = (table, lens) to write to, other memory than the old ones."""
     return _op.paged_fork(refs, table, lens, parent, page, out, status)
 

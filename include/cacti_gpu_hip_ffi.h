@@ -515,7 +515,7 @@ int cacti_hip_distill_topk_bwd(int64_t N, int64_t V, int64_t K, const void *logi
 /* logp[n] = log softmax(logit[n] / temperature)[tok[n]], and its adjoint dlogit[j] (+)= f16(dlogp[n] / temperature * ([j = tok[n]] - p_j)).
  * logit16 [N,V] f16 of pitch ld, tok [N] u16, logp, dlogp [N] f32; stats [N,2] f32: maximum and sum, written by the forward call, read by
  * the adjoint.  mask [N] u8 or NULL: a row where it is 0, or whose token is >= V (status [1] i32 or NULL: 1 + the row), has logp 0 and is
- * not read; in the adjoint a row with dlogp 0 or such a token has gradient 0 and is not read.  V <= 65536, N < 2^23, any alignment of the
+ * not read; in the adjoint such a row, and one with dlogp 0, has gradient 0 and is not read.  V <= 65536, N < 2^23, any alignment of the
  * rows.  dlogit16 may be logit16 itself, with the same pitch, and shares no memory with it otherwise.  acc as everywhere.  Sums in fp32. */
 int cacti_hip_token_logp_fwd(int64_t N, int64_t V, const void *logit16, int64_t ld, const void *tok, const void *mask, double temperature,
                              void *logp, void *stats, void *status, void *stream);
@@ -545,15 +545,17 @@ int cacti_hip_preference_loss(int64_t N, int64_t pairs, const void *logp, const 
 /* Low-rank adapters of many requests beside a shared projection.  Rows starts[s] .. starts[s + 1] - 1 of x [T,K] are those of sequence s
  * (starts [S + 1], ids [S] i32 on the device, not read by the host; starts does not fall), which has adapter a = ids[s] of n, or none (-1):
  *   h = x A_a^T,  y = f16(base + scale[a] h B_a^T)        A [n,R,K], B [n,N,R] f16, contiguous; scale [n] f32; h [T,R] f32
- * Rows of a sequence without an adapter: y = base, h = 0.  Rows of no sequence are left as they are in y and h.  base NULL: 0; it may be y,
+ * Rows of a sequence without an adapter: y = base, h = 0.  Rows of no sequence are left as they are in y, h and dx.  base NULL: 0; it may be y,
  * with the same pitch (so that the adapters' part is added to a product), and shares no memory with it otherwise; nor does x.  The
  * adjoint, with dy [T,N] and h as the forward call wrote it:
  *   dh = dy B_a,  dx (+)= f16(scale[a] dh A_a),  dA_a (+)= f16(scale[a] sum dh^T x),  dB_a (+)= f16(scale[a] sum dy^T h)   (over a's rows)
  * (an adapter without rows: 0).  *_acc: 0 first write, 1 added in fp32 before the one rounding.  Sums in fp32 and in a fixed order; h and dh
- * meet the second product as two f16 terms, 22 bits, 2^-25 of the largest of their row (for dA and dB: 2^-24 of the adapter's largest).  K, N, R multiples of 8, R <= 128; rows of x, y, base,
- * dy, dx of pitches that are multiples of 8; all 16-byte aligned; n <= 1024.  max_new: no sequence has more rows.  status [1] i32 or NULL: 1 + s
- * where the rows of sequence s are not there or more than max_new (it has none then), or its id is neither -1 nor below n (it has no
- * adapter then); the caller clears it.  workspace: cacti_hip_adapter_{fwd,bwd}_workspace bytes (0: NULL will do), 16-byte aligned, contents undefined on return. */
+ * meet the second product as two f16 terms, 22 bits, 2^-25 of the largest of their row (for dA and dB: 2^-24 of the adapter's largest).
+ * dx, dA and dB share no memory with x, dy or each other.  K, N, R multiples of 8, R <= 128; rows of x, y, base, dy, dx of pitches that are
+ * multiples of 8; all 16-byte aligned; n <= 1024; T <= 2^24, S <= 2^20, K and N <= 2^20, less where that would be 2^24 blocks of rows and
+ * columns.  max_new: no sequence has more rows.  status [1] i32 or NULL: 1 + s where the rows of sequence s are not there or more than
+ * max_new (it has none then), or its id is neither -1 nor below n (it has no adapter then); the caller clears it.  workspace:
+ * cacti_hip_adapter_{fwd,bwd}_workspace bytes (0: NULL will do), 16-byte aligned, contents undefined on return. */
 size_t cacti_hip_adapter_fwd_workspace(int64_t T, int64_t S, int64_t K, int64_t N, int64_t R, int64_t max_new);
 int cacti_hip_adapter_fwd(int64_t T, int64_t S, int64_t K, int64_t N, int64_t R, int64_t n, int64_t max_new, const void *x, int64_t ldx,
                           const void *A, const void *B, const void *starts, const void *ids, const void *scale, const void *base,
@@ -567,9 +569,10 @@ int cacti_hip_adapter_bwd(int64_t T, int64_t S, int64_t K, int64_t N, int64_t R,
 /* Pages of the cache above, handed out on the device.  refs [P] i32: how many hold a page (sequences of the table, and whoever else the
  * caller counts); table [B,W] i32 of pitch ldt: a sequence's pages in order, -1 behind them; lens [B] i32: its positions, page to a page.
  * Where nothing else is said lengths are 0 to W page.  A number that is no page of the cache is handed on and not counted.  P, B <= 2^28,
- * 2^20; W page <= 2^30.  status [1] i32 or NULL: 1 + a sequence whose numbers do not fit, or for which there was no page.
+ * 2^20; W page <= 2^30; B W < 2^31.  What is written shares no memory with anything else but refs and table, changed in place.  status [1]
+ * i32 or NULL: 1 + a sequence whose numbers do not fit, or for which there was no page.
  *
- * Sequence b goes on as sequence parent[b] (itself: as it is; -1: empty): row b of new_table = row parent[b] of table as far as its
+ * Sequence b goes on as sequence parent[b] (which may be b; -1: empty): row b of new_table = row parent[b] of table as far as its
  * positions go, -1 behind; new_lens[b] = lens[parent[b]].  All at once, into other memory; refs is brought up to date.  Pages are shared then, also
  * one that is not full: cacti_hip_paged_fit before the next append.  A sequence whose parent or whose parent's length cannot be stays
  * as it is and is named. */

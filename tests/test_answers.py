@@ -175,6 +175,23 @@ def test_gradients_against_differences():
 
 
 @GPU
+def test_rows_that_the_mask_left_out_have_no_gradient_whatever_theirs_is():
+    import torch
+    from cacti_amd import ops
+    for V in (40, 2056, 20001):
+        r, z, tok = make(V, 6, V)
+        mask = np.array([True, False, True, False, False, True])
+        z[1], z[3], d = np.nan, 60000, np.ones(6, np.float32)
+        logp, stats = ops.token_logp_fwd(dev(z), dev(tok), mask=dev(mask))
+        grad = ops.token_logp_bwd(dev(z), dev(tok), stats, dev(d))
+        want = ops.token_logp_bwd(dev(z), dev(tok), stats, dev(d * mask))
+        assert torch.equal(grad, want) and not bool(grad[dev(~mask)].any()) and not bool(logp[dev(~mask)].any())
+        into = torch.full_like(grad, 3.0)
+        ops.token_logp_bwd(dev(z), dev(tok), stats, dev(d), acc=into)
+        assert bool((into[dev(~mask)] == 3).all()) and torch.isfinite(into).all()
+
+
+@GPU
 def test_rows_that_are_left_out_are_not_read():
     """Masked rows, tokens beyond the vocabulary, coefficients of 0: nothing of them, whatever their logits are; added to: left as it is."""
     import torch
