@@ -996,10 +996,11 @@ CACTI_API int cacti_hip_adapter_bwd(int64_t T, int64_t S, int64_t K, int64_t N, 
     CACTI_REQUIRE(lddy >= N && lddy % 8 == 0 && lddx >= K && lddx % 8 == 0, CACTI_E_INVALID, "adapter_bwd: row pitch below a row, or no multiple of 8");
     CACTI_REQUIRE(!rows_share(T, x, ldx, K, dx, lddx, K) && !rows_share(T, dy, lddy, N, dx, lddx, K), CACTI_E_INVALID,
                   "adapter_bwd: dx shares memory with x or dy");
+    CACTI_REQUIRE(!rows_share(1, dA, n * R * K, n * R * K, dB, n * N * R, n * N * R), CACTI_E_INVALID, "adapter_bwd: dA shares memory with dB");
     const Workspace w = workspace(T, K, N, R, n);
     CACTI_REQUIRE(ws_bytes >= w.bytes, CACTI_E_INVALID, "adapter_bwd: workspace of %zu bytes, %zu needed", ws_bytes, w.bytes);
     const int64_t chunks = (K + kCols - 1) / kCols + (N + kCols - 1) / kCols, size = R * (K + N);
-    CACTI_REQUIRE(w.blocks * chunks <= INT32_MAX, CACTI_E_NOTIMPL, "adapter_bwd: too many tiles");
+    CACTI_REQUIRE(w.blocks * chunks < (1 << 24), CACTI_E_NOTIMPL, "adapter_bwd: too many tiles");
     char *p = (char *)ws;
     d.f.h = (float *)const_cast<void *>(h);
     d.f.y = (half_t *)dx, d.f.ldy = lddx;

@@ -328,7 +328,7 @@ int check(const char *who, int64_t P, int64_t B, int64_t W, int64_t page, const 
 {
     CACTI_REQUIRE(P > 0 && B > 0 && W > 0 && page > 0, CACTI_E_INVALID, "%s: empty shape", who);
     CACTI_REQUIRE(refs && table, CACTI_E_INVALID, "%s: null pointer", who);
-    CACTI_REQUIRE(P <= (1 << 28) && B <= (1 << 20) && W <= (1 << 30) / page && ldt >= W, CACTI_E_NOTIMPL,
+    CACTI_REQUIRE(P <= (1 << 28) && B <= (1 << 20) && W <= (1 << 30) / page && B * W <= INT32_MAX && ldt >= W, CACTI_E_NOTIMPL,
                   "%s: too many pages or sequences, or a table pitch below its width", who);
     CACTI_REQUIRE(aligned(refs, 4) && aligned(table, 4) && aligned(status, 4), CACTI_E_INVALID, "%s: misaligned operand", who);
     return 0;

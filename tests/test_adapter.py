@@ -33,6 +33,11 @@ REFUSED = [("cacti_hip_adapter_fwd", FWD, c) for c in COMMON + [
               (dict(ws_bytes=4096), "workspace"), (dict(dB=P0 + 7 * STEP + 8), "aligned")]]
 
 
+REFUSED += [("cacti_hip_adapter_bwd", BWD, c) for c in [
+    (dict(dB=P0 + 6 * STEP + 1024), "dA shares"), (dict(dA=P0 + 7 * STEP), "dA shares"),
+    (dict(T=1 << 24, max_new=1 << 24, K=1 << 16, ldx=1 << 16, lddx=1 << 16, dy=1 << 44, dx=1 << 46, dB=1 << 47, ws_bytes=1 << 60), "too many tiles")]]
+
+
 @pytest.mark.parametrize("entry,args,change", REFUSED)
 def test_refuses(entry, args, change):
     change, why = change

@@ -24,6 +24,10 @@ REFUSED = [("cacti_hip_paged_fork", FORK, c) for c in BOOK + [
               (dict(src=None), "null"), (dict(used=None), "null"), (dict(used=66), "misaligned"), (dict(ws_bytes=32), "workspace")]]
 
 
+REFUSED += [(e, a, (dict(W=1 << 11, B=1 << 20, ldt=1 << 11, ldn=1 << 11), "too many")) for e, a in (("cacti_hip_paged_fork", FORK), ("cacti_hip_paged_fit", FIT),
+                                                                                                   ("cacti_hip_paged_compact", COMPACT))]
+
+
 @pytest.mark.parametrize("entry,args,change", REFUSED)
 def test_refuses(entry, args, change):
     change, why = change
