@@ -240,6 +240,22 @@ def test_pages_that_others_hold():
 
 
 @GPU
+@pytest.mark.parametrize("P,share", [(1, 0.0), (2, 1.0), (1023, 0.5), (1025, 0.97), (16384, 0.999), (16385, 0.5), (40001, 0.9995), (70000, 0.02), (33000, 1.0)])
+def test_pools_of_many_pages_with_gaps(P, share):
+    """Pages that others hold, at random: the free ones among them are few, or far up, or more than one look finds."""
+    k = Book(P, 40, 9, 16, P)
+    k.refs = [int(k.r.random() < share) * k.r.choice([1, 3]) for _ in range(P)]
+    if share > 0.9:
+        k.refs[P // 2:] = [1] * (P - P // 2 - 1) + [0]
+    k.d_refs.copy_(ints(k.refs))
+    for lens in ([k.r.choice([0, 1, 16, 17, 144]) for _ in range(40)], [k.r.randrange(145) for _ in range(40)]):
+        k.fit([min(a, b) for a, b in zip(k.lens, lens)], lens)
+    k.compact()
+    k.fit([0] * 40, [0] * 40)
+    k.compact()
+
+
+@GPU
 def test_numbers_of_a_table_that_are_no_pages():
     k = Book(2, 2, 4, 16, 10)
     k.fit([0, 0], [40, 20])
