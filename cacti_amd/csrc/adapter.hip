@@ -887,7 +887,7 @@ Workspace workspace(int64_t T, int64_t K, int64_t N, int64_t R, int64_t n)
 //     1200 rows 33 and 53; not with K = 3200, whose 600 rows with R = 128 take 27.2 and 24.3;
 //   there are rows for several rounds of tiles: 16 x 600 rows of 2048 to 2048, R = 8 27 and 29, R = 32 33 and 38, R = 128 70 and 80;
 //   the tiles are too few to fill the device and too many to split their columns, and A and B are large: 4 x 557 rows of 3200 to 8640,
-//     R = 64 34 and 45, but R = 16 24.0 and 23.4.
+//     R = 64 33 and 45, but R = 16 24.0 and 23.4.
 // Everywhere else the first: one row of 3200 to 8640, R = 16 8.5 and 6.2, 2048 rows of 3200 to 3200 12.9 and 10.2, 4096 19.3 and 15.7.
 struct ForwardPlan {
     bool two;
@@ -900,19 +900,24 @@ ForwardPlan forward_plan(int64_t T, int64_t S, int64_t K, int64_t N, int64_t R, 
     ForwardPlan w{};
     auto units = [&](int64_t rows) { return make_units(T, S, rows, 1, 1, (max_new + rows - 1) / rows); };
     auto fill = [](int64_t target, int64_t count, int64_t most) { return (int)std::max<int64_t>(1, std::min(target / count, most)); };
+    // splits of the columns among workgroups of some waves: no more than give the busiest wave fewer
+    auto columns = [&](int64_t target, int64_t count, int64_t waves) {
+        const int64_t blocks = (N + 31) / 32, most = fill(target, count, (blocks + waves - 1) / waves), turns = (blocks + waves * most - 1) / (waves * most);
+        return (int)((blocks + waves * turns - 1) / (waves * turns));
+    };
     const int64_t cus = device_cus();
     const int rank = rank_of(R);
     const int64_t tiles = units(kTile).count;
     w.two = (K > 4096 && R * K > (1 << 18) && tiles <= cus / 2) || T >= 32 * cus ||
             (tiles > cus / 2 && tiles < cus * 7 / 8 && R * (K + N) > (1 << 18));
     if (!w.two) {
-        w.splits = fill(cus, tiles, (N + 32 * one_waves(rank) - 1) / (32 * one_waves(rank)));
+        w.splits = columns(cus, tiles, one_waves(rank));
         return w;
     }
     w.h_units = units(16 * h_blocks(rank));
     w.y_units = units(kRows);
     w.planes = fill(cus, w.h_units.count, std::min<int64_t>(8, (K + 255) / 256));
-    w.splits = fill(2 * cus, w.y_units.count, (N + 255) / 256);
+    w.splits = columns(rank == 8 ? cus : 2 * cus, w.y_units.count, 8);       // (as many as a CU's LDS has room for: R = 128 47 us, by two 54)
     w.bytes = w.planes > 1 ? (size_t)w.planes * T * R * 4 : 0;
     return w;
 }
