@@ -846,11 +846,12 @@ int rank_of(int64_t R) { return R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8; }
         else launch(8);                 \
     } while (0)
 
-// rows of a block: some hundred workgroups at least, and no more parts than that needs
-int64_t block_rows(int64_t T, int64_t K, int64_t N)
+// rows of a block: as many workgroups as the device holds at once, counting those of blocks that are not full.  (4096 rows of 3200 to 3200,
+// R = 64: about 640 54 us, 768 57, 384 59; R = 128, two to a CU: 384 90, 640 101.)
+int64_t block_rows(int64_t T, int64_t K, int64_t N, int64_t R)
 {
     const int64_t chunks = (K + kCols - 1) / kCols + (N + kCols - 1) / kCols, steps = (T + kRows - 1) / kRows;
-    int64_t per = steps * chunks / 768;
+    int64_t per = steps * chunks / (R > 64 ? 384 : 640);
     per = per < 1 ? 1 : per > kMostRows / kRows ? kMostRows / kRows : per;
     return per * kRows;
 }
@@ -868,7 +869,7 @@ Workspace workspace(int64_t T, int64_t K, int64_t N, int64_t R, int64_t n)
         w.bytes += (b + 255) / 256 * 256;
         return at;
     };
-    w.per = block_rows(T, K, N);
+    w.per = block_rows(T, K, N, R);
     w.blocks = T / w.per + n;
     for (int i = 0; i < 2; i++) {
         w.terms[i] = room((size_t)T * 64 * rank_of(R));
