@@ -240,6 +240,19 @@ def test_pages_that_others_hold():
 
 
 @GPU
+def test_more_sequences_than_a_workgroup_remembers():
+    k = Book(5, 2300, 3, 16, 6000)
+    r = k.r
+    k.fit([0] * 2300, [r.randrange(49) for _ in range(2300)])
+    k.fork([r.choice([b, r.randrange(2300)]) for b in range(2300)])
+    k.fit(k.lens, [min(48, l + r.randrange(3)) for l in k.lens])
+    back = [r.randrange(l + 1) for l in k.lens]
+    k.fit(back, [r.choice([l, min(48, l + 7), 49]) for l in back])
+    k.lens = [min(l, 48) for l in k.lens]
+    k.compact()
+
+
+@GPU
 @pytest.mark.parametrize("P,share", [(1, 0.0), (2, 1.0), (1023, 0.5), (1025, 0.97), (16384, 0.999), (16385, 0.5), (40001, 0.9995), (70000, 0.02), (33000, 1.0)])
 def test_pools_of_many_pages_with_gaps(P, share):
     """Pages that others hold, at random: the free ones among them are few, or far up, or more than one look finds."""

@@ -283,3 +283,43 @@ def test_losses_back_to_adapters(counts, ids, K, N, R, loss):
         want = step()
         torch.cuda.synchronize()
         assert all(torch.equal(u, v) for u, v in zip(got, want)), i
+
+
+@GPU
+def test_two_graphs_and_another_stream():
+    """Two captured steps and one on a stream of its own, one after the other and in turn: each has its own workspaces."""
+    import torch
+    from cacti_amd import ops
+    cases = [Case(20 + i, counts, [0, 1, -1, 1], 8640 if i == 1 else 136, 264, 32, 2) for i, counts in enumerate(([5, 9, 2, 1], [40, 1, 7, 3], [300, 2, 90, 11]))]
+    r = np.random.default_rng(6)
+    steps = []
+    for c in cases:
+        x, A, B, starts, ids, scale, base = c.of("x A B starts ids scale base")
+        tok, old, adv, weight = dev(r.integers(0, 264, c.T)), dev(np.full(c.T, -5, np.float32)), dev(r.standard_normal(c.T).astype(np.float32)), dev(np.ones(c.T, np.float32))
+
+        def step(x=x, A=A, B=B, starts=starts, ids=ids, scale=scale, base=base, tok=tok, old=old, adv=adv, weight=weight, most=max(c.counts)):
+            z, h = ops.adapter_fwd(x, A, B, starts, ids, scale, base=base, max_new=most)
+            loss, logp, dz = ops.policy_loss(z, tok, old, adv, weight)
+            return [z, h, loss, logp, dz, *ops.adapter_bwd(x, A, B, starts, ids, scale, h, dz, max_new=most)]
+        steps.append(step)
+    want = [[t.clone() for t in step()] for step in steps]
+    torch.cuda.synchronize()
+    graphs, got = [], []
+    for step in steps[:2]:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            got.append(step())
+    side = torch.cuda.Stream()
+    for i in range(6):
+        with torch.cuda.stream(side):
+            third = steps[2]()
+        graphs[i % 2].replay()
+        graphs[(i + 1) % 2].replay()
+        if i % 2:
+            for t in got[0] + got[1]:
+                t.fill_(3)
+            torch.cuda.synchronize()
+            graphs[0].replay(), graphs[1].replay()
+        torch.cuda.synchronize()
+        for g, w in zip(got + [third], want):
+            assert all(torch.equal(a, b) for a, b in zip(g, w))
