@@ -11,7 +11,7 @@
 // workgroup: what is free depends on everything that is given back, and a barrier costs less there than a launch (a batch's table and
 // counts are some ten kilobytes).  Copying is bound by memory.
 //
-// On the device: fork 3 us for 8 as for 128 sequences, a launch's own time; fit 7.1 us for 8 sequences, 10.4 for 128, some six barriers with
+// On the device: fork 3 us for 8 as for 128 sequences, a launch's own time; fit 7.2 us for 8 sequences, 9.7 for 128, some six barriers with
 // a look at memory between each two; copies of 8 to 128 pages 4.4 to 6.9; packing 6.6 + 4.6 us and its 492 MB of copies 95, 5.2 TB/s.
 #include "common.h"
 
@@ -214,19 +214,31 @@ __global__ void __launch_bounds__(kThreads) fit_kernel(FitArgs a)
         a.slots[b] = a.asked[b] = 0;
     }
     __syncthreads();
-    // what is not needed goes back
+    // what is not needed goes back; some entries under way together
     {
+        constexpr int kAhead = 4;
         int b = (int)threadIdx.x / a.W, j = (int)threadIdx.x - b * a.W;
         const int db = kThreads / a.W, dj = kThreads - db * a.W;
-        for (; b < a.B; b += db, j += dj) {
-            if (j >= a.W && ++b >= a.B) break;
-            if (j >= a.W) j -= a.W;
-            bool ok;
-            const Span s = b < kHeld ? held[b] : span(a, b, &ok);
-            if (j < s.begin || j < s.need) continue;
-            const int x = *entry(b, j);
-            if (page(x)) less_one(a.refs + x);
-            if (x != -1) *entry(b, j) = -1;
+        while (b < a.B) {
+            int x[kAhead], *at[kAhead];
+            bool gone[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; i++) {
+                bool ok;
+                const int own = min(b, a.B - 1);
+                const Span s = own < kHeld ? held[own] : span(a, own, &ok);
+                gone[i] = b < a.B && j >= s.begin && j >= s.need;
+                at[i] = entry(own, j);
+                x[i] = *at[i];
+                b += db, j += dj;
+                if (j >= a.W) b++, j -= a.W;
+            }
+#pragma unroll
+            for (int i = 0; i < kAhead; i++) {
+                if (!gone[i]) continue;
+                if (page(x[i])) less_one(a.refs + x[i]);
+                if (x[i] != -1) *at[i] = -1;
+            }
         }
     }
     // what is written on is let go of

@@ -583,7 +583,7 @@ int cacti_hip_paged_fork(int64_t P, int64_t B, int64_t W, int64_t page, void *re
  * too is given up: where everybody who holds it does so, the first of them keeps it.  What is missing then is taken from the pages that
  * no one holds (refs 0), the lowest first, in the order of sequences and positions.  src, dst, slots [B] i32: the page of sequence b that
  * is to be copied, where to, and how many of its slots (-1, -1, 0: none) -- by cacti_hip_paged_copy, before anything is appended.
- * Where pages run out entries stay -1 and the sequence is named.  One workgroup: 5 to 10 us for a batch of up to 128, 60 for 2000, and 4 us
+ * Where pages run out entries stay -1 and the sequence is named.  One workgroup: 5 to 10 us for a batch of up to 128, 50 for 2000, and 4 us
  * more for 30000 pages that it has to look through. */
 size_t cacti_hip_paged_fit_workspace(int64_t P, int64_t B);
 int cacti_hip_paged_fit(int64_t P, int64_t B, int64_t W, int64_t page, void *refs, void *table, int64_t ldt, const void *first,
