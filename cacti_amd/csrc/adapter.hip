@@ -890,12 +890,13 @@ Workspace workspace(int64_t T, int64_t K, int64_t N, int64_t R, int64_t n)
 // How the forward pass is cut: in one launch, whose workgroups of 16 rows each form the h that they need, over all of K, with the columns
 // split until the device is full; or h first, from parts of K, and then y by 64 rows: a launch more, but A and B are read less often.  The
 // second, by us of both (the second's first), where
-//   K is long and A large, and the tiles leave half of the device idle: one row of 8640 to 3200, R = 32 10.9 and 13.3, R = 128 18.7 and 32.5,
-//     1200 rows 33 and 53; not with K = 3200, whose 600 rows with R = 128 take 27.2 and 24.3;
-//   there are rows for several rounds of tiles: 16 x 600 rows of 2048 to 2048, R = 8 27 and 29, R = 32 33 and 38, R = 128 70 and 80;
+//   K is long and A large, and the tiles leave half of the device idle: one row of 8640 to 3200, R = 32 10.6 and 13.3, R = 128 18.6 and 32.5,
+//     1200 rows 33 and 52; not with K = 3200, whose 600 rows with R = 128 take 27.1 and 23.4;
+//   there are rows for several rounds of tiles: 16 x 600 rows of 2048 to 2048, R = 8 27 and 29, R = 32 33 and 38, R = 128 67 and 80;
 //   the tiles are too few to fill the device and too many to split their columns, and A and B are large: 4 x 557 rows of 3200 to 8640,
-//     R = 64 33 and 45, but R = 16 24.0 and 23.4.
-// Everywhere else the first: one row of 3200 to 8640, R = 16 8.5 and 6.2, 2048 rows of 3200 to 3200 12.9 and 10.2, 4096 19.3 and 15.7.
+//     R = 64 33 and 45, but R = 16 23.3 either way.
+// Everywhere else the first: one row of 3200 to 8640, R = 16 8.5 and 6.2, 2048 rows of 3200 to 3200 13.2 and 10.4, 4096 19.1 and 15.7.
+// (Over 125 shapes the rule's choice is 0.6 % slower than the better one in the mean, 13 % at most.)
 struct ForwardPlan {
     bool two;
     int splits, planes;
@@ -916,7 +917,7 @@ ForwardPlan forward_plan(int64_t T, int64_t S, int64_t K, int64_t N, int64_t R, 
     const int rank = rank_of(R);
     const int64_t tiles = units(kTile).count;
     w.two = (K > 4096 && R * K > (1 << 18) && tiles <= cus / 2) || T >= 32 * cus ||
-            (tiles > cus / 2 && tiles < cus * 7 / 8 && R * (K + N) > (1 << 18));
+            (tiles > cus / 2 && tiles < cus && R * (K + N) > (1 << 18));
     if (!w.two) {
         w.splits = columns(cus, tiles, one_waves(rank));
         return w;
