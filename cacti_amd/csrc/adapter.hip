@@ -542,51 +542,80 @@ struct GradArgs {
     int64_t blocks;
 };
 
-// The rows of each adapter, sequence after sequence, by one workgroup of 8 waves.  A wave to an adapter.  (Sums no larger than T:
-// sequences that overlap may have more rows than there are.)
+// The rows of each adapter, sequence after sequence, by one workgroup of 8 waves: each of up to 8 counts the rows of its share of the
+// sequences by adapter (room: ints of LDS), then gives them their places, 64 sequences at a time.  (Sums no larger than T: sequences that
+// overlap may have more rows than there are.  300 sequences of 300 adapters, each adapter looking through them all: 111 us.)
 constexpr int kMaxAdapters = 1024;
-__device__ void plan(const GradArgs &d, int *counts)
+__device__ void plan(const GradArgs &d, int *room, int ints, int *totals)
 {
     const AdapterArgs &g = d.f;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int a = wave; a < g.n; a += 8) {
-        int c = 0;
-        for (int b0 = 0; b0 < g.pb.B; b0 += 64) {
-            int s0, n;
-            const int b = min(b0 + lane, g.pb.B - 1);
-            if (b0 + lane < g.pb.B && rows_of(g, b, &s0, &n) && adapter_of(g, b) == a) c = min(c + n, g.pb.T);
-        }
-        for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o);
-        if (lane == 0) counts[a] = min(c, g.pb.T);
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        int s = 0;
-        for (int a = 0; a < g.n; a++) {
-            const int c = counts[a];
-            counts[a] = s;
-            s = min(s + c, g.pb.T);
-        }
-        counts[g.n] = s;
-    }
-    __syncthreads();
-    for (int a = threadIdx.x; a <= g.n; a += 512) d.begin[a] = counts[a];
-    for (int a = wave; a < g.n; a += 8) {
-        int at = counts[a];
-        for (int b0 = 0; b0 < g.pb.B; b0 += 64) {
+    const int lane = threadIdx.x & 63, wave = wave_id(), T = g.pb.T, chunks = (g.pb.B + 63) / 64, shares = max(1, min(8, min(ints / g.n, chunks)));
+    int *const own = room + wave * g.n;
+    auto add = [&](int x, int y) __attribute__((always_inline)) { return min(x + y, T); };
+    auto each = [&](auto f) __attribute__((always_inline)) {     // f(adapter or -1, first row, rows, sequences)
+        if (wave >= shares) return;
+        for (int c = chunks * wave / shares; c < chunks * (wave + 1) / shares; c++) {
+            const int b = 64 * c + lane;
             int s0 = 0, n = 0;
-            const int b = min(b0 + lane, g.pb.B - 1);
-            const bool mine = b0 + lane < g.pb.B && rows_of(g, b, &s0, &n) && adapter_of(g, b) == a;
-            uint64_t todo = __ballot(mine && n > 0);
-            while (todo) {
-                const int l = __builtin_ctzll(todo);
-                todo &= todo - 1;
-                const int first = __builtin_amdgcn_readlane(s0, l), count = __builtin_amdgcn_readlane(n, l);
-                for (int i = lane; i < count && at + i < g.pb.T; i += 64) d.rows[at + i] = first + i;
-                at = min(at + count, g.pb.T);
-            }
+            const bool there = rows_of(g, min(b, g.pb.B - 1), &s0, &n) && b < g.pb.B && n > 0;
+            f(there ? adapter_of(g, b) : -1, s0, n, min(64, g.pb.B - 64 * c));
         }
+    };
+    auto count = [&](int a, int n) __attribute__((always_inline)) {
+        if (a < 0) return;
+        atomicAdd(own + a, n);                 // (64 of 2^24 and what was there: within 32 bits)
+        atomicMin(own + a, T);
+    };
+    for (int e = threadIdx.x; e < shares * g.n; e += 512) room[e] = 0;
+    __syncthreads();
+    each([&](int a, int, int n, int) __attribute__((always_inline)) { count(a, n); });
+    __syncthreads();
+    // two adapters to a thread: where their rows begin
+    const int a0 = 2 * (int)threadIdx.x;
+    int mine[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        for (int s = 0; s < shares && a0 + i < g.n; s++) mine[i] = add(mine[i], room[s * g.n + a0 + i]);
+    int before = add(mine[0], mine[1]);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(before, o);
+        if (lane >= o) before = add(before, x);
     }
+    if (lane == 63) totals[wave] = before;
+    before = __shfl_up(before, 1);
+    if (lane == 0) before = 0;
+    __syncthreads();
+    for (int w = 0; w < wave; w++) before = add(before, totals[w]);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        if (a0 + i >= g.n) break;
+        d.begin[a0 + i] = before;
+        int at = before;
+        for (int s = 0; s < shares; s++) {
+            const int c = room[s * g.n + a0 + i];
+            room[s * g.n + a0 + i] = at;
+            at = add(at, c);
+        }
+        before = at;
+        if (a0 + i == g.n - 1) d.begin[g.n] = at;
+    }
+    __syncthreads();
+    each([&](int a, int s0, int n, int sequences) __attribute__((always_inline)) {
+        int at = a >= 0 ? own[a] : T;
+        for (int l = 0; l < sequences; l++) {
+            const int al = __builtin_amdgcn_readlane(a, l), nl = __builtin_amdgcn_readlane(n, l);
+            if (l < lane && al == a) at = add(at, nl);
+        }
+        count(a, n);
+        uint64_t todo = __ballot(a >= 0);
+        while (todo) {
+            const int l = __builtin_ctzll(todo);
+            todo &= todo - 1;
+            const int first = __builtin_amdgcn_readlane(s0, l), rows = __builtin_amdgcn_readlane(n, l), to = __builtin_amdgcn_readlane(at, l);
+            for (int i = lane; i < rows && to + i < T; i += 64) d.rows[to + i] = first + i;
+        }
+    });
 }
 
 // The two terms of dh and h of 16 rows of a sequence; dx of rows without an adapter.  The first workgroup: the plan, the last: what does not fit.
@@ -597,9 +626,10 @@ __global__ void __launch_bounds__(512) dh_kernel(GradArgs d)
     typedef TileH<RT, 1, W, true> H;
     typedef Terms<RT> Two;
     __shared__ __attribute__((aligned(16))) half_t lds[std::max(W * H::kLds, 2 * W * kTile * C)], hs[kTile * Two::kPitch];
-    __shared__ int counts[kMaxAdapters + 1], largest[2][kTile];
+    __shared__ int largest[2][kTile];
+    static_assert(sizeof(lds) / 4 >= kMaxAdapters && 2 * 512 >= kMaxAdapters, "room for a count, a thread for two");
     const AdapterArgs &g = d.f;
-    if (blockIdx.x == 0) return plan(d, counts);
+    if (blockIdx.x == 0) return plan(d, reinterpret_cast<int *>(lds), (int)sizeof(lds) / 4, largest[0]);
     const int u = (int)blockIdx.x - 1;
     if (u >= (int)g.units.count) return look_over(g);
     const Tile t = find_tile(g, u, kTile);
@@ -776,24 +806,27 @@ __global__ void __launch_bounds__(256, RT == 8 ? 2 : 1) grad_kernel(GradArgs d)
         __syncthreads();
     }
     const float up = two_to(max(top, -126));
-    float *part = d.parts + (int64_t)u * R * (K + N);
+    const bool alone = d.begin[a + 1] - d.begin[a] <= d.per;      // (the only block: nothing to be joined)
+    const int64_t ofA = (int64_t)R * K, ofB = (int64_t)R * N;
+    float *const part = d.parts + (int64_t)u * (ofA + ofB) + (of_x ? 0 : ofA);
+    half_t *const to = of_x ? d.dA + a * ofA : d.dB + a * ofB;
+    const bool add = of_x ? d.dA_acc : d.dB_acc;
 #pragma unroll
     for (int i = 0; i < RT; i++)
 #pragma unroll
         for (int c = 0; c < 2; c++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                if (of_x) {
-                    const int r = 16 * i + 4 * q4 + e, k = c0 + 32 * wave + 16 * c + m;
-                    if (r < R && k < K) part[(int64_t)r * K + k] = up * acc[i][c][e];
-                } else {
-                    const int n = c0 + 32 * wave + 16 * c + 4 * q4 + e, r = 16 * i + m;
-                    if (r < R && n < N) part[(int64_t)R * K + (int64_t)n * R + r] = up * acc[i][c][e];
-                }
+                const int r = 16 * i + (of_x ? 4 * q4 + e : m), col = c0 + 32 * wave + 16 * c + (of_x ? m : 4 * q4 + e);
+                if (r >= R || col >= width) continue;
+                const int64_t at = of_x ? (int64_t)r * K + col : (int64_t)col * R + r;
+                const float v = up * acc[i][c][e];
+                if (alone) to[at] = add ? f2h(h2f(to[at]) + scale * v) : f2h(scale * v);
+                else part[at] = v;
             }
 }
 
-// The blocks' parts of an adapter's gradients added up, 4 elements to a thread
+// The parts of an adapter that has several blocks added up, and what has none made 0; 4 elements to a thread
 __global__ void __launch_bounds__(256) join_kernel(GradArgs d)
 {
     const AdapterArgs &g = d.f;
@@ -804,7 +837,7 @@ __global__ void __launch_bounds__(256) join_kernel(GradArgs d)
     half_t *to = isA ? d.dA + a * ofA + e : d.dB + (int64_t)a * g.R * g.N + (e - ofA);
     const bool acc = isA ? d.dA_acc : d.dB_acc;
     const int count = d.begin[a + 1] - d.begin[a], parts = (count + d.per - 1) / d.per;
-    if (parts == 0 && acc) return;
+    if (parts == 1 || (parts == 0 && acc)) return;
     const float *p = d.parts + unit_of(d, a) * size + e;
     float4_t s = zero4();
     for (int i = 0; i < parts; i++) s += *reinterpret_cast<const float4_t *>(p + i * size);

@@ -209,6 +209,14 @@ def test_in_two_launches(counts, ids, K, N, R):
 
 
 @GPU
+@pytest.mark.parametrize("S,n,most,R", [(1500, 1024, 1, 8), (700, 700, 2, 16), (130, 900, 7, 24), (2100, 3, 1, 8), (65, 2, 9, 72)])
+def test_many_sequences_and_many_adapters(S, n, most, R):
+    """Lists of rows by several waves, adapters without rows, with one block of them and with more."""
+    r = np.random.default_rng(S)
+    check(Case(S + n, [int(x) for x in r.integers(0, most + 1, S)], [int(x) for x in r.integers(-1, n, S)], 24, 40, R, n, behind=2), max_new=most)
+
+
+@GPU
 def test_gradient_against_differences():
     """Differences of sum(dy y) in float64 along random directions, at the kernel's gradients: y is linear in each of x, A and B, so a
     central difference is exact but for its own rounding."""
