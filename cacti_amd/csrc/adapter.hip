@@ -549,16 +549,17 @@ constexpr int kMaxAdapters = 1024;
 __device__ void plan(const GradArgs &d, int *room, int ints, int *totals)
 {
     const AdapterArgs &g = d.f;
-    const int lane = threadIdx.x & 63, wave = wave_id(), T = g.pb.T, chunks = (g.pb.B + 63) / 64, shares = max(1, min(8, min(ints / g.n, chunks)));
+    const int lane = threadIdx.x & 63, wave = wave_id(), T = g.pb.T, B = g.pb.B, shares = max(1, min(8, min(ints / g.n, B)));
     int *const own = room + wave * g.n;
     auto add = [&](int x, int y) __attribute__((always_inline)) { return min(x + y, T); };
     auto each = [&](auto f) __attribute__((always_inline)) {     // f(adapter or -1, first row, rows, sequences)
         if (wave >= shares) return;
-        for (int c = chunks * wave / shares; c < chunks * (wave + 1) / shares; c++) {
-            const int b = 64 * c + lane;
+        const int end = B * (wave + 1) / shares;
+        for (int b0 = B * wave / shares; b0 < end; b0 += 64) {
+            const int b = b0 + lane;
             int s0 = 0, n = 0;
-            const bool there = rows_of(g, min(b, g.pb.B - 1), &s0, &n) && b < g.pb.B && n > 0;
-            f(there ? adapter_of(g, b) : -1, s0, n, min(64, g.pb.B - 64 * c));
+            const bool there = rows_of(g, min(b, end - 1), &s0, &n) && b < end && n > 0;
+            f(there ? adapter_of(g, b) : -1, s0, n, min(64, end - b0));
         }
     };
     auto count = [&](int a, int n) __attribute__((always_inline)) {
