@@ -681,30 +681,33 @@ __device__ __forceinline__ int64_t unit_of(const GradArgs &d, int a) { return (i
 // in LDS, the next ones under way.
 constexpr int kMostRows = 512;                 // of a block
 template <int RT>
-__global__ void __launch_bounds__(256, RT == 8 ? 2 : 1) grad_kernel(GradArgs d)
+struct GradLds {
+    static constexpr int HP = Terms<RT>::kPitch, XP = kCols + 16;
+    // (A is in registers before the first rows come)
+    __attribute__((aligned(16))) half_t rows_and_terms[std::max(kRows * (XP + HP), 16 * RT * XP)], tiles[4][kTileHalves], less[4][kRows];
+    int exps[2][kRows], rows[kMostRows];
+};
+// rows first .. first + count - 1 of those of adapter a, unit u; columns from c0 on of x (and dx) or of dy.  (Either by itself: the operands of the
+// sums change places, and the compiler makes a branch at each instruction of one that does both.)
+template <int RT, bool of_x>
+__device__ __forceinline__ void grad(const GradArgs &d, GradLds<RT> &l, int u, int a, int first, int count, int c0)
 {
     typedef Terms<RT> Two;
-    constexpr int HP = Two::kPitch, XP = kCols + 16, NX = kRows * kCols / 8 / 256;
-    // (A is in registers before the first rows come)
-    __shared__ __attribute__((aligned(16))) half_t lds[std::max(kRows * (XP + HP), 16 * RT * XP)], tiles[4][kTileHalves], less[4][kRows];
-    __shared__ int exps[2][kRows], rows[kMostRows];
-    half_t *const xs = lds, *const hs = lds + kRows * XP, *const as = lds;
+    constexpr int HP = GradLds<RT>::HP, XP = GradLds<RT>::XP, NX = kRows * kCols / 8 / 256;
+    half_t *const xs = l.rows_and_terms, *const hs = xs + kRows * XP, *const as = xs;
+    auto &tiles = l.tiles;
+    auto &less = l.less;
+    auto &exps = l.exps;
+    auto &rows = l.rows;
     const AdapterArgs &g = d.f;
-    const int R = g.R, K = g.K, N = g.N, kchunks = (K + kCols - 1) / kCols, chunks = kchunks + (N + kCols - 1) / kCols;
-    const int u = (int)blockIdx.x / chunks, chunk = (int)blockIdx.x - u * chunks;
-    const bool of_x = chunk < kchunks;
-    const int c0 = kCols * (of_x ? chunk : chunk - kchunks), width = of_x ? K : N;
-    // (unit 0 is adapter 0's: one more than the adapters that begin behind it)
-    const int a = __builtin_amdgcn_readfirstlane(count_below(g.n - 1, u, [&](int i) { return unit_of(d, i); }));
-    const int first = d.begin[a] + (int)(u - unit_of(d, a)) * d.per, count = min(d.per, d.begin[a + 1] - first);
-    if (count <= 0) return;
+    const int R = g.R, K = g.K, N = g.N, width = of_x ? K : N;
     const int lane = threadIdx.x & 63, wave = wave_id(), m = lane & 15, q4 = lane >> 4;
     const float scale = g.scale[a];
     const half_t *src = of_x ? g.x : d.dy, *terms = d.terms[of_x ? 0 : 1];
     const int64_t ld = of_x ? g.ldx : d.lddy;
     const int *from_exps = d.exps[of_x ? 0 : 1];
     for (int e = threadIdx.x; e < count; e += 256) rows[e] = d.rows[first + e];
-    if (of_x)
+    if constexpr (of_x)
         for (int e = threadIdx.x; e < 16 * RT * (kCols / 8); e += 256) {
             const int r = e / (kCols / 8), c = 8 * (e % (kCols / 8));
             const half8_t w = load8(g.A + ((int64_t)a * R + min(r, R - 1)) * K + min(c0 + c, K - 8));
@@ -724,6 +727,7 @@ __global__ void __launch_bounds__(256, RT == 8 ? 2 : 1) grad_kernel(GradArgs d)
     load(0);
     // A of 32 columns a wave, 8 of them side by side in a lane
     half8_t w[Two::kN][2];
+    if constexpr (of_x)
 #pragma unroll
     for (int i = 0; i < Two::kN; i++)
 #pragma unroll
@@ -736,6 +740,30 @@ __global__ void __launch_bounds__(256, RT == 8 ? 2 : 1) grad_kernel(GradArgs d)
 #pragma unroll
     for (int i = 0; i < RT; i++) acc[i][0] = acc[i][1] = zero4();
     int top = -127;                            // exponent that the sums are scaled by
+    // the sums over rows: step s has rows 32 s + 4 q4 + 0 .. 3 and those 16 further, in both operands
+    auto sums = [&] () __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < kRows / 32; s++) {
+            const int row = 32 * s + 4 * q4 + (m >> 2);
+            const half_t *f = less[wave] + 32 * s + 4 * q4;
+            const half8_t part = both(*reinterpret_cast<const half4_t *>(f), *reinterpret_cast<const half4_t *>(f + 16));
+            half8_t xf[2];
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                const half_t *q = xs + row * XP + 32 * wave + 16 * c + 4 * (m & 3);
+                xf[c] = both(read_tr(q), read_tr(q + 16 * XP));
+            }
+#pragma unroll
+            for (int i = 0; i < RT; i++)
+#pragma unroll
+                for (int p = 0; p < 2; p++) {
+                    const half_t *q = hs + row * HP + p * Two::kLo + 16 * i + 4 * (m & 3);
+                    const half8_t hf = both(read_tr(q), read_tr(q + 16 * HP)) * part;
+#pragma unroll
+                    for (int c = 0; c < 2; c++) acc[i][c] = of_x ? mfma(hf, xf[c], acc[i][c]) : mfma(xf[c], hf, acc[i][c]);
+                }
+        }
+    };
     for (int r0 = 0, turn = 0; r0 < count; r0 += kRows, turn ^= 1) {
         const int left = count - r0;
 #pragma unroll
@@ -761,29 +789,8 @@ __global__ void __launch_bounds__(256, RT == 8 ? 2 : 1) grad_kernel(GradArgs d)
         }
         load(r0 + kRows);
         __syncthreads();
-        // the sums over rows: step s has rows 32 s + 4 q4 + 0 .. 3 and those 16 further, in both operands
-#pragma unroll
-        for (int s = 0; s < kRows / 32; s++) {
-            const int row = 32 * s + 4 * q4 + (m >> 2);
-            const half_t *f = less[wave] + 32 * s + 4 * q4;
-            const half8_t part = both(*reinterpret_cast<const half4_t *>(f), *reinterpret_cast<const half4_t *>(f + 16));
-            half8_t xf[2];
-#pragma unroll
-            for (int c = 0; c < 2; c++) {
-                const half_t *q = xs + row * XP + 32 * wave + 16 * c + 4 * (m & 3);
-                xf[c] = both(read_tr(q), read_tr(q + 16 * XP));
-            }
-#pragma unroll
-            for (int i = 0; i < RT; i++)
-#pragma unroll
-                for (int p = 0; p < 2; p++) {
-                    const half_t *q = hs + row * HP + p * Two::kLo + 16 * i + 4 * (m & 3);
-                    const half8_t hf = both(read_tr(q), read_tr(q + 16 * HP)) * part;
-#pragma unroll
-                    for (int c = 0; c < 2; c++) acc[i][c] = of_x ? mfma(hf, xf[c], acc[i][c]) : mfma(xf[c], hf, acc[i][c]);
-                }
-        }
-        if (of_x)
+        sums();
+        if constexpr (of_x)
 #pragma unroll
             for (int t = 0; t < kRows / 16; t++) {
                 if (16 * t >= left) break;
@@ -825,6 +832,20 @@ __global__ void __launch_bounds__(256, RT == 8 ? 2 : 1) grad_kernel(GradArgs d)
                 if (alone) to[at] = add ? f2h(h2f(to[at]) + scale * v) : f2h(scale * v);
                 else part[at] = v;
             }
+}
+
+template <int RT>
+__global__ void __launch_bounds__(256, RT == 8 ? 2 : RT == 4 ? 3 : 4) grad_kernel(GradArgs d)
+{
+    __shared__ GradLds<RT> l;
+    const int kchunks = (d.f.K + kCols - 1) / kCols, chunks = kchunks + (d.f.N + kCols - 1) / kCols;
+    const int u = (int)blockIdx.x / chunks, chunk = (int)blockIdx.x - u * chunks;
+    // (unit 0 is adapter 0's: one more than the adapters that begin behind it)
+    const int a = __builtin_amdgcn_readfirstlane(count_below(d.f.n - 1, u, [&](int i) { return unit_of(d, i); }));
+    const int first = d.begin[a] + (int)(u - unit_of(d, a)) * d.per, count = min(d.per, d.begin[a + 1] - first);
+    if (count <= 0) return;
+    if (chunk < kchunks) grad<RT, true>(d, l, u, a, first, count, kCols * chunk);
+    else grad<RT, false>(d, l, u, a, first, count, kCols * (chunk - kchunks));
 }
 
 // The parts of an adapter that has several blocks added up, and what has none made 0; 4 elements to a thread
