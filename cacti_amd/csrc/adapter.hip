@@ -835,17 +835,19 @@ __device__ __forceinline__ void grad(const GradArgs &d, GradLds<RT> &l, int u, i
 }
 
 template <int RT>
-__global__ void __launch_bounds__(256, RT == 8 ? 2 : RT == 4 ? 3 : 4) grad_kernel(GradArgs d)
+__global__ void __launch_bounds__(256, RT == 8 ? 2 : RT == 4 ? 3 : RT == 2 ? 4 : 5) grad_kernel(GradArgs d)
 {
     __shared__ GradLds<RT> l;
-    const int kchunks = (d.f.K + kCols - 1) / kCols, chunks = kchunks + (d.f.N + kCols - 1) / kCols;
-    const int u = (int)blockIdx.x / chunks, chunk = (int)blockIdx.x - u * chunks;
+    // (x's columns, which take longer, before dy's)
+    const int kchunks = (d.f.K + kCols - 1) / kCols, nchunks = (d.f.N + kCols - 1) / kCols, of_x = (int)d.blocks * kchunks;
+    const bool x = (int)blockIdx.x < of_x;
+    const int i = x ? (int)blockIdx.x : (int)blockIdx.x - of_x, u = i / (x ? kchunks : nchunks), chunk = i - u * (x ? kchunks : nchunks);
     // (unit 0 is adapter 0's: one more than the adapters that begin behind it)
     const int a = __builtin_amdgcn_readfirstlane(count_below(d.f.n - 1, u, [&](int i) { return unit_of(d, i); }));
     const int first = d.begin[a] + (int)(u - unit_of(d, a)) * d.per, count = min(d.per, d.begin[a + 1] - first);
     if (count <= 0) return;
-    if (chunk < kchunks) grad<RT, true>(d, l, u, a, first, count, kCols * chunk);
-    else grad<RT, false>(d, l, u, a, first, count, kCols * (chunk - kchunks));
+    if (x) grad<RT, true>(d, l, u, a, first, count, kCols * chunk);
+    else grad<RT, false>(d, l, u, a, first, count, kCols * chunk);
 }
 
 // The parts of an adapter that has several blocks added up, and what has none made 0; 4 elements to a thread
