@@ -15,8 +15,9 @@
 // What bounds it, with times on the device, 3200 to 3200, R = 16 where nothing else is said.  A few rows: the chain of a launch, numbers of
 // the sequence, x and A, the sum over the waves, B (one row 6.5 us, 64 sequences of up to 5 rows 8.1).  Many: memory.  2227 rows, 3200 to
 // 8640, R = 64: h 10.1 us, y 22.1 for 77 MB of base and y, 3.5 TB/s; between loads and stores stand the turns in LDS.  The adjoint of 4096
-// rows: 9.7 us for the terms of dh and h (dy read once), 20.6 for dx and the parts of dA and dB (79 MB, 3.8 TB/s), 4.0 to join those;
-// 269 rows of 1024 to 2816 take 7.7, 6.1 and 3.8, little more than launches.
+// rows: 9.8 us for the terms of dh and h (dy read once), 18.0 for dx and the parts of dA and dB (79 MB, 4.4 TB/s), 3.9 to join those;
+// 269 rows of 1024 to 2816 take 7.7, 5.9 and 3.8, little more than launches.  R = 128: 24, 44 and 7, of those 44 the matrix pipe 8, vector
+// operations 12 and LDS 13, which two waves to a SIMD do not bring together.
 #include <algorithm>
 
 #include "operands.h"
@@ -910,7 +911,7 @@ int rank_of(int64_t R) { return R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8; }
     } while (0)
 
 // rows of a block: as many workgroups as the device holds at once, counting those of blocks that are not full.  (4096 rows of 3200 to 3200,
-// R = 64: about 640 54 us, 768 57, 384 59; R = 128, two to a CU: 384 90, 640 101.)
+// R = 64: about 640 54 us, 768 57, 384 59; R = 128, two to a CU: 384 90, 640 101; before other steps that took 5 and 14 us off either.)
 int64_t block_rows(int64_t T, int64_t K, int64_t N, int64_t R)
 {
     const int64_t chunks = (K + kCols - 1) / kCols + (N + kCols - 1) / kCols, steps = (T + kRows - 1) / kRows;

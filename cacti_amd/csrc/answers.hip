@@ -11,7 +11,7 @@
 // depends on that row alone, so it is written from the same registers: one read and one write of the logits in all.  The pairs'
 // factors depend on whole texts: two reads and one write, and a launch of one workgroup a pair between them.
 //
-// Bound by memory.  On the device: the policy loss of 2048 rows of 32000, a third of them left out, 41.6 us, 5.4 TB/s of logits read and
+// Bound by memory.  On the device: the policy loss of 2048 rows of 32000, a third of them left out, 40.9 us, 5.4 TB/s of logits read and
 // gradient written; pairs of 1666 rows of 32000 15.5 + 5.5 + 26.4 us, 5.0 TB/s; 192 rows of 1024 4.0 us, a launch's own time.  Two
 // workgroups and more to a compute unit cover what a row waits for its sums.
 #include "operands.h"
