@@ -788,6 +788,13 @@ __device__ __forceinline__ void grad(const GradArgs &d, GradLds<RT> &l, int u, i
 #pragma unroll
             for (int i = 0; i < RT; i++) acc[i][0] *= f, acc[i][1] *= f;
         }
+        // (what dx is added to: before the next rows, which the wait for it would be one for too)
+        half8_t old[kRows / 16];
+        if constexpr (of_x)
+            if (g.base)
+#pragma unroll
+                for (int t = 0; t < kRows / 16; t++)
+                    old[t] = load8(g.base + (int64_t)rows[r0 + min(16 * t + mem_row(), left - 1)] * g.ldb + min(c0 + 32 * wave + mem_col(), K - 8));
         load(r0 + kRows);
         __syncthreads();
         sums();
@@ -808,7 +815,7 @@ __device__ __forceinline__ void grad(const GradArgs &d, GradLds<RT> &l, int u, i
                 const int r = 16 * t + mem_row(), c = c0 + 32 * wave + mem_col();
                 const int64_t row = rows[r0 + min(r, left - 1)];
                 half8_t y;
-                if (g.base) y = turned<true>(tiles[wave], load8(g.base + row * g.ldb + min(c, K - 8)), o, factor);
+                if (g.base) y = turned<true>(tiles[wave], old[t], o, factor);
                 else y = turned<false>(tiles[wave], zero8(), o, factor);
                 if (r < left && c < K) *reinterpret_cast<half8_t *>(g.y + row * g.ldy + c) = y;
             }
@@ -836,7 +843,7 @@ __device__ __forceinline__ void grad(const GradArgs &d, GradLds<RT> &l, int u, i
 }
 
 template <int RT>
-__global__ void __launch_bounds__(256, RT == 8 ? 2 : RT == 4 ? 3 : RT == 2 ? 4 : 5) grad_kernel(GradArgs d)
+__global__ void __launch_bounds__(256, RT == 8 ? 2 : RT == 4 ? 3 : 4) grad_kernel(GradArgs d)
 {
     __shared__ GradLds<RT> l;
     // (x's columns, which take longer, before dy's)
