@@ -125,6 +125,9 @@ __device__ __forceinline__ half_t *as_operand(half_t *tile)
     return tile + place(lane & 15, lane >> 4);
 }
 __device__ __forceinline__ void put8(half_t *p, half8_t v) { *reinterpret_cast<half8_t *>(p) = v; }
+// Waits for what a register is loaded with.  (Where a path goes by without a use of it the compiler waits before the register's next load, and for
+// all stores under way with it.)
+__device__ __forceinline__ void arrived(half8_t &v) { asm volatile("" : "+v"(v)); }
 // what a wave's lanes have written to LDS before is there for its lanes after (they take turns in order)
 __device__ __forceinline__ void in_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
@@ -333,9 +336,12 @@ struct Columns {
         in_order();
 #pragma unroll
         for (int i = 0; i < RT; i++) {
-            const int piece = 64 * i + lane;
-            if (piece < 32 * per) put8(bl + (piece / per) * pitch + 8 * (piece % per), w[i]);
+            const int piece = min(64 * i + lane, 4 * g.R - 1);       // (as it was loaded: behind the last the last again)
+            put8(bl + (piece / per) * pitch + 8 * (piece % per), w[i]);
         }
+        if constexpr (BASE)
+#pragma unroll
+            for (int b = 0; b < TB; b++) arrived(old[b]);
         in_order();
         half8_t wf[2][H::kN];
 #pragma unroll
@@ -347,7 +353,7 @@ struct Columns {
             }
 #pragma unroll
         for (int b = 0; b < TB; b++) {
-            if (16 * b >= t.rows) break;
+            if (b && 16 * b >= t.rows) break;
             float4_t o[2] = {zero4(), zero4()};
 #pragma unroll
             for (int i = 0; i < H::kN; i++)
