@@ -290,7 +290,8 @@ def distill_topk_bwd(logit, idx, val, stats, scale, temperature=1.0, acc=None):
 def token_logp_fwd(logit, tok, temperature=1.0, mask=None, status=None):
     """Log-probabilities of drawn tokens: (log softmax(logit / temperature)[tok] f32 [N], stats f32 [N, 2] for the adjoint).
 
-    logit f16 [N, V], rows may be strided; tok u16-as-int16 [N]; mask bool [N]: rows where it is False have 0 and are not read."""
+    logit f16 [N, V], rows may be strided; tok u16-as-int16 [N]; mask bool [N]: rows where it is False have 0 and are not read.  status: a
+    cleared int32 tensor of one element that becomes 1 + a row whose token is no token (it is left out too)."""
     return _op.token_logp_fwd(logit, tok, temperature, mask, status)
 
 
@@ -305,7 +306,8 @@ def policy_loss(logit, tok, old, adv, scale, ref=None, mask=None, clip=(0.2, 0.2
     logit f16), in one pass over the logits.
 
     With r = exp(logp - old) and d = ref - logp the loss of a row is -min(r adv, clip(r, 1 - clip[0], 1 + clip[1]) adv)
-    + beta (exp(d) - d - 1), the last term where ref is given.  old, adv, scale, ref: f32 [N]; mask as in token_logp_fwd."""
+    + beta (exp(d) - d - 1), the last term where ref is given.  old, adv, scale, ref: f32 [N]; mask and status as in token_logp_fwd; the
+    gradient is added to acc where given."""
     return _op.policy_loss(logit, tok, old, adv, scale, ref, mask, clip[0], clip[1], beta, temperature, acc, status)
 
 
@@ -315,7 +317,8 @@ def preference_loss(logp, ref, starts, scale, beta=0.1, smoothing=0.0, mask=None
 
     Rows starts[t] .. starts[t+1]-1 (int32 [2 pairs + 1] on the GPU) are text t, texts 2 i and 2 i + 1 pair i.  A text's reward is beta times
     the sum (mean: the mean) of logp - ref over its rows where mask is True, the loss -log sigmoid of the rewards' difference, with
-    smoothing a share of that of its opposite.  ref f32 [N] or None; scale f32 [pairs]."""
+    smoothing a share of that of its opposite.  ref f32 [N] or None; scale f32 [pairs].  status: a cleared int32 tensor of one element that
+    becomes 1 + a pair whose rows there are not (loss, rewards and gradient 0)."""
     return _op.preference_loss(logp, ref, starts, scale, beta, smoothing, mask, mean, status)
 
 
@@ -325,13 +328,14 @@ def adapter_fwd(x, A, B, starts, ids, scale, base=None, out=None, max_new=None, 
 
     Rows starts[s] .. starts[s+1]-1 of x f16 [T, K] are those of sequence s, whose adapter is a = ids[s] (-1: none, y = base): int32 tensors
     on the GPU that the host does not read.  A f16 [adapters, R, K], B f16 [adapters, N, R], scale f32 [adapters]; K, N, R multiples of 8,
-    R <= 128.  Rows of x, base and out may be strided by multiples of 8.  max_new: no sequence has more rows than that.  status: a
+    R <= 128.  Rows of x, base and out may be strided by multiples of 8; rows of no sequence are not written.  max_new: no sequence has more rows than that.  status: a
     cleared int32 tensor of one element that becomes 1 + s where the numbers of sequence s do not fit."""
     return _op.adapter_fwd(x, A, B, starts, ids, scale, base, out, max_new, status)
 
 
 def adapter_bwd(x, A, B, starts, ids, scale, h, dy, dx_acc=None, dA_acc=None, dB_acc=None, max_new=None, status=None):
-    """Its adjoint: (dx, dA, dB), f16.  h: what adapter_fwd returned; *_acc: tensors to add to, in place."""
+    """Its adjoint: (dx, dA, dB), f16.  h: what adapter_fwd returned; *_acc: tensors to add to, in place.  Rows of no sequence are not written
+    in dx."""
     return _op.adapter_bwd(x, A, B, starts, ids, scale, h, dy, dx_acc, dA_acc, dB_acc, max_new, status)
 
 
