@@ -3,7 +3,8 @@
 //
 //   fork     sequence b goes on as sequence parent[b]: its row becomes that one's, up to the pages that its positions take
 //   fit      each sequence gets what its positions need: pages behind them go back, missing ones are the lowest free ones, in the
-//            order of sequences and positions, and a page that is going to be written on by others too is copied first
+//            order of sequences and positions, and a page that is going to be written on by others too is copied first; one that there is
+//            no page for stays with who holds it and is not written on, its entry -2 - page
 //   compact  the held pages to the lowest places
 //   copy     the pages that the other two say, of all layers' caches in one launch
 //
@@ -23,6 +24,7 @@ namespace {
 __device__ __forceinline__ int load_now(const int *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
 __device__ __forceinline__ void store_now(int *p, int v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
 __device__ __forceinline__ void less_one(int *p) { __hip_atomic_fetch_add(p, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
+__device__ __forceinline__ void one_more(int *p) { __hip_atomic_fetch_add(p, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
 __device__ __forceinline__ void no_more_than(int *p, int v) { __hip_atomic_fetch_min(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
 // A barrier behind which the workgroup's counts in memory are what it made them: they are written and read past the first cache, in
 // an order that the barrier alone does not promise.
@@ -36,6 +38,8 @@ __device__ __forceinline__ void name(int *status, int b)
 {
     if (status) atomicMax(status, b + 1);
 }
+// The page that an entry holds, or an entry that holds none as it is
+__device__ __forceinline__ int page_of(int x, int P) { return x < -1 && -2 - x < P ? -2 - x : x; }
 __device__ __forceinline__ bool fits(int len, int W, int page) { return len >= 0 && len <= W * page; }
 
 // ---------------------------------------------------------------- fork
@@ -67,8 +71,8 @@ __global__ void __launch_bounds__(256) fork_kernel(ForkArgs a)
     const int *was = a.table + b * a.ldt, *from = a.table + max(p, 0) * a.ldt;
     int *to = a.new_table + b * a.ldn;
     for (int j = threadIdx.x; j < a.W; j += 256) {
-        const int x = was[j], y = j < need ? from[j] : -1;
-        to[j] = y;
+        const int x = page_of(was[j], a.P), raw = j < need ? from[j] : -1, y = page_of(raw, a.P);
+        to[j] = stays ? raw : y;
         if (x == y) continue;
         if (x >= 0 && x < a.P) atomicSub(a.refs + x, 1);
         if (y >= 0 && y < a.P) atomicAdd(a.refs + y, 1);
@@ -205,6 +209,7 @@ __global__ void __launch_bounds__(kThreads) fit_kernel(FitArgs a)
     __shared__ Span held[kHeld];
     auto entry = [&](int b, int j) __attribute__((always_inline)) { return a.table + b * a.ldt + j; };
     auto page = [&](int x) __attribute__((always_inline)) { return x >= 0 && x < a.P; };
+    auto held_by = [&](const int *entry) __attribute__((always_inline)) { return page_of(*entry, a.P); };
     for (int b = threadIdx.x; b < a.B; b += kThreads) {
         bool ok;
         const Span s = span(a, b, &ok);
@@ -236,29 +241,31 @@ __global__ void __launch_bounds__(kThreads) fit_kernel(FitArgs a)
 #pragma unroll
             for (int i = 0; i < kAhead; i++) {
                 if (!gone[i]) continue;
-                if (page(x[i])) less_one(a.refs + x[i]);
+                const int own = page_of(x[i], a.P);
+                if (page(own)) less_one(a.refs + own);
                 if (x[i] != -1) *at[i] = -1;
             }
         }
     }
     // what is written on is let go of
     each(a, held, [&](int b, const Span &s, int j, bool) __attribute__((always_inline)) {
-        const int x = j < s.need ? *entry(b, j) : -1;
+        const int x = j < s.need ? held_by(entry(b, j)) : -1;
         if (page(x)) less_one(a.refs + x);
     });
     settled();
     // a page that no one keeps goes to the first of those who want it again: b - B, below all counts
     each(a, held, [&](int b, const Span &s, int j, bool) __attribute__((always_inline)) {
-        const int x = j < s.need ? *entry(b, j) : -1;
+        const int x = j < s.need ? held_by(entry(b, j)) : -1;
         if (page(x) && load_now(a.refs + x) <= 0) no_more_than(a.refs + x, b - a.B);
     });
     settled();
     // who has none of its own asks for one
     each(a, held, [&](int b, const Span &s, int j, bool first) __attribute__((always_inline)) {
-        const int x = j < s.need ? *entry(b, j) : -1;
+        const int raw = j < s.need ? *entry(b, j) : -1, x = page_of(raw, a.P);
         const bool asks = j < s.need && !(page(x) && load_now(a.refs + x) == b - a.B);
         if (asks && s.part && j == s.begin && page(x)) a.src[b] = x;
         if (asks) *entry(b, j) = -1;
+        else if (x != raw) *entry(b, j) = x;
         const int n = __popc(lanes_with(asks));
         if (threadIdx.x % kLanes == 0) a.asked[b] = (first ? 0 : a.asked[b]) + n;
     });
@@ -291,7 +298,26 @@ __global__ void __launch_bounds__(kThreads) fit_kernel(FitArgs a)
         const bool copied = s.part && j == s.begin && a.src[b] >= 0;
         if (x < 0) name(a.status, b);
         if (copied && x >= 0) a.dst[b] = x, a.slots[b] = s.part;
-        if (copied && x < 0) a.src[b] = -1;
+    });
+    if (found >= all) return;
+    // pages ran out: what was to be copied and cannot be stays with its sequence
+    settled();
+    for (int b = threadIdx.x; b < a.B; b += kThreads) {
+        if (a.src[b] < 0 || a.dst[b] >= 0) continue;
+        bool ok;
+        one_more(a.refs + a.src[b]);
+        *entry(b, span(a, b, &ok).begin) = -2 - a.src[b];
+        a.src[b] = -1;
+    }
+    settled();
+    // .. and who would have kept such a page for itself does not write on it either
+    each(a, held, [&](int b, const Span &s, int j, bool) __attribute__((always_inline)) {
+        const int x = j < s.need ? *entry(b, j) : -1;
+        if (x < 0 || load_now(a.refs + x) <= 1) return;
+        name(a.status, b);
+        const bool part = s.part && j == s.begin;
+        *entry(b, j) = part ? -2 - x : -1;
+        if (!part) less_one(a.refs + x);
     });
 }
 
@@ -333,8 +359,8 @@ __global__ void __launch_bounds__(256) renumber_kernel(CompactArgs a)
     const int used = *a.used;
     int *row = a.table + blockIdx.x * a.ldt;
     for (int j = threadIdx.x; j < a.W; j += 256) {
-        const int x = row[j];
-        if (x >= used && x < a.P) row[j] = a.to[x];
+        const int x = row[j], p = page_of(x, a.P);
+        if (p >= used && p < a.P) row[j] = x < 0 ? -2 - a.to[p] : a.to[p];
     }
 }
 

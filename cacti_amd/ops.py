@@ -349,7 +349,9 @@ def paged_fork(refs, table, lens, parent, page, out=None, status=None):
 def paged_fit(refs, table, first, lens, page, status=None):
     """Gives each sequence the pages that lens[b] positions need, of which the first first[b] are there and the others will be written;
     pages behind them go back, and a page that others hold too is not written on.  refs and table are changed in place; returns (src, dst,
-    slots) for paged_copy, which comes before the append.  first <= lens; lens 0 frees a sequence.  status becomes 1 + b where there was no page."""
+    slots) for paged_copy, which comes before the append.  first <= lens; lens 0 frees a sequence.  status becomes 1 + b where there was no page:
+    its entry is -1, or -2 - page where that page was to be copied, which stays the sequence's and is written on by no one.  Append and
+    attention name such a sequence too; with pages free again the same call goes on from there."""
     return _op.paged_fit(refs, table, first, lens, page, status)
 
 

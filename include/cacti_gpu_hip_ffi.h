@@ -568,14 +568,16 @@ int cacti_hip_adapter_bwd(int64_t T, int64_t S, int64_t K, int64_t N, int64_t R,
 
 /* Pages of the cache above, handed out on the device.  refs [P] i32: how many hold a page (sequences of the table, and whoever else the
  * caller counts); table [B,W] i32 of pitch ldt: a sequence's pages in order, -1 behind them; lens [B] i32: its positions, page to a page.
- * Where nothing else is said lengths are 0 to W page.  A number that is no page of the cache is handed on and not counted.  P, B <= 2^28,
- * 2^20; W page <= 2^30; B W < 2^31.  What is written shares no memory with anything else but refs and table, changed in place.  status [1]
- * i32 or NULL: 1 + a sequence whose numbers do not fit, or for which there was no page.
+ * Where nothing else is said lengths are 0 to W page.  -2 - page: a page that the sequence holds but may not write on before it has a copy,
+ * which only cacti_hip_paged_fit makes, where pages run out; append and attention take it for a page that is not in the cache.  Any other number
+ * that is no page of the cache is handed on and not counted.  P, B <= 2^28, 2^20; W page <= 2^30; B W < 2^31.  What is written shares no memory with
+ * anything else but refs and table, changed in place.  status [1] i32 or NULL: 1 + a sequence whose numbers do not fit, or for which there was
+ * no page.
  *
  * Sequence b goes on as sequence parent[b] (which may be b; -1: empty): row b of new_table = row parent[b] of table as far as its
  * positions go, -1 behind; new_lens[b] = lens[parent[b]].  All at once, into other memory; refs is brought up to date.  Pages are shared then, also
- * one that is not full: cacti_hip_paged_fit before the next append.  A sequence whose parent or whose parent's length cannot be stays
- * as it is and is named. */
+ * one that is not full, and a -2 - page is its page again: cacti_hip_paged_fit before the next append.  A sequence whose parent or whose parent's
+ * length cannot be stays as it is and is named. */
 int cacti_hip_paged_fork(int64_t P, int64_t B, int64_t W, int64_t page, void *refs, const void *table, int64_t ldt, const void *lens,
                          const void *parent, void *new_table, int64_t ldn, void *new_lens, void *status, void *stream);
 /* Each sequence gets the pages that lens[b] positions need, of which the first first[b] are there and the others are going to be written
@@ -583,8 +585,10 @@ int cacti_hip_paged_fork(int64_t P, int64_t B, int64_t W, int64_t page, void *re
  * too is given up: where everybody who holds it does so, the first of them keeps it.  What is missing then is taken from the pages that
  * no one holds (refs 0), the lowest first, in the order of sequences and positions.  src, dst, slots [B] i32: the page of sequence b that
  * is to be copied, where to, and how many of its slots (-1, -1, 0: none) -- by cacti_hip_paged_copy, before anything is appended.
- * Where pages run out entries stay -1 and the sequence is named.  One workgroup: 5 to 10 us for a batch of up to 128, 50 for 2000, and 4 us
- * more for 30000 pages that it has to look through. */
+ * Where pages run out entries stay -1 and the sequence is named; one that was to be copied becomes -2 - page and nobody writes on its page: who
+ * would have kept it is named too and has -2 - page or, where it has nothing there, -1.  Once the copies that were named are made and pages are
+ * free again the same call, for those that were left out, goes on from there.  One workgroup: 5 to 10 us for a batch of up to 128, 50 for 2000,
+ * and 4 us more for 30000 pages that it has to look through. */
 size_t cacti_hip_paged_fit_workspace(int64_t P, int64_t B);
 int cacti_hip_paged_fit(int64_t P, int64_t B, int64_t W, int64_t page, void *refs, void *table, int64_t ldt, const void *first,
                         const void *lens, void *src, void *dst, void *slots, void *workspace, size_t workspace_bytes, void *status,

@@ -394,3 +394,174 @@ def test_captured_and_replayed():
                     if s >= 0:
                         x[d, :, :n] = x[s, :, :n]
                 assert torch.equal(got, x)
+
+
+# ---------------------------------------------------------------- pages that run out
+def page_of(x, P):
+    """The page that an entry holds, or what is none as it is: -2 - page is one that the sequence may not write on before there is a copy."""
+    return -2 - x if x < -1 and -2 - x < P else x
+
+
+def fit_that_keeps(refs, table, first, lens, page, W):
+    """The walk above.  A sequence that there is no page for keeps the one that it was to copy, and nobody writes on that."""
+    P = len(refs)
+    own = [[page_of(x, P) for x in row] for row in table]
+    refs, rows, src, dst, slots, bad = fit(refs, own, first, lens, page, W)
+    short, spans, bad = set(), [], set(bad)
+    for b in range(len(table)):
+        ok = 0 <= first[b] <= lens[b] <= W * page
+        need = -(-lens[b] // page)
+        spans.append((first[b] // page if first[b] < lens[b] else need, need) if ok else (W, 0))
+        rows[b][:spans[b][0]] = table[b][:spans[b][0]]
+    for b, (lo, need) in enumerate(spans):
+        if lo < need and first[b] % page and 0 <= own[b][lo] < P and rows[b][lo] == -1:
+            short.add(own[b][lo])
+            refs[own[b][lo]] += 1
+            rows[b][lo] = -2 - own[b][lo]
+    for b, (lo, need) in enumerate(spans):
+        for j in range(lo, need):
+            if rows[b][j] == own[b][j] and rows[b][j] in short:
+                bad.add(b)
+                if j == lo and first[b] % page:
+                    rows[b][j] = -2 - own[b][j]
+                else:
+                    rows[b][j] = -1
+                    refs[own[b][j]] -= 1
+    return refs, rows, src, dst, slots, bad
+
+
+class Short(Book):
+    """.. with what each position holds: a number of its own, written by the sequence that it is appended to."""
+
+    def __init__(self, *args):
+        super().__init__(*args)
+        self.slots = [[None] * self.page for _ in range(self.P)]
+        self.texts, self.next = [[] for _ in range(self.B)], 0
+
+    def at(self, b, p):
+        return page_of(self.table[b][p // self.page], self.P), p % self.page
+
+    def grow(self, lens, back=None):
+        """To these lengths, from those now or from `back` on; the sequences that were left out."""
+        from cacti_amd import ops
+        first = [min(a, b) for a, b in zip(back or self.lens, lens)]
+        out = [x.cpu().tolist() for x in ops.paged_fit(self.d_refs, self.d_table, ints(first), ints(lens), self.page, status=self.status)]
+        self.refs, self.table, *want, bad = fit_that_keeps(self.refs, self.table, first, lens, self.page, self.W)
+        self.same()
+        assert out == want
+        self.named(bad)
+        was = [list(x) for x in self.slots]
+        for s, d, n in zip(*out):
+            if s >= 0:
+                self.slots[d][:n] = was[s][:n]
+        for b in range(self.B):
+            self.lens[b] = first[b] if b in bad else lens[b]
+            del self.texts[b][first[b]:]
+            for p in range(first[b], self.lens[b]):
+                self.texts[b].append(self.next)
+                x, slot = self.at(b, p)
+                assert x == self.table[b][p // self.page]
+                self.slots[x][slot] = self.next
+                self.next += 1
+        self.right()
+        return sorted(bad)
+
+    def right(self):
+        for b in range(self.B):
+            assert [self.slots[x][i] for x, i in (self.at(b, p) for p in range(self.lens[b]))] == self.texts[b]
+        held = [0] * self.P
+        for row in self.table:
+            for x in row:
+                if page_of(x, self.P) >= 0:
+                    held[page_of(x, self.P)] += 1
+        assert held == self.refs
+
+    def go_on(self, parent):
+        self.table = [[page_of(x, self.P) for x in row] for row in self.table]
+        self.fork(parent)
+        self.texts = [list(self.texts[p]) if p >= 0 else [] for p in parent]
+        self.right()
+
+    def pack(self):
+        from cacti_amd import ops
+        src, dst, used = [x.cpu().tolist() for x in ops.paged_compact(self.d_refs, self.d_table)]
+        marked = [[x < -1 for x in row] for row in self.table]
+        self.refs, table, *want = compact(self.refs, [[page_of(x, self.P) for x in row] for row in self.table])
+        self.table = [[-2 - x if m else x for x, m in zip(*rows)] for rows in zip(table, marked)]
+        self.same()
+        assert [src, dst, used] == want
+        for s, d in zip(src, dst):
+            if s >= 0:
+                self.slots[d] = list(self.slots[s])
+        self.right()
+
+
+@GPU
+def test_a_page_that_there_was_no_copy_for_stays_the_sequences():
+    k = Short(1, 3, 3, 16, 3)
+    assert k.grow([20, 0, 0]) == []
+    k.go_on([0, 0, 0])
+    # all three write on page 1: the second gets the last page there is, the third none, and so the first, who would keep it, does not write on it
+    assert k.grow([21, 21, 21]) == [0, 2]
+    assert k.table == [[0, -3, -1], [0, 2, -1], [0, -3, -1]] and k.refs == [3, 2, 1]
+    assert k.grow([21, 21, 21]) == [0, 2] and k.table[2] == [0, -3, -1]
+    assert k.grow([20, 0, 21]) == [] and k.table == [[0, -3, -1], [-1] * 3, [0, 2, -1]]
+    assert k.grow([21, 0, 22]) == [] and k.table == [[0, 1, -1], [-1] * 3, [0, 2, -1]]
+    # .. of others who hold it and do not write
+    k = Short(2, 2, 2, 16, 2)
+    k.grow([24, 0])
+    k.go_on([0, 0])
+    assert k.grow([24, 25]) == [1] and k.table == [[0, 1], [0, -3]] and k.refs == [2, 2]
+    # .. of one who goes back and would write over all of it
+    k = Short(3, 2, 3, 16, 2)
+    k.grow([24, 0])
+    k.go_on([0, 0])
+    assert k.grow([17, 25], back=[16, 24]) == [0, 1] and k.table == [[0, -1, -1], [0, -3, -1]] and k.refs == [2, 1]
+    assert k.grow([0, 25]) == [] and k.table[1] == [0, 1, -1]
+    # a sequence that ends, forks and packs with such an entry
+    k = Short(4, 3, 2, 16, 3)
+    k.grow([24, 0, 0])
+    k.go_on([0, 0, -1])
+    assert k.grow([24, 24, 16]) == [] and k.grow([25, 25, 17]) == [0, 1, 2]
+    k.grow([24, 24, 0])
+    k.go_on([1, 1, 1])
+    assert k.grow([25, 24, 24]) == [] and k.grow([25, 25, 25]) == [1, 2]
+    assert k.grow([0, 24, 24]) == []
+    k.pack()
+    assert min(k.table[1]) < -1
+    assert k.grow([0, 0, 25]) == [] and k.refs == [1, 1, 0]
+
+
+@GPU
+@pytest.mark.parametrize("seed,B,W,page,P", [(1, 5, 4, 16, 6), (2, 12, 5, 16, 14), (3, 40, 6, 32, 45), (4, 3, 2, 16, 3), (5, 200, 3, 16, 180)])
+def test_answers_from_a_pool_that_is_too_small(seed, B, W, page, P):
+    """Sequences that grow, fork and end while pages run out again and again: what each has written is there, and who was left out goes on
+    when there are pages."""
+    print("pages", seed, B, W, page, P, flush=True)
+    k, out, copied = Short(seed, B, W, page, P), 0, 0
+    r, most = k.r, W * page
+    for step in range(25):
+        alive = [b for b in range(B) if k.lens[b]]
+        kind = r.choice(["grow", "fork", "fork", "free", "back", "pack"]) if alive else "prompts"
+        if kind == "prompts":
+            k.grow([r.randint(1, 2 * page) if b % 3 == 0 else 0 for b in range(B)])
+        elif kind == "fork":
+            k.go_on([b if r.random() < 0.4 else r.choice(alive) for b in range(B)])
+        elif kind == "free":
+            k.grow([l if r.random() < 0.7 else 0 for l in k.lens])
+        elif kind == "back":
+            back = [r.randint(max(0, l - 5), l) for l in k.lens]
+            k.grow([min(most, l + r.randint(0, 4)) for l in back], back)
+        elif kind == "pack":
+            k.pack()
+        parts = [page_of(k.table[b][l // page], P) for b, l in enumerate(k.lens) if l % page]
+        bad = k.grow([min(most, l + r.choice([0, 1, 1, 3])) if l else 0 for l in k.lens])
+        out += len(bad)
+        copied += len(parts) - len(set(parts))
+    assert out > 0 and copied > 0
+    while True:                                # the others end, one by one, until everybody goes on
+        bad = k.grow([min(most, l + 1) if l else 0 for l in k.lens])
+        if not bad:
+            break
+        alive = [b for b in range(B) if k.lens[b] and b not in bad] or bad[1:]
+        k.grow([0 if b == alive[0] else l for b, l in enumerate(k.lens)])
