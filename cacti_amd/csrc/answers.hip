@@ -189,6 +189,16 @@ __device__ __forceinline__ float exp_beyond_line(float d)
     return s * d * d;
 }
 
+// a e^x, also where only e^x is beyond fp32 (e^64 = kFar is taken out of it first, exactly where it matters); of a = 0 nothing, unless x is no number
+constexpr float kFar = 6.2351490808116169e27f;
+__device__ __forceinline__ float times_exp(float a, float x)
+{
+    if (a == 0.f && x == x) return a;
+    const bool far = x > 64.f;
+    const float e = a * expf(far ? x - 64.f : x);
+    return far ? e * kFar : e;
+}
+
 template <int T, int NP>
 __global__ void __launch_bounds__(T) policy_kernel(TokenArgs a)
 {
@@ -205,20 +215,21 @@ __global__ void __launch_bounds__(T) policy_kernel(TokenArgs a)
     const float zx = h2f(z.row[x]), old = a.old[n], adv = a.adv[n], ref = a.ref ? a.ref[n] : 0.f, scale = a.scale[n];
     const RowStats r = row_stats(h, zx, a.inv_temp);
     const float ratio = expf(r.logp - old), clipped = fminf(fmaxf(ratio, 1.f - a.lo), 1.f + a.hi);
-    const float free = ratio * adv, bound = clipped * adv;
+    const float free = times_exp(adv, r.logp - old), bound = clipped * adv;
     // (a NaN in either stays one)
     float loss = free <= bound ? -free : free > bound ? -bound : NAN;
     float slope = free <= bound ? -free : free > bound ? 0.f : NAN;
-    if (a.ref) {
+    if (a.ref && a.beta > 0.f) {
         const float d = ref - r.logp;
-        loss += a.beta * exp_beyond_line(d);
-        slope -= a.beta * expm1f(d);
+        const bool far = d > 64.f;             // (1 and d are below 2^-80 of e^d)
+        loss += far ? times_exp(a.beta, d) : a.beta * exp_beyond_line(d);
+        slope -= far ? times_exp(a.beta, d) : a.beta * expm1f(d);
     }
     if (threadIdx.x == 0) {
         a.loss[n] = loss;
         a.logp[n] = r.logp;
     }
-    const float c = slope * scale * a.inv_temp;
+    const float c = scale == 0.f && slope == slope ? 0.f : slope * scale * a.inv_temp;       // (none of an infinite slope is nothing)
     if (c == 0.f) return put_nothing(a, to, g, h);
     put_gradient(a, to, g, h, x, r.mx, r.sum, c);
 }

@@ -306,8 +306,8 @@ def policy_loss(logit, tok, old, adv, scale, ref=None, mask=None, clip=(0.2, 0.2
     logit f16), in one pass over the logits.
 
     With r = exp(logp - old) and d = ref - logp the loss of a row is -min(r adv, clip(r, 1 - clip[0], 1 + clip[1]) adv)
-    + beta (exp(d) - d - 1), the last term where ref is given.  old, adv, scale, ref: f32 [N]; mask and status as in token_logp_fwd; the
-    gradient is added to acc where given."""
+    + beta (exp(d) - d - 1), the last term where ref is given and beta is not 0.  old, adv, scale, ref: f32 [N]; mask and status as in
+    token_logp_fwd; the gradient is added to acc where given."""
     return _op.policy_loss(logit, tok, old, adv, scale, ref, mask, clip[0], clip[1], beta, temperature, acc, status)
 
 

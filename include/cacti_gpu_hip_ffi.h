@@ -525,8 +525,9 @@ int cacti_hip_token_logp_bwd(int64_t N, int64_t V, const void *logit16, int64_t 
 /* Clipped policy loss of drawn tokens and its gradient in one pass over the logits: with lp as above, r = exp(lp - old), d = ref - lp
  *   loss[n] = -min(r A, clip(r, 1 - clip_lo, 1 + clip_hi) A) + beta (exp(d) - d - 1)
  *   dlogit[j] (+)= f16(scale[n] / temperature * dloss/dlp * ([j = tok[n]] - p_j)),  dloss/dlp = -[r A <= clip(r) A] r A + beta (1 - exp(d))
- * old, adv (A), scale, loss, logp (lp), ref: [N] f32; ref NULL: without the last term.  mask, tok, status, dlogit16 as above (a row that is
- * left out: loss 0, logp 0, gradient 0). */
+ * old, adv (A), scale, loss, logp (lp), ref: [N] f32; ref NULL or beta 0: without the last term.  A and beta are taken into r and exp(d) before
+ * either leaves fp32's range, and of an A or a scale of 0 there is nothing, however large what it is multiplied with.  mask, tok, status,
+ * dlogit16 as above (a row that is left out: loss 0, logp 0, gradient 0). */
 int cacti_hip_policy_loss(int64_t N, int64_t V, const void *logit16, int64_t ld, const void *tok, const void *mask, const void *old,
                           const void *adv, const void *ref, const void *scale, double clip_lo, double clip_hi, double beta,
                           double temperature, void *loss, void *logp, void *dlogit16, int64_t ldd, int acc, void *status, void *stream);

@@ -414,3 +414,50 @@ def test_captured_and_replayed():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
         z.copy_(torch.roll(z, 3, 1))
+
+
+@GPU
+def test_a_reference_or_an_old_policy_far_off():
+    """Ratios and e^d beyond fp32, which a coefficient brings back or makes nothing of: without a divergence term (beta 0) what ref is does not
+    matter, an advantage of 0 has no loss, and what fp32 can hold is held (e^x's error is that of x, as bounded above)."""
+    from cacti_amd import ops
+    r, z, tok = make(13, 9, 64)
+    old, adv, ref, scale = policy_inputs(r, z, tok, 1.0)
+    scale[:] = 1
+    z[0, tok[0]] = -np.inf                                                             # a token that the model rules out
+    for n, d in ((1, 90), (2, 95), (3, 70)):
+        z[n, tok[n]] = z[n].max() - d
+    old[:4] = rows64(z, tok, 1.0)[1][:4]
+    old[0], ref[:4], adv[:4] = 0, 0, 0.5
+    lp = rows64(z, tok, 1.0)[1]
+    old[4:8], adv[4:8] = lp[4:8] - [95, 92, 200, 95], [-1e-4, 0, 0, 0.3]
+    args = [dev(x) for x in (z, tok, old, adv, scale)]
+    bare, off = ops.policy_loss(*args), ops.policy_loss(*args, ref=dev(ref))
+    for a, b in zip(bare, off):
+        assert np.array_equal(a.cpu().numpy(), b.cpu().numpy(), equal_nan=True)
+    at = np.arange(1, 9)                                                               # (the first row: no numbers to compare with)
+    for out, beta in ((bare, 0.0), (ops.policy_loss(*args, ref=dev(ref), beta=0.01), 0.01)):
+        loss, logp, grad = (x.cpu().numpy() for x in out)
+        wl, tl, wp, tp, wg, tg = policy64(z[at], tok[at], old[at], adv[at], ref[at] if beta else None, scale[at], 0.2, 0.2, beta, 1.0)
+        near(logp[at], wp, tp, "logp")
+        # (the bound of a loss has the ratio's error also where the ratio is clipped; there it is that of adv = 0 and one product)
+        clipped = np.where(at == 7, 0, adv[at]).astype(np.float32)
+        tl[6] = policy64(z[at], tok[at], old[at], clipped, ref[at] if beta else None, scale[at], 0.2, 0.2, beta, 1.0)[1][6] + 2.0 ** -22
+        # what fp32 cannot hold is infinite, and no number of its gradient one that could be taken for it
+        fits32 = np.abs(wl) < 3.4e38
+        assert np.array_equal(fits32, at != 2) if beta else fits32.all()
+        assert np.isposinf(loss[at][~fits32]).all() and not np.isfinite(grad[at][~fits32]).any()
+        near(loss[at][fits32], wl[fits32], tl[fits32], "loss")
+        wg, tg, grad = wg[fits32], tg[fits32], grad[at][fits32]
+        fits = np.abs(wg) < 60000                                                      # (beyond: infinite in f16)
+        assert np.isinf(grad[np.abs(wg) > 70000]).all() and not np.isnan(grad).any()
+        near(np.where(fits, grad, 0), np.where(fits, wg, 0), tg, "gradient")
+        assert np.isneginf(logp[0]) and (np.isposinf(loss[0]) if beta else loss[0] == 0 and not bool(out[2][0].any()))
+    assert bare[0][5] == 0 and bare[0][6] == 0 and not bare[2][5:8].any()
+    # .. and none of an infinite slope
+    scale[:2] = 0
+    _, _, grad = ops.policy_loss(*args[:4], dev(scale), ref=dev(ref), beta=0.01)
+    assert not grad[:2].any()
+    old[6] = np.nan                                                                    # (what is no number stays one)
+    loss, _, grad = ops.policy_loss(args[0], args[1], dev(old), *args[3:])
+    assert bool(loss[6].isnan()) and bool(grad[6].isnan().all())
