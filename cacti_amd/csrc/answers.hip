@@ -309,25 +309,44 @@ __device__ __forceinline__ double block_sum_f64(double v, double *red)
 
 __device__ __forceinline__ double log_sigmoid(double x) { return fmin(x, 0.) - log1p(exp(-fabs(x))); }
 
-// A workgroup to a pair; the last one: rows of no pair
+// Whether the rows of pair i are there
+__device__ __forceinline__ bool there(const PairArgs &a, int i)
+{
+    const int *s = a.starts + 2 * i;
+    return s[0] >= 0 && s[1] >= s[0] && s[2] >= s[1] && s[2] <= a.N;
+}
+
+// A workgroup to a pair, and one for the rows before the first and behind the last.  Where pairs are not there the first of a run of them clears what
+// lies between those on either side that are: a number that is wrong says nothing of where other pairs' rows are.
 __global__ void __launch_bounds__(kPairThreads) preference_kernel(PairArgs a)
 {
     __shared__ double red[kPairThreads / 64];
+    __shared__ int next;
     const int i = blockIdx.x, N = (int)a.N;
+    auto clear = [&](int first, int last) __attribute__((always_inline)) {
+        for (int n = first + (int)threadIdx.x; n < last; n += kPairThreads) a.dlogp[n] = 0.f;
+    };
     if (i == a.pairs) {
-        const int first = min(max(a.starts[0], 0), N), last = min(max(a.starts[2 * a.pairs], 0), N);
-        for (int n = threadIdx.x; n < N; n += kPairThreads)
-            if (n < first || n >= last) a.dlogp[n] = 0.f;
+        if (there(a, 0)) clear(0, a.starts[0]);
+        if (there(a, a.pairs - 1)) clear(a.starts[2 * a.pairs], N);
         return;
     }
     const int s[3] = {a.starts[2 * i], a.starts[2 * i + 1], a.starts[2 * i + 2]};
-    if (!(s[0] >= 0 && s[1] >= s[0] && s[2] >= s[1] && s[2] <= N)) {
-        const int first = max(min(s[0], min(s[1], s[2])), 0), last = min(max(s[0], max(s[1], s[2])), N);
-        for (int n = first + (int)threadIdx.x; n < last; n += kPairThreads) a.dlogp[n] = 0.f;
+    if (!there(a, i)) {
         if (threadIdx.x == 0) {
             a.loss[i] = a.reward[2 * i] = a.reward[2 * i + 1] = 0.f;
             if (a.status) atomicMax(a.status, i + 1);
+            next = a.pairs;
         }
+        if (i > 0 && !there(a, i - 1)) return;
+        __syncthreads();
+        for (int j = i + 1 + (int)threadIdx.x; j < a.pairs; j += kPairThreads)
+            if (there(a, j)) {
+                atomicMin(&next, j);
+                break;
+            }
+        __syncthreads();
+        clear(i > 0 ? s[0] : 0, next < a.pairs ? a.starts[2 * next] : N);
         return;
     }
     double reward[2], each[2];

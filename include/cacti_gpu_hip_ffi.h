@@ -538,7 +538,8 @@ int cacti_hip_policy_loss(int64_t N, int64_t V, const void *logit16, int64_t ld,
  *   h = reward[2 i] - reward[2 i + 1],  loss[i] = -(1 - smoothing) log sigma(h) - smoothing log sigma(-h)
  *   dlogp[n] = scale[i] dloss/dlogp, 0 for rows that the mask leaves out and rows of no text
  * logp, ref (or NULL: 0), dlogp: [N] f32; scale, loss: [pairs]; reward: [2 pairs].  In fp64.  status: 1 + a pair whose rows there are not
- * (its loss, rewards and gradient are 0; what others that share rows with it get is unspecified). */
+ * (its loss, rewards and gradient are 0).  Pairs that are there have their own values, whatever the others' numbers are, as long as no two of
+ * them share rows and each begins behind those before it. */
 int cacti_hip_preference_loss(int64_t N, int64_t pairs, const void *logp, const void *ref, const void *mask, const void *starts,
                               const void *scale, double beta, double smoothing, int mean, void *loss, void *reward, void *dlogp,
                               void *status, void *stream);

@@ -461,3 +461,50 @@ def test_a_reference_or_an_old_policy_far_off():
     old[6] = np.nan                                                                    # (what is no number stays one)
     loss, _, grad = ops.policy_loss(args[0], args[1], dev(old), *args[3:])
     assert bool(loss[6].isnan()) and bool(grad[6].isnan().all())
+
+
+@GPU
+@pytest.mark.parametrize("wrong", [{k: v} for k in range(9) for v in (-5, 100, 2 ** 31 - 1, -2 ** 31)] +
+                         [{0: 24}, {8: 1}, {8: 0}, {3: 4}, {5: 3}, {2: 99, 5: -1}, {1: -1, 3: 99, 5: -1, 7: 99}, {0: 30, 8: -1}])
+def test_a_wrong_number_costs_its_own_pairs_alone(wrong):
+    """All rows that a good pair has hold what they do where all numbers are right, whatever the others are; all else is 0."""
+    import torch
+    from cacti_amd import ops
+    r = np.random.default_rng(14)
+    good = [2, 5, 7, 11, 12, 16, 19, 22, 25]
+    logp, ref, scale = r.standard_normal(28).astype(np.float32), r.standard_normal(28).astype(np.float32), r.standard_normal(4).astype(np.float32)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    run = lambda s: [x.cpu().numpy() for x in ops.preference_loss(dev(logp), dev(ref), dev(np.array(s, np.int32)), dev(scale), 0.2, status=status)]
+    want = run(good)
+    bad = sorted({i for k in wrong for i in (k // 2, (k - 1) // 2) if 0 <= i < 4})
+    for i in bad:
+        want[0][i] = want[1][2 * i] = want[1][2 * i + 1] = 0
+        want[2][good[2 * i]:good[2 * i + 2]] = 0
+    assert int(status) == 0
+    for _ in range(3):
+        status.zero_()
+        out = run([wrong.get(k, s) for k, s in enumerate(good)])
+        assert int(status) == 1 + max(bad)
+        for got, w in zip(out, want):
+            assert np.array_equal(got, w)
+
+
+@GPU
+def test_many_pairs_that_there_are_not():
+    """Runs of them longer than a workgroup looks at in one go, between pairs that there are."""
+    from cacti_amd import ops
+    r = np.random.default_rng(15)
+    P, N = 1500, 6000
+    good = 2 * np.arange(2 * P + 1)
+    logp, scale = r.standard_normal(N + 5).astype(np.float32), r.standard_normal(P).astype(np.float32)
+    for runs in ([(0, P)], [(3, 700), (701, 1490)], [(0, 256), (257, 300), (900, P)], [(1, 2)]):
+        starts, ok = good.copy(), np.ones(P, bool)
+        for lo, hi in runs:
+            starts[2 * lo + 1:2 * hi:2] = -7
+            ok[lo:hi] = False
+        loss, reward, d = (x.cpu().numpy() for x in ops.preference_loss(dev(logp), None, dev(starts.astype(np.int32)), dev(scale), 0.3))
+        wl, wr, wd = pairs64(logp, None, good, scale, 0.3, 0.0, None, False)
+        wd[:N] *= np.repeat(ok, 4)
+        for got, want in ((loss, wl * ok), (reward, wr * np.repeat(ok, 2)), (d, wd)):
+            near(got, want, 2.0 ** -24 * np.abs(want) + 1e-12, "of a pair")
+            assert not got[want == 0].any()
