@@ -19,6 +19,7 @@
 // 269 rows of 1024 to 2816 take 7.7, 5.9 and 3.8, little more than launches.  R = 128: 24, 44 and 7, of those 44 the matrix pipe 8, vector
 // operations 12 and LDS 13, which two waves to a SIMD do not bring together.
 #include <algorithm>
+#include <initializer_list>
 
 #include "operands.h"
 #include "paged.h"
@@ -913,6 +914,19 @@ int check(const char *who, int64_t T, int64_t S, int64_t K, int64_t N, int64_t R
     return 0;
 }
 
+// Memory that a call reads or writes, from its first element to its last, in halves
+struct Extent {
+    const void *at;
+    int64_t size;
+};
+Extent rows_extent(int64_t T, const void *p, int64_t ld, int64_t width) { return {p, p ? (T - 1) * ld + width : 0}; }
+bool share(const Extent &a, std::initializer_list<Extent> others)
+{
+    for (const Extent &b : others)
+        if (b.size && rows_share(1, a.at, 0, a.size, b.at, 0, b.size)) return true;
+    return false;
+}
+
 // RT of 1, 2, 4 or 8: R rounded up to 16 of them
 int rank_of(int64_t R) { return R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8; }
 #define CACTI_BY_RANK(R, launch)        \
@@ -1028,6 +1042,10 @@ CACTI_API int cacti_hip_adapter_fwd(int64_t T, int64_t S, int64_t K, int64_t N, 
     const ForwardPlan w = forward_plan(T, S, K, N, R, g.max_new);
     CACTI_REQUIRE(ws_bytes >= w.bytes && (ws || !w.bytes) && aligned(ws, 16), CACTI_E_INVALID, "adapter_fwd: workspace of %zu bytes, %zu needed, 16-byte aligned",
                   ws_bytes, w.bytes);
+    // (some workgroups read while others write)
+    const Extent eA = {A, n * R * K}, eB = {B, n * N * R}, eh = {h, 2 * T * R};
+    CACTI_REQUIRE(!share(rows_extent(T, y, ldy, N), {eA, eB, eh}) && !share(eh, {rows_extent(T, x, ldx, K), rows_extent(T, base, ldb, N), eA, eB}), CACTI_E_INVALID,
+                  "adapter_fwd: y or h shares memory with an operand or the other");
     hipStream_t st = (hipStream_t)stream;
     if (!w.two) {
         g.splits = w.splits;
@@ -1085,6 +1103,12 @@ CACTI_API int cacti_hip_adapter_bwd(int64_t T, int64_t S, int64_t K, int64_t N, 
     CACTI_REQUIRE(ws_bytes >= w.bytes, CACTI_E_INVALID, "adapter_bwd: workspace of %zu bytes, %zu needed", ws_bytes, w.bytes);
     const int64_t chunks = (K + kCols - 1) / kCols + (N + kCols - 1) / kCols, size = R * (K + N);
     CACTI_REQUIRE(w.blocks * chunks < (1 << 24), CACTI_E_NOTIMPL, "adapter_bwd: too many tiles");
+    // (an adapter's gradient is written while others are formed)
+    const Extent eA = {A, n * R * K}, eB = {B, n * N * R}, eh = {h, 2 * T * R}, edx = rows_extent(T, dx, lddx, K);
+    CACTI_REQUIRE(!share(edx, {eA, eB, eh}), CACTI_E_INVALID, "adapter_bwd: dx shares memory with A, B or h");
+    const Extent ex = rows_extent(T, x, ldx, K), edy = rows_extent(T, dy, lddy, N);
+    CACTI_REQUIRE(!share({dA, eA.size}, {ex, edy, edx, eA, eB, eh}) && !share({dB, eB.size}, {ex, edy, edx, eA, eB, eh}), CACTI_E_INVALID,
+                  "adapter_bwd: dA or dB shares memory with an operand or dx");
     char *p = (char *)ws;
     d.f.h = (float *)const_cast<void *>(h);
     d.f.y = (half_t *)dx, d.f.ldy = lddx;

@@ -401,3 +401,17 @@ def test_captured_and_replayed():
         assert all(torch.equal(a, b) for a, b in zip(got, want))
         ids.copy_(torch.roll(ids, 1))
         x.copy_(torch.roll(x, 5, 1))
+
+
+# Results over what is read or written beside them.  (Places far enough apart for each operand's size.)
+APART = [("cacti_hip_adapter_fwd", FWD, c) for c in [
+    (dict(y=P0 + STEP), "y or h"), (dict(y=P0 + 2 * STEP - 496), "y or h"), (dict(h=P0 + 4 * STEP + 128), "y or h"), (dict(h=P0), "y or h"),
+    (dict(h=P0 + 3 * STEP + 384), "y or h"), (dict(h=P0 + 2 * STEP - 240), "y or h"), (dict(h=P0 + 2 * STEP + 4080), "y or h")]] + \
+        [("cacti_hip_adapter_bwd", BWD, c) for c in [
+            (dict(dx=P0 + STEP + 4080), "dx shares"), (dict(dx=P0 + 2 * STEP), "dx shares"), (dict(dx=P0 + 3 * STEP + 240), "dx shares")] +
+         [({w: P0 + i * STEP + o}, "dA or dB") for w in ("dA", "dB") for i, o in ((0, 0), (0, 496), (1, 0), (2, 4080), (3, 240), (4, -4080), (5, 496), (5, -4080))]]
+
+
+@pytest.mark.parametrize("entry,args,change", APART)
+def test_refuses_results_over_operands(entry, args, change):
+    test_refuses(entry, args, change)
