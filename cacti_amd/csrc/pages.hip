@@ -421,9 +421,17 @@ CACTI_API int cacti_hip_paged_fork(int64_t P, int64_t B, int64_t W, int64_t page
     CACTI_REQUIRE(lens && parent && new_table && new_lens, CACTI_E_INVALID, "paged_fork: null pointer");
     CACTI_REQUIRE(aligned(lens, 4) && aligned(parent, 4) && aligned(new_table, 4) && aligned(new_lens, 4), CACTI_E_INVALID, "paged_fork: misaligned operand");
     CACTI_REQUIRE(ldn >= W, CACTI_E_INVALID, "paged_fork: a table pitch below its width");
-    const char *t = (const char *)table, *n = (const char *)new_table, *l = (const char *)lens, *m = (const char *)new_lens;
-    CACTI_REQUIRE(n >= t + 4 * ((B - 1) * ldt + W) || t >= n + 4 * ((B - 1) * ldn + W), CACTI_E_INVALID, "paged_fork: the new table shares memory with the old one");
-    CACTI_REQUIRE(m >= l + 4 * B || l >= m + 4 * B, CACTI_E_INVALID, "paged_fork: the new lengths share memory with the old ones");
+    auto share = [](const void *a, int64_t na, const void *b, int64_t nb) {      // na numbers at a, nb at b
+        const char *p = (const char *)a, *q = (const char *)b;
+        return p < q + 4 * nb && q < p + 4 * na;
+    };
+    const int64_t size = (B - 1) * ldn + W;
+    CACTI_REQUIRE(!share(new_table, size, table, (B - 1) * ldt + W), CACTI_E_INVALID, "paged_fork: the new table shares memory with the old one");
+    CACTI_REQUIRE(!share(new_lens, B, lens, B), CACTI_E_INVALID, "paged_fork: the new lengths share memory with the old ones");
+    // (a sequence's row and length are written while others' are read)
+    CACTI_REQUIRE(!share(new_table, size, lens, B) && !share(new_table, size, parent, B) && !share(new_table, size, refs, P) && !share(new_table, size, new_lens, B) &&
+                      !share(new_lens, B, parent, B) && !share(new_lens, B, refs, P) && !share(new_lens, B, table, (B - 1) * ldt + W),
+                  CACTI_E_INVALID, "paged_fork: the new table or the new lengths share memory with another operand");
     const ForkArgs a = {(int)P, (int)B, (int)W, (int)page, ldt, ldn, (int *)refs, (const int *)table, (const int *)lens, (const int *)parent,
                         (int *)new_table, (int *)new_lens, (int *)status};
     hipLaunchKernelGGL(fork_kernel, dim3((unsigned)B), dim3(256), 0, (hipStream_t)stream, a);

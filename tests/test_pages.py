@@ -565,3 +565,9 @@ def test_answers_from_a_pool_that_is_too_small(seed, B, W, page, P):
             break
         alive = [b for b in range(B) if k.lens[b] and b not in bad] or bad[1:]
         k.grow([0 if b == alive[0] else l for b, l in enumerate(k.lens)])
+
+
+@pytest.mark.parametrize("change", [dict(parent=0x3000), dict(parent=0x2004), dict(lens=0x201c), dict(refs=0x2000 - 32), dict(refs=0x3004), dict(new_lens=0x1000),
+                                    dict(new_lens=0x2000 - 4), dict(new_lens=0x1018)])
+def test_fork_refuses_results_over_operands(change):
+    test_refuses("cacti_hip_paged_fork", FORK, (change, "another operand"))
