@@ -544,6 +544,7 @@ struct GradArgs {
     half_t *terms[2];                          // of dh (without the scale) and h: rows of 32 RT, as in LDS, scaled by
     int *exps[2];                              // powers of two of their own
     int *rows, *begin;                         // rows of adapter a: rows[begin[a]] .. rows[begin[a + 1] - 1]
+    int *part;                                 // the first part of adapter a, which has parts where it has several blocks
     float *parts;                              // of dA [R, K] and dB [N, R], a block of rows each
     half_t *dA, *dB;
     int dA_acc, dB_acc, per;                   // rows of a block
@@ -585,21 +586,26 @@ __device__ void plan(const GradArgs &d, int *room, int ints, int *totals)
 #pragma unroll
     for (int i = 0; i < 2; i++)
         for (int s = 0; s < shares && a0 + i < g.n; s++) mine[i] = add(mine[i], room[s * g.n + a0 + i]);
-    int before = add(mine[0], mine[1]);
+    auto before_this = [&](int v, auto plus) __attribute__((always_inline)) {      // of the threads before this one
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int x = __shfl_up(before, o);
-        if (lane >= o) before = add(before, x);
-    }
-    if (lane == 63) totals[wave] = before;
-    before = __shfl_up(before, 1);
-    if (lane == 0) before = 0;
-    __syncthreads();
-    for (int w = 0; w < wave; w++) before = add(before, totals[w]);
+        for (int o = 1; o < 64; o <<= 1) {
+            const int x = __shfl_up(v, o);
+            if (lane >= o) v = plus(v, x);
+        }
+        if (lane == 63) totals[wave] = v;
+        v = __shfl_up(v, 1);
+        if (lane == 0) v = 0;
+        __syncthreads();
+        for (int w = 0; w < wave; w++) v = plus(v, totals[w]);
+        __syncthreads();
+        return v;
+    };
+    int before = before_this(add(mine[0], mine[1]), add), parts[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < 2; i++) {
         if (a0 + i >= g.n) break;
         d.begin[a0 + i] = before;
+        const int first = before;
         int at = before;
         for (int s = 0; s < shares; s++) {
             const int c = room[s * g.n + a0 + i];
@@ -608,8 +614,12 @@ __device__ void plan(const GradArgs &d, int *room, int ints, int *totals)
         }
         before = at;
         if (a0 + i == g.n - 1) d.begin[g.n] = at;
+        parts[i] = at - first > d.per ? (at - first + d.per - 1) / d.per : 0;
     }
-    __syncthreads();
+    const int part = before_this(parts[0] + parts[1], [](int x, int y) { return x + y; });
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        if (a0 + i < g.n) d.part[a0 + i] = part + (i ? parts[0] : 0);
     each([&](int a, int s0, int n, int sequences) __attribute__((always_inline)) {
         int at = a >= 0 ? own[a] : T;
         for (int l = 0; l < sequences; l++) {
@@ -695,10 +705,10 @@ struct GradLds {
     __attribute__((aligned(16))) half_t rows_and_terms[std::max(kRows * (XP + HP), 16 * RT * XP)], tiles[4][kTileHalves], less[4][kRows];
     int exps[2][kRows], rows[kMostRows];
 };
-// rows first .. first + count - 1 of those of adapter a, unit u; columns from c0 on of x (and dx) or of dy.  (Either by itself: the operands of the
+// rows first .. first + count - 1 of those of adapter a, its block `block`; columns from c0 on of x (and dx) or of dy.  (Either by itself: the operands of the
 // sums change places, and the compiler makes a branch at each instruction of one that does both.)
 template <int RT, bool of_x>
-__device__ __forceinline__ void grad(const GradArgs &d, GradLds<RT> &l, int u, int a, int first, int count, int c0)
+__device__ __forceinline__ void grad(const GradArgs &d, GradLds<RT> &l, int block, int a, int first, int count, int c0)
 {
     typedef Terms<RT> Two;
     constexpr int HP = GradLds<RT>::HP, XP = GradLds<RT>::XP, NX = kRows * kCols / 8 / 256;
@@ -831,7 +841,7 @@ __device__ __forceinline__ void grad(const GradArgs &d, GradLds<RT> &l, int u, i
     const float up = two_to(max(top, -126));
     const bool alone = d.begin[a + 1] - d.begin[a] <= d.per;      // (the only block: nothing to be joined)
     const int64_t ofA = (int64_t)R * K, ofB = (int64_t)R * N;
-    float *const part = d.parts + (int64_t)u * (ofA + ofB) + (of_x ? 0 : ofA);
+    float *const part = d.parts + (int64_t)(d.part[a] + block) * (ofA + ofB) + (of_x ? 0 : ofA);
     half_t *const to = of_x ? d.dA + a * ofA : d.dB + a * ofB;
     const bool add = of_x ? d.dA_acc : d.dB_acc;
 #pragma unroll
@@ -859,10 +869,10 @@ __global__ void __launch_bounds__(256, RT == 8 ? 2 : RT == 4 ? 3 : 4) grad_kerne
     const int i = x ? (int)blockIdx.x : (int)blockIdx.x - of_x, u = i / (x ? kchunks : nchunks), chunk = i - u * (x ? kchunks : nchunks);
     // (unit 0 is adapter 0's: one more than the adapters that begin behind it)
     const int a = __builtin_amdgcn_readfirstlane(count_below(d.f.n - 1, u, [&](int i) { return unit_of(d, i); }));
-    const int first = d.begin[a] + (int)(u - unit_of(d, a)) * d.per, count = min(d.per, d.begin[a + 1] - first);
+    const int block = (int)(u - unit_of(d, a)), first = d.begin[a] + block * d.per, count = min(d.per, d.begin[a + 1] - first);
     if (count <= 0) return;
-    if (x) grad<RT, true>(d, l, u, a, first, count, kCols * chunk);
-    else grad<RT, false>(d, l, u, a, first, count, kCols * chunk);
+    if (x) grad<RT, true>(d, l, block, a, first, count, kCols * chunk);
+    else grad<RT, false>(d, l, block, a, first, count, kCols * chunk);
 }
 
 // The parts of an adapter that has several blocks added up, and what has none made 0; 4 elements to a thread
@@ -877,7 +887,7 @@ __global__ void __launch_bounds__(256) join_kernel(GradArgs d)
     const bool acc = isA ? d.dA_acc : d.dB_acc;
     const int count = d.begin[a + 1] - d.begin[a], parts = (count + d.per - 1) / d.per;
     if (parts == 1 || (parts == 0 && acc)) return;
-    const float *p = d.parts + unit_of(d, a) * size + e;
+    const float *p = d.parts + (int64_t)d.part[a] * size + e;
     float4_t s = zero4();
     for (int i = 0; i < parts; i++) s += *reinterpret_cast<const float4_t *>(p + i * size);
     const float scale = g.scale[a];
@@ -948,7 +958,7 @@ int64_t block_rows(int64_t T, int64_t K, int64_t N, int64_t R)
 }
 
 struct Workspace {
-    size_t terms[2], exps[2], rows, begin, parts, bytes;
+    size_t terms[2], exps[2], rows, begin, part, parts, bytes;
     int64_t per, blocks;
 };
 Workspace workspace(int64_t T, int64_t K, int64_t N, int64_t R, int64_t n)
@@ -968,7 +978,12 @@ Workspace workspace(int64_t T, int64_t K, int64_t N, int64_t R, int64_t n)
     }
     w.rows = room((size_t)T * 4);
     w.begin = room((size_t)(n + 1) * 4);
-    w.parts = room((size_t)w.blocks * R * (K + N) * 4);
+    w.part = room((size_t)n * 4);
+    // Parts are those of adapters with more than a block of rows: of c > per rows ceil(c / per) <= 2 c / (per + 1).  (With one for every adapter
+    // 512 rows of 1024 adapters, 3200 to 8640, R = 128, took 6 GB.  There is room for one for each as long as that is no more than 32 MB.)
+    const size_t size = (size_t)R * (K + N) * 4;
+    const int64_t parts = std::min(2 * T / (w.per + 1), w.blocks), spare = std::min<int64_t>(n, (32 << 20) / size);
+    w.parts = room(std::max(parts, spare) * size);
     return w;
 }
 
@@ -1115,7 +1130,7 @@ CACTI_API int cacti_hip_adapter_bwd(int64_t T, int64_t S, int64_t K, int64_t N, 
     d.f.base = dx_acc ? (const half_t *)dx : nullptr, d.f.ldb = lddx;
     d.dy = (const half_t *)dy, d.lddy = lddy;
     for (int i = 0; i < 2; i++) d.terms[i] = (half_t *)(p + w.terms[i]), d.exps[i] = (int *)(p + w.exps[i]);
-    d.rows = (int *)(p + w.rows), d.begin = (int *)(p + w.begin);
+    d.rows = (int *)(p + w.rows), d.begin = (int *)(p + w.begin), d.part = (int *)(p + w.part);
     d.parts = (float *)(p + w.parts);
     d.dA = (half_t *)dA, d.dB = (half_t *)dB, d.dA_acc = dA_acc, d.dB_acc = dB_acc;
     d.per = (int)w.per, d.blocks = w.blocks;

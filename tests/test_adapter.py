@@ -415,3 +415,22 @@ APART = [("cacti_hip_adapter_fwd", FWD, c) for c in [
 @pytest.mark.parametrize("entry,args,change", APART)
 def test_refuses_results_over_operands(entry, args, change):
     test_refuses(entry, args, change)
+
+
+@pytest.mark.parametrize("T,K,N,R,n", [(512, 3200, 8640, 128, 1024), (64, 3200, 8640, 128, 64), (1, 3200, 3200, 128, 1024), (2048, 8640, 3200, 64, 1000),
+                                       (4096, 3200, 3200, 16, 3), (9600, 256, 256, 8, 1024)])
+def test_workspace_goes_by_the_rows(T, K, N, R, n):
+    """No more parts of gradients than adapters with more than a block of 64 rows may have, or 32 MB of them."""
+    rest = T * 2 * 64 * 8 + 3 * 4 * T + 8 * (n + 1) + (1 << 13)
+    assert ffi.lib().cacti_hip_adapter_bwd_workspace(T, K, N, R, n) <= rest + max(2 * T // 65 * R * (K + N) * 4, 32 << 20)
+
+
+@GPU
+@pytest.mark.parametrize("counts", [[65] * 40, [129] * 21, [64, 65] * 20, [1, 200, 64, 0, 65, 66, 3] * 6])
+def test_adapters_of_several_blocks_among_others(counts):
+    """As many parts as there can be (65 rows: two blocks), and adapters with and without between them."""
+    print("adapter", counts[:2], len(counts), flush=True)
+    n = len(counts)
+    ids = [(7 * i) % n for i in range(n)]
+    assert len(set(ids)) == n or n % 7 == 0
+    check(Case(n, counts, ids, 24, 40, 16, n), max_new=max(counts))
