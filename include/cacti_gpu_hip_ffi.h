@@ -553,6 +553,7 @@ int cacti_hip_preference_loss(int64_t N, int64_t pairs, const void *logp, const 
  *   dh = dy B_a,  dx (+)= f16(scale[a] dh A_a),  dA_a (+)= f16(scale[a] sum dh^T x),  dB_a (+)= f16(scale[a] sum dy^T h)   (over a's rows)
  * (an adapter without rows: 0).  *_acc: 0 first write, 1 added in fp32 before the one rounding.  Sums in fp32 and in a fixed order; h and dh
  * meet the second product as two f16 terms, 22 bits, 2^-25 of the largest of their row (for dA and dB: 2^-24 of the adapter's largest).
+ * What an infinite element of x, A, B or dy reaches is infinite or no number (the two terms of h or dh may be of different signs, or one 0).
  * y and h, and dx, dA and dB, share no memory with A, B, x, dy or each other, nor dx, dA and dB with h.  K, N, R multiples of 8, R <= 128; rows of x, y, base, dy, dx of pitches that are
  * multiples of 8; all 16-byte aligned; n <= 1024; T <= 2^24, S <= 2^20, K and N <= 2^20, less where that would be 2^24 blocks of rows and
  * columns.  max_new: no sequence has more rows.  status [1] i32 or NULL: 1 + s where the rows of sequence s are not there or more than

@@ -434,3 +434,82 @@ def test_adapters_of_several_blocks_among_others(counts):
     ids = [(7 * i) % n for i in range(n)]
     assert len(set(ids)) == n or n % 7 == 0
     check(Case(n, counts, ids, 24, 40, 16, n), max_new=max(counts))
+
+
+def rows_by_powers_of_two(c, order, top=2):
+    """Rows of dy and x by powers of two of 2^-20 .. 2^2 and 2^-12 .. 2^2, so that the largest row so far changes from step to step."""
+    r = np.random.default_rng(c.T)
+    e = np.linspace(-20, top, c.T).round()
+    e = dict(rising=e, falling=e[::-1], mixed=r.permutation(e))[order]
+    c.dy = (c.dy * 2.0 ** e[:, None]).astype(np.float16)
+    c.x = (c.x * 2.0 ** ((e[::-1, None] - top) * 14 / 22 + top).round()).astype(np.float16)
+
+
+STEPS = [([1001, 5, 697], [0, 1, 0], 3200, 3200, 16, 2), ([300, 813], [0, 0], 3200, 3200, 128, 1), ([900, 1131], [1, 0], 3200, 3200, 64, 3),
+         ([129, 1, 1500], [0, 2, 2], 1024, 8640, 24, 3)]
+
+
+@pytest.mark.parametrize("counts,ids,K,N,R,n", STEPS)
+def test_blocks_of_more_than_a_step(counts, ids, K, N, R, n):
+    """The cases below have blocks of more than 64 rows: their parts are fewer than blocks of 64."""
+    T, terms = sum(counts), 2 * 64 * (1 if R <= 16 else 2 if R <= 32 else 4 if R <= 64 else 8)
+    assert (ffi.lib().cacti_hip_adapter_bwd_workspace(T, K, N, R, n) - T * terms) // (R * (K + N) * 4) < T // 64
+
+
+@GPU
+@pytest.mark.parametrize("counts,ids,K,N,R,n", STEPS)
+@pytest.mark.parametrize("order", ["rising", "falling", "mixed", None])
+def test_gradients_in_several_steps(counts, ids, K, N, R, n, order):
+    print("adapter", counts, K, N, R, order, flush=True)
+    c = Case(K + N + R, counts, ids, K, N, R, n, behind=1)
+    if order:
+        rows_by_powers_of_two(c, order)
+    check(c, max_new=max(counts))
+
+
+TURNS = [([8200], [1], 264, 1032, 24), ([600, 33, 800, 667], [2, -1, 0, 1], 264, 4104, 64)]
+
+
+@GPU
+@pytest.mark.parametrize("counts,ids,K,N,R", TURNS)
+def test_columns_in_several_turns(counts, ids, K, N, R):
+    """A second launch whose waves have more than one block of 32 columns each: 8 waves to a workgroup, at most two workgroups to a compute unit."""
+    T, units = sum(counts), sum(counts) // 64 + len(counts)
+    assert T >= 8192 or ffi.lib().cacti_hip_adapter_fwd_workspace(T, len(ids), K, N, R, max(counts)) > 0
+    assert -(-N // 32) > 8 * max(1, 512 // units)
+    print("adapter", counts, K, N, R, flush=True)
+    c = Case(K + N + R, counts, ids, K, N, R, 3, behind=2)
+    check(c, max_new=max(counts))
+    rows_by_powers_of_two(c, "mixed")
+    check(c, max_new=max(counts))
+
+
+@GPU
+def test_infinite_values_reach_what_they_meet_and_nothing_else():
+    """(Infinite there or no number: the two terms of a value may be of different signs.)"""
+    from cacti_amd import ops
+    c = Case(16, [5, 70, 7], [2, 0, 2], 72, 88, 16, 3)
+    x, A, B, starts, ids, scale, base, dy = c.of("x A B starts ids scale base dy")
+    own, every = np.array([i < 5 or i >= 75 for i in range(82)]), slice(None)
+
+    def run():
+        y, h = ops.adapter_fwd(x, A, B, starts, ids, scale, base=base)
+        return dict(zip("y h dx dA dB".split(), (y, h, *ops.adapter_bwd(x, A, B, starts, ids, scale, h, dy))))
+
+    clean = run()["h"].cpu().numpy()
+    wy, ty, wh, th = c.forward(True)
+    want = dict(zip("y h dx dA dB".split(), [(wy, ty), (wh, th), *c.adjoint(clean, False)]))
+    for t, at, hit in ((B, (2, 5, 3), dict(y=[(own, 5)], dx=[(own, every)], dA=[(2, 3)])),
+                       (A, (2, 1, 4), dict(h=[(own, 1)], y=[(own, every)], dx=[(own, 4)], dB=[(2, every, 1)])),
+                       (x, (3, 9), dict(h=[(3, every)], y=[(3, every)], dA=[(2, every, 9)], dB=[(2, every)])),
+                       (dy, (40, 7), dict(dx=[(40, every)], dA=[(0, every)], dB=[(0, 7)]))):
+        was = t.clone()
+        t[at] = float("inf")
+        for k, got in run().items():
+            got = got.cpu().numpy()
+            where = np.zeros(got.shape, bool)
+            for place in hit.get(k, []):
+                where[place] = True
+            assert not np.isfinite(got[where]).any(), (k, at)
+            near(got[~where], want[k][0][~where], want[k][1][~where], k)
+        t.copy_(was)
