@@ -370,7 +370,8 @@ struct Columns {
         }
     }
 };
-// The columns of a wave, the next ones' operands under way: those from 32 first on, every `stride`-th 32
+// The columns of a wave: those from 32 first on, every `stride`-th 32, each block's operands loaded when the last is done (the next ones' under way beside
+// it cost registers: 2227 rows of 3200 to 8640, R = 64 34.2 us, 32.7 without)
 template <int RT, int TB, bool BASE>
 struct Wave {
     typedef Columns<RT, TB, BASE> C;
@@ -465,7 +466,7 @@ __global__ void __launch_bounds__(64 * one_waves(RT)) one_kernel(AdapterArgs g)
 }
 
 // In two, h first: 16 TB rows of a sequence and 1 / splits of the contraction to a workgroup, sums to a plane of [splits][T, R]
-constexpr int h_blocks(int) { return 2; }
+constexpr int kHBlocks = 2;
 template <int RT, int TB>
 __global__ void __launch_bounds__(512) h_kernel(AdapterArgs g, float *planes)
 {
@@ -554,7 +555,7 @@ struct GradArgs {
 // The rows of each adapter, sequence after sequence, by one workgroup of 8 waves: each of up to 8 counts the rows of its share of the
 // sequences by adapter (room: ints of LDS), then gives them their places, 64 sequences at a time.  (Sums no larger than T: sequences that
 // overlap may have more rows than there are.  300 sequences of 300 adapters, each adapter looking through them all: 111 us.)
-constexpr int kMaxAdapters = 1024;
+constexpr int kMaxAdapters = 1024;            // (the forward call takes no more than its adjoint)
 __device__ void plan(const GradArgs &d, int *room, int ints, int *totals)
 {
     const AdapterArgs &g = d.f;
@@ -996,7 +997,8 @@ Workspace workspace(int64_t T, int64_t K, int64_t N, int64_t R, int64_t n)
 //   the tiles are too few to fill the device and too many to split their columns, and A and B are large: 4 x 557 rows of 3200 to 8640,
 //     R = 64 33 and 45, but R = 16 23.3 either way.
 // Everywhere else the first: one row of 3200 to 8640, R = 16 8.5 and 6.2, 2048 rows of 3200 to 3200 13.2 and 10.4, 4096 19.1 and 15.7.
-// (Over 125 shapes the rule's choice is 0.6 % slower than the better one in the mean, 13 % at most.)
+// Over 125 shapes (profiles/adapter_forward_launches.txt) the rule's choice is 0.7 % slower than the better one in the mean, 13 % at most.  None of
+// them has K between 3200 and 8640: that the border is 4096 there is a guess.
 struct ForwardPlan {
     bool two;
     int splits, planes;
@@ -1022,7 +1024,7 @@ ForwardPlan forward_plan(int64_t T, int64_t S, int64_t K, int64_t N, int64_t R, 
         w.splits = columns(cus, tiles, one_waves(rank));
         return w;
     }
-    w.h_units = units(16 * h_blocks(rank));
+    w.h_units = units(16 * kHBlocks);
     w.y_units = units(kRows);
     w.planes = fill(cus, w.h_units.count, std::min<int64_t>(8, (K + 255) / 256));
     w.splits = columns(rank == 8 ? cus : 2 * cus, w.y_units.count, 8);       // (as many as a CU's LDS has room for: R = 128 47 us, by two 54)
@@ -1085,7 +1087,7 @@ CACTI_API int cacti_hip_adapter_fwd(int64_t T, int64_t S, int64_t K, int64_t N, 
     CACTI_REQUIRE(blocks1 <= INT32_MAX && blocks2 <= INT32_MAX, CACTI_E_NOTIMPL, "adapter_fwd: too many tiles");
 #define LAUNCH(RT)                                                                                                       \
     do {                                                                                                                 \
-        hipLaunchKernelGGL((h_kernel<RT, h_blocks(RT)>), dim3((unsigned)blocks1), dim3(512), 0, st, first, planes);                 \
+        hipLaunchKernelGGL((h_kernel<RT, kHBlocks>), dim3((unsigned)blocks1), dim3(512), 0, st, first, planes);                     \
         if (base) hipLaunchKernelGGL((y_kernel<RT, true>), dim3((unsigned)blocks2), dim3(512), 0, st, g, (const float *)planes, w.planes); \
         else hipLaunchKernelGGL((y_kernel<RT, false>), dim3((unsigned)blocks2), dim3(512), 0, st, g, (const float *)planes, w.planes);     \
     } while (0)

@@ -370,7 +370,7 @@ struct CopyArgs {
     char *k[kLayers], *v[kLayers];
     float *ks[kLayers], *vs[kLayers];
     const int *src, *dst, *slots;
-    int64_t n, P;
+    int64_t P;
     unsigned items;
     int parts, layers, heads, page, slot_bytes;        // (of a position of a head)
 };
@@ -503,7 +503,7 @@ CACTI_API int cacti_hip_paged_copy(int64_t layers, void *const *k_pages, void *c
         a.heads = (int)Hkv, a.page = (int)page, a.slot_bytes = (int)((Dh + 15) / 16 * 16 * bits / 8);
         const int64_t parts = (Hkv + 3) / 4, items = n * 2 * a.layers * parts;
         CACTI_REQUIRE(items <= INT32_MAX, CACTI_E_NOTIMPL, "paged_copy: too many pages");
-        a.n = n, a.P = P, a.parts = (int)parts, a.items = (unsigned)items;
+        a.P = P, a.parts = (int)parts, a.items = (unsigned)items;
         const int64_t blocks = a.items < 4096 ? a.items : 4096;
         hipLaunchKernelGGL(copy_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
     }
