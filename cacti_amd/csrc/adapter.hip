@@ -17,7 +17,8 @@
 // 8640, R = 64: h 10.1 us, y 22.1 for 77 MB of base and y, 3.5 TB/s; between loads and stores stand the turns in LDS.  The adjoint of 4096
 // rows: 9.8 us for the terms of dh and h (dy read once), 18.0 for dx and the parts of dA and dB (79 MB, 4.4 TB/s), 3.9 to join those;
 // 269 rows of 1024 to 2816 take 7.7, 5.9 and 3.8, little more than launches.  R = 128: 24, 44 and 7, of those 44 the matrix pipe 8, vector
-// operations 12 and LDS 13, which two waves to a SIMD do not bring together.
+// operations 12 and LDS 13 (every wave reads and scales all terms for its 32 columns), which two waves to a SIMD do not bring together; the 24
+// are those of B, read and turned for every 16 rows.
 #include <algorithm>
 #include <initializer_list>
 

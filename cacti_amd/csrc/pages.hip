@@ -12,7 +12,7 @@
 // workgroup: what is free depends on everything that is given back, and a barrier costs less there than a launch (a batch's table and
 // counts are some ten kilobytes).  Copying is bound by memory.
 //
-// On the device: fork 3 us for 8 as for 128 sequences, a launch's own time; fit 7.2 us for 8 sequences, 9.7 for 128, some six barriers with
+// On the device: fork 3 us for 8 as for 128 sequences, a launch's own time; fit 7.3 us for 8 sequences, 10.0 for 128, some six barriers with
 // a look at memory between each two; copies of 8 to 128 pages 4.4 to 6.9; packing 6.6 + 4.6 us and its 492 MB of copies 95, 5.2 TB/s.
 #include "common.h"
 
