@@ -323,3 +323,35 @@ def test_two_graphs_and_another_stream():
         torch.cuda.synchronize()
         for g, w in zip(got + [third], want):
             assert all(torch.equal(a, b) for a, b in zip(g, w))
+
+
+@GPU
+@pytest.mark.parametrize("bits", [8, 16])
+def test_a_step_that_pages_run_out_in_and_the_same_step_again(bits):
+    """Three answers to a prompt whose last page is not full, and a single page that is free: one goes on, nothing is written on the page that
+    the others share, and with pages free again they go on as answers do that have their own."""
+    import torch
+    m, ids = Model(4, bits), ints([0, -1, 2])
+    r = np.random.default_rng(7)
+    text, tok = dev(r.integers(0, V, 20)), dev(r.integers(0, V, 3))
+    a, b = Answers(m, 3, True), Answers(m, 3, False)
+    for k in (a, b):
+        k.grow(ints([20, 0, 0]))
+        m.run(k.cache, k.table, text, ints([0, 20, 20, 20]), k.lens, ids, 20, k.status)
+        k.fork(ints([0, 0, 0]))
+    a.refs[3:] += 1                            # (of somebody else)
+    b.grow(ints([21, 21, 21]))
+    want = m.run(b.cache, b.table, tok, ints([0, 1, 2, 3]), b.lens, ids, 1, b.status)
+    a.grow(ints([21, 21, 21]))
+    bits_of = lambda: [x.view(torch.uint8)[1].clone() for x in a.cache if x is not None]
+    assert int(a.status) == 3 and a.table[:, 1].tolist() == [-3, 2, -3] and a.refs[:3].tolist() == [3, 2, 1]
+    before = bits_of()
+    z = m.run(a.cache, a.table, tok, ints([0, 1, 2, 3]), a.lens, ids, 1, a.status)
+    assert torch.equal(z[1], want[1]) and all(torch.equal(x, y) for x, y in zip(bits_of(), before))
+    a.status.zero_()
+    a.lens = ints([20, 21, 20])
+    a.refs[3:5] -= 1
+    a.grow(ints([21, 21, 21]))
+    z = m.run(a.cache, a.table, tok[[0, 2]].contiguous(), ints([0, 1, 1, 2]), a.lens, ids, 1, a.status)
+    assert torch.equal(z, want[[0, 2]]) and int(a.status) == 0
+    assert a.table[:, 1].tolist() == [1, 2, 3] and a.refs[:5].tolist() == [3, 1, 1, 1, 0]
