@@ -571,3 +571,16 @@ def test_answers_from_a_pool_that_is_too_small(seed, B, W, page, P):
                                     dict(new_lens=0x2000 - 4), dict(new_lens=0x1018)])
 def test_fork_refuses_results_over_operands(change):
     test_refuses("cacti_hip_paged_fork", FORK, (change, "another operand"))
+
+
+@GPU
+def test_more_sequences_than_a_workgroup_remembers_and_too_few_pages():
+    k = Short(9, 2100, 2, 16, 1000)
+    k.grow([20 if b % 100 == 0 else 0 for b in range(2100)])
+    k.go_on([b // 100 * 100 for b in range(2100)])
+    bad = k.grow([21] * 2100)
+    assert len(bad) > 1000 and bad[-1] == 2099
+    k.grow([0 if b in bad[::3] else l for b, l in enumerate(k.lens)])
+    assert k.grow([l and 21 for l in k.lens])
+    k.grow([l if b % 2 else 0 for b, l in enumerate(k.lens)])
+    assert k.grow([l and 21 for l in k.lens]) == []
